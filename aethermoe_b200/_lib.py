@@ -110,6 +110,25 @@ _SIGS = {
     "aem_capacity_route_workspace": (ctypes.c_size_t, [_i64, _int]),
     "aem_capacity_route": (_int, [_vp, _vp, _vp, _i64, _int, _u64, _vp, _vp, ctypes.c_size_t,
                                   _vp]),
+    "aem_token_sort_workspace": (ctypes.c_size_t, [_i64, _int, _int]),
+    "aem_token_sort": (_int, [_vp, _i64, _int, _i64, _i64, _int, _vp, _vp, _vp, _vp,
+                              ctypes.c_size_t, _vp]),
+    "aem_dispatch": (_int, [_vp, _int, _i64, _i64, _vp, _i64, _int, _i64, _i64, _int, _vp, _i64, _vp,
+                            _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "aem_dispatch_rows": (_int, [_vp, _int, _i64, _i64, _vp, _vp, _i64, _int, _int, _vp, _i64, _vp]),
+    "aem_dispatch_backward": (_int, [_vp, _int, _i64, _vp, _i64, _int, _i64, _vp, _int, _i64, _vp]),
+    "aem_combine": (_int, [_vp, _int, _i64, _vp, _i64, _vp, _i64, _int, _i64, _vp, _int, _i64, _vp]),
+    "aem_combine_backward": (_int, [_vp, _int, _i64, _vp, _int, _i64, _vp, _i64, _vp, _vp, _i64, _int,
+                                    _int, _i64, _vp, _i64, _vp, _vp]),
+    "aem_quantize_q4": (_int, [_vp, _int, _i64, _i64, _i64, _int, _vp, _vp, _int, _vp]),
+    "aem_q4weight_pack": (_int, [_vp, _vp, _int, _i64, _i64, _i64, _int, _int, ctypes.POINTER(_vp)]),
+    "aem_q4weight_pack_device": (_int, [_vp, _vp, _int, _i64, _i64, _i64, _int, _vp,
+                                        ctypes.POINTER(_vp)]),
+    "aem_q4weight_free": (_int, [_vp]),
+    "aem_q4weight_shape": (_int, [_vp, ctypes.POINTER(_i64), ctypes.POINTER(_i64),
+                                  ctypes.POINTER(_i64), ctypes.POINTER(_int)]),
+    "aem_q4gemm": (_int, [_vp, _i64, _vp, _int, _i64, _i64, _vp, _int, _i64, _vp]),
+    "aem_grouped_q4gemm": (_int, [_vp, _vp, _vp, _int, _i64, _i64, _vp, _int, _i64, _int, _vp]),
     "aem_moe_create": (_int, [ctypes.POINTER(MoeConfig), _vp, _vp, _vp, ctypes.POINTER(_vp)]),
     "aem_moe_free": (_int, [_vp]),
     "aem_moe_forward": (_int, [_vp, _vp, _int, _i64, _vp, _int, _vp]),

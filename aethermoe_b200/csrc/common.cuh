@@ -57,6 +57,8 @@ enum : int {
     ERR_EP_BOUNDS = 1 << 5,       // expert-parallel row index outside its buffer (skipped)
     ERR_EP_PEER_TIMEOUT = 1 << 6, // a peer rank did not signal within the deadline
     ERR_EP_PEER_FAILED = 1 << 7,  // a peer rank signalled that its step failed
+    ERR_ROW_INDEX = 1 << 8,       // a token order names a row past its units (skipped)
+    ERR_Q4_VALUE = 1 << 9,        // a 4-bit weight outside [-8, 7] (clamped)
 };
 
 

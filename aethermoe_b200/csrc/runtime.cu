@@ -123,6 +123,14 @@ aem_status check_device_errors(cudaStream_t stream, const char* what) {
                   what, bits);
         return AEM_EDEVICE;
     }
+    if (bits & ERR_ROW_INDEX) {
+        set_error("%s: a token order names a row past its units (error bits 0x%x)", what, bits);
+        return AEM_EDEVICE;
+    }
+    if (bits & ERR_Q4_VALUE) {
+        set_error("%s: a 4-bit weight is outside [-8, 7] (error bits 0x%x)", what, bits);
+        return AEM_EDEVICE;
+    }
     set_error("%s: in-kernel check failed (error bits 0x%x)", what, bits);
     return AEM_EDEVICE;
 }

@@ -1,0 +1,145 @@
+"""4-bit weights with group scales: quantisation, the packed weight, and the
+products of a decoding step's rows with it, dense and grouped by expert.
+
+    q, s = quantize_q4(w, 128)                   # w [K, N] or [G, K, N]
+    weight = Q4Weight(q, s, 128)                 # packed once, K*N/2 bytes a group
+    y = q4_matmul(x, weight)                     # x [M, K]
+    h = grouped_q4_matmul(rows, weight, order.starts, relu=True)
+
+Tensors are torch CUDA tensors; every kernel is in ``libaethermoe.so``
+(``aem_quantize_q4`` and the following calls of ``include/aem.h``, which
+define the results).
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .dispatch import _DT, _matrix, _on, _output
+
+
+def _quantize(w, group_size, scale_dtype, s):
+    g = 1 if w.dim() == 2 else w.shape[0]
+    k, n = w.shape[-2:]
+    kb = -(-k // group_size)
+    q = torch.empty(w.shape, dtype=torch.int8, device=w.device)
+    scale = torch.empty(w.shape[:-2] + (kb, n), dtype=scale_dtype, device=w.device)
+    _lib.check(_lib.lib().aem_quantize_q4(w.data_ptr(), _DT[w.dtype], g, k, n, group_size,
+                                          q.data_ptr(), scale.data_ptr(), _DT[scale_dtype], s),
+               "aem_quantize_q4")
+    return q, scale
+
+
+def quantize_q4(w, group_size=128, scale_dtype=torch.float32, stream=None):
+    """``w [K, N]`` or ``[G, K, N]`` (float32 or bfloat16) -> ``(q int8, scale)`` with
+    ``scale [(G,) ceil(K/group_size), N]``: symmetric, values in [-7, 7], the
+    ``group_size`` (32, 64, 128) consecutive k of a column sharing a scale."""
+    if w.dim() not in (2, 3):
+        raise ValueError("w must be [K, N] or [G, K, N]")
+    if w.dtype not in _DT or scale_dtype not in _DT:
+        raise ValueError(f"unsupported dtype {w.dtype} / {scale_dtype} (float32 or bfloat16)")
+    if group_size not in (32, 64, 128):
+        raise ValueError(f"group_size={group_size} is not 32, 64 or 128")
+    return _on(stream, _quantize, (w,), (w.contiguous(), group_size, scale_dtype))
+
+
+class Q4Weight:
+    """Packed 4-bit weight groups: ``q [K, N]`` or ``[G, K, N]`` int8 with values in
+    [-8, 7] and ``scale [(G,) ceil(K/group_size), N]`` (float32 or bfloat16).
+    CUDA tensors are packed on the device (the call waits for it and raises on
+    a value out of range), CPU tensors and NumPy arrays through
+    ``aem_q4weight_pack`` onto ``device``."""
+
+    def __init__(self, q, scale, group_size, device=0, stream=None):
+        self.handle = None
+        q, scale = torch.as_tensor(q), torch.as_tensor(scale)
+        if q.dtype != torch.int8 or q.dim() not in (2, 3):
+            raise ValueError(f"q must be [K, N] or [G, K, N] int8, got {tuple(q.shape)} {q.dtype}")
+        if scale.dtype not in _DT:
+            raise ValueError(f"scale: unsupported dtype {scale.dtype} (float32 or bfloat16)")
+        if group_size not in (32, 64, 128):
+            raise ValueError(f"group_size={group_size} is not 32, 64 or 128")
+        g = 1 if q.dim() == 2 else q.shape[0]
+        k, n = q.shape[-2:]
+        want = tuple(q.shape[:-2]) + (-(-k // group_size), n)
+        if tuple(scale.shape) != want:
+            raise ValueError(f"scale must be {want}, got {tuple(scale.shape)}")
+        q, scale = q.contiguous(), scale.contiguous()
+        h = ctypes.c_void_p()
+        if q.is_cuda:
+            def pack(s):
+                L = _lib.lib()
+                _lib.check(L.aem_q4weight_pack_device(q.data_ptr(), scale.data_ptr(), _DT[scale.dtype], g,
+                                                      k, n, group_size, s, ctypes.byref(h)),
+                           "aem_q4weight_pack_device")
+                st = L.aem_device_status(s)
+                if st != _lib.AEM_OK:
+                    message = _lib.last_error()
+                    L.aem_q4weight_free(h.value)
+                    if st == _lib.AEM_EDEVICE:
+                        raise ValueError(f"Q4Weight: {message}")
+                    raise _lib.AemError(st, message)
+            _on(stream, pack, (q, scale), ())
+            device = q.device.index
+        else:
+            _lib.check(_lib.lib().aem_q4weight_pack(q.data_ptr(), scale.data_ptr(), _DT[scale.dtype], g,
+                                                    k, n, group_size, device, ctypes.byref(h)),
+                       "aem_q4weight_pack")
+        self.handle = h.value
+        self.G, self.K, self.N, self.group_size, self.device = g, k, n, group_size, device
+
+    def close(self):
+        if getattr(self, "handle", None):
+            _lib.lib().aem_q4weight_free(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def _check_weight(w, device):
+    if not w.handle:
+        raise ValueError("the weight is closed")
+    if device.index != w.device:
+        raise ValueError(f"x is on {device}, the weight on cuda:{w.device}")
+
+
+def _matmul(x, w, group, out_dtype, out, s):
+    x, ldx = _matrix(x, "x", d=w.K)
+    _check_weight(w, x.device)
+    m = x.shape[0]
+    out, ldo = _output(out, (m, w.N), out_dtype or (x.dtype if out is None else out.dtype), x.device)
+    _lib.check(_lib.lib().aem_q4gemm(w.handle, group, x.data_ptr(), _DT[x.dtype], ldx, m,
+                                     out.data_ptr(), _DT[out.dtype], ldo, s), "aem_q4gemm")
+    return out
+
+
+def _grouped(x, w, starts, relu, out_dtype, out, s):
+    x, ldx = _matrix(x, "x", d=w.K)
+    _check_weight(w, x.device)
+    if starts.dtype != torch.int32 or tuple(starts.shape) != (w.G + 1,) or not starts.is_contiguous():
+        raise ValueError(f"starts must be {w.G + 1} contiguous int32 offsets")
+    m = x.shape[0]
+    out, ldo = _output(out, (m, w.N), out_dtype or (x.dtype if out is None else out.dtype), x.device)
+    _lib.check(_lib.lib().aem_grouped_q4gemm(w.handle, starts.data_ptr(), x.data_ptr(), _DT[x.dtype],
+                                             ldx, m, out.data_ptr(), _DT[out.dtype], ldo,
+                                             1 if relu else 0, s), "aem_grouped_q4gemm")
+    return out
+
+
+def q4_matmul(x, w, group=0, out_dtype=None, out=None, stream=None):
+    """``x [M, K] @`` group ``group`` of ``w`` -> ``[M, N]`` (``out_dtype`` defaults to
+    x's): the weight stream of a decoding step."""
+    return _on(stream, _matmul, (x,), (x, w, group, out_dtype, out))
+
+
+def grouped_q4_matmul(x, w, starts, relu=False, out_dtype=None, out=None, stream=None):
+    """Rows ``[starts[g], starts[g+1])`` of ``x [M, K]`` times group ``g`` of ``w``,
+    for every group, with an optional ReLU.  Rows outside every group are not
+    written (uninitialised where ``out`` is not given)."""
+    return _on(stream, _grouped, (x, starts), (x, w, starts, relu, out_dtype, out))

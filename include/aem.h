@@ -272,6 +272,119 @@ aem_status aem_capacity_route_static(const uint32_t* primary, const uint32_t* se
                                      const uint32_t* batch_position, int64_t n, int E,
                                      uint64_t capacity, uint32_t* effective, void* stream);
 
+/* ---- token dispatch and combine around expert products, with gradients ------------ */
+
+/* The pieces of a layer step for callers that run their own experts (another
+ * activation, 4-bit weights, training).  A unit u = t*k + j is slot j of token
+ * t, with expert id ids[t*stride_t + j*stride_k] (int32: aem_gating's out_idx
+ * with stride_t = its row length, or the slot-major effective experts of
+ * aem_capacity_route with stride_t = 1, stride_k = T).  A negative id is a
+ * unit without an expert (a padded token, a dropped choice): it gets no row,
+ * contributes nothing and its gradients are zero.  An id of E or more is
+ * treated the same and reported by aem_device_status.  The order:
+ *   starts  [E+1]  first row of each expert; starts[E] = rows in use
+ *   row_of  [T*k]  row of each unit, -1 for none
+ *   unit_of [T*k]  unit of each row, -1 from starts[E] on
+ * Rows of one expert follow the units' order (a stable sort).  k <=
+ * AEM_MAX_TOPK, E <= AEM_MAX_EXPERTS, T*k < 2^31.  All pointers are DEVICE
+ * pointers, row strides (ld*) count elements and d is the contiguous one; any
+ * alignment of the element type works, 16-byte rows run widest.  Sums are
+ * float32 in a fixed order (no atomics): results repeat bit for bit.  Calls
+ * share nothing and are ordered by their stream alone; make the first call
+ * on a device before a stream capture.  The reference's scatter and
+ * reassembly are Router::route_batch (src/orchestration/router.hpp:67-100,
+ * 268-313); it has no gradients. */
+
+/* Scratch of aem_token_sort and aem_dispatch, in bytes (0 for small batches). */
+size_t aem_token_sort_workspace(int64_t T, int k, int E);
+/* The order of a batch.  workspace: device scratch of
+ * aem_token_sort_workspace(T, k, E) bytes, or NULL to have the call allocate
+ * and free it in stream order.  T == 0 writes zero starts. */
+aem_status aem_token_sort(const int32_t* ids, int64_t T, int k, int64_t stride_t, int64_t stride_k,
+                          int E, int32_t* starts, int32_t* row_of, int32_t* unit_of,
+                          void* workspace, size_t workspace_bytes, void* stream);
+/* The same, and rows[row_of[t*k + j]] = x[t] (rows [T*k, d], x [T, d], one
+ * dtype).  Rows from starts[E] on are zero. */
+aem_status aem_dispatch(const void* x, aem_dtype dtype, int64_t ldx, int64_t d, const int32_t* ids,
+                        int64_t T, int k, int64_t stride_t, int64_t stride_k, int E, void* rows,
+                        int64_t ldr, int32_t* starts, int32_t* row_of, int32_t* unit_of,
+                        void* workspace, size_t workspace_bytes, void* stream);
+/* Rows of another x by an order that exists. */
+aem_status aem_dispatch_rows(const void* x, aem_dtype dtype, int64_t ldx, int64_t d,
+                             const int32_t* row_of, const int32_t* starts, int64_t T, int k, int E,
+                             void* rows, int64_t ldr, void* stream);
+/* Gradient of the dispatch: grad_x[t] = sum_j grad_rows[row_of[t*k + j]]. */
+aem_status aem_dispatch_backward(const void* grad_rows, aem_dtype rows_dtype, int64_t ldr,
+                                 const int32_t* row_of, int64_t T, int k, int64_t d, void* grad_x,
+                                 aem_dtype x_dtype, int64_t ldx, void* stream);
+/* out[t] = sum_j weights[t*ldw + j] * rows[row_of[t*k + j]]; weights NULL
+ * means 1.  A token without any expert gets zero.  The weight of a unit
+ * without an expert is not read. */
+aem_status aem_combine(const void* rows, aem_dtype rows_dtype, int64_t ldr, const float* weights,
+                       int64_t ldw, const int32_t* row_of, int64_t T, int k, int64_t d, void* out,
+                       aem_dtype out_dtype, int64_t ldo, void* stream);
+/* Gradients of the combine, in one pass over the rows:
+ *   grad_rows[row_of[t*k + j]] = weights[t, j] * grad_out[t]   (rows' dtype;
+ *                                rows from starts[E] on are zero)
+ *   grad_weights[t*k + j]      = <grad_out[t], rows[row_of[t*k + j]]>
+ * Either may be NULL; rows may be NULL without grad_weights.  grad_rows must
+ * not overlap rows. */
+aem_status aem_combine_backward(const void* grad_out, aem_dtype out_dtype, int64_t ldg,
+                                const void* rows, aem_dtype rows_dtype, int64_t ldr,
+                                const float* weights, int64_t ldw, const int32_t* row_of,
+                                const int32_t* starts, int64_t T, int k, int E, int64_t d,
+                                void* grad_rows, int64_t ldgr, float* grad_weights, void* stream);
+
+/* ---- 4-bit weights with group scales ------------------------------------------------ */
+
+/* Symmetric 4-bit quantisation of w [G][K][N] (float32 or bf16, device): the
+ * group_size (32, 64 or 128) consecutive k of a column share
+ *   scale = max(max |w| / 7, 1e-12), rounded to scale_dtype,
+ *   q     = clip(rint(w / scale), -7, 7)   with that rounded scale,
+ * in IEEE float32.  q int8 [G][K][N], scale [G][ceil(K/group_size)][N]; the
+ * last group of a column may be short.  The reference quantises to 8 bits
+ * only (src/kernels/quantized_gemm.py:70-76). */
+aem_status aem_quantize_q4(const void* w, aem_dtype w_dtype, int64_t G, int64_t K, int64_t N,
+                           int group_size, int8_t* q, void* scale, aem_dtype scale_dtype,
+                           void* stream);
+
+typedef struct aem_q4weight_s* aem_q4weight_t;
+
+/* Packs G groups (experts) of 4-bit weights, q [G][K][N] int8 holding values
+ * in [-8, 7] and scale [G][ceil(K/group_size)][N] (float32 or bf16, kept as
+ * given), into a device-resident copy of K*N/2 bytes per group laid out as
+ * the product's matrix fragments.  Same from HOST memory (a value outside
+ * [-8, 7] -> AEM_EINVAL) and from DEVICE memory (stream-ordered; such a value
+ * is clamped and reported by aem_device_status). */
+aem_status aem_q4weight_pack(const int8_t* q, const void* scale, aem_dtype scale_dtype, int64_t G,
+                             int64_t K, int64_t N, int group_size, int device, aem_q4weight_t* out);
+aem_status aem_q4weight_pack_device(const int8_t* q, const void* scale, aem_dtype scale_dtype,
+                                    int64_t G, int64_t K, int64_t N, int group_size, void* stream,
+                                    aem_q4weight_t* out);
+aem_status aem_q4weight_free(aem_q4weight_t w);
+/* Dimensions of a packed weight (any pointer may be NULL). */
+aem_status aem_q4weight_shape(aem_q4weight_t w, int64_t* G, int64_t* K, int64_t* N, int* group_size);
+
+/* out[M, N] = x[M, K] @ (q[group] * scale[group]) for the few rows of a
+ * decoding step: one pass over the weights for up to 64 bf16 or 21 float32
+ * rows, one more for every further such tile of rows.  The integers are
+ * exact in the MMAs' bf16 operands, each scale multiplies a float32 sum, and
+ * float32 x takes part in full (three bf16 terms), so nothing is rounded
+ * before out.  Rows of x are ldx elements apart, rows of out ldo; any
+ * alignment works, 16-byte rows with K % 8 == 0 run fastest.  The weights'
+ * device must be the current one.  Results repeat bit for bit. */
+aem_status aem_q4gemm(aem_q4weight_t w, int64_t group, const void* x, aem_dtype x_dtype,
+                      int64_t ldx, int64_t M, void* out, aem_dtype out_dtype, int64_t ldo,
+                      void* stream);
+/* Grouped form (expert products of dispatched rows): rows
+ * [group_rows[g], group_rows[g+1]) of x (device int32 array of G+1 increasing
+ * offsets: aem_dispatch's starts) times weight group g, for all G <=
+ * AEM_MAX_EXPERTS groups of w, with out = relu(...) when relu != 0.  Offsets
+ * are clamped to [0, M]; rows of out outside every group are not written. */
+aem_status aem_grouped_q4gemm(aem_q4weight_t w, const int32_t* group_rows, const void* x,
+                              aem_dtype x_dtype, int64_t ldx, int64_t M, void* out,
+                              aem_dtype out_dtype, int64_t ldo, int relu, void* stream);
+
 /* ---- MoE layer (gating -> routing -> grouped INT8 expert FFN -> combine) --------- */
 
 typedef struct {
