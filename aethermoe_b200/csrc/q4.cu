@@ -30,8 +30,8 @@ namespace aem {
 // k = 32h + 8t + 4(i & 1) + {0..3} for its words i = 0..3, h = i >> 1: nibble
 // pair r of a word (bits 4r and 16 + 4r) is A register r of MMA i, i.e. the
 // k offsets {0,1} (r < 2) or {2,3} of channel c + 8*(r & 1).  The nibble is
-// q + 8; padding holds 8.  scale: [G][KB][NT][8][2], channel c of a tile
-// beside channel c + 8, in the caller's type, padding zero.
+// q + 8; padding holds 8.  scale: [G][KB][NT/2][8][4], channels c, c+8, c+16,
+// c+24 of 32 side by side, in the caller's type, padding zero.
 struct Q4Weight {
     int device = 0;
     int64_t G = 0, K = 0, N = 0, NT = 0, KT = 0, KB = 0;
@@ -43,7 +43,7 @@ struct Q4Weight {
 
 namespace {
 
-constexpr int kThreads = 256, kWarps = 8;
+constexpr int kThreads = 256, kWarps = 8;  // quantise, pack
 
 // ------------------------------------------------------------------ quantise
 // One block per (128 columns, scale group): warp w holds rows w, w+8, ... of
@@ -160,31 +160,41 @@ __global__ void __launch_bounds__(kThreads)
     for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < total;
          i += static_cast<int64_t>(gridDim.x) * kThreads) {
         const int64_t b = i / (NT * 16), r = i % (NT * 16);
-        const int64_t n = r / 16 * 16 + (r & 1) * 8 + (r % 16) / 2;
+        const int64_t n = r / 32 * 32 + (r & 3) * 8 + (r % 32) / 4;
         out[i] = n < N ? s[b * N + n] : ST(0.0f);
     }
 }
 
 // ------------------------------------------------------------------ product
+// Columns of the MMAs: the rows of x as they are (bf16), or three per row
+// (float32: the terms that add up to it).
 struct Q4Args {
     const uint4* q;
     const void* scale;
-    const void* x;
+    const __nv_bfloat16* x;     // [M * terms][ldx], 16-byte rows, readable to a multiple of 8 k
     void* out;
     const int32_t* group_rows;  // nullptr: one group of M rows, weight group `group`
     int64_t ldx, ldo, M, K, N, NT, KT, KB;
     int64_t group;
-    int G, gs, S, rows;  // S: CTAs (one cluster) that split K; rows: rows of a row tile
-    bool scale_bf16, out_bf16, relu;
+    int G, S, rows, terms;  // S: CTAs (one cluster) that split K; rows: rows of a row tile
+    bool out_bf16, relu, dependent;
 };
 
+template <bool ZERO>
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                          uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    if constexpr (ZERO)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+            "{%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+            "{%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // Eight 4-bit weights -> four bf16 pairs.  0x4300 is bf16 128, whose last
@@ -200,60 +210,35 @@ __device__ __forceinline__ void unpack_q4(uint32_t w, uint32_t (&a)[4]) {
     }
 }
 
-// Upper halves of two float32 bit patterns as a bf16 pair.
-__device__ __forceinline__ uint32_t pack_hi(float a, float b) {
-    return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
-}
-
-// Term `m1, m2` of a float32: masks 0, 0 give v (its upper half is the first
-// term), ~0, 0 what the first term leaves, ~0, ~0 what the first two leave
-// (truncated terms: the differences are exact).  An infinity is all in the
-// first term.
-__device__ __forceinline__ float f32_term(float v, uint32_t m1, uint32_t m2) {
-    float r = v - __uint_as_float(__float_as_uint(v) & m1);
-    r = r - __uint_as_float(__float_as_uint(r) & m2);
-    return r == r || m1 == 0 ? r : 0.0f;
-}
-
-// The lane's B fragments of one 64-k tile and one 8-column tile: b[i] of MMA
-// i.  p: the column's activation row (nullptr: column unused, zeros).
-template <bool F32, bool FAST>
-__device__ __forceinline__ void load_x(const void* p, int64_t k0, int64_t K, uint32_t m1,
-                                       uint32_t m2, uint32_t (&b)[4][2]) {
+// Activations in the form the products read: [M * terms][KP] bf16, KP = K
+// rounded up to 8, zero padded.  float32 gives three truncated terms v =
+// t0 + t1 + t2 (8 mantissa bits each, every difference exact; an infinity or
+// NaN is all in t0), bf16 is copied (rows that are not 16-byte aligned).
+template <typename XT>
+__global__ void __launch_bounds__(kThreads)
+    q4_terms_kernel(const XT* __restrict__ x, int64_t ldx, int64_t M, int64_t K, int64_t KP,
+                    __nv_bfloat16* __restrict__ out) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int64_t total = M * KP;
+    for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < total;
+         i += static_cast<int64_t>(gridDim.x) * kThreads) {
+        const int64_t m = i / KP, k = i - m * KP;
+        if constexpr (sizeof(XT) == 2) {
+            out[i] = k < K ? x[m * ldx + k] : __float2bfloat16_rn(0.0f);
+        } else {
+            const float v = k < K ? x[m * ldx + k] : 0.0f;
+            const uint32_t u = __float_as_uint(v);
+            float r1 = v - __uint_as_float(u & 0xffff0000u);
+            if ((u & 0x7f800000u) == 0x7f800000u) r1 = 0.0f;
+            const float r2 = r1 - __uint_as_float(__float_as_uint(r1) & 0xffff0000u);
+            const float t[3] = {v, r1, r2};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int64_t k = k0 + 32 * h;
-        uint32_t u[4] = {0, 0, 0, 0};
-        if constexpr (FAST) {  // 16-byte rows, K a multiple of 8
-            if (p && k < K) {
-                if constexpr (F32) {
-                    const float4* f = reinterpret_cast<const float4*>(static_cast<const float*>(p) + k);
-                    const float4 lo = __ldg(f), hi = __ldg(f + 1);
-                    u[0] = pack_hi(f32_term(lo.x, m1, m2), f32_term(lo.y, m1, m2));
-                    u[1] = pack_hi(f32_term(lo.z, m1, m2), f32_term(lo.w, m1, m2));
-                    u[2] = pack_hi(f32_term(hi.x, m1, m2), f32_term(hi.y, m1, m2));
-                    u[3] = pack_hi(f32_term(hi.z, m1, m2), f32_term(hi.w, m1, m2));
-                } else {
-                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p) + k));
-                    u[0] = v.x, u[1] = v.y, u[2] = v.z, u[3] = v.w;
-                }
-            }
-        } else if (p) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float e[2];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int64_t kk = k + 2 * i + j;
-                    if constexpr (F32)
-                        e[j] = kk < K ? f32_term(static_cast<const float*>(p)[kk], m1, m2) : 0.0f;
-                    else
-                        e[j] = kk < K ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[kk]) : 0.0f;
-                }
-                u[i] = pack_hi(e[0], e[1]);
+            for (int j = 0; j < 3; ++j) {
+                uint16_t h = static_cast<uint16_t>(__float_as_uint(t[j]) >> 16);
+                if (j == 0 && v != v) h = 0x7fff;
+                out[(3 * m + j) * KP + k] = __ushort_as_bfloat16(h);
             }
         }
-        b[2 * h][0] = u[0], b[2 * h][1] = u[1], b[2 * h + 1][0] = u[2], b[2 * h + 1][1] = u[3];
     }
 }
 
@@ -307,14 +292,134 @@ __device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
     return v;
 }
 
-// A CTA computes 32 channels of one row tile; its 8 warps (and the S CTAs of
-// its cluster) split K and their float32 sums are added in a fixed order.
-// NT: 8-column tiles; G32: scale groups of 32 (two per 64-k tile).
-template <int NT, bool F32, bool FAST, bool G32>
-__global__ void __launch_bounds__(kThreads) q4_kernel(const Q4Args a) {
-    constexpr int PF = 4;  // weight tiles in flight
-    constexpr int NS = G32 ? 2 : 1;
-    __shared__ float red[kWarps][NT * 4 * 32];
+// The scales of one lane and scale group: channels c, c+8, c+16, c+24 of 32.
+template <typename ST>
+struct Scales;
+template <>
+struct Scales<float> {
+    float4 v;
+    __device__ __forceinline__ void load(const void* p, int64_t i) {
+        v = __ldg(reinterpret_cast<const float4*>(p) + i);
+    }
+    __device__ __forceinline__ float get(int c, int hi) const {
+        return c ? (hi ? v.w : v.z) : (hi ? v.y : v.x);
+    }
+};
+template <>
+struct Scales<__nv_bfloat16> {
+    uint2 v;
+    __device__ __forceinline__ void load(const void* p, int64_t i) {
+        v = __ldg(reinterpret_cast<const uint2*>(p) + i);
+    }
+    __device__ __forceinline__ float get(int c, int hi) const {
+        const uint32_t u = c ? v.y : v.x;
+        return __uint_as_float(hi ? u & 0xffff0000u : u << 16);
+    }
+};
+
+// The weight stream of one warp: 32 channels, 64-k tiles [kt0, kt1), PF tiles
+// in flight in registers.
+constexpr int PF = 4;
+template <int GS, typename ST>
+struct Stream {
+    static constexpr int NS = GS == 32 ? 2 : 1;
+    uint4 w[PF][2];
+    Scales<ST> s[PF][NS];
+    const uint4* wp;
+    const void* sp;
+    int64_t wstep, s0, sstep;
+    int kt1;
+    int64_t last;
+
+    __device__ __forceinline__ void start(const Q4Args& a, int64_t g, int64_t pair, int end) {
+        const int lane = threadIdx.x & 31;
+        wp = a.q + (g * a.NT + pair * 2) * a.KT * 32 + lane;
+        wstep = a.KT * 32;
+        sp = a.scale;
+        s0 = (g * a.KB * (a.NT / 2) + pair) * 8 + (lane >> 2);
+        sstep = a.NT / 2 * 8;
+        kt1 = end;
+        last = a.KB - 1;
+    }
+    __device__ __forceinline__ void fetch(int slot, int kt) {
+        if (kt >= kt1) return;
+        w[slot][0] = __ldg(wp + static_cast<int64_t>(kt) * 32);
+        w[slot][1] = __ldg(wp + static_cast<int64_t>(kt) * 32 + wstep);
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+            const int64_t b = GS == 32 ? min(static_cast<int64_t>(2 * kt + j), last) : kt / (GS / 64);
+            s[slot][j].load(sp, s0 + b * sstep);
+        }
+    }
+};
+
+// One 64-k tile: NT column tiles of B fragments from `b(nt, h)` (uint4: MMAs
+// 2h and 2h+1) times the 32 channels of w, scaled into acc.  FIRST / LAST:
+// the tile opens / closes a scale group (GS >= 64).
+template <int NT, int GS, typename ST, typename B>
+__device__ __forceinline__ void tile_product(const uint4 (&w)[2], const Scales<ST>* s, bool first,
+                                             bool last, float (&acc)[2][NT][4],
+                                             float (&sum)[2][NT][4], B b) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t wa[2][2][4];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            unpack_q4(h ? w[c].z : w[c].x, wa[c][0]);
+            unpack_q4(h ? w[c].w : w[c].y, wa[c][1]);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const uint4 x = b(nt, h);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                if constexpr (GS == 32) {
+                    float p[4];
+                    mma_bf16<true>(p, wa[c][0], x.x, x.y);
+                    mma_bf16<false>(p, wa[c][1], x.z, x.w);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        acc[c][nt][i] = fmaf(s[h].get(c, i >> 1), p[i], acc[c][nt][i]);
+                } else {
+                    if (h == 0 && first)
+                        mma_bf16<true>(sum[c][nt], wa[c][0], x.x, x.y);
+                    else
+                        mma_bf16<false>(sum[c][nt], wa[c][0], x.x, x.y);
+                    mma_bf16<false>(sum[c][nt], wa[c][1], x.z, x.w);
+                    if (h == 1 && last)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            acc[c][nt][i] = fmaf(s[0].get(c, i >> 1), sum[c][nt][i], acc[c][nt][i]);
+                }
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ void store_out(const Q4Args& a, int64_t m, int64_t n, float v) {
+    if (a.relu && v < 0.0f) v = 0.0f;
+    if (a.out_bf16)
+        static_cast<__nv_bfloat16*>(a.out)[m * a.ldo + n] = __float2bfloat16_rn(v);
+    else
+        static_cast<float*>(a.out)[m * a.ldo + n] = v;
+}
+
+// Part `part` of `parts` of the 64-k tiles, cut at scale groups.
+__device__ __forceinline__ void k_range(const Q4Args& a, int gran, int64_t part, int64_t parts,
+                                        int* kt0, int* kt1) {
+    const int64_t units = (a.KT + gran - 1) / gran;
+    *kt0 = static_cast<int>(units * part / parts * gran);
+    *kt1 = static_cast<int>(min(units * (part + 1) / parts * gran, a.KT));
+}
+
+// Few columns (8 NT <= 16): a CTA computes 32 channels, its 4 warps (and the S
+// CTAs of its cluster) split K, and their float32 sums meet in a fixed order.
+// Each warp reads the B fragments of its own k straight from x (cached), one
+// tile ahead.
+template <int NT, int GS, typename ST>
+__global__ void __launch_bounds__(128) q4_narrow_kernel(const Q4Args a) {
+    constexpr int W = 4;
+    __shared__ float red[W][NT * 8 * 32];
     __shared__ float fin[32][NT * 8 + 1];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int64_t tile = blockIdx.x / a.S;
@@ -322,211 +427,228 @@ __global__ void __launch_bounds__(kThreads) q4_kernel(const Q4Args a) {
     int64_t g, m0;
     int rows;
     if (!find_rows(a, blockIdx.y, &g, &m0, &rows)) return;
+    int kt0, kt1;
+    k_range(a, GS > 64 ? GS / 64 : 1, ks * W + w, a.S * W, &kt0, &kt1);
+    Stream<GS, ST> st;
+    st.start(a, g, tile, kt1);
+#pragma unroll
+    for (int i = 0; i < PF; ++i) st.fetch(i, kt0 + i);
+    if (a.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");  // x is the terms kernel's
 
-    // columns of this lane: B column 8*nt + lane/4
-    const void* xp[NT];
-    uint32_t m1[NT], m2[NT];
+    const __nv_bfloat16* xp[NT];
     const int t8 = 8 * (lane & 3);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int col = 8 * nt + (lane >> 2);
-        const int r = F32 ? col / 3 : col, term = F32 ? col % 3 : 0;
-        m1[nt] = term > 0 ? 0xffff0000u : 0u;
-        m2[nt] = term > 1 ? 0xffff0000u : 0u;
-        xp[nt] = nullptr;
-        if (r < rows) {
-            const int64_t off = (m0 + r) * a.ldx;
-            xp[nt] = F32 ? static_cast<const void*>(static_cast<const float*>(a.x) + off)
-                         : static_cast<const void*>(static_cast<const __nv_bfloat16*>(a.x) + off);
-        }
+        xp[nt] = col < rows * a.terms ? a.x + (m0 * a.terms + col) * a.ldx : nullptr;
     }
-
-    // this warp's 64-k tiles, whole scale groups
-    const int gran = a.gs > 64 ? a.gs / 64 : 1;
-    const int64_t units = (a.KT + gran - 1) / gran;
-    const int64_t part = ks * kWarps + w, parts = a.S * kWarps;
-    const int kt0 = static_cast<int>(units * part / parts * gran);
-    const int kt1 = static_cast<int>(min(units * (part + 1) / parts * gran, a.KT));
-
-    const uint4* wq = a.q + ((g * a.NT + tile * 2) * a.KT) * 32 + lane;
-    const int64_t wstep = a.KT * 32;  // to the second 16 channels
-    const char* sp = static_cast<const char*>(a.scale);
-    const int64_t sbase = ((g * a.KB) * a.NT + tile * 2) * 16 + (lane >> 2) * 2;
-
-    uint4 wr[PF][2];
-    uint2 sr[PF][2][NS];
-    auto fetch = [&](int slot, int kt) {
-        if (kt >= kt1) return;
+    uint4 xb[2][NT][2];
+    auto load_x = [&](int slot, int kt) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            wr[slot][c] = __ldg(wq + static_cast<int64_t>(kt) * 32 + c * wstep);
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int j = 0; j < NS; ++j) {
-                const int64_t b = G32 ? min(static_cast<int64_t>(2 * kt + j), a.KB - 1) : static_cast<int64_t>(kt) * 64 / a.gs;
-                const int64_t at = sbase + b * a.NT * 16 + c * 16;
-                if (a.scale_bf16)
-                    sr[slot][c][j].x = __ldg(reinterpret_cast<const uint32_t*>(sp + at * 2));
-                else
-                    sr[slot][c][j] = __ldg(reinterpret_cast<const uint2*>(sp + at * 4));
+            for (int h = 0; h < 2; ++h) {
+                const int64_t k = kt * 64ll + 32 * h + t8;
+                xb[slot][nt][h] = make_uint4(0, 0, 0, 0);
+                if (xp[nt] && kt < kt1 && k < a.K)
+                    xb[slot][nt][h] = *reinterpret_cast<const uint4*>(xp[nt] + k);
             }
-        }
     };
     float acc[2][NT][4] = {}, sum[2][NT][4] = {};
-    auto apply = [&](int slot, int j) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const uint2 u = sr[slot][c][j];
-            const float s0 = __uint_as_float(a.scale_bf16 ? u.x << 16 : u.x);
-            const float s1 = __uint_as_float(a.scale_bf16 ? u.x & 0xffff0000u : u.y);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    acc[c][nt][i] = fmaf(i < 2 ? s0 : s1, sum[c][nt][i], acc[c][nt][i]);
-                    sum[c][nt][i] = 0.0f;
-                }
-        }
-    };
-#pragma unroll
-    for (int i = 0; i < PF; ++i) fetch(i, kt0 + i);
+    load_x(0, kt0);
     for (int kb = kt0; kb < kt1; kb += PF) {
 #pragma unroll
         for (int i = 0; i < PF; ++i) {
             const int kt = kb + i;
             if (kt >= kt1) break;
-            uint32_t wa[2][4][4];
+            load_x((i + 1) & 1, kt + 1);
+            const uint4 wt[2] = {st.w[i][0], st.w[i][1]};
+            Scales<ST> sc[Stream<GS, ST>::NS];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                unpack_q4(wr[i][c].x, wa[c][0]);
-                unpack_q4(wr[i][c].y, wa[c][1]);
-                unpack_q4(wr[i][c].z, wa[c][2]);
-                unpack_q4(wr[i][c].w, wa[c][3]);
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                uint32_t b[4][2];
-                load_x<F32, FAST>(xp[nt], static_cast<int64_t>(kt) * 64 + t8, a.K, m1[nt], m2[nt], b);
-                if constexpr (G32) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            float p[4] = {0.f, 0.f, 0.f, 0.f};
-                            mma_bf16(p, wa[c][2 * h], b[2 * h][0], b[2 * h][1]);
-                            mma_bf16(p, wa[c][2 * h + 1], b[2 * h + 1][0], b[2 * h + 1][1]);
-                            const uint2 u = sr[i][c][h < NS ? h : 0];
-                            const float s0 = __uint_as_float(a.scale_bf16 ? u.x << 16 : u.x);
-                            const float s1 = __uint_as_float(a.scale_bf16 ? u.x & 0xffff0000u : u.y);
-                            acc[c][nt][0] = fmaf(s0, p[0], acc[c][nt][0]);
-                            acc[c][nt][1] = fmaf(s0, p[1], acc[c][nt][1]);
-                            acc[c][nt][2] = fmaf(s1, p[2], acc[c][nt][2]);
-                            acc[c][nt][3] = fmaf(s1, p[3], acc[c][nt][3]);
-                        }
-                } else {
-#pragma unroll
-                    for (int m = 0; m < 4; ++m)
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) mma_bf16(sum[c][nt], wa[c][m], b[m][0], b[m][1]);
-                }
-            }
-            if constexpr (!G32)
-                if ((kt + 1) % gran == 0 || kt + 1 == kt1) apply(i, 0);
-            fetch(i, kt + PF);
+            for (int j = 0; j < Stream<GS, ST>::NS; ++j) sc[j] = st.s[i][j];
+            st.fetch(i, kt + PF);
+            const bool first = GS <= 64 || i % 2 == 0;
+            const bool last = GS <= 64 || i % 2 == 1 || kt + 1 == kt1;
+            tile_product<NT, GS, ST>(wt, sc, first, last, acc, sum,
+                                     [&](int nt, int h) { return xb[i & 1][nt][h]; });
         }
     }
 
     // the warps' sums, in warp order, into fin[channel][column]
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-        if (c) __syncthreads();
+    for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) red[w][(nt * 4 + i) * 32 + lane] = acc[c][nt][i];
-        __syncthreads();
-        for (int i = threadIdx.x; i < NT * 4 * 32; i += kThreads) {
-            float s = 0.0f;
+            for (int i = 0; i < 4; ++i) red[w][((c * NT + nt) * 4 + i) * 32 + lane] = acc[c][nt][i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < NT * 8 * 32; i += 128) {
+        float s = 0.0f;
 #pragma unroll
-            for (int j = 0; j < kWarps; ++j) s += red[j][i];
-            const int l = i & 31, e = (i >> 5) & 3, nt = i >> 7;
-            fin[c * 16 + (l >> 2) + 8 * (e >> 1)][nt * 8 + 2 * (l & 3) + (e & 1)] = s;
-        }
+        for (int j = 0; j < W; ++j) s += red[j][i];
+        const int l = i & 31, e = (i >> 5) & 3, cn = i >> 7, c = cn / NT, nt = cn % NT;
+        fin[c * 16 + (l >> 2) + 8 * (e >> 1)][nt * 8 + 2 * (l & 3) + (e & 1)] = s;
     }
     __syncthreads();
     if (a.S > 1) cluster_barrier();
-    if (ks == 0) {
-        for (int i = threadIdx.x; i < rows * 32; i += kThreads) {
+    if (ks == 0)
+        for (int i = threadIdx.x; i < rows * 32; i += 128) {
             const int r = i >> 5, ch = i & 31;
             const int64_t n = tile * 32 + ch;
             float v = 0.0f;
             for (int s = 0; s < a.S; ++s)
-#pragma unroll
-                for (int j = 0; j < (F32 ? 3 : 1); ++j) {
-                    const float* p = &fin[ch][F32 ? 3 * r + j : r];
+                for (int j = 0; j < a.terms; ++j) {
+                    const float* p = &fin[ch][r * a.terms + j];
                     v += s == 0 ? *p : ld_cluster(p, s);
                 }
-            if (n >= a.N) continue;
-            if (a.relu && v < 0.0f) v = 0.0f;
-            if (a.out_bf16)
-                static_cast<__nv_bfloat16*>(a.out)[(m0 + r) * a.ldo + n] = __float2bfloat16_rn(v);
-            else
-                static_cast<float*>(a.out)[(m0 + r) * a.ldo + n] = v;
+            if (n < a.N) store_out(a, m0 + r, n, v);
         }
-    }
     if (a.S > 1) cluster_barrier();  // the others' fin stays until rank 0 has read it
 }
 
-template <int NT, bool F32>
-aem_status launch_nt(const Q4Args& a, bool fast, dim3 grid, cudaStream_t s) {
+// Many columns: a CTA computes 128 channels, 32 per warp; the B fragments of a
+// 64-k tile are copied once per CTA into a shared-memory ring, in the order
+// the lanes read them (16 bytes a lane, no bank conflicts).  The S CTAs of
+// the cluster split K; each adds up its share of the channels in rank order.
+template <int NT, int GS, typename ST>
+__global__ void __launch_bounds__(128) q4_wide_kernel(const Q4Args a) {
+    constexpr int W = 4, COLS = 8 * NT, LD = W * 32 + 4;
+    constexpr int kRing = PF * NT * 64 * 16, kFin = COLS * LD * 4;
+    __shared__ __align__(16) char smem[kRing > kFin ? kRing : kFin];
+    auto* ring = reinterpret_cast<uint4*>(smem);  // [PF][NT][2][32]
+    auto* fin = reinterpret_cast<float*>(smem);   // [COLS][LD], after the loop
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int64_t tile = blockIdx.x / a.S;
+    const int ks = blockIdx.x % a.S;
+    int64_t g, m0;
+    int rows;
+    if (!find_rows(a, blockIdx.y, &g, &m0, &rows)) return;
+    int kt0, kt1;
+    k_range(a, GS > 64 ? GS / 64 : 1, ks, a.S, &kt0, &kt1);
+    const int64_t pair = tile * W + w;
+    const bool mine = pair < a.NT / 2;
+    Stream<GS, ST> st;
+    st.start(a, g, mine ? pair : 0, mine ? kt1 : kt0);
+#pragma unroll
+    for (int i = 0; i < PF; ++i) st.fetch(i, kt0 + i);
+    if (a.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    constexpr int COPIES = NT / 2;  // 16-byte pieces per thread: NT * 64 / 128
+    const __nv_bfloat16* src[COPIES];
+    int koff[COPIES];
+#pragma unroll
+    for (int j = 0; j < COPIES; ++j) {
+        const int i = threadIdx.x + 128 * j, l = i & 31;
+        const int col = 8 * (i >> 6) + (l >> 2);
+        koff[j] = 32 * ((i >> 5) & 1) + 8 * (l & 3);
+        src[j] = col < rows * a.terms ? a.x + (m0 * a.terms + col) * a.ldx : nullptr;
+    }
+    auto copy_x = [&](int slot, int kt) {
+        if (kt < kt1)
+#pragma unroll
+            for (int j = 0; j < COPIES; ++j) {
+                const int64_t k = kt * 64ll + koff[j];
+                const bool on = src[j] && k < a.K;
+                const uint32_t to = dev::smem_u32(ring + slot * NT * 64 + threadIdx.x + 128 * j);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to),
+                             "l"(on ? src[j] + k : a.x), "r"(on ? 16 : 0)
+                             : "memory");
+            }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    float acc[2][NT][4] = {}, sum[2][NT][4] = {};
+#pragma unroll
+    for (int i = 0; i < PF - 1; ++i) copy_x(i, kt0 + i);
+    for (int kb = kt0; kb < kt1; kb += PF) {
+#pragma unroll
+        for (int i = 0; i < PF; ++i) {
+            const int kt = kb + i;
+            if (kt >= kt1) break;
+            asm volatile("cp.async.wait_group %0;" ::"n"(PF - 2) : "memory");
+            __syncthreads();  // tile kt has landed; every warp is past tile kt - 1
+            copy_x((i + PF - 1) % PF, kt + PF - 1);
+            const uint4 wt[2] = {st.w[i][0], st.w[i][1]};
+            Scales<ST> sc[Stream<GS, ST>::NS];
+#pragma unroll
+            for (int j = 0; j < Stream<GS, ST>::NS; ++j) sc[j] = st.s[i][j];
+            st.fetch(i, kt + PF);
+            const bool first = GS <= 64 || i % 2 == 0;
+            const bool last = GS <= 64 || i % 2 == 1 || kt + 1 == kt1;
+            if (mine)
+                tile_product<NT, GS, ST>(wt, sc, first, last, acc, sum, [&](int nt, int h) {
+                    return ring[((i * NT + nt) * 2 + h) * 32 + lane];
+                });
+        }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                fin[(nt * 8 + 2 * (lane & 3) + (i & 1)) * LD + w * 32 + c * 16 + (lane >> 2) + 8 * (i >> 1)] =
+                    acc[c][nt][i];
+    __syncthreads();
+    if (a.S > 1) cluster_barrier();
+    for (int i = ks * 128 + threadIdx.x; i < rows * W * 32; i += a.S * 128) {
+        const int r = i / (W * 32), ch = i % (W * 32);
+        const int64_t n = tile * W * 32 + ch;
+        float v = 0.0f;
+        for (int s = 0; s < a.S; ++s)
+            for (int j = 0; j < a.terms; ++j) {
+                const float* p = fin + (r * a.terms + j) * LD + ch;
+                v += s == ks ? *p : ld_cluster(p, s);
+            }
+        if (n < a.N) store_out(a, m0 + r, n, v);
+    }
+    if (a.S > 1) cluster_barrier();
+}
+
+template <int NT, int GS, typename ST>
+aem_status launch_q4(const Q4Args& a, dim3 grid, cudaStream_t s) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(128);
     cfg.stream = s;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = a.S;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = a.S > 1 ? 1 : 0;
-    if (a.gs == 32)
-        AEM_TRY_CUDA(fast ? cudaLaunchKernelEx(&cfg, q4_kernel<NT, F32, true, true>, a)
-                          : cudaLaunchKernelEx(&cfg, q4_kernel<NT, F32, false, true>, a));
+    cudaLaunchAttribute at[2] = {};
+    int n = 0;
+    if (a.S > 1) {
+        at[n].id = cudaLaunchAttributeClusterDimension;
+        at[n].val.clusterDim.x = a.S;
+        at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    if (a.dependent) {
+        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+    }
+    cfg.attrs = at;
+    cfg.numAttrs = n;
+    if constexpr (NT <= 2)
+        AEM_TRY_CUDA(cudaLaunchKernelEx(&cfg, q4_narrow_kernel<NT, GS, ST>, a));
     else
-        AEM_TRY_CUDA(fast ? cudaLaunchKernelEx(&cfg, q4_kernel<NT, F32, true, false>, a)
-                          : cudaLaunchKernelEx(&cfg, q4_kernel<NT, F32, false, false>, a));
+        AEM_TRY_CUDA(cudaLaunchKernelEx(&cfg, q4_wide_kernel<NT, GS, ST>, a));
     count_launches(1);
     return AEM_OK;
 }
 
-template <bool F32>
-aem_status launch_q4(Q4Args a, bool fast, int64_t want_rows, cudaStream_t s) {
-    // columns of a row tile: as many as the rows need, up to 64
-    constexpr int per = F32 ? 3 : 1;
-    int nt = 8;
-    for (int n : {1, 2, 4})
-        if (want_rows * per <= 8 * n) {
-            nt = n;
-            break;
-        }
-    a.rows = 8 * nt / per;
-    const int64_t slots = a.group_rows
-                              ? std::min<int64_t>(a.G, a.M) + a.M / a.rows
-                              : (a.M + a.rows - 1) / a.rows;
-    AEM_REQUIRE(slots <= 65535, "q4 product: M=%lld rows are too many for one call", (long long)a.M);
-    const int64_t tiles = a.NT / 2, ctas = tiles * slots;
-    a.S = 1;
-    while (a.S < 8 && ctas * a.S < 148 * 2 && a.KT >= 2 * kWarps * a.S) a.S *= 2;
-    AEM_REQUIRE(tiles * a.S < (1ll << 31), "q4 product: N=%lld out of range", (long long)a.N);
-    const dim3 grid(static_cast<unsigned>(tiles * a.S), static_cast<unsigned>(slots));
-    switch (nt) {
-        case 1: return launch_nt<1, F32>(a, fast, grid, s);
-        case 2: return launch_nt<2, F32>(a, fast, grid, s);
-        case 4: return launch_nt<4, F32>(a, fast, grid, s);
-        default: return launch_nt<8, F32>(a, fast, grid, s);
-    }
+template <int NT>
+aem_status launch_nt(const Q4Args& a, int gs, bool sb, dim3 grid, cudaStream_t s) {
+    if (sb)
+        return gs == 32   ? launch_q4<NT, 32, __nv_bfloat16>(a, grid, s)
+               : gs == 64 ? launch_q4<NT, 64, __nv_bfloat16>(a, grid, s)
+                          : launch_q4<NT, 128, __nv_bfloat16>(a, grid, s);
+    return gs == 32   ? launch_q4<NT, 32, float>(a, grid, s)
+           : gs == 64 ? launch_q4<NT, 64, float>(a, grid, s)
+                      : launch_q4<NT, 128, float>(a, grid, s);
 }
 
-aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, aem_dtype xd, cudaStream_t s) {
+// x: the caller's rows; a.x and a.terms are set here.
+aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, const void* x, aem_dtype xd,
+                      void* workspace, size_t workspace_bytes, cudaStream_t s) {
     AEM_REQUIRE(current_device() == w->device, "%s: the weights are on device %d, the current one is %d",
                 what, w->device, current_device());
     a.q = w->q;
@@ -536,13 +658,60 @@ aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, aem_dtype x
     a.NT = w->NT;
     a.KT = w->KT;
     a.KB = w->KB;
-    a.gs = w->gs;
-    a.scale_bf16 = w->scale_bf16;
-    const int es = xd == AEM_F32 ? 4 : 2;
-    const bool fast = a.K % 8 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && (a.ldx * es) % 16 == 0;
-    // grouped: the rows that a group has on average
-    const int64_t want = a.group_rows ? (a.M + std::min<int64_t>(a.G, a.M) - 1) / std::min<int64_t>(a.G, a.M) : a.M;
-    return xd == AEM_F32 ? launch_q4<true>(a, fast, want, s) : launch_q4<false>(a, fast, want, s);
+    a.terms = xd == AEM_F32 ? 3 : 1;
+    const bool as_is = xd == AEM_BF16 && a.K % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 &&
+                       a.ldx % 8 == 0;
+    void* own = nullptr;
+    if (as_is) {
+        a.x = static_cast<const __nv_bfloat16*>(x);
+    } else {
+        const int64_t KP = (a.K + 7) / 8 * 8;
+        const size_t need = static_cast<size_t>(a.M) * a.terms * KP * 2;
+        AEM_REQUIRE(!workspace || (workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
+                    "%s: workspace of %zu bytes (%zu needed, 16-byte aligned)", what, workspace_bytes, need);
+        if (!workspace) {
+            AEM_TRY_CUDA(cudaMallocAsync(&own, need, s));
+            workspace = own;
+        }
+        auto* t = static_cast<__nv_bfloat16*>(workspace);
+        const unsigned g = static_cast<unsigned>(std::min<int64_t>((a.M * KP + kThreads - 1) / kThreads, 148 * 8));
+        if (xd == AEM_F32)
+            q4_terms_kernel<float><<<g, kThreads, 0, s>>>(static_cast<const float*>(x), a.ldx, a.M, a.K, KP, t);
+        else
+            q4_terms_kernel<__nv_bfloat16><<<g, kThreads, 0, s>>>(static_cast<const __nv_bfloat16*>(x), a.ldx,
+                                                                  a.M, a.K, KP, t);
+        AEM_CHECK_LAUNCH();
+        count_launches(1);
+        a.x = t;
+        a.ldx = KP;
+        a.dependent = true;
+    }
+    // columns of a row tile: as many as the rows (grouped: an average group's) need, up to 64
+    const int64_t groups = std::min<int64_t>(a.G, a.M);
+    const int64_t want = (a.group_rows ? (a.M + groups - 1) / groups : a.M) * a.terms;
+    const int nt = want <= 8 ? 1 : want <= 16 ? 2 : want <= 32 ? 4 : 8;
+    a.rows = 8 * nt / a.terms;
+    const int64_t slots = a.group_rows ? groups + a.M / a.rows : (a.M + a.rows - 1) / a.rows;
+    const int64_t per = nt <= 2 ? 1 : 4, tiles = (a.NT / 2 + per - 1) / per, ctas = tiles * slots;
+    const int64_t kparts = nt <= 2 ? 4 : 1;  // K shares inside a CTA
+    a.S = 1;
+    while (a.S < 8 && ctas * a.S < 148 * 2 && a.KT >= 4 * kparts * a.S) a.S *= 2;
+    aem_status st = AEM_OK;
+    const dim3 grid(static_cast<unsigned>(tiles * a.S), static_cast<unsigned>(slots));
+    if (slots > 65535) {
+        set_error("%s: M=%lld rows are too many for one call", what, (long long)a.M);
+        st = AEM_EINVAL;
+    } else if (nt == 1) {
+        st = launch_nt<1>(a, w->gs, w->scale_bf16, grid, s);
+    } else if (nt == 2) {
+        st = launch_nt<2>(a, w->gs, w->scale_bf16, grid, s);
+    } else if (nt == 4) {
+        st = launch_nt<4>(a, w->gs, w->scale_bf16, grid, s);
+    } else {
+        st = launch_nt<8>(a, w->gs, w->scale_bf16, grid, s);
+    }
+    if (own) cudaFreeAsync(own, s);
+    return st;
 }
 
 bool is_dtype(aem_dtype t) { return t == AEM_F32 || t == AEM_BF16; }
@@ -728,9 +897,15 @@ aem_status aem_q4weight_shape(aem_q4weight_t wh, int64_t* G, int64_t* K, int64_t
     return AEM_OK;
 }
 
+size_t aem_q4gemm_workspace(aem_q4weight_t wh, aem_dtype x_dtype, int64_t M) {
+    if (!wh || M < 1 || !aem::is_dtype(x_dtype)) return 0;
+    const int64_t KP = (reinterpret_cast<aem::Q4Weight*>(wh)->K + 7) / 8 * 8;
+    return static_cast<size_t>(M) * (x_dtype == AEM_F32 ? 3 : 1) * KP * 2;
+}
+
 aem_status aem_q4gemm(aem_q4weight_t wh, int64_t group, const void* x, aem_dtype x_dtype,
                       int64_t ldx, int64_t M, void* out, aem_dtype out_dtype, int64_t ldo,
-                      void* stream) {
+                      void* workspace, size_t workspace_bytes, void* stream) {
     AEM_REQUIRE(wh != nullptr, "aem_q4gemm: weight handle is NULL");
     auto* w = reinterpret_cast<aem::Q4Weight*>(wh);
     AEM_REQUIRE(group >= 0 && group < w->G, "aem_q4gemm: group %lld out of range [0, %lld)",
@@ -741,7 +916,6 @@ aem_status aem_q4gemm(aem_q4weight_t wh, int64_t group, const void* x, aem_dtype
     if (M == 0) return AEM_OK;
     AEM_REQUIRE(x && out, "aem_q4gemm: NULL buffer");
     aem::Q4Args a{};
-    a.x = x;
     a.ldx = ldx;
     a.out = out;
     a.ldo = ldo;
@@ -749,12 +923,14 @@ aem_status aem_q4gemm(aem_q4weight_t wh, int64_t group, const void* x, aem_dtype
     a.group = group;
     a.G = 1;
     a.out_bf16 = out_dtype == AEM_BF16;
-    return aem::q4_product(w, "aem_q4gemm", a, x_dtype, static_cast<cudaStream_t>(stream));
+    return aem::q4_product(w, "aem_q4gemm", a, x, x_dtype, workspace, workspace_bytes,
+                           static_cast<cudaStream_t>(stream));
 }
 
 aem_status aem_grouped_q4gemm(aem_q4weight_t wh, const int32_t* group_rows, const void* x,
                               aem_dtype x_dtype, int64_t ldx, int64_t M, void* out,
-                              aem_dtype out_dtype, int64_t ldo, int relu, void* stream) {
+                              aem_dtype out_dtype, int64_t ldo, int relu, void* workspace,
+                              size_t workspace_bytes, void* stream) {
     AEM_REQUIRE(wh != nullptr, "aem_grouped_q4gemm: weight handle is NULL");
     auto* w = reinterpret_cast<aem::Q4Weight*>(wh);
     AEM_REQUIRE(w->G <= AEM_MAX_EXPERTS, "aem_grouped_q4gemm: %lld weight groups, at most %d",
@@ -765,7 +941,6 @@ aem_status aem_grouped_q4gemm(aem_q4weight_t wh, const int32_t* group_rows, cons
     if (M == 0) return AEM_OK;
     AEM_REQUIRE(group_rows && x && out, "aem_grouped_q4gemm: NULL buffer");
     aem::Q4Args a{};
-    a.x = x;
     a.ldx = ldx;
     a.out = out;
     a.ldo = ldo;
@@ -774,7 +949,8 @@ aem_status aem_grouped_q4gemm(aem_q4weight_t wh, const int32_t* group_rows, cons
     a.G = static_cast<int>(w->G);
     a.out_bf16 = out_dtype == AEM_BF16;
     a.relu = relu != 0;
-    return aem::q4_product(w, "aem_grouped_q4gemm", a, x_dtype, static_cast<cudaStream_t>(stream));
+    return aem::q4_product(w, "aem_grouped_q4gemm", a, x, x_dtype, workspace, workspace_bytes,
+                           static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -371,19 +371,24 @@ aem_status aem_q4weight_shape(aem_q4weight_t w, int64_t* G, int64_t* K, int64_t*
  * exact in the MMAs' bf16 operands, each scale multiplies a float32 sum, and
  * float32 x takes part in full (three bf16 terms), so nothing is rounded
  * before out.  Rows of x are ldx elements apart, rows of out ldo; any
- * alignment works, 16-byte rows with K % 8 == 0 run fastest.  The weights'
- * device must be the current one.  Results repeat bit for bit. */
+ * alignment works.  bf16 x with 16-byte rows and K % 8 == 0 is read in place;
+ * other x first becomes bf16 terms in the workspace: device scratch of
+ * aem_q4gemm_workspace(w, x_dtype, M) bytes, 16-byte aligned, or NULL to have
+ * the call allocate and free it in stream order.  The weights' device must be
+ * the current one.  Results repeat bit for bit. */
+size_t aem_q4gemm_workspace(aem_q4weight_t w, aem_dtype x_dtype, int64_t M);
 aem_status aem_q4gemm(aem_q4weight_t w, int64_t group, const void* x, aem_dtype x_dtype,
                       int64_t ldx, int64_t M, void* out, aem_dtype out_dtype, int64_t ldo,
-                      void* stream);
+                      void* workspace, size_t workspace_bytes, void* stream);
 /* Grouped form (expert products of dispatched rows): rows
  * [group_rows[g], group_rows[g+1]) of x (device int32 array of G+1 increasing
  * offsets: aem_dispatch's starts) times weight group g, for all G <=
- * AEM_MAX_EXPERTS groups of w, with out = relu(...) when relu != 0.  Offsets
- * are clamped to [0, M]; rows of out outside every group are not written. */
+ * AEM_MAX_EXPERTS groups of w, with out = relu(...) when relu != 0; workspace
+ * as above.  Offsets are clamped to [0, M]; rows of out outside every group are not written. */
 aem_status aem_grouped_q4gemm(aem_q4weight_t w, const int32_t* group_rows, const void* x,
                               aem_dtype x_dtype, int64_t ldx, int64_t M, void* out,
-                              aem_dtype out_dtype, int64_t ldo, int relu, void* stream);
+                              aem_dtype out_dtype, int64_t ldo, int relu, void* workspace,
+                              size_t workspace_bytes, void* stream);
 
 /* ---- MoE layer (gating -> routing -> grouped INT8 expert FFN -> combine) --------- */
 

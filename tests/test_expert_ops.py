@@ -92,8 +92,8 @@ def test_q4_refusals():
     assert L().aem_quantize_q4(P, _lib.F32, 1, 64, 32, 64, P, P, 4, None) == EINVAL
     assert L().aem_quantize_q4(None, _lib.F32, 1, 64, 32, 64, P, P, _lib.F32, None) == EINVAL
     assert L().aem_quantize_q4(P, _lib.F32, 0, 64, 32, 64, P, P, _lib.F32, None) == EINVAL
-    assert L().aem_q4gemm(None, 0, P, _lib.F32, 64, 1, P, _lib.F32, 32, None) == EINVAL
-    assert L().aem_grouped_q4gemm(None, P, P, _lib.F32, 64, 1, P, _lib.F32, 32, 0, None) == EINVAL
+    assert L().aem_q4gemm(None, 0, P, _lib.F32, 64, 1, P, _lib.F32, 32, None, 0, None) == EINVAL
+    assert L().aem_grouped_q4gemm(None, P, P, _lib.F32, 64, 1, P, _lib.F32, 32, 0, None, 0, None) == EINVAL
     assert L().aem_q4weight_shape(None, None, None, None, None) == EINVAL
     assert L().aem_q4weight_free(None) == _lib.AEM_OK
 
