@@ -4,19 +4,23 @@
 // Weight (k, n) of group g of G is q[g][k][n] * scale[g][k / gs][n] with q an
 // integer in [-8, 7] and gs = 32, 64 or 128 consecutive k sharing a scale:
 //   out[m, n] = sum_b scale[b, n] * sum_{k in block b} q[k, n] x[m, k]
-// A 4-bit integer is exact in bf16, so each inner sum runs on warp MMAs
-// (bf16 operands, float32 accumulators) and the scale multiplies its float32
-// result: no rounded weight ever exists.  bf16 x enters as it is; float32 x
-// enters as three bf16 terms that add up to it exactly (8 + 8 + 8 mantissa
-// bits), in three MMA columns whose sums are added at the end.
+// A 4-bit integer is exact in bf16, so each inner sum runs on the tensor cores
+// (tcgen05, bf16 operands, float32 accumulators in TMEM) and the scale
+// multiplies its float32 result: no rounded weight ever exists.  bf16 x enters
+// as it is; float32 x enters as three bf16 terms that add up to it exactly
+// (8 + 8 + 8 mantissa bits), in three MMA columns whose sums are added at the
+// end.
 //
-// What bounds it is the weight stream, K*N/2 bytes plus the scales, so the
-// layout serves that stream: a tile of 16 channels x 64 k is 512 contiguous
-// bytes, 16 per lane, and those 16 bytes are the lane's own A fragments of
-// four m16n8k16 MMAs -- one 16-byte load, no shared memory, no shuffles.
+// What bounds it is the weight stream, K*N/2 bytes plus the scales.  Warp MMAs
+// (mma.sync) cannot keep up with it on this chip: one m16n8k16 occupies its
+// sub-core's tensor pipe for 32 cycles, 12400 cycles for a 4096 x 14336
+// weight and 8 columns, and the time grows with the columns (measured 16.6 us
+// for 1 row, 47.6 us for 64).  So 128 channels are the M of a tcgen05.mma and
+// the weights, converted in registers, are its A operand in tensor memory.
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <new>
 
 #include "common.cuh"
@@ -24,21 +28,20 @@
 
 namespace aem {
 
-// Packed 4-bit weight (device).  q: [G][NT][KT][32][16 B] with NT = channels
-// in tiles of 16 (an even number), KT = ceil(K/64).  In a tile lane
-// l = 4*c + t holds the weights of channels c and c+8 at
-// k = 32h + 8t + 4(i & 1) + {0..3} for its words i = 0..3, h = i >> 1: nibble
-// pair r of a word (bits 4r and 16 + 4r) is A register r of MMA i, i.e. the
-// k offsets {0,1} (r < 2) or {2,3} of channel c + 8*(r & 1).  The nibble is
-// q + 8; padding holds 8.  scale: [G][KB][NT/2][8][4], channels c, c+8, c+16,
-// c+24 of 32 side by side, in the caller's type, padding zero.
+// Packed 4-bit weight (device): [G][NC][NP] blocks of `block` bytes, NC =
+// ceil(N / 128) channel blocks and NP = ceil(K / 128).  A block holds 128
+// channels x 128 k and their scales, so one bulk copy brings both:
+//   [2][2][128][16 B]  weights: 64-k tile, half of it, channel.  The word j
+//                      (of 8) of a channel's tile holds k = 8j .. 8j + 7: the
+//                      pair (8j + 2r, 8j + 2r + 1) at bits 4r and 16 + 4r, as
+//                      q + 8; padding holds 8
+//   [128 / gs][128]    scales in the caller's type; padding is zero
 struct Q4Weight {
     int device = 0;
-    int64_t G = 0, K = 0, N = 0, NT = 0, KT = 0, KB = 0;
-    int gs = 0;
+    int64_t G = 0, K = 0, N = 0, NC = 0, NP = 0;
+    int gs = 0, block = 0;
     bool scale_bf16 = false;
-    uint4* q = nullptr;
-    void* scale = nullptr;
+    uint8_t* data = nullptr;
 };
 
 namespace {
@@ -122,85 +125,69 @@ __global__ void __launch_bounds__(kThreads)
 
 // ------------------------------------------------------------------ pack
 __global__ void __launch_bounds__(kThreads)
-    pack_q4_kernel(const int8_t* __restrict__ q, int64_t K, int64_t N, int64_t NT, int64_t KT,
-                   int64_t tiles, uint4* __restrict__ out, int* err) {
-    const int lane = threadIdx.x & 31, c = lane >> 2, t = lane & 3;
+    pack_q4_kernel(const int8_t* __restrict__ q, int64_t K, int64_t N, int64_t NC, int64_t NP,
+                   int64_t pieces, int block, uint8_t* __restrict__ out, int* err) {
     bool bad = false;
-    for (int64_t tile = blockIdx.x * static_cast<int64_t>(kWarps) + (threadIdx.x >> 5); tile < tiles;
-         tile += static_cast<int64_t>(gridDim.x) * kWarps) {
-        const int64_t kt = tile % KT, nt = tile / KT % NT, g = tile / KT / NT;
+    for (int64_t p = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; p < pieces;
+         p += static_cast<int64_t>(gridDim.x) * kThreads) {
+        const int64_t blk = p >> 9, kp = blk % NP, nc = blk / NP % NC, g = blk / NP / NC;
+        const int64_t n = nc * 128 + (p & 127), k0 = kp * 128 + (p >> 7 & 3) * 32;
         uint32_t word[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            word[i] = 0;
+        for (int j = 0; j < 4; ++j) {
+            word[j] = 0;
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int hi = 0; hi < 2; ++hi) {
-                    const int64_t k = kt * 64 + 32 * (i >> 1) + 8 * t + 4 * (i & 1) + 2 * (r >> 1) + hi;
-                    const int64_t n = nt * 16 + c + 8 * (r & 1);
-                    int v = k < K && n < N ? q[(g * K + k) * N + n] : 0;
-                    if (v < -8 || v > 7) {
-                        bad = true;
-                        v = v < 0 ? -8 : 7;
-                    }
-                    word[i] |= static_cast<uint32_t>(v + 8) << (4 * r + 16 * hi);
+            for (int e = 0; e < 8; ++e) {
+                const int64_t k = k0 + 8 * j + e;
+                int v = k < K && n < N ? q[(g * K + k) * N + n] : 0;
+                if (v < -8 || v > 7) {
+                    bad = true;
+                    v = v < 0 ? -8 : 7;
                 }
+                word[j] |= static_cast<uint32_t>(v + 8) << (4 * (e >> 1) + 16 * (e & 1));
+            }
         }
-        out[tile * 32 + lane] = make_uint4(word[0], word[1], word[2], word[3]);
+        *reinterpret_cast<uint4*>(out + blk * block + (p & 511) * 16) =
+            make_uint4(word[0], word[1], word[2], word[3]);
     }
     if (bad) atomicOr(err, ERR_Q4_VALUE);
 }
 
+// s: [G][KB][N]; per block, `per` rows of 128 scales behind the weights.
 template <typename ST>
 __global__ void __launch_bounds__(kThreads)
-    pack_q4_scale_kernel(const ST* __restrict__ s, int64_t GB, int64_t N, int64_t NT,
-                         ST* __restrict__ out) {
-    const int64_t total = GB * NT * 16;
+    pack_q4_scale_kernel(const ST* __restrict__ s, int64_t KB, int64_t N, int64_t NC, int64_t NP,
+                         int64_t total, int per, int block, uint8_t* __restrict__ out) {
     for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < total;
          i += static_cast<int64_t>(gridDim.x) * kThreads) {
-        const int64_t b = i / (NT * 16), r = i % (NT * 16);
-        const int64_t n = r / 32 * 32 + (r & 3) * 8 + (r % 32) / 4;
-        out[i] = n < N ? s[b * N + n] : ST(0.0f);
+        const int64_t row = i >> 7, blk = row / per, kp = blk % NP, nc = blk / NP % NC, g = blk / NP / NC;
+        const int j = static_cast<int>(row % per);
+        const int64_t n = nc * 128 + (i & 127), b = kp * per + j;
+        reinterpret_cast<ST*>(out + blk * block + 8192)[j * 128 + (i & 127)] =
+            n < N && b < KB ? s[(g * KB + b) * N + n] : ST(0.0f);
     }
 }
 
 // ------------------------------------------------------------------ product
+using namespace aem::dev;
+
 // Columns of the MMAs: the rows of x as they are (bf16), or three per row
 // (float32: the terms that add up to it).
 struct Q4Args {
-    const uint4* q;
-    const void* scale;
-    const __nv_bfloat16* x;     // [M * terms][ldx], 16-byte rows, readable to a multiple of 8 k
+    const uint8_t* w;
     void* out;
     const int32_t* group_rows;  // nullptr: one group of M rows, weight group `group`
-    int64_t ldx, ldo, M, K, N, NT, KT, KB;
+    int64_t ldo, M, N, NC, NP;
     int64_t group;
-    int G, S, rows, terms;  // S: CTAs (one cluster) that split K; rows: rows of a row tile
-    bool out_bf16, relu, dependent;
+    int* err;
+    int G, block, S, rows, terms;  // S: CTAs (one cluster) that split K; rows: rows of a row tile
+    bool scale_bf16, out_bf16, relu, dependent;
 };
-
-template <bool ZERO>
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                         uint32_t b1) {
-    if constexpr (ZERO)
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-            "{%8,%9}, {%10,%10,%10,%10};"
-            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
-    else
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-            "{%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 
 // Eight 4-bit weights -> four bf16 pairs.  0x4300 is bf16 128, whose last
 // mantissa bit is 1: 0x4300 | nibble = 128 + nibble, and subtracting 136
 // leaves q exactly.
-__device__ __forceinline__ void unpack_q4(uint32_t w, uint32_t (&a)[4]) {
+__device__ __forceinline__ void unpack_q4(uint32_t w, uint32_t* a) {
     const __nv_bfloat162 off = __halves2bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308));
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -211,7 +198,7 @@ __device__ __forceinline__ void unpack_q4(uint32_t w, uint32_t (&a)[4]) {
 }
 
 // Activations in the form the products read: [M * terms][KP] bf16, KP = K
-// rounded up to 8, zero padded.  float32 gives three truncated terms v =
+// rounded up to 64, zero padded.  float32 gives three truncated terms v =
 // t0 + t1 + t2 (8 mantissa bits each, every difference exact; an infinity or
 // NaN is all in t0), bf16 is copied (rows that are not 16-byte aligned).
 template <typename XT>
@@ -281,119 +268,10 @@ __device__ __forceinline__ bool find_rows(const Q4Args& a, int64_t slot, int64_t
     return false;
 }
 
-__device__ __forceinline__ void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
-}
 __device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
-    uint32_t at;
     float v;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(dev::smem_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_u32(p, rank)) : "memory");
     return v;
-}
-
-// The scales of one lane and scale group: channels c, c+8, c+16, c+24 of 32.
-template <typename ST>
-struct Scales;
-template <>
-struct Scales<float> {
-    float4 v;
-    __device__ __forceinline__ void load(const void* p, int64_t i) {
-        v = __ldg(reinterpret_cast<const float4*>(p) + i);
-    }
-    __device__ __forceinline__ float get(int c, int hi) const {
-        return c ? (hi ? v.w : v.z) : (hi ? v.y : v.x);
-    }
-};
-template <>
-struct Scales<__nv_bfloat16> {
-    uint2 v;
-    __device__ __forceinline__ void load(const void* p, int64_t i) {
-        v = __ldg(reinterpret_cast<const uint2*>(p) + i);
-    }
-    __device__ __forceinline__ float get(int c, int hi) const {
-        const uint32_t u = c ? v.y : v.x;
-        return __uint_as_float(hi ? u & 0xffff0000u : u << 16);
-    }
-};
-
-// The weight stream of one warp: 32 channels, 64-k tiles [kt0, kt1), PF tiles
-// in flight in registers.
-constexpr int PF = 4;
-template <int GS, typename ST>
-struct Stream {
-    static constexpr int NS = GS == 32 ? 2 : 1;
-    uint4 w[PF][2];
-    Scales<ST> s[PF][NS];
-    const uint4* wp;
-    const void* sp;
-    int64_t wstep, s0, sstep;
-    int kt1;
-    int64_t last;
-
-    __device__ __forceinline__ void start(const Q4Args& a, int64_t g, int64_t pair, int end) {
-        const int lane = threadIdx.x & 31;
-        wp = a.q + (g * a.NT + pair * 2) * a.KT * 32 + lane;
-        wstep = a.KT * 32;
-        sp = a.scale;
-        s0 = (g * a.KB * (a.NT / 2) + pair) * 8 + (lane >> 2);
-        sstep = a.NT / 2 * 8;
-        kt1 = end;
-        last = a.KB - 1;
-    }
-    __device__ __forceinline__ void fetch(int slot, int kt) {
-        if (kt >= kt1) return;
-        w[slot][0] = __ldg(wp + static_cast<int64_t>(kt) * 32);
-        w[slot][1] = __ldg(wp + static_cast<int64_t>(kt) * 32 + wstep);
-#pragma unroll
-        for (int j = 0; j < NS; ++j) {
-            const int64_t b = GS == 32 ? min(static_cast<int64_t>(2 * kt + j), last) : kt / (GS / 64);
-            s[slot][j].load(sp, s0 + b * sstep);
-        }
-    }
-};
-
-// One 64-k tile: NT column tiles of B fragments from `b(nt, h)` (uint4: MMAs
-// 2h and 2h+1) times the 32 channels of w, scaled into acc.  FIRST / LAST:
-// the tile opens / closes a scale group (GS >= 64).
-template <int NT, int GS, typename ST, typename B>
-__device__ __forceinline__ void tile_product(const uint4 (&w)[2], const Scales<ST>* s, bool first,
-                                             bool last, float (&acc)[2][NT][4],
-                                             float (&sum)[2][NT][4], B b) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        uint32_t wa[2][2][4];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            unpack_q4(h ? w[c].z : w[c].x, wa[c][0]);
-            unpack_q4(h ? w[c].w : w[c].y, wa[c][1]);
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const uint4 x = b(nt, h);
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                if constexpr (GS == 32) {
-                    float p[4];
-                    mma_bf16<true>(p, wa[c][0], x.x, x.y);
-                    mma_bf16<false>(p, wa[c][1], x.z, x.w);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        acc[c][nt][i] = fmaf(s[h].get(c, i >> 1), p[i], acc[c][nt][i]);
-                } else {
-                    if (h == 0 && first)
-                        mma_bf16<true>(sum[c][nt], wa[c][0], x.x, x.y);
-                    else
-                        mma_bf16<false>(sum[c][nt], wa[c][0], x.x, x.y);
-                    mma_bf16<false>(sum[c][nt], wa[c][1], x.z, x.w);
-                    if (h == 1 && last)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            acc[c][nt][i] = fmaf(s[0].get(c, i >> 1), sum[c][nt][i], acc[c][nt][i]);
-                }
-            }
-        }
-    }
 }
 
 __device__ __forceinline__ void store_out(const Q4Args& a, int64_t m, int64_t n, float v) {
@@ -404,213 +282,272 @@ __device__ __forceinline__ void store_out(const Q4Args& a, int64_t m, int64_t n,
         static_cast<float*>(a.out)[m * a.ldo + n] = v;
 }
 
-// Part `part` of `parts` of the 64-k tiles, cut at scale groups.
-__device__ __forceinline__ void k_range(const Q4Args& a, int gran, int64_t part, int64_t parts,
-                                        int* kt0, int* kt1) {
-    const int64_t units = (a.KT + gran - 1) / gran;
-    *kt0 = static_cast<int>(units * part / parts * gran);
-    *kt1 = static_cast<int>(min(units * (part + 1) / parts * gran, a.KT));
-}
+// Shape of the product kernel for COLS MMA columns and scale groups of GS k.
+// Work moves in pairs of 64-k tiles.  A batch is what one accumulator buffer
+// takes before the scales are applied: a pair, with one accumulator per scale
+// group side by side, or a single tile where that would need too many columns.
+template <int COLS, int GS>
+struct Q4Cfg {
+    static constexpr int RES = COLS <= 32 ? 2 : 1;     // CTAs per SM
+    static constexpr int TMEM = 512 / RES;
+    static constexpr int TW = TMEM / 2;                // columns of one warpgroup
+    static constexpr int BK = GS == 32 && COLS > 16 ? 1 : 2;  // tiles per batch
+    static constexpr int SUB = GS == 128 ? 1 : BK * 64 / GS;  // accumulators per batch
+    static constexpr int NA = RES == 2 ? 2 : 4;        // weight tiles in TMEM
+    static constexpr int ND_RAW = (TW - 32 * NA) / (SUB * COLS);
+    static constexpr int ND = ND_RAW > 2 ? 2 : ND_RAW;  // accumulator buffers
+    static constexpr int XB = COLS * 128;              // bytes of an activation tile
+    static constexpr int NSC = 128 / GS;               // scale groups of a pair
+    // a pair's activations, then its block of weights and scales
+    static constexpr int STAGE = 2 * XB + 8192 + (NSC * 512 + 1023) / 1024 * 1024;
+    // an even ring: a stage always comes back to the warpgroup that saw its
+    // previous phase, so no parity wait can mistake a phase for the one two back
+    static constexpr int FIT = ((228 / RES - 1) * 1024 - 2048) / STAGE / 2 * 2;
+    static constexpr int NS = FIT > 8 ? 8 : FIT;
+    static constexpr int LD = 128 + 4;
+    static constexpr int BARS = 2 * NS + 2 * (2 * NA + 2 * ND);
+    static constexpr int USED = 1024 + NS * STAGE + BARS * 8 + 16;
+    // no more CTAs on an SM than TMEM holds: none ever waits for its columns
+    static constexpr int FLOOR = 228 * 1024 / (RES + 1) + 1024;
+    static constexpr int SMEM = USED > FLOOR ? USED : FLOOR;
+    static_assert(ND >= 1 && NS >= 4 && NS * STAGE >= COLS * LD * 4 && SMEM <= (228 / RES - 1) * 1024, "budgets");
+};
+constexpr int kQ4Threads = 12 * 32;
 
-// Few columns (8 NT <= 16): a CTA computes 32 channels, its 4 warps (and the S
-// CTAs of its cluster) split K, and their float32 sums meet in a fixed order.
-// Each warp reads the B fragments of its own k straight from x (cached), one
-// tile ahead.
-template <int NT, int GS, typename ST>
-__global__ void __launch_bounds__(128) q4_narrow_kernel(const Q4Args a) {
-    constexpr int W = 4;
-    __shared__ float red[W][NT * 8 * 32];
-    __shared__ float fin[32][NT * 8 + 1];
+// A CTA computes 128 channels of one row tile over its part of K:
+//   warps 0-7   two warpgroups, thread = channel = TMEM lane, that take the
+//               pairs of 64-k tiles in turn: the channel's 4-bit weights come
+//               from the shared-memory ring, 32 columns of bf16 pairs a tile
+//               go to tensor memory, and one batch later the finished
+//               accumulator comes back and scale * sum is added to float32
+//               registers.
+//   warps 8-9   one per warpgroup, issue its MMAs (M = 128 channels, N =
+//               columns, K = 16).
+//   warp 10     copies the weights, one 8 KB bulk copy per pair.
+//   warp 11     copies the activations, one TMA box per pair (128-byte swizzle).
+// The S CTAs of a cluster take parts of K; their sums are added in rank order.
+// Every wait is bounded; a timeout sets the error word and ends all roles.
+// (Weights held in registers ahead of their use stay one tile ahead at most,
+// whatever the depth written: a warp has too few load scoreboards.  The ring
+// replaced that form, 28 us for one row.)
+template <int COLS, int GS>
+__global__ void __launch_bounds__(kQ4Threads, Q4Cfg<COLS, GS>::RES)
+    q4_kernel(const __grid_constant__ CUtensorMap xmap, const Q4Args a) {
+    using C = Q4Cfg<COLS, GS>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                               ~static_cast<uintptr_t>(1023));
+    float* fin = reinterpret_cast<float*>(ring);  // [COLS][LD], after the loop
+    uint64_t* in_full = reinterpret_cast<uint64_t*>(ring + C::NS * C::STAGE);
+    uint64_t* in_empty = in_full + C::NS;
+    uint64_t* wg_bars = in_empty + C::NS;  // per warpgroup: a_full, a_empty, d_full, d_empty
+    constexpr int WB = 2 * C::NA + 2 * C::ND;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(wg_bars + 2 * WB);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int64_t tile = blockIdx.x / a.S;
     const int ks = blockIdx.x % a.S;
     int64_t g, m0;
     int rows;
-    if (!find_rows(a, blockIdx.y, &g, &m0, &rows)) return;
-    int kt0, kt1;
-    k_range(a, GS > 64 ? GS / 64 : 1, ks * W + w, a.S * W, &kt0, &kt1);
-    Stream<GS, ST> st;
-    st.start(a, g, tile, kt1);
-#pragma unroll
-    for (int i = 0; i < PF; ++i) st.fetch(i, kt0 + i);
-    if (a.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");  // x is the terms kernel's
+    if (!find_rows(a, blockIdx.y, &g, &m0, &rows)) return;  // the whole cluster alike
+    const int cols = rows * a.terms;
+    const int p0 = static_cast<int>(a.NP * ks / a.S), np = static_cast<int>(a.NP * (ks + 1) / a.S) - p0;
 
-    const __nv_bfloat16* xp[NT];
-    const int t8 = 8 * (lane & 3);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const int col = 8 * nt + (lane >> 2);
-        xp[nt] = col < rows * a.terms ? a.x + (m0 * a.terms + col) * a.ldx : nullptr;
-    }
-    uint4 xb[2][NT][2];
-    auto load_x = [&](int slot, int kt) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int64_t k = kt * 64ll + 32 * h + t8;
-                xb[slot][nt][h] = make_uint4(0, 0, 0, 0);
-                if (xp[nt] && kt < kt1 && k < a.K)
-                    xb[slot][nt][h] = *reinterpret_cast<const uint4*>(xp[nt] + k);
-            }
-    };
-    float acc[2][NT][4] = {}, sum[2][NT][4] = {};
-    load_x(0, kt0);
-    for (int kb = kt0; kb < kt1; kb += PF) {
-#pragma unroll
-        for (int i = 0; i < PF; ++i) {
-            const int kt = kb + i;
-            if (kt >= kt1) break;
-            load_x((i + 1) & 1, kt + 1);
-            const uint4 wt[2] = {st.w[i][0], st.w[i][1]};
-            Scales<ST> sc[Stream<GS, ST>::NS];
-#pragma unroll
-            for (int j = 0; j < Stream<GS, ST>::NS; ++j) sc[j] = st.s[i][j];
-            st.fetch(i, kt + PF);
-            const bool first = GS <= 64 || i % 2 == 0;
-            const bool last = GS <= 64 || i % 2 == 1 || kt + 1 == kt1;
-            tile_product<NT, GS, ST>(wt, sc, first, last, acc, sum,
-                                     [&](int nt, int h) { return xb[i & 1][nt][h]; });
+    if (threadIdx.x == 8 * 32) {
+        for (int i = 0; i < C::NS; ++i) {
+            mbar_init(&in_full[i], 2);   // both copies
+            mbar_init(&in_empty[i], 5);  // four warps, the MMAs' commit
         }
+        for (int j = 0; j < 2; ++j)
+            for (int i = 0; i < WB; ++i)  // a_full and d_empty: four warps; the others: a commit
+                mbar_init(&wg_bars[j * WB + i], i < C::NA || i >= 2 * C::NA + C::ND ? 4 : 1);
+        *abort_flag = 0;
+        fence_barrier_init();
     }
+    if (w == 9) {
+        tmem_alloc(tmem_slot, C::TMEM);
+        tmem_relinquish();
+    }
+    if (w == 11 && lane == 0) tma_prefetch_desc(&xmap);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
 
-    // the warps' sums, in warp order, into fin[channel][column]
+    const int wg = w < 8 ? w >> 2 : w & 1;  // the warpgroup a channel or MMA warp belongs to
+    uint64_t* a_full = wg_bars + wg * WB;
+    uint64_t* a_empty = a_full + C::NA;
+    uint64_t* d_full = a_empty + C::NA;
+    uint64_t* d_empty = d_full + C::ND;
+    const uint32_t tw = tmem + static_cast<uint32_t>(wg * C::TW);  // accumulators, then weight tiles
+    const uint32_t ta = tw + C::ND * C::SUB * COLS;
+    auto wait = [&](uint64_t* bar, int phase) {  // whole warps
+        return __all_sync(~0u, mbar_wait_bounded(bar, phase & 1, abort_flag, a.err, ERR_GEMM_TIMEOUT)) != 0;
+    };
+
+    float acc[COLS] = {};
+    const int ch = threadIdx.x & 127;
+    if (w < 8) {
+        const uint32_t quarter = static_cast<uint32_t>(32 * (w & 3)) << 16;
+        auto take = [&](int b, const float (&s)[C::SUB]) {  // batch b's sums, scaled
+            if (!wait(&d_full[b % C::ND], b / C::ND)) return false;
+            tc_fence_after();
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
+            for (int j = 0; j < C::SUB; ++j) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+                for (int c = 0; c < COLS; c += 16) {
+                    if (c >= cols) continue;
+                    uint32_t r[16];
+                    tc_ld_32x32b_x16(tw + quarter + (b % C::ND * C::SUB + j) * COLS + c, r);
+                    tc_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) red[w][((c * NT + nt) * 4 + i) * 32 + lane] = acc[c][nt][i];
-    __syncthreads();
-    for (int i = threadIdx.x; i < NT * 8 * 32; i += 128) {
-        float s = 0.0f;
-#pragma unroll
-        for (int j = 0; j < W; ++j) s += red[j][i];
-        const int l = i & 31, e = (i >> 5) & 3, cn = i >> 7, c = cn / NT, nt = cn % NT;
-        fin[c * 16 + (l >> 2) + 8 * (e >> 1)][nt * 8 + 2 * (l & 3) + (e & 1)] = s;
-    }
-    __syncthreads();
-    if (a.S > 1) cluster_barrier();
-    if (ks == 0)
-        for (int i = threadIdx.x; i < rows * 32; i += 128) {
-            const int r = i >> 5, ch = i & 31;
-            const int64_t n = tile * 32 + ch;
-            float v = 0.0f;
-            for (int s = 0; s < a.S; ++s)
-                for (int j = 0; j < a.terms; ++j) {
-                    const float* p = &fin[ch][r * a.terms + j];
-                    v += s == 0 ? *p : ld_cluster(p, s);
+                    for (int i = 0; i < 16; ++i) acc[c + i] = fmaf(s[j], __uint_as_float(r[i]), acc[c + i]);
                 }
-            if (n < a.N) store_out(a, m0 + r, n, v);
-        }
-    if (a.S > 1) cluster_barrier();  // the others' fin stays until rank 0 has read it
-}
-
-// Many columns: a CTA computes 128 channels, 32 per warp; the B fragments of a
-// 64-k tile are copied once per CTA into a shared-memory ring, in the order
-// the lanes read them (16 bytes a lane, no bank conflicts).  The S CTAs of
-// the cluster split K; each adds up its share of the channels in rank order.
-template <int NT, int GS, typename ST>
-__global__ void __launch_bounds__(128) q4_wide_kernel(const Q4Args a) {
-    constexpr int W = 4, COLS = 8 * NT, LD = W * 32 + 4;
-    constexpr int kRing = PF * NT * 64 * 16, kFin = COLS * LD * 4;
-    __shared__ __align__(16) char smem[kRing > kFin ? kRing : kFin];
-    auto* ring = reinterpret_cast<uint4*>(smem);  // [PF][NT][2][32]
-    auto* fin = reinterpret_cast<float*>(smem);   // [COLS][LD], after the loop
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int64_t tile = blockIdx.x / a.S;
-    const int ks = blockIdx.x % a.S;
-    int64_t g, m0;
-    int rows;
-    if (!find_rows(a, blockIdx.y, &g, &m0, &rows)) return;
-    int kt0, kt1;
-    k_range(a, GS > 64 ? GS / 64 : 1, ks, a.S, &kt0, &kt1);
-    const int64_t pair = tile * W + w;
-    const bool mine = pair < a.NT / 2;
-    Stream<GS, ST> st;
-    st.start(a, g, mine ? pair : 0, mine ? kt1 : kt0);
-#pragma unroll
-    for (int i = 0; i < PF; ++i) st.fetch(i, kt0 + i);
-    if (a.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
-
-    constexpr int COPIES = NT / 2;  // 16-byte pieces per thread: NT * 64 / 128
-    const __nv_bfloat16* src[COPIES];
-    int koff[COPIES];
-#pragma unroll
-    for (int j = 0; j < COPIES; ++j) {
-        const int i = threadIdx.x + 128 * j, l = i & 31;
-        const int col = 8 * (i >> 6) + (l >> 2);
-        koff[j] = 32 * ((i >> 5) & 1) + 8 * (l & 3);
-        src[j] = col < rows * a.terms ? a.x + (m0 * a.terms + col) * a.ldx : nullptr;
-    }
-    auto copy_x = [&](int slot, int kt) {
-        if (kt < kt1)
-#pragma unroll
-            for (int j = 0; j < COPIES; ++j) {
-                const int64_t k = kt * 64ll + koff[j];
-                const bool on = src[j] && k < a.K;
-                const uint32_t to = dev::smem_u32(ring + slot * NT * 64 + threadIdx.x + 128 * j);
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to),
-                             "l"(on ? src[j] + k : a.x), "r"(on ? 16 : 0)
-                             : "memory");
             }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    float acc[2][NT][4] = {}, sum[2][NT][4] = {};
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&d_empty[b % C::ND]);
+            return true;
+        };
+        float s_prev[C::SUB];
+        int n = 0, b = 0;  // tiles and batches of this warpgroup so far
+        bool ok = true;
+        for (int p = wg; ok && p < np; p += 2) {
+            const uint8_t* st = ring + p % C::NS * C::STAGE + 2 * C::XB;
+            ok = wait(&in_full[p % C::NS], p / C::NS);
+            if (!ok) break;
+            float s[C::NSC];
 #pragma unroll
-    for (int i = 0; i < PF - 1; ++i) copy_x(i, kt0 + i);
-    for (int kb = kt0; kb < kt1; kb += PF) {
+            for (int j = 0; j < C::NSC; ++j)
+                s[j] = a.scale_bf16
+                           ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(st + 8192)[j * 128 + ch])
+                           : reinterpret_cast<const float*>(st + 8192)[j * 128 + ch];
 #pragma unroll
-        for (int i = 0; i < PF; ++i) {
-            const int kt = kb + i;
-            if (kt >= kt1) break;
-            asm volatile("cp.async.wait_group %0;" ::"n"(PF - 2) : "memory");
-            __syncthreads();  // tile kt has landed; every warp is past tile kt - 1
-            copy_x((i + PF - 1) % PF, kt + PF - 1);
-            const uint4 wt[2] = {st.w[i][0], st.w[i][1]};
-            Scales<ST> sc[Stream<GS, ST>::NS];
+            for (int j = 0; j < 2; ++j) {
+                const uint4 q0 = *reinterpret_cast<const uint4*>(st + j * 4096 + ch * 16);
+                const uint4 q1 = *reinterpret_cast<const uint4*>(st + j * 4096 + 2048 + ch * 16);
+                const int slot = n % C::NA;
+                ok = ok && wait(&a_empty[slot], n / C::NA + 1);
+                if (!ok) break;
+                tc_fence_after();
+                uint32_t v[16];
+                unpack_q4(q0.x, v), unpack_q4(q0.y, v + 4), unpack_q4(q0.z, v + 8), unpack_q4(q0.w, v + 12);
+                tc_st_32x32b_x16(ta + quarter + 32 * slot, v);
+                unpack_q4(q1.x, v), unpack_q4(q1.y, v + 4), unpack_q4(q1.z, v + 8), unpack_q4(q1.w, v + 12);
+                tc_st_32x32b_x16(ta + quarter + 32 * slot + 16, v);
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&a_full[slot]);
+                    if (j == 1) mbar_arrive(&in_empty[p % C::NS]);
+                }
+                ++n;
+                if (C::BK == 1 || j == 1) {  // batch b is converted; the one before is done or nearly
+                    if (b) ok = take(b - 1, s_prev);
+                    ++b;
 #pragma unroll
-            for (int j = 0; j < Stream<GS, ST>::NS; ++j) sc[j] = st.s[i][j];
-            st.fetch(i, kt + PF);
-            const bool first = GS <= 64 || i % 2 == 0;
-            const bool last = GS <= 64 || i % 2 == 1 || kt + 1 == kt1;
-            if (mine)
-                tile_product<NT, GS, ST>(wt, sc, first, last, acc, sum, [&](int nt, int h) {
-                    return ring[((i * NT + nt) * 2 + h) * 32 + lane];
-                });
+                    for (int i = 0; i < C::SUB; ++i) s_prev[i] = s[C::BK == 2 ? i : j * C::SUB + i];
+                }
+            }
         }
+        if (ok && b) take(b - 1, s_prev);
+    } else if (w < 10) {
+        const uint32_t idesc = idesc_bf16_f32(128, static_cast<uint32_t>((cols + 15) & ~15));
+        int n = 0, b = 0;
+        bool ok = true;
+        for (int p = wg; ok && p < np; p += 2) {
+            ok = wait(&in_full[p % C::NS], p / C::NS);
+            const uint64_t bd = smem_desc_sw128(smem_u32(ring + p % C::NS * C::STAGE));
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                if (C::BK == 1 || j == 0) ok = ok && wait(&d_empty[b % C::ND], b / C::ND + 1);
+                const int slot = n % C::NA;
+                ok = ok && wait(&a_full[slot], n / C::NA);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t d = tw + static_cast<uint32_t>(b % C::ND * C::SUB * COLS);
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    const int grp = (C::BK == 2 ? 64 * j : 0) + 16 * m;  // k inside the batch
+                    tc_mma_f16_ts_elect(d + grp / GS * COLS, ta + 32 * slot + 8 * m,
+                                        bd + j * (C::XB >> 4) + 2 * m, idesc, grp % GS ? 1u : 0u);
+                }
+                tc_commit_elect(&a_empty[slot]);
+                ++n;
+                if (j == 1) tc_commit_elect(&in_empty[p % C::NS]);
+                if (C::BK == 1 || j == 1) {
+                    tc_commit_elect(&d_full[b % C::ND]);
+                    ++b;
+                }
+            }
+        }
+    } else if (lane == 0) {
+        const bool weights = w == 10;
+        if (!weights && a.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");  // x is the terms kernel's
+        const uint8_t* src = a.w + ((g * a.NC + tile) * a.NP + p0) * a.block;
+        int p = 0;
+        for (; p < np; ++p) {
+            uint64_t* full = &in_full[p % C::NS];
+            if (!mbar_wait_bounded(&in_empty[p % C::NS], (p / C::NS & 1) ^ 1, abort_flag, a.err, ERR_GEMM_TIMEOUT))
+                break;
+            uint8_t* st = ring + p % C::NS * C::STAGE;
+            if (weights) {
+                mbar_arrive_expect_tx(full, a.block);
+                bulk_load(st + 2 * C::XB, src + static_cast<int64_t>(p) * a.block, a.block, full);
+            } else {
+                mbar_arrive_expect_tx(full, 2 * C::XB);
+                tma_load_3d(st, &xmap, full, 0, static_cast<int>(m0 * a.terms), 2 * (p0 + p));
+            }
+        }
+        if (*abort_flag)  // a failed call leaves no copy in flight behind (bounded as well)
+            for (int i = max(0, p - C::NS); i < p; ++i)
+                for (int t = 0; t < 1 << 14 && !mbar_try_wait(&in_full[i % C::NS], i / C::NS & 1); ++t) {
+                }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
+
+    // every MMA has been waited for by the channel warps (or the call failed):
+    // give the tensor memory back before any wait on another CTA
+    tc_fence_before();
     __syncthreads();
+    tc_fence_after();
+    if (w == 9) tmem_dealloc(tmem, C::TMEM);
+    for (int j = 0; j < 2; ++j) {  // the warpgroups' sums
+        if (w < 8 && wg == j)
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                fin[(nt * 8 + 2 * (lane & 3) + (i & 1)) * LD + w * 32 + c * 16 + (lane >> 2) + 8 * (i >> 1)] =
-                    acc[c][nt][i];
-    __syncthreads();
-    if (a.S > 1) cluster_barrier();
-    for (int i = ks * 128 + threadIdx.x; i < rows * W * 32; i += a.S * 128) {
-        const int r = i / (W * 32), ch = i % (W * 32);
-        const int64_t n = tile * W * 32 + ch;
+            for (int c = 0; c < COLS; ++c)
+                if (c < cols) fin[c * C::LD + ch] = j ? fin[c * C::LD + ch] + acc[c] : acc[c];
+        __syncthreads();
+    }
+    if (a.S > 1) cluster_sync();
+    for (int i = ks * kQ4Threads + threadIdx.x; i < rows * 128; i += a.S * kQ4Threads) {
+        const int r = i >> 7, c = i & 127;
         float v = 0.0f;
         for (int s = 0; s < a.S; ++s)
             for (int j = 0; j < a.terms; ++j) {
-                const float* p = fin + (r * a.terms + j) * LD + ch;
+                const float* p = fin + (r * a.terms + j) * C::LD + c;
                 v += s == ks ? *p : ld_cluster(p, s);
             }
-        if (n < a.N) store_out(a, m0 + r, n, v);
+        if (tile * 128 + c < a.N) store_out(a, m0 + r, tile * 128 + c, v);
     }
-    if (a.S > 1) cluster_barrier();
+    if (a.S > 1) cluster_sync();  // the sums stay until every rank has read them
 }
 
-template <int NT, int GS, typename ST>
-aem_status launch_q4(const Q4Args& a, dim3 grid, cudaStream_t s) {
+template <int COLS, int GS>
+aem_status launch_q4(const CUtensorMap& xmap, const Q4Args& a, dim3 grid, cudaStream_t s) {
+    using C = Q4Cfg<COLS, GS>;
+    auto kern = q4_kernel<COLS, GS>;
+    static std::atomic<uint64_t> ready{0};  // bit per device: the shared memory opt-in is done
+    const uint64_t bit = 1ull << (current_device() & 63);
+    if (!(ready.load(std::memory_order_relaxed) & bit)) {
+        AEM_TRY_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        ready.fetch_or(bit, std::memory_order_relaxed);
+    }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(128);
+    cfg.blockDim = dim3(kQ4Threads);
+    cfg.dynamicSmemBytes = C::SMEM;
     cfg.stream = s;
     cudaLaunchAttribute at[2] = {};
     int n = 0;
@@ -627,45 +564,60 @@ aem_status launch_q4(const Q4Args& a, dim3 grid, cudaStream_t s) {
     }
     cfg.attrs = at;
     cfg.numAttrs = n;
-    if constexpr (NT <= 2)
-        AEM_TRY_CUDA(cudaLaunchKernelEx(&cfg, q4_narrow_kernel<NT, GS, ST>, a));
-    else
-        AEM_TRY_CUDA(cudaLaunchKernelEx(&cfg, q4_wide_kernel<NT, GS, ST>, a));
+    AEM_TRY_CUDA(cudaLaunchKernelEx(&cfg, kern, xmap, a));
     count_launches(1);
     return AEM_OK;
 }
 
-template <int NT>
-aem_status launch_nt(const Q4Args& a, int gs, bool sb, dim3 grid, cudaStream_t s) {
-    if (sb)
-        return gs == 32   ? launch_q4<NT, 32, __nv_bfloat16>(a, grid, s)
-               : gs == 64 ? launch_q4<NT, 64, __nv_bfloat16>(a, grid, s)
-                          : launch_q4<NT, 128, __nv_bfloat16>(a, grid, s);
-    return gs == 32   ? launch_q4<NT, 32, float>(a, grid, s)
-           : gs == 64 ? launch_q4<NT, 64, float>(a, grid, s)
-                      : launch_q4<NT, 128, float>(a, grid, s);
+template <int COLS>
+aem_status launch_cols(const void* x, int64_t ldx, int64_t K, Q4Args a, int gs, int64_t slots,
+                       cudaStream_t s) {
+    CUtensorMap xmap;  // [K / 64][rows][64]: one box holds a pair of 64-k tiles
+    AEM_TRY(make_tmap_3d(&xmap, x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 64, a.M * a.terms, K / 64, ldx * 2, 128,
+                         64, COLS, 2, CU_TENSOR_MAP_SWIZZLE_128B));
+    // K is split until the CTAs fill the SMs: waves x (a CTA's own latency, as
+    // long as about 8 pairs, and its pairs)
+    const int64_t ctas = a.NC * slots, fit = 148 * (COLS <= 32 ? 2 : 1), pairs = a.NP;
+    int64_t best = INT64_MAX;
+    for (int S = 1; S <= 8 && S <= std::max<int64_t>(1, pairs / 2); ++S) {
+        const int64_t cost = (ctas * S + fit - 1) / fit * (8 + (pairs + S - 1) / S);
+        if (cost < best) {
+            best = cost;
+            a.S = S;
+        }
+    }
+    const dim3 grid(static_cast<unsigned>(a.NC * a.S), static_cast<unsigned>(slots));
+    return gs == 32   ? launch_q4<COLS, 32>(xmap, a, grid, s)
+           : gs == 64 ? launch_q4<COLS, 64>(xmap, a, grid, s)
+                      : launch_q4<COLS, 128>(xmap, a, grid, s);
 }
 
-// x: the caller's rows; a.x and a.terms are set here.
+// x: the caller's rows.
 aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, const void* x, aem_dtype xd,
-                      void* workspace, size_t workspace_bytes, cudaStream_t s) {
+                      int64_t ldx, void* workspace, size_t workspace_bytes, cudaStream_t s) {
     AEM_REQUIRE(current_device() == w->device, "%s: the weights are on device %d, the current one is %d",
                 what, w->device, current_device());
-    a.q = w->q;
-    a.scale = w->scale;
-    a.K = w->K;
+    a.w = w->data;
+    a.block = w->block;
+    a.scale_bf16 = w->scale_bf16;
     a.N = w->N;
-    a.NT = w->NT;
-    a.KT = w->KT;
-    a.KB = w->KB;
+    a.NC = w->NC;
+    a.NP = w->NP;
+    a.err = device_error_word(w->device);
     a.terms = xd == AEM_F32 ? 3 : 1;
-    const bool as_is = xd == AEM_BF16 && a.K % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 &&
-                       a.ldx % 8 == 0;
+    AEM_REQUIRE(a.M * a.terms < (1ll << 31), "%s: M=%lld out of range", what, (long long)a.M);
+    // columns of a row tile: as many as the rows (grouped: an average group's) need, up to 64
+    const int64_t groups = std::min<int64_t>(a.G, a.M);
+    const int64_t want = (a.group_rows ? (a.M + groups - 1) / groups : a.M) * a.terms;
+    const int cols = want <= 16 ? 16 : want <= 32 ? 32 : 64;
+    a.rows = cols / a.terms;
+    const int64_t slots = a.group_rows ? groups + a.M / a.rows : (a.M + a.rows - 1) / a.rows;
+    AEM_REQUIRE(slots <= 65535, "%s: M=%lld rows are too many for one call", what, (long long)a.M);
+    const int64_t K = w->K;
+    int64_t KP = K;
     void* own = nullptr;
-    if (as_is) {
-        a.x = static_cast<const __nv_bfloat16*>(x);
-    } else {
-        const int64_t KP = (a.K + 7) / 8 * 8;
+    if (xd != AEM_BF16 || K % 64 != 0 || (reinterpret_cast<uintptr_t>(x) & 15) != 0 || ldx % 8 != 0 || ldx < K) {
+        KP = (K + 63) / 64 * 64;
         const size_t need = static_cast<size_t>(a.M) * a.terms * KP * 2;
         AEM_REQUIRE(!workspace || (workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
                     "%s: workspace of %zu bytes (%zu needed, 16-byte aligned)", what, workspace_bytes, need);
@@ -676,39 +628,24 @@ aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, const void*
         auto* t = static_cast<__nv_bfloat16*>(workspace);
         const unsigned g = static_cast<unsigned>(std::min<int64_t>((a.M * KP + kThreads - 1) / kThreads, 148 * 8));
         if (xd == AEM_F32)
-            q4_terms_kernel<float><<<g, kThreads, 0, s>>>(static_cast<const float*>(x), a.ldx, a.M, a.K, KP, t);
+            q4_terms_kernel<float><<<g, kThreads, 0, s>>>(static_cast<const float*>(x), ldx, a.M, K, KP, t);
         else
-            q4_terms_kernel<__nv_bfloat16><<<g, kThreads, 0, s>>>(static_cast<const __nv_bfloat16*>(x), a.ldx,
-                                                                  a.M, a.K, KP, t);
-        AEM_CHECK_LAUNCH();
+            q4_terms_kernel<__nv_bfloat16><<<g, kThreads, 0, s>>>(static_cast<const __nv_bfloat16*>(x), ldx,
+                                                                  a.M, K, KP, t);
         count_launches(1);
-        a.x = t;
-        a.ldx = KP;
         a.dependent = true;
+        x = t;
+        ldx = KP;
     }
-    // columns of a row tile: as many as the rows (grouped: an average group's) need, up to 64
-    const int64_t groups = std::min<int64_t>(a.G, a.M);
-    const int64_t want = (a.group_rows ? (a.M + groups - 1) / groups : a.M) * a.terms;
-    const int nt = want <= 8 ? 1 : want <= 16 ? 2 : want <= 32 ? 4 : 8;
-    a.rows = 8 * nt / a.terms;
-    const int64_t slots = a.group_rows ? groups + a.M / a.rows : (a.M + a.rows - 1) / a.rows;
-    const int64_t per = nt <= 2 ? 1 : 4, tiles = (a.NT / 2 + per - 1) / per, ctas = tiles * slots;
-    const int64_t kparts = nt <= 2 ? 4 : 1;  // K shares inside a CTA
-    a.S = 1;
-    while (a.S < 8 && ctas * a.S < 148 * 2 && a.KT >= 4 * kparts * a.S) a.S *= 2;
-    aem_status st = AEM_OK;
-    const dim3 grid(static_cast<unsigned>(tiles * a.S), static_cast<unsigned>(slots));
-    if (slots > 65535) {
-        set_error("%s: M=%lld rows are too many for one call", what, (long long)a.M);
-        st = AEM_EINVAL;
-    } else if (nt == 1) {
-        st = launch_nt<1>(a, w->gs, w->scale_bf16, grid, s);
-    } else if (nt == 2) {
-        st = launch_nt<2>(a, w->gs, w->scale_bf16, grid, s);
-    } else if (nt == 4) {
-        st = launch_nt<4>(a, w->gs, w->scale_bf16, grid, s);
+    const cudaError_t e = cudaGetLastError();
+    aem_status st;
+    if (e != cudaSuccess) {
+        set_error("%s: launch failed: %s", what, cudaGetErrorString(e));
+        st = AEM_ECUDA;
     } else {
-        st = launch_nt<8>(a, w->gs, w->scale_bf16, grid, s);
+        st = cols == 16   ? launch_cols<16>(x, ldx, KP, a, w->gs, slots, s)
+             : cols == 32 ? launch_cols<32>(x, ldx, KP, a, w->gs, slots, s)
+                          : launch_cols<64>(x, ldx, KP, a, w->gs, slots, s);
     }
     if (own) cudaFreeAsync(own, s);
     return st;
@@ -735,8 +672,7 @@ void launch_quantize(const void* w, int64_t G, int64_t K, int64_t N, int gs, int
 }
 
 void free_q4(Q4Weight* w) {
-    cudaFree(w->q);
-    cudaFree(w->scale);
+    cudaFree(w->data);
     delete w;
 }
 
@@ -798,29 +734,29 @@ aem_status aem_q4weight_pack_device(const int8_t* q, const void* scale, aem_dtyp
     w->G = G;
     w->K = K;
     w->N = N;
-    w->NT = (N + 31) / 32 * 2;
-    w->KT = (K + 63) / 64;
-    w->KB = (K + group_size - 1) / group_size;
+    w->NC = (N + 127) / 128;
+    w->NP = (K + 127) / 128;
     w->gs = group_size;
     w->scale_bf16 = scale_dtype == AEM_BF16;
-    const int64_t tiles = G * w->NT * w->KT, scales = G * w->KB * w->NT * 16;
-    if (cudaMalloc(&w->q, static_cast<size_t>(tiles) * 512) != cudaSuccess ||
-        cudaMalloc(&w->scale, static_cast<size_t>(scales) * (w->scale_bf16 ? 2 : 4)) != cudaSuccess) {
+    const int per = 128 / group_size;
+    w->block = 8192 + per * 128 * (w->scale_bf16 ? 2 : 4);
+    const int64_t blocks = G * w->NC * w->NP, KB = (K + group_size - 1) / group_size;
+    if (cudaMalloc(&w->data, static_cast<size_t>(blocks) * w->block) != cudaSuccess) {
         cudaGetLastError();
         aem::free_q4(w);
         set_error("aem_q4weight_pack: device allocation failed");
         return AEM_ENOMEM;
     }
-    aem::pack_q4_kernel<<<static_cast<unsigned>(std::min<int64_t>((tiles + 7) / 8, 148 * 64)),
-                          aem::kThreads, 0, s>>>(q, K, N, w->NT, w->KT, tiles, w->q, err);
-    const unsigned gr = static_cast<unsigned>(std::min<int64_t>((scales + 255) / 256, 148 * 64));
+    const unsigned g1 = static_cast<unsigned>(std::min<int64_t>(blocks * 2, 148 * 64));
+    aem::pack_q4_kernel<<<g1, aem::kThreads, 0, s>>>(q, K, N, w->NC, w->NP, blocks * 512, w->block, w->data, err);
+    const int64_t scales = blocks * per * 128;
+    const unsigned g2 = static_cast<unsigned>(std::min<int64_t>((scales + 255) / 256, 148 * 64));
     if (w->scale_bf16)
-        aem::pack_q4_scale_kernel<__nv_bfloat16><<<gr, aem::kThreads, 0, s>>>(
-            static_cast<const __nv_bfloat16*>(scale), G * w->KB, N, w->NT,
-            static_cast<__nv_bfloat16*>(w->scale));
+        aem::pack_q4_scale_kernel<__nv_bfloat16><<<g2, aem::kThreads, 0, s>>>(
+            static_cast<const __nv_bfloat16*>(scale), KB, N, w->NC, w->NP, scales, per, w->block, w->data);
     else
-        aem::pack_q4_scale_kernel<float><<<gr, aem::kThreads, 0, s>>>(
-            static_cast<const float*>(scale), G * w->KB, N, w->NT, static_cast<float*>(w->scale));
+        aem::pack_q4_scale_kernel<float><<<g2, aem::kThreads, 0, s>>>(
+            static_cast<const float*>(scale), KB, N, w->NC, w->NP, scales, per, w->block, w->data);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) {
         aem::free_q4(w);
@@ -899,7 +835,7 @@ aem_status aem_q4weight_shape(aem_q4weight_t wh, int64_t* G, int64_t* K, int64_t
 
 size_t aem_q4gemm_workspace(aem_q4weight_t wh, aem_dtype x_dtype, int64_t M) {
     if (!wh || M < 1 || !aem::is_dtype(x_dtype)) return 0;
-    const int64_t KP = (reinterpret_cast<aem::Q4Weight*>(wh)->K + 7) / 8 * 8;
+    const int64_t KP = (reinterpret_cast<aem::Q4Weight*>(wh)->K + 63) / 64 * 64;
     return static_cast<size_t>(M) * (x_dtype == AEM_F32 ? 3 : 1) * KP * 2;
 }
 
@@ -916,14 +852,13 @@ aem_status aem_q4gemm(aem_q4weight_t wh, int64_t group, const void* x, aem_dtype
     if (M == 0) return AEM_OK;
     AEM_REQUIRE(x && out, "aem_q4gemm: NULL buffer");
     aem::Q4Args a{};
-    a.ldx = ldx;
     a.out = out;
     a.ldo = ldo;
     a.M = M;
     a.group = group;
     a.G = 1;
     a.out_bf16 = out_dtype == AEM_BF16;
-    return aem::q4_product(w, "aem_q4gemm", a, x, x_dtype, workspace, workspace_bytes,
+    return aem::q4_product(w, "aem_q4gemm", a, x, x_dtype, ldx, workspace, workspace_bytes,
                            static_cast<cudaStream_t>(stream));
 }
 
@@ -941,7 +876,6 @@ aem_status aem_grouped_q4gemm(aem_q4weight_t wh, const int32_t* group_rows, cons
     if (M == 0) return AEM_OK;
     AEM_REQUIRE(group_rows && x && out, "aem_grouped_q4gemm: NULL buffer");
     aem::Q4Args a{};
-    a.ldx = ldx;
     a.out = out;
     a.ldo = ldo;
     a.M = M;
@@ -949,7 +883,7 @@ aem_status aem_grouped_q4gemm(aem_q4weight_t wh, const int32_t* group_rows, cons
     a.G = static_cast<int>(w->G);
     a.out_bf16 = out_dtype == AEM_BF16;
     a.relu = relu != 0;
-    return aem::q4_product(w, "aem_grouped_q4gemm", a, x, x_dtype, workspace, workspace_bytes,
+    return aem::q4_product(w, "aem_grouped_q4gemm", a, x, x_dtype, ldx, workspace, workspace_bytes,
                            static_cast<cudaStream_t>(stream));
 }
 
