@@ -231,36 +231,44 @@ __global__ void __launch_bounds__(kThreads)
 
 // Row tile `slot` of the groups' row tiles: its group, first row and rows.
 // Every warp searches alike.  Offsets are clamped to [0, M].
-__device__ __forceinline__ bool find_rows(const Q4Args& a, int64_t slot, int64_t* g, int64_t* m0,
-                                          int* rows) {
+__device__ __forceinline__ bool find_rows(const Q4Args& a, int slot, int64_t* g, int64_t* m0, int* rows) {
     if (!a.group_rows) {
         *g = a.group;
-        *m0 = slot * a.rows;
+        *m0 = static_cast<int64_t>(slot) * a.rows;
         *rows = static_cast<int>(min(static_cast<int64_t>(a.rows), a.M - *m0));
         return *rows > 0;
     }
-    const int lane = threadIdx.x & 31;
-    int64_t before = 0;
-    for (int e0 = 0; e0 < a.G; e0 += 32) {
-        const int e = e0 + lane;
-        const int64_t lo = e < a.G ? min(max(static_cast<int64_t>(a.group_rows[e]), 0l), a.M) : 0;
-        const int64_t hi = e < a.G ? min(max(static_cast<int64_t>(a.group_rows[e + 1]), 0l), a.M) : 0;
-        const int n = hi > lo ? static_cast<int>((hi - lo + a.rows - 1) / a.rows) : 0;
+    const int lane = threadIdx.x & 31, M = static_cast<int>(a.M);
+    int lo[8], hi[8];  // all offsets on their way at once
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        lo[i] = hi[i] = 0;
+        if (i * 32 + lane < a.G) {
+            lo[i] = a.group_rows[i * 32 + lane];
+            hi[i] = a.group_rows[i * 32 + lane + 1];
+        }
+    }
+    int before = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (i * 32 >= a.G) break;
+        lo[i] = min(max(lo[i], 0), M);
+        hi[i] = min(max(hi[i], 0), M);
+        const int n = hi[i] > lo[i] ? (hi[i] - lo[i] + a.rows - 1) / a.rows : 0;
         int s = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(~0u, s, o);
             if (lane >= o) s += v;
         }
-        const int64_t first = before + s - n;
+        const int first = before + s - n;
         const unsigned hit = __ballot_sync(~0u, slot >= first && slot < first + n);
         if (hit) {
             const int l = __ffs(hit) - 1;
-            const int64_t m = lo + (slot - first) * a.rows;
-            const int r = static_cast<int>(min(static_cast<int64_t>(a.rows), hi - m));
-            *g = e0 + l;
+            const int m = lo[i] + (slot - first) * a.rows;
+            *g = i * 32 + l;
             *m0 = __shfl_sync(~0u, m, l);
-            *rows = __shfl_sync(~0u, r, l);
+            *rows = __shfl_sync(~0u, min(a.rows, hi[i] - m), l);
             return true;
         }
         before += __shfl_sync(~0u, s, 31);
@@ -283,55 +291,53 @@ __device__ __forceinline__ void store_out(const Q4Args& a, int64_t m, int64_t n,
 }
 
 // Shape of the product kernel for COLS MMA columns and scale groups of GS k.
-// Work moves in pairs of 64-k tiles.  A batch is what one accumulator buffer
-// takes before the scales are applied: a pair, with one accumulator per scale
-// group side by side, or a single tile where that would need too many columns.
+// A block of the packed weight (128 channels x 128 k) is a pair of 64-k tiles;
+// a unit is what a warpgroup hands to the tensor core at once: a pair, with
+// one accumulator per scale group side by side, or one tile where a pair's
+// accumulators would not fit.
 template <int COLS, int GS>
 struct Q4Cfg {
-    static constexpr int RES = COLS <= 32 ? 2 : 1;     // CTAs per SM
-    static constexpr int TMEM = 512 / RES;
-    static constexpr int TW = TMEM / 2;                // columns of one warpgroup
-    static constexpr int BK = GS == 32 && COLS > 16 ? 1 : 2;  // tiles per batch
-    static constexpr int SUB = GS == 128 ? 1 : BK * 64 / GS;  // accumulators per batch
-    static constexpr int NA = RES == 2 ? 2 : 4;        // weight tiles in TMEM
-    static constexpr int ND_RAW = (TW - 32 * NA) / (SUB * COLS);
-    static constexpr int ND = ND_RAW > 2 ? 2 : ND_RAW;  // accumulator buffers
-    static constexpr int XB = COLS * 128;              // bytes of an activation tile
+    static constexpr int TW = 128;                     // TMEM columns of a warpgroup: 4 per SM
+    static constexpr int UT = GS == 32 && COLS == 32 ? 1 : 2;  // tiles per unit
+    static constexpr int SUB = UT * 64 < GS ? 1 : UT * 64 / GS;  // accumulators per unit
     static constexpr int NSC = 128 / GS;               // scale groups of a pair
+    static constexpr int ND = 32 * UT + 2 * SUB * COLS <= TW ? 2 : 1;  // accumulator buffers
+    static constexpr int XB = COLS * 128;              // bytes of an activation tile
     // a pair's activations, then its block of weights and scales
     static constexpr int STAGE = 2 * XB + 8192 + (NSC * 512 + 1023) / 1024 * 1024;
     // an even ring: a stage always comes back to the warpgroup that saw its
     // previous phase, so no parity wait can mistake a phase for the one two back
-    static constexpr int FIT = ((228 / RES - 1) * 1024 - 2048) / STAGE / 2 * 2;
+    static constexpr int FIT = (113 * 1024 - 2048) / STAGE / 2 * 2;
     static constexpr int NS = FIT > 8 ? 8 : FIT;
     static constexpr int LD = 128 + 4;
-    static constexpr int BARS = 2 * NS + 2 * (2 * NA + 2 * ND);
-    static constexpr int USED = 1024 + NS * STAGE + BARS * 8 + 16;
-    // no more CTAs on an SM than TMEM holds: none ever waits for its columns
-    static constexpr int FLOOR = 228 * 1024 / (RES + 1) + 1024;
-    static constexpr int SMEM = USED > FLOOR ? USED : FLOOR;
-    static_assert(ND >= 1 && NS >= 4 && NS * STAGE >= COLS * LD * 4 && SMEM <= (228 / RES - 1) * 1024, "budgets");
+    static constexpr int USED = 1024 + NS * STAGE + (2 * NS + 4) * 8 + 16;
+    // two CTAs on an SM, never three: no CTA ever waits for tensor memory
+    static constexpr int SMEM = USED > 78 * 1024 ? USED : 78 * 1024;
+    static_assert(32 * UT + ND * SUB * COLS <= TW && NS >= 4 && SMEM <= 113 * 1024, "budgets");
+    static_assert(NS * STAGE >= COLS * LD * 4, "the sums fit the ring");
 };
 constexpr int kQ4Threads = 12 * 32;
 
 // A CTA computes 128 channels of one row tile over its part of K:
 //   warps 0-7   two warpgroups, thread = channel = TMEM lane, that take the
-//               pairs of 64-k tiles in turn: the channel's 4-bit weights come
-//               from the shared-memory ring, 32 columns of bf16 pairs a tile
-//               go to tensor memory, and one batch later the finished
-//               accumulator comes back and scale * sum is added to float32
-//               registers.
+//               pairs of 64-k tiles in turn.  Per unit: the channel's 4-bit
+//               weights come from the shared-memory ring and go to tensor
+//               memory as bf16 pairs (32 columns a tile) once the MMAs of the
+//               unit before are done; then that unit's accumulators come back
+//               and scale * sum is added to float32 registers.
 //   warps 8-9   one per warpgroup, issue its MMAs (M = 128 channels, N =
-//               columns, K = 16).
-//   warp 10     copies the weights, one 8 KB bulk copy per pair.
+//               columns, K = 16); one commit per unit.
+//   warp 10     copies the weights, one bulk copy per pair.
 //   warp 11     copies the activations, one TMA box per pair (128-byte swizzle).
+// Four warpgroups share an SM (two CTAs).  Converting is what they compete
+// for: 7 logic operations (half rate) and 4 subtractions per 8 weights, 224
+// cycles of a scheduler per pair.  Two accumulator buffers let the sums be
+// taken back under the next unit's MMAs; where only one fits they are taken
+// before the unit is handed over.
 // The S CTAs of a cluster take parts of K; their sums are added in rank order.
 // Every wait is bounded; a timeout sets the error word and ends all roles.
-// (Weights held in registers ahead of their use stay one tile ahead at most,
-// whatever the depth written: a warp has too few load scoreboards.  The ring
-// replaced that form, 28 us for one row.)
 template <int COLS, int GS>
-__global__ void __launch_bounds__(kQ4Threads, Q4Cfg<COLS, GS>::RES)
+__global__ void __launch_bounds__(kQ4Threads, 2)
     q4_kernel(const __grid_constant__ CUtensorMap xmap, const Q4Args a) {
     using C = Q4Cfg<COLS, GS>;
     extern __shared__ uint8_t smem_raw[];
@@ -340,9 +346,9 @@ __global__ void __launch_bounds__(kQ4Threads, Q4Cfg<COLS, GS>::RES)
     float* fin = reinterpret_cast<float*>(ring);  // [COLS][LD], after the loop
     uint64_t* in_full = reinterpret_cast<uint64_t*>(ring + C::NS * C::STAGE);
     uint64_t* in_empty = in_full + C::NS;
-    uint64_t* wg_bars = in_empty + C::NS;  // per warpgroup: a_full, a_empty, d_full, d_empty
-    constexpr int WB = 2 * C::NA + 2 * C::ND;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(wg_bars + 2 * WB);
+    uint64_t* a_full = in_empty + C::NS;  // [2]: a unit's weights are in tensor memory
+    uint64_t* done = a_full + 2;          // [2]: its MMAs have finished
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -354,35 +360,46 @@ __global__ void __launch_bounds__(kQ4Threads, Q4Cfg<COLS, GS>::RES)
     const int cols = rows * a.terms;
     const int p0 = static_cast<int>(a.NP * ks / a.S), np = static_cast<int>(a.NP * (ks + 1) / a.S) - p0;
 
-    if (threadIdx.x == 8 * 32) {
+    const uint8_t* src = a.w + ((g * a.NC + tile) * a.NP + p0) * a.block;
+    auto copy_weights = [&](int p) {
+        uint64_t* full = &in_full[p % C::NS];
+        mbar_arrive_expect_tx(full, a.block);
+        bulk_load(ring + p % C::NS * C::STAGE + 2 * C::XB, src + static_cast<int64_t>(p) * a.block, a.block, full);
+    };
+    auto copy_x = [&](int p) {
+        uint64_t* full = &in_full[p % C::NS];
+        mbar_arrive_expect_tx(full, 2 * C::XB);
+        tma_load_3d(ring + p % C::NS * C::STAGE, &xmap, full, 0, static_cast<int>(m0 * a.terms), 2 * (p0 + p));
+    };
+    if (w == 9) {
+        tmem_alloc(tmem_slot, 2 * C::TW);
+        tmem_relinquish();
+    } else if (w == 10 && lane == 0) {
+        // the first weights are on their way before the rest of the set-up
         for (int i = 0; i < C::NS; ++i) {
             mbar_init(&in_full[i], 2);   // both copies
-            mbar_init(&in_empty[i], 5);  // four warps, the MMAs' commit
+            mbar_init(&in_empty[i], 4);  // the four warps of the pair's warpgroup
         }
-        for (int j = 0; j < 2; ++j)
-            for (int i = 0; i < WB; ++i)  // a_full and d_empty: four warps; the others: a commit
-                mbar_init(&wg_bars[j * WB + i], i < C::NA || i >= 2 * C::NA + C::ND ? 4 : 1);
+        for (int j = 0; j < 2; ++j) {
+            mbar_init(&a_full[j], 4);
+            mbar_init(&done[j], 1);
+        }
         *abort_flag = 0;
         fence_barrier_init();
+        for (int p = 0; p < min(np, C::NS); ++p) copy_weights(p);
+    } else if (w == 11 && lane == 0) {
+        tma_prefetch_desc(&xmap);
     }
-    if (w == 9) {
-        tmem_alloc(tmem_slot, C::TMEM);
-        tmem_relinquish();
-    }
-    if (w == 11 && lane == 0) tma_prefetch_desc(&xmap);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
     const int wg = w < 8 ? w >> 2 : w & 1;  // the warpgroup a channel or MMA warp belongs to
-    uint64_t* a_full = wg_bars + wg * WB;
-    uint64_t* a_empty = a_full + C::NA;
-    uint64_t* d_full = a_empty + C::NA;
-    uint64_t* d_empty = d_full + C::ND;
-    const uint32_t tw = tmem + static_cast<uint32_t>(wg * C::TW);  // accumulators, then weight tiles
-    const uint32_t ta = tw + C::ND * C::SUB * COLS;
+    const uint32_t td = tmem + static_cast<uint32_t>(wg * C::TW);  // accumulators, then the unit's weights
+    const uint32_t ta = td + C::ND * C::SUB * COLS;
     auto wait = [&](uint64_t* bar, int phase) {  // whole warps
+        if (__all_sync(~0u, mbar_try_wait(bar, phase & 1))) return true;
         return __all_sync(~0u, mbar_wait_bounded(bar, phase & 1, abort_flag, a.err, ERR_GEMM_TIMEOUT)) != 0;
     };
 
@@ -390,116 +407,104 @@ __global__ void __launch_bounds__(kQ4Threads, Q4Cfg<COLS, GS>::RES)
     const int ch = threadIdx.x & 127;
     if (w < 8) {
         const uint32_t quarter = static_cast<uint32_t>(32 * (w & 3)) << 16;
-        auto take = [&](int b, const float (&s)[C::SUB]) {  // batch b's sums, scaled
-            if (!wait(&d_full[b % C::ND], b / C::ND)) return false;
-            tc_fence_after();
+        auto take = [&](int u, const float (&s)[C::SUB]) {  // unit u's sums, scaled
 #pragma unroll
-            for (int j = 0; j < C::SUB; ++j) {
+            for (int j = 0; j < C::SUB; ++j)
 #pragma unroll
                 for (int c = 0; c < COLS; c += 16) {
                     if (c >= cols) continue;
                     uint32_t r[16];
-                    tc_ld_32x32b_x16(tw + quarter + (b % C::ND * C::SUB + j) * COLS + c, r);
+                    tc_ld_32x32b_x16(td + quarter + (u % C::ND * C::SUB + j) * COLS + c, r);
                     tc_wait_ld();
 #pragma unroll
                     for (int i = 0; i < 16; ++i) acc[c + i] = fmaf(s[j], __uint_as_float(r[i]), acc[c + i]);
                 }
-            }
             tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&d_empty[b % C::ND]);
-            return true;
         };
         float s_prev[C::SUB];
-        int n = 0, b = 0;  // tiles and batches of this warpgroup so far
+        int u = 0;  // units of this warpgroup so far
         bool ok = true;
         for (int p = wg; ok && p < np; p += 2) {
             const uint8_t* st = ring + p % C::NS * C::STAGE + 2 * C::XB;
-            ok = wait(&in_full[p % C::NS], p / C::NS);
-            if (!ok) break;
+            if (!(ok = wait(&in_full[p % C::NS], p / C::NS))) break;
             float s[C::NSC];
 #pragma unroll
             for (int j = 0; j < C::NSC; ++j)
                 s[j] = a.scale_bf16
                            ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(st + 8192)[j * 128 + ch])
                            : reinterpret_cast<const float*>(st + 8192)[j * 128 + ch];
+            auto weights = [&](int i) { return *reinterpret_cast<const uint4*>(st + i * 2048 + ch * 16); };
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const uint4 q0 = *reinterpret_cast<const uint4*>(st + j * 4096 + ch * 16);
-                const uint4 q1 = *reinterpret_cast<const uint4*>(st + j * 4096 + 2048 + ch * 16);
-                const int slot = n % C::NA;
-                ok = ok && wait(&a_empty[slot], n / C::NA + 1);
-                if (!ok) break;
-                tc_fence_after();
                 uint32_t v[16];
-                unpack_q4(q0.x, v), unpack_q4(q0.y, v + 4), unpack_q4(q0.z, v + 8), unpack_q4(q0.w, v + 12);
-                tc_st_32x32b_x16(ta + quarter + 32 * slot, v);
+                if (C::ND == 2) {  // registers allow converting under the wait
+                    const uint4 q0 = weights(2 * j);
+                    unpack_q4(q0.x, v), unpack_q4(q0.y, v + 4), unpack_q4(q0.z, v + 8), unpack_q4(q0.w, v + 12);
+                }
+                if (u && (C::UT == 1 || j == 0)) {
+                    // the unit before is done: its weights' columns, its
+                    // accumulators and (at a pair's start) its stage are free
+                    if (!(ok = wait(&done[wg], u - 1))) break;
+                    tc_fence_after();
+                    if (j == 0 && lane == 0) mbar_arrive(&in_empty[(p - 2) % C::NS]);
+                    if (C::ND == 1) take(u - 1, s_prev);
+                }
+                if (C::ND == 1) {
+                    const uint4 q0 = weights(2 * j);
+                    unpack_q4(q0.x, v), unpack_q4(q0.y, v + 4), unpack_q4(q0.z, v + 8), unpack_q4(q0.w, v + 12);
+                }
+                const uint32_t at = ta + quarter + (C::UT == 2 ? 32 * j : 0);
+                tc_st_32x32b_x16(at, v);
+                const uint4 q1 = weights(2 * j + 1);
                 unpack_q4(q1.x, v), unpack_q4(q1.y, v + 4), unpack_q4(q1.z, v + 8), unpack_q4(q1.w, v + 12);
-                tc_st_32x32b_x16(ta + quarter + 32 * slot + 16, v);
+                tc_st_32x32b_x16(at + 16, v);
+                if (C::UT == 2 && j == 0) continue;
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&a_full[slot]);
-                    if (j == 1) mbar_arrive(&in_empty[p % C::NS]);
-                }
-                ++n;
-                if (C::BK == 1 || j == 1) {  // batch b is converted; the one before is done or nearly
-                    if (b) ok = take(b - 1, s_prev);
-                    ++b;
+                if (lane == 0) mbar_arrive(&a_full[wg]);
+                if (C::ND == 2 && u) take(u - 1, s_prev);
 #pragma unroll
-                    for (int i = 0; i < C::SUB; ++i) s_prev[i] = s[C::BK == 2 ? i : j * C::SUB + i];
-                }
+                for (int i = 0; i < C::SUB; ++i) s_prev[i] = s[C::UT == 2 ? i : j * C::SUB + i];
+                ++u;
             }
         }
-        if (ok && b) take(b - 1, s_prev);
+        if (ok && u && wait(&done[wg], u - 1)) {
+            tc_fence_after();
+            take(u - 1, s_prev);
+        }
     } else if (w < 10) {
         const uint32_t idesc = idesc_bf16_f32(128, static_cast<uint32_t>((cols + 15) & ~15));
-        int n = 0, b = 0;
+        int u = 0;
         bool ok = true;
         for (int p = wg; ok && p < np; p += 2) {
-            ok = wait(&in_full[p % C::NS], p / C::NS);
+            if (!(ok = wait(&in_full[p % C::NS], p / C::NS))) break;
             const uint64_t bd = smem_desc_sw128(smem_u32(ring + p % C::NS * C::STAGE));
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                if (C::BK == 1 || j == 0) ok = ok && wait(&d_empty[b % C::ND], b / C::ND + 1);
-                const int slot = n % C::NA;
-                ok = ok && wait(&a_full[slot], n / C::NA);
-                if (!ok) break;
+            for (int j = 0; j < 2 / C::UT; ++j) {
+                if (!(ok = wait(&a_full[wg], u))) break;
                 tc_fence_after();
-                const uint32_t d = tw + static_cast<uint32_t>(b % C::ND * C::SUB * COLS);
+                const uint32_t d = td + static_cast<uint32_t>(u % C::ND * C::SUB * COLS);
 #pragma unroll
-                for (int m = 0; m < 4; ++m) {
-                    const int grp = (C::BK == 2 ? 64 * j : 0) + 16 * m;  // k inside the batch
-                    tc_mma_f16_ts_elect(d + grp / GS * COLS, ta + 32 * slot + 8 * m,
-                                        bd + j * (C::XB >> 4) + 2 * m, idesc, grp % GS ? 1u : 0u);
-                }
-                tc_commit_elect(&a_empty[slot]);
-                ++n;
-                if (j == 1) tc_commit_elect(&in_empty[p % C::NS]);
-                if (C::BK == 1 || j == 1) {
-                    tc_commit_elect(&d_full[b % C::ND]);
-                    ++b;
-                }
+                for (int m = 0; m < 4 * C::UT; ++m)
+                    tc_mma_f16_ts_elect(d + 16 * m / GS * COLS, ta + 8 * m,
+                                        bd + (j + m / 4) * (C::XB >> 4) + 2 * (m % 4), idesc,
+                                        16 * m % GS ? 1u : 0u);
+                tc_commit_elect(&done[wg]);
+                ++u;
             }
         }
     } else if (lane == 0) {
         const bool weights = w == 10;
         if (!weights && a.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");  // x is the terms kernel's
-        const uint8_t* src = a.w + ((g * a.NC + tile) * a.NP + p0) * a.block;
-        int p = 0;
+        int p = weights ? min(np, C::NS) : 0;
         for (; p < np; ++p) {
-            uint64_t* full = &in_full[p % C::NS];
             if (!mbar_wait_bounded(&in_empty[p % C::NS], (p / C::NS & 1) ^ 1, abort_flag, a.err, ERR_GEMM_TIMEOUT))
                 break;
-            uint8_t* st = ring + p % C::NS * C::STAGE;
-            if (weights) {
-                mbar_arrive_expect_tx(full, a.block);
-                bulk_load(st + 2 * C::XB, src + static_cast<int64_t>(p) * a.block, a.block, full);
-            } else {
-                mbar_arrive_expect_tx(full, 2 * C::XB);
-                tma_load_3d(st, &xmap, full, 0, static_cast<int>(m0 * a.terms), 2 * (p0 + p));
-            }
+            if (weights)
+                copy_weights(p);
+            else
+                copy_x(p);
         }
         if (*abort_flag)  // a failed call leaves no copy in flight behind (bounded as well)
             for (int i = max(0, p - C::NS); i < p; ++i)
@@ -512,7 +517,7 @@ __global__ void __launch_bounds__(kQ4Threads, Q4Cfg<COLS, GS>::RES)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (w == 9) tmem_dealloc(tmem, C::TMEM);
+    if (w == 9) tmem_dealloc(tmem, 2 * C::TW);
     for (int j = 0; j < 2; ++j) {  // the warpgroups' sums
         if (w < 8 && wg == j)
 #pragma unroll
@@ -577,7 +582,7 @@ aem_status launch_cols(const void* x, int64_t ldx, int64_t K, Q4Args a, int gs, 
                          64, COLS, 2, CU_TENSOR_MAP_SWIZZLE_128B));
     // K is split until the CTAs fill the SMs: waves x (a CTA's own latency, as
     // long as about 8 pairs, and its pairs)
-    const int64_t ctas = a.NC * slots, fit = 148 * (COLS <= 32 ? 2 : 1), pairs = a.NP;
+    const int64_t ctas = a.NC * slots, fit = 148 * 2, pairs = a.NP;
     int64_t best = INT64_MAX;
     for (int S = 1; S <= 8 && S <= std::max<int64_t>(1, pairs / 2); ++S) {
         const int64_t cost = (ctas * S + fit - 1) / fit * (8 + (pairs + S - 1) / S);
@@ -606,10 +611,10 @@ aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, const void*
     a.err = device_error_word(w->device);
     a.terms = xd == AEM_F32 ? 3 : 1;
     AEM_REQUIRE(a.M * a.terms < (1ll << 31), "%s: M=%lld out of range", what, (long long)a.M);
-    // columns of a row tile: as many as the rows (grouped: an average group's) need, up to 64
+    // columns of a row tile: as many as the rows (grouped: an average group's) need, up to 32
     const int64_t groups = std::min<int64_t>(a.G, a.M);
     const int64_t want = (a.group_rows ? (a.M + groups - 1) / groups : a.M) * a.terms;
-    const int cols = want <= 16 ? 16 : want <= 32 ? 32 : 64;
+    const int cols = want <= 16 ? 16 : 32;
     a.rows = cols / a.terms;
     const int64_t slots = a.group_rows ? groups + a.M / a.rows : (a.M + a.rows - 1) / a.rows;
     AEM_REQUIRE(slots <= 65535, "%s: M=%lld rows are too many for one call", what, (long long)a.M);
@@ -643,9 +648,8 @@ aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, const void*
         set_error("%s: launch failed: %s", what, cudaGetErrorString(e));
         st = AEM_ECUDA;
     } else {
-        st = cols == 16   ? launch_cols<16>(x, ldx, KP, a, w->gs, slots, s)
-             : cols == 32 ? launch_cols<32>(x, ldx, KP, a, w->gs, slots, s)
-                          : launch_cols<64>(x, ldx, KP, a, w->gs, slots, s);
+        st = cols == 16 ? launch_cols<16>(x, ldx, KP, a, w->gs, slots, s)
+                        : launch_cols<32>(x, ldx, KP, a, w->gs, slots, s);
     }
     if (own) cudaFreeAsync(own, s);
     return st;
