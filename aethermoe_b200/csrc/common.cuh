@@ -58,7 +58,7 @@ enum : int {
     ERR_EP_PEER_TIMEOUT = 1 << 6, // a peer rank did not signal within the deadline
     ERR_EP_PEER_FAILED = 1 << 7,  // a peer rank signalled that its step failed
     ERR_ROW_INDEX = 1 << 8,       // a token order names a row past its units (skipped)
-    ERR_Q4_VALUE = 1 << 9,        // a 4-bit weight outside [-8, 7] (clamped)
+    ERR_Q4_VALUE = 1 << 9,        // a 4-bit weight outside [-7, 7] (clamped)
 };
 
 
@@ -78,11 +78,6 @@ bool is_sm100(int device);
 aem_status make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype,
                         int elem_bytes, uint64_t cols, uint64_t rows, uint32_t box_cols,
                         uint32_t box_rows, CUtensorMapSwizzle swizzle);
-// 3-D bf16-like map: dim0 elements innermost, dim1 stride1 bytes apart, dim2
-// stride2 bytes apart (strides multiples of 16).
-aem_status make_tmap_3d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, uint64_t dim0,
-                        uint64_t dim1, uint64_t dim2, uint64_t stride1, uint64_t stride2,
-                        uint32_t box0, uint32_t box1, uint32_t box2, CUtensorMapSwizzle swizzle);
 
 }  // namespace aem
 
@@ -182,15 +177,6 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const void* map, uint64_t
         : "memory");
 }
 
-__device__ __forceinline__ void tma_load_3d(void* dst, const void* map, uint64_t* bar, int x,
-                                            int y, int z) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
-        "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
-        : "memory");
-}
-
 // Non-tensor bulk copy global -> shared (16-byte aligned, size a multiple of 16).
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes,
                                           uint64_t* bar) {
@@ -243,17 +229,18 @@ __device__ __forceinline__ void tc_mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, 
         "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// The same, issued by one elected lane of a warp that runs the issue loop
-// together (elect.sync picks the lowest active lane every time), and the
+// The 8-bit form (kind::f8f6f4, four values per 32-bit column, one K = 32 step
+// spans 8 columns), issued by one elected lane of a warp that runs the issue
+// loop together (elect.sync picks the lowest active lane every time), and the
 // commit of the MMAs that lane issued.
-__device__ __forceinline__ void tc_mma_f16_ts_elect(uint32_t d_tmem, uint32_t a_tmem,
-                                                    uint64_t b_desc, uint32_t idesc,
-                                                    uint32_t accumulate) {
+__device__ __forceinline__ void tc_mma_f8_ts_elect(uint32_t d_tmem, uint32_t a_tmem,
+                                                   uint64_t b_desc, uint32_t idesc,
+                                                   uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p, e;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
         "elect.sync _|e, 0xffffffff;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
         "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
@@ -263,6 +250,15 @@ __device__ __forceinline__ void tc_commit_elect(uint64_t* bar) {
         "elect.sync _|e, 0xffffffff;\n\t"
         "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
             smem_u32(bar))
+        : "memory");
+}
+// 32 lanes x 8 columns.
+__device__ __forceinline__ void tc_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7])
+        : "r"(taddr)
         : "memory");
 }
 // Thread i of the warp writes lane (warp's lane base + i), columns [col, col+16).
@@ -446,6 +442,15 @@ __host__ __device__ constexpr uint32_t idesc_bf16_f32(uint32_t m, uint32_t n) {
     return (1u << 4)              // D format f32
            | (1u << 7)            // A format bf16
            | (1u << 10)           // B format bf16
+           | ((n >> 3) << 17)     // N >> 3
+           | ((m >> 4) << 24);    // M >> 4
+}
+
+// Instruction descriptor of kind::f8f6f4: e4m3 A, e5m2 B (K-major), f32 D.
+__host__ __device__ constexpr uint32_t idesc_e4m3_e5m2_f32(uint32_t m, uint32_t n) {
+    return (1u << 4)              // D format f32
+           | (0u << 7)            // A format e4m3
+           | (1u << 10)           // B format e5m2
            | ((n >> 3) << 17)     // N >> 3
            | ((m >> 4) << 24);    // M >> 4
 }

@@ -2,22 +2,31 @@
 // a few activation rows with them (decode), dense and grouped by expert.
 //
 // Weight (k, n) of group g of G is q[g][k][n] * scale[g][k / gs][n] with q an
-// integer in [-8, 7] and gs = 32, 64 or 128 consecutive k sharing a scale:
+// integer in [-7, 7] and gs = 32, 64 or 128 consecutive k sharing a scale:
 //   out[m, n] = sum_b scale[b, n] * sum_{k in block b} q[k, n] x[m, k]
-// A 4-bit integer is exact in bf16, so each inner sum runs on the tensor cores
-// (tcgen05, bf16 operands, float32 accumulators in TMEM) and the scale
-// multiplies its float32 result: no rounded weight ever exists.  bf16 x enters
-// as it is; float32 x enters as three bf16 terms that add up to it exactly
-// (8 + 8 + 8 mantissa bits), in three MMA columns whose sums are added at the
-// end.
 //
-// What bounds it is the weight stream, K*N/2 bytes plus the scales.  Warp MMAs
-// (mma.sync) cannot keep up with it on this chip: one m16n8k16 occupies its
-// sub-core's tensor pipe for 32 cycles, 12400 cycles for a 4096 x 14336
-// weight and 8 columns, and the time grows with the columns (measured 16.6 us
-// for 1 row, 47.6 us for 64).  So 128 channels are the M of a tcgen05.mma and
-// the weights, converted in registers, are its A operand in tensor memory.
+// The weights need no arithmetic to reach the tensor cores: an 8-bit float
+// (e4m3) whose exponent field is zero is m * 2^-9 for its mantissa m = 0..7,
+// so a sign and three magnitude bits ARE the e4m3 code of q * 2^-9.  Eight
+// packed weights become two operand registers by one mask, one rotation and
+// another mask.  The activations take part as e5m2 terms: with rho = the
+// power of two that brings the row's largest finite magnitude into
+// [2^14, 2^15), x * rho = t_0 + t_1 + ... where t_j is what is left after
+// t_0 .. t_{j-1}, truncated to e5m2's three significant bits (down to 2^-16).
+// Three terms hold a bf16 value and eight a float32 value exactly unless its
+// last bits lie below rho * |x| = 2^-16; what is cut off there is under 2^-30
+// of the row's largest magnitude, below the rounding of a float32 sum that
+// holds it.  Every product is exact, sums are float32 (tcgen05, accumulators
+// in TMEM), the terms' sums are added and the scales multiply the result in
+// float32: no rounded weight ever exists.
+//
+// What bounds it is the weight stream, K*N/2 bytes plus the scales.  Forms
+// that could not keep up with it (4096 x 14336, 1 row): warp MMAs (mma.sync
+// m16n8k16 occupies its sub-core's tensor pipe for 32 cycles: 16.6 us, 47.6
+// for 64 rows), and bf16 operands for tcgen05 (7 logic operations and 4
+// subtractions per 8 weights, the logic pipe the bound: 17.3 us).
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 
 #include <algorithm>
 #include <atomic>
@@ -31,11 +40,12 @@ namespace aem {
 // Packed 4-bit weight (device): [G][NC][NP] blocks of `block` bytes, NC =
 // ceil(N / 128) channel blocks and NP = ceil(K / 128).  A block holds 128
 // channels x 128 k and their scales, so one bulk copy brings both:
-//   [2][2][128][16 B]  weights: 64-k tile, half of it, channel.  The word j
-//                      (of 8) of a channel's tile holds k = 8j .. 8j + 7: the
-//                      pair (8j + 2r, 8j + 2r + 1) at bits 4r and 16 + 4r, as
-//                      q + 8; padding holds 8
-//   [128 / gs][128]    scales in the caller's type; padding is zero
+//   [4][128][16 B]   weights: 32-k quarter, channel.  A word holds 8
+//                    consecutive k.  Byte j < 4: magnitude of weight j in bits
+//                    0-2, its sign in bit 7; magnitude of weight 4 + j in bits
+//                    4-6, its sign in bit 3 of byte (j + 1) % 4
+//   [128 / gs][128]  scales in the caller's type
+// Padding is zero.
 struct Q4Weight {
     int device = 0;
     int64_t G = 0, K = 0, N = 0, NC = 0, NP = 0;
@@ -140,11 +150,13 @@ __global__ void __launch_bounds__(kThreads)
             for (int e = 0; e < 8; ++e) {
                 const int64_t k = k0 + 8 * j + e;
                 int v = k < K && n < N ? q[(g * K + k) * N + n] : 0;
-                if (v < -8 || v > 7) {
+                if (v < -7 || v > 7) {
                     bad = true;
-                    v = v < 0 ? -8 : 7;
+                    v = v < 0 ? -7 : 7;
                 }
-                word[j] |= static_cast<uint32_t>(v + 8) << (4 * (e >> 1) + 16 * (e & 1));
+                const uint32_t mag = static_cast<uint32_t>(v < 0 ? -v : v), neg = v < 0 ? 1u : 0u;
+                word[j] |= e < 4 ? mag << (8 * e) | neg << (8 * e + 7)
+                                 : mag << (8 * (e - 4) + 4) | neg << ((8 * (e - 4) + 11) & 31);
             }
         }
         *reinterpret_cast<uint4*>(out + blk * block + (p & 511) * 16) =
@@ -171,61 +183,92 @@ __global__ void __launch_bounds__(kThreads)
 // ------------------------------------------------------------------ product
 using namespace aem::dev;
 
-// Columns of the MMAs: the rows of x as they are (bf16), or three per row
-// (float32: the terms that add up to it).
 struct Q4Args {
     const uint8_t* w;
+    const float* unscale;       // [M]: 2^9 / rho of a row of x
     void* out;
     const int32_t* group_rows;  // nullptr: one group of M rows, weight group `group`
     int64_t ldo, M, N, NC, NP;
     int64_t group;
     int* err;
-    int G, block, S, rows, terms;  // S: CTAs (one cluster) that split K; rows: rows of a row tile
-    bool scale_bf16, out_bf16, relu, dependent;
+    int G, block, S, rows;  // S: CTAs (one cluster) that split K; rows: rows of a row tile
+    bool scale_bf16, out_bf16, relu;
 };
 
-// Eight 4-bit weights -> four bf16 pairs.  0x4300 is bf16 128, whose last
-// mantissa bit is 1: 0x4300 | nibble = 128 + nibble, and subtracting 136
-// leaves q exactly.
-__device__ __forceinline__ void unpack_q4(uint32_t w, uint32_t* a) {
-    const __nv_bfloat162 off = __halves2bfloat162(__ushort_as_bfloat16(0x4308), __ushort_as_bfloat16(0x4308));
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const uint32_t v = ((w >> (4 * r)) & 0x000f000fu) | 0x43004300u;
-        const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), off);
-        a[r] = *reinterpret_cast<const uint32_t*>(&d);
-    }
-}
+constexpr int kTermsBf16 = 3, kTermsF32 = 8;
 
-// Activations in the form the products read: [M * terms][KP] bf16, KP = K
-// rounded up to 64, zero padded.  float32 gives three truncated terms v =
-// t0 + t1 + t2 (8 mantissa bits each, every difference exact; an infinity or
-// NaN is all in t0), bf16 is copied (rows that are not 16-byte aligned).
-template <typename XT>
-__global__ void __launch_bounds__(kThreads)
-    q4_terms_kernel(const XT* __restrict__ x, int64_t ldx, int64_t M, int64_t K, int64_t KP,
-                    __nv_bfloat16* __restrict__ out) {
+// Activations as the products read them, one block per row: out [M * terms]
+// [KP] e5m2 bytes (KP = K rounded up to 128, zero padded), unscale [M].  An
+// infinity or NaN is all in the first term.  e5m2 is the upper byte of an
+// fp16, so truncating the fp16 truncates the term.
+template <typename XT, int TERMS>
+__global__ void __launch_bounds__(512)
+    q4_terms_kernel(const XT* __restrict__ x, int64_t ldx, int64_t K, int64_t KP, bool vec,
+                    uint8_t* __restrict__ out, float* __restrict__ unscale) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int64_t total = M * KP;
-    for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < total;
-         i += static_cast<int64_t>(gridDim.x) * kThreads) {
-        const int64_t m = i / KP, k = i - m * KP;
-        if constexpr (sizeof(XT) == 2) {
-            out[i] = k < K ? x[m * ldx + k] : __float2bfloat16_rn(0.0f);
+    __shared__ uint32_t top[16];
+    const XT* row = x + blockIdx.x * ldx;
+    auto load4 = [&](int64_t k, float (&v)[4]) {
+        if (vec && k + 4 <= K) {
+            if constexpr (sizeof(XT) == 4) {
+                const float4 f = *reinterpret_cast<const float4*>(row + k);
+                v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+            } else {
+                const uint2 u = *reinterpret_cast<const uint2*>(row + k);
+                v[0] = __uint_as_float(u.x << 16), v[1] = __uint_as_float(u.x & 0xffff0000u);
+                v[2] = __uint_as_float(u.y << 16), v[3] = __uint_as_float(u.y & 0xffff0000u);
+            }
         } else {
-            const float v = k < K ? x[m * ldx + k] : 0.0f;
-            const uint32_t u = __float_as_uint(v);
-            float r1 = v - __uint_as_float(u & 0xffff0000u);
-            if ((u & 0x7f800000u) == 0x7f800000u) r1 = 0.0f;
-            const float r2 = r1 - __uint_as_float(__float_as_uint(r1) & 0xffff0000u);
-            const float t[3] = {v, r1, r2};
 #pragma unroll
-            for (int j = 0; j < 3; ++j) {
-                uint16_t h = static_cast<uint16_t>(__float_as_uint(t[j]) >> 16);
-                if (j == 0 && v != v) h = 0x7fff;
-                out[(3 * m + j) * KP + k] = __ushort_as_bfloat16(h);
+            for (int i = 0; i < 4; ++i) v[i] = k + i < K ? static_cast<float>(row[k + i]) : 0.0f;
+        }
+    };
+    uint32_t mine = 0;  // magnitudes order as their bits do
+    for (int64_t k = threadIdx.x * 4; k < K; k += 512 * 4) {
+        float v[4];
+        load4(k, v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t u = __float_as_uint(v[i]) & 0x7fffffffu;
+            if (u < 0x7f800000u) mine = max(mine, u);
+        }
+    }
+    mine = __reduce_max_sync(~0u, mine);
+    if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = mine;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mine = max(mine, top[i]);
+    // rho = 2^up, up = 14 - exponent, in two factors (it may be beyond float32)
+    const int up = 141 - static_cast<int>(mine >> 23);
+    const float f1 = __uint_as_float(static_cast<uint32_t>(127 + up / 2) << 23);
+    const float f2 = __uint_as_float(static_cast<uint32_t>(127 + up - up / 2) << 23);
+    if (threadIdx.x == 0) unscale[blockIdx.x] = ldexpf(1.0f, 9 - up);
+    uint8_t* o = out + blockIdx.x * TERMS * KP;
+    for (int64_t k = threadIdx.x * 4; k < KP; k += 512 * 4) {
+        float v[4];
+        load4(k, v);
+        uint32_t t[TERMS];
+#pragma unroll
+        for (int j = 0; j < TERMS; ++j) t[j] = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool finite = (__float_as_uint(v[i]) & 0x7f800000u) != 0x7f800000u;
+            float r = v[i] * f1 * f2;
+#pragma unroll
+            for (int j = 0; j < TERMS; ++j) {
+                const uint32_t h = __half_as_ushort(__float2half_rz(r)) & 0xff00u;
+                t[j] |= (h >> 8) << (8 * i);
+                r -= __half2float(__ushort_as_half(static_cast<unsigned short>(h)));
+            }
+            if (!finite) {
+                const uint32_t code = v[i] != v[i] ? 0x7fu : v[i] > 0.0f ? 0x7cu : 0xfcu;
+#pragma unroll
+                for (int j = 0; j < TERMS; ++j)
+                    t[j] = (t[j] & ~(0xffu << (8 * i))) | (j == 0 ? code << (8 * i) : 0u);
             }
         }
+#pragma unroll
+        for (int j = 0; j < TERMS; ++j) *reinterpret_cast<uint32_t*>(o + j * KP + k) = t[j];
     }
 }
 
@@ -290,21 +333,22 @@ __device__ __forceinline__ void store_out(const Q4Args& a, int64_t m, int64_t n,
         static_cast<float*>(a.out)[m * a.ldo + n] = v;
 }
 
-// Shape of the product kernel for COLS MMA columns and scale groups of GS k.
-// A block of the packed weight (128 channels x 128 k) is a pair of 64-k tiles;
-// a unit is what a warpgroup hands to the tensor core at once: a pair, with
-// one accumulator per scale group side by side, or one tile where a pair's
-// accumulators would not fit.
-template <int COLS, int GS>
+// Shape of the product kernel for COLS MMA columns, scale groups of GS k and
+// TERMS columns a row.  A block of the packed weight is 128 channels x 128 k;
+// a unit is what a warpgroup hands to the tensor core at once: a block, with
+// one accumulator per scale group side by side, or half of one where a
+// block's accumulators would not fit.
+template <int COLS, int GS, int TERMS>
 struct Q4Cfg {
+    static constexpr int ROWS = COLS / TERMS;
     static constexpr int TW = 128;                     // TMEM columns of a warpgroup: 4 per SM
-    static constexpr int UT = GS == 32 && COLS == 32 ? 1 : 2;  // tiles per unit
-    static constexpr int SUB = UT * 64 < GS ? 1 : UT * 64 / GS;  // accumulators per unit
-    static constexpr int NSC = 128 / GS;               // scale groups of a pair
-    static constexpr int ND = 32 * UT + 2 * SUB * COLS <= TW ? 2 : 1;  // accumulator buffers
-    static constexpr int XB = COLS * 128;              // bytes of an activation tile
-    // a pair's activations, then its block of weights and scales
-    static constexpr int STAGE = 2 * XB + 8192 + (NSC * 512 + 1023) / 1024 * 1024;
+    static constexpr int FULL = GS == 128 ? 1 : 128 / GS;  // scale groups of a block
+    static constexpr int UK = FULL * COLS <= 96 ? 128 : 64;  // k of a unit
+    static constexpr int SUB = UK < GS ? 1 : UK / GS;  // accumulators per unit
+    static constexpr int UA = UK / 4;                  // columns of a unit's weights
+    static constexpr int ND = UA + 2 * SUB * COLS <= TW ? 2 : 1;  // accumulator buffers
+    static constexpr int XB = COLS * 128;              // activation bytes of a block
+    static constexpr int STAGE = XB + 8192 + (FULL * 512 + 1023) / 1024 * 1024;
     // an even ring: a stage always comes back to the warpgroup that saw its
     // previous phase, so no parity wait can mistake a phase for the one two back
     static constexpr int FIT = (113 * 1024 - 2048) / STAGE / 2 * 2;
@@ -313,37 +357,36 @@ struct Q4Cfg {
     static constexpr int USED = 1024 + NS * STAGE + (2 * NS + 4) * 8 + 16;
     // two CTAs on an SM, never three: no CTA ever waits for tensor memory
     static constexpr int SMEM = USED > 78 * 1024 ? USED : 78 * 1024;
-    static_assert(32 * UT + ND * SUB * COLS <= TW && NS >= 4 && SMEM <= 113 * 1024, "budgets");
-    static_assert(NS * STAGE >= COLS * LD * 4, "the sums fit the ring");
+    static_assert(UA + ND * SUB * COLS <= TW && NS >= 4 && SMEM <= 113 * 1024, "budgets");
+    static_assert(UK >= GS || UK == 128, "a scale group inside a unit");
+    static_assert(NS * STAGE >= ROWS * LD * 4, "the sums fit the ring");
 };
 constexpr int kQ4Threads = 12 * 32;
 
 // A CTA computes 128 channels of one row tile over its part of K:
 //   warps 0-7   two warpgroups, thread = channel = TMEM lane, that take the
-//               pairs of 64-k tiles in turn.  Per unit: the channel's 4-bit
+//               weight's blocks in turn.  Per unit: the channel's 4-bit
 //               weights come from the shared-memory ring and go to tensor
-//               memory as bf16 pairs (32 columns a tile) once the MMAs of the
-//               unit before are done; then that unit's accumulators come back
-//               and scale * sum is added to float32 registers.
+//               memory as e4m3 codes (8 columns per 32 k) once the MMAs of
+//               the unit before are done; then that unit's accumulators come
+//               back, a row's terms are added and scale * sum is added to the
+//               row's float32 register.
 //   warps 8-9   one per warpgroup, issue its MMAs (M = 128 channels, N =
-//               columns, K = 16); one commit per unit.
-//   warp 10     copies the weights, one bulk copy per pair.
-//   warp 11     copies the activations, one TMA box per pair (128-byte swizzle).
-// Four warpgroups share an SM (two CTAs).  Converting is what they compete
-// for: 7 logic operations (half rate) and 4 subtractions per 8 weights, 224
-// cycles of a scheduler per pair.  Two accumulator buffers let the sums be
-// taken back under the next unit's MMAs; where only one fits they are taken
-// before the unit is handed over.
+//               columns, K = 32); one commit per unit.
+//   warp 10     copies the weights with their scales, one bulk copy per block.
+//   warp 11     copies the activations, one TMA box per block (128-byte swizzle).
+// Two accumulator buffers let the sums be taken back under the next unit's
+// MMAs; where only one fits they are taken before the unit is handed over.
 // The S CTAs of a cluster take parts of K; their sums are added in rank order.
 // Every wait is bounded; a timeout sets the error word and ends all roles.
-template <int COLS, int GS>
+template <int COLS, int GS, int TERMS>
 __global__ void __launch_bounds__(kQ4Threads, 2)
     q4_kernel(const __grid_constant__ CUtensorMap xmap, const Q4Args a) {
-    using C = Q4Cfg<COLS, GS>;
+    using C = Q4Cfg<COLS, GS, TERMS>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                ~static_cast<uintptr_t>(1023));
-    float* fin = reinterpret_cast<float*>(ring);  // [COLS][LD], after the loop
+    float* fin = reinterpret_cast<float*>(ring);  // [ROWS][LD], after the loop
     uint64_t* in_full = reinterpret_cast<uint64_t*>(ring + C::NS * C::STAGE);
     uint64_t* in_empty = in_full + C::NS;
     uint64_t* a_full = in_empty + C::NS;  // [2]: a unit's weights are in tensor memory
@@ -357,19 +400,13 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
     int64_t g, m0;
     int rows;
     if (!find_rows(a, blockIdx.y, &g, &m0, &rows)) return;  // the whole cluster alike
-    const int cols = rows * a.terms;
     const int p0 = static_cast<int>(a.NP * ks / a.S), np = static_cast<int>(a.NP * (ks + 1) / a.S) - p0;
 
     const uint8_t* src = a.w + ((g * a.NC + tile) * a.NP + p0) * a.block;
     auto copy_weights = [&](int p) {
         uint64_t* full = &in_full[p % C::NS];
         mbar_arrive_expect_tx(full, a.block);
-        bulk_load(ring + p % C::NS * C::STAGE + 2 * C::XB, src + static_cast<int64_t>(p) * a.block, a.block, full);
-    };
-    auto copy_x = [&](int p) {
-        uint64_t* full = &in_full[p % C::NS];
-        mbar_arrive_expect_tx(full, 2 * C::XB);
-        tma_load_3d(ring + p % C::NS * C::STAGE, &xmap, full, 0, static_cast<int>(m0 * a.terms), 2 * (p0 + p));
+        bulk_load(ring + p % C::NS * C::STAGE + C::XB, src + static_cast<int64_t>(p) * a.block, a.block, full);
     };
     if (w == 9) {
         tmem_alloc(tmem_slot, 2 * C::TW);
@@ -378,7 +415,7 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
         // the first weights are on their way before the rest of the set-up
         for (int i = 0; i < C::NS; ++i) {
             mbar_init(&in_full[i], 2);   // both copies
-            mbar_init(&in_empty[i], 4);  // the four warps of the pair's warpgroup
+            mbar_init(&in_empty[i], 4);  // the four warps of the block's warpgroup
         }
         for (int j = 0; j < 2; ++j) {
             mbar_init(&a_full[j], 4);
@@ -403,21 +440,31 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
         return __all_sync(~0u, mbar_wait_bounded(bar, phase & 1, abort_flag, a.err, ERR_GEMM_TIMEOUT)) != 0;
     };
 
-    float acc[COLS] = {};
+    float acc[C::ROWS] = {};
     const int ch = threadIdx.x & 127;
     if (w < 8) {
         const uint32_t quarter = static_cast<uint32_t>(32 * (w & 3)) << 16;
+        // RB rows' terms at a time, whole 8-column loads
+        constexpr int RB = TERMS == kTermsF32 ? 2 : COLS == 16 ? 5 : 8, CB = (RB * TERMS + 7) / 8 * 8;
         auto take = [&](int u, const float (&s)[C::SUB]) {  // unit u's sums, scaled
 #pragma unroll
             for (int j = 0; j < C::SUB; ++j)
 #pragma unroll
-                for (int c = 0; c < COLS; c += 16) {
-                    if (c >= cols) continue;
-                    uint32_t r[16];
-                    tc_ld_32x32b_x16(td + quarter + (u % C::ND * C::SUB + j) * COLS + c, r);
+                for (int r0 = 0; r0 < C::ROWS; r0 += RB) {
+                    if (r0 >= rows) continue;
+                    uint32_t r[CB];
+                    const uint32_t at = td + quarter + (u % C::ND * C::SUB + j) * COLS + r0 * TERMS;
+#pragma unroll
+                    for (int c = 0; c < CB; c += 8) tc_ld_32x32b_x8(at + c, *reinterpret_cast<uint32_t(*)[8]>(r + c));
                     tc_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[c + i] = fmaf(s[j], __uint_as_float(r[i]), acc[c + i]);
+                    for (int i = 0; i < RB; ++i) {
+                        if (r0 + i >= C::ROWS) continue;
+                        float v = __uint_as_float(r[i * TERMS]);
+#pragma unroll
+                        for (int t = 1; t < TERMS; ++t) v += __uint_as_float(r[i * TERMS + t]);
+                        acc[r0 + i] = fmaf(s[j], v, acc[r0 + i]);
+                    }
                 }
             tc_fence_before();
         };
@@ -425,47 +472,46 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
         int u = 0;  // units of this warpgroup so far
         bool ok = true;
         for (int p = wg; ok && p < np; p += 2) {
-            const uint8_t* st = ring + p % C::NS * C::STAGE + 2 * C::XB;
+            const uint8_t* st = ring + p % C::NS * C::STAGE + C::XB;
             if (!(ok = wait(&in_full[p % C::NS], p / C::NS))) break;
-            float s[C::NSC];
+            float s[C::FULL];
 #pragma unroll
-            for (int j = 0; j < C::NSC; ++j)
+            for (int j = 0; j < C::FULL; ++j)
                 s[j] = a.scale_bf16
                            ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(st + 8192)[j * 128 + ch])
                            : reinterpret_cast<const float*>(st + 8192)[j * 128 + ch];
-            auto weights = [&](int i) { return *reinterpret_cast<const uint4*>(st + i * 2048 + ch * 16); };
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                uint32_t v[16];
-                if (C::ND == 2) {  // registers allow converting under the wait
-                    const uint4 q0 = weights(2 * j);
-                    unpack_q4(q0.x, v), unpack_q4(q0.y, v + 4), unpack_q4(q0.z, v + 8), unpack_q4(q0.w, v + 12);
+            for (int j = 0; j < 128 / C::UK; ++j) {
+                uint32_t v[C::UA];
+#pragma unroll
+                for (int i = 0; i < C::UK / 32; ++i) {
+                    const uint4 q = *reinterpret_cast<const uint4*>(st + (j * (C::UK / 32) + i) * 2048 + ch * 16);
+                    const uint32_t word[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        v[8 * i + 2 * e] = word[e] & 0x87878787u;
+                        v[8 * i + 2 * e + 1] = __funnelshift_r(word[e], word[e], 4) & 0x87878787u;
+                    }
                 }
-                if (u && (C::UT == 1 || j == 0)) {
+                if (u) {
                     // the unit before is done: its weights' columns, its
-                    // accumulators and (at a pair's start) its stage are free
+                    // accumulators and (at a block's start) its stage are free
                     if (!(ok = wait(&done[wg], u - 1))) break;
                     tc_fence_after();
                     if (j == 0 && lane == 0) mbar_arrive(&in_empty[(p - 2) % C::NS]);
                     if (C::ND == 1) take(u - 1, s_prev);
                 }
-                if (C::ND == 1) {
-                    const uint4 q0 = weights(2 * j);
-                    unpack_q4(q0.x, v), unpack_q4(q0.y, v + 4), unpack_q4(q0.z, v + 8), unpack_q4(q0.w, v + 12);
-                }
-                const uint32_t at = ta + quarter + (C::UT == 2 ? 32 * j : 0);
-                tc_st_32x32b_x16(at, v);
-                const uint4 q1 = weights(2 * j + 1);
-                unpack_q4(q1.x, v), unpack_q4(q1.y, v + 4), unpack_q4(q1.z, v + 8), unpack_q4(q1.w, v + 12);
-                tc_st_32x32b_x16(at + 16, v);
-                if (C::UT == 2 && j == 0) continue;
+                if constexpr (C::UA == 32)
+                    tc_st_32x32b_x32(ta + quarter, v);
+                else
+                    tc_st_32x32b_x16(ta + quarter, v);
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&a_full[wg]);
                 if (C::ND == 2 && u) take(u - 1, s_prev);
 #pragma unroll
-                for (int i = 0; i < C::SUB; ++i) s_prev[i] = s[C::UT == 2 ? i : j * C::SUB + i];
+                for (int i = 0; i < C::SUB; ++i) s_prev[i] = s[C::UK == 128 ? i : j * 64 / GS + i];
                 ++u;
             }
         }
@@ -474,37 +520,39 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
             take(u - 1, s_prev);
         }
     } else if (w < 10) {
-        const uint32_t idesc = idesc_bf16_f32(128, static_cast<uint32_t>((cols + 15) & ~15));
+        const uint32_t idesc = idesc_e4m3_e5m2_f32(128, static_cast<uint32_t>((rows * TERMS + 15) & ~15));
         int u = 0;
         bool ok = true;
         for (int p = wg; ok && p < np; p += 2) {
             if (!(ok = wait(&in_full[p % C::NS], p / C::NS))) break;
             const uint64_t bd = smem_desc_sw128(smem_u32(ring + p % C::NS * C::STAGE));
 #pragma unroll
-            for (int j = 0; j < 2 / C::UT; ++j) {
+            for (int j = 0; j < 128 / C::UK; ++j) {
                 if (!(ok = wait(&a_full[wg], u))) break;
                 tc_fence_after();
                 const uint32_t d = td + static_cast<uint32_t>(u % C::ND * C::SUB * COLS);
 #pragma unroll
-                for (int m = 0; m < 4 * C::UT; ++m)
-                    tc_mma_f16_ts_elect(d + 16 * m / GS * COLS, ta + 8 * m,
-                                        bd + (j + m / 4) * (C::XB >> 4) + 2 * (m % 4), idesc,
-                                        16 * m % GS ? 1u : 0u);
+                for (int m = 0; m < C::UK / 32; ++m)
+                    tc_mma_f8_ts_elect(d + 32 * m / GS * COLS, ta + 8 * m, bd + 2 * (j * (C::UK / 32) + m), idesc,
+                                       32 * m % GS ? 1u : 0u);
                 tc_commit_elect(&done[wg]);
                 ++u;
             }
         }
     } else if (lane == 0) {
         const bool weights = w == 10;
-        if (!weights && a.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");  // x is the terms kernel's
+        if (!weights) asm volatile("griddepcontrol.wait;" ::: "memory");  // x is the terms kernel's
         int p = weights ? min(np, C::NS) : 0;
         for (; p < np; ++p) {
+            uint64_t* full = &in_full[p % C::NS];
             if (!mbar_wait_bounded(&in_empty[p % C::NS], (p / C::NS & 1) ^ 1, abort_flag, a.err, ERR_GEMM_TIMEOUT))
                 break;
-            if (weights)
+            if (weights) {
                 copy_weights(p);
-            else
-                copy_x(p);
+            } else {
+                mbar_arrive_expect_tx(full, C::XB);
+                tma_load_2d(ring + p % C::NS * C::STAGE, &xmap, full, (p0 + p) * 128, static_cast<int>(m0 * TERMS));
+            }
         }
         if (*abort_flag)  // a failed call leaves no copy in flight behind (bounded as well)
             for (int i = max(0, p - C::NS); i < p; ++i)
@@ -521,28 +569,26 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
     for (int j = 0; j < 2; ++j) {  // the warpgroups' sums
         if (w < 8 && wg == j)
 #pragma unroll
-            for (int c = 0; c < COLS; ++c)
-                if (c < cols) fin[c * C::LD + ch] = j ? fin[c * C::LD + ch] + acc[c] : acc[c];
+            for (int c = 0; c < C::ROWS; ++c)
+                if (c < rows) fin[c * C::LD + ch] = j ? fin[c * C::LD + ch] + acc[c] : acc[c];
         __syncthreads();
     }
     if (a.S > 1) cluster_sync();
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // unscale is the terms kernel's
     for (int i = ks * kQ4Threads + threadIdx.x; i < rows * 128; i += a.S * kQ4Threads) {
         const int r = i >> 7, c = i & 127;
+        const float* p = fin + r * C::LD + c;
         float v = 0.0f;
-        for (int s = 0; s < a.S; ++s)
-            for (int j = 0; j < a.terms; ++j) {
-                const float* p = fin + (r * a.terms + j) * C::LD + c;
-                v += s == ks ? *p : ld_cluster(p, s);
-            }
-        if (tile * 128 + c < a.N) store_out(a, m0 + r, tile * 128 + c, v);
+        for (int s = 0; s < a.S; ++s) v += s == ks ? *p : ld_cluster(p, s);
+        if (tile * 128 + c < a.N) store_out(a, m0 + r, tile * 128 + c, v * a.unscale[m0 + r]);
     }
     if (a.S > 1) cluster_sync();  // the sums stay until every rank has read them
 }
 
-template <int COLS, int GS>
+template <int COLS, int GS, int TERMS>
 aem_status launch_q4(const CUtensorMap& xmap, const Q4Args& a, dim3 grid, cudaStream_t s) {
-    using C = Q4Cfg<COLS, GS>;
-    auto kern = q4_kernel<COLS, GS>;
+    using C = Q4Cfg<COLS, GS, TERMS>;
+    auto kern = q4_kernel<COLS, GS, TERMS>;
     static std::atomic<uint64_t> ready{0};  // bit per device: the shared memory opt-in is done
     const uint64_t bit = 1ull << (current_device() & 63);
     if (!(ready.load(std::memory_order_relaxed) & bit)) {
@@ -555,51 +601,51 @@ aem_status launch_q4(const CUtensorMap& xmap, const Q4Args& a, dim3 grid, cudaSt
     cfg.dynamicSmemBytes = C::SMEM;
     cfg.stream = s;
     cudaLaunchAttribute at[2] = {};
-    int n = 0;
-    if (a.S > 1) {
-        at[n].id = cudaLaunchAttributeClusterDimension;
-        at[n].val.clusterDim.x = a.S;
-        at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
-        ++n;
-    }
-    if (a.dependent) {
-        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        at[n].val.programmaticStreamSerializationAllowed = 1;
-        ++n;
-    }
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // starts under the terms kernel
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = a.S;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = n;
+    cfg.numAttrs = a.S > 1 ? 2 : 1;
     AEM_TRY_CUDA(cudaLaunchKernelEx(&cfg, kern, xmap, a));
     count_launches(1);
     return AEM_OK;
 }
 
-template <int COLS>
-aem_status launch_cols(const void* x, int64_t ldx, int64_t K, Q4Args a, int gs, int64_t slots,
-                       cudaStream_t s) {
-    CUtensorMap xmap;  // [K / 64][rows][64]: one box holds a pair of 64-k tiles
-    AEM_TRY(make_tmap_3d(&xmap, x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 64, a.M * a.terms, K / 64, ldx * 2, 128,
-                         64, COLS, 2, CU_TENSOR_MAP_SWIZZLE_128B));
+template <int COLS, int TERMS>
+aem_status launch_cols(const uint8_t* x, Q4Args a, int gs, int64_t slots, cudaStream_t s) {
+    CUtensorMap xmap;
+    AEM_TRY(make_tmap_2d(&xmap, x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.NP * 128, a.M * TERMS, 128, COLS,
+                         CU_TENSOR_MAP_SWIZZLE_128B));
     // K is split until the CTAs fill the SMs: waves x (a CTA's own latency, as
-    // long as about 8 pairs, and its pairs)
-    const int64_t ctas = a.NC * slots, fit = 148 * 2, pairs = a.NP;
+    // long as about 8 blocks, and its blocks)
+    const int64_t ctas = a.NC * slots, fit = 148 * 2;
     int64_t best = INT64_MAX;
-    for (int S = 1; S <= 8 && S <= std::max<int64_t>(1, pairs / 2); ++S) {
-        const int64_t cost = (ctas * S + fit - 1) / fit * (8 + (pairs + S - 1) / S);
+    for (int S = 1; S <= 8 && S <= std::max<int64_t>(1, a.NP / 2); ++S) {
+        const int64_t cost = (ctas * S + fit - 1) / fit * (8 + (a.NP + S - 1) / S);
         if (cost < best) {
             best = cost;
             a.S = S;
         }
     }
     const dim3 grid(static_cast<unsigned>(a.NC * a.S), static_cast<unsigned>(slots));
-    return gs == 32   ? launch_q4<COLS, 32>(xmap, a, grid, s)
-           : gs == 64 ? launch_q4<COLS, 64>(xmap, a, grid, s)
-                      : launch_q4<COLS, 128>(xmap, a, grid, s);
+    if (gs == 128) return launch_q4<COLS, 128, TERMS>(xmap, a, grid, s);
+    if (gs == 64) return launch_q4<COLS, 64, TERMS>(xmap, a, grid, s);
+    if constexpr (COLS <= 48)  // the largest row tile has no room for groups of 32
+        return launch_q4<COLS, 32, TERMS>(xmap, a, grid, s);
+    set_error("q4 product: no such row tile");
+    return AEM_EINVAL;
+}
+
+size_t q4_workspace(const Q4Weight* w, int terms, int64_t M) {
+    return static_cast<size_t>(M) * terms * w->NP * 128 + static_cast<size_t>(M) * 4;
 }
 
 // x: the caller's rows.
-aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, const void* x, aem_dtype xd,
-                      int64_t ldx, void* workspace, size_t workspace_bytes, cudaStream_t s) {
+template <typename XT, int TERMS>
+aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, const XT* x, int64_t ldx,
+                      void* workspace, size_t workspace_bytes, cudaStream_t s) {
     AEM_REQUIRE(current_device() == w->device, "%s: the weights are on device %d, the current one is %d",
                 what, w->device, current_device());
     a.w = w->data;
@@ -609,50 +655,49 @@ aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, const void*
     a.NC = w->NC;
     a.NP = w->NP;
     a.err = device_error_word(w->device);
-    a.terms = xd == AEM_F32 ? 3 : 1;
-    AEM_REQUIRE(a.M * a.terms < (1ll << 31), "%s: M=%lld out of range", what, (long long)a.M);
-    // columns of a row tile: as many as the rows (grouped: an average group's) need, up to 32
+    AEM_REQUIRE(a.M * TERMS < (1ll << 31), "%s: M=%lld out of range", what, (long long)a.M);
+    // columns of a row tile: as many as the rows (grouped: an average group's) need
     const int64_t groups = std::min<int64_t>(a.G, a.M);
-    const int64_t want = (a.group_rows ? (a.M + groups - 1) / groups : a.M) * a.terms;
-    const int cols = want <= 16 ? 16 : 32;
-    a.rows = cols / a.terms;
+    const int64_t want = a.group_rows ? (a.M + groups - 1) / groups : a.M;
+    const int cols = want <= 16 / TERMS ? 16 : want <= 48 / TERMS || w->gs == 32 ? 48 : 96;
+    a.rows = cols / TERMS;
     const int64_t slots = a.group_rows ? groups + a.M / a.rows : (a.M + a.rows - 1) / a.rows;
     AEM_REQUIRE(slots <= 65535, "%s: M=%lld rows are too many for one call", what, (long long)a.M);
-    const int64_t K = w->K;
-    int64_t KP = K;
+    const size_t need = q4_workspace(w, TERMS, a.M);
+    AEM_REQUIRE(!workspace || (workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
+                "%s: workspace of %zu bytes (%zu needed, 16-byte aligned)", what, workspace_bytes, need);
     void* own = nullptr;
-    if (xd != AEM_BF16 || K % 64 != 0 || (reinterpret_cast<uintptr_t>(x) & 15) != 0 || ldx % 8 != 0 || ldx < K) {
-        KP = (K + 63) / 64 * 64;
-        const size_t need = static_cast<size_t>(a.M) * a.terms * KP * 2;
-        AEM_REQUIRE(!workspace || (workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
-                    "%s: workspace of %zu bytes (%zu needed, 16-byte aligned)", what, workspace_bytes, need);
-        if (!workspace) {
-            AEM_TRY_CUDA(cudaMallocAsync(&own, need, s));
-            workspace = own;
-        }
-        auto* t = static_cast<__nv_bfloat16*>(workspace);
-        const unsigned g = static_cast<unsigned>(std::min<int64_t>((a.M * KP + kThreads - 1) / kThreads, 148 * 8));
-        if (xd == AEM_F32)
-            q4_terms_kernel<float><<<g, kThreads, 0, s>>>(static_cast<const float*>(x), ldx, a.M, K, KP, t);
-        else
-            q4_terms_kernel<__nv_bfloat16><<<g, kThreads, 0, s>>>(static_cast<const __nv_bfloat16*>(x), ldx,
-                                                                  a.M, K, KP, t);
-        count_launches(1);
-        a.dependent = true;
-        x = t;
-        ldx = KP;
+    if (!workspace) {
+        AEM_TRY_CUDA(cudaMallocAsync(&own, need, s));
+        workspace = own;
     }
+    auto* terms = static_cast<uint8_t*>(workspace);
+    auto* unscale = reinterpret_cast<float*>(terms + static_cast<size_t>(a.M) * TERMS * w->NP * 128);
+    a.unscale = unscale;
+    const bool vec = reinterpret_cast<uintptr_t>(x) % (4 * sizeof(XT)) == 0 && ldx % 4 == 0;
+    q4_terms_kernel<XT, TERMS><<<static_cast<unsigned>(a.M), 512, 0, s>>>(x, ldx, w->K, w->NP * 128, vec, terms,
+                                                                          unscale);
+    count_launches(1);
     const cudaError_t e = cudaGetLastError();
     aem_status st;
     if (e != cudaSuccess) {
         set_error("%s: launch failed: %s", what, cudaGetErrorString(e));
         st = AEM_ECUDA;
     } else {
-        st = cols == 16 ? launch_cols<16>(x, ldx, KP, a, w->gs, slots, s)
-                        : launch_cols<32>(x, ldx, KP, a, w->gs, slots, s);
+        st = cols == 16   ? launch_cols<16, TERMS>(terms, a, w->gs, slots, s)
+             : cols == 48 ? launch_cols<48, TERMS>(terms, a, w->gs, slots, s)
+                          : launch_cols<96, TERMS>(terms, a, w->gs, slots, s);
     }
     if (own) cudaFreeAsync(own, s);
     return st;
+}
+
+aem_status q4_any(const Q4Weight* w, const char* what, const Q4Args& a, const void* x, aem_dtype xd,
+                  int64_t ldx, void* workspace, size_t bytes, cudaStream_t s) {
+    if (xd == AEM_F32)
+        return q4_product<float, kTermsF32>(w, what, a, static_cast<const float*>(x), ldx, workspace, bytes, s);
+    return q4_product<__nv_bfloat16, kTermsBf16>(w, what, a, static_cast<const __nv_bfloat16*>(x), ldx, workspace,
+                                                 bytes, s);
 }
 
 bool is_dtype(aem_dtype t) { return t == AEM_F32 || t == AEM_BF16; }
@@ -780,7 +825,7 @@ aem_status aem_q4weight_pack(const int8_t* q, const void* scale, aem_dtype scale
     AEM_REQUIRE(q && scale, "aem_q4weight_pack: NULL buffer");
     const int64_t count = G * K * N, KB = (K + group_size - 1) / group_size;
     for (int64_t i = 0; i < count; ++i)
-        AEM_REQUIRE(q[i] >= -8 && q[i] <= 7, "aem_q4weight_pack: q[%lld]=%d is outside [-8, 7]",
+        AEM_REQUIRE(q[i] >= -7 && q[i] <= 7, "aem_q4weight_pack: q[%lld]=%d is outside [-7, 7]",
                     (long long)i, q[i]);
     if (!aem::is_sm100(device)) {
         set_error("aem_q4weight_pack: device %d is not an sm_100 (B200) GPU", device);
@@ -839,8 +884,7 @@ aem_status aem_q4weight_shape(aem_q4weight_t wh, int64_t* G, int64_t* K, int64_t
 
 size_t aem_q4gemm_workspace(aem_q4weight_t wh, aem_dtype x_dtype, int64_t M) {
     if (!wh || M < 1 || !aem::is_dtype(x_dtype)) return 0;
-    const int64_t KP = (reinterpret_cast<aem::Q4Weight*>(wh)->K + 63) / 64 * 64;
-    return static_cast<size_t>(M) * (x_dtype == AEM_F32 ? 3 : 1) * KP * 2;
+    return aem::q4_workspace(reinterpret_cast<aem::Q4Weight*>(wh), x_dtype == AEM_F32 ? aem::kTermsF32 : aem::kTermsBf16, M);
 }
 
 aem_status aem_q4gemm(aem_q4weight_t wh, int64_t group, const void* x, aem_dtype x_dtype,
@@ -862,7 +906,7 @@ aem_status aem_q4gemm(aem_q4weight_t wh, int64_t group, const void* x, aem_dtype
     a.group = group;
     a.G = 1;
     a.out_bf16 = out_dtype == AEM_BF16;
-    return aem::q4_product(w, "aem_q4gemm", a, x, x_dtype, ldx, workspace, workspace_bytes,
+    return aem::q4_any(w, "aem_q4gemm", a, x, x_dtype, ldx, workspace, workspace_bytes,
                            static_cast<cudaStream_t>(stream));
 }
 
@@ -887,7 +931,7 @@ aem_status aem_grouped_q4gemm(aem_q4weight_t wh, const int32_t* group_rows, cons
     a.G = static_cast<int>(w->G);
     a.out_bf16 = out_dtype == AEM_BF16;
     a.relu = relu != 0;
-    return aem::q4_product(w, "aem_grouped_q4gemm", a, x, x_dtype, ldx, workspace, workspace_bytes,
+    return aem::q4_any(w, "aem_grouped_q4gemm", a, x, x_dtype, ldx, workspace, workspace_bytes,
                            static_cast<cudaStream_t>(stream));
 }
 

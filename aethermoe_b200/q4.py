@@ -47,7 +47,7 @@ def quantize_q4(w, group_size=128, scale_dtype=torch.float32, stream=None):
 
 class Q4Weight:
     """Packed 4-bit weight groups: ``q [K, N]`` or ``[G, K, N]`` int8 with values in
-    [-8, 7] and ``scale [(G,) ceil(K/group_size), N]`` (float32 or bfloat16).
+    [-7, 7] and ``scale [(G,) ceil(K/group_size), N]`` (float32 or bfloat16).
     CUDA tensors are packed on the device (the call waits for it and raises on
     a value out of range), CPU tensors and NumPy arrays through
     ``aem_q4weight_pack`` onto ``device``."""
@@ -109,13 +109,9 @@ def _check_weight(w, device):
         raise ValueError(f"x is on {device}, the weight on cuda:{w.device}")
 
 
-def _scratch(x, ldx, w):
-    """Scratch of a product, or None where x is read in place."""
-    if x.dtype == torch.bfloat16 and w.K % 8 == 0 and ldx % 8 == 0 and x.data_ptr() % 16 == 0:
-        return None, 0, None
+def _scratch(x, w):
     n = _lib.lib().aem_q4gemm_workspace(w.handle, _DT[x.dtype], x.shape[0])
-    ws = torch.empty(max(n, 1), dtype=torch.uint8, device=x.device)
-    return ws.data_ptr(), n, ws
+    return torch.empty(max(n, 1), dtype=torch.uint8, device=x.device), n
 
 
 def _matmul(x, w, group, out_dtype, out, s):
@@ -123,9 +119,9 @@ def _matmul(x, w, group, out_dtype, out, s):
     _check_weight(w, x.device)
     m = x.shape[0]
     out, ldo = _output(out, (m, w.N), out_dtype or (x.dtype if out is None else out.dtype), x.device)
-    ws, n, keep = _scratch(x, ldx, w)
+    ws, n = _scratch(x, w)
     _lib.check(_lib.lib().aem_q4gemm(w.handle, group, x.data_ptr(), _DT[x.dtype], ldx, m,
-                                     out.data_ptr(), _DT[out.dtype], ldo, ws, n, s), "aem_q4gemm")
+                                     out.data_ptr(), _DT[out.dtype], ldo, ws.data_ptr(), n, s), "aem_q4gemm")
     return out
 
 
@@ -136,10 +132,10 @@ def _grouped(x, w, starts, relu, out_dtype, out, s):
         raise ValueError(f"starts must be {w.G + 1} contiguous int32 offsets")
     m = x.shape[0]
     out, ldo = _output(out, (m, w.N), out_dtype or (x.dtype if out is None else out.dtype), x.device)
-    ws, n, keep = _scratch(x, ldx, w)
+    ws, n = _scratch(x, w)
     _lib.check(_lib.lib().aem_grouped_q4gemm(w.handle, starts.data_ptr(), x.data_ptr(), _DT[x.dtype],
                                              ldx, m, out.data_ptr(), _DT[out.dtype], ldo,
-                                             1 if relu else 0, ws, n, s), "aem_grouped_q4gemm")
+                                             1 if relu else 0, ws.data_ptr(), n, s), "aem_grouped_q4gemm")
     return out
 
 

@@ -351,10 +351,10 @@ aem_status aem_quantize_q4(const void* w, aem_dtype w_dtype, int64_t G, int64_t 
 typedef struct aem_q4weight_s* aem_q4weight_t;
 
 /* Packs G groups (experts) of 4-bit weights, q [G][K][N] int8 holding values
- * in [-8, 7] and scale [G][ceil(K/group_size)][N] (float32 or bf16, kept as
+ * in [-7, 7] and scale [G][ceil(K/group_size)][N] (float32 or bf16, kept as
  * given), into a device-resident copy of K*N/2 bytes per group laid out as
  * the product's matrix fragments.  Same from HOST memory (a value outside
- * [-8, 7] -> AEM_EINVAL) and from DEVICE memory (stream-ordered; such a value
+ * [-7, 7] -> AEM_EINVAL) and from DEVICE memory (stream-ordered; such a value
  * is clamped and reported by aem_device_status). */
 aem_status aem_q4weight_pack(const int8_t* q, const void* scale, aem_dtype scale_dtype, int64_t G,
                              int64_t K, int64_t N, int group_size, int device, aem_q4weight_t* out);
@@ -366,16 +366,18 @@ aem_status aem_q4weight_free(aem_q4weight_t w);
 aem_status aem_q4weight_shape(aem_q4weight_t w, int64_t* G, int64_t* K, int64_t* N, int* group_size);
 
 /* out[M, N] = x[M, K] @ (q[group] * scale[group]) for the few rows of a
- * decoding step: one pass over the weights for up to 64 bf16 or 21 float32
- * rows, one more for every further such tile of rows.  The integers are
- * exact in the MMAs' bf16 operands, each scale multiplies a float32 sum, and
- * float32 x takes part in full (three bf16 terms), so nothing is rounded
- * before out.  Rows of x are ldx elements apart, rows of out ldo; any
- * alignment works.  bf16 x with 16-byte rows and K % 8 == 0 is read in place;
- * other x first becomes bf16 terms in the workspace: device scratch of
- * aem_q4gemm_workspace(w, x_dtype, M) bytes, 16-byte aligned, or NULL to have
- * the call allocate and free it in stream order.  The weights' device must be
- * the current one.  Results repeat bit for bit. */
+ * decoding step: one pass over the weights for up to 32 bf16 or 12 float32
+ * rows (16 or 6 with groups of 32), one more for every further such tile.
+ * The integers are exact in the MMAs' operands, each scale multiplies a
+ * float32 sum, and x takes part in full: what is cut from an element is
+ * under 2^-30 of its row's largest finite magnitude (nothing for bf16
+ * elements down to 2^-23 of it), so nothing is rounded before out but the
+ * float32 sums.  Infinities and NaN act as in x @ w.  Rows of x are ldx
+ * elements apart, rows of out ldo; any alignment works.  The workspace holds
+ * x in the products' form: device scratch of aem_q4gemm_workspace(w,
+ * x_dtype, M) bytes, 16-byte aligned, or NULL to have the call allocate and
+ * free it in stream order.  The weights' device must be the current one.
+ * Results repeat bit for bit. */
 size_t aem_q4gemm_workspace(aem_q4weight_t w, aem_dtype x_dtype, int64_t M);
 aem_status aem_q4gemm(aem_q4weight_t w, int64_t group, const void* x, aem_dtype x_dtype,
                       int64_t ldx, int64_t M, void* out, aem_dtype out_dtype, int64_t ldo,

@@ -82,8 +82,8 @@ def test_q4_refusals():
         assert pack(**bad) == EINVAL, bad
     wrong = q.copy()
     wrong[5, 7] = 8
-    assert pack(q=wrong) == EINVAL and "[-8, 7]" in _lib.last_error()
-    wrong[5, 7] = -9
+    assert pack(q=wrong) == EINVAL and "[-7, 7]" in _lib.last_error()
+    wrong[5, 7] = -8
     assert pack(q=wrong) == EINVAL
     if _lib.device_count() == 0:
         assert pack() == _lib.AEM_EUNSUPPORTED
@@ -121,5 +121,5 @@ def test_python_forms_refuse_before_the_library():
         q4.Q4Weight(torch.zeros(64, 32), torch.zeros(2, 32), 32)
     with pytest.raises(ValueError, match="scale must be"):
         q4.Q4Weight(torch.zeros(65, 32, dtype=torch.int8), torch.zeros(2, 32), 32)
-    with pytest.raises(ValueError, match="-8, 7"):
+    with pytest.raises(ValueError, match="-7, 7"):
         q4.Q4Weight(torch.full((64, 32), 9, dtype=torch.int8), torch.zeros(2, 32), 32)
