@@ -127,7 +127,7 @@ _SIGS = {
     "aem_q4weight_free": (_int, [_vp]),
     "aem_q4weight_shape": (_int, [_vp, ctypes.POINTER(_i64), ctypes.POINTER(_i64),
                                   ctypes.POINTER(_i64), ctypes.POINTER(_int)]),
-    "aem_q4gemm_workspace": (ctypes.c_size_t, [_vp, _int, _i64]),
+    "aem_q4gemm_workspace": (ctypes.c_size_t, [_vp, _int, _i64, _int]),
     "aem_q4gemm": (_int, [_vp, _i64, _vp, _int, _i64, _i64, _vp, _int, _i64, _vp, ctypes.c_size_t, _vp]),
     "aem_grouped_q4gemm": (_int, [_vp, _vp, _vp, _int, _i64, _i64, _vp, _int, _i64, _int, _vp,
                                   ctypes.c_size_t, _vp]),

@@ -78,6 +78,10 @@ bool is_sm100(int device);
 aem_status make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype,
                         int elem_bytes, uint64_t cols, uint64_t rows, uint32_t box_cols,
                         uint32_t box_rows, CUtensorMapSwizzle swizzle);
+// 3-D byte map: dim0 bytes innermost, dim1 rows row_bytes apart, dim2 planes
+// plane_bytes apart (multiples of 16); 128-byte swizzle.
+aem_status make_tmap_3d_u8(CUtensorMap* map, const void* base, uint64_t dim0, uint64_t dim1, uint64_t dim2,
+                           uint64_t row_bytes, uint64_t plane_bytes, uint32_t box1, uint32_t box2);
 
 }  // namespace aem
 
@@ -174,6 +178,15 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const void* map, uint64_t
         "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
         " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
         "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const void* map, uint64_t* bar, int x,
+                                            int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
         : "memory");
 }
 

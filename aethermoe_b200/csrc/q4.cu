@@ -16,9 +16,11 @@
 // Three terms hold a bf16 value and eight a float32 value exactly unless its
 // last bits lie below rho * |x| = 2^-16; what is cut off there is under 2^-30
 // of the row's largest magnitude, below the rounding of a float32 sum that
-// holds it.  Every product is exact, sums are float32 (tcgen05, accumulators
-// in TMEM), the terms' sums are added and the scales multiply the result in
-// float32: no rounded weight ever exists.
+// holds it.  A row's terms sit side by side in MMA columns whose sums are
+// added (few rows: a tile is 16 columns at least), or follow one another into
+// the same column.  Every product is exact, sums are float32 (tcgen05,
+// accumulators in TMEM), and the scales multiply them in float32: no rounded
+// weight ever exists.
 //
 // What bounds it is the weight stream, K*N/2 bytes plus the scales.  Forms
 // that could not keep up with it (4096 x 14336, 1 row): warp MMAs (mma.sync
@@ -185,90 +187,162 @@ using namespace aem::dev;
 
 struct Q4Args {
     const uint8_t* w;
-    const float* unscale;       // [M]: 2^9 / rho of a row of x
+    const void* x;              // the caller's rows (ldx elements apart), for kernels that make the terms
+    const float* unscale;       // [M]: 2^9 / rho of a row, from the terms kernel
     void* out;
     const int32_t* group_rows;  // nullptr: one group of M rows, weight group `group`
-    int64_t ldo, M, N, NC, NP;
+    int64_t ldx, ldo, M, N, K;
     int64_t group;
     int* err;
-    int G, block, S, rows;  // S: CTAs (one cluster) that split K; rows: rows of a row tile
-    bool scale_bf16, out_bf16, relu;
+    int NC, NP, G, block, S, rows;  // S: CTAs (one cluster) that split K; rows: rows of a row tile
+    bool scale_bf16, out_bf16, relu, vec;  // vec: x can be read in vectors of 4
 };
 
-constexpr int kTermsBf16 = 3, kTermsF32 = 8;
+template <typename XT>
+constexpr int kTerms = sizeof(XT) == 4 ? 8 : 3;
 
-// Activations as the products read them, one block per row: out [M * terms]
-// [KP] e5m2 bytes (KP = K rounded up to 128, zero padded), unscale [M].  An
-// infinity or NaN is all in the first term.  e5m2 is the upper byte of an
-// fp16, so truncating the fp16 truncates the term.
-template <typename XT, int TERMS>
-__global__ void __launch_bounds__(512)
-    q4_terms_kernel(const XT* __restrict__ x, int64_t ldx, int64_t K, int64_t KP, bool vec,
-                    uint8_t* __restrict__ out, float* __restrict__ unscale) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    __shared__ uint32_t top[16];
-    const XT* row = x + blockIdx.x * ldx;
-    auto load4 = [&](int64_t k, float (&v)[4]) {
+// Four elements of a row from k on, zero past K, as they lie in memory.
+template <typename XT>
+struct Four {
+    uint32_t w[sizeof(XT)];
+    __device__ __forceinline__ void load(const XT* row, int64_t k, int64_t K, bool vec) {
         if (vec && k + 4 <= K) {
             if constexpr (sizeof(XT) == 4) {
-                const float4 f = *reinterpret_cast<const float4*>(row + k);
-                v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+                const uint4 u = *reinterpret_cast<const uint4*>(row + k);
+                w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
             } else {
                 const uint2 u = *reinterpret_cast<const uint2*>(row + k);
-                v[0] = __uint_as_float(u.x << 16), v[1] = __uint_as_float(u.x & 0xffff0000u);
-                v[2] = __uint_as_float(u.y << 16), v[3] = __uint_as_float(u.y & 0xffff0000u);
+                w[0] = u.x, w[1] = u.y;
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = k + i < K ? static_cast<float>(row[k + i]) : 0.0f;
-        }
-    };
-    uint32_t mine = 0;  // magnitudes order as their bits do
-    for (int64_t k = threadIdx.x * 4; k < K; k += 512 * 4) {
-        float v[4];
-        load4(k, v);
+            for (int i = 0; i < static_cast<int>(sizeof(XT)); ++i) w[i] = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t u = __float_as_uint(v[i]) & 0x7fffffffu;
-            if (u < 0x7f800000u) mine = max(mine, u);
+            for (int i = 0; i < 4; ++i)
+                if (k + i < K) {
+                    if constexpr (sizeof(XT) == 4)
+                        w[i] = __float_as_uint(row[k + i]);
+                    else
+                        w[i / 2] |= static_cast<uint32_t>(__bfloat16_as_ushort(row[k + i])) << (16 * (i & 1));
+                }
         }
     }
-    mine = __reduce_max_sync(~0u, mine);
-    if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = mine;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 16; ++i) mine = max(mine, top[i]);
-    // rho = 2^up, up = 14 - exponent, in two factors (it may be beyond float32)
-    const int up = 141 - static_cast<int>(mine >> 23);
-    const float f1 = __uint_as_float(static_cast<uint32_t>(127 + up / 2) << 23);
-    const float f2 = __uint_as_float(static_cast<uint32_t>(127 + up - up / 2) << 23);
-    if (threadIdx.x == 0) unscale[blockIdx.x] = ldexpf(1.0f, 9 - up);
-    uint8_t* o = out + blockIdx.x * TERMS * KP;
-    for (int64_t k = threadIdx.x * 4; k < KP; k += 512 * 4) {
-        float v[4];
-        load4(k, v);
-        uint32_t t[TERMS];
-#pragma unroll
-        for (int j = 0; j < TERMS; ++j) t[j] = 0;
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (sizeof(XT) == 4) return __uint_as_float(w[i]);
+        return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    }
+    // Bits of the largest finite magnitude (they order as the magnitudes do).
+    __device__ __forceinline__ uint32_t top() const {
+        uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const bool finite = (__float_as_uint(v[i]) & 0x7f800000u) != 0x7f800000u;
-            float r = v[i] * f1 * f2;
+            const uint32_t u = __float_as_uint(get(i)) & 0x7fffffffu;
+            if (u < 0x7f800000u) m = max(m, u);
+        }
+        return m;
+    }
+};
+// rho = 2^up for a row whose top magnitude has these bits; 2^9 / rho.
+__device__ __forceinline__ int rho_exponent(uint32_t top) { return 141 - static_cast<int>(top >> 23); }
+__device__ __forceinline__ float unscale_of(uint32_t top) {
+    const int e = 9 - rho_exponent(top);  // -132 .. 122
+    return __uint_as_float(e >= -126 ? static_cast<uint32_t>(127 + e) << 23 : 1u << (149 + e));
+}
+
+// The terms of four elements, one byte each.  e5m2 is the upper byte of an
+// fp16, so truncating an fp16 by a mask truncates the term; a scaled bf16 is
+// an fp16 (down to 2^-24, where the terms end at 2^-16), and a scaled float32
+// is taken apart nine bits, three terms, at a time.  An infinity or NaN is
+// all in the first term.
+template <typename XT>
+__device__ __forceinline__ void terms4(const Four<XT>& x, int up, uint32_t (&t)[kTerms<XT>]) {
+    constexpr int TERMS = kTerms<XT>, STEPS = (TERMS + 2) / 3;
+    // two factors: rho itself may be beyond float32
+    const float f1 = __uint_as_float(static_cast<uint32_t>(127 + up / 2) << 23);
+    const float f2 = __uint_as_float(static_cast<uint32_t>(127 + up - up / 2) << 23);
+    float r[4];
+    uint32_t special = 0;
 #pragma unroll
-            for (int j = 0; j < TERMS; ++j) {
-                const uint32_t h = __half_as_ushort(__float2half_rz(r)) & 0xff00u;
-                t[j] |= (h >> 8) << (8 * i);
-                r -= __half2float(__ushort_as_half(static_cast<unsigned short>(h)));
-            }
-            if (!finite) {
-                const uint32_t code = v[i] != v[i] ? 0x7fu : v[i] > 0.0f ? 0x7cu : 0xfcu;
+    for (int i = 0; i < 4; ++i) {
+        const float v = x.get(i);
+        r[i] = v * f1 * f2;
+        if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) {
+            r[i] = 0.0f;
+            special |= (v != v ? 0x7fu : v > 0.0f ? 0x7cu : 0xfcu) << (8 * i);
+        }
+    }
 #pragma unroll
-                for (int j = 0; j < TERMS; ++j)
-                    t[j] = (t[j] & ~(0xffu << (8 * i))) | (j == 0 ? code << (8 * i) : 0u);
+    for (int s = 0; s < STEPS; ++s) {
+        uint32_t h[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(h[i]) : "f"(r[2 * i + 1]), "f"(r[2 * i]));
+            if (STEPS > 1) {
+                h[i] &= 0xfffcfffcu;
+                const __half2 hh = *reinterpret_cast<const __half2*>(&h[i]);
+                r[2 * i] -= __low2float(hh);
+                r[2 * i + 1] -= __high2float(hh);
             }
         }
 #pragma unroll
-        for (int j = 0; j < TERMS; ++j) *reinterpret_cast<uint32_t*>(o + j * KP + k) = t[j];
+        for (int j = 0; j < 3; ++j) {
+            if (3 * s + j >= TERMS) continue;
+            t[3 * s + j] = __byte_perm(h[0], h[1], 0x7531);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t m = h[i] & 0xff00ff00u;
+                const __half2 left = __hsub2(*reinterpret_cast<const __half2*>(&h[i]), *reinterpret_cast<const __half2*>(&m));
+                h[i] = *reinterpret_cast<const uint32_t*>(&left);
+            }
+        }
+    }
+    t[0] |= special;
+}
+
+// Activations as the products read them, one block per row: bytes
+// [terms / tn][M][tn][KP] (KP = K rounded up to 128, zero padded), unscale [M].
+template <typename XT>
+__global__ void __launch_bounds__(1024)
+    q4_terms_kernel(const XT* __restrict__ x, int64_t ldx, int64_t K, int64_t KP, int tn, bool vec,
+                    uint8_t* __restrict__ out, float* __restrict__ unscale) {
+    constexpr int TERMS = kTerms<XT>, HELD = 4;  // up to 16384 k stay in registers
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    __shared__ uint32_t tops[32];
+    const XT* row = x + blockIdx.x * ldx;
+    Four<XT> v[HELD];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) v[i].load(row, (i * 1024 + threadIdx.x) * 4, K, vec);
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) top = max(top, v[i].top());
+    for (int64_t k = (HELD * 1024 + threadIdx.x) * 4; k < K; k += 4096) {
+        Four<XT> u;
+        u.load(row, k, K, vec);
+        top = max(top, u.top());
+    }
+    top = __reduce_max_sync(~0u, top);
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+    top = __reduce_max_sync(~0u, tops[threadIdx.x & 31]);
+    const int up = rho_exponent(top);
+    if (threadIdx.x == 0) unscale[blockIdx.x] = unscale_of(top);
+    auto put = [&](int64_t k, const Four<XT>& u) {
+        uint32_t t[TERMS];
+        terms4(u, up, t);
+#pragma unroll
+        for (int j = 0; j < TERMS; ++j)
+            *reinterpret_cast<uint32_t*>(
+                out + ((j / tn * static_cast<int64_t>(gridDim.x) + blockIdx.x) * tn + j % tn) * KP + k) = t[j];
+    };
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+        const int64_t k = (i * 1024 + threadIdx.x) * 4;
+        if (k < KP) put(k, v[i]);
+    }
+    for (int64_t k = (HELD * 1024 + threadIdx.x) * 4; k < KP; k += 4096) {
+        Four<XT> u;
+        u.load(row, k, K, vec);
+        put(k, u);
     }
 }
 
@@ -319,10 +393,8 @@ __device__ __forceinline__ bool find_rows(const Q4Args& a, int slot, int64_t* g,
     return false;
 }
 
-__device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_u32(p, rank)) : "memory");
-    return v;
+__device__ __forceinline__ void st_cluster(const float* p, uint32_t rank, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_u32(p, rank)), "f"(v) : "memory");
 }
 
 __device__ __forceinline__ void store_out(const Q4Args& a, int64_t m, int64_t n, float v) {
@@ -333,33 +405,39 @@ __device__ __forceinline__ void store_out(const Q4Args& a, int64_t m, int64_t n,
         static_cast<float*>(a.out)[m * a.ldo + n] = v;
 }
 
-// Shape of the product kernel for COLS MMA columns, scale groups of GS k and
-// TERMS columns a row.  A block of the packed weight is 128 channels x 128 k;
-// a unit is what a warpgroup hands to the tensor core at once: a block, with
-// one accumulator per scale group side by side, or half of one where a
-// block's accumulators would not fit.
-template <int COLS, int GS, int TERMS>
+// Shape of the product kernel: COLS MMA columns, scale groups of GS k, a row's
+// TN * TK terms in TN columns, TK after one another.  A block of the packed
+// weight is 128 channels x 128 k; a unit is what a warpgroup hands to the
+// tensor core at once: a block, with one accumulator per scale group side by
+// side, or half of one where a block's accumulators would not fit.  With TK ==
+// 1 (few rows) the CTA makes the terms of its part of K itself and keeps them
+// in shared memory; otherwise a terms kernel has made them and they come with
+// the ring.
+template <int COLS, int GS, int TN, int TK>
 struct Q4Cfg {
-    static constexpr int ROWS = COLS / TERMS;
+    static constexpr int ROWS = COLS / TN;
+    static constexpr bool XIN = TK == 1;
     static constexpr int TW = 128;                     // TMEM columns of a warpgroup: 4 per SM
     static constexpr int FULL = GS == 128 ? 1 : 128 / GS;  // scale groups of a block
     static constexpr int UK = FULL * COLS <= 96 ? 128 : 64;  // k of a unit
     static constexpr int SUB = UK < GS ? 1 : UK / GS;  // accumulators per unit
     static constexpr int UA = UK / 4;                  // columns of a unit's weights
     static constexpr int ND = UA + 2 * SUB * COLS <= TW ? 2 : 1;  // accumulator buffers
-    static constexpr int XB = COLS * 128;              // activation bytes of a block
-    static constexpr int STAGE = XB + 8192 + (FULL * 512 + 1023) / 1024 * 1024;
+    static constexpr int XB = TK * COLS * 128;         // activation bytes of a block
+    static constexpr int MAXP = 20;                    // XIN: blocks whose terms are kept
+    static constexpr int XRES = XIN ? MAXP * XB : 0;
+    static constexpr int STAGE = (XIN ? 0 : XB) + 8192 + (FULL * 512 + 1023) / 1024 * 1024;
+    static constexpr int RECV = (ROWS * 128 + 8) * 4;  // the cluster's sums, S equal shares
     // an even ring: a stage always comes back to the warpgroup that saw its
     // previous phase, so no parity wait can mistake a phase for the one two back
-    static constexpr int FIT = (113 * 1024 - 2048) / STAGE / 2 * 2;
+    static constexpr int FIT = (113 * 1024 - 2048 - XRES - RECV) / STAGE / 2 * 2;
     static constexpr int NS = FIT > 8 ? 8 : FIT;
-    static constexpr int LD = 128 + 4;
-    static constexpr int USED = 1024 + NS * STAGE + (2 * NS + 4) * 8 + 16;
+    static constexpr int USED = 1024 + NS * STAGE + XRES + RECV + (2 * NS + 5) * 8 + 16 + ROWS * 4;
     // two CTAs on an SM, never three: no CTA ever waits for tensor memory
     static constexpr int SMEM = USED > 78 * 1024 ? USED : 78 * 1024;
     static_assert(UA + ND * SUB * COLS <= TW && NS >= 4 && SMEM <= 113 * 1024, "budgets");
     static_assert(UK >= GS || UK == 128, "a scale group inside a unit");
-    static_assert(NS * STAGE >= ROWS * LD * 4, "the sums fit the ring");
+    static_assert(STAGE * NS >= RECV, "a warpgroup's sums fit the ring");
 };
 constexpr int kQ4Threads = 12 * 32;
 
@@ -374,39 +452,58 @@ constexpr int kQ4Threads = 12 * 32;
 //   warps 8-9   one per warpgroup, issue its MMAs (M = 128 channels, N =
 //               columns, K = 32); one commit per unit.
 //   warp 10     copies the weights with their scales, one bulk copy per block.
-//   warp 11     copies the activations, one TMA box per block (128-byte swizzle).
+//   warp 11     copies the activations' terms, one TMA box per block
+//               (128-byte swizzle), where the CTA does not make them itself.
 // Two accumulator buffers let the sums be taken back under the next unit's
 // MMAs; where only one fits they are taken before the unit is handed over.
-// The S CTAs of a cluster take parts of K; their sums are added in rank order.
+// The S CTAs of a cluster take parts of K: each sends its sums to the rank
+// that writes those outputs, which adds them in rank order.
 // Every wait is bounded; a timeout sets the error word and ends all roles.
-template <int COLS, int GS, int TERMS>
+template <typename XT, int COLS, int GS, int TN, int TK>
 __global__ void __launch_bounds__(kQ4Threads, 2)
     q4_kernel(const __grid_constant__ CUtensorMap xmap, const Q4Args a) {
-    using C = Q4Cfg<COLS, GS, TERMS>;
+    using C = Q4Cfg<COLS, GS, TN, TK>;
     extern __shared__ uint8_t smem_raw[];
-    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+    uint8_t* xres = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                ~static_cast<uintptr_t>(1023));
-    float* fin = reinterpret_cast<float*>(ring);  // [ROWS][LD], after the loop
-    uint64_t* in_full = reinterpret_cast<uint64_t*>(ring + C::NS * C::STAGE);
+    uint8_t* ring = xres + C::XRES;
+    float* recv = reinterpret_cast<float*>(ring + C::NS * C::STAGE);  // [S][share of ROWS * 128]
+    uint64_t* in_full = reinterpret_cast<uint64_t*>(recv + C::RECV / 4);
     uint64_t* in_empty = in_full + C::NS;
     uint64_t* a_full = in_empty + C::NS;  // [2]: a unit's weights are in tensor memory
     uint64_t* done = a_full + 2;          // [2]: its MMAs have finished
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 2);
+    uint64_t* x_made = done + 2;          // XIN: the terms are in shared memory
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(x_made + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    uint32_t* row_top = tmem_slot + 2;    // [ROWS], XIN
 
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int64_t tile = blockIdx.x / a.S;
-    const int ks = blockIdx.x % a.S;
+    const int tile = static_cast<int>(blockIdx.x) / a.S, ks = static_cast<int>(blockIdx.x) % a.S;
     int64_t g, m0;
     int rows;
     if (!find_rows(a, blockIdx.y, &g, &m0, &rows)) return;  // the whole cluster alike
-    const int p0 = static_cast<int>(a.NP * ks / a.S), np = static_cast<int>(a.NP * (ks + 1) / a.S) - p0;
+    const int p0 = a.NP * ks / a.S, np = a.NP * (ks + 1) / a.S - p0;
 
-    const uint8_t* src = a.w + ((g * a.NC + tile) * a.NP + p0) * a.block;
+    // XIN: a warp takes 128 k of a row, a lane four of them.  These loads go out
+    // ahead of the weights, behind which they would wait for microseconds.
+    constexpr int HELD = C::XIN ? (C::ROWS * C::MAXP + 7) / 8 : 1;
+    Four<XT> xv[HELD];
+    if (C::XIN && w < 8) {
+        const XT* x = static_cast<const XT*>(a.x) + m0 * a.ldx + static_cast<int64_t>(p0) * 128 + lane * 4;
+        const int64_t left = a.K - static_cast<int64_t>(p0) * 128 - lane * 4;
+        int r = 0, p = w;
+#pragma unroll
+        for (int h = 0; h < HELD; ++h, p += 8) {
+            while (p >= np) p -= np, ++r;
+            if (r >= rows) break;
+            xv[h].load(x + r * a.ldx, p * 128, left, a.vec);
+        }
+    }
+    const uint8_t* src = a.w + ((g * a.NC + tile) * a.NP + p0) * static_cast<int64_t>(a.block);
     auto copy_weights = [&](int p) {
         uint64_t* full = &in_full[p % C::NS];
         mbar_arrive_expect_tx(full, a.block);
-        bulk_load(ring + p % C::NS * C::STAGE + C::XB, src + static_cast<int64_t>(p) * a.block, a.block, full);
+        bulk_load(ring + p % C::NS * C::STAGE, src + static_cast<int64_t>(p) * a.block, a.block, full);
     };
     if (w == 9) {
         tmem_alloc(tmem_slot, 2 * C::TW);
@@ -414,22 +511,26 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
     } else if (w == 10 && lane == 0) {
         // the first weights are on their way before the rest of the set-up
         for (int i = 0; i < C::NS; ++i) {
-            mbar_init(&in_full[i], 2);   // both copies
-            mbar_init(&in_empty[i], 4);  // the four warps of the block's warpgroup
+            mbar_init(&in_full[i], C::XIN ? 1 : 2);  // the copies
+            mbar_init(&in_empty[i], 4);              // the four warps of the block's warpgroup
         }
         for (int j = 0; j < 2; ++j) {
             mbar_init(&a_full[j], 4);
             mbar_init(&done[j], 1);
         }
+        mbar_init(x_made, 8);
         *abort_flag = 0;
         fence_barrier_init();
         for (int p = 0; p < min(np, C::NS); ++p) copy_weights(p);
-    } else if (w == 11 && lane == 0) {
-        tma_prefetch_desc(&xmap);
+    } else if (w == 11) {
+        if (C::XIN && lane < C::ROWS) row_top[lane] = 0;
+        if (!C::XIN && lane == 0) tma_prefetch_desc(&xmap);
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    // the ranks' shared memory may be written from here on (waited for below)
+    if (a.S > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
 
     const int wg = w < 8 ? w >> 2 : w & 1;  // the warpgroup a channel or MMA warp belongs to
@@ -443,9 +544,39 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
     float acc[C::ROWS] = {};
     const int ch = threadIdx.x & 127;
     if (w < 8) {
+        if constexpr (C::XIN) {
+            // terms of rows x [128 p0, 128 (p0 + np)), relative to the largest
+            // magnitude in that part of the row
+            int r = 0, p = w;
+#pragma unroll
+            for (int h = 0; h < HELD; ++h, p += 8) {
+                while (p >= np) p -= np, ++r;
+                if (r >= rows) break;
+                const uint32_t top = __reduce_max_sync(~0u, xv[h].top());
+                if (lane == 0) atomicMax(&row_top[r], top);
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            r = 0, p = w;
+#pragma unroll
+            for (int h = 0; h < HELD; ++h, p += 8) {
+                while (p >= np) p -= np, ++r;
+                if (r >= rows) break;
+                uint32_t t[TN];
+                terms4(xv[h], rho_exponent(row_top[r]), t);
+#pragma unroll
+                for (int j = 0; j < TN; ++j) {
+                    const int col = r * TN + j;  // a 128-byte row of the swizzled tile
+                    *reinterpret_cast<uint32_t*>(xres + p * C::XB + col * 128 +
+                                                 (((lane >> 2) ^ (col & 7)) << 4) + (lane & 3) * 4) = t[j];
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(x_made);
+        }
         const uint32_t quarter = static_cast<uint32_t>(32 * (w & 3)) << 16;
-        // RB rows' terms at a time, whole 8-column loads
-        constexpr int RB = TERMS == kTermsF32 ? 2 : COLS == 16 ? 5 : 8, CB = (RB * TERMS + 7) / 8 * 8;
+        // RB rows at a time, whole 8-column loads
+        constexpr int RB = 16 / TN < C::ROWS ? 16 / TN : C::ROWS, CB = (RB * TN + 7) / 8 * 8;
         auto take = [&](int u, const float (&s)[C::SUB]) {  // unit u's sums, scaled
 #pragma unroll
             for (int j = 0; j < C::SUB; ++j)
@@ -453,16 +584,16 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
                 for (int r0 = 0; r0 < C::ROWS; r0 += RB) {
                     if (r0 >= rows) continue;
                     uint32_t r[CB];
-                    const uint32_t at = td + quarter + (u % C::ND * C::SUB + j) * COLS + r0 * TERMS;
+                    const uint32_t at = td + quarter + (u % C::ND * C::SUB + j) * COLS + r0 * TN;
 #pragma unroll
                     for (int c = 0; c < CB; c += 8) tc_ld_32x32b_x8(at + c, *reinterpret_cast<uint32_t(*)[8]>(r + c));
                     tc_wait_ld();
 #pragma unroll
                     for (int i = 0; i < RB; ++i) {
                         if (r0 + i >= C::ROWS) continue;
-                        float v = __uint_as_float(r[i * TERMS]);
+                        float v = __uint_as_float(r[i * TN]);
 #pragma unroll
-                        for (int t = 1; t < TERMS; ++t) v += __uint_as_float(r[i * TERMS + t]);
+                        for (int t = 1; t < TN; ++t) v += __uint_as_float(r[i * TN + t]);
                         acc[r0 + i] = fmaf(s[j], v, acc[r0 + i]);
                     }
                 }
@@ -472,7 +603,7 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
         int u = 0;  // units of this warpgroup so far
         bool ok = true;
         for (int p = wg; ok && p < np; p += 2) {
-            const uint8_t* st = ring + p % C::NS * C::STAGE + C::XB;
+            const uint8_t* st = ring + p % C::NS * C::STAGE;
             if (!(ok = wait(&in_full[p % C::NS], p / C::NS))) break;
             float s[C::FULL];
 #pragma unroll
@@ -520,12 +651,13 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
             take(u - 1, s_prev);
         }
     } else if (w < 10) {
-        const uint32_t idesc = idesc_e4m3_e5m2_f32(128, static_cast<uint32_t>((rows * TERMS + 15) & ~15));
+        const uint32_t idesc = idesc_e4m3_e5m2_f32(128, static_cast<uint32_t>((rows * TN + 15) & ~15));
         int u = 0;
-        bool ok = true;
+        bool ok = !C::XIN || wait(x_made, 0);
         for (int p = wg; ok && p < np; p += 2) {
-            if (!(ok = wait(&in_full[p % C::NS], p / C::NS))) break;
-            const uint64_t bd = smem_desc_sw128(smem_u32(ring + p % C::NS * C::STAGE));
+            if (!C::XIN && !(ok = wait(&in_full[p % C::NS], p / C::NS))) break;
+            const uint64_t bd = smem_desc_sw128(
+                smem_u32(C::XIN ? xres + p * C::XB : ring + p % C::NS * C::STAGE + C::STAGE - C::XB));
 #pragma unroll
             for (int j = 0; j < 128 / C::UK; ++j) {
                 if (!(ok = wait(&a_full[wg], u))) break;
@@ -533,13 +665,16 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
                 const uint32_t d = td + static_cast<uint32_t>(u % C::ND * C::SUB * COLS);
 #pragma unroll
                 for (int m = 0; m < C::UK / 32; ++m)
-                    tc_mma_f8_ts_elect(d + 32 * m / GS * COLS, ta + 8 * m, bd + 2 * (j * (C::UK / 32) + m), idesc,
-                                       32 * m % GS ? 1u : 0u);
+#pragma unroll
+                    for (int t = 0; t < TK; ++t)
+                        tc_mma_f8_ts_elect(d + 32 * m / GS * COLS, ta + 8 * m,
+                                           bd + t * (COLS * 8) + 2 * (j * (C::UK / 32) + m), idesc,
+                                           32 * m % GS || t ? 1u : 0u);
                 tc_commit_elect(&done[wg]);
                 ++u;
             }
         }
-    } else if (lane == 0) {
+    } else if (lane == 0 && (w == 10 || !C::XIN)) {
         const bool weights = w == 10;
         if (!weights) asm volatile("griddepcontrol.wait;" ::: "memory");  // x is the terms kernel's
         int p = weights ? min(np, C::NS) : 0;
@@ -551,7 +686,8 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
                 copy_weights(p);
             } else {
                 mbar_arrive_expect_tx(full, C::XB);
-                tma_load_2d(ring + p % C::NS * C::STAGE, &xmap, full, (p0 + p) * 128, static_cast<int>(m0 * TERMS));
+                tma_load_3d(ring + p % C::NS * C::STAGE + C::STAGE - C::XB, &xmap, full, (p0 + p) * 128,
+                            static_cast<int>(m0 * TN), 0);
             }
         }
         if (*abort_flag)  // a failed call leaves no copy in flight behind (bounded as well)
@@ -566,29 +702,47 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
     __syncthreads();
     tc_fence_after();
     if (w == 9) tmem_dealloc(tmem, 2 * C::TW);
-    for (int j = 0; j < 2; ++j) {  // the warpgroups' sums
-        if (w < 8 && wg == j)
+    float* fin = reinterpret_cast<float*>(ring);  // [ROWS][128]: the second warpgroup's sums
+    if (w >= 4 && w < 8)
 #pragma unroll
-            for (int c = 0; c < C::ROWS; ++c)
-                if (c < rows) fin[c * C::LD + ch] = j ? fin[c * C::LD + ch] + acc[c] : acc[c];
+        for (int c = 0; c < C::ROWS; ++c)
+            if (c < rows) fin[c * 128 + ch] = acc[c];
+    __syncthreads();
+    if (a.S > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    const int share = (rows * 128 + a.S - 1) / a.S;  // outputs that a rank writes
+    if (w < 4)
+#pragma unroll
+        for (int c = 0; c < C::ROWS; ++c) {
+            if (c >= rows) continue;
+            float v = acc[c] + fin[c * 128 + ch];
+            if (C::XIN) v *= unscale_of(row_top[c]);
+            const int i = c * 128 + ch, to = i / share;
+            const float* p = recv + ks * share + i - to * share;
+            if (to == ks)
+                recv[ks * share + i - to * share] = v;
+            else
+                st_cluster(p, to, v);
+        }
+    if (a.S > 1)
+        cluster_sync();
+    else
         __syncthreads();
-    }
-    if (a.S > 1) cluster_sync();
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // unscale is the terms kernel's
-    for (int i = ks * kQ4Threads + threadIdx.x; i < rows * 128; i += a.S * kQ4Threads) {
-        const int r = i >> 7, c = i & 127;
-        const float* p = fin + r * C::LD + c;
+    if (!C::XIN) asm volatile("griddepcontrol.wait;" ::: "memory");  // unscale is the terms kernel's
+    for (int j = threadIdx.x; j < share; j += kQ4Threads) {
+        const int i = ks * share + j, r = i >> 7;
+        if (r >= rows) break;
         float v = 0.0f;
-        for (int s = 0; s < a.S; ++s) v += s == ks ? *p : ld_cluster(p, s);
-        if (tile * 128 + c < a.N) store_out(a, m0 + r, tile * 128 + c, v * a.unscale[m0 + r]);
+        for (int s = 0; s < a.S; ++s) v += recv[s * share + j];
+        if (!C::XIN) v *= a.unscale[m0 + r];
+        const int64_t n = tile * 128ll + (i & 127);
+        if (n < a.N) store_out(a, m0 + r, n, v);
     }
-    if (a.S > 1) cluster_sync();  // the sums stay until every rank has read them
 }
 
-template <int COLS, int GS, int TERMS>
+template <typename XT, int COLS, int GS, int TN, int TK>
 aem_status launch_q4(const CUtensorMap& xmap, const Q4Args& a, dim3 grid, cudaStream_t s) {
-    using C = Q4Cfg<COLS, GS, TERMS>;
-    auto kern = q4_kernel<COLS, GS, TERMS>;
+    using C = Q4Cfg<COLS, GS, TN, TK>;
+    auto kern = q4_kernel<XT, COLS, GS, TN, TK>;
     static std::atomic<uint64_t> ready{0};  // bit per device: the shared memory opt-in is done
     const uint64_t bit = 1ull << (current_device() & 63);
     if (!(ready.load(std::memory_order_relaxed) & bit)) {
@@ -601,103 +755,139 @@ aem_status launch_q4(const CUtensorMap& xmap, const Q4Args& a, dim3 grid, cudaSt
     cfg.dynamicSmemBytes = C::SMEM;
     cfg.stream = s;
     cudaLaunchAttribute at[2] = {};
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // starts under the terms kernel
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = a.S;
-    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    int n = 0;
+    if (!C::XIN) {  // starts under the terms kernel
+        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (a.S > 1) {
+        at[n].id = cudaLaunchAttributeClusterDimension;
+        at[n].val.clusterDim.x = a.S;
+        at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+        ++n;
+    }
     cfg.attrs = at;
-    cfg.numAttrs = a.S > 1 ? 2 : 1;
+    cfg.numAttrs = n;
     AEM_TRY_CUDA(cudaLaunchKernelEx(&cfg, kern, xmap, a));
     count_launches(1);
     return AEM_OK;
 }
 
-template <int COLS, int TERMS>
-aem_status launch_cols(const uint8_t* x, Q4Args a, int gs, int64_t slots, cudaStream_t s) {
-    CUtensorMap xmap;
-    AEM_TRY(make_tmap_2d(&xmap, x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.NP * 128, a.M * TERMS, 128, COLS,
-                         CU_TENSOR_MAP_SWIZZLE_128B));
-    // K is split until the CTAs fill the SMs: waves x (a CTA's own latency, as
-    // long as about 8 blocks, and its blocks)
-    const int64_t ctas = a.NC * slots, fit = 148 * 2;
-    int64_t best = INT64_MAX;
-    for (int S = 1; S <= 8 && S <= std::max<int64_t>(1, a.NP / 2); ++S) {
-        const int64_t cost = (ctas * S + fit - 1) / fit * (8 + (a.NP + S - 1) / S);
-        if (cost < best) {
-            best = cost;
-            a.S = S;
+// CTAs (at most 8, one cluster) that split K: until they fill the SMs, by
+// waves x (a CTA's own latency, as long as about 8 blocks, and its blocks).
+int split_k(int64_t ctas, int64_t blocks, int64_t most_blocks) {
+    int best = 8;
+    int64_t least = INT64_MAX;
+    for (int S = 1; S <= 8; ++S) {
+        const int64_t each = (blocks + S - 1) / S;
+        if (each > most_blocks || (S > 1 && each < 2)) continue;
+        const int64_t cost = (ctas * S + 295) / 296 * (8 + each);
+        if (cost < least) {
+            least = cost;
+            best = S;
         }
     }
+    return best;
+}
+
+template <typename XT, int COLS, int TN, int TK>
+aem_status launch_tile(const uint8_t* terms, Q4Args a, int gs, int64_t slots, cudaStream_t s) {
+    CUtensorMap xmap{};
+    constexpr bool XIN = TK == 1;
+    const int64_t KP = a.NP * 128ll;
+    if (!XIN)
+        AEM_TRY(make_tmap_3d_u8(&xmap, terms, KP, a.M * TN, TK, KP, a.M * TN * KP, COLS, TK));
+    a.S = split_k(a.NC * slots, a.NP, XIN ? Q4Cfg<COLS, 128, TN, TK>::MAXP : INT64_MAX);
     const dim3 grid(static_cast<unsigned>(a.NC * a.S), static_cast<unsigned>(slots));
-    if (gs == 128) return launch_q4<COLS, 128, TERMS>(xmap, a, grid, s);
-    if (gs == 64) return launch_q4<COLS, 64, TERMS>(xmap, a, grid, s);
-    if constexpr (COLS <= 48)  // the largest row tile has no room for groups of 32
-        return launch_q4<COLS, 32, TERMS>(xmap, a, grid, s);
-    set_error("q4 product: no such row tile");
+    if (gs == 128) return launch_q4<XT, COLS, 128, TN, TK>(xmap, a, grid, s);
+    if (gs == 64) return launch_q4<XT, COLS, 64, TN, TK>(xmap, a, grid, s);
+    if constexpr (TK < 8) return launch_q4<XT, COLS, 32, TN, TK>(xmap, a, grid, s);
+    set_error("q4 product: no such row tile");  // eight terms and 32-k scales do not fit a ring of four
     return AEM_EINVAL;
 }
 
-size_t q4_workspace(const Q4Weight* w, int terms, int64_t M) {
-    return static_cast<size_t>(M) * terms * w->NP * 128 + static_cast<size_t>(M) * 4;
+// Rows of a tile: as many as the call (grouped: an average group) has; few
+// rows put their terms side by side in the 16 columns of the narrowest MMA.
+struct Q4Plan {
+    bool few;
+    int rows;
+};
+Q4Plan q4_plan(const Q4Weight* w, bool f32, int64_t M, bool grouped) {
+    const int64_t groups = std::min<int64_t>(w->G, M);
+    const int64_t want = grouped ? (M + groups - 1) / groups : M;
+    Q4Plan p;
+    p.few = want <= (f32 ? 2 : 5) && w->NP <= 8 * Q4Cfg<16, 128, 3, 1>::MAXP;
+    if (f32)
+        p.rows = p.few ? 2 : want <= 4 ? 4 : want <= 8 || w->gs == 32 ? 8 : 16;
+    else
+        p.rows = p.few ? 5 : want <= 16 ? 16 : 32;
+    return p;
+}
+size_t q4_workspace(const Q4Weight* w, bool f32, int64_t M, bool grouped) {
+    if (q4_plan(w, f32, M, grouped).few) return 0;
+    return static_cast<size_t>(M) * ((f32 ? kTerms<float> : kTerms<__nv_bfloat16>) * w->NP * 128 + 4);
 }
 
 // x: the caller's rows.
-template <typename XT, int TERMS>
-aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, const XT* x, int64_t ldx,
-                      void* workspace, size_t workspace_bytes, cudaStream_t s) {
+template <typename XT>
+aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, const XT* x, void* workspace,
+                      size_t workspace_bytes, cudaStream_t s) {
+    constexpr bool F32 = sizeof(XT) == 4;
     AEM_REQUIRE(current_device() == w->device, "%s: the weights are on device %d, the current one is %d",
                 what, w->device, current_device());
     a.w = w->data;
     a.block = w->block;
     a.scale_bf16 = w->scale_bf16;
     a.N = w->N;
-    a.NC = w->NC;
-    a.NP = w->NP;
+    a.K = w->K;
+    a.NC = static_cast<int>(w->NC);
+    a.NP = static_cast<int>(w->NP);
+    a.x = x;
     a.err = device_error_word(w->device);
-    AEM_REQUIRE(a.M * TERMS < (1ll << 31), "%s: M=%lld out of range", what, (long long)a.M);
-    // columns of a row tile: as many as the rows (grouped: an average group's) need
-    const int64_t groups = std::min<int64_t>(a.G, a.M);
-    const int64_t want = a.group_rows ? (a.M + groups - 1) / groups : a.M;
-    const int cols = want <= 16 / TERMS ? 16 : want <= 48 / TERMS || w->gs == 32 ? 48 : 96;
-    a.rows = cols / TERMS;
-    const int64_t slots = a.group_rows ? groups + a.M / a.rows : (a.M + a.rows - 1) / a.rows;
-    AEM_REQUIRE(slots <= 65535, "%s: M=%lld rows are too many for one call", what, (long long)a.M);
-    const size_t need = q4_workspace(w, TERMS, a.M);
+    a.vec = reinterpret_cast<uintptr_t>(x) % (4 * sizeof(XT)) == 0 && a.ldx % 4 == 0;
+    AEM_REQUIRE(a.M * kTerms<XT> < (1ll << 31), "%s: M=%lld out of range", what, (long long)a.M);
+    const Q4Plan plan = q4_plan(w, F32, a.M, a.group_rows != nullptr);
+    const size_t need = q4_workspace(w, F32, a.M, a.group_rows != nullptr);
     AEM_REQUIRE(!workspace || (workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
                 "%s: workspace of %zu bytes (%zu needed, 16-byte aligned)", what, workspace_bytes, need);
+    a.rows = plan.rows;
+    const int64_t slots =
+        a.group_rows ? std::min<int64_t>(a.G, a.M) + a.M / a.rows : (a.M + a.rows - 1) / a.rows;
+    AEM_REQUIRE(slots <= 65535, "%s: M=%lld rows are too many for one call", what, (long long)a.M);
+    if (plan.few) return launch_tile<XT, 16, F32 ? 8 : 3, 1>(nullptr, a, w->gs, slots, s);
     void* own = nullptr;
     if (!workspace) {
         AEM_TRY_CUDA(cudaMallocAsync(&own, need, s));
         workspace = own;
     }
     auto* terms = static_cast<uint8_t*>(workspace);
-    auto* unscale = reinterpret_cast<float*>(terms + static_cast<size_t>(a.M) * TERMS * w->NP * 128);
+    auto* unscale = reinterpret_cast<float*>(terms + static_cast<size_t>(a.M) * kTerms<XT> * w->NP * 128);
     a.unscale = unscale;
-    const bool vec = reinterpret_cast<uintptr_t>(x) % (4 * sizeof(XT)) == 0 && ldx % 4 == 0;
-    q4_terms_kernel<XT, TERMS><<<static_cast<unsigned>(a.M), 512, 0, s>>>(x, ldx, w->K, w->NP * 128, vec, terms,
-                                                                          unscale);
+    const int tn = F32 ? 16 / a.rows : 1;
+    q4_terms_kernel<XT><<<static_cast<unsigned>(a.M), 1024, 0, s>>>(x, a.ldx, w->K, w->NP * 128, tn, a.vec, terms,
+                                                                    unscale);
     count_launches(1);
     const cudaError_t e = cudaGetLastError();
     aem_status st;
     if (e != cudaSuccess) {
         set_error("%s: launch failed: %s", what, cudaGetErrorString(e));
         st = AEM_ECUDA;
+    } else if constexpr (F32) {
+        st = tn == 4   ? launch_tile<XT, 16, 4, 2>(terms, a, w->gs, slots, s)
+             : tn == 2 ? launch_tile<XT, 16, 2, 4>(terms, a, w->gs, slots, s)
+                       : launch_tile<XT, 16, 1, 8>(terms, a, w->gs, slots, s);
     } else {
-        st = cols == 16   ? launch_cols<16, TERMS>(terms, a, w->gs, slots, s)
-             : cols == 48 ? launch_cols<48, TERMS>(terms, a, w->gs, slots, s)
-                          : launch_cols<96, TERMS>(terms, a, w->gs, slots, s);
+        st = a.rows == 16 ? launch_tile<XT, 16, 1, 3>(terms, a, w->gs, slots, s)
+                          : launch_tile<XT, 32, 1, 3>(terms, a, w->gs, slots, s);
     }
     if (own) cudaFreeAsync(own, s);
     return st;
 }
 
 aem_status q4_any(const Q4Weight* w, const char* what, const Q4Args& a, const void* x, aem_dtype xd,
-                  int64_t ldx, void* workspace, size_t bytes, cudaStream_t s) {
-    if (xd == AEM_F32)
-        return q4_product<float, kTermsF32>(w, what, a, static_cast<const float*>(x), ldx, workspace, bytes, s);
-    return q4_product<__nv_bfloat16, kTermsBf16>(w, what, a, static_cast<const __nv_bfloat16*>(x), ldx, workspace,
-                                                 bytes, s);
+                  void* workspace, size_t bytes, cudaStream_t s) {
+    if (xd == AEM_F32) return q4_product(w, what, a, static_cast<const float*>(x), workspace, bytes, s);
+    return q4_product(w, what, a, static_cast<const __nv_bfloat16*>(x), workspace, bytes, s);
 }
 
 bool is_dtype(aem_dtype t) { return t == AEM_F32 || t == AEM_BF16; }
@@ -728,7 +918,7 @@ void free_q4(Q4Weight* w) {
 aem_status check_q4_shape(const char* what, int64_t G, int64_t K, int64_t N, int gs, aem_dtype sd) {
     AEM_REQUIRE(G >= 1 && K >= 1 && N >= 1, "%s: G=%lld K=%lld N=%lld must be >= 1", what,
                 (long long)G, (long long)K, (long long)N);
-    AEM_REQUIRE(K < (1ll << 31) && N < (1ll << 31) && G < (1ll << 31) && G * N < (1ll << 40),
+    AEM_REQUIRE(K < (1ll << 30) && N < (1ll << 30) && G < (1ll << 31) && G * N < (1ll << 40),
                 "%s: dimensions out of range", what);
     AEM_REQUIRE(is_group(gs), "%s: group_size=%d is not 32, 64 or 128", what, gs);
     AEM_REQUIRE(is_dtype(sd), "%s: bad scale dtype", what);
@@ -882,9 +1072,9 @@ aem_status aem_q4weight_shape(aem_q4weight_t wh, int64_t* G, int64_t* K, int64_t
     return AEM_OK;
 }
 
-size_t aem_q4gemm_workspace(aem_q4weight_t wh, aem_dtype x_dtype, int64_t M) {
+size_t aem_q4gemm_workspace(aem_q4weight_t wh, aem_dtype x_dtype, int64_t M, int grouped) {
     if (!wh || M < 1 || !aem::is_dtype(x_dtype)) return 0;
-    return aem::q4_workspace(reinterpret_cast<aem::Q4Weight*>(wh), x_dtype == AEM_F32 ? aem::kTermsF32 : aem::kTermsBf16, M);
+    return aem::q4_workspace(reinterpret_cast<aem::Q4Weight*>(wh), x_dtype == AEM_F32, M, grouped != 0);
 }
 
 aem_status aem_q4gemm(aem_q4weight_t wh, int64_t group, const void* x, aem_dtype x_dtype,
@@ -900,13 +1090,14 @@ aem_status aem_q4gemm(aem_q4weight_t wh, int64_t group, const void* x, aem_dtype
     if (M == 0) return AEM_OK;
     AEM_REQUIRE(x && out, "aem_q4gemm: NULL buffer");
     aem::Q4Args a{};
+    a.ldx = ldx;
     a.out = out;
     a.ldo = ldo;
     a.M = M;
     a.group = group;
     a.G = 1;
     a.out_bf16 = out_dtype == AEM_BF16;
-    return aem::q4_any(w, "aem_q4gemm", a, x, x_dtype, ldx, workspace, workspace_bytes,
+    return aem::q4_any(w, "aem_q4gemm", a, x, x_dtype, workspace, workspace_bytes,
                            static_cast<cudaStream_t>(stream));
 }
 
@@ -924,6 +1115,7 @@ aem_status aem_grouped_q4gemm(aem_q4weight_t wh, const int32_t* group_rows, cons
     if (M == 0) return AEM_OK;
     AEM_REQUIRE(group_rows && x && out, "aem_grouped_q4gemm: NULL buffer");
     aem::Q4Args a{};
+    a.ldx = ldx;
     a.out = out;
     a.ldo = ldo;
     a.M = M;
@@ -931,7 +1123,7 @@ aem_status aem_grouped_q4gemm(aem_q4weight_t wh, const int32_t* group_rows, cons
     a.G = static_cast<int>(w->G);
     a.out_bf16 = out_dtype == AEM_BF16;
     a.relu = relu != 0;
-    return aem::q4_any(w, "aem_grouped_q4gemm", a, x, x_dtype, ldx, workspace, workspace_bytes,
+    return aem::q4_any(w, "aem_grouped_q4gemm", a, x, x_dtype, workspace, workspace_bytes,
                            static_cast<cudaStream_t>(stream));
 }
 

@@ -135,23 +135,25 @@ aem_status check_device_errors(cudaStream_t stream, const char* what) {
     return AEM_EDEVICE;
 }
 
+static aem_status tmap_encoder() {
+    std::lock_guard<std::mutex> lk(g_dev_mutex);
+    if (!g_encode) {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
+        if (e != cudaSuccess || q != cudaDriverEntryPointSuccess || !fn) {
+            set_error("cuTensorMapEncodeTiled unavailable");
+            return AEM_EUNSUPPORTED;
+        }
+        g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    }
+    return AEM_OK;
+}
+
 aem_status make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype,
                         int elem_bytes, uint64_t cols, uint64_t rows, uint32_t box_cols,
                         uint32_t box_rows, CUtensorMapSwizzle swizzle) {
-    {
-        std::lock_guard<std::mutex> lk(g_dev_mutex);
-        if (!g_encode) {
-            void* fn = nullptr;
-            cudaDriverEntryPointQueryResult q;
-            cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn,
-                                                    cudaEnableDefault, &q);
-            if (e != cudaSuccess || q != cudaDriverEntryPointSuccess || !fn) {
-                set_error("cuTensorMapEncodeTiled unavailable");
-                return AEM_EUNSUPPORTED;
-            }
-            g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
-        }
-    }
+    AEM_TRY(tmap_encoder());
     AEM_REQUIRE((reinterpret_cast<uintptr_t>(base) & 15) == 0,
                 "TMA base address must be 16-byte aligned");
     AEM_REQUIRE((cols * elem_bytes) % 16 == 0, "TMA row stride must be a multiple of 16 bytes");
@@ -165,6 +167,26 @@ aem_status make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType 
     if (r != CUDA_SUCCESS) {
         set_error("cuTensorMapEncodeTiled failed (%d): cols=%llu rows=%llu box=%ux%u", (int)r,
                   (unsigned long long)cols, (unsigned long long)rows, box_cols, box_rows);
+        return AEM_ECUDA;
+    }
+    return AEM_OK;
+}
+
+aem_status make_tmap_3d_u8(CUtensorMap* map, const void* base, uint64_t dim0, uint64_t dim1, uint64_t dim2,
+                           uint64_t row_bytes, uint64_t plane_bytes, uint32_t box1, uint32_t box2) {
+    AEM_TRY(tmap_encoder());
+    AEM_REQUIRE((reinterpret_cast<uintptr_t>(base) & 15) == 0 && row_bytes % 16 == 0 && plane_bytes % 16 == 0,
+                "TMA base address and strides must be multiples of 16 bytes");
+    cuuint64_t dims[3] = {dim0, dim1, dim2};
+    cuuint64_t strides[2] = {row_bytes, plane_bytes};
+    cuuint32_t box[3] = {128, box1, box2};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("cuTensorMapEncodeTiled failed (%d): %llu x %llu x %llu", (int)r, (unsigned long long)dim0,
+                  (unsigned long long)dim1, (unsigned long long)dim2);
         return AEM_ECUDA;
     }
     return AEM_OK;

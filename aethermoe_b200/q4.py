@@ -109,9 +109,13 @@ def _check_weight(w, device):
         raise ValueError(f"x is on {device}, the weight on cuda:{w.device}")
 
 
-def _scratch(x, w):
-    n = _lib.lib().aem_q4gemm_workspace(w.handle, _DT[x.dtype], x.shape[0])
-    return torch.empty(max(n, 1), dtype=torch.uint8, device=x.device), n
+def _scratch(x, w, grouped):
+    """``(pointer, bytes, tensor)`` of a product's scratch."""
+    n = _lib.lib().aem_q4gemm_workspace(w.handle, _DT[x.dtype], x.shape[0], grouped)
+    if not n:
+        return None, 0, None
+    t = torch.empty(n, dtype=torch.uint8, device=x.device)
+    return t.data_ptr(), n, t
 
 
 def _matmul(x, w, group, out_dtype, out, s):
@@ -119,9 +123,9 @@ def _matmul(x, w, group, out_dtype, out, s):
     _check_weight(w, x.device)
     m = x.shape[0]
     out, ldo = _output(out, (m, w.N), out_dtype or (x.dtype if out is None else out.dtype), x.device)
-    ws, n = _scratch(x, w)
+    ws, n, keep = _scratch(x, w, 0)
     _lib.check(_lib.lib().aem_q4gemm(w.handle, group, x.data_ptr(), _DT[x.dtype], ldx, m,
-                                     out.data_ptr(), _DT[out.dtype], ldo, ws.data_ptr(), n, s), "aem_q4gemm")
+                                     out.data_ptr(), _DT[out.dtype], ldo, ws, n, s), "aem_q4gemm")
     return out
 
 
@@ -132,10 +136,10 @@ def _grouped(x, w, starts, relu, out_dtype, out, s):
         raise ValueError(f"starts must be {w.G + 1} contiguous int32 offsets")
     m = x.shape[0]
     out, ldo = _output(out, (m, w.N), out_dtype or (x.dtype if out is None else out.dtype), x.device)
-    ws, n = _scratch(x, w)
+    ws, n, keep = _scratch(x, w, 1)
     _lib.check(_lib.lib().aem_grouped_q4gemm(w.handle, starts.data_ptr(), x.data_ptr(), _DT[x.dtype],
                                              ldx, m, out.data_ptr(), _DT[out.dtype], ldo,
-                                             1 if relu else 0, ws.data_ptr(), n, s), "aem_grouped_q4gemm")
+                                             1 if relu else 0, ws, n, s), "aem_grouped_q4gemm")
     return out
 
 

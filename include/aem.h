@@ -366,8 +366,8 @@ aem_status aem_q4weight_free(aem_q4weight_t w);
 aem_status aem_q4weight_shape(aem_q4weight_t w, int64_t* G, int64_t* K, int64_t* N, int* group_size);
 
 /* out[M, N] = x[M, K] @ (q[group] * scale[group]) for the few rows of a
- * decoding step: one pass over the weights for up to 32 bf16 or 12 float32
- * rows (16 or 6 with groups of 32), one more for every further such tile.
+ * decoding step: one pass over the weights for up to 32 bf16 or 16 float32
+ * rows (8 with groups of 32), one more for every further such tile.
  * The integers are exact in the MMAs' operands, each scale multiplies a
  * float32 sum, and x takes part in full: what is cut from an element is
  * under 2^-30 of its row's largest finite magnitude (nothing for bf16
@@ -375,10 +375,10 @@ aem_status aem_q4weight_shape(aem_q4weight_t w, int64_t* G, int64_t* K, int64_t*
  * float32 sums.  Infinities and NaN act as in x @ w.  Rows of x are ldx
  * elements apart, rows of out ldo; any alignment works.  The workspace holds
  * x in the products' form: device scratch of aem_q4gemm_workspace(w,
- * x_dtype, M) bytes, 16-byte aligned, or NULL to have the call allocate and
- * free it in stream order.  The weights' device must be the current one.
+ * x_dtype, M, 0) bytes (0 for the fewest rows), 16-byte aligned, or NULL to
+ * have the call allocate and free it in stream order.  The weights' device must be the current one.
  * Results repeat bit for bit. */
-size_t aem_q4gemm_workspace(aem_q4weight_t w, aem_dtype x_dtype, int64_t M);
+size_t aem_q4gemm_workspace(aem_q4weight_t w, aem_dtype x_dtype, int64_t M, int grouped);
 aem_status aem_q4gemm(aem_q4weight_t w, int64_t group, const void* x, aem_dtype x_dtype,
                       int64_t ldx, int64_t M, void* out, aem_dtype out_dtype, int64_t ldo,
                       void* workspace, size_t workspace_bytes, void* stream);
@@ -386,7 +386,7 @@ aem_status aem_q4gemm(aem_q4weight_t w, int64_t group, const void* x, aem_dtype 
  * [group_rows[g], group_rows[g+1]) of x (device int32 array of G+1 increasing
  * offsets: aem_dispatch's starts) times weight group g, for all G <=
  * AEM_MAX_EXPERTS groups of w, with out = relu(...) when relu != 0; workspace
- * as above.  Offsets are clamped to [0, M]; rows of out outside every group are not written. */
+ * as above (aem_q4gemm_workspace(w, x_dtype, M, 1)).  Offsets are clamped to [0, M]; rows of out outside every group are not written. */
 aem_status aem_grouped_q4gemm(aem_q4weight_t w, const int32_t* group_rows, const void* x,
                               aem_dtype x_dtype, int64_t ldx, int64_t M, void* out,
                               aem_dtype out_dtype, int64_t ldo, int relu, void* workspace,
