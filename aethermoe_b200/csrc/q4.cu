@@ -413,19 +413,22 @@ __device__ __forceinline__ void store_out(const Q4Args& a, int64_t m, int64_t n,
 // 1 (few rows) the CTA makes the terms of its part of K itself and keeps them
 // in shared memory; otherwise a terms kernel has made them and they come with
 // the ring.
-template <int COLS, int GS, int TN, int TK>
+template <int COLS, int GS, int ROWS, int TN, int TK>
 struct Q4Cfg {
-    static constexpr int ROWS = COLS / TN;
     static constexpr bool XIN = TK == 1;
     static constexpr int TW = 128;                     // TMEM columns of a warpgroup: 4 per SM
     static constexpr int FULL = GS == 128 ? 1 : 128 / GS;  // scale groups of a block
-    static constexpr int UK = FULL * COLS <= 96 ? 128 : 64;  // k of a unit
+    static constexpr int UK = 32 + 2 * FULL * COLS <= TW ? 128 : 64;  // k of a unit
     static constexpr int SUB = UK < GS ? 1 : UK / GS;  // accumulators per unit
     static constexpr int UA = UK / 4;                  // columns of a unit's weights
     static constexpr int ND = UA + 2 * SUB * COLS <= TW ? 2 : 1;  // accumulator buffers
     static constexpr int XB = TK * COLS * 128;         // activation bytes of a block
-    static constexpr int MAXP = 20;                    // XIN: blocks whose terms are kept
-    static constexpr int XRES = XIN ? MAXP * XB : 0;
+    // XIN: bytes between the blocks' terms.  A tile of at most 8 columns takes
+    // 1 KB; the MMA's other 8 columns, never read back, are then the next
+    // block's bytes
+    static constexpr int XSTEP = ROWS * TN <= 8 ? 1024 : XB;
+    static constexpr int MAXP = XSTEP == 1024 ? 32 : 24;  // XIN: blocks whose terms are kept
+    static constexpr int XRES = XIN ? MAXP * XSTEP : 0;
     static constexpr int STAGE = (XIN ? 0 : XB) + 8192 + (FULL * 512 + 1023) / 1024 * 1024;
     static constexpr int RECV = (ROWS * 128 + 8) * 4;  // the cluster's sums, S equal shares
     // an even ring: a stage always comes back to the warpgroup that saw its
@@ -436,7 +439,7 @@ struct Q4Cfg {
     // two CTAs on an SM, never three: no CTA ever waits for tensor memory
     static constexpr int SMEM = USED > 78 * 1024 ? USED : 78 * 1024;
     static_assert(UA + ND * SUB * COLS <= TW && NS >= 4 && SMEM <= 113 * 1024, "budgets");
-    static_assert(UK >= GS || UK == 128, "a scale group inside a unit");
+    static_assert(ROWS * TN <= COLS && (UK >= GS || UK == 128), "a scale group inside a unit");
     static_assert(STAGE * NS >= RECV, "a warpgroup's sums fit the ring");
 };
 constexpr int kQ4Threads = 12 * 32;
@@ -459,10 +462,10 @@ constexpr int kQ4Threads = 12 * 32;
 // The S CTAs of a cluster take parts of K: each sends its sums to the rank
 // that writes those outputs, which adds them in rank order.
 // Every wait is bounded; a timeout sets the error word and ends all roles.
-template <typename XT, int COLS, int GS, int TN, int TK>
+template <typename XT, int COLS, int GS, int ROWS, int TN, int TK>
 __global__ void __launch_bounds__(kQ4Threads, 2)
     q4_kernel(const __grid_constant__ CUtensorMap xmap, const Q4Args a) {
-    using C = Q4Cfg<COLS, GS, TN, TK>;
+    using C = Q4Cfg<COLS, GS, ROWS, TN, TK>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* xres = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                ~static_cast<uintptr_t>(1023));
@@ -486,7 +489,7 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
 
     // XIN: a warp takes 128 k of a row, a lane four of them.  These loads go out
     // ahead of the weights, behind which they would wait for microseconds.
-    constexpr int HELD = C::XIN ? (C::ROWS * C::MAXP + 7) / 8 : 1;
+    constexpr int HELD = C::XIN ? (ROWS * C::MAXP + 7) / 8 : 1;
     Four<XT> xv[HELD];
     if (C::XIN && w < 8) {
         const XT* x = static_cast<const XT*>(a.x) + m0 * a.ldx + static_cast<int64_t>(p0) * 128 + lane * 4;
@@ -523,7 +526,7 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
         fence_barrier_init();
         for (int p = 0; p < min(np, C::NS); ++p) copy_weights(p);
     } else if (w == 11) {
-        if (C::XIN && lane < C::ROWS) row_top[lane] = 0;
+        if (C::XIN && lane < ROWS) row_top[lane] = 0;
         if (!C::XIN && lane == 0) tma_prefetch_desc(&xmap);
     }
     tc_fence_before();
@@ -541,7 +544,7 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
         return __all_sync(~0u, mbar_wait_bounded(bar, phase & 1, abort_flag, a.err, ERR_GEMM_TIMEOUT)) != 0;
     };
 
-    float acc[C::ROWS] = {};
+    float acc[ROWS] = {};
     const int ch = threadIdx.x & 127;
     if (w < 8) {
         if constexpr (C::XIN) {
@@ -566,7 +569,7 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
 #pragma unroll
                 for (int j = 0; j < TN; ++j) {
                     const int col = r * TN + j;  // a 128-byte row of the swizzled tile
-                    *reinterpret_cast<uint32_t*>(xres + p * C::XB + col * 128 +
+                    *reinterpret_cast<uint32_t*>(xres + p * C::XSTEP + col * 128 +
                                                  (((lane >> 2) ^ (col & 7)) << 4) + (lane & 3) * 4) = t[j];
                 }
             }
@@ -575,28 +578,28 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
             if (lane == 0) mbar_arrive(x_made);
         }
         const uint32_t quarter = static_cast<uint32_t>(32 * (w & 3)) << 16;
-        // RB rows at a time, whole 8-column loads
-        constexpr int RB = 16 / TN < C::ROWS ? 16 / TN : C::ROWS, CB = (RB * TN + 7) / 8 * 8;
+        // columns taken back at once (the widest row tile's registers allow 16)
+        constexpr int TC = C::SUB * COLS, CH = COLS == 32 || TC == 16 ? 16 : 32;
         auto take = [&](int u, const float (&s)[C::SUB]) {  // unit u's sums, scaled
 #pragma unroll
-            for (int j = 0; j < C::SUB; ++j)
+            for (int c0 = 0; c0 < TC; c0 += CH) {
+                uint32_t r[CH];
+                const uint32_t at = td + quarter + u % C::ND * TC + c0;
+                if constexpr (CH == 16)
+                    tc_ld_32x32b_x16(at, r);
+                else
+                    tc_ld_32x32b_x32(at, r);
+                tc_wait_ld();
 #pragma unroll
-                for (int r0 = 0; r0 < C::ROWS; r0 += RB) {
-                    if (r0 >= rows) continue;
-                    uint32_t r[CB];
-                    const uint32_t at = td + quarter + (u % C::ND * C::SUB + j) * COLS + r0 * TN;
+                for (int i = 0; i < CH / 16 * (16 / TN); ++i) {  // 16 columns hold 16 / TN whole rows
+                    const int c = i / (16 / TN) * 16 + i % (16 / TN) * TN, row = (c0 + c) % COLS / TN;
+                    if (row >= ROWS) continue;
+                    float v = __uint_as_float(r[c]);
 #pragma unroll
-                    for (int c = 0; c < CB; c += 8) tc_ld_32x32b_x8(at + c, *reinterpret_cast<uint32_t(*)[8]>(r + c));
-                    tc_wait_ld();
-#pragma unroll
-                    for (int i = 0; i < RB; ++i) {
-                        if (r0 + i >= C::ROWS) continue;
-                        float v = __uint_as_float(r[i * TN]);
-#pragma unroll
-                        for (int t = 1; t < TN; ++t) v += __uint_as_float(r[i * TN + t]);
-                        acc[r0 + i] = fmaf(s[j], v, acc[r0 + i]);
-                    }
+                    for (int t = 1; t < TN; ++t) v += __uint_as_float(r[c + t]);
+                    acc[row] = fmaf(s[(c0 + c) / COLS], v, acc[row]);
                 }
+            }
             tc_fence_before();
         };
         float s_prev[C::SUB];
@@ -624,12 +627,16 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
                         v[8 * i + 2 * e + 1] = __funnelshift_r(word[e], word[e], 4) & 0x87878787u;
                     }
                 }
+                if (C::XIN && j == 128 / C::UK - 1) {  // the stage held weights only: it is free
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&in_empty[p % C::NS]);
+                }
                 if (u) {
                     // the unit before is done: its weights' columns, its
                     // accumulators and (at a block's start) its stage are free
                     if (!(ok = wait(&done[wg], u - 1))) break;
                     tc_fence_after();
-                    if (j == 0 && lane == 0) mbar_arrive(&in_empty[(p - 2) % C::NS]);
+                    if (!C::XIN && j == 0 && lane == 0) mbar_arrive(&in_empty[(p - 2) % C::NS]);
                     if (C::ND == 1) take(u - 1, s_prev);
                 }
                 if constexpr (C::UA == 32)
@@ -657,7 +664,7 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
         for (int p = wg; ok && p < np; p += 2) {
             if (!C::XIN && !(ok = wait(&in_full[p % C::NS], p / C::NS))) break;
             const uint64_t bd = smem_desc_sw128(
-                smem_u32(C::XIN ? xres + p * C::XB : ring + p % C::NS * C::STAGE + C::STAGE - C::XB));
+                smem_u32(C::XIN ? xres + p * C::XSTEP : ring + p % C::NS * C::STAGE + C::STAGE - C::XB));
 #pragma unroll
             for (int j = 0; j < 128 / C::UK; ++j) {
                 if (!(ok = wait(&a_full[wg], u))) break;
@@ -705,14 +712,14 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
     float* fin = reinterpret_cast<float*>(ring);  // [ROWS][128]: the second warpgroup's sums
     if (w >= 4 && w < 8)
 #pragma unroll
-        for (int c = 0; c < C::ROWS; ++c)
+        for (int c = 0; c < ROWS; ++c)
             if (c < rows) fin[c * 128 + ch] = acc[c];
     __syncthreads();
     if (a.S > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     const int share = (rows * 128 + a.S - 1) / a.S;  // outputs that a rank writes
     if (w < 4)
 #pragma unroll
-        for (int c = 0; c < C::ROWS; ++c) {
+        for (int c = 0; c < ROWS; ++c) {
             if (c >= rows) continue;
             float v = acc[c] + fin[c * 128 + ch];
             if (C::XIN) v *= unscale_of(row_top[c]);
@@ -739,10 +746,10 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
     }
 }
 
-template <typename XT, int COLS, int GS, int TN, int TK>
+template <typename XT, int COLS, int GS, int ROWS, int TN, int TK>
 aem_status launch_q4(const CUtensorMap& xmap, const Q4Args& a, dim3 grid, cudaStream_t s) {
-    using C = Q4Cfg<COLS, GS, TN, TK>;
-    auto kern = q4_kernel<XT, COLS, GS, TN, TK>;
+    using C = Q4Cfg<COLS, GS, ROWS, TN, TK>;
+    auto kern = q4_kernel<XT, COLS, GS, ROWS, TN, TK>;
     static std::atomic<uint64_t> ready{0};  // bit per device: the shared memory opt-in is done
     const uint64_t bit = 1ull << (current_device() & 63);
     if (!(ready.load(std::memory_order_relaxed) & bit)) {
@@ -774,14 +781,14 @@ aem_status launch_q4(const CUtensorMap& xmap, const Q4Args& a, dim3 grid, cudaSt
 }
 
 // CTAs (at most 8, one cluster) that split K: until they fill the SMs, by
-// waves x (a CTA's own latency, as long as about 8 blocks, and its blocks).
+// waves x (a CTA's set-up and end, as long as about 14 blocks, and its blocks).
 int split_k(int64_t ctas, int64_t blocks, int64_t most_blocks) {
     int best = 8;
     int64_t least = INT64_MAX;
     for (int S = 1; S <= 8; ++S) {
         const int64_t each = (blocks + S - 1) / S;
         if (each > most_blocks || (S > 1 && each < 2)) continue;
-        const int64_t cost = (ctas * S + 295) / 296 * (8 + each);
+        const int64_t cost = (ctas * S + 295) / 296 * (14 + each);
         if (cost < least) {
             least = cost;
             best = S;
@@ -790,18 +797,18 @@ int split_k(int64_t ctas, int64_t blocks, int64_t most_blocks) {
     return best;
 }
 
-template <typename XT, int COLS, int TN, int TK>
+template <typename XT, int COLS, int ROWS, int TN, int TK>
 aem_status launch_tile(const uint8_t* terms, Q4Args a, int gs, int64_t slots, cudaStream_t s) {
     CUtensorMap xmap{};
     constexpr bool XIN = TK == 1;
     const int64_t KP = a.NP * 128ll;
     if (!XIN)
         AEM_TRY(make_tmap_3d_u8(&xmap, terms, KP, a.M * TN, TK, KP, a.M * TN * KP, COLS, TK));
-    a.S = split_k(a.NC * slots, a.NP, XIN ? Q4Cfg<COLS, 128, TN, TK>::MAXP : INT64_MAX);
+    a.S = split_k(a.NC * slots, a.NP, XIN ? Q4Cfg<COLS, 128, ROWS, TN, TK>::MAXP : INT64_MAX);
     const dim3 grid(static_cast<unsigned>(a.NC * a.S), static_cast<unsigned>(slots));
-    if (gs == 128) return launch_q4<XT, COLS, 128, TN, TK>(xmap, a, grid, s);
-    if (gs == 64) return launch_q4<XT, COLS, 64, TN, TK>(xmap, a, grid, s);
-    if constexpr (TK < 8) return launch_q4<XT, COLS, 32, TN, TK>(xmap, a, grid, s);
+    if (gs == 128) return launch_q4<XT, COLS, 128, ROWS, TN, TK>(xmap, a, grid, s);
+    if (gs == 64) return launch_q4<XT, COLS, 64, ROWS, TN, TK>(xmap, a, grid, s);
+    if constexpr (TK < 8) return launch_q4<XT, COLS, 32, ROWS, TN, TK>(xmap, a, grid, s);
     set_error("q4 product: no such row tile");  // eight terms and 32-k scales do not fit a ring of four
     return AEM_EINVAL;
 }
@@ -816,11 +823,11 @@ Q4Plan q4_plan(const Q4Weight* w, bool f32, int64_t M, bool grouped) {
     const int64_t groups = std::min<int64_t>(w->G, M);
     const int64_t want = grouped ? (M + groups - 1) / groups : M;
     Q4Plan p;
-    p.few = want <= (f32 ? 2 : 5) && w->NP <= 8 * Q4Cfg<16, 128, 3, 1>::MAXP;
+    p.few = want <= (f32 ? 2 : 5) && w->NP <= 8 * 24;
     if (f32)
-        p.rows = p.few ? 2 : want <= 4 ? 4 : want <= 8 || w->gs == 32 ? 8 : 16;
+        p.rows = p.few ? (want <= 1 ? 1 : 2) : want <= 4 ? 4 : want <= 8 || w->gs == 32 ? 8 : 16;
     else
-        p.rows = p.few ? 5 : want <= 16 ? 16 : 32;
+        p.rows = p.few ? (want <= 2 ? 2 : 5) : want <= 16 ? 16 : 32;
     return p;
 }
 size_t q4_workspace(const Q4Weight* w, bool f32, int64_t M, bool grouped) {
@@ -851,10 +858,13 @@ aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, const XT* x
     AEM_REQUIRE(!workspace || (workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
                 "%s: workspace of %zu bytes (%zu needed, 16-byte aligned)", what, workspace_bytes, need);
     a.rows = plan.rows;
-    const int64_t slots =
-        a.group_rows ? std::min<int64_t>(a.G, a.M) + a.M / a.rows : (a.M + a.rows - 1) / a.rows;
+    // row tiles at most: n groups with rows have up to n + (M - n) / rows
+    const int64_t n = std::min<int64_t>(a.G, a.M);
+    const int64_t slots = a.group_rows ? n + (a.M - n) / a.rows : (a.M + a.rows - 1) / a.rows;
     AEM_REQUIRE(slots <= 65535, "%s: M=%lld rows are too many for one call", what, (long long)a.M);
-    if (plan.few) return launch_tile<XT, 16, F32 ? 8 : 3, 1>(nullptr, a, w->gs, slots, s);
+    if (plan.few)
+        return a.rows == (F32 ? 1 : 2) ? launch_tile<XT, 16, F32 ? 1 : 2, F32 ? 8 : 3, 1>(nullptr, a, w->gs, slots, s)
+                                       : launch_tile<XT, 16, F32 ? 2 : 5, F32 ? 8 : 3, 1>(nullptr, a, w->gs, slots, s);
     void* own = nullptr;
     if (!workspace) {
         AEM_TRY_CUDA(cudaMallocAsync(&own, need, s));
@@ -873,12 +883,12 @@ aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, const XT* x
         set_error("%s: launch failed: %s", what, cudaGetErrorString(e));
         st = AEM_ECUDA;
     } else if constexpr (F32) {
-        st = tn == 4   ? launch_tile<XT, 16, 4, 2>(terms, a, w->gs, slots, s)
-             : tn == 2 ? launch_tile<XT, 16, 2, 4>(terms, a, w->gs, slots, s)
-                       : launch_tile<XT, 16, 1, 8>(terms, a, w->gs, slots, s);
+        st = tn == 4   ? launch_tile<XT, 16, 4, 4, 2>(terms, a, w->gs, slots, s)
+             : tn == 2 ? launch_tile<XT, 16, 8, 2, 4>(terms, a, w->gs, slots, s)
+                       : launch_tile<XT, 16, 16, 1, 8>(terms, a, w->gs, slots, s);
     } else {
-        st = a.rows == 16 ? launch_tile<XT, 16, 1, 3>(terms, a, w->gs, slots, s)
-                          : launch_tile<XT, 32, 1, 3>(terms, a, w->gs, slots, s);
+        st = a.rows == 16 ? launch_tile<XT, 16, 16, 1, 3>(terms, a, w->gs, slots, s)
+                          : launch_tile<XT, 32, 32, 1, 3>(terms, a, w->gs, slots, s);
     }
     if (own) cudaFreeAsync(own, s);
     return st;
