@@ -18,6 +18,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "runtime.h"
@@ -139,7 +140,7 @@ struct MoveArgs {
 // taken from pair i0 in strides of `step`.  Each vector of x is read once and
 // stored k times.
 template <typename V>
-__device__ __forceinline__ void move_rows(const MoveArgs& m, int64_t t0, int nt, int i0, int step,
+__device__ __forceinline__ void move_flat(const MoveArgs& m, int64_t t0, int nt, int i0, int step,
                                           int k, const int* dest) {
     int t = i0 / m.cols, c = i0 % m.cols;
     const int dt = step / m.cols, dc = step % m.cols;
@@ -155,6 +156,39 @@ __device__ __forceinline__ void move_rows(const MoveArgs& m, int64_t t0, int nt,
         if (c >= m.cols) {
             c -= m.cols;
             ++t;
+        }
+    }
+}
+
+// The same for a block's own tokens: a warp per token, four vectors a lane in
+// flight, where a row has enough of them (short rows go flat).
+template <typename V>
+__device__ __forceinline__ void move_rows(const MoveArgs& m, int64_t t0, int nt, int k,
+                                          const int* dest) {
+    if (m.cols < 64) return move_flat<V>(m, t0, nt, threadIdx.x, kThreads, k, dest);
+    constexpr int U = 4;
+    const int lane = threadIdx.x & 31;
+    for (int t = threadIdx.x >> 5; t < nt; t += kWarps) {
+        const char* x = m.x + (t0 + t) * m.ldx + lane * sizeof(V);
+        int c = lane;
+        for (; c + 32 * (U - 1) < m.cols; c += 32 * U, x += 32 * U * sizeof(V)) {
+            V v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const V*>(x + u * 32 * sizeof(V));
+            for (int j = 0; j < k; ++j) {
+                const int r = dest[t * k + j];
+                if (r < 0) continue;
+                char* to = m.rows + r * m.ldr + static_cast<int64_t>(c) * sizeof(V);
+#pragma unroll
+                for (int u = 0; u < U; ++u) *reinterpret_cast<V*>(to + u * 32 * sizeof(V)) = v[u];
+            }
+        }
+        for (; c < m.cols; c += 32, x += 32 * sizeof(V)) {
+            const V v = *reinterpret_cast<const V*>(x);
+            for (int j = 0; j < k; ++j) {
+                const int r = dest[t * k + j];
+                if (r >= 0) *reinterpret_cast<V*>(m.rows + r * m.ldr + static_cast<int64_t>(c) * sizeof(V)) = v;
+            }
         }
     }
 }
@@ -201,7 +235,7 @@ __global__ void __launch_bounds__(kThreads)
         for (int r = total + threadIdx.x; r < n; r += kThreads) so.unit_of[r] = -1;
     if (!m.x) return;
     __syncthreads();
-    move_rows<V>(m, 0, n / ids.k, blockIdx.x * kThreads + threadIdx.x, gridDim.x * kThreads, ids.k,
+    move_flat<V>(m, 0, n / ids.k, blockIdx.x * kThreads + threadIdx.x, gridDim.x * kThreads, ids.k,
                  dest);
     zero_rows<V>(m, total, n);
 }
@@ -211,6 +245,7 @@ __global__ void __launch_bounds__(kThreads)
 // in totals[e]; (3) ranks inside the chunk, the order, and the moved rows.
 __global__ void __launch_bounds__(kThreads)
     sort_count_kernel(Ids ids, int64_t U, int tc, int C, int* counts, int* err) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     __shared__ int hist[AEM_MAX_EXPERTS];
     hist[threadIdx.x] = 0;
     __syncthreads();
@@ -225,6 +260,7 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 __global__ void __launch_bounds__(kThreads) sort_scan_kernel(int C, int* counts, int* totals) {
+    asm volatile("griddepcontrol.launch_dependents;\ngriddepcontrol.wait;" ::: "memory");
     __shared__ int ws[kWarps];
     int* c = counts + static_cast<int64_t>(blockIdx.x) * C;
     int carry = 0;
@@ -241,8 +277,8 @@ __global__ void __launch_bounds__(kThreads) sort_scan_kernel(int C, int* counts,
 
 template <typename V>
 __global__ void __launch_bounds__(kThreads)
-    sort_move_kernel(Ids ids, SortOut so, int tc, int C, const int* __restrict__ counts,
-                     const int* __restrict__ totals, MoveArgs m, int* err) {
+    sort_move_kernel(Ids ids, SortOut so, int tc, int C, const int* counts,
+                     const int* totals, MoveArgs m, int* err) {
     __shared__ SortSmem sm;
     __shared__ int dest[kBlockUnits];
     constexpr int ITERS = kBlockUnits / kThreads;
@@ -250,6 +286,7 @@ __global__ void __launch_bounds__(kThreads)
     const int64_t u0 = blockIdx.x * static_cast<int64_t>(tc) * ids.k;
     const int n = static_cast<int>(min(static_cast<int64_t>(tc) * ids.k, so.U - u0));
     const int iters = rank_units<ITERS>(ids, u0, n, sm, key, row, err, [&](int) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");  // the scan's sums
         const bool e = threadIdx.x < ids.E;
         const int s = block_scan(e ? totals[threadIdx.x] : 0, sm.warp_sums, &total);
         if (blockIdx.x == 0 && e) so.starts[threadIdx.x] = s;
@@ -269,7 +306,7 @@ __global__ void __launch_bounds__(kThreads)
         so.unit_of[r] = -1;
     if (!m.x) return;
     __syncthreads();
-    move_rows<V>(m, u0 / ids.k, n / ids.k, threadIdx.x, kThreads, ids.k, dest);
+    move_rows<V>(m, u0 / ids.k, n / ids.k, ids.k, dest);
     zero_rows<V>(m, total, so.U);
 }
 
@@ -290,49 +327,74 @@ __global__ void __launch_bounds__(kThreads)
         dest[i] = r;
     }
     __syncthreads();
-    move_rows<V>(m, t0, nt, threadIdx.x, kThreads, k, dest);
+    move_rows<V>(m, t0, nt, k, dest);
     zero_rows<V>(m, max(0, *total), U);
 }
 
 // ------------------------------------------------------------------ combine
+// VE = 8 consecutive elements as they lie in memory (or one).  Loads are kept
+// apart from their conversion and made without conditions (a row that does
+// not count is replaced by row 0 and dropped afterwards): a load inside a
+// branch is waited for inside it, and the rows of a token would come one
+// after the other (164 instead of 88 us for the gradients below).
 template <typename T, int VE>
 struct Vec {
-    float v[VE];
+    static constexpr int W = VE == 1 ? 1 : VE * static_cast<int>(sizeof(T)) / 4;
+    uint32_t w[W];
     __device__ __forceinline__ void load(const T* p) {
         if constexpr (VE == 1) {
-            v[0] = static_cast<float>(p[0]);
-        } else if constexpr (sizeof(T) == 4) {
-            const float4 a = reinterpret_cast<const float4*>(p)[0];
-            const float4 b = reinterpret_cast<const float4*>(p)[1];
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-            v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+            if constexpr (sizeof(T) == 2)
+                w[0] = static_cast<uint32_t>(__bfloat16_as_ushort(p[0])) << 16;
+            else
+                w[0] = __float_as_uint(p[0]);
         } else {
-            const uint4 u = *reinterpret_cast<const uint4*>(p);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {  // bf16 is the upper half of a float32
-                v[2 * i] = __uint_as_float(w[i] << 16);
-                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            for (int i = 0; i < W / 4; ++i) {
+                const uint4 u = reinterpret_cast<const uint4*>(p)[i];
+                w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
             }
         }
     }
-    __device__ __forceinline__ void store(T* p) const {
-        if constexpr (VE == 1) {
-            if constexpr (sizeof(T) == 2)
-                p[0] = __float2bfloat16_rn(v[0]);
-            else
-                p[0] = v[0];
-        } else if constexpr (sizeof(T) == 4) {
-            reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-            reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-            __nv_bfloat162 h[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-            *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
-        }
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (VE == 1 || sizeof(T) == 4) return __uint_as_float(w[i]);
+        // bf16 is the upper half of a float32
+        return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
     }
 };
+template <typename T, int VE>
+__device__ __forceinline__ void store_vec(T* p, const float (&v)[VE]) {
+    if constexpr (VE == 1) {
+        if constexpr (sizeof(T) == 2)
+            p[0] = __float2bfloat16_rn(v[0]);
+        else
+            p[0] = v[0];
+    } else if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+        __nv_bfloat162 h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
+    }
+}
+
+// Rows of units j0 .. j0 + KB of a token (-1: none, or past its units, which
+// is reported).
+template <int KB>
+__device__ __forceinline__ void unit_rows(const int32_t* at, int j0, int k, int64_t U, int* err,
+                                          int (&r)[KB]) {
+#pragma unroll
+    for (int j = 0; j < KB; ++j) r[j] = at[min(j0 + j, k - 1)];
+#pragma unroll
+    for (int j = 0; j < KB; ++j) {
+        if (r[j] >= U) {
+            atomicOr(err, ERR_ROW_INDEX);
+            r[j] = -1;
+        }
+        if (j0 + j >= k) r[j] = -1;
+    }
+}
 
 struct CombineArgs {
     const void* rows;
@@ -344,8 +406,9 @@ struct CombineArgs {
     int* err;
 };
 
-// One thread per (token, vector): tpt threads of a block share a token.
-template <typename RT, typename OT, int VE>
+// One thread per (token, vector): tpt threads of a block share a token, KB
+// units' rows are in flight at a time.
+template <typename RT, typename OT, int VE, int KB>
 __global__ void __launch_bounds__(kThreads) combine_units_kernel(CombineArgs a, int tpt) {
     const int per = kThreads / tpt, lane = threadIdx.x % tpt;
     const int64_t U = a.T * a.k;
@@ -354,24 +417,24 @@ __global__ void __launch_bounds__(kThreads) combine_units_kernel(CombineArgs a, 
         const int32_t* at = a.row_of + t * a.k;
         for (int c = lane; c < a.cols; c += tpt) {
             float acc[VE] = {};
-#pragma unroll 4
-            for (int j = 0; j < a.k; ++j) {
-                const int r = at[j];
-                if (r < 0) continue;
-                if (r >= U) {
-                    atomicOr(a.err, ERR_ROW_INDEX);
-                    continue;
-                }
-                const float w = a.weights ? a.weights[t * a.ldw + j] : 1.0f;
-                Vec<RT, VE> x;
-                x.load(static_cast<const RT*>(a.rows) + r * a.ldr + static_cast<int64_t>(c) * VE);
+            for (int j0 = 0; j0 < a.k; j0 += KB) {
+                int r[KB];
+                unit_rows<KB>(at, j0, a.k, U, a.err, r);
+                Vec<RT, VE> x[KB];
+                float w[KB];
 #pragma unroll
-                for (int i = 0; i < VE; ++i) acc[i] = fmaf(w, x.v[i], acc[i]);
+                for (int j = 0; j < KB; ++j)
+                    x[j].load(static_cast<const RT*>(a.rows) + max(r[j], 0) * a.ldr + static_cast<int64_t>(c) * VE);
+#pragma unroll
+                for (int j = 0; j < KB; ++j)
+                    w[j] = a.weights ? a.weights[t * a.ldw + min(j0 + j, a.k - 1)] : 1.0f;
+#pragma unroll
+                for (int j = 0; j < KB; ++j)
+                    if (r[j] >= 0)
+#pragma unroll
+                        for (int i = 0; i < VE; ++i) acc[i] = fmaf(w[j], x[j].get(i), acc[i]);
             }
-            Vec<OT, VE> y;
-#pragma unroll
-            for (int i = 0; i < VE; ++i) y.v[i] = acc[i];
-            y.store(static_cast<OT*>(a.out) + t * a.ldo + static_cast<int64_t>(c) * VE);
+            store_vec<OT, VE>(static_cast<OT*>(a.out) + t * a.ldo + static_cast<int64_t>(c) * VE, acc);
         }
     }
 }
@@ -389,63 +452,59 @@ struct CombineGradArgs {
     int* err;
 };
 
-// wpt warps of a block share a token; JB units at a time keep their dot
-// products in registers.
-template <typename GT, typename RT, int VE>
-__global__ void __launch_bounds__(kThreads) combine_grad_kernel(CombineGradArgs a, int wpt) {
-    constexpr int JB = 8;
-    __shared__ float part[kWarps][JB];
+// wpt warps of a block share a token; KB units at a time keep their rows in
+// flight and their dot products in registers.
+template <typename GT, typename RT, int VE, int KB>
+__global__ void __launch_bounds__(kThreads, sizeof(RT) == 2 ? 3 : 2) combine_grad_kernel(CombineGradArgs a, int wpt) {
+    __shared__ float part[kWarps][KB];
     const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int per = kWarps / wpt, wt = w % wpt;
     const int64_t U = a.T * a.k;
     for (int64_t tb = blockIdx.x * static_cast<int64_t>(per); tb < a.T;
          tb += static_cast<int64_t>(gridDim.x) * per) {
-        const int64_t t = tb + w / wpt;
-        for (int j0 = 0; j0 < a.k; j0 += JB) {
-            float dot[JB] = {};
-            int r[JB];
-            float wj[JB];
+        const bool on = tb + w / wpt < a.T;
+        const int64_t t = on ? tb + w / wpt : a.T - 1;
+        for (int j0 = 0; j0 < a.k; j0 += KB) {
+            float dot[KB] = {}, wj[KB];
+            int r[KB];
+            unit_rows<KB>(a.row_of + t * a.k, j0, a.k, U, a.err, r);
 #pragma unroll
-            for (int j = 0; j < JB; ++j) {
-                r[j] = t < a.T && j0 + j < a.k ? a.row_of[t * a.k + j0 + j] : -1;
-                if (r[j] >= U) {
-                    atomicOr(a.err, ERR_ROW_INDEX);
-                    r[j] = -1;
-                }
-                wj[j] = r[j] >= 0 && a.weights ? a.weights[t * a.ldw + j0 + j] : 1.0f;
-            }
-            if (t < a.T)
+            for (int j = 0; j < KB; ++j)
+                wj[j] = a.weights ? a.weights[t * a.ldw + min(j0 + j, a.k - 1)] : 1.0f;
+            if (on)
                 for (int c = wt * 32 + lane; c < a.cols; c += wpt * 32) {
+                    const int64_t at = static_cast<int64_t>(c) * VE;
                     Vec<GT, VE> g;
-                    g.load(static_cast<const GT*>(a.grad_out) + t * a.ldg + static_cast<int64_t>(c) * VE);
+                    Vec<RT, VE> x[KB];
+                    g.load(static_cast<const GT*>(a.grad_out) + t * a.ldg + at);
+                    if (a.grad_weights)
 #pragma unroll
-                    for (int j = 0; j < JB; ++j) {
-                        if (r[j] < 0) continue;
-                        if (a.grad_weights) {
-                            Vec<RT, VE> x;
-                            x.load(static_cast<const RT*>(a.rows) + r[j] * a.ldr +
-                                   static_cast<int64_t>(c) * VE);
+                        for (int j = 0; j < KB; ++j)
+                            x[j].load(static_cast<const RT*>(a.rows) + max(r[j], 0) * a.ldr + at);
+                    if (a.grad_rows)
 #pragma unroll
-                            for (int i = 0; i < VE; ++i) dot[j] = fmaf(g.v[i], x.v[i], dot[j]);
+                        for (int j = 0; j < KB; ++j) {
+                            if (r[j] < 0) continue;
+                            float y[VE];
+#pragma unroll
+                            for (int i = 0; i < VE; ++i) y[i] = wj[j] * g.get(i);
+                            store_vec<RT, VE>(static_cast<RT*>(a.grad_rows) + r[j] * a.ldgr + at, y);
                         }
-                        if (a.grad_rows) {
-                            Vec<RT, VE> y;
+                    if (a.grad_weights)
 #pragma unroll
-                            for (int i = 0; i < VE; ++i) y.v[i] = wj[j] * g.v[i];
-                            y.store(static_cast<RT*>(a.grad_rows) + r[j] * a.ldgr +
-                                    static_cast<int64_t>(c) * VE);
-                        }
-                    }
+                        for (int j = 0; j < KB; ++j)
+#pragma unroll
+                            for (int i = 0; i < VE; ++i) dot[j] = fmaf(g.get(i), x[j].get(i), dot[j]);
                 }
             if (!a.grad_weights) continue;
 #pragma unroll
-            for (int j = 0; j < JB; ++j) {
+            for (int j = 0; j < KB; ++j) {
 #pragma unroll
                 for (int o = 16; o; o >>= 1) dot[j] += __shfl_xor_sync(~0u, dot[j], o);
-                if (lane == 0) part[w][j] = dot[j];
+                if (lane == 0) part[w][j] = r[j] < 0 ? 0.0f : dot[j];
             }
             __syncthreads();
-            if (wt == 0 && lane < JB && j0 + lane < a.k && t < a.T) {
+            if (wt == 0 && lane < KB && j0 + lane < a.k && on) {
                 float s = 0.0f;
                 for (int i = 0; i < wpt; ++i) s += part[w + i][lane];
                 a.grad_weights[t * a.k + j0 + lane] = s;
@@ -458,8 +517,8 @@ __global__ void __launch_bounds__(kThreads) combine_grad_kernel(CombineGradArgs 
         for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < n;
              i += static_cast<int64_t>(gridDim.x) * kThreads) {
             const int64_t r = i / a.cols;
-            Vec<RT, VE> z{};
-            z.store(static_cast<RT*>(a.grad_rows) + (first + r) * a.ldgr + (i - r * a.cols) * VE);
+            const float z[VE] = {};
+            store_vec<RT, VE>(static_cast<RT*>(a.grad_rows) + (first + r) * a.ldgr + (i - r * a.cols) * VE, z);
         }
     }
 }
@@ -495,6 +554,21 @@ void with_vec(int bytes, F f) {
         f(uint16_t{});
 }
 
+// Units whose rows a thread keeps in flight.
+template <typename F>
+void with_units(int k, F f) {
+    if (k == 1)
+        f(std::integral_constant<int, 1>{});
+    else if (k == 2)
+        f(std::integral_constant<int, 2>{});
+    else if (k <= 4)
+        f(std::integral_constant<int, 4>{});
+    else if (k <= 6)
+        f(std::integral_constant<int, 6>{});
+    else
+        f(std::integral_constant<int, 8>{});
+}
+
 aem_status sort_and_move(const Ids& ids, const SortOut& so, int64_t T, MoveArgs m, int vb,
                          void* ws, cudaStream_t s) {
     int* err = device_error_word(current_device());
@@ -517,13 +591,25 @@ aem_status sort_and_move(const Ids& ids, const SortOut& so, int64_t T, MoveArgs 
     int* totals = counts + static_cast<int64_t>(p.C) * ids.E;
     sort_count_kernel<<<p.C, kThreads, 0, s>>>(ids, so.U, p.tc, p.C, counts, err);
     AEM_CHECK_LAUNCH();
-    sort_scan_kernel<<<ids.E, kThreads, 0, s>>>(p.C, counts, totals);
-    AEM_CHECK_LAUNCH();
+    // the scan and the ranking start under their predecessors and wait for
+    // them where they read their results
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = s;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    cfg.gridDim = dim3(ids.E);
+    AEM_TRY_CUDA(cudaLaunchKernelEx(&cfg, sort_scan_kernel, p.C, counts, totals));
+    cfg.gridDim = dim3(p.C);
+    cudaError_t e = cudaSuccess;
     with_vec(vb, [&](auto v) {
-        sort_move_kernel<decltype(v)>
-            <<<p.C, kThreads, 0, s>>>(ids, so, p.tc, p.C, counts, totals, m, err);
+        e = cudaLaunchKernelEx(&cfg, sort_move_kernel<decltype(v)>, ids, so, p.tc, p.C,
+                               static_cast<const int*>(counts), static_cast<const int*>(totals), m, err);
     });
-    AEM_CHECK_LAUNCH();
+    AEM_TRY_CUDA(e);
     count_launches(3);
     return AEM_OK;
 }
@@ -673,10 +759,12 @@ aem_status aem_combine(const void* rows, aem_dtype rows_dtype, int64_t ldr, cons
     auto go = [&](auto r, auto o) {
         using RT = decltype(r);
         using OT = decltype(o);
-        if (vec)
-            aem::combine_units_kernel<RT, OT, 8><<<g, aem::kThreads, 0, s>>>(a, tpt);
+        if (!vec)
+            aem::combine_units_kernel<RT, OT, 1, 4><<<g, aem::kThreads, 0, s>>>(a, tpt);
         else
-            aem::combine_units_kernel<RT, OT, 1><<<g, aem::kThreads, 0, s>>>(a, tpt);
+            aem::with_units(k, [&](auto kb) {
+                aem::combine_units_kernel<RT, OT, 8, decltype(kb)::value><<<g, aem::kThreads, 0, s>>>(a, tpt);
+            });
     };
     const __nv_bfloat16 h{};
     if (rows_dtype == AEM_BF16)
@@ -736,10 +824,12 @@ aem_status aem_combine_backward(const void* grad_out, aem_dtype out_dtype, int64
     auto go = [&](auto o, auto r) {
         using GT = decltype(o);
         using RT = decltype(r);
-        if (vec)
-            aem::combine_grad_kernel<GT, RT, 8><<<g, aem::kThreads, 0, s>>>(a, wpt);
+        if (!vec)
+            aem::combine_grad_kernel<GT, RT, 1, 4><<<g, aem::kThreads, 0, s>>>(a, wpt);
         else
-            aem::combine_grad_kernel<GT, RT, 1><<<g, aem::kThreads, 0, s>>>(a, wpt);
+            aem::with_units(k, [&](auto kb) {
+                aem::combine_grad_kernel<GT, RT, 8, decltype(kb)::value><<<g, aem::kThreads, 0, s>>>(a, wpt);
+            });
     };
     const __nv_bfloat16 h{};
     if (out_dtype == AEM_BF16)

@@ -33,6 +33,7 @@
 #include <algorithm>
 #include <atomic>
 #include <new>
+#include <type_traits>
 
 #include "common.cuh"
 #include "runtime.h"
@@ -58,79 +59,96 @@ struct Q4Weight {
 
 namespace {
 
-constexpr int kThreads = 256, kWarps = 8;  // quantise, pack
+constexpr int kThreads = 256;  // pack
 
 // ------------------------------------------------------------------ quantise
-// One block per (128 columns, scale group): warp w holds rows w, w+8, ... of
-// the group in registers, 4 columns per lane, so w is read once; the column
+// One block per (128 columns, scale group): GS / 8 warps hold 8 rows of the
+// group each in registers, 4 columns per lane, so w is read once; the column
 // maxima meet in shared memory.  scale = max(amax / 7, 1e-12), rounded to
 // the scale's type before q = clip(rint(w / scale), -7, 7) is taken with it
-// (IEEE float32 division, ties to even).
-template <typename WT, typename ST, int GS>
-__global__ void __launch_bounds__(kThreads)
-    quantize_q4_kernel(const WT* __restrict__ w, int64_t K, int64_t N, int64_t KB, bool vec,
+// (IEEE float32 division, ties to even).  |w / scale| is about 7 at most and
+// w * (1 / scale) is within 2^-20 of it, so the division itself is only made
+// where the product lies that near a half.  Adding 1.5 * 2^23 rounds to a
+// whole number, ties to even, and leaves it in the low byte (the conversion
+// instructions run at a quarter of the rate).
+constexpr float kRint = 12582912.0f;
+template <typename WT, typename ST, int GS, bool VEC>
+__global__ void __launch_bounds__(4 * GS, GS == 128 ? 2 : 1)
+    quantize_q4_kernel(const WT* __restrict__ w, int64_t K, int64_t N, int64_t KB,
                        int8_t* __restrict__ q, ST* __restrict__ scale) {
-    constexpr int R = GS / kWarps;
-    __shared__ float amax[kWarps][128];
+    constexpr int R = 8, W = GS / R;
+    __shared__ float4 amax[W][32], scales[32], inverses[32];
     const int lane = threadIdx.x & 31, wi = threadIdx.x >> 5;
     const int64_t g = blockIdx.x / KB, b = blockIdx.x % KB;
     const int64_t n0 = blockIdx.y * 128ll + lane * 4, k0 = b * GS + wi;
-    const WT* src = w + g * K * N;
+    const int rows = static_cast<int>(min(static_cast<int64_t>(R), (K - k0 + W - 1) / W));  // k0 + i * W < K
+    const int64_t at = (g * K + k0) * N + n0, step = W * N;
+    const bool on = n0 < N;
     float v[R][4];
-    float m[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        const int64_t k = k0 + i * kWarps;
         v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.f;
-        if (k < K && n0 < N) {
-            const WT* p = src + k * N + n0;
-            if (vec) {
-                if constexpr (sizeof(WT) == 4) {
-                    const float4 f = *reinterpret_cast<const float4*>(p);
-                    v[i][0] = f.x, v[i][1] = f.y, v[i][2] = f.z, v[i][3] = f.w;
-                } else {
-                    const uint2 u = *reinterpret_cast<const uint2*>(p);
-                    v[i][0] = __uint_as_float(u.x << 16), v[i][1] = __uint_as_float(u.x & 0xffff0000u);
-                    v[i][2] = __uint_as_float(u.y << 16), v[i][3] = __uint_as_float(u.y & 0xffff0000u);
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (n0 + j < N) v[i][j] = static_cast<float>(p[j]);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) m[j] = fmaxf(m[j], fabsf(v[i][j]));
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) amax[wi][lane * 4 + j] = m[j];
-    __syncthreads();
-    float s[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-#pragma unroll
-        for (int i = 0; i < kWarps; ++i) m[j] = fmaxf(m[j], amax[i][lane * 4 + j]);
-        s[j] = fmaxf(__fdiv_rn(m[j], 7.0f), 1e-12f);
-        if constexpr (sizeof(ST) == 2) s[j] = __bfloat162float(__float2bfloat16_rn(s[j]));
-        if (wi == 0 && n0 + j < N) scale[(g * KB + b) * N + n0 + j] = static_cast<ST>(s[j]);
-    }
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int64_t k = k0 + i * kWarps;
-        if (k >= K || n0 >= N) continue;
-        int8_t c[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float r = fminf(fmaxf(rintf(__fdiv_rn(v[i][j], s[j])), -7.0f), 7.0f);
-            c[j] = static_cast<int8_t>(static_cast<int>(r));
-        }
-        int8_t* p = q + (g * K + k) * N + n0;
-        if (vec) {
-            *reinterpret_cast<char4*>(p) = make_char4(c[0], c[1], c[2], c[3]);
+        if (i >= rows || !on) continue;
+        const WT* p = w + at + i * step;
+        if constexpr (VEC && sizeof(WT) == 4) {
+            const float4 f = *reinterpret_cast<const float4*>(p);
+            v[i][0] = f.x, v[i][1] = f.y, v[i][2] = f.z, v[i][3] = f.w;
+        } else if constexpr (VEC) {
+            const uint2 u = *reinterpret_cast<const uint2*>(p);
+            v[i][0] = __uint_as_float(u.x << 16), v[i][1] = __uint_as_float(u.x & 0xffff0000u);
+            v[i][2] = __uint_as_float(u.y << 16), v[i][3] = __uint_as_float(u.y & 0xffff0000u);
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (n0 + j < N) p[j] = c[j];
+                if (n0 + j < N) v[i][j] = static_cast<float>(p[j]);
+        }
+    }
+    float m[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m[j] = fmaxf(m[j], fabsf(v[i][j]));
+    amax[wi][lane] = make_float4(m[0], m[1], m[2], m[3]);
+    __syncthreads();
+    if (threadIdx.x < 128) {  // one thread per column
+        const float* col = reinterpret_cast<const float*>(amax) + threadIdx.x;
+        float a = 0.0f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) a = fmaxf(a, col[i * 128]);
+        float sc = fmaxf(__fdiv_rn(a, 7.0f), 1e-12f);
+        if constexpr (sizeof(ST) == 2) sc = __bfloat162float(__float2bfloat16_rn(sc));
+        reinterpret_cast<float*>(scales)[threadIdx.x] = sc;
+        reinterpret_cast<float*>(inverses)[threadIdx.x] = __frcp_rn(sc);
+        const int64_t n = blockIdx.y * 128ll + threadIdx.x;
+        if (n < N) scale[(g * KB + b) * N + n] = static_cast<ST>(sc);
+    }
+    __syncthreads();
+    const float4 s4 = scales[lane], i4 = inverses[lane];
+    const float s[4] = {s4.x, s4.y, s4.z, s4.w}, inv[4] = {i4.x, i4.y, i4.z, i4.w};
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        if (i >= rows || !on) continue;
+        uint32_t c[4];
+        bool near = false;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float d = fminf(fmaxf(v[i][j] * inv[j], -7.0f), 7.0f);  // clipping commutes with rint
+            const float r = d + kRint;
+            near |= fabsf(d - (r - kRint)) > 0.5f - 0x1p-18f;
+            c[j] = __float_as_uint(r);
+        }
+        if (near)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                c[j] = __float_as_uint(fminf(fmaxf(__fdiv_rn(v[i][j], s[j]), -7.0f), 7.0f) + kRint);
+        int8_t* p = q + at + i * step;
+        if constexpr (VEC) {
+            *reinterpret_cast<uint32_t*>(p) =
+                __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (n0 + j < N) p[j] = static_cast<int8_t>(c[j] & 0xff);
         }
     }
 }
@@ -912,12 +930,19 @@ void launch_quantize(const void* w, int64_t G, int64_t K, int64_t N, int gs, int
                      reinterpret_cast<uintptr_t>(q) % 4 == 0;
     auto* wt = static_cast<const WT*>(w);
     auto* st = static_cast<ST*>(scale);
+    auto go = [&](auto size) {
+        constexpr int GS = decltype(size)::value;
+        if (vec)
+            quantize_q4_kernel<WT, ST, GS, true><<<grid, 4 * GS, 0, s>>>(wt, K, N, KB, q, st);
+        else
+            quantize_q4_kernel<WT, ST, GS, false><<<grid, 4 * GS, 0, s>>>(wt, K, N, KB, q, st);
+    };
     if (gs == 32)
-        quantize_q4_kernel<WT, ST, 32><<<grid, kThreads, 0, s>>>(wt, K, N, KB, vec, q, st);
+        go(std::integral_constant<int, 32>{});
     else if (gs == 64)
-        quantize_q4_kernel<WT, ST, 64><<<grid, kThreads, 0, s>>>(wt, K, N, KB, vec, q, st);
+        go(std::integral_constant<int, 64>{});
     else
-        quantize_q4_kernel<WT, ST, 128><<<grid, kThreads, 0, s>>>(wt, K, N, KB, vec, q, st);
+        go(std::integral_constant<int, 128>{});
 }
 
 void free_q4(Q4Weight* w) {
