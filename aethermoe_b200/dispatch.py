@@ -34,7 +34,7 @@ class TokenOrder:
     unit, -1 for none), ``unit_of [T*k]`` (unit ``t*k + j`` of each row, -1 past
     the last).  int32 CUDA tensors."""
 
-    __slots__ = ("starts", "row_of", "unit_of")
+    __slots__ = ("_buf", "_starts", "_row_of", "_unit_of", "shape", "num_experts", "device")
 
     def __init__(self, starts, row_of, unit_of):
         for name, t, dim in (("starts", starts, 1), ("row_of", row_of, 2), ("unit_of", unit_of, 1)):
@@ -44,11 +44,57 @@ class TokenOrder:
                 raise ValueError("starts, row_of and unit_of must be on one device")
         if starts.numel() < 2 or unit_of.numel() != row_of.numel():
             raise ValueError("starts needs E + 1 entries and unit_of one per unit of row_of")
-        self.starts, self.row_of, self.unit_of = starts, row_of, unit_of
+        self._buf = None
+        self._starts, self._row_of, self._unit_of = starts, row_of, unit_of
+        self.shape, self.num_experts, self.device = tuple(row_of.shape), starts.numel() - 1, starts.device
+
+    @classmethod
+    def _new(cls, t, k, num_experts, like):
+        """An order to be filled in: one buffer, row_of then unit_of then starts."""
+        self = cls.__new__(cls)
+        self._buf = like.new_empty(2 * t * k + num_experts + 1, dtype=torch.int32)
+        self._starts = self._row_of = self._unit_of = None
+        self.shape, self.num_experts, self.device = (t, k), num_experts, like.device
+        return self
+
+    def _pointers(self):
+        """Addresses of (row_of, unit_of, starts)."""
+        if self._buf is None:
+            return self._row_of.data_ptr(), self._unit_of.data_ptr(), self._starts.data_ptr()
+        p, u = self._buf.data_ptr(), 4 * self.shape[0] * self.shape[1]
+        return p, p + u, p + 2 * u
 
     @property
-    def num_experts(self):
-        return self.starts.numel() - 1
+    def row_of(self):
+        if self._row_of is None:
+            t, k = self.shape
+            self._row_of = self._buf.as_strided((t, k), (k, 1), 0)
+        return self._row_of
+
+    @property
+    def unit_of(self):
+        if self._unit_of is None:
+            n = self.shape[0] * self.shape[1]
+            self._unit_of = self._buf.as_strided((n,), (1,), n)
+        return self._unit_of
+
+    @property
+    def starts(self):
+        if self._starts is None:
+            self._starts = self._buf.as_strided((self.num_experts + 1,), (1,), 2 * self.shape[0] * self.shape[1])
+        return self._starts
+
+    def record_stream(self, stream):
+        for t in (self._buf, self._starts, self._row_of, self._unit_of):
+            if t is not None:
+                t.record_stream(stream)
+
+
+try:  # the handle alone, without a Stream object (3 us of a call's 15 on the host)
+    _stream_handle = torch._C._cuda_getCurrentRawStream
+except AttributeError:
+    def _stream_handle(device):
+        return torch.cuda.current_stream(device).cuda_stream
 
 
 def _on(stream, fn, tensors, args):
@@ -62,7 +108,7 @@ def _on(stream, fn, tensors, args):
         if t is not None and t.device != dev:
             raise ValueError(f"tensors are on {dev} and {t.device}")
     if stream is None and torch.cuda.current_device() == dev.index:
-        return fn(*args, torch.cuda.current_stream().cuda_stream)
+        return fn(*args, _stream_handle(dev.index))
     if stream is None:
         stream = torch.cuda.current_stream(dev)
     elif stream.device != dev:
@@ -136,24 +182,21 @@ def _differentiable(what, out, *tensors):
 def _sort_and_move(x, ldx, ids, num_experts, rows, ldr, s):
     L = _lib.lib()
     t, k = ids.shape
-    dev = ids.device
-    starts = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
-    row_of = torch.empty((t, k), dtype=torch.int32, device=dev)
-    unit_of = torch.empty(t * k, dtype=torch.int32, device=dev)
-    need = L.aem_token_sort_workspace(t, k, num_experts)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    order = TokenOrder._new(t, k, num_experts, ids)
+    row_of, unit_of, starts = order._pointers()
+    ws, need = None, 0
+    if t * k > 1024:  # smaller batches need no scratch
+        need = L.aem_token_sort_workspace(t, k, num_experts)
+        keep = ids.new_empty(need // 4)
+        ws = keep.data_ptr()
     st, sk = ids.stride()
     if x is None:
-        _lib.check(L.aem_token_sort(ids.data_ptr(), t, k, st, sk, num_experts, starts.data_ptr(),
-                                    row_of.data_ptr(), unit_of.data_ptr(),
-                                    ws.data_ptr() if need else None, need, s), "aem_token_sort")
+        _lib.check(L.aem_token_sort(ids.data_ptr(), t, k, st, sk, num_experts, starts, row_of, unit_of, ws,
+                                    need, s), "aem_token_sort")
     else:
-        _lib.check(L.aem_dispatch(x.data_ptr(), _DT[x.dtype], ldx, x.shape[1], ids.data_ptr(), t, k,
-                                  st, sk, num_experts, rows.data_ptr(), ldr, starts.data_ptr(),
-                                  row_of.data_ptr(), unit_of.data_ptr(),
-                                  ws.data_ptr() if need else None, need, s), "aem_dispatch")
-    order = TokenOrder.__new__(TokenOrder)
-    order.starts, order.row_of, order.unit_of = starts, row_of, unit_of
+        _lib.check(L.aem_dispatch(x.data_ptr(), _DT[x.dtype], ldx, x.shape[1], ids.data_ptr(), t, k, st, sk,
+                                  num_experts, rows.data_ptr(), ldr, starts, row_of, unit_of, ws, need, s),
+                   "aem_dispatch")
     return order
 
 
@@ -166,18 +209,18 @@ def _dispatch(x, ids, num_experts, out, s):
 
 
 def _dispatch_rows(x, order, out, s):
-    t, k = order.row_of.shape
+    t, k = order.shape
     x, ldx = _matrix(x, "x", rows=t)
     rows, ldr = _output(out, (t * k, x.shape[1]), x.dtype, x.device, "rows")
-    _lib.check(_lib.lib().aem_dispatch_rows(x.data_ptr(), _DT[x.dtype], ldx, x.shape[1],
-                                            order.row_of.data_ptr(), order.starts.data_ptr(), t, k,
+    row_of, _, starts = order._pointers()
+    _lib.check(_lib.lib().aem_dispatch_rows(x.data_ptr(), _DT[x.dtype], ldx, x.shape[1], row_of, starts, t, k,
                                             order.num_experts, rows.data_ptr(), ldr, s),
                "aem_dispatch_rows")
     return rows
 
 
 def _combine(rows, weights, order, out_dtype, out, s):
-    t, k = order.row_of.shape
+    t, k = order.shape
     rows, ldr = _matrix(rows, "rows", rows=t * k)
     d = rows.shape[1]
     ldw = 0
@@ -186,13 +229,14 @@ def _combine(rows, weights, order, out_dtype, out, s):
     out, ldo = _output(out, (t, d), out_dtype or (rows.dtype if out is None else out.dtype), rows.device)
     _lib.check(_lib.lib().aem_combine(rows.data_ptr(), _DT[rows.dtype], ldr,
                                       None if weights is None else weights.data_ptr(), ldw,
-                                      order.row_of.data_ptr(), t, k, d, out.data_ptr(),
+                                      order._pointers()[0], t, k, d, out.data_ptr(),
                                       _DT[out.dtype], ldo, s), "aem_combine")
     return out
 
 
 def _combine_backward(grad_out, rows, weights, order, rows_dtype, want_rows, want_weights, s):
-    t, k = order.row_of.shape
+    t, k = order.shape
+    row_of, _, starts = order._pointers()
     grad_out, ldg = _matrix(grad_out, "grad_out", rows=t)
     d = grad_out.shape[1]
     ldr = ldw = ldgr = 0
@@ -206,8 +250,7 @@ def _combine_backward(grad_out, rows, weights, order, rows_dtype, want_rows, wan
         grad_rows, ldgr = _output(None, (t * k, d), rows_dtype, grad_out.device, "grad_rows")
     _lib.check(_lib.lib().aem_combine_backward(
         grad_out.data_ptr(), _DT[grad_out.dtype], ldg, rows.data_ptr() if want_weights else None,
-        _DT[rows_dtype], ldr, weights.data_ptr(), ldw, order.row_of.data_ptr(),
-        order.starts.data_ptr(), t, k, order.num_experts, d,
+        _DT[rows_dtype], ldr, weights.data_ptr(), ldw, row_of, starts, t, k, order.num_experts, d,
         grad_rows.data_ptr() if want_rows else None, ldgr,
         grad_weights.data_ptr() if want_weights else None, s), "aem_combine_backward")
     return grad_rows, grad_weights
@@ -220,7 +263,7 @@ class _DispatchFn(torch.autograd.Function):
             rows, order = _on(stream, _dispatch, (x, ids), (x, ids, num_experts, None))
             holder.append(order)
         else:
-            rows = _on(stream, _dispatch_rows, (x, order.row_of), (x, order, None))
+            rows = _on(stream, _dispatch_rows, (x, order), (x, order, None))
         ctx.order, ctx.x_dtype = order, x.dtype
         return rows
 
@@ -234,7 +277,7 @@ class _DispatchFn(torch.autograd.Function):
 class _CombineFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, weights, order, out_dtype, stream):
-        out = _on(stream, _combine, (rows, weights, order.row_of), (rows, weights, order, out_dtype, None))
+        out = _on(stream, _combine, (rows, weights, order), (rows, weights, order, out_dtype, None))
         ctx.save_for_backward(rows, weights)
         ctx.order = order
         return out
@@ -244,7 +287,7 @@ class _CombineFn(torch.autograd.Function):
     def backward(ctx, grad):
         _refuse_capture("combine")
         rows, weights = ctx.saved_tensors
-        gr, gw = _on(None, _combine_backward, (grad, rows, weights, ctx.order.row_of),
+        gr, gw = _on(None, _combine_backward, (grad, rows, weights, ctx.order),
                      (grad, rows, weights, ctx.order, rows.dtype, ctx.needs_input_grad[0],
                       ctx.needs_input_grad[1]))
         return gr, gw, None, None, None
@@ -278,12 +321,12 @@ def dispatch_rows(x, order, out=None, stream=None):
     """Rows of another ``x [T, d]`` by an existing order."""
     if _differentiable("dispatch_rows", out, x):
         return _DispatchFn.apply(x, None, 0, order, None, stream)
-    return _on(stream, _dispatch_rows, (x, order.row_of), (x, order, out))
+    return _on(stream, _dispatch_rows, (x, order), (x, order, out))
 
 
 def dispatch_backward(grad_rows, order, out_dtype=None, out=None, stream=None):
     """Gradient of ``dispatch``: ``grad_x[t] = sum_j grad_rows[row_of[t, j]]``."""
-    return _on(stream, _combine, (grad_rows, order.row_of), (grad_rows, None, order, out_dtype, out))
+    return _on(stream, _combine, (grad_rows, order), (grad_rows, None, order, out_dtype, out))
 
 
 def combine(rows, weights, order, out_dtype=None, out=None, stream=None):
@@ -291,11 +334,11 @@ def combine(rows, weights, order, out_dtype=None, out=None, stream=None):
     ``weights [T, k]`` float32; ``out_dtype`` defaults to the rows')."""
     if _differentiable("combine", out, rows, weights):
         return _CombineFn.apply(rows, weights, order, out_dtype, stream)
-    return _on(stream, _combine, (rows, weights, order.row_of), (rows, weights, order, out_dtype, out))
+    return _on(stream, _combine, (rows, weights, order), (rows, weights, order, out_dtype, out))
 
 
 def combine_backward(grad_out, rows, weights, order, stream=None):
     """Gradients of ``combine``: ``(grad_rows [T*k, d]`` in the rows' dtype,
     ``grad_weights [T, k]`` float32``)``."""
-    return _on(stream, _combine_backward, (grad_out, rows, weights, order.row_of),
+    return _on(stream, _combine_backward, (grad_out, rows, weights, order),
                (grad_out, rows, weights, order, rows.dtype, True, True))

@@ -87,7 +87,7 @@ class Q4Weight:
             _lib.check(_lib.lib().aem_q4weight_pack(q.data_ptr(), scale.data_ptr(), _DT[scale.dtype], g,
                                                     k, n, group_size, device, ctypes.byref(h)),
                        "aem_q4weight_pack")
-        self.handle = h.value
+        self.handle, self._scratch = h.value, {}
         self.G, self.K, self.N, self.group_size, self.device = g, k, n, group_size, device
 
     def close(self):
@@ -111,7 +111,12 @@ def _check_weight(w, device):
 
 def _scratch(x, w, grouped):
     """``(pointer, bytes, tensor)`` of a product's scratch."""
-    n = _lib.lib().aem_q4gemm_workspace(w.handle, _DT[x.dtype], x.shape[0], grouped)
+    key = (x.dtype, x.shape[0], grouped)
+    n = w._scratch.get(key)
+    if n is None:
+        n = _lib.lib().aem_q4gemm_workspace(w.handle, _DT[x.dtype], x.shape[0], grouped)
+        if len(w._scratch) < 1024:
+            w._scratch[key] = n
     if not n:
         return None, 0, None
     t = torch.empty(n, dtype=torch.uint8, device=x.device)
