@@ -332,7 +332,8 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // ------------------------------------------------------------------ combine
-// VE = 8 consecutive elements as they lie in memory (or one).  Loads are kept
+// VE consecutive elements (8 or 4: 16 bytes of the widest type; or one) as
+// they lie in memory.  Loads are kept
 // apart from their conversion and made without conditions (a row that does
 // not count is replaced by row 0 and dropped afterwards): a load inside a
 // branch is waited for inside it, and the rows of a token would come one
@@ -348,6 +349,10 @@ struct Vec {
             else
                 w[0] = __float_as_uint(p[0]);
         } else {
+            if constexpr (W == 2) {
+                const uint2 u = *reinterpret_cast<const uint2*>(p);
+                w[0] = u.x, w[1] = u.y;
+            }
 #pragma unroll
             for (int i = 0; i < W / 4; ++i) {
                 const uint4 u = reinterpret_cast<const uint4*>(p)[i];
@@ -369,13 +374,20 @@ __device__ __forceinline__ void store_vec(T* p, const float (&v)[VE]) {
         else
             p[0] = v[0];
     } else if constexpr (sizeof(T) == 4) {
-        reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-        __nv_bfloat162 h[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-        *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
+        for (int i = 0; i < VE / 4; ++i)
+            reinterpret_cast<float4*>(p)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    } else {
+        uint32_t h[VE / 2];
+#pragma unroll
+        for (int i = 0; i < VE / 2; ++i) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            h[i] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+        if constexpr (VE == 4)
+            *reinterpret_cast<uint2*>(p) = make_uint2(h[0], h[1]);
+        else
+            *reinterpret_cast<uint4*>(p) = make_uint4(h[0], h[1], h[2], h[3]);
     }
 }
 
@@ -529,7 +541,7 @@ struct Plan {  // chunks of the three-kernel sort
 };
 Plan plan_of(int64_t T, int k) {
     Plan p;
-    const int64_t want = (T + 148 * 4 - 1) / (148 * 4);
+    const int64_t want = (T + 148 * 8 - 1) / (148 * 8);
     p.tc = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, kBlockUnits / k)));
     p.C = static_cast<int>((T + p.tc - 1) / p.tc);
     return p;
@@ -750,11 +762,12 @@ aem_status aem_combine(const void* rows, aem_dtype rows_dtype, int64_t ldr, cons
                           static_cast<uint64_t>(ldr * aem::elem(rows_dtype)) |
                           static_cast<uint64_t>(ldo * aem::elem(out_dtype));
     const bool vec = bits % 16 == 0 && d % 8 == 0;
+    const int ve = rows_dtype == AEM_F32 ? 4 : 8;
     aem::CombineArgs a{rows, weights, row_of, out, ldr, ldw, ldo, T, k,
-                       static_cast<int>(vec ? d / 8 : d), err};
+                       static_cast<int>(vec ? d / ve : d), err};
     const int tpt = aem::threads_per_token(T, a.cols);
     const int64_t per = aem::kThreads / tpt;
-    const unsigned g = static_cast<unsigned>(std::min<int64_t>((T + per - 1) / per, 148 * 64));
+    const unsigned g = static_cast<unsigned>(std::min<int64_t>((T + per - 1) / per, 148 * 16));
     auto s = static_cast<cudaStream_t>(stream);
     auto go = [&](auto r, auto o) {
         using RT = decltype(r);
@@ -763,7 +776,7 @@ aem_status aem_combine(const void* rows, aem_dtype rows_dtype, int64_t ldr, cons
             aem::combine_units_kernel<RT, OT, 1, 4><<<g, aem::kThreads, 0, s>>>(a, tpt);
         else
             aem::with_units(k, [&](auto kb) {
-                aem::combine_units_kernel<RT, OT, 8, decltype(kb)::value><<<g, aem::kThreads, 0, s>>>(a, tpt);
+                aem::combine_units_kernel<RT, OT, (sizeof(RT) == 4 ? 4 : 8), decltype(kb)::value><<<g, aem::kThreads, 0, s>>>(a, tpt);
             });
     };
     const __nv_bfloat16 h{};
@@ -814,8 +827,9 @@ aem_status aem_combine_backward(const void* grad_out, aem_dtype out_dtype, int64
     if (grad_rows)
         bits |= reinterpret_cast<uintptr_t>(grad_rows) | static_cast<uint64_t>(ldgr * aem::elem(rows_dtype));
     const bool vec = bits % 16 == 0 && d % 8 == 0;
+    const int ve = rows_dtype == AEM_F32 || out_dtype == AEM_F32 ? 4 : 8;
     aem::CombineGradArgs a{grad_out, rows, weights, row_of, starts + E, grad_rows, grad_weights,
-                           ldg, ldr, ldw, ldgr, T, k, static_cast<int>(vec ? d / 8 : d), err};
+                           ldg, ldr, ldw, ldgr, T, k, static_cast<int>(vec ? d / ve : d), err};
     int wpt = 1;  // more warps for a token while the batch leaves SMs idle
     while (wpt < aem::kWarps && T * wpt < 148 * 16 && a.cols > 32 * wpt) wpt *= 2;
     const int64_t per = aem::kWarps / wpt;
@@ -828,7 +842,7 @@ aem_status aem_combine_backward(const void* grad_out, aem_dtype out_dtype, int64
             aem::combine_grad_kernel<GT, RT, 1, 4><<<g, aem::kThreads, 0, s>>>(a, wpt);
         else
             aem::with_units(k, [&](auto kb) {
-                aem::combine_grad_kernel<GT, RT, 8, decltype(kb)::value><<<g, aem::kThreads, 0, s>>>(a, wpt);
+                aem::combine_grad_kernel<GT, RT, (sizeof(GT) + sizeof(RT) > 4 ? 4 : 8), decltype(kb)::value><<<g, aem::kThreads, 0, s>>>(a, wpt);
             });
     };
     const __nv_bfloat16 h{};

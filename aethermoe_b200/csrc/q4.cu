@@ -323,17 +323,20 @@ template <typename XT>
 __global__ void __launch_bounds__(1024)
     q4_terms_kernel(const XT* __restrict__ x, int64_t ldx, int64_t K, int64_t KP, int tn, bool vec,
                     uint8_t* __restrict__ out, float* __restrict__ unscale) {
-    constexpr int TERMS = kTerms<XT>, HELD = 4;  // up to 16384 k stay in registers
+    constexpr int TERMS = kTerms<XT>, HELD = 4;  // 16 k a thread stay in registers
+    const int64_t nt = blockDim.x;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     __shared__ uint32_t tops[32];
+    if (threadIdx.x < 32) tops[threadIdx.x] = 0;
+    __syncthreads();
     const XT* row = x + blockIdx.x * ldx;
     Four<XT> v[HELD];
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) v[i].load(row, (i * 1024 + threadIdx.x) * 4, K, vec);
+    for (int i = 0; i < HELD; ++i) v[i].load(row, (i * nt + threadIdx.x) * 4, K, vec);
 #pragma unroll
     for (int i = 0; i < HELD; ++i) top = max(top, v[i].top());
-    for (int64_t k = (HELD * 1024 + threadIdx.x) * 4; k < K; k += 4096) {
+    for (int64_t k = (HELD * nt + threadIdx.x) * 4; k < K; k += nt * 4) {
         Four<XT> u;
         u.load(row, k, K, vec);
         top = max(top, u.top());
@@ -354,10 +357,10 @@ __global__ void __launch_bounds__(1024)
     };
 #pragma unroll
     for (int i = 0; i < HELD; ++i) {
-        const int64_t k = (i * 1024 + threadIdx.x) * 4;
+        const int64_t k = (i * nt + threadIdx.x) * 4;
         if (k < KP) put(k, v[i]);
     }
-    for (int64_t k = (HELD * 1024 + threadIdx.x) * 4; k < KP; k += 4096) {
+    for (int64_t k = (HELD * nt + threadIdx.x) * 4; k < KP; k += nt * 4) {
         Four<XT> u;
         u.load(row, k, K, vec);
         put(k, u);
@@ -448,7 +451,8 @@ struct Q4Cfg {
     static constexpr int MAXP = XSTEP == 1024 ? 32 : 24;  // XIN: blocks whose terms are kept
     static constexpr int XRES = XIN ? MAXP * XSTEP : 0;
     static constexpr int STAGE = (XIN ? 0 : XB) + 8192 + (FULL * 512 + 1023) / 1024 * 1024;
-    static constexpr int RECV = (ROWS * 128 + 8) * 4;  // the cluster's sums, S equal shares
+    // the cluster's sums: S shares of ceil(rows / S) rows, for any S up to 8
+    static constexpr int RECV = (ROWS < 8 ? 8 : ROWS < 16 ? 14 : ROWS < 32 ? 21 : 36) * 128 * 4;
     // an even ring: a stage always comes back to the warpgroup that saw its
     // previous phase, so no parity wait can mistake a phase for the one two back
     static constexpr int FIT = (113 * 1024 - 2048 - XRES - RECV) / STAGE / 2 * 2;
@@ -458,7 +462,7 @@ struct Q4Cfg {
     static constexpr int SMEM = USED > 78 * 1024 ? USED : 78 * 1024;
     static_assert(UA + ND * SUB * COLS <= TW && NS >= 4 && SMEM <= 113 * 1024, "budgets");
     static_assert(ROWS * TN <= COLS && (UK >= GS || UK == 128), "a scale group inside a unit");
-    static_assert(STAGE * NS >= RECV, "a warpgroup's sums fit the ring");
+    static_assert(STAGE * NS >= ROWS * 512, "a warpgroup's sums fit the ring");
 };
 constexpr int kQ4Threads = 12 * 32;
 
@@ -496,7 +500,7 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
     uint64_t* x_made = done + 2;          // XIN: the terms are in shared memory
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(x_made + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    uint32_t* row_top = tmem_slot + 2;    // [ROWS], XIN
+    uint32_t* row_top = tmem_slot + 2;    // [ROWS]: XIN, top magnitudes; else the rows' unscale
 
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int tile = static_cast<int>(blockIdx.x) / a.S, ks = static_cast<int>(blockIdx.x) % a.S;
@@ -623,9 +627,13 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
         float s_prev[C::SUB];
         int u = 0;  // units of this warpgroup so far
         bool ok = true;
+        int at = wg, phase = 0;  // ring position of block p
         for (int p = wg; ok && p < np; p += 2) {
-            const uint8_t* st = ring + p % C::NS * C::STAGE;
-            if (!(ok = wait(&in_full[p % C::NS], p / C::NS))) break;
+            const uint8_t* st = ring + at * C::STAGE;
+            if (!(ok = wait(&in_full[at], phase))) break;
+            uint64_t* empty = &in_empty[at];
+            uint64_t* before = &in_empty[at >= 2 ? at - 2 : at + C::NS - 2];
+            if ((at += 2) >= C::NS) at -= C::NS, phase ^= 1;
             float s[C::FULL];
 #pragma unroll
             for (int j = 0; j < C::FULL; ++j)
@@ -647,14 +655,14 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
                 }
                 if (C::XIN && j == 128 / C::UK - 1) {  // the stage held weights only: it is free
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&in_empty[p % C::NS]);
+                    if (lane == 0) mbar_arrive(empty);
                 }
                 if (u) {
                     // the unit before is done: its weights' columns, its
                     // accumulators and (at a block's start) its stage are free
                     if (!(ok = wait(&done[wg], u - 1))) break;
                     tc_fence_after();
-                    if (!C::XIN && j == 0 && lane == 0) mbar_arrive(&in_empty[(p - 2) % C::NS]);
+                    if (!C::XIN && j == 0 && lane == 0) mbar_arrive(before);
                     if (C::ND == 1) take(u - 1, s_prev);
                 }
                 if constexpr (C::UA == 32)
@@ -679,10 +687,12 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
         const uint32_t idesc = idesc_e4m3_e5m2_f32(128, static_cast<uint32_t>((rows * TN + 15) & ~15));
         int u = 0;
         bool ok = !C::XIN || wait(x_made, 0);
+        int at = wg, phase = 0;
         for (int p = wg; ok && p < np; p += 2) {
-            if (!C::XIN && !(ok = wait(&in_full[p % C::NS], p / C::NS))) break;
+            if (!C::XIN && !(ok = wait(&in_full[at], phase))) break;
             const uint64_t bd = smem_desc_sw128(
-                smem_u32(C::XIN ? xres + p * C::XSTEP : ring + p % C::NS * C::STAGE + C::STAGE - C::XB));
+                smem_u32(C::XIN ? xres + p * C::XSTEP : ring + at * C::STAGE + C::STAGE - C::XB));
+            if ((at += 2) >= C::NS) at -= C::NS, phase ^= 1;
 #pragma unroll
             for (int j = 0; j < 128 / C::UK; ++j) {
                 if (!(ok = wait(&a_full[wg], u))) break;
@@ -699,10 +709,13 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
                 ++u;
             }
         }
-    } else if (lane == 0 && (w == 10 || !C::XIN)) {
+    } else if (w == 10 || !C::XIN) {
         const bool weights = w == 10;
-        if (!weights) asm volatile("griddepcontrol.wait;" ::: "memory");  // x is the terms kernel's
-        int p = weights ? min(np, C::NS) : 0;
+        if (!weights) {  // x and its unscale are the terms kernel's
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            if (lane < rows) row_top[lane] = __float_as_uint(a.unscale[m0 + lane]);
+        }
+        int p = lane != 0 ? np : weights ? min(np, C::NS) : 0;
         for (; p < np; ++p) {
             uint64_t* full = &in_full[p % C::NS];
             if (!mbar_wait_bounded(&in_empty[p % C::NS], (p / C::NS & 1) ^ 1, abort_flag, a.err, ERR_GEMM_TIMEOUT))
@@ -715,7 +728,7 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
                             static_cast<int>(m0 * TN), 0);
             }
         }
-        if (*abort_flag)  // a failed call leaves no copy in flight behind (bounded as well)
+        if (lane == 0 && *abort_flag)  // a failed call leaves no copy in flight behind (bounded as well)
             for (int i = max(0, p - C::NS); i < p; ++i)
                 for (int t = 0; t < 1 << 14 && !mbar_try_wait(&in_full[i % C::NS], i / C::NS & 1); ++t) {
                 }
@@ -734,33 +747,33 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
             if (c < rows) fin[c * 128 + ch] = acc[c];
     __syncthreads();
     if (a.S > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-    const int share = (rows * 128 + a.S - 1) / a.S;  // outputs that a rank writes
-    if (w < 4)
+    const int share = (rows + a.S - 1) / a.S;  // rows that a rank writes
+    const int64_t n = tile * 128ll + ch;
+    if (w < 4) {
+        int to = 0, r = 0;  // row c is row r of rank `to`
 #pragma unroll
         for (int c = 0; c < ROWS; ++c) {
             if (c >= rows) continue;
             float v = acc[c] + fin[c * 128 + ch];
-            if (C::XIN) v *= unscale_of(row_top[c]);
-            const int i = c * 128 + ch, to = i / share;
-            const float* p = recv + ks * share + i - to * share;
+            v *= C::XIN ? unscale_of(row_top[c]) : __uint_as_float(row_top[c]);
+            if (a.S == 1) {
+                if (n < a.N) store_out(a, m0 + c, n, v);
+                continue;
+            }
+            float* p = recv + (ks * share + r) * 128 + ch;
             if (to == ks)
-                recv[ks * share + i - to * share] = v;
+                *p = v;
             else
                 st_cluster(p, to, v);
+            if (++r == share) r = 0, ++to;
         }
-    if (a.S > 1)
-        cluster_sync();
-    else
-        __syncthreads();
-    if (!C::XIN) asm volatile("griddepcontrol.wait;" ::: "memory");  // unscale is the terms kernel's
-    for (int j = threadIdx.x; j < share; j += kQ4Threads) {
-        const int i = ks * share + j, r = i >> 7;
-        if (r >= rows) break;
+    }
+    if (a.S == 1) return;
+    cluster_sync();
+    for (int r = threadIdx.x >> 7; r < share && ks * share + r < rows; r += kQ4Threads / 128) {
         float v = 0.0f;
-        for (int s = 0; s < a.S; ++s) v += recv[s * share + j];
-        if (!C::XIN) v *= a.unscale[m0 + r];
-        const int64_t n = tile * 128ll + (i & 127);
-        if (n < a.N) store_out(a, m0 + r, n, v);
+        for (int s = 0; s < a.S; ++s) v += recv[(s * share + r) * 128 + ch];
+        if (n < a.N) store_out(a, m0 + ks * share + r, n, v);
     }
 }
 
@@ -892,7 +905,8 @@ aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, const XT* x
     auto* unscale = reinterpret_cast<float*>(terms + static_cast<size_t>(a.M) * kTerms<XT> * w->NP * 128);
     a.unscale = unscale;
     const int tn = F32 ? 16 / a.rows : 1;
-    q4_terms_kernel<XT><<<static_cast<unsigned>(a.M), 1024, 0, s>>>(x, a.ldx, w->K, w->NP * 128, tn, a.vec, terms,
+    const int threads = w->K <= 2048 ? 128 : w->K <= 4096 ? 256 : 1024;  // 16 k a thread
+    q4_terms_kernel<XT><<<static_cast<unsigned>(a.M), threads, 0, s>>>(x, a.ldx, w->K, w->NP * 128, tn, a.vec, terms,
                                                                     unscale);
     count_launches(1);
     const cudaError_t e = cudaGetLastError();
