@@ -223,18 +223,22 @@ constexpr int kTerms = sizeof(XT) == 4 ? 8 : 3;
 template <typename XT>
 struct Four {
     uint32_t w[sizeof(XT)];
-    __device__ __forceinline__ void load(const XT* row, int64_t k, int64_t K, bool vec) {
-        if (vec && k + 4 <= K) {
-            if constexpr (sizeof(XT) == 4) {
+    // VEC: rows of 4-element vectors, K a multiple of 4
+    template <bool VEC>
+    __device__ __forceinline__ void load(const XT* row, int64_t k, int64_t K) {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(XT)); ++i) w[i] = 0;
+        if constexpr (VEC && sizeof(XT) == 4) {
+            if (k < K) {
                 const uint4 u = *reinterpret_cast<const uint4*>(row + k);
                 w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
-            } else {
+            }
+        } else if constexpr (VEC) {
+            if (k < K) {
                 const uint2 u = *reinterpret_cast<const uint2*>(row + k);
                 w[0] = u.x, w[1] = u.y;
             }
         } else {
-#pragma unroll
-            for (int i = 0; i < static_cast<int>(sizeof(XT)); ++i) w[i] = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (k + i < K) {
@@ -319,9 +323,9 @@ __device__ __forceinline__ void terms4(const Four<XT>& x, int up, uint32_t (&t)[
 
 // Activations as the products read them, one block per row: bytes
 // [terms / tn][M][tn][KP] (KP = K rounded up to 128, zero padded), unscale [M].
-template <typename XT>
+template <typename XT, bool VEC>
 __global__ void __launch_bounds__(1024)
-    q4_terms_kernel(const XT* __restrict__ x, int64_t ldx, int64_t K, int64_t KP, int tn, bool vec,
+    q4_terms_kernel(const XT* __restrict__ x, int64_t ldx, int64_t K, int64_t KP, int tn,
                     uint8_t* __restrict__ out, float* __restrict__ unscale) {
     constexpr int TERMS = kTerms<XT>, HELD = 4;  // 16 k a thread stay in registers
     const int64_t nt = blockDim.x;
@@ -333,12 +337,12 @@ __global__ void __launch_bounds__(1024)
     Four<XT> v[HELD];
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) v[i].load(row, (i * nt + threadIdx.x) * 4, K, vec);
+    for (int i = 0; i < HELD; ++i) v[i].template load<VEC>(row, (i * nt + threadIdx.x) * 4, K);
 #pragma unroll
     for (int i = 0; i < HELD; ++i) top = max(top, v[i].top());
     for (int64_t k = (HELD * nt + threadIdx.x) * 4; k < K; k += nt * 4) {
         Four<XT> u;
-        u.load(row, k, K, vec);
+        u.template load<VEC>(row, k, K);
         top = max(top, u.top());
     }
     top = __reduce_max_sync(~0u, top);
@@ -362,7 +366,7 @@ __global__ void __launch_bounds__(1024)
     }
     for (int64_t k = (HELD * nt + threadIdx.x) * 4; k < KP; k += nt * 4) {
         Four<XT> u;
-        u.load(row, k, K, vec);
+        u.template load<VEC>(row, k, K);
         put(k, u);
     }
 }
@@ -439,7 +443,7 @@ struct Q4Cfg {
     static constexpr bool XIN = TK == 1;
     static constexpr int TW = 128;                     // TMEM columns of a warpgroup: 4 per SM
     static constexpr int FULL = GS == 128 ? 1 : 128 / GS;  // scale groups of a block
-    static constexpr int UK = 32 + 2 * FULL * COLS <= TW ? 128 : 64;  // k of a unit
+    static constexpr int UK = 32 + FULL * COLS <= TW ? 128 : 64;  // k of a unit
     static constexpr int SUB = UK < GS ? 1 : UK / GS;  // accumulators per unit
     static constexpr int UA = UK / 4;                  // columns of a unit's weights
     static constexpr int ND = UA + 2 * SUB * COLS <= TW ? 2 : 1;  // accumulator buffers
@@ -462,7 +466,7 @@ struct Q4Cfg {
     static constexpr int SMEM = USED > 78 * 1024 ? USED : 78 * 1024;
     static_assert(UA + ND * SUB * COLS <= TW && NS >= 4 && SMEM <= 113 * 1024, "budgets");
     static_assert(ROWS * TN <= COLS && (UK >= GS || UK == 128), "a scale group inside a unit");
-    static_assert(STAGE * NS >= ROWS * 512, "a warpgroup's sums fit the ring");
+    static_assert(STAGE * NS >= ROWS * 1024, "the warpgroups' sums fit the ring");
 };
 constexpr int kQ4Threads = 12 * 32;
 
@@ -516,13 +520,19 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
     if (C::XIN && w < 8) {
         const XT* x = static_cast<const XT*>(a.x) + m0 * a.ldx + static_cast<int64_t>(p0) * 128 + lane * 4;
         const int64_t left = a.K - static_cast<int64_t>(p0) * 128 - lane * 4;
-        int r = 0, p = w;
+        auto load = [&](auto vec) {
+            int r = 0, p = w;
 #pragma unroll
-        for (int h = 0; h < HELD; ++h, p += 8) {
-            while (p >= np) p -= np, ++r;
-            if (r >= rows) break;
-            xv[h].load(x + r * a.ldx, p * 128, left, a.vec);
-        }
+            for (int h = 0; h < HELD; ++h, p += 8) {
+                while (p >= np) p -= np, ++r;
+                if (r >= rows) break;
+                xv[h].template load<decltype(vec)::value>(x + r * a.ldx, p * 128, left);
+            }
+        };
+        if (a.vec)
+            load(std::true_type{});
+        else
+            load(std::false_type{});
     }
     const uint8_t* src = a.w + ((g * a.NC + tile) * a.NP + p0) * static_cast<int64_t>(a.block);
     auto copy_weights = [&](int p) {
@@ -642,17 +652,23 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
                            : reinterpret_cast<const float*>(st + 8192)[j * 128 + ch];
 #pragma unroll
             for (int j = 0; j < 128 / C::UK; ++j) {
+                uint4 q[C::UK / 32];
+#pragma unroll
+                for (int i = 0; i < C::UK / 32; ++i)
+                    q[i] = *reinterpret_cast<const uint4*>(st + (j * (C::UK / 32) + i) * 2048 + ch * 16);
                 uint32_t v[C::UA];
+                auto unpack = [&]() {
 #pragma unroll
-                for (int i = 0; i < C::UK / 32; ++i) {
-                    const uint4 q = *reinterpret_cast<const uint4*>(st + (j * (C::UK / 32) + i) * 2048 + ch * 16);
-                    const uint32_t word[4] = {q.x, q.y, q.z, q.w};
+                    for (int i = 0; i < C::UK / 32; ++i) {
+                        const uint32_t word[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        v[8 * i + 2 * e] = word[e] & 0x87878787u;
-                        v[8 * i + 2 * e + 1] = __funnelshift_r(word[e], word[e], 4) & 0x87878787u;
+                        for (int e = 0; e < 4; ++e) {
+                            v[8 * i + 2 * e] = word[e] & 0x87878787u;
+                            v[8 * i + 2 * e + 1] = __funnelshift_r(word[e], word[e], 4) & 0x87878787u;
+                        }
                     }
-                }
+                };
+                if (C::ND == 2) unpack();
                 if (C::XIN && j == 128 / C::UK - 1) {  // the stage held weights only: it is free
                     __syncwarp();
                     if (lane == 0) mbar_arrive(empty);
@@ -665,6 +681,7 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
                     if (!C::XIN && j == 0 && lane == 0) mbar_arrive(before);
                     if (C::ND == 1) take(u - 1, s_prev);
                 }
+                if (C::ND == 1) unpack();
                 if constexpr (C::UA == 32)
                     tc_st_32x32b_x32(ta + quarter, v);
                 else
@@ -740,33 +757,27 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
     __syncthreads();
     tc_fence_after();
     if (w == 9) tmem_dealloc(tmem, 2 * C::TW);
-    float* fin = reinterpret_cast<float*>(ring);  // [ROWS][128]: the second warpgroup's sums
-    if (w >= 4 && w < 8)
+    // (This end runs once per CTA, from a cold instruction cache: the sums leave
+    // the registers in one short unrolled piece and the rest is a loop.)
+    float* fin = reinterpret_cast<float*>(ring);  // [2][ROWS][128]: the warpgroups' sums
+    if (w < 8)
 #pragma unroll
-        for (int c = 0; c < ROWS; ++c)
-            if (c < rows) fin[c * 128 + ch] = acc[c];
+        for (int c = 0; c < ROWS; ++c) fin[(wg * ROWS + c) * 128 + ch] = acc[c];
     __syncthreads();
     if (a.S > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     const int share = (rows + a.S - 1) / a.S;  // rows that a rank writes
     const int64_t n = tile * 128ll + ch;
-    if (w < 4) {
-        int to = 0, r = 0;  // row c is row r of rank `to`
-#pragma unroll
-        for (int c = 0; c < ROWS; ++c) {
-            if (c >= rows) continue;
-            float v = acc[c] + fin[c * 128 + ch];
-            v *= C::XIN ? unscale_of(row_top[c]) : __uint_as_float(row_top[c]);
-            if (a.S == 1) {
-                if (n < a.N) store_out(a, m0 + c, n, v);
-                continue;
-            }
-            float* p = recv + (ks * share + r) * 128 + ch;
-            if (to == ks)
-                *p = v;
-            else
-                st_cluster(p, to, v);
-            if (++r == share) r = 0, ++to;
-        }
+    for (int c = w >> 2, to = 0, r = c; c < rows; c += kQ4Threads / 128, r += kQ4Threads / 128) {
+        while (r >= share) r -= share, ++to;  // row c is row r of rank `to`
+        float v = fin[c * 128 + ch] + fin[(ROWS + c) * 128 + ch];
+        v *= C::XIN ? unscale_of(row_top[c]) : __uint_as_float(row_top[c]);
+        float* p = recv + (ks * share + r) * 128 + ch;
+        if (a.S > 1 && to != ks)
+            st_cluster(p, to, v);
+        else if (a.S > 1)
+            *p = v;
+        else if (n < a.N)
+            store_out(a, m0 + c, n, v);
     }
     if (a.S == 1) return;
     cluster_sync();
@@ -882,7 +893,7 @@ aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, const XT* x
     a.NP = static_cast<int>(w->NP);
     a.x = x;
     a.err = device_error_word(w->device);
-    a.vec = reinterpret_cast<uintptr_t>(x) % (4 * sizeof(XT)) == 0 && a.ldx % 4 == 0;
+    a.vec = reinterpret_cast<uintptr_t>(x) % (4 * sizeof(XT)) == 0 && a.ldx % 4 == 0 && a.K % 4 == 0;
     AEM_REQUIRE(a.M * kTerms<XT> < (1ll << 31), "%s: M=%lld out of range", what, (long long)a.M);
     const Q4Plan plan = q4_plan(w, F32, a.M, a.group_rows != nullptr);
     const size_t need = q4_workspace(w, F32, a.M, a.group_rows != nullptr);
@@ -906,8 +917,8 @@ aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, const XT* x
     a.unscale = unscale;
     const int tn = F32 ? 16 / a.rows : 1;
     const int threads = w->K <= 2048 ? 128 : w->K <= 4096 ? 256 : 1024;  // 16 k a thread
-    q4_terms_kernel<XT><<<static_cast<unsigned>(a.M), threads, 0, s>>>(x, a.ldx, w->K, w->NP * 128, tn, a.vec, terms,
-                                                                    unscale);
+    auto make_terms = a.vec ? q4_terms_kernel<XT, true> : q4_terms_kernel<XT, false>;
+    make_terms<<<static_cast<unsigned>(a.M), threads, 0, s>>>(x, a.ldx, w->K, w->NP * 128, tn, terms, unscale);
     count_launches(1);
     const cudaError_t e = cudaGetLastError();
     aem_status st;
