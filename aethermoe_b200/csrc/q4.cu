@@ -454,19 +454,22 @@ struct Q4Cfg {
     static constexpr int XSTEP = ROWS * TN <= 8 ? 1024 : XB;
     static constexpr int MAXP = XSTEP == 1024 ? 32 : 24;  // XIN: blocks whose terms are kept
     static constexpr int XRES = XIN ? MAXP * XSTEP : 0;
-    static constexpr int STAGE = (XIN ? 0 : XB) + 8192 + (FULL * 512 + 1023) / 1024 * 1024;
+    static constexpr int WB = 8192 + (FULL * 512 + 1023) / 1024 * 1024;  // a block of weights and scales
     // the cluster's sums: S shares of ceil(rows / S) rows, for any S up to 8
     static constexpr int RECV = (ROWS < 8 ? 8 : ROWS < 16 ? 14 : ROWS < 32 ? 21 : 36) * 128 * 4;
-    // an even ring: a stage always comes back to the warpgroup that saw its
-    // previous phase, so no parity wait can mistake a phase for the one two back
-    static constexpr int FIT = (113 * 1024 - 2048 - XRES - RECV) / STAGE / 2 * 2;
-    static constexpr int NS = FIT > 8 ? 8 : FIT;
-    static constexpr int USED = 1024 + NS * STAGE + XRES + RECV + (2 * NS + 5) * 8 + 16 + ROWS * 4;
+    // Even rings: a stage always comes back to the warpgroup that saw its
+    // previous phase, so no parity wait can mistake a phase for the one two
+    // back.  Activations stay in theirs until the MMAs are done, weights only
+    // until they are read.
+    static constexpr int NX = XIN ? 0 : 4;
+    static constexpr int FIT = (113 * 1024 - 2048 - XRES - RECV - NX * XB) / WB / 2 * 2;
+    static constexpr int NW = FIT > 8 ? 8 : FIT;
+    static constexpr int USED = 1024 + NW * WB + NX * XB + XRES + RECV + (2 * (NW + NX) + 5) * 8 + 16 + ROWS * 4;
     // two CTAs on an SM, never three: no CTA ever waits for tensor memory
     static constexpr int SMEM = USED > 78 * 1024 ? USED : 78 * 1024;
-    static_assert(UA + ND * SUB * COLS <= TW && NS >= 4 && SMEM <= 113 * 1024, "budgets");
+    static_assert(UA + ND * SUB * COLS <= TW && NW >= 4 && SMEM <= 113 * 1024, "budgets");
     static_assert(ROWS * TN <= COLS && (UK >= GS || UK == 128), "a scale group inside a unit");
-    static_assert(STAGE * NS >= ROWS * 1024, "the warpgroups' sums fit the ring");
+    static_assert(NW * WB >= ROWS * 1024, "the warpgroups' sums fit the ring");
 };
 constexpr int kQ4Threads = 12 * 32;
 
@@ -495,17 +498,21 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
     extern __shared__ uint8_t smem_raw[];
     uint8_t* xres = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                ~static_cast<uintptr_t>(1023));
-    uint8_t* ring = xres + C::XRES;
-    float* recv = reinterpret_cast<float*>(ring + C::NS * C::STAGE);  // [S][share of ROWS * 128]
-    uint64_t* in_full = reinterpret_cast<uint64_t*>(recv + C::RECV / 4);
-    uint64_t* in_empty = in_full + C::NS;
-    uint64_t* a_full = in_empty + C::NS;  // [2]: a unit's weights are in tensor memory
+    uint8_t* xring = xres + C::XRES;
+    uint8_t* ring = xring + C::NX * C::XB;
+    float* recv = reinterpret_cast<float*>(ring + C::NW * C::WB);  // [S][share of ROWS * 128]
+    uint64_t* w_full = reinterpret_cast<uint64_t*>(recv + C::RECV / 4);
+    uint64_t* w_empty = w_full + C::NW;
+    uint64_t* x_full = w_empty + C::NW;
+    uint64_t* x_empty = x_full + C::NX;
+    uint64_t* a_full = x_empty + C::NX;   // [2]: a unit's weights are in tensor memory
     uint64_t* done = a_full + 2;          // [2]: its MMAs have finished
     uint64_t* x_made = done + 2;          // XIN: the terms are in shared memory
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(x_made + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     uint32_t* row_top = tmem_slot + 2;    // [ROWS]: XIN, top magnitudes; else the rows' unscale
 
+    constexpr int NX = C::XIN ? 1 : C::NX;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int tile = static_cast<int>(blockIdx.x) / a.S, ks = static_cast<int>(blockIdx.x) % a.S;
     int64_t g, m0;
@@ -536,18 +543,22 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
     }
     const uint8_t* src = a.w + ((g * a.NC + tile) * a.NP + p0) * static_cast<int64_t>(a.block);
     auto copy_weights = [&](int p) {
-        uint64_t* full = &in_full[p % C::NS];
+        uint64_t* full = &w_full[p % C::NW];
         mbar_arrive_expect_tx(full, a.block);
-        bulk_load(ring + p % C::NS * C::STAGE, src + static_cast<int64_t>(p) * a.block, a.block, full);
+        bulk_load(ring + p % C::NW * C::WB, src + static_cast<int64_t>(p) * a.block, a.block, full);
     };
     if (w == 9) {
         tmem_alloc(tmem_slot, 2 * C::TW);
         tmem_relinquish();
     } else if (w == 10 && lane == 0) {
         // the first weights are on their way before the rest of the set-up
-        for (int i = 0; i < C::NS; ++i) {
-            mbar_init(&in_full[i], C::XIN ? 1 : 2);  // the copies
-            mbar_init(&in_empty[i], 4);              // the four warps of the block's warpgroup
+        for (int i = 0; i < C::NW; ++i) {
+            mbar_init(&w_full[i], 1);
+            mbar_init(&w_empty[i], 4);  // the four warps of the block's warpgroup
+        }
+        for (int i = 0; i < C::NX; ++i) {
+            mbar_init(&x_full[i], 1);
+            mbar_init(&x_empty[i], 4);
         }
         for (int j = 0; j < 2; ++j) {
             mbar_init(&a_full[j], 4);
@@ -556,7 +567,7 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
         mbar_init(x_made, 8);
         *abort_flag = 0;
         fence_barrier_init();
-        for (int p = 0; p < min(np, C::NS); ++p) copy_weights(p);
+        for (int p = 0; p < min(np, C::NW); ++p) copy_weights(p);
     } else if (w == 11) {
         if (C::XIN && lane < ROWS) row_top[lane] = 0;
         if (!C::XIN && lane == 0) tma_prefetch_desc(&xmap);
@@ -637,13 +648,9 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
         float s_prev[C::SUB];
         int u = 0;  // units of this warpgroup so far
         bool ok = true;
-        int at = wg, phase = 0;  // ring position of block p
         for (int p = wg; ok && p < np; p += 2) {
-            const uint8_t* st = ring + at * C::STAGE;
-            if (!(ok = wait(&in_full[at], phase))) break;
-            uint64_t* empty = &in_empty[at];
-            uint64_t* before = &in_empty[at >= 2 ? at - 2 : at + C::NS - 2];
-            if ((at += 2) >= C::NS) at -= C::NS, phase ^= 1;
+            const uint8_t* st = ring + p % C::NW * C::WB;
+            if (!(ok = wait(&w_full[p % C::NW], p / C::NW))) break;
             float s[C::FULL];
 #pragma unroll
             for (int j = 0; j < C::FULL; ++j)
@@ -653,9 +660,13 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
 #pragma unroll
             for (int j = 0; j < 128 / C::UK; ++j) {
                 uint4 q[C::UK / 32];
+                auto read = [&]() {
 #pragma unroll
-                for (int i = 0; i < C::UK / 32; ++i)
-                    q[i] = *reinterpret_cast<const uint4*>(st + (j * (C::UK / 32) + i) * 2048 + ch * 16);
+                    for (int i = 0; i < C::UK / 32; ++i)
+                        q[i] = *reinterpret_cast<const uint4*>(st + (j * (C::UK / 32) + i) * 2048 + ch * 16);
+                };
+                constexpr bool EARLY = C::ND == 2 || COLS == 16;  // the widest tile has no registers for it
+                if (EARLY) read();
                 uint32_t v[C::UA];
                 auto unpack = [&]() {
 #pragma unroll
@@ -669,19 +680,26 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
                     }
                 };
                 if (C::ND == 2) unpack();
-                if (C::XIN && j == 128 / C::UK - 1) {  // the stage held weights only: it is free
+                if (C::ND == 2 && j == 128 / C::UK - 1) {  // the block has been read
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(empty);
+                    if (lane == 0) mbar_arrive(&w_empty[p % C::NW]);
                 }
                 if (u) {
                     // the unit before is done: its weights' columns, its
-                    // accumulators and (at a block's start) its stage are free
+                    // accumulators and (at a block's start) its activations are free
                     if (!(ok = wait(&done[wg], u - 1))) break;
                     tc_fence_after();
-                    if (!C::XIN && j == 0 && lane == 0) mbar_arrive(before);
+                    if (!C::XIN && j == 0 && lane == 0) mbar_arrive(&x_empty[(p - 2) % NX]);
                     if (C::ND == 1) take(u - 1, s_prev);
                 }
-                if (C::ND == 1) unpack();
+                if (C::ND == 1) {
+                    if (!EARLY) read();
+                    unpack();
+                    if (j == 128 / C::UK - 1) {
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&w_empty[p % C::NW]);
+                    }
+                }
                 if constexpr (C::UA == 32)
                     tc_st_32x32b_x32(ta + quarter, v);
                 else
@@ -704,12 +722,9 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
         const uint32_t idesc = idesc_e4m3_e5m2_f32(128, static_cast<uint32_t>((rows * TN + 15) & ~15));
         int u = 0;
         bool ok = !C::XIN || wait(x_made, 0);
-        int at = wg, phase = 0;
         for (int p = wg; ok && p < np; p += 2) {
-            if (!C::XIN && !(ok = wait(&in_full[at], phase))) break;
-            const uint64_t bd = smem_desc_sw128(
-                smem_u32(C::XIN ? xres + p * C::XSTEP : ring + at * C::STAGE + C::STAGE - C::XB));
-            if ((at += 2) >= C::NS) at -= C::NS, phase ^= 1;
+            if (!C::XIN && !(ok = wait(&x_full[p % NX], p / NX))) break;
+            const uint64_t bd = smem_desc_sw128(smem_u32(C::XIN ? xres + p * C::XSTEP : xring + p % NX * C::XB));
 #pragma unroll
             for (int j = 0; j < 128 / C::UK; ++j) {
                 if (!(ok = wait(&a_full[wg], u))) break;
@@ -732,22 +747,22 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
             asm volatile("griddepcontrol.wait;" ::: "memory");
             if (lane < rows) row_top[lane] = __float_as_uint(a.unscale[m0 + lane]);
         }
-        int p = lane != 0 ? np : weights ? min(np, C::NS) : 0;
-        for (; p < np; ++p) {
-            uint64_t* full = &in_full[p % C::NS];
-            if (!mbar_wait_bounded(&in_empty[p % C::NS], (p / C::NS & 1) ^ 1, abort_flag, a.err, ERR_GEMM_TIMEOUT))
-                break;
+        const int ns = weights ? C::NW : C::NX;
+        uint64_t *full = weights ? w_full : x_full, *empty = weights ? w_empty : x_empty;
+        int p = lane != 0 ? np : weights ? min(np, C::NW) : 0;
+        for (int at = 0, phase = weights ? 0 : 1; p < np; ++p) {
+            if (!mbar_wait_bounded(&empty[at], phase, abort_flag, a.err, ERR_GEMM_TIMEOUT)) break;
             if (weights) {
                 copy_weights(p);
             } else {
-                mbar_arrive_expect_tx(full, C::XB);
-                tma_load_3d(ring + p % C::NS * C::STAGE + C::STAGE - C::XB, &xmap, full, (p0 + p) * 128,
-                            static_cast<int>(m0 * TN), 0);
+                mbar_arrive_expect_tx(&full[at], C::XB);
+                tma_load_3d(xring + at * C::XB, &xmap, &full[at], (p0 + p) * 128, static_cast<int>(m0 * TN), 0);
             }
+            if (++at == ns) at = 0, phase ^= 1;
         }
         if (lane == 0 && *abort_flag)  // a failed call leaves no copy in flight behind (bounded as well)
-            for (int i = max(0, p - C::NS); i < p; ++i)
-                for (int t = 0; t < 1 << 14 && !mbar_try_wait(&in_full[i % C::NS], i / C::NS & 1); ++t) {
+            for (int i = max(0, p - ns); i < p; ++i)
+                for (int t = 0; t < 1 << 14 && !mbar_try_wait(&full[i % ns], i / ns & 1); ++t) {
                 }
     }
 
