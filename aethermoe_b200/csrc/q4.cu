@@ -213,7 +213,7 @@ struct Q4Args {
     int64_t group;
     int* err;
     int NC, NP, G, block, S, rows;  // S: CTAs (one cluster) that split K; rows: rows of a row tile
-    bool scale_bf16, out_bf16, relu, vec;  // vec: x can be read in vectors of 4
+    bool scale_bf16, out_bf16, relu, vec, ovec;  // vec, ovec: x, out can be moved in vectors of 4
 };
 
 template <typename XT>
@@ -253,6 +253,17 @@ struct Four {
         if constexpr (sizeof(XT) == 4) return __uint_as_float(w[i]);
         return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
     }
+    // Running maximum of the magnitudes, non-finite ones included, in any form
+    // that special() and bits() read.
+    __device__ __forceinline__ void any_top(uint32_t& m) const {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(XT)); ++i)
+            m = sizeof(XT) == 4 ? max(m, w[i] & 0x7fffffffu) : __vmaxu2(m, w[i] & 0x7fff7fffu);
+    }
+    __device__ static __forceinline__ uint32_t bits(uint32_t m) {
+        return sizeof(XT) == 4 ? m : max(m << 16, m & 0xffff0000u);
+    }
+    __device__ static __forceinline__ bool special(uint32_t m) { return bits(m) >= 0x7f800000u; }
     // Bits of the largest finite magnitude (they order as the magnitudes do).
     __device__ __forceinline__ uint32_t top() const {
         uint32_t m = 0;
@@ -321,26 +332,33 @@ __device__ __forceinline__ void terms4(const Four<XT>& x, int up, uint32_t (&t)[
     t[0] |= special;
 }
 
-// Activations as the products read them, one block per row: bytes
-// [terms / tn][M][tn][KP] (KP = K rounded up to 128, zero padded), unscale [M].
+// Activations as the products read them: bytes [terms / tn][M][tn][KP] (KP = K
+// rounded up to 128, zero padded), unscale [M].  gridDim.y blocks share a row:
+// each reads all of it for the largest magnitude and turns its slots (4 k a
+// thread) into terms.
 template <typename XT, bool VEC>
-__global__ void __launch_bounds__(1024)
+__global__ void __launch_bounds__(512)
     q4_terms_kernel(const XT* __restrict__ x, int64_t ldx, int64_t K, int64_t KP, int tn,
                     uint8_t* __restrict__ out, float* __restrict__ unscale) {
-    constexpr int TERMS = kTerms<XT>, HELD = 4;  // 16 k a thread stay in registers
-    const int64_t nt = blockDim.x;
+    constexpr int TERMS = kTerms<XT>, HELD = 8;  // slots that stay in registers
+    const int nt = blockDim.x, P = gridDim.y, y = blockIdx.y;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    __shared__ uint32_t tops[32];
-    if (threadIdx.x < 32) tops[threadIdx.x] = 0;
-    __syncthreads();
+    __shared__ uint32_t tops[16];
     const XT* row = x + blockIdx.x * ldx;
     Four<XT> v[HELD];
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) v[i].template load<VEC>(row, (i * nt + threadIdx.x) * 4ll, K);
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) v[i].template load<VEC>(row, (i * nt + threadIdx.x) * 4, K);
+    for (int i = 0; i < HELD; ++i) v[i].any_top(top);
+    if (Four<XT>::special(top)) {
+        top = 0;
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) top = max(top, v[i].top());
-    for (int64_t k = (HELD * nt + threadIdx.x) * 4; k < K; k += nt * 4) {
+        for (int i = 0; i < HELD; ++i) top = max(top, v[i].top());
+    } else {
+        top = Four<XT>::bits(top);
+    }
+    for (int64_t k = (HELD * nt + threadIdx.x) * 4ll; k < K; k += nt * 4) {
         Four<XT> u;
         u.template load<VEC>(row, k, K);
         top = max(top, u.top());
@@ -348,9 +366,9 @@ __global__ void __launch_bounds__(1024)
     top = __reduce_max_sync(~0u, top);
     if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
     __syncthreads();
-    top = __reduce_max_sync(~0u, tops[threadIdx.x & 31]);
+    top = __reduce_max_sync(~0u, tops[threadIdx.x & (nt / 32 - 1)]);
     const int up = rho_exponent(top);
-    if (threadIdx.x == 0) unscale[blockIdx.x] = unscale_of(top);
+    if (threadIdx.x == 0 && y == 0) unscale[blockIdx.x] = unscale_of(top);
     auto put = [&](int64_t k, const Four<XT>& u) {
         uint32_t t[TERMS];
         terms4(u, up, t);
@@ -359,12 +377,15 @@ __global__ void __launch_bounds__(1024)
             *reinterpret_cast<uint32_t*>(
                 out + ((j / tn * static_cast<int64_t>(gridDim.x) + blockIdx.x) * tn + j % tn) * KP + k) = t[j];
     };
+    int next = y;  // this block's next slot
 #pragma unroll
     for (int i = 0; i < HELD; ++i) {
-        const int64_t k = (i * nt + threadIdx.x) * 4;
+        if (i != next) continue;
+        next += P;
+        const int64_t k = (i * nt + threadIdx.x) * 4ll;
         if (k < KP) put(k, v[i]);
     }
-    for (int64_t k = (HELD * nt + threadIdx.x) * 4; k < KP; k += nt * 4) {
+    for (int64_t k = (static_cast<int64_t>(next) * nt + threadIdx.x) * 4; k < KP; k += P * nt * 4ll) {
         Four<XT> u;
         u.template load<VEC>(row, k, K);
         put(k, u);
@@ -418,16 +439,44 @@ __device__ __forceinline__ bool find_rows(const Q4Args& a, int slot, int64_t* g,
     return false;
 }
 
-__device__ __forceinline__ void st_cluster(const float* p, uint32_t rank, float v) {
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_u32(p, rank)), "f"(v) : "memory");
+__device__ __forceinline__ void st_cluster(const float4* p, uint32_t rank, float4 v) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(mapa_u32(p, rank)), "f"(v.x),
+                 "f"(v.y), "f"(v.z), "f"(v.w)
+                 : "memory");
 }
 
-__device__ __forceinline__ void store_out(const Q4Args& a, int64_t m, int64_t n, float v) {
-    if (a.relu && v < 0.0f) v = 0.0f;
-    if (a.out_bf16)
-        static_cast<__nv_bfloat16*>(a.out)[m * a.ldo + n] = __float2bfloat16_rn(v);
-    else
-        static_cast<float*>(a.out)[m * a.ldo + n] = v;
+__device__ __forceinline__ void store_out(const Q4Args& a, int64_t m, int64_t n, float4 v) {
+    if (a.relu) {
+        v.x = v.x < 0.0f ? 0.0f : v.x, v.y = v.y < 0.0f ? 0.0f : v.y;
+        v.z = v.z < 0.0f ? 0.0f : v.z, v.w = v.w < 0.0f ? 0.0f : v.w;
+    }
+    const int64_t at = m * a.ldo + n;
+    if (a.ovec && n + 3 < a.N) {
+        if (a.out_bf16) {
+            __nv_bfloat162 h[2] = {__floats2bfloat162_rn(v.x, v.y), __floats2bfloat162_rn(v.z, v.w)};
+            *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + at) = *reinterpret_cast<uint2*>(h);
+        } else {
+            *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = v;
+        }
+        return;
+    }
+    const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (n + j >= a.N) return;
+        if (a.out_bf16)
+            static_cast<__nv_bfloat16*>(a.out)[at + j] = __float2bfloat16_rn(e[j]);
+        else
+            static_cast<float*>(a.out)[at + j] = e[j];
+    }
+}
+
+// a0 += s * v0, a1 += s * v1
+__device__ __forceinline__ void fma2(float& a0, float& a1, float s, uint32_t v0, uint32_t v1) {
+    asm("{\n.reg .b64 a, s, v;\nmov.b64 a, {%0, %1};\nmov.b64 s, {%2, %2};\nmov.b64 v, {%3, %4};\n"
+        "fma.rn.f32x2 a, s, v, a;\nmov.b64 {%0, %1}, a;\n}"
+        : "+f"(a0), "+f"(a1)
+        : "f"(s), "r"(v0), "r"(v1));
 }
 
 // Shape of the product kernel: COLS MMA columns, scale groups of GS k, a row's
@@ -517,7 +566,10 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
     const int tile = static_cast<int>(blockIdx.x) / a.S, ks = static_cast<int>(blockIdx.x) % a.S;
     int64_t g, m0;
     int rows;
-    if (!find_rows(a, blockIdx.y, &g, &m0, &rows)) return;  // the whole cluster alike
+    if (!find_rows(a, blockIdx.y, &g, &m0, &rows)) {  // the whole cluster alike
+        if (!C::XIN) asm volatile("griddepcontrol.wait;" ::: "memory");  // this grid ends after the terms kernel
+        return;
+    }
     const int p0 = a.NP * ks / a.S, np = a.NP * (ks + 1) / a.S - p0;
 
     // XIN: a warp takes 128 k of a row, a lane four of them.  These loads go out
@@ -637,6 +689,10 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
                 for (int i = 0; i < CH / 16 * (16 / TN); ++i) {  // 16 columns hold 16 / TN whole rows
                     const int c = i / (16 / TN) * 16 + i % (16 / TN) * TN, row = (c0 + c) % COLS / TN;
                     if (row >= ROWS) continue;
+                    if constexpr (TN == 1) {  // two rows an instruction
+                        if (i % 2 == 0) fma2(acc[row], acc[row + 1], s[(c0 + c) / COLS], r[c], r[c + 1]);
+                        continue;
+                    }
                     float v = __uint_as_float(r[c]);
 #pragma unroll
                     for (int t = 1; t < TN; ++t) v += __uint_as_float(r[c + t]);
@@ -781,25 +837,31 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
     __syncthreads();
     if (a.S > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     const int share = (rows + a.S - 1) / a.S;  // rows that a rank writes
-    const int64_t n = tile * 128ll + ch;
-    for (int c = w >> 2, to = 0, r = c; c < rows; c += kQ4Threads / 128, r += kQ4Threads / 128) {
+    const int64_t n = tile * 128ll + lane * 4;  // a warp has a row, a lane four channels of it
+    const float4* fin4 = reinterpret_cast<const float4*>(fin) + lane;
+    float4* recv4 = reinterpret_cast<float4*>(recv) + lane;
+    for (int c = w, to = 0, r = c; c < rows; c += kQ4Threads / 32, r += kQ4Threads / 32) {
         while (r >= share) r -= share, ++to;  // row c is row r of rank `to`
-        float v = fin[c * 128 + ch] + fin[(ROWS + c) * 128 + ch];
-        v *= C::XIN ? unscale_of(row_top[c]) : __uint_as_float(row_top[c]);
-        float* p = recv + (ks * share + r) * 128 + ch;
+        const float4 u = fin4[c * 32], v = fin4[(ROWS + c) * 32];
+        const float f = C::XIN ? unscale_of(row_top[c]) : __uint_as_float(row_top[c]);
+        const float4 o = make_float4((u.x + v.x) * f, (u.y + v.y) * f, (u.z + v.z) * f, (u.w + v.w) * f);
+        float4* p = recv4 + (ks * share + r) * 32;
         if (a.S > 1 && to != ks)
-            st_cluster(p, to, v);
+            st_cluster(p, to, o);
         else if (a.S > 1)
-            *p = v;
-        else if (n < a.N)
-            store_out(a, m0 + c, n, v);
+            *p = o;
+        else
+            store_out(a, m0 + c, n, o);
     }
     if (a.S == 1) return;
     cluster_sync();
-    for (int r = threadIdx.x >> 7; r < share && ks * share + r < rows; r += kQ4Threads / 128) {
-        float v = 0.0f;
-        for (int s = 0; s < a.S; ++s) v += recv[(s * share + r) * 128 + ch];
-        if (n < a.N) store_out(a, m0 + ks * share + r, n, v);
+    for (int r = w; r < share && ks * share + r < rows; r += kQ4Threads / 32) {
+        float4 v = recv4[r * 32];
+        for (int s = 1; s < a.S; ++s) {
+            const float4 u = recv4[(s * share + r) * 32];
+            v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+        }
+        store_out(a, m0 + ks * share + r, n, v);
     }
 }
 
@@ -837,15 +899,22 @@ aem_status launch_q4(const CUtensorMap& xmap, const Q4Args& a, dim3 grid, cudaSt
     return AEM_OK;
 }
 
-// CTAs (at most 8, one cluster) that split K: until they fill the SMs, by
-// waves x (a CTA's set-up and end, as long as about 14 blocks, and its blocks).
-int split_k(int64_t ctas, int64_t blocks, int64_t most_blocks) {
+// CTAs (at most 8, one cluster) that split K.  In blocks of a CTA that shares
+// its SM, a CTA's set-up and end take about 14; one with the SM to itself does
+// its blocks in 0.64 of the time and starts 1.5 sooner.  16 rows, 4096 x 4096:
+// 4 CTAs (128 in all) 9.8 us, 8 CTAs 10.8; 14336 x 4096: 4 CTAs 19.1, 8 CTAs
+// 17.2.  Wide clusters leave slots of a GPC empty, more of them while blocks of
+// the terms kernel hold some: 32 clusters of 8 took 19.4 us where 7 took 14.6
+// (14336 x 4096, 4 float32 rows), so 240 of the 296 slots are counted on (264
+// without that kernel).
+int split_k(int64_t ctas, int64_t blocks, int64_t most_blocks, bool terms) {
     int best = 8;
     int64_t least = INT64_MAX;
     for (int S = 1; S <= 8; ++S) {
-        const int64_t each = (blocks + S - 1) / S;
+        const int64_t each = (blocks + S - 1) / S, slots = S <= 4 ? 296 : terms ? 240 : 264;
         if (each > most_blocks || (S > 1 && each < 2)) continue;
-        const int64_t cost = (ctas * S + 295) / 296 * (14 + each);
+        const int64_t cost = ctas * S <= 148 ? 1400 + 64 * each
+                                             : (ctas * S + slots - 1) / slots * (1550 + 100 * each);
         if (cost < least) {
             least = cost;
             best = S;
@@ -861,7 +930,7 @@ aem_status launch_tile(const uint8_t* terms, Q4Args a, int gs, int64_t slots, cu
     const int64_t KP = a.NP * 128ll;
     if (!XIN)
         AEM_TRY(make_tmap_3d_u8(&xmap, terms, KP, a.M * TN, TK, KP, a.M * TN * KP, COLS, TK));
-    a.S = split_k(a.NC * slots, a.NP, XIN ? Q4Cfg<COLS, 128, ROWS, TN, TK>::MAXP : INT64_MAX);
+    a.S = split_k(a.NC * slots, a.NP, XIN ? Q4Cfg<COLS, 128, ROWS, TN, TK>::MAXP : INT64_MAX, !XIN);
     const dim3 grid(static_cast<unsigned>(a.NC * a.S), static_cast<unsigned>(slots));
     if (gs == 128) return launch_q4<XT, COLS, 128, ROWS, TN, TK>(xmap, a, grid, s);
     if (gs == 64) return launch_q4<XT, COLS, 64, ROWS, TN, TK>(xmap, a, grid, s);
@@ -880,11 +949,11 @@ Q4Plan q4_plan(const Q4Weight* w, bool f32, int64_t M, bool grouped) {
     const int64_t groups = std::min<int64_t>(w->G, M);
     const int64_t want = grouped ? (M + groups - 1) / groups : M;
     Q4Plan p;
-    p.few = want <= (f32 ? 2 : 5) && w->NP <= 8 * 24;
+    p.few = want <= (f32 ? 2 : 4) && w->NP <= 8 * 24;
     if (f32)
         p.rows = p.few ? (want <= 1 ? 1 : 2) : want <= 4 ? 4 : want <= 8 || w->gs == 32 ? 8 : 16;
     else
-        p.rows = p.few ? (want <= 2 ? 2 : 5) : want <= 16 ? 16 : 32;
+        p.rows = p.few ? (want <= 2 ? 2 : 4) : want <= 16 ? 16 : 32;
     return p;
 }
 size_t q4_workspace(const Q4Weight* w, bool f32, int64_t M, bool grouped) {
@@ -909,6 +978,7 @@ aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, const XT* x
     a.x = x;
     a.err = device_error_word(w->device);
     a.vec = reinterpret_cast<uintptr_t>(x) % (4 * sizeof(XT)) == 0 && a.ldx % 4 == 0 && a.K % 4 == 0;
+    a.ovec = reinterpret_cast<uintptr_t>(a.out) % (a.out_bf16 ? 8 : 16) == 0 && a.ldo % 4 == 0;
     AEM_REQUIRE(a.M * kTerms<XT> < (1ll << 31), "%s: M=%lld out of range", what, (long long)a.M);
     const Q4Plan plan = q4_plan(w, F32, a.M, a.group_rows != nullptr);
     const size_t need = q4_workspace(w, F32, a.M, a.group_rows != nullptr);
@@ -921,7 +991,7 @@ aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, const XT* x
     AEM_REQUIRE(slots <= 65535, "%s: M=%lld rows are too many for one call", what, (long long)a.M);
     if (plan.few)
         return a.rows == (F32 ? 1 : 2) ? launch_tile<XT, 16, F32 ? 1 : 2, F32 ? 8 : 3, 1>(nullptr, a, w->gs, slots, s)
-                                       : launch_tile<XT, 16, F32 ? 2 : 5, F32 ? 8 : 3, 1>(nullptr, a, w->gs, slots, s);
+                                       : launch_tile<XT, 16, F32 ? 2 : 4, F32 ? 8 : 3, 1>(nullptr, a, w->gs, slots, s);
     void* own = nullptr;
     if (!workspace) {
         AEM_TRY_CUDA(cudaMallocAsync(&own, need, s));
@@ -931,9 +1001,13 @@ aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, const XT* x
     auto* unscale = reinterpret_cast<float*>(terms + static_cast<size_t>(a.M) * kTerms<XT> * w->NP * 128);
     a.unscale = unscale;
     const int tn = F32 ? 16 / a.rows : 1;
-    const int threads = w->K <= 2048 ? 128 : w->K <= 4096 ? 256 : 1024;  // 16 k a thread
+    // at most 8 slots in registers up to K = 16384, and about two blocks an SM
+    const int threads = w->K <= 4096 ? 128 : w->K <= 8192 ? 256 : 512;
+    const int64_t slots_x = (w->NP * 32 + threads - 1) / threads;
+    const dim3 blocks(static_cast<unsigned>(a.M),
+                      static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(slots_x, 296 / a.M))));
     auto make_terms = a.vec ? q4_terms_kernel<XT, true> : q4_terms_kernel<XT, false>;
-    make_terms<<<static_cast<unsigned>(a.M), threads, 0, s>>>(x, a.ldx, w->K, w->NP * 128, tn, terms, unscale);
+    make_terms<<<blocks, threads, 0, s>>>(x, a.ldx, w->K, w->NP * 128, tn, terms, unscale);
     count_launches(1);
     const cudaError_t e = cudaGetLastError();
     aem_status st;
