@@ -14,7 +14,10 @@
 // Sums run in float32 in increasing j (over d: a fixed tree), and no kernel
 // uses floating atomics, so results do not change from call to call.  All of
 // it is bound by memory: every row crosses HBM once in each direction that
-// the formula names.
+// the formula names.  16384 tokens of 2048 bf16, 6 of 64 experts: dispatch 86.5
+// us (5.4 TB/s, six sevenths of it writes), combine 73 (6.4 TB/s), its backward
+// pass for 8191 tokens 75.5 (5.6 TB/s); for one token a call is its launch (2.9
+// us on the device).
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -29,7 +32,9 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = 8;
 // Units that one block ranks: 8 per thread.  Batches of at most kFusedUnits
-// are sorted again by every block of the moving kernel (one launch).
+// are sorted again by every block of the moving kernel, one launch instead of
+// three: 48 units of 2048 bf16 3.4 us (three kernels 6.1), 1024 units of 4096
+// 7.9 (10.5).
 constexpr int kBlockUnits = 2048, kFusedUnits = 1024;
 
 struct Ids {
@@ -161,7 +166,8 @@ __device__ __forceinline__ void move_flat(const MoveArgs& m, int64_t t0, int nt,
 }
 
 // The same for a block's own tokens: a warp per token, four vectors a lane in
-// flight, where a row has enough of them (short rows go flat).
+// flight, where a row has enough of them (short rows go flat).  At 16384 tokens
+// (above): 90 us, 100 with one vector in flight.
 template <typename V>
 __device__ __forceinline__ void move_rows(const MoveArgs& m, int64_t t0, int nt, int k,
                                           const int* dest) {
@@ -333,11 +339,12 @@ __global__ void __launch_bounds__(kThreads)
 
 // ------------------------------------------------------------------ combine
 // VE consecutive elements (8 or 4: 16 bytes of the widest type; or one) as
-// they lie in memory.  Loads are kept
-// apart from their conversion and made without conditions (a row that does
-// not count is replaced by row 0 and dropped afterwards): a load inside a
-// branch is waited for inside it, and the rows of a token would come one
-// after the other (164 instead of 88 us for the gradients below).
+// they lie in memory; with 8 float32 elements a lane, two loads half a line
+// apart, dispatch's backward pass took 40.2 us instead of 34.4.  Loads are kept
+// apart from their conversion and made without conditions (a row that does not
+// count is replaced by row 0 and dropped afterwards): a load inside a branch is
+// waited for inside it, and the rows of a token would come one after the other
+// (the backward pass 163 us instead of 76, the forward one 87 instead of 77).
 template <typename T, int VE>
 struct Vec {
     static constexpr int W = VE == 1 ? 1 : VE * static_cast<int>(sizeof(T)) / 4;
@@ -419,7 +426,8 @@ struct CombineArgs {
 };
 
 // One thread per (token, vector): tpt threads of a block share a token, KB
-// units' rows are in flight at a time.
+// units' rows are in flight at a time.  At most 16 blocks an SM, which go on to
+// further tokens: 72.6 us (16384 tokens), 76.1 with 64 blocks an SM.
 template <typename RT, typename OT, int VE, int KB>
 __global__ void __launch_bounds__(kThreads) combine_units_kernel(CombineArgs a, int tpt) {
     const int per = kThreads / tpt, lane = threadIdx.x % tpt;
@@ -536,7 +544,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(RT) == 2 ? 3 : 2) combine_gra
 }
 
 // ------------------------------------------------------------------ host side
-struct Plan {  // chunks of the three-kernel sort
+// Chunks of the three-kernel sort: about 8 a SM.  16384 tokens: 86 us, 92.5
+// with 4 (the last ones run alone), 90 with 16 (more to scan).
+struct Plan {
     int tc = 0, C = 0;
 };
 Plan plan_of(int64_t T, int k) {

@@ -22,11 +22,16 @@
 // accumulators in TMEM), and the scales multiply them in float32: no rounded
 // weight ever exists.
 //
-// What bounds it is the weight stream, K*N/2 bytes plus the scales.  Forms
-// that could not keep up with it (4096 x 14336, 1 row): warp MMAs (mma.sync
-// m16n8k16 occupies its sub-core's tensor pipe for 32 cycles: 16.6 us, 47.6
-// for 64 rows), and bf16 operands for tcgen05 (7 logic operations and 4
-// subtractions per 8 weights, the logic pipe the bound: 17.3 us).
+// What has to be moved is the weight stream, K*N/2 bytes plus the scales.
+// 4096 x 14336, groups of 128, one bf16 row: 10.9 us, 2.8 TB/s of that stream
+// (about 2 us to the first product, 4 of products at the memory's rate, 1.5 of
+// sums between CTAs, the rest the launch).  64 rows of 14336 x 4096, groups of
+// 64: 25.6 us, where taking the sums back from tensor memory and the latency
+// from one unit to the next bound it.  Forms that could not keep up (4096 x
+// 14336, one row): warp MMAs (mma.sync m16n8k16 occupies its sub-core's tensor
+// pipe for 32 cycles: 16.6 us, 47.6 for 64 rows), and bf16 operands for tcgen05
+// (7 logic operations and 4 subtractions per 8 weights, the logic pipe the
+// bound: 17.3 us).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -70,7 +75,8 @@ constexpr int kThreads = 256;  // pack
 // w * (1 / scale) is within 2^-20 of it, so the division itself is only made
 // where the product lies that near a half.  Adding 1.5 * 2^23 rounds to a
 // whole number, ties to even, and leaves it in the low byte (the conversion
-// instructions run at a quarter of the rate).
+// instructions run at a quarter of the rate).  Memory bound: 14336 x 4096
+// float32, groups of 128, 57 us = 5.2 TB/s; with a division per element 103.
 constexpr float kRint = 12582912.0f;
 template <typename WT, typename ST, int GS, bool VEC>
 __global__ void __launch_bounds__(4 * GS, GS == 128 ? 2 : 1)
@@ -154,6 +160,8 @@ __global__ void __launch_bounds__(4 * GS, GS == 128 ? 2 : 1)
 }
 
 // ------------------------------------------------------------------ pack
+// Once per weight: a thread gathers the 32 k of one channel, lanes lie along
+// the channels.
 __global__ void __launch_bounds__(kThreads)
     pack_q4_kernel(const int8_t* __restrict__ q, int64_t K, int64_t N, int64_t NC, int64_t NP,
                    int64_t pieces, int block, uint8_t* __restrict__ out, int* err) {
@@ -335,7 +343,9 @@ __device__ __forceinline__ void terms4(const Four<XT>& x, int up, uint32_t (&t)[
 // Activations as the products read them: bytes [terms / tn][M][tn][KP] (KP = K
 // rounded up to 128, zero padded), unscale [M].  gridDim.y blocks share a row:
 // each reads all of it for the largest magnitude and turns its slots (4 k a
-// thread) into terms.
+// thread) into terms.  32 rows of 14336: done 2.4 us after the first block's
+// start; one block of 1024 threads a row took 4.3 and kept whole SMs from the
+// product's CTAs.
 template <typename XT, bool VEC>
 __global__ void __launch_bounds__(512)
     q4_terms_kernel(const XT* __restrict__ x, int64_t ldx, int64_t K, int64_t KP, int tn,
@@ -485,8 +495,8 @@ __device__ __forceinline__ void fma2(float& a0, float& a1, float s, uint32_t v0,
 // tensor core at once: a block, with one accumulator per scale group side by
 // side, or half of one where a block's accumulators would not fit.  With TK ==
 // 1 (few rows) the CTA makes the terms of its part of K itself and keeps them
-// in shared memory; otherwise a terms kernel has made them and they come with
-// the ring.
+// in shared memory; otherwise a terms kernel has made them and they come in a
+// ring of their own.
 template <int COLS, int GS, int ROWS, int TN, int TK>
 struct Q4Cfg {
     static constexpr bool XIN = TK == 1;
@@ -941,6 +951,11 @@ aem_status launch_tile(const uint8_t* terms, Q4Args a, int gs, int64_t slots, cu
 
 // Rows of a tile: as many as the call (grouped: an average group) has; few
 // rows put their terms side by side in the 16 columns of the narrowest MMA.
+// A CTA that makes its own terms spares the terms kernel and its wait, but
+// every CTA of a row then does that work.  4096 x 14336, bf16: one row 11.2 us
+// (with the kernel 14.5), three 13.9 (14.8), five 16.7 (14.9); 4096 x 4096: one
+// 8.2 (9.2), five 10.1 (9.5).  A tile of 32 rows where 16 would do: 17.9 us
+// instead of 15.0 (6 rows).
 struct Q4Plan {
     bool few;
     int rows;

@@ -2,7 +2,7 @@
 products of a decoding step's rows with it, dense and grouped by expert.
 
     q, s = quantize_q4(w, 128)                   # w [K, N] or [G, K, N]
-    weight = Q4Weight(q, s, 128)                 # packed once, K*N/2 bytes a group
+    weight = Q4Weight(q, s, 128)                 # packed once, about K*N/2 bytes a group
     y = q4_matmul(x, weight)                     # x [M, K]
     h = grouped_q4_matmul(rows, weight, order.starts, relu=True)
 

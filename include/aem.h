@@ -289,8 +289,9 @@ aem_status aem_capacity_route_static(const uint32_t* primary, const uint32_t* se
  * AEM_MAX_TOPK, E <= AEM_MAX_EXPERTS, T*k < 2^31.  All pointers are DEVICE
  * pointers, row strides (ld*) count elements and d is the contiguous one; any
  * alignment of the element type works, 16-byte rows run widest.  Sums are
- * float32 in a fixed order (no atomics): results repeat bit for bit.  Calls
- * share nothing and are ordered by their stream alone; make the first call
+ * float32 in a fixed order (no atomics): results repeat bit for bit.  No
+ * output may overlap an input.  Calls share nothing and are ordered by their
+ * stream alone; make the first call
  * on a device before a stream capture.  The reference's scatter and
  * reassembly are Router::route_batch (src/orchestration/router.hpp:67-100,
  * 268-313); it has no gradients. */
@@ -327,8 +328,7 @@ aem_status aem_combine(const void* rows, aem_dtype rows_dtype, int64_t ldr, cons
  *   grad_rows[row_of[t*k + j]] = weights[t, j] * grad_out[t]   (rows' dtype;
  *                                rows from starts[E] on are zero)
  *   grad_weights[t*k + j]      = <grad_out[t], rows[row_of[t*k + j]]>
- * Either may be NULL; rows may be NULL without grad_weights.  grad_rows must
- * not overlap rows. */
+ * Either may be NULL; rows may be NULL without grad_weights. */
 aem_status aem_combine_backward(const void* grad_out, aem_dtype out_dtype, int64_t ldg,
                                 const void* rows, aem_dtype rows_dtype, int64_t ldr,
                                 const float* weights, int64_t ldw, const int32_t* row_of,
@@ -352,8 +352,9 @@ typedef struct aem_q4weight_s* aem_q4weight_t;
 
 /* Packs G groups (experts) of 4-bit weights, q [G][K][N] int8 holding values
  * in [-7, 7] and scale [G][ceil(K/group_size)][N] (float32 or bf16, kept as
- * given), into a device-resident copy of K*N/2 bytes per group laid out as
- * the product's matrix fragments.  Same from HOST memory (a value outside
+ * given), into a device-resident copy laid out in blocks of 128 k x 128
+ * channels with their scales: K*N/2 bytes per group and the scales, K and N
+ * rounded up to 128.  Same from HOST memory (a value outside
  * [-7, 7] -> AEM_EINVAL) and from DEVICE memory (stream-ordered; such a value
  * is clamped and reported by aem_device_status). */
 aem_status aem_q4weight_pack(const int8_t* q, const void* scale, aem_dtype scale_dtype, int64_t G,
@@ -376,8 +377,10 @@ aem_status aem_q4weight_shape(aem_q4weight_t w, int64_t* G, int64_t* K, int64_t*
  * elements apart, rows of out ldo; any alignment works.  The workspace holds
  * x in the products' form: device scratch of aem_q4gemm_workspace(w,
  * x_dtype, M, 0) bytes (0 for the fewest rows), 16-byte aligned, or NULL to
- * have the call allocate and free it in stream order.  The weights' device must be the current one.
- * Results repeat bit for bit. */
+ * have the call allocate and free it in stream order.  Scales of magnitudes
+ * 2^-100 to 2^100 keep all of float32's precision.  out must not overlap x or
+ * the workspace; the weights' device must be the current one; make the first
+ * call on a device before a stream capture.  Results repeat bit for bit. */
 size_t aem_q4gemm_workspace(aem_q4weight_t w, aem_dtype x_dtype, int64_t M, int grouped);
 aem_status aem_q4gemm(aem_q4weight_t w, int64_t group, const void* x, aem_dtype x_dtype,
                       int64_t ldx, int64_t M, void* out, aem_dtype out_dtype, int64_t ldo,
@@ -386,7 +389,8 @@ aem_status aem_q4gemm(aem_q4weight_t w, int64_t group, const void* x, aem_dtype 
  * [group_rows[g], group_rows[g+1]) of x (device int32 array of G+1 increasing
  * offsets: aem_dispatch's starts) times weight group g, for all G <=
  * AEM_MAX_EXPERTS groups of w, with out = relu(...) when relu != 0; workspace
- * as above (aem_q4gemm_workspace(w, x_dtype, M, 1)).  Offsets are clamped to [0, M]; rows of out outside every group are not written. */
+ * as above (aem_q4gemm_workspace(w, x_dtype, M, 1)).  Offsets are clamped to
+ * [0, M]; rows of out outside every group are not written. */
 aem_status aem_grouped_q4gemm(aem_q4weight_t w, const int32_t* group_rows, const void* x,
                               aem_dtype x_dtype, int64_t ldx, int64_t M, void* out,
                               aem_dtype out_dtype, int64_t ldo, int relu, void* workspace,
