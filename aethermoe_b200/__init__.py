@@ -10,7 +10,10 @@ Python kernel API:
   naive_quantized_matmul, fused_quantized_matmul}``
 
 plus the composed layer (``aethermoe_b200.moe``): a single-GPU MoE layer and
-the expert-parallel layer over NCCL.
+the expert-parallel layer over NCCL; and the pieces for callers that run their
+own experts: token dispatch and combine with their gradients
+(``aethermoe_b200.dispatch``) and 4-bit weights with group scales
+(``aethermoe_b200.q4``).
 """
 from ._lib import (AemError, AemTimeout, CAPACITY_UNLIMITED, GATING_EXACT, GATING_FAST, Gate,
                    MoeConfig, QWeight, check, context, device_count, lib)

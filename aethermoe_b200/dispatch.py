@@ -150,6 +150,28 @@ def _output(out, shape, dtype, device, name="out"):
     return out, out.stride(0) if shape[0] > 1 else shape[1]
 
 
+def _overlap(a, b):
+    """Whether two matrices of unit column stride may share bytes (column ranges
+    of one row-strided buffer do not)."""
+    ea, eb = a.element_size(), b.element_size()
+    la, lb = a.stride(0) * ea, b.stride(0) * eb
+    a0, b0 = a.data_ptr(), b.data_ptr()
+    if not a.numel() or not b.numel():
+        return False
+    if b0 >= a0 + (a.shape[0] - 1) * la + a.shape[1] * ea or a0 >= b0 + (b.shape[0] - 1) * lb + b.shape[1] * eb:
+        return False
+    if la != lb or la == 0:
+        return True
+    at = (b0 - a0) % la
+    return not (at >= a.shape[1] * ea and at + b.shape[1] * eb <= la)
+
+
+def _apart(out, *tensors):
+    """Refuses an output given by the caller that overlaps an input."""
+    if out is not None and any(t is not None and _overlap(out, t) for t in tensors):
+        raise ValueError("out overlaps an input")
+
+
 def _ids(ids, num_experts):
     if ids.dtype != torch.int32 or ids.dim() != 2:
         raise ValueError(f"expert ids must be [T, k] int32, got {tuple(ids.shape)} {ids.dtype}")
@@ -205,6 +227,7 @@ def _dispatch(x, ids, num_experts, out, s):
     if x.shape[1] == 0:
         raise ValueError("x has no columns")
     rows, ldr = _output(out, (ids.numel(), x.shape[1]), x.dtype, x.device, "rows")
+    _apart(out, x)
     return rows, _sort_and_move(x, ldx, ids, num_experts, rows, ldr, s)
 
 
@@ -212,6 +235,7 @@ def _dispatch_rows(x, order, out, s):
     t, k = order.shape
     x, ldx = _matrix(x, "x", rows=t)
     rows, ldr = _output(out, (t * k, x.shape[1]), x.dtype, x.device, "rows")
+    _apart(out, x)
     row_of, _, starts = order._pointers()
     _lib.check(_lib.lib().aem_dispatch_rows(x.data_ptr(), _DT[x.dtype], ldx, x.shape[1], row_of, starts, t, k,
                                             order.num_experts, rows.data_ptr(), ldr, s),
@@ -226,7 +250,9 @@ def _combine(rows, weights, order, out_dtype, out, s):
     ldw = 0
     if weights is not None:
         weights, ldw = _weights(weights, (t, k))
+    given = out
     out, ldo = _output(out, (t, d), out_dtype or (rows.dtype if out is None else out.dtype), rows.device)
+    _apart(given, rows, weights)
     _lib.check(_lib.lib().aem_combine(rows.data_ptr(), _DT[rows.dtype], ldr,
                                       None if weights is None else weights.data_ptr(), ldw,
                                       order._pointers()[0], t, k, d, out.data_ptr(),
@@ -314,19 +340,19 @@ def dispatch(x, ids, num_experts, out=None, stream=None):
         holder = []
         rows = _DispatchFn.apply(x, ids, num_experts, None, holder, stream)
         return rows, holder[0]
-    return _on(stream, _dispatch, (x, ids), (x, ids, num_experts, out))
+    return _on(stream, _dispatch, (x, ids, out), (x, ids, num_experts, out))
 
 
 def dispatch_rows(x, order, out=None, stream=None):
     """Rows of another ``x [T, d]`` by an existing order."""
     if _differentiable("dispatch_rows", out, x):
         return _DispatchFn.apply(x, None, 0, order, None, stream)
-    return _on(stream, _dispatch_rows, (x, order), (x, order, out))
+    return _on(stream, _dispatch_rows, (x, order, out), (x, order, out))
 
 
 def dispatch_backward(grad_rows, order, out_dtype=None, out=None, stream=None):
     """Gradient of ``dispatch``: ``grad_x[t] = sum_j grad_rows[row_of[t, j]]``."""
-    return _on(stream, _combine, (grad_rows, order), (grad_rows, None, order, out_dtype, out))
+    return _on(stream, _combine, (grad_rows, order, out), (grad_rows, None, order, out_dtype, out))
 
 
 def combine(rows, weights, order, out_dtype=None, out=None, stream=None):
@@ -334,7 +360,7 @@ def combine(rows, weights, order, out_dtype=None, out=None, stream=None):
     ``weights [T, k]`` float32; ``out_dtype`` defaults to the rows')."""
     if _differentiable("combine", out, rows, weights):
         return _CombineFn.apply(rows, weights, order, out_dtype, stream)
-    return _on(stream, _combine, (rows, weights, order), (rows, weights, order, out_dtype, out))
+    return _on(stream, _combine, (rows, weights, order, out), (rows, weights, order, out_dtype, out))
 
 
 def combine_backward(grad_out, rows, weights, order, stream=None):

@@ -17,7 +17,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .dispatch import _DT, _matrix, _on, _output
+from .dispatch import _DT, _apart, _matrix, _on, _output
 
 
 def _quantize(w, group_size, scale_dtype, s):
@@ -127,7 +127,9 @@ def _matmul(x, w, group, out_dtype, out, s):
     x, ldx = _matrix(x, "x", d=w.K)
     _check_weight(w, x.device)
     m = x.shape[0]
+    given = out
     out, ldo = _output(out, (m, w.N), out_dtype or (x.dtype if out is None else out.dtype), x.device)
+    _apart(given, x)
     ws, n, keep = _scratch(x, w, 0)
     _lib.check(_lib.lib().aem_q4gemm(w.handle, group, x.data_ptr(), _DT[x.dtype], ldx, m,
                                      out.data_ptr(), _DT[out.dtype], ldo, ws, n, s), "aem_q4gemm")
@@ -140,7 +142,9 @@ def _grouped(x, w, starts, relu, out_dtype, out, s):
     if starts.dtype != torch.int32 or tuple(starts.shape) != (w.G + 1,) or not starts.is_contiguous():
         raise ValueError(f"starts must be {w.G + 1} contiguous int32 offsets")
     m = x.shape[0]
+    given = out
     out, ldo = _output(out, (m, w.N), out_dtype or (x.dtype if out is None else out.dtype), x.device)
+    _apart(given, x)
     ws, n, keep = _scratch(x, w, 1)
     _lib.check(_lib.lib().aem_grouped_q4gemm(w.handle, starts.data_ptr(), x.data_ptr(), _DT[x.dtype],
                                              ldx, m, out.data_ptr(), _DT[out.dtype], ldo,
@@ -148,14 +152,21 @@ def _grouped(x, w, starts, relu, out_dtype, out, s):
     return out
 
 
+def _no_gradient(what, x):
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{what} has no gradient: detach x or call it under torch.no_grad()")
+
+
 def q4_matmul(x, w, group=0, out_dtype=None, out=None, stream=None):
     """``x [M, K] @`` group ``group`` of ``w`` -> ``[M, N]`` (``out_dtype`` defaults to
-    x's): the weight stream of a decoding step."""
-    return _on(stream, _matmul, (x,), (x, w, group, out_dtype, out))
+    x's): the weight stream of a decoding step.  For inference: no gradient."""
+    _no_gradient("q4_matmul", x)
+    return _on(stream, _matmul, (x, out), (x, w, group, out_dtype, out))
 
 
 def grouped_q4_matmul(x, w, starts, relu=False, out_dtype=None, out=None, stream=None):
     """Rows ``[starts[g], starts[g+1])`` of ``x [M, K]`` times group ``g`` of ``w``,
     for every group, with an optional ReLU.  Rows outside every group are not
-    written (uninitialised where ``out`` is not given)."""
-    return _on(stream, _grouped, (x, starts), (x, w, starts, relu, out_dtype, out))
+    written (uninitialised where ``out`` is not given).  For inference: no gradient."""
+    _no_gradient("grouped_q4_matmul", x)
+    return _on(stream, _grouped, (x, starts, out), (x, w, starts, relu, out_dtype, out))

@@ -123,3 +123,12 @@ def test_python_forms_refuse_before_the_library():
         q4.Q4Weight(torch.zeros(65, 32, dtype=torch.int8), torch.zeros(2, 32), 32)
     with pytest.raises(ValueError, match="-7, 7"):
         q4.Q4Weight(torch.full((64, 32), 9, dtype=torch.int8), torch.zeros(2, 32), 32)
+
+
+def test_overlapping_matrices():
+    b = torch.zeros(8, 192)
+    assert D._overlap(b, b) and D._overlap(b[:, :64], b[:, 63:100]) and D._overlap(b[:, 100:], b[:4, :101])
+    assert not D._overlap(b[:, :64], b[:, 64:]) and not D._overlap(b[:, 64:128], b[:, :64])
+    assert not D._overlap(b[:4], b[4:]) and D._overlap(b[:5], b[4:])
+    assert not D._overlap(b[:0], b) and not D._overlap(b, torch.zeros(8, 192))
+    assert D._overlap(b[:1].expand(8, 192), b[1:, :1]) is False and D._overlap(b[:1].expand(8, 192), b)
