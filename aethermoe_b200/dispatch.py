@@ -136,15 +136,15 @@ def _matrix(t, name, d=None, rows=None):
     return t, t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _output(out, shape, dtype, device, name="out"):
+def _output(out, shape, dtype, like, name="out"):
     if out is None:
         if dtype not in _DT:
             raise ValueError(f"{name}: unsupported dtype {dtype} (float32 or bfloat16)")
-        return torch.empty(shape, dtype=dtype, device=device), shape[1]
+        return like.new_empty(shape, dtype=dtype), shape[1]
     if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
         raise ValueError(f"{name} must be {tuple(shape)} {dtype}, got {tuple(out.shape)} {out.dtype}")
-    if out.device != device:
-        raise ValueError(f"{name} is on {out.device}, expected {device}")
+    if out.device != like.device:
+        raise ValueError(f"{name} is on {out.device}, expected {like.device}")
     if shape[1] > 1 and out.stride(1) != 1 or shape[0] > 1 and out.stride(0) < shape[1]:
         raise ValueError(f"{name} needs rows of unit stride that do not overlap")
     return out, out.stride(0) if shape[0] > 1 else shape[1]
@@ -226,7 +226,7 @@ def _dispatch(x, ids, num_experts, out, s):
     x, ldx = _matrix(x, "x", rows=ids.shape[0])
     if x.shape[1] == 0:
         raise ValueError("x has no columns")
-    rows, ldr = _output(out, (ids.numel(), x.shape[1]), x.dtype, x.device, "rows")
+    rows, ldr = _output(out, (ids.numel(), x.shape[1]), x.dtype, x, "rows")
     _apart(out, x)
     return rows, _sort_and_move(x, ldx, ids, num_experts, rows, ldr, s)
 
@@ -234,7 +234,7 @@ def _dispatch(x, ids, num_experts, out, s):
 def _dispatch_rows(x, order, out, s):
     t, k = order.shape
     x, ldx = _matrix(x, "x", rows=t)
-    rows, ldr = _output(out, (t * k, x.shape[1]), x.dtype, x.device, "rows")
+    rows, ldr = _output(out, (t * k, x.shape[1]), x.dtype, x, "rows")
     _apart(out, x)
     row_of, _, starts = order._pointers()
     _lib.check(_lib.lib().aem_dispatch_rows(x.data_ptr(), _DT[x.dtype], ldx, x.shape[1], row_of, starts, t, k,
@@ -251,7 +251,7 @@ def _combine(rows, weights, order, out_dtype, out, s):
     if weights is not None:
         weights, ldw = _weights(weights, (t, k))
     given = out
-    out, ldo = _output(out, (t, d), out_dtype or (rows.dtype if out is None else out.dtype), rows.device)
+    out, ldo = _output(out, (t, d), out_dtype or (rows.dtype if out is None else out.dtype), rows)
     _apart(given, rows, weights)
     _lib.check(_lib.lib().aem_combine(rows.data_ptr(), _DT[rows.dtype], ldr,
                                       None if weights is None else weights.data_ptr(), ldw,
@@ -270,10 +270,10 @@ def _combine_backward(grad_out, rows, weights, order, rows_dtype, want_rows, wan
     if want_weights:
         rows, ldr = _matrix(rows, "rows", d=d, rows=t * k)
         rows_dtype = rows.dtype
-        grad_weights = torch.empty((t, k), dtype=torch.float32, device=grad_out.device)
+        grad_weights = grad_out.new_empty((t, k), dtype=torch.float32)
     weights, ldw = _weights(weights, (t, k))
     if want_rows:
-        grad_rows, ldgr = _output(None, (t * k, d), rows_dtype, grad_out.device, "grad_rows")
+        grad_rows, ldgr = _output(None, (t * k, d), rows_dtype, grad_out, "grad_rows")
     _lib.check(_lib.lib().aem_combine_backward(
         grad_out.data_ptr(), _DT[grad_out.dtype], ldg, rows.data_ptr() if want_weights else None,
         _DT[rows_dtype], ldr, weights.data_ptr(), ldw, row_of, starts, t, k, order.num_experts, d,

@@ -24,8 +24,8 @@ def _quantize(w, group_size, scale_dtype, s):
     g = 1 if w.dim() == 2 else w.shape[0]
     k, n = w.shape[-2:]
     kb = -(-k // group_size)
-    q = torch.empty(w.shape, dtype=torch.int8, device=w.device)
-    scale = torch.empty(w.shape[:-2] + (kb, n), dtype=scale_dtype, device=w.device)
+    q = w.new_empty(w.shape, dtype=torch.int8)
+    scale = w.new_empty((kb, n) if w.dim() == 2 else (g, kb, n), dtype=scale_dtype)
     _lib.check(_lib.lib().aem_quantize_q4(w.data_ptr(), _DT[w.dtype], g, k, n, group_size,
                                           q.data_ptr(), scale.data_ptr(), _DT[scale_dtype], s),
                "aem_quantize_q4")
@@ -119,7 +119,7 @@ def _scratch(x, w, grouped):
             w._scratch[key] = n
     if not n:
         return None, 0, None
-    t = torch.empty(n, dtype=torch.uint8, device=x.device)
+    t = x.new_empty(n, dtype=torch.uint8)
     return t.data_ptr(), n, t
 
 
@@ -128,7 +128,7 @@ def _matmul(x, w, group, out_dtype, out, s):
     _check_weight(w, x.device)
     m = x.shape[0]
     given = out
-    out, ldo = _output(out, (m, w.N), out_dtype or (x.dtype if out is None else out.dtype), x.device)
+    out, ldo = _output(out, (m, w.N), out_dtype or (x.dtype if out is None else out.dtype), x)
     _apart(given, x)
     ws, n, keep = _scratch(x, w, 0)
     _lib.check(_lib.lib().aem_q4gemm(w.handle, group, x.data_ptr(), _DT[x.dtype], ldx, m,
@@ -143,7 +143,7 @@ def _grouped(x, w, starts, relu, out_dtype, out, s):
         raise ValueError(f"starts must be {w.G + 1} contiguous int32 offsets")
     m = x.shape[0]
     given = out
-    out, ldo = _output(out, (m, w.N), out_dtype or (x.dtype if out is None else out.dtype), x.device)
+    out, ldo = _output(out, (m, w.N), out_dtype or (x.dtype if out is None else out.dtype), x)
     _apart(given, x)
     ws, n, keep = _scratch(x, w, 1)
     _lib.check(_lib.lib().aem_grouped_q4gemm(w.handle, starts.data_ptr(), x.data_ptr(), _DT[x.dtype],
