@@ -500,12 +500,19 @@ __device__ __forceinline__ void fma2(float& a0, float& a1, float s, uint32_t v0,
 template <int COLS, int GS, int ROWS, int TN, int TK>
 struct Q4Cfg {
     static constexpr bool XIN = TK == 1;
-    static constexpr int TW = 128;                     // TMEM columns of a warpgroup: 4 per SM
+    static constexpr int CTAS = COLS == 16 ? 2 : 1;    // on an SM
+    static constexpr int TW = 256 / CTAS;              // TMEM columns of a warpgroup
     static constexpr int FULL = GS == 128 ? 1 : 128 / GS;  // scale groups of a block
-    static constexpr int UK = 32 + FULL * COLS <= TW ? 128 : 64;  // k of a unit
-    static constexpr int SUB = UK < GS ? 1 : UK / GS;  // accumulators per unit
+    static constexpr bool QUEUE = CTAS == 1;           // a unit's MMAs queue behind the last one's
+    static constexpr int UB = QUEUE ? 2 : 1;           // units that tensor memory has to hold
+    static constexpr int UK = UB * (32 + FULL * COLS) <= TW ? 128   // k of a unit
+                              : UB * (16 + (64 / GS ? 64 / GS : 1) * COLS) <= TW ? 64 : 32;
+    static constexpr int SUB = UK / GS;                // accumulators per unit
     static constexpr int UA = UK / 4;                  // columns of a unit's weights
-    static constexpr int ND = UA + 2 * SUB * COLS <= TW ? 2 : 1;  // accumulator buffers
+    static constexpr int ND = UA + 2 * SUB * COLS <= TW ? 2 : 1;  // buffers of accumulators,
+    static constexpr int NA = QUEUE || (ND == 1 && !XIN) ? 2 : 1;  // of weights
+    static constexpr bool LATE = ND == 1 && NA == 1;   // weights unpacked after the sums are taken
+    static constexpr int NB = QUEUE ? 2 : 1;           // units under way: their barriers
     static constexpr int XB = TK * COLS * 128;         // activation bytes of a block
     // XIN: bytes between the blocks' terms.  A tile of at most 8 columns takes
     // 1 KB; the MMA's other 8 columns, never read back, are then the next
@@ -515,19 +522,21 @@ struct Q4Cfg {
     static constexpr int XRES = XIN ? MAXP * XSTEP : 0;
     static constexpr int WB = 8192 + (FULL * 512 + 1023) / 1024 * 1024;  // a block of weights and scales
     // the cluster's sums: S shares of ceil(rows / S) rows, for any S up to 8
-    static constexpr int RECV = (ROWS < 8 ? 8 : ROWS < 16 ? 14 : ROWS < 32 ? 21 : 36) * 128 * 4;
+    static constexpr int RECV = (ROWS < 8 ? 8 : ROWS < 16 ? 14 : ROWS < 32 ? 21 : ROWS < 64 ? 36 : 70) * 128 * 4;
     // Even rings: a stage always comes back to the warpgroup that saw its
     // previous phase, so no parity wait can mistake a phase for the one two
     // back.  Activations stay in theirs until the MMAs are done, weights only
     // until they are read.
     static constexpr int NX = XIN ? 0 : 4;
-    static constexpr int FIT = (113 * 1024 - 2048 - XRES - RECV - NX * XB) / WB / 2 * 2;
+    static constexpr int MOST = CTAS == 2 ? 113 * 1024 : 226 * 1024;
+    static constexpr int FIT = (MOST - 2048 - XRES - RECV - NX * XB) / WB / 2 * 2;
     static constexpr int NW = FIT > 8 ? 8 : FIT;
-    static constexpr int USED = 1024 + NW * WB + NX * XB + XRES + RECV + (2 * (NW + NX) + 5) * 8 + 16 + ROWS * 4;
-    // two CTAs on an SM, never three: no CTA ever waits for tensor memory
-    static constexpr int SMEM = USED > 78 * 1024 ? USED : 78 * 1024;
-    static_assert(UA + ND * SUB * COLS <= TW && NW >= 4 && SMEM <= 113 * 1024, "budgets");
-    static_assert(ROWS * TN <= COLS && (UK >= GS || UK == 128), "a scale group inside a unit");
+    static constexpr int USED = 1024 + NW * WB + NX * XB + XRES + RECV + (2 * (NW + NX) + 9) * 8 + 16 + ROWS * 4;
+    // so many CTAs on an SM and no more: no CTA ever waits for tensor memory
+    static constexpr int LEAST = CTAS == 2 ? 78 * 1024 : 116 * 1024;
+    static constexpr int SMEM = USED > LEAST ? USED : LEAST;
+    static_assert(NA * UA + ND * SUB * COLS <= TW && NW >= 4 && SMEM <= MOST, "budgets");
+    static_assert(ROWS * TN <= COLS && SUB >= 1, "a scale group inside a unit");
     static_assert(NW * WB >= ROWS * 1024, "the warpgroups' sums fit the ring");
 };
 constexpr int kQ4Threads = 12 * 32;
@@ -546,12 +555,14 @@ constexpr int kQ4Threads = 12 * 32;
 //   warp 11     copies the activations' terms, one TMA box per block
 //               (128-byte swizzle), where the CTA does not make them itself.
 // Two accumulator buffers let the sums be taken back under the next unit's
-// MMAs; where only one fits they are taken before the unit is handed over.
+// MMAs.  Where only one fits, a second buffer of weights lets the next unit be
+// unpacked under them, and it is handed over once the sums are taken.  The
+// widest tile has an SM to itself and two of both: its MMAs queue up.
 // The S CTAs of a cluster take parts of K: each sends its sums to the rank
 // that writes those outputs, which adds them in rank order.
 // Every wait is bounded; a timeout sets the error word and ends all roles.
 template <typename XT, int COLS, int GS, int ROWS, int TN, int TK>
-__global__ void __launch_bounds__(kQ4Threads, 2)
+__global__ void __launch_bounds__(kQ4Threads, COLS == 16 ? 2 : 1)
     q4_kernel(const __grid_constant__ CUtensorMap xmap, const Q4Args a) {
     using C = Q4Cfg<COLS, GS, ROWS, TN, TK>;
     extern __shared__ uint8_t smem_raw[];
@@ -564,9 +575,9 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
     uint64_t* w_empty = w_full + C::NW;
     uint64_t* x_full = w_empty + C::NW;
     uint64_t* x_empty = x_full + C::NX;
-    uint64_t* a_full = x_empty + C::NX;   // [2]: a unit's weights are in tensor memory
-    uint64_t* done = a_full + 2;          // [2]: its MMAs have finished
-    uint64_t* x_made = done + 2;          // XIN: the terms are in shared memory
+    uint64_t* a_full = x_empty + C::NX;   // [2][2]: a unit's weights are in tensor memory
+    uint64_t* done = a_full + 4;          // [2][2]: its MMAs have finished
+    uint64_t* x_made = done + 4;          // XIN: the terms are in shared memory
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(x_made + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     uint32_t* row_top = tmem_slot + 2;    // [ROWS]: XIN, top magnitudes; else the rows' unscale
@@ -622,7 +633,7 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
             mbar_init(&x_full[i], 1);
             mbar_init(&x_empty[i], 4);
         }
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < 4; ++j) {
             mbar_init(&a_full[j], 4);
             mbar_init(&done[j], 1);
         }
@@ -644,6 +655,8 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
     const int wg = w < 8 ? w >> 2 : w & 1;  // the warpgroup a channel or MMA warp belongs to
     const uint32_t td = tmem + static_cast<uint32_t>(wg * C::TW);  // accumulators, then the unit's weights
     const uint32_t ta = td + C::ND * C::SUB * COLS;
+    a_full += 2 * wg;
+    done += 2 * wg;
     auto wait = [&](uint64_t* bar, int phase) {  // whole warps
         if (__all_sync(~0u, mbar_try_wait(bar, phase & 1))) return true;
         return __all_sync(~0u, mbar_wait_bounded(bar, phase & 1, abort_flag, a.err, ERR_GEMM_TIMEOUT)) != 0;
@@ -683,8 +696,8 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
             if (lane == 0) mbar_arrive(x_made);
         }
         const uint32_t quarter = static_cast<uint32_t>(32 * (w & 3)) << 16;
-        // columns taken back at once (the widest row tile's registers allow 16)
-        constexpr int TC = C::SUB * COLS, CH = COLS == 32 || TC == 16 ? 16 : 32;
+        // columns taken back at once
+        constexpr int TC = C::SUB * COLS, CH = TC == 16 ? 16 : 32;
         auto take = [&](int u, const float (&s)[C::SUB]) {  // unit u's sums, scaled
 #pragma unroll
             for (int c0 = 0; c0 < TC; c0 += CH) {
@@ -726,13 +739,9 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
 #pragma unroll
             for (int j = 0; j < 128 / C::UK; ++j) {
                 uint4 q[C::UK / 32];
-                auto read = [&]() {
 #pragma unroll
-                    for (int i = 0; i < C::UK / 32; ++i)
-                        q[i] = *reinterpret_cast<const uint4*>(st + (j * (C::UK / 32) + i) * 2048 + ch * 16);
-                };
-                constexpr bool EARLY = C::ND == 2 || COLS == 16;  // the widest tile has no registers for it
-                if (EARLY) read();
+                for (int i = 0; i < C::UK / 32; ++i)
+                    q[i] = *reinterpret_cast<const uint4*>(st + (j * (C::UK / 32) + i) * 2048 + ch * 16);
                 uint32_t v[C::UA];
                 auto unpack = [&]() {
 #pragma unroll
@@ -744,43 +753,49 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
                             v[8 * i + 2 * e + 1] = __funnelshift_r(word[e], word[e], 4) & 0x87878787u;
                         }
                     }
-                };
-                if (C::ND == 2) unpack();
-                if (C::ND == 2 && j == 128 / C::UK - 1) {  // the block has been read
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&w_empty[p % C::NW]);
-                }
-                if (u) {
-                    // the unit before is done: its weights' columns, its
-                    // accumulators and (at a block's start) its activations are free
-                    if (!(ok = wait(&done[wg], u - 1))) break;
-                    tc_fence_after();
-                    if (!C::XIN && j == 0 && lane == 0) mbar_arrive(&x_empty[(p - 2) % NX]);
-                    if (C::ND == 1) take(u - 1, s_prev);
-                }
-                if (C::ND == 1) {
-                    if (!EARLY) read();
-                    unpack();
-                    if (j == 128 / C::UK - 1) {
+                    if (j == 128 / C::UK - 1) {  // the block has been read
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&w_empty[p % C::NW]);
                     }
+                };
+                auto put = [&]() {
+                    const uint32_t to = ta + quarter + u % C::NA * C::UA;
+                    if constexpr (C::UA == 32)
+                        tc_st_32x32b_x32(to, v);
+                    else if constexpr (C::UA == 16)
+                        tc_st_32x32b_x16(to, v);
+                    else
+                        tc_st_32x32b_x8(to, v);
+                };
+                auto hand_over = [&]() {
+                    tc_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&a_full[u % C::NB]);
+                };
+                // With two buffers of weights, unit u - 2's is free: its MMAs
+                // were waited for a unit ago.
+                if (!C::LATE) unpack();
+                if (C::NA == 2) put();
+                if (C::QUEUE) hand_over();
+                if (u) {
+                    // the unit before is done: its weights' columns, its
+                    // accumulators and (at a block's start) its activations are free
+                    if (!(ok = wait(&done[(u - 1) % C::NB], (u - 1) / C::NB))) break;
+                    tc_fence_after();
+                    if (!C::XIN && j == 0 && lane == 0) mbar_arrive(&x_empty[(p - 2) % NX]);
+                    if (C::ND == 1 || C::QUEUE) take(u - 1, s_prev);
                 }
-                if constexpr (C::UA == 32)
-                    tc_st_32x32b_x32(ta + quarter, v);
-                else
-                    tc_st_32x32b_x16(ta + quarter, v);
-                tc_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&a_full[wg]);
-                if (C::ND == 2 && u) take(u - 1, s_prev);
+                if (C::LATE) unpack();
+                if (C::NA == 1) put();
+                if (!C::QUEUE) hand_over();
+                if (C::ND == 2 && !C::QUEUE && u) take(u - 1, s_prev);
 #pragma unroll
-                for (int i = 0; i < C::SUB; ++i) s_prev[i] = s[C::UK == 128 ? i : j * 64 / GS + i];
+                for (int i = 0; i < C::SUB; ++i) s_prev[i] = s[j * C::SUB + i];
                 ++u;
             }
         }
-        if (ok && u && wait(&done[wg], u - 1)) {
+        if (ok && u && wait(&done[(u - 1) % C::NB], (u - 1) / C::NB)) {
             tc_fence_after();
             take(u - 1, s_prev);
         }
@@ -793,17 +808,17 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
             const uint64_t bd = smem_desc_sw128(smem_u32(C::XIN ? xres + p * C::XSTEP : xring + p % NX * C::XB));
 #pragma unroll
             for (int j = 0; j < 128 / C::UK; ++j) {
-                if (!(ok = wait(&a_full[wg], u))) break;
+                if (!(ok = wait(&a_full[u % C::NB], u / C::NB))) break;
                 tc_fence_after();
                 const uint32_t d = td + static_cast<uint32_t>(u % C::ND * C::SUB * COLS);
 #pragma unroll
                 for (int m = 0; m < C::UK / 32; ++m)
 #pragma unroll
                     for (int t = 0; t < TK; ++t)
-                        tc_mma_f8_ts_elect(d + 32 * m / GS * COLS, ta + 8 * m,
+                        tc_mma_f8_ts_elect(d + 32 * m / GS * COLS, ta + u % C::NA * C::UA + 8 * m,
                                            bd + t * (COLS * 8) + 2 * (j * (C::UK / 32) + m), idesc,
                                            32 * m % GS || t ? 1u : 0u);
-                tc_commit_elect(&done[wg]);
+                tc_commit_elect(&done[u % C::NB]);
                 ++u;
             }
         }
@@ -811,7 +826,7 @@ __global__ void __launch_bounds__(kQ4Threads, 2)
         const bool weights = w == 10;
         if (!weights) {  // x and its unscale are the terms kernel's
             asm volatile("griddepcontrol.wait;" ::: "memory");
-            if (lane < rows) row_top[lane] = __float_as_uint(a.unscale[m0 + lane]);
+            for (int r = lane; r < rows; r += 32) row_top[r] = __float_as_uint(a.unscale[m0 + r]);
         }
         const int ns = weights ? C::NW : C::NX;
         uint64_t *full = weights ? w_full : x_full, *empty = weights ? w_empty : x_empty;
@@ -913,18 +928,22 @@ aem_status launch_q4(const CUtensorMap& xmap, const Q4Args& a, dim3 grid, cudaSt
 // its SM, a CTA's set-up and end take about 14; one with the SM to itself does
 // its blocks in 0.64 of the time and starts 1.5 sooner.  16 rows, 4096 x 4096:
 // 4 CTAs (128 in all) 9.8 us, 8 CTAs 10.8; 14336 x 4096: 4 CTAs 19.1, 8 CTAs
-// 17.2.  Wide clusters leave slots of a GPC empty, more of them while blocks of
-// the terms kernel hold some: 32 clusters of 8 took 19.4 us where 7 took 14.6
-// (14336 x 4096, 4 float32 rows), so 240 of the 296 slots are counted on (264
-// without that kernel).
-int split_k(int64_t ctas, int64_t blocks, int64_t most_blocks, bool terms) {
+// 17.2.  The wide tiles (`alone`) have an SM each and a wave costs 20 of their
+// blocks: 32 rows, 14336 x 4096: 2, 3, 4, 5 CTAs 23.9, 18.8, 16.6, 25.2 us.
+// Wide clusters leave slots of a GPC empty, more of them while blocks of the
+// terms kernel hold some: 32 clusters of 8 took 19.4 us where 7 took 14.6
+// (14336 x 4096, 4 float32 rows), so not all slots are counted on.
+int split_k(int64_t ctas, int64_t blocks, int64_t most_blocks, bool terms, bool alone) {
     int best = 8;
     int64_t least = INT64_MAX;
     for (int S = 1; S <= 8; ++S) {
-        const int64_t each = (blocks + S - 1) / S, slots = S <= 4 ? 296 : terms ? 240 : 264;
+        const int64_t each = (blocks + S - 1) / S, n = ctas * S;
         if (each > most_blocks || (S > 1 && each < 2)) continue;
-        const int64_t cost = ctas * S <= 148 ? 1400 + 64 * each
-                                             : (ctas * S + slots - 1) / slots * (1550 + 100 * each);
+        const int64_t slots = alone ? (S == 3 ? 132 : S <= 4 ? 148 : S == 7 ? 104 : 120)
+                                    : (S <= 4 ? 296 : terms ? 240 : 264);
+        const int64_t waves = (n + slots - 1) / slots;
+        const int64_t cost = alone ? waves * (2000 + 100 * each)
+                             : n <= 148 ? 1400 + 64 * each : waves * (1550 + 100 * each);
         if (cost < least) {
             least = cost;
             best = S;
@@ -940,11 +959,11 @@ aem_status launch_tile(const uint8_t* terms, Q4Args a, int gs, int64_t slots, cu
     const int64_t KP = a.NP * 128ll;
     if (!XIN)
         AEM_TRY(make_tmap_3d_u8(&xmap, terms, KP, a.M * TN, TK, KP, a.M * TN * KP, COLS, TK));
-    a.S = split_k(a.NC * slots, a.NP, XIN ? Q4Cfg<COLS, 128, ROWS, TN, TK>::MAXP : INT64_MAX, !XIN);
+    a.S = split_k(a.NC * slots, a.NP, XIN ? Q4Cfg<COLS, 128, ROWS, TN, TK>::MAXP : INT64_MAX, !XIN, COLS > 16);
     const dim3 grid(static_cast<unsigned>(a.NC * a.S), static_cast<unsigned>(slots));
     if (gs == 128) return launch_q4<XT, COLS, 128, ROWS, TN, TK>(xmap, a, grid, s);
     if (gs == 64) return launch_q4<XT, COLS, 64, ROWS, TN, TK>(xmap, a, grid, s);
-    if constexpr (TK < 8) return launch_q4<XT, COLS, 32, ROWS, TN, TK>(xmap, a, grid, s);
+    if constexpr (COLS > 16 || TK < 8) return launch_q4<XT, COLS, 32, ROWS, TN, TK>(xmap, a, grid, s);
     set_error("q4 product: no such row tile");  // eight terms and 32-k scales do not fit a ring of four
     return AEM_EINVAL;
 }
@@ -966,9 +985,9 @@ Q4Plan q4_plan(const Q4Weight* w, bool f32, int64_t M, bool grouped) {
     Q4Plan p;
     p.few = want <= (f32 ? 2 : 4) && w->NP <= 8 * 24;
     if (f32)
-        p.rows = p.few ? (want <= 1 ? 1 : 2) : want <= 4 ? 4 : want <= 8 || w->gs == 32 ? 8 : 16;
+        p.rows = p.few ? (want <= 1 ? 1 : 2) : want <= 4 ? 4 : want <= 8 ? 8 : want <= 16 && w->gs > 32 ? 16 : 32;
     else
-        p.rows = p.few ? (want <= 2 ? 2 : 4) : want <= 16 ? 16 : 32;
+        p.rows = p.few ? (want <= 2 ? 2 : 4) : want <= 16 ? 16 : want <= 32 ? 32 : 64;
     return p;
 }
 size_t q4_workspace(const Q4Weight* w, bool f32, int64_t M, bool grouped) {
@@ -1015,7 +1034,7 @@ aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, const XT* x
     auto* terms = static_cast<uint8_t*>(workspace);
     auto* unscale = reinterpret_cast<float*>(terms + static_cast<size_t>(a.M) * kTerms<XT> * w->NP * 128);
     a.unscale = unscale;
-    const int tn = F32 ? 16 / a.rows : 1;
+    const int tn = F32 && a.rows < 16 ? 16 / a.rows : 1;
     // at most 8 slots in registers up to K = 16384, and about two blocks an SM
     const int threads = w->K <= 4096 ? 128 : w->K <= 8192 ? 256 : 512;
     const int64_t slots_x = (w->NP * 32 + threads - 1) / threads;
@@ -1030,12 +1049,14 @@ aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, const XT* x
         set_error("%s: launch failed: %s", what, cudaGetErrorString(e));
         st = AEM_ECUDA;
     } else if constexpr (F32) {
-        st = tn == 4   ? launch_tile<XT, 16, 4, 4, 2>(terms, a, w->gs, slots, s)
-             : tn == 2 ? launch_tile<XT, 16, 8, 2, 4>(terms, a, w->gs, slots, s)
-                       : launch_tile<XT, 16, 16, 1, 8>(terms, a, w->gs, slots, s);
+        st = a.rows == 4    ? launch_tile<XT, 16, 4, 4, 2>(terms, a, w->gs, slots, s)
+             : a.rows == 8  ? launch_tile<XT, 16, 8, 2, 4>(terms, a, w->gs, slots, s)
+             : a.rows == 16 ? launch_tile<XT, 16, 16, 1, 8>(terms, a, w->gs, slots, s)
+                            : launch_tile<XT, 32, 32, 1, 8>(terms, a, w->gs, slots, s);
     } else {
-        st = a.rows == 16 ? launch_tile<XT, 16, 16, 1, 3>(terms, a, w->gs, slots, s)
-                          : launch_tile<XT, 32, 32, 1, 3>(terms, a, w->gs, slots, s);
+        st = a.rows == 16   ? launch_tile<XT, 16, 16, 1, 3>(terms, a, w->gs, slots, s)
+             : a.rows == 32 ? launch_tile<XT, 32, 32, 1, 3>(terms, a, w->gs, slots, s)
+                            : launch_tile<XT, 64, 64, 1, 3>(terms, a, w->gs, slots, s);
     }
     if (own) cudaFreeAsync(own, s);
     return st;
