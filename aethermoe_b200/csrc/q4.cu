@@ -497,13 +497,13 @@ __device__ __forceinline__ void fma2(float& a0, float& a1, float s, uint32_t v0,
 // 1 (few rows) the CTA makes the terms of its part of K itself and keeps them
 // in shared memory; otherwise a terms kernel has made them and they come in a
 // ring of their own.
-template <int COLS, int GS, int ROWS, int TN, int TK>
+template <int COLS, int GS, int ROWS, int TN, int TK, bool ALONE>
 struct Q4Cfg {
     static constexpr bool XIN = TK == 1;
-    static constexpr int CTAS = COLS == 16 ? 2 : 1;    // on an SM
+    static constexpr int CTAS = ALONE ? 1 : 2;         // on an SM
     static constexpr int TW = 256 / CTAS;              // TMEM columns of a warpgroup
     static constexpr int FULL = GS == 128 ? 1 : 128 / GS;  // scale groups of a block
-    static constexpr bool QUEUE = CTAS == 1;           // a unit's MMAs queue behind the last one's
+    static constexpr bool QUEUE = ALONE;               // a unit's MMAs queue behind the last one's
     static constexpr int UB = QUEUE ? 2 : 1;           // units that tensor memory has to hold
     static constexpr int UK = UB * (32 + FULL * COLS) <= TW ? 128   // k of a unit
                               : UB * (16 + (64 / GS ? 64 / GS : 1) * COLS) <= TW ? 64 : 32;
@@ -539,7 +539,7 @@ struct Q4Cfg {
     static_assert(ROWS * TN <= COLS && SUB >= 1, "a scale group inside a unit");
     static_assert(NW * WB >= ROWS * 1024, "the warpgroups' sums fit the ring");
 };
-constexpr int kQ4Threads = 12 * 32;
+constexpr int kQ4Threads = 12 * 32, kSMs = 148;
 
 // A CTA computes 128 channels of one row tile over its part of K:
 //   warps 0-7   two warpgroups, thread = channel = TMEM lane, that take the
@@ -561,10 +561,10 @@ constexpr int kQ4Threads = 12 * 32;
 // The S CTAs of a cluster take parts of K: each sends its sums to the rank
 // that writes those outputs, which adds them in rank order.
 // Every wait is bounded; a timeout sets the error word and ends all roles.
-template <typename XT, int COLS, int GS, int ROWS, int TN, int TK>
-__global__ void __launch_bounds__(kQ4Threads, COLS == 16 ? 2 : 1)
+template <typename XT, int COLS, int GS, int ROWS, int TN, int TK, bool ALONE>
+__global__ void __launch_bounds__(kQ4Threads, ALONE ? 1 : 2)
     q4_kernel(const __grid_constant__ CUtensorMap xmap, const Q4Args a) {
-    using C = Q4Cfg<COLS, GS, ROWS, TN, TK>;
+    using C = Q4Cfg<COLS, GS, ROWS, TN, TK, ALONE>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* xres = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                ~static_cast<uintptr_t>(1023));
@@ -890,10 +890,10 @@ __global__ void __launch_bounds__(kQ4Threads, COLS == 16 ? 2 : 1)
     }
 }
 
-template <typename XT, int COLS, int GS, int ROWS, int TN, int TK>
+template <typename XT, int COLS, int GS, int ROWS, int TN, int TK, bool ALONE>
 aem_status launch_q4(const CUtensorMap& xmap, const Q4Args& a, dim3 grid, cudaStream_t s) {
-    using C = Q4Cfg<COLS, GS, ROWS, TN, TK>;
-    auto kern = q4_kernel<XT, COLS, GS, ROWS, TN, TK>;
+    using C = Q4Cfg<COLS, GS, ROWS, TN, TK, ALONE>;
+    auto kern = q4_kernel<XT, COLS, GS, ROWS, TN, TK, ALONE>;
     static std::atomic<uint64_t> ready{0};  // bit per device: the shared memory opt-in is done
     const uint64_t bit = 1ull << (current_device() & 63);
     if (!(ready.load(std::memory_order_relaxed) & bit)) {
@@ -952,18 +952,18 @@ int split_k(int64_t ctas, int64_t blocks, int64_t most_blocks, bool terms, bool 
     return best;
 }
 
-template <typename XT, int COLS, int ROWS, int TN, int TK>
+template <typename XT, int COLS, int ROWS, int TN, int TK, bool ALONE = false>
 aem_status launch_tile(const uint8_t* terms, Q4Args a, int gs, int64_t slots, cudaStream_t s) {
     CUtensorMap xmap{};
     constexpr bool XIN = TK == 1;
     const int64_t KP = a.NP * 128ll;
     if (!XIN)
         AEM_TRY(make_tmap_3d_u8(&xmap, terms, KP, a.M * TN, TK, KP, a.M * TN * KP, COLS, TK));
-    a.S = split_k(a.NC * slots, a.NP, XIN ? Q4Cfg<COLS, 128, ROWS, TN, TK>::MAXP : INT64_MAX, !XIN, COLS > 16);
+    a.S = split_k(a.NC * slots, a.NP, XIN ? Q4Cfg<COLS, 128, ROWS, TN, TK, ALONE>::MAXP : INT64_MAX, !XIN, ALONE);
     const dim3 grid(static_cast<unsigned>(a.NC * a.S), static_cast<unsigned>(slots));
-    if (gs == 128) return launch_q4<XT, COLS, 128, ROWS, TN, TK>(xmap, a, grid, s);
-    if (gs == 64) return launch_q4<XT, COLS, 64, ROWS, TN, TK>(xmap, a, grid, s);
-    if constexpr (COLS > 16 || TK < 8) return launch_q4<XT, COLS, 32, ROWS, TN, TK>(xmap, a, grid, s);
+    if (gs == 128) return launch_q4<XT, COLS, 128, ROWS, TN, TK, ALONE>(xmap, a, grid, s);
+    if (gs == 64) return launch_q4<XT, COLS, 64, ROWS, TN, TK, ALONE>(xmap, a, grid, s);
+    if constexpr (ALONE || TK < 8) return launch_q4<XT, COLS, 32, ROWS, TN, TK, ALONE>(xmap, a, grid, s);
     set_error("q4 product: no such row tile");  // eight terms and 32-k scales do not fit a ring of four
     return AEM_EINVAL;
 }
@@ -1052,11 +1052,15 @@ aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, const XT* x
         st = a.rows == 4    ? launch_tile<XT, 16, 4, 4, 2>(terms, a, w->gs, slots, s)
              : a.rows == 8  ? launch_tile<XT, 16, 8, 2, 4>(terms, a, w->gs, slots, s)
              : a.rows == 16 ? launch_tile<XT, 16, 16, 1, 8>(terms, a, w->gs, slots, s)
-                            : launch_tile<XT, 32, 32, 1, 8>(terms, a, w->gs, slots, s);
+                            : launch_tile<XT, 32, 32, 1, 8, true>(terms, a, w->gs, slots, s);
     } else {
-        st = a.rows == 16   ? launch_tile<XT, 16, 16, 1, 3>(terms, a, w->gs, slots, s)
-             : a.rows == 32 ? launch_tile<XT, 32, 32, 1, 3>(terms, a, w->gs, slots, s)
-                            : launch_tile<XT, 64, 64, 1, 3>(terms, a, w->gs, slots, s);
+        // 16 rows: an SM for each CTA while there are SMs (8 rows, 14336 x 4096:
+        // 14.5 us, sharing 16.7), but not for many groups' tiles (64 tokens, 64
+        // experts of 2048 x 1408: 39.2 us, sharing 29.4)
+        st = a.rows == 64           ? launch_tile<XT, 64, 64, 1, 3, true>(terms, a, w->gs, slots, s)
+             : a.rows == 32         ? launch_tile<XT, 32, 32, 1, 3, true>(terms, a, w->gs, slots, s)
+             : a.NC * slots <= kSMs ? launch_tile<XT, 16, 16, 1, 3, true>(terms, a, w->gs, slots, s)
+                                    : launch_tile<XT, 16, 16, 1, 3>(terms, a, w->gs, slots, s);
     }
     if (own) cudaFreeAsync(own, s);
     return st;
