@@ -26,8 +26,9 @@
 // 4096 x 14336, groups of 128, one bf16 row: 10.9 us, 2.8 TB/s of that stream
 // (about 2 us to the first product, 4 of products at the memory's rate, 1.5 of
 // sums between CTAs, the rest the launch).  64 rows of 14336 x 4096, groups of
-// 64: 25.6 us, where taking the sums back from tensor memory and the latency
-// from one unit to the next bound it.  Forms that could not keep up (4096 x
+// 64: 22.2 us (18.8 for 4096 x 14336, groups of 128), where unpacking, taking
+// the sums back from tensor memory and the latency from one unit to the next
+// bound it.  Forms that could not keep up (4096 x
 // 14336, one row): warp MMAs (mma.sync m16n8k16 occupies its sub-core's tensor
 // pipe for 32 cycles: 16.6 us, 47.6 for 64 rows), and bf16 operands for tcgen05
 // (7 logic operations and 4 subtractions per 8 weights, the logic pipe the
@@ -493,7 +494,13 @@ __device__ __forceinline__ void fma2(float& a0, float& a1, float s, uint32_t v0,
 // TN * TK terms in TN columns, TK after one another.  A block of the packed
 // weight is 128 channels x 128 k; a unit is what a warpgroup hands to the
 // tensor core at once: a block, with one accumulator per scale group side by
-// side, or half of one where a block's accumulators would not fit.  With TK ==
+// side, or a half or quarter where a block's accumulators would not fit.  Two
+// CTAs share an SM, so that one's set-up and end lie under the other's products,
+// or a CTA has one to itself (ALONE) with room for two units in tensor memory
+// and twice the registers: 32 rows, 4096 x 14336: 17.6 us shared, 15.7 alone; 64
+// rows 25.0 as two shared tiles, 18.8 as one alone; few rows 11.0 shared, 11.5
+// alone (one row), where the stream is the bound and more CTAs ask for it.
+// With TK ==
 // 1 (few rows) the CTA makes the terms of its part of K itself and keeps them
 // in shared memory; otherwise a terms kernel has made them and they come in a
 // ring of their own.
@@ -557,7 +564,8 @@ constexpr int kQ4Threads = 12 * 32, kSMs = 148;
 // Two accumulator buffers let the sums be taken back under the next unit's
 // MMAs.  Where only one fits, a second buffer of weights lets the next unit be
 // unpacked under them, and it is handed over once the sums are taken.  The
-// widest tile has an SM to itself and two of both: its MMAs queue up.
+// CTAs with an SM to themselves have two of both: a unit's MMAs queue up behind
+// those of the one before.
 // The S CTAs of a cluster take parts of K: each sends its sums to the rank
 // that writes those outputs, which adds them in rank order.
 // Every wait is bounded; a timeout sets the error word and ends all roles.
@@ -974,20 +982,23 @@ aem_status launch_tile(const uint8_t* terms, Q4Args a, int gs, int64_t slots, cu
 // every CTA of a row then does that work.  4096 x 14336, bf16: one row 11.2 us
 // (with the kernel 14.5), three 13.9 (14.8), five 16.7 (14.9); 4096 x 4096: one
 // 8.2 (9.2), five 10.1 (9.5).  A tile of 32 rows where 16 would do: 17.9 us
-// instead of 15.0 (6 rows).
+// instead of 15.0 (6 rows).  One of 64 takes 18.8 us where two of 32 take 25
+// (4096 x 14336), but 9.7 where those take 8.5 with K split three ways or more
+// inside one wave (2048 x 1408).
 struct Q4Plan {
     bool few;
     int rows;
 };
 Q4Plan q4_plan(const Q4Weight* w, bool f32, int64_t M, bool grouped) {
-    const int64_t groups = std::min<int64_t>(w->G, M);
-    const int64_t want = grouped ? (M + groups - 1) / groups : M;
+    const int64_t groups = grouped ? std::min<int64_t>(w->G, M) : 1;
+    const int64_t want = (M + groups - 1) / groups;
+    const bool small = w->NC * groups * ((want + 31) / 32) * 3 <= kSMs;
     Q4Plan p;
     p.few = want <= (f32 ? 2 : 4) && w->NP <= 8 * 24;
     if (f32)
         p.rows = p.few ? (want <= 1 ? 1 : 2) : want <= 4 ? 4 : want <= 8 ? 8 : want <= 16 && w->gs > 32 ? 16 : 32;
     else
-        p.rows = p.few ? (want <= 2 ? 2 : 4) : want <= 16 ? 16 : want <= 32 ? 32 : 64;
+        p.rows = p.few ? (want <= 2 ? 2 : 4) : want <= 16 ? 16 : want <= 32 || small ? 32 : 64;
     return p;
 }
 size_t q4_workspace(const Q4Weight* w, bool f32, int64_t M, bool grouped) {

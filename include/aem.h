@@ -367,8 +367,8 @@ aem_status aem_q4weight_free(aem_q4weight_t w);
 aem_status aem_q4weight_shape(aem_q4weight_t w, int64_t* G, int64_t* K, int64_t* N, int* group_size);
 
 /* out[M, N] = x[M, K] @ (q[group] * scale[group]) for the few rows of a
- * decoding step: one pass over the weights for up to 32 bf16 or 16 float32
- * rows (8 with groups of 32), one more for every further such tile.
+ * decoding step: one pass over the weights for up to 64 bf16 or 32 float32
+ * rows, one more for every further such tile.
  * The integers are exact in the MMAs' operands, each scale multiplies a
  * float32 sum, and x takes part in full: what is cut from an element is
  * under 2^-30 of its row's largest finite magnitude (nothing for bf16

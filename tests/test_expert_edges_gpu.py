@@ -161,3 +161,32 @@ def test_training_step(cuda, T, k, E):
     assert torch.equal(out.double(), ref)
     for a, b in ((x, x2), (w, w2), (val, v2)):
         assert torch.equal(a.grad.double(), b.grad)
+
+
+@pytest.mark.parametrize("gs", [32, 64, 128])
+@pytest.mark.parametrize("xdt,most", [("bfloat16", 14), ("bfloat16", 30), ("float32", 6), ("float32", 12)])
+@pytest.mark.parametrize("K", [100, 384, 1300])
+def test_more_tiles_than_a_wave(cuda, K, xdt, most, gs):
+    """Ragged groups whose tiles are several waves of CTAs, over one, three and eleven
+    blocks of K; empty groups lie first, last and between."""
+    import torch
+    from aethermoe_b200 import q4
+    G, N = 96, 700
+    q, s = weights(cuda, G, K, N, gs, torch.float32, seed=K)
+    w = q4.Q4Weight(q, s, gs)
+    counts = torch.randint(0, most + 1, (G,), generator=torch.Generator().manual_seed(K + most))
+    counts[0] = counts[50] = counts[-1] = 0
+    counts[7] = 3 * most + 1
+    starts = torch.cat([torch.zeros(1, dtype=torch.int64), counts.cumsum(0)])
+    M = int(starts[-1]) + 5
+    x = torch.randn(M, K, device=cuda).to(getattr(torch, xdt))
+    buf = torch.full((M, N), 7.0, device=cuda)
+    out = q4.grouped_q4_matmul(x, w, starts.int().to(cuda), out=buf)
+    assert (out[M - 5:] == 7).all()
+    for g in range(G):
+        a, b = int(starts[g]), int(starts[g + 1])
+        if a < b:
+            ref, A = product(x[a:b], q[g], s[g], gs)
+            check(out[a:b], ref, A, s.shape[1])
+    again = q4.grouped_q4_matmul(x, w, starts.int().to(cuda), relu=True, out_dtype=torch.float32)
+    assert torch.equal(again[:M - 5], out[:M - 5].clamp(min=0))
