@@ -271,12 +271,13 @@ def _combine_backward(grad_out, rows, weights, order, rows_dtype, want_rows, wan
         rows, ldr = _matrix(rows, "rows", d=d, rows=t * k)
         rows_dtype = rows.dtype
         grad_weights = grad_out.new_empty((t, k), dtype=torch.float32)
-    weights, ldw = _weights(weights, (t, k))
+    if weights is not None:
+        weights, ldw = _weights(weights, (t, k))
     if want_rows:
         grad_rows, ldgr = _output(None, (t * k, d), rows_dtype, grad_out, "grad_rows")
     _lib.check(_lib.lib().aem_combine_backward(
         grad_out.data_ptr(), _DT[grad_out.dtype], ldg, rows.data_ptr() if want_weights else None,
-        _DT[rows_dtype], ldr, weights.data_ptr(), ldw, row_of, starts, t, k, order.num_experts, d,
+        _DT[rows_dtype], ldr, None if weights is None else weights.data_ptr(), ldw, row_of, starts, t, k, order.num_experts, d,
         grad_rows.data_ptr() if want_rows else None, ldgr,
         grad_weights.data_ptr() if want_weights else None, s), "aem_combine_backward")
     return grad_rows, grad_weights
@@ -357,7 +358,8 @@ def dispatch_backward(grad_rows, order, out_dtype=None, out=None, stream=None):
 
 def combine(rows, weights, order, out_dtype=None, out=None, stream=None):
     """``out[t] = sum_j weights[t, j] * rows[row_of[t, j]]`` (``rows [T*k, d]``,
-    ``weights [T, k]`` float32; ``out_dtype`` defaults to the rows')."""
+    ``weights [T, k]`` float32 or ``None`` for 1; ``out_dtype`` defaults to the
+    rows')."""
     if _differentiable("combine", out, rows, weights):
         return _CombineFn.apply(rows, weights, order, out_dtype, stream)
     return _on(stream, _combine, (rows, weights, order, out), (rows, weights, order, out_dtype, out))

@@ -190,3 +190,37 @@ def test_more_tiles_than_a_wave(cuda, K, xdt, most, gs):
             check(out[a:b], ref, A, s.shape[1])
     again = q4.grouped_q4_matmul(x, w, starts.int().to(cuda), relu=True, out_dtype=torch.float32)
     assert torch.equal(again[:M - 5], out[:M - 5].clamp(min=0))
+
+
+@pytest.mark.parametrize("gs", [32, 64, 128])
+@pytest.mark.parametrize("xdt,M", [("bfloat16", 33), ("bfloat16", 64), ("bfloat16", 65), ("bfloat16", 150),
+                                   ("float32", 32), ("float32", 33)])
+@pytest.mark.parametrize("K,N", [(100, 7000), (1500, 6500), (5000, 6500)])
+def test_widest_row_tiles(cuda, K, N, M, xdt, gs):
+    """Enough channels that the widest row tiles are taken, with and without a split K."""
+    import torch
+    from aethermoe_b200 import q4
+    q, s = weights(cuda, 1, K, N, gs, torch.bfloat16, seed=M)
+    w = q4.Q4Weight(q[0], s[0], gs)
+    x = torch.randn(M, K, device=cuda).to(getattr(torch, xdt))
+    ref, A = product(x, q[0], s[0], gs)
+    check(q4.q4_matmul(x, w, out_dtype=torch.float32), ref, A, s.shape[1])
+
+
+def test_combine_without_weights(cuda):
+    """No weights mean weights of 1, in the sum and in the gradients."""
+    import torch
+    from aethermoe_b200 import dispatch as D
+    T, k, E, d = 40, 3, 8, 20
+    ids = torch.randint(-1, E, (T, k), device=cuda, dtype=torch.int32)
+    order = D.sort_tokens(ids, E)
+    rows = torch.randn(T * k, d, device=cuda, requires_grad=True)
+    go = torch.randn(T, d, device=cuda)
+    one = torch.ones(T, k, device=cuda)
+    out = D.combine(rows, None, order)
+    assert torch.equal(out, D.combine(rows.detach(), one, order))
+    out.backward(go)
+    want, gw = D.combine_backward(go, rows.detach(), one, order)
+    assert torch.equal(rows.grad, want)
+    again, gw2 = D.combine_backward(go, rows.detach(), None, order)
+    assert torch.equal(again, want) and torch.equal(gw2, gw)
