@@ -79,6 +79,12 @@ constexpr int kThreads = 256;  // pack
 // instructions run at a quarter of the rate).  Memory bound: 14336 x 4096
 // float32, groups of 128, 57 us = 5.2 TB/s; with a division per element 103.
 constexpr float kRint = 12582912.0f;
+// Maximum that keeps a NaN: its group's scale has to be one.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
 template <typename WT, typename ST, int GS, bool VEC>
 __global__ void __launch_bounds__(4 * GS, GS == 128 ? 2 : 1)
     quantize_q4_kernel(const WT* __restrict__ w, int64_t K, int64_t N, int64_t KB,
@@ -114,15 +120,15 @@ __global__ void __launch_bounds__(4 * GS, GS == 128 ? 2 : 1)
 #pragma unroll
     for (int i = 0; i < R; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) m[j] = fmaxf(m[j], fabsf(v[i][j]));
+        for (int j = 0; j < 4; ++j) m[j] = max_nan(m[j], fabsf(v[i][j]));
     amax[wi][lane] = make_float4(m[0], m[1], m[2], m[3]);
     __syncthreads();
     if (threadIdx.x < 128) {  // one thread per column
         const float* col = reinterpret_cast<const float*>(amax) + threadIdx.x;
         float a = 0.0f;
 #pragma unroll
-        for (int i = 0; i < W; ++i) a = fmaxf(a, col[i * 128]);
-        float sc = fmaxf(__fdiv_rn(a, 7.0f), 1e-12f);
+        for (int i = 0; i < W; ++i) a = max_nan(a, col[i * 128]);
+        float sc = max_nan(__fdiv_rn(a, 7.0f), 1e-12f);
         if constexpr (sizeof(ST) == 2) sc = __bfloat162float(__float2bfloat16_rn(sc));
         reinterpret_cast<float*>(scales)[threadIdx.x] = sc;
         reinterpret_cast<float*>(inverses)[threadIdx.x] = __frcp_rn(sc);

@@ -342,7 +342,8 @@ aem_status aem_combine_backward(const void* grad_out, aem_dtype out_dtype, int64
  *   scale = max(max |w| / 7, 1e-12), rounded to scale_dtype,
  *   q     = clip(rint(w / scale), -7, 7)   with that rounded scale,
  * in IEEE float32.  q int8 [G][K][N], scale [G][ceil(K/group_size)][N]; the
- * last group of a column may be short.  The reference quantises to 8 bits
+ * last group of a column may be short.  A NaN or infinity in a group makes its
+ * scale one, so that products with the group show it.  The reference quantises to 8 bits
  * only (src/kernels/quantized_gemm.py:70-76). */
 aem_status aem_quantize_q4(const void* w, aem_dtype w_dtype, int64_t G, int64_t K, int64_t N,
                            int group_size, int8_t* q, void* scale, aem_dtype scale_dtype,

@@ -224,3 +224,19 @@ def test_combine_without_weights(cuda):
     assert torch.equal(rows.grad, want)
     again, gw2 = D.combine_backward(go, rows.detach(), None, order)
     assert torch.equal(again, want) and torch.equal(gw2, gw)
+
+
+@pytest.mark.parametrize("sdt", ["float32", "bfloat16"])
+@pytest.mark.parametrize("wdt", ["float32", "bfloat16"])
+@pytest.mark.parametrize("N", [33, 36])
+def test_quantize_shows_non_finite_weights(cuda, N, wdt, sdt):
+    import torch
+    from aethermoe_b200 import q4
+    wdt, sdt = getattr(torch, wdt), getattr(torch, sdt)
+    w = torch.randn(200, N, device=cuda).to(wdt)
+    q0, s0 = q4.quantize_q4(w, 64, sdt)
+    w[70, 3], w[5, 30] = float("nan"), -float("inf")
+    q, s = q4.quantize_q4(w, 64, sdt)
+    assert s[1, 3].isnan() and s[0, 30] == float("inf") and (q.abs() <= 7).all()
+    q[64:128, 3], s[1, 3], q[:64, 30], s[0, 30] = q0[64:128, 3], s0[1, 3], q0[:64, 30], s0[0, 30]
+    assert torch.equal(q, q0) and torch.equal(s, s0)
