@@ -72,9 +72,9 @@ constexpr int kThreads = 256;  // pack
 // group each in registers, 4 columns per lane, so w is read once; the column
 // maxima meet in shared memory.  scale = max(amax / 7, 1e-12), rounded to
 // the scale's type before q = clip(rint(w / scale), -7, 7) is taken with it
-// (IEEE float32 division, ties to even).  |w / scale| is about 7 at most and
-// w * (1 / scale) is within 2^-20 of it, so the division itself is only made
-// where the product lies that near a half.  Adding 1.5 * 2^23 rounds to a
+// (IEEE float32 division, ties to even).  |w / scale| is at most 7 (1 + 2^-8),
+// so nothing is left to clip, and w * (1 / scale) is within 2^-20 of it, so the
+// division itself is only made where the product lies that near a half.  Adding 1.5 * 2^23 rounds to a
 // whole number, ties to even, and leaves it in the low byte (the conversion
 // instructions run at a quarter of the rate).  Memory bound: 14336 x 4096
 // float32, groups of 128, 57 us = 5.2 TB/s; with a division per element 103.
@@ -86,7 +86,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return m;
 }
 template <typename WT, typename ST, int GS, bool VEC>
-__global__ void __launch_bounds__(4 * GS, GS == 128 ? 2 : 1)
+__global__ void __launch_bounds__(4 * GS, 256 / GS)
     quantize_q4_kernel(const WT* __restrict__ w, int64_t K, int64_t N, int64_t KB,
                        int8_t* __restrict__ q, ST* __restrict__ scale) {
     constexpr int R = 8, W = GS / R;
@@ -142,18 +142,21 @@ __global__ void __launch_bounds__(4 * GS, GS == 128 ? 2 : 1)
     for (int i = 0; i < R; ++i) {
         if (i >= rows || !on) continue;
         uint32_t c[4];
-        bool near = false;
+        float off = 0.0f;  // the largest distance from a whole number
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float d = fminf(fmaxf(v[i][j] * inv[j], -7.0f), 7.0f);  // clipping commutes with rint
-            const float r = d + kRint;
-            near |= fabsf(d - (r - kRint)) > 0.5f - 0x1p-18f;
-            c[j] = __float_as_uint(r);
+        for (int j = 0; j < 4; j += 2) {
+            float r0, r1, e0, e1;
+            asm("{\n.reg .b64 v, s, k, r, e;\nmov.b64 v, {%4, %5};\nmov.b64 s, {%6, %7};\nmov.b64 k, {%8, %8};\n"
+                "fma.rn.f32x2 r, v, s, k;\nsub.rn.f32x2 e, k, r;\nfma.rn.f32x2 e, v, s, e;\n"
+                "mov.b64 {%0, %1}, r;\nmov.b64 {%2, %3}, e;\n}"
+                : "=f"(r0), "=f"(r1), "=f"(e0), "=f"(e1)
+                : "f"(v[i][j]), "f"(v[i][j + 1]), "f"(inv[j]), "f"(inv[j + 1]), "f"(kRint));
+            c[j] = __float_as_uint(r0), c[j + 1] = __float_as_uint(r1);
+            off = fmaxf(off, fmaxf(fabsf(e0), fabsf(e1)));
         }
-        if (near)
+        if (off > 0.5f - 0x1p-18f)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                c[j] = __float_as_uint(fminf(fmaxf(__fdiv_rn(v[i][j], s[j]), -7.0f), 7.0f) + kRint);
+            for (int j = 0; j < 4; ++j) c[j] = __float_as_uint(__fdiv_rn(v[i][j], s[j]) + kRint);
         int8_t* p = q + at + i * step;
         if constexpr (VEC) {
             *reinterpret_cast<uint32_t*>(p) =
