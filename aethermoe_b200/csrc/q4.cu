@@ -68,16 +68,18 @@ namespace {
 constexpr int kThreads = 256;  // pack
 
 // ------------------------------------------------------------------ quantise
-// One block per (128 columns, scale group): GS / 8 warps hold 8 rows of the
-// group each in registers, 4 columns per lane, so w is read once; the column
-// maxima meet in shared memory.  scale = max(amax / 7, 1e-12), rounded to
-// the scale's type before q = clip(rint(w / scale), -7, 7) is taken with it
-// (IEEE float32 division, ties to even).  |w / scale| is at most 7 (1 + 2^-8),
-// so nothing is left to clip, and w * (1 / scale) is within 2^-20 of it, so the
-// division itself is only made where the product lies that near a half.  Adding 1.5 * 2^23 rounds to a
-// whole number, ties to even, and leaves it in the low byte (the conversion
-// instructions run at a quarter of the rate).  Memory bound: 14336 x 4096
-// float32, groups of 128, 57 us = 5.2 TB/s; with a division per element 103.
+// One block per (128 float32 or 256 bf16 columns, scale group): GS / 8 warps
+// hold 8 rows of the group each in registers, 16 bytes a lane, so w is read
+// once; the column maxima meet in shared memory.  scale = max(amax / 7, 1e-12),
+// rounded to the scale's type before q = clip(rint(w / scale), -7, 7) is taken
+// with it (IEEE float32 division, ties to even).  |w / scale| is at most
+// 7 (1 + 2^-8), so nothing is left to clip, and w * (1 / scale) is within 2^-20
+// of it, so the division itself is only made where the product lies that near a
+// half.  Adding 1.5 * 2^23 rounds to a whole number, ties to even, and leaves it
+// in the low byte (the conversion instructions run at a quarter of the rate).
+// 14336 x 4096, groups of 128: float32 53.4 us = 5.5 TB/s, memory bound (with a
+// division per element 103); bf16 47.7, the wait for the maxima between loads
+// and stores the bound.
 constexpr float kRint = 12582912.0f;
 // Maximum that keeps a NaN: its group's scale has to be one.
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -89,78 +91,101 @@ template <typename WT, typename ST, int GS, bool VEC>
 __global__ void __launch_bounds__(4 * GS, 256 / GS)
     quantize_q4_kernel(const WT* __restrict__ w, int64_t K, int64_t N, int64_t KB,
                        int8_t* __restrict__ q, ST* __restrict__ scale) {
-    constexpr int R = 8, W = GS / R;
-    __shared__ float4 amax[W][32], scales[32], inverses[32];
+    // CL columns a lane: 16 bytes, kept as loaded
+    constexpr int R = 8, W = GS / R, CL = VEC && sizeof(WT) == 2 ? 8 : 4, COLS = 32 * CL;
+    __shared__ __align__(16) float amax[W][COLS], scales[COLS], inverses[COLS];
     const int lane = threadIdx.x & 31, wi = threadIdx.x >> 5;
     const int64_t g = blockIdx.x / KB, b = blockIdx.x % KB;
-    const int64_t n0 = blockIdx.y * 128ll + lane * 4, k0 = b * GS + wi;
+    const int64_t c0 = static_cast<int64_t>(blockIdx.y) * COLS, n0 = c0 + lane * CL, k0 = b * GS + wi;
     const int rows = static_cast<int>(min(static_cast<int64_t>(R), (K - k0 + W - 1) / W));  // k0 + i * W < K
     const int64_t at = (g * K + k0) * N + n0, step = W * N;
     const bool on = n0 < N;
-    float v[R][4];
+    uint32_t v[R][4];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.f;
+        v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0;
         if (i >= rows || !on) continue;
         const WT* p = w + at + i * step;
-        if constexpr (VEC && sizeof(WT) == 4) {
-            const float4 f = *reinterpret_cast<const float4*>(p);
-            v[i][0] = f.x, v[i][1] = f.y, v[i][2] = f.z, v[i][3] = f.w;
-        } else if constexpr (VEC) {
-            const uint2 u = *reinterpret_cast<const uint2*>(p);
-            v[i][0] = __uint_as_float(u.x << 16), v[i][1] = __uint_as_float(u.x & 0xffff0000u);
-            v[i][2] = __uint_as_float(u.y << 16), v[i][3] = __uint_as_float(u.y & 0xffff0000u);
+        if constexpr (VEC) {
+            const uint4 u = *reinterpret_cast<const uint4*>(p);
+            v[i][0] = u.x, v[i][1] = u.y, v[i][2] = u.z, v[i][3] = u.w;
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (n0 + j < N) v[i][j] = static_cast<float>(p[j]);
+                if (n0 + j < N) v[i][j] = __float_as_uint(static_cast<float>(p[j]));
         }
     }
-    float m[4] = {0.f, 0.f, 0.f, 0.f};
+    auto value = [&](int i, int j) {
+        if constexpr (CL == 8) return __uint_as_float(j & 1 ? v[i][j / 2] & 0xffff0000u : v[i][j / 2] << 16);
+        return __uint_as_float(v[i][j]);
+    };
+    float m[CL] = {};
+    if constexpr (CL == 8) {  // two magnitudes at a time, as they are
+        __nv_bfloat162 top[4] = {};
 #pragma unroll
-    for (int i = 0; i < R; ++i)
+        for (int i = 0; i < R; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) m[j] = max_nan(m[j], fabsf(v[i][j]));
-    amax[wi][lane] = make_float4(m[0], m[1], m[2], m[3]);
+            for (int j = 0; j < 4; ++j)
+                top[j] = __hmax2_nan(top[j], __habs2(*reinterpret_cast<const __nv_bfloat162*>(&v[i][j])));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m[j] = j & 1 ? __high2float(top[j / 2]) : __low2float(top[j / 2]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int j = 0; j < CL; ++j) m[j] = max_nan(m[j], fabsf(value(i, j)));
+    }
+#pragma unroll
+    for (int j = 0; j < CL; j += 4)
+        *reinterpret_cast<float4*>(&amax[wi][lane * CL + j]) = make_float4(m[j], m[j + 1], m[j + 2], m[j + 3]);
     __syncthreads();
-    if (threadIdx.x < 128) {  // one thread per column
-        const float* col = reinterpret_cast<const float*>(amax) + threadIdx.x;
+    for (int c = threadIdx.x; c < COLS; c += 4 * GS) {  // one thread per column
         float a = 0.0f;
 #pragma unroll
-        for (int i = 0; i < W; ++i) a = max_nan(a, col[i * 128]);
+        for (int i = 0; i < W; ++i) a = max_nan(a, amax[i][c]);
         float sc = max_nan(__fdiv_rn(a, 7.0f), 1e-12f);
         if constexpr (sizeof(ST) == 2) sc = __bfloat162float(__float2bfloat16_rn(sc));
-        reinterpret_cast<float*>(scales)[threadIdx.x] = sc;
-        reinterpret_cast<float*>(inverses)[threadIdx.x] = __frcp_rn(sc);
-        const int64_t n = blockIdx.y * 128ll + threadIdx.x;
-        if (n < N) scale[(g * KB + b) * N + n] = static_cast<ST>(sc);
+        scales[c] = sc;
+        inverses[c] = __frcp_rn(sc);
+        if (c0 + c < N) scale[(g * KB + b) * N + c0 + c] = static_cast<ST>(sc);
     }
     __syncthreads();
-    const float4 s4 = scales[lane], i4 = inverses[lane];
-    const float s[4] = {s4.x, s4.y, s4.z, s4.w}, inv[4] = {i4.x, i4.y, i4.z, i4.w};
+    float inv[CL];
+#pragma unroll
+    for (int j = 0; j < CL; j += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(&inverses[lane * CL + j]);
+        inv[j] = f.x, inv[j + 1] = f.y, inv[j + 2] = f.z, inv[j + 3] = f.w;
+    }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         if (i >= rows || !on) continue;
-        uint32_t c[4];
+        uint32_t c[CL];
         float off = 0.0f;  // the largest distance from a whole number
 #pragma unroll
-        for (int j = 0; j < 4; j += 2) {
+        for (int j = 0; j < CL; j += 2) {
             float r0, r1, e0, e1;
             asm("{\n.reg .b64 v, s, k, r, e;\nmov.b64 v, {%4, %5};\nmov.b64 s, {%6, %7};\nmov.b64 k, {%8, %8};\n"
                 "fma.rn.f32x2 r, v, s, k;\nsub.rn.f32x2 e, k, r;\nfma.rn.f32x2 e, v, s, e;\n"
                 "mov.b64 {%0, %1}, r;\nmov.b64 {%2, %3}, e;\n}"
                 : "=f"(r0), "=f"(r1), "=f"(e0), "=f"(e1)
-                : "f"(v[i][j]), "f"(v[i][j + 1]), "f"(inv[j]), "f"(inv[j + 1]), "f"(kRint));
+                : "f"(value(i, j)), "f"(value(i, j + 1)), "f"(inv[j]), "f"(inv[j + 1]), "f"(kRint));
             c[j] = __float_as_uint(r0), c[j + 1] = __float_as_uint(r1);
             off = fmaxf(off, fmaxf(fabsf(e0), fabsf(e1)));
         }
         if (off > 0.5f - 0x1p-18f)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) c[j] = __float_as_uint(__fdiv_rn(v[i][j], s[j]) + kRint);
+            for (int j = 0; j < CL; ++j)
+                c[j] = __float_as_uint(__fdiv_rn(value(i, j), scales[lane * CL + j]) + kRint);
         int8_t* p = q + at + i * step;
         if constexpr (VEC) {
-            *reinterpret_cast<uint32_t*>(p) =
-                __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+            uint32_t o[CL / 4];
+#pragma unroll
+            for (int j = 0; j < CL; j += 4)
+                o[j / 4] = __byte_perm(__byte_perm(c[j], c[j + 1], 0x0040), __byte_perm(c[j + 2], c[j + 3], 0x0040), 0x5410);
+            if constexpr (CL == 8)
+                *reinterpret_cast<uint2*>(p) = make_uint2(o[0], o[1]);
+            else
+                *reinterpret_cast<uint32_t*>(p) = o[0];
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -1099,9 +1124,11 @@ template <typename WT, typename ST>
 void launch_quantize(const void* w, int64_t G, int64_t K, int64_t N, int gs, int8_t* q, void* scale,
                      cudaStream_t s) {
     const int64_t KB = (K + gs - 1) / gs;
-    const dim3 grid(static_cast<unsigned>(G * KB), static_cast<unsigned>((N + 127) / 128));
-    const bool vec = N % 4 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0 &&
-                     reinterpret_cast<uintptr_t>(q) % 4 == 0;
+    constexpr int CL = 16 / sizeof(WT);  // columns of a lane where rows can be read in vectors
+    const bool vec = N % CL == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0 &&
+                     reinterpret_cast<uintptr_t>(q) % CL == 0;
+    const int64_t cols = 32 * (vec ? CL : 4);
+    const dim3 grid(static_cast<unsigned>(G * KB), static_cast<unsigned>((N + cols - 1) / cols));
     auto* wt = static_cast<const WT*>(w);
     auto* st = static_cast<ST*>(scale);
     auto go = [&](auto size) {
