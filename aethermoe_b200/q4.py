@@ -21,6 +21,7 @@ from .dispatch import _DT, _apart, _matrix, _on, _output
 
 
 def _quantize(w, group_size, scale_dtype, s):
+    w = w.contiguous()  # on the call's stream, like everything that reads it
     g = 1 if w.dim() == 2 else w.shape[0]
     k, n = w.shape[-2:]
     kb = -(-k // group_size)
@@ -42,7 +43,7 @@ def quantize_q4(w, group_size=128, scale_dtype=torch.float32, stream=None):
         raise ValueError(f"unsupported dtype {w.dtype} / {scale_dtype} (float32 or bfloat16)")
     if group_size not in (32, 64, 128):
         raise ValueError(f"group_size={group_size} is not 32, 64 or 128")
-    return _on(stream, _quantize, (w,), (w.contiguous(), group_size, scale_dtype))
+    return _on(stream, _quantize, (w,), (w, group_size, scale_dtype))
 
 
 class Q4Weight:
@@ -66,10 +67,10 @@ class Q4Weight:
         want = tuple(q.shape[:-2]) + (-(-k // group_size), n)
         if tuple(scale.shape) != want:
             raise ValueError(f"scale must be {want}, got {tuple(scale.shape)}")
-        q, scale = q.contiguous(), scale.contiguous()
         h = ctypes.c_void_p()
         if q.is_cuda:
-            def pack(s):
+            def pack(q, scale, s):
+                q, scale = q.contiguous(), scale.contiguous()  # on the call's stream
                 L = _lib.lib()
                 _lib.check(L.aem_q4weight_pack_device(q.data_ptr(), scale.data_ptr(), _DT[scale.dtype], g,
                                                       k, n, group_size, s, ctypes.byref(h)),
@@ -81,9 +82,10 @@ class Q4Weight:
                     if st == _lib.AEM_EDEVICE:
                         raise ValueError(f"Q4Weight: {message}")
                     raise _lib.AemError(st, message)
-            _on(stream, pack, (q, scale), ())
+            _on(stream, pack, (q, scale), (q, scale))
             device = q.device.index
         else:
+            q, scale = q.contiguous(), scale.contiguous()
             _lib.check(_lib.lib().aem_q4weight_pack(q.data_ptr(), scale.data_ptr(), _DT[scale.dtype], g,
                                                     k, n, group_size, device, ctypes.byref(h)),
                        "aem_q4weight_pack")

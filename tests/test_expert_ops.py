@@ -132,3 +132,32 @@ def test_overlapping_matrices():
     assert not D._overlap(b[:4], b[4:]) and D._overlap(b[:5], b[4:])
     assert not D._overlap(b[:0], b) and not D._overlap(b, torch.zeros(8, 192))
     assert D._overlap(b[:1].expand(8, 192), b[1:, :1]) is False and D._overlap(b[:1].expand(8, 192), b)
+
+
+def test_copies_of_strided_weights_wait_for_the_stream(monkeypatch):
+    """A strided weight is copied on the stream that the call was given, so not before
+    that stream is entered: a copy on the caller's stream would not be waited for."""
+    class Entered(Exception):
+        pass
+
+    seen = []
+
+    class Weight(torch.Tensor):
+        is_cuda = True
+
+        def contiguous(self, *args, **kwargs):
+            seen.append("copied")
+            return super().contiguous(*args, **kwargs)
+
+    def enter(stream, fn, tensors, args):
+        seen.append("entered")
+        raise Entered
+
+    monkeypatch.setattr(q4, "_on", enter)
+    w = torch.zeros(32, 64).as_subclass(Weight).t()
+    q = torch.zeros(32, 64, dtype=torch.int8).as_subclass(Weight).t()
+    scale = torch.ones(32, 2).as_subclass(Weight).t()
+    for call in (lambda: q4.quantize_q4(w, 32, stream="side"), lambda: q4.Q4Weight(q, scale, 32, stream="side")):
+        with pytest.raises(Entered):
+            call()
+    assert seen == ["entered", "entered"]
