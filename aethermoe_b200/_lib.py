@@ -124,6 +124,8 @@ _SIGS = {
     "aem_q4weight_pack": (_int, [_vp, _vp, _int, _i64, _i64, _i64, _int, _int, ctypes.POINTER(_vp)]),
     "aem_q4weight_pack_device": (_int, [_vp, _vp, _int, _i64, _i64, _i64, _int, _vp,
                                         ctypes.POINTER(_vp)]),
+    "aem_q4weight_pack_checked": (_int, [_vp, _vp, _int, _i64, _i64, _i64, _int, _vp,
+                                         ctypes.POINTER(_vp)]),
     "aem_q4weight_free": (_int, [_vp]),
     "aem_q4weight_shape": (_int, [_vp, ctypes.POINTER(_i64), ctypes.POINTER(_i64),
                                   ctypes.POINTER(_i64), ctypes.POINTER(_int)]),

@@ -1161,6 +1161,73 @@ aem_status check_q4_shape(const char* what, int64_t G, int64_t K, int64_t N, int
     return AEM_OK;
 }
 
+// Packs from device memory.  checked: waits, and a value out of range is an
+// error of this call alone, through a flag behind the weight's blocks; else it
+// is reported in the device's error word.
+aem_status pack_q4(const int8_t* q, const void* scale, aem_dtype scale_dtype, int64_t G, int64_t K,
+                   int64_t N, int group_size, cudaStream_t s, bool checked, aem_q4weight_t* out) {
+    AEM_REQUIRE(out != nullptr, "aem_q4weight_pack: out is NULL");
+    *out = nullptr;
+    AEM_TRY(check_q4_shape("aem_q4weight_pack", G, K, N, group_size, scale_dtype));
+    AEM_REQUIRE(q && scale, "aem_q4weight_pack: NULL buffer");
+    int* err = device_error_word(current_device());
+    auto* w = new (std::nothrow) Q4Weight();
+    if (!err || !w) {
+        delete w;
+        set_error("aem_q4weight_pack: out of memory");
+        return AEM_ENOMEM;
+    }
+    w->device = current_device();
+    w->G = G;
+    w->K = K;
+    w->N = N;
+    w->NC = (N + 127) / 128;
+    w->NP = (K + 127) / 128;
+    w->gs = group_size;
+    w->scale_bf16 = scale_dtype == AEM_BF16;
+    const int per = 128 / group_size;
+    w->block = 8192 + per * 128 * (w->scale_bf16 ? 2 : 4);
+    const int64_t blocks = G * w->NC * w->NP, KB = (K + group_size - 1) / group_size;
+    const size_t bytes = static_cast<size_t>(blocks) * w->block;
+    if (cudaMalloc(&w->data, bytes + sizeof(int)) != cudaSuccess) {
+        cudaGetLastError();
+        free_q4(w);
+        set_error("aem_q4weight_pack: device allocation failed");
+        return AEM_ENOMEM;
+    }
+    int* flag = reinterpret_cast<int*>(w->data + bytes);
+    if (checked) {
+        cudaMemsetAsync(flag, 0, sizeof(int), s);
+        err = flag;
+    }
+    const unsigned g1 = static_cast<unsigned>(std::min<int64_t>(blocks * 2, 148 * 64));
+    pack_q4_kernel<<<g1, kThreads, 0, s>>>(q, K, N, w->NC, w->NP, blocks * 512, w->block, w->data, err);
+    const int64_t scales = blocks * per * 128;
+    const unsigned g2 = static_cast<unsigned>(std::min<int64_t>((scales + 255) / 256, 148 * 64));
+    if (w->scale_bf16)
+        pack_q4_scale_kernel<__nv_bfloat16><<<g2, kThreads, 0, s>>>(
+            static_cast<const __nv_bfloat16*>(scale), KB, N, w->NC, w->NP, scales, per, w->block, w->data);
+    else
+        pack_q4_scale_kernel<float><<<g2, kThreads, 0, s>>>(
+            static_cast<const float*>(scale), KB, N, w->NC, w->NP, scales, per, w->block, w->data);
+    cudaError_t e = cudaGetLastError();
+    int bad = 0;
+    if (checked && e == cudaSuccess) e = cudaMemcpyAsync(&bad, flag, sizeof(int), cudaMemcpyDeviceToHost, s);
+    if (checked && e == cudaSuccess) e = cudaStreamSynchronize(s);
+    if (e != cudaSuccess || bad) {
+        free_q4(w);
+        if (e == cudaSuccess) {
+            set_error("aem_q4weight_pack: a 4-bit weight is outside [-7, 7]");
+            return AEM_EINVAL;
+        }
+        set_error("aem_q4weight_pack: %s", cudaGetErrorString(e));
+        return AEM_ECUDA;
+    }
+    count_launches(2);
+    *out = reinterpret_cast<aem_q4weight_t>(w);
+    return AEM_OK;
+}
+
 }  // namespace
 
 }  // namespace aem
@@ -1193,54 +1260,13 @@ aem_status aem_quantize_q4(const void* w, aem_dtype w_dtype, int64_t G, int64_t 
 aem_status aem_q4weight_pack_device(const int8_t* q, const void* scale, aem_dtype scale_dtype,
                                     int64_t G, int64_t K, int64_t N, int group_size, void* stream,
                                     aem_q4weight_t* out) {
-    AEM_REQUIRE(out != nullptr, "aem_q4weight_pack: out is NULL");
-    *out = nullptr;
-    AEM_TRY(aem::check_q4_shape("aem_q4weight_pack", G, K, N, group_size, scale_dtype));
-    AEM_REQUIRE(q && scale, "aem_q4weight_pack: NULL buffer");
-    auto s = static_cast<cudaStream_t>(stream);
-    int* err = aem::device_error_word(aem::current_device());
-    auto* w = new (std::nothrow) aem::Q4Weight();
-    if (!err || !w) {
-        delete w;
-        set_error("aem_q4weight_pack: out of memory");
-        return AEM_ENOMEM;
-    }
-    w->device = aem::current_device();
-    w->G = G;
-    w->K = K;
-    w->N = N;
-    w->NC = (N + 127) / 128;
-    w->NP = (K + 127) / 128;
-    w->gs = group_size;
-    w->scale_bf16 = scale_dtype == AEM_BF16;
-    const int per = 128 / group_size;
-    w->block = 8192 + per * 128 * (w->scale_bf16 ? 2 : 4);
-    const int64_t blocks = G * w->NC * w->NP, KB = (K + group_size - 1) / group_size;
-    if (cudaMalloc(&w->data, static_cast<size_t>(blocks) * w->block) != cudaSuccess) {
-        cudaGetLastError();
-        aem::free_q4(w);
-        set_error("aem_q4weight_pack: device allocation failed");
-        return AEM_ENOMEM;
-    }
-    const unsigned g1 = static_cast<unsigned>(std::min<int64_t>(blocks * 2, 148 * 64));
-    aem::pack_q4_kernel<<<g1, aem::kThreads, 0, s>>>(q, K, N, w->NC, w->NP, blocks * 512, w->block, w->data, err);
-    const int64_t scales = blocks * per * 128;
-    const unsigned g2 = static_cast<unsigned>(std::min<int64_t>((scales + 255) / 256, 148 * 64));
-    if (w->scale_bf16)
-        aem::pack_q4_scale_kernel<__nv_bfloat16><<<g2, aem::kThreads, 0, s>>>(
-            static_cast<const __nv_bfloat16*>(scale), KB, N, w->NC, w->NP, scales, per, w->block, w->data);
-    else
-        aem::pack_q4_scale_kernel<float><<<g2, aem::kThreads, 0, s>>>(
-            static_cast<const float*>(scale), KB, N, w->NC, w->NP, scales, per, w->block, w->data);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) {
-        aem::free_q4(w);
-        set_error("aem_q4weight_pack: launch failed: %s", cudaGetErrorString(e));
-        return AEM_ECUDA;
-    }
-    aem::count_launches(2);
-    *out = reinterpret_cast<aem_q4weight_t>(w);
-    return AEM_OK;
+    return aem::pack_q4(q, scale, scale_dtype, G, K, N, group_size, static_cast<cudaStream_t>(stream), false, out);
+}
+
+aem_status aem_q4weight_pack_checked(const int8_t* q, const void* scale, aem_dtype scale_dtype,
+                                     int64_t G, int64_t K, int64_t N, int group_size, void* stream,
+                                     aem_q4weight_t* out) {
+    return aem::pack_q4(q, scale, scale_dtype, G, K, N, group_size, static_cast<cudaStream_t>(stream), true, out);
 }
 
 aem_status aem_q4weight_pack(const int8_t* q, const void* scale, aem_dtype scale_dtype, int64_t G,

@@ -71,17 +71,9 @@ class Q4Weight:
         if q.is_cuda:
             def pack(q, scale, s):
                 q, scale = q.contiguous(), scale.contiguous()  # on the call's stream
-                L = _lib.lib()
-                _lib.check(L.aem_q4weight_pack_device(q.data_ptr(), scale.data_ptr(), _DT[scale.dtype], g,
-                                                      k, n, group_size, s, ctypes.byref(h)),
-                           "aem_q4weight_pack_device")
-                st = L.aem_device_status(s)
-                if st != _lib.AEM_OK:
-                    message = _lib.last_error()
-                    L.aem_q4weight_free(h.value)
-                    if st == _lib.AEM_EDEVICE:
-                        raise ValueError(f"Q4Weight: {message}")
-                    raise _lib.AemError(st, message)
+                st = _lib.lib().aem_q4weight_pack_checked(q.data_ptr(), scale.data_ptr(), _DT[scale.dtype], g,
+                                                          k, n, group_size, s, ctypes.byref(h))
+                _lib.check(st, "aem_q4weight_pack_checked")
             _on(stream, pack, (q, scale), (q, scale))
             device = q.device.index
         else:

@@ -356,13 +356,18 @@ typedef struct aem_q4weight_s* aem_q4weight_t;
  * given), into a device-resident copy laid out in blocks of 128 k x 128
  * channels with their scales: K*N/2 bytes per group and the scales, K and N
  * rounded up to 128.  Same from HOST memory (a value outside
- * [-7, 7] -> AEM_EINVAL) and from DEVICE memory (stream-ordered; such a value
- * is clamped and reported by aem_device_status). */
+ * [-7, 7] -> AEM_EINVAL) and from DEVICE memory: either stream-ordered (such a
+ * value is clamped and reported by aem_device_status, which every caller of the
+ * device shares) or checked, where the call waits for the stream and such a
+ * value is AEM_EINVAL of this call alone. */
 aem_status aem_q4weight_pack(const int8_t* q, const void* scale, aem_dtype scale_dtype, int64_t G,
                              int64_t K, int64_t N, int group_size, int device, aem_q4weight_t* out);
 aem_status aem_q4weight_pack_device(const int8_t* q, const void* scale, aem_dtype scale_dtype,
                                     int64_t G, int64_t K, int64_t N, int group_size, void* stream,
                                     aem_q4weight_t* out);
+aem_status aem_q4weight_pack_checked(const int8_t* q, const void* scale, aem_dtype scale_dtype,
+                                     int64_t G, int64_t K, int64_t N, int group_size, void* stream,
+                                     aem_q4weight_t* out);
 aem_status aem_q4weight_free(aem_q4weight_t w);
 /* Dimensions of a packed weight (any pointer may be NULL). */
 aem_status aem_q4weight_shape(aem_q4weight_t w, int64_t* G, int64_t* K, int64_t* N, int* group_size);

@@ -161,3 +161,13 @@ def test_copies_of_strided_weights_wait_for_the_stream(monkeypatch):
         with pytest.raises(Entered):
             call()
     assert seen == ["entered", "entered"]
+
+
+def test_checked_pack_refusals():
+    h = ctypes.c_void_p(1)
+
+    def pack(q=P, s=P, sd=_lib.F32, G=1, K=64, N=32, gs=32, out=True):
+        return L().aem_q4weight_pack_checked(q, s, sd, G, K, N, gs, None, ctypes.byref(h) if out else None)
+    for bad in (dict(q=None), dict(s=None), dict(sd=5), dict(G=0), dict(K=0), dict(N=-1), dict(gs=16)):
+        assert pack(**bad) == EINVAL and not h.value, bad
+    assert pack(out=False) == EINVAL
