@@ -189,12 +189,28 @@ def _weights(weights, shape):
     return weights, weights.stride(0) if shape[0] > 1 else shape[1]
 
 
-def _differentiable(what, out, *tensors):
+def _capturing(stream):
+    if stream is None:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.stream(stream):
+        return torch.cuda.is_current_stream_capturing()
+
+
+def _apply(fn, stream, *args):
+    """``fn.apply`` on ``stream``: autograd runs the backward pass on the stream that
+    was current here, which so is the one that owns what the forward pass kept."""
+    if stream is None:
+        return fn.apply(*args, None)
+    with torch.cuda.stream(stream):
+        return fn.apply(*args, stream)
+
+
+def _differentiable(what, out, stream, *tensors):
     if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
         return False
     if out is not None:
         raise RuntimeError(f"{what}: out= does not take part in autograd, but an input requires a gradient")
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing(stream):
         raise RuntimeError(f"{what}: the differentiable form cannot be captured into a CUDA graph; "
                            "capture detached tensors and the *_backward call")
     return True
@@ -337,17 +353,17 @@ def dispatch(x, ids, num_experts, out=None, stream=None):
     """``(rows [T*k, d], TokenOrder)``: token ``t``'s row of ``x [T, d]`` at every
     ``order.row_of[t, j]``; rows from ``order.starts[E]`` on are zero."""
     _ids(ids, num_experts)
-    if _differentiable("dispatch", out, x):
+    if _differentiable("dispatch", out, stream, x):
         holder = []
-        rows = _DispatchFn.apply(x, ids, num_experts, None, holder, stream)
+        rows = _apply(_DispatchFn, stream, x, ids, num_experts, None, holder)
         return rows, holder[0]
     return _on(stream, _dispatch, (x, ids, out), (x, ids, num_experts, out))
 
 
 def dispatch_rows(x, order, out=None, stream=None):
     """Rows of another ``x [T, d]`` by an existing order."""
-    if _differentiable("dispatch_rows", out, x):
-        return _DispatchFn.apply(x, None, 0, order, None, stream)
+    if _differentiable("dispatch_rows", out, stream, x):
+        return _apply(_DispatchFn, stream, x, None, 0, order, None)
     return _on(stream, _dispatch_rows, (x, order, out), (x, order, out))
 
 
@@ -360,8 +376,8 @@ def combine(rows, weights, order, out_dtype=None, out=None, stream=None):
     """``out[t] = sum_j weights[t, j] * rows[row_of[t, j]]`` (``rows [T*k, d]``,
     ``weights [T, k]`` float32 or ``None`` for 1; ``out_dtype`` defaults to the
     rows')."""
-    if _differentiable("combine", out, rows, weights):
-        return _CombineFn.apply(rows, weights, order, out_dtype, stream)
+    if _differentiable("combine", out, stream, rows, weights):
+        return _apply(_CombineFn, stream, rows, weights, order, out_dtype)
     return _on(stream, _combine, (rows, weights, order, out), (rows, weights, order, out_dtype, out))
 
 

@@ -171,3 +171,33 @@ def test_checked_pack_refusals():
     for bad in (dict(q=None), dict(s=None), dict(sd=5), dict(G=0), dict(K=0), dict(N=-1), dict(gs=16)):
         assert pack(**bad) == EINVAL and not h.value, bad
     assert pack(out=False) == EINVAL
+
+
+def test_gradients_belong_to_the_stream_of_the_call(monkeypatch):
+    """The differentiable forms are applied with the given stream current, so autograd
+    runs their backward pass there, on the stream that owns the order it reads."""
+    seen = []
+
+    class Stream:
+        def __init__(self, stream):
+            self.stream = stream
+
+        def __enter__(self):
+            seen.append(("enter", self.stream))
+
+        def __exit__(self, *args):
+            seen.append(("exit", self.stream))
+
+    monkeypatch.setattr(torch.cuda, "stream", Stream)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    for fn in (D._DispatchFn, D._CombineFn):
+        monkeypatch.setattr(fn, "apply", lambda *args: seen.append("apply"))
+    order = D.TokenOrder(torch.zeros(3, dtype=torch.int32), torch.zeros(4, 2, dtype=torch.int32),
+                         torch.zeros(8, dtype=torch.int32))
+    x = torch.zeros(4, 8, requires_grad=True)
+    for call in (lambda: D.dispatch_rows(x, order, stream="side"),
+                 lambda: D.combine(x.new_zeros(8, 8).requires_grad_(), torch.ones(4, 2), order, stream="side")):
+        seen.clear()
+        call()
+        at = seen.index("apply")
+        assert seen[at - 1:] == [("enter", "side"), "apply", ("exit", "side")]
