@@ -17,11 +17,12 @@ take part in autograd when an input requires a gradient; a training step that
 is captured into a CUDA graph calls ``dispatch_backward`` and
 ``combine_backward`` itself, because autograd's accumulation into leaves runs
 on streams that the capture does not own (the differentiable forms refuse to
-be captured).
+be captured).  Forward-mode tangents are refused everywhere.
 """
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -205,7 +206,15 @@ def _apply(fn, stream, *args):
         return fn.apply(*args, stream)
 
 
+def _no_tangent(what, *tensors):
+    """Refuses dual tensors: no call carries forward-mode tangents."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode gradient")
+
+
 def _differentiable(what, out, stream, *tensors):
+    _no_tangent(what, *tensors)
     if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
         return False
     if out is not None:
@@ -369,6 +378,7 @@ def dispatch_rows(x, order, out=None, stream=None):
 
 def dispatch_backward(grad_rows, order, out_dtype=None, out=None, stream=None):
     """Gradient of ``dispatch``: ``grad_x[t] = sum_j grad_rows[row_of[t, j]]``."""
+    _no_tangent("dispatch_backward", grad_rows)
     return _on(stream, _combine, (grad_rows, order, out), (grad_rows, None, order, out_dtype, out))
 
 
@@ -384,5 +394,6 @@ def combine(rows, weights, order, out_dtype=None, out=None, stream=None):
 def combine_backward(grad_out, rows, weights, order, stream=None):
     """Gradients of ``combine``: ``(grad_rows [T*k, d]`` in the rows' dtype,
     ``grad_weights [T, k]`` float32``)``."""
+    _no_tangent("combine_backward", grad_out, rows, weights)
     return _on(stream, _combine_backward, (grad_out, rows, weights, order),
                (grad_out, rows, weights, order, rows.dtype, True, True))

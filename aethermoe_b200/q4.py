@@ -17,7 +17,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .dispatch import _DT, _apart, _matrix, _on, _output
+from .dispatch import _DT, _apart, _matrix, _no_tangent, _on, _output
 
 
 def _quantize(w, group_size, scale_dtype, s):
@@ -147,6 +147,7 @@ def _grouped(x, w, starts, relu, out_dtype, out, s):
 
 
 def _no_gradient(what, x):
+    _no_tangent(what, x)
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{what} has no gradient: detach x or call it under torch.no_grad()")
 

@@ -201,3 +201,26 @@ def test_gradients_belong_to_the_stream_of_the_call(monkeypatch):
         call()
         at = seen.index("apply")
         assert seen[at - 1:] == [("enter", "side"), "apply", ("exit", "side")]
+
+
+def test_forward_mode_is_refused():
+    """A dual tensor does not require a gradient, so its tangent would be dropped."""
+    from torch.autograd import forward_ad
+    order = D.TokenOrder(torch.zeros(3, dtype=torch.int32), torch.zeros(4, 2, dtype=torch.int32),
+                         torch.zeros(8, dtype=torch.int32))
+    ids = torch.zeros(4, 2, dtype=torch.int32)
+    starts = torch.zeros(2, dtype=torch.int32)
+    x, rows, w = torch.zeros(4, 8), torch.zeros(8, 8), torch.ones(4, 2)
+    with forward_ad.dual_level():
+        dx, drows, dw = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, rows, w))
+        for call in (lambda: D.dispatch(dx, ids, 2), lambda: D.dispatch_rows(dx, order),
+                     lambda: D.combine(drows, w, order), lambda: D.combine(rows, dw, order),
+                     lambda: D.combine(drows, None, order), lambda: D.dispatch_backward(drows, order),
+                     lambda: D.combine_backward(dx, rows, w, order), lambda: D.combine_backward(x, rows, dw, order),
+                     lambda: q4.q4_matmul(dx, None), lambda: q4.grouped_q4_matmul(dx, None, starts)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        with pytest.raises(ValueError, match="CUDA"):  # no tangent: past that check
+            D.dispatch(x, ids, 2)
+    with pytest.raises(ValueError, match="CUDA"):
+        D.dispatch(x, ids, 2)
