@@ -20,6 +20,12 @@ from . import _lib
 from .dispatch import _DT, _apart, _matrix, _no_tangent, _on, _output
 
 
+def _no_gradient(what, x, name="x"):
+    _no_tangent(what, x)
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{what} has no gradient: detach {name} or call it under torch.no_grad()")
+
+
 def _quantize(w, group_size, scale_dtype, s):
     w = w.contiguous()  # on the call's stream, like everything that reads it
     g = 1 if w.dim() == 2 else w.shape[0]
@@ -36,7 +42,8 @@ def _quantize(w, group_size, scale_dtype, s):
 def quantize_q4(w, group_size=128, scale_dtype=torch.float32, stream=None):
     """``w [K, N]`` or ``[G, K, N]`` (float32 or bfloat16) -> ``(q int8, scale)`` with
     ``scale [(G,) ceil(K/group_size), N]``: symmetric, values in [-7, 7], the
-    ``group_size`` (32, 64, 128) consecutive k of a column sharing a scale."""
+    ``group_size`` (32, 64, 128) consecutive k of a column sharing a scale.  No gradient."""
+    _no_gradient("quantize_q4", w, "w")
     if w.dim() not in (2, 3):
         raise ValueError("w must be [K, N] or [G, K, N]")
     if w.dtype not in _DT or scale_dtype not in _DT:
@@ -144,12 +151,6 @@ def _grouped(x, w, starts, relu, out_dtype, out, s):
                                              ldx, m, out.data_ptr(), _DT[out.dtype], ldo,
                                              1 if relu else 0, ws, n, s), "aem_grouped_q4gemm")
     return out
-
-
-def _no_gradient(what, x):
-    _no_tangent(what, x)
-    if x.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError(f"{what} has no gradient: detach x or call it under torch.no_grad()")
 
 
 def q4_matmul(x, w, group=0, out_dtype=None, out=None, stream=None):

@@ -224,3 +224,14 @@ def test_forward_mode_is_refused():
             D.dispatch(x, ids, 2)
     with pytest.raises(ValueError, match="CUDA"):
         D.dispatch(x, ids, 2)
+
+
+def test_quantisation_refuses_gradients():
+    from torch.autograd import forward_ad
+    w = torch.zeros(64, 32, requires_grad=True)
+    with pytest.raises(RuntimeError, match="quantize_q4 has no gradient: detach w"):
+        q4.quantize_q4(w, 32)
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):  # past that check
+        q4.quantize_q4(w, 32)
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        q4.quantize_q4(forward_ad.make_dual(w.detach(), torch.ones(64, 32)), 32)
