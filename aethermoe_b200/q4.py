@@ -74,6 +74,8 @@ class Q4Weight:
         want = tuple(q.shape[:-2]) + (-(-k // group_size), n)
         if tuple(scale.shape) != want:
             raise ValueError(f"scale must be {want}, got {tuple(scale.shape)}")
+        if q.device.type not in ("cpu", "cuda") or scale.device != q.device:
+            raise ValueError(f"q and scale must be on one CUDA device or the CPU, got {q.device} and {scale.device}")
         h = ctypes.c_void_p()
         if q.is_cuda:
             def pack(q, scale, s):

@@ -235,3 +235,11 @@ def test_quantisation_refuses_gradients():
         q4.quantize_q4(w, 32)
     with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
         q4.quantize_q4(forward_ad.make_dual(w.detach(), torch.ones(64, 32)), 32)
+
+
+def test_packing_refuses_tensors_of_two_devices():
+    """The host pack reads both through their addresses: neither may be a device's."""
+    q, s = torch.zeros(64, 32, dtype=torch.int8), torch.ones(2, 32)
+    for a, b in ((q, s.to("meta")), (q.to("meta"), s), (q.to("meta"), s.to("meta"))):
+        with pytest.raises(ValueError, match="one CUDA device or the CPU"):
+            q4.Q4Weight(a, b, 32)

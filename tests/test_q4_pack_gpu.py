@@ -88,3 +88,12 @@ def test_stream_ordered_pack_reports_in_the_shared_word(cuda):
     assert _lib.lib().aem_q4weight_pack_checked(q.data_ptr(), s.data_ptr(), _lib.F32, 1, 128, 64, 64, st,
                                                 ctypes.byref(h)) == _lib.AEM_EINVAL and not h.value
     assert _lib.lib().aem_device_status(st) == _lib.AEM_OK
+
+
+def test_packing_refuses_tensors_of_two_devices(cuda):
+    import torch
+    from aethermoe_b200 import q4
+    q, s = weights(cuda, 1, 64, 32, 32, torch.float32)
+    for a, b in ((q.cpu(), s), (q, s.cpu())):
+        with pytest.raises(ValueError, match="one CUDA device or the CPU"):
+            q4.Q4Weight(a, b, 32)
