@@ -1283,6 +1283,11 @@ aem_status aem_q4weight_pack(const int8_t* q, const void* scale, aem_dtype scale
         set_error("aem_q4weight_pack: device %d is not an sm_100 (B200) GPU", device);
         return AEM_EUNSUPPORTED;
     }
+    struct Device {  // the caller's device is current again at the end
+        int before = 0;
+        Device() { cudaGetDevice(&before); }
+        ~Device() { cudaSetDevice(before); }
+    } restore;
     AEM_TRY_CUDA(cudaSetDevice(device));
     const size_t sb = static_cast<size_t>(G * KB * N) * (scale_dtype == AEM_BF16 ? 2 : 4);
     int8_t* dq = nullptr;
@@ -1300,12 +1305,8 @@ aem_status aem_q4weight_pack(const int8_t* q, const void* scale, aem_dtype scale
         set_error("aem_q4weight_pack: copy failed");
         st = AEM_ECUDA;
     }
-    if (st == AEM_OK)
-        st = aem_q4weight_pack_device(dq, ds, scale_dtype, G, K, N, group_size, nullptr, out);
-    if (st == AEM_OK && cudaDeviceSynchronize() != cudaSuccess) {
-        set_error("aem_q4weight_pack: %s", cudaGetErrorString(cudaGetLastError()));
-        st = AEM_ECUDA;
-    }
+    // waits, so the copies may go
+    if (st == AEM_OK) st = aem::pack_q4(dq, ds, scale_dtype, G, K, N, group_size, nullptr, true, out);
     cudaFree(dq);
     cudaFree(ds);
     return st;

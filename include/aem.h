@@ -356,7 +356,8 @@ typedef struct aem_q4weight_s* aem_q4weight_t;
  * given), into a device-resident copy laid out in blocks of 128 k x 128
  * channels with their scales: K*N/2 bytes per group and the scales, K and N
  * rounded up to 128.  Same from HOST memory (a value outside
- * [-7, 7] -> AEM_EINVAL) and from DEVICE memory: either stream-ordered (such a
+ * [-7, 7] -> AEM_EINVAL), onto `device`, which need not be the current one and
+ * does not become it, and from DEVICE memory: either stream-ordered (such a
  * value is clamped and reported by aem_device_status, which every caller of the
  * device shares) or checked, where the call waits for the stream and such a
  * value is AEM_EINVAL of this call alone. */

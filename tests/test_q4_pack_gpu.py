@@ -97,3 +97,16 @@ def test_packing_refuses_tensors_of_two_devices(cuda):
     for a, b in ((q.cpu(), s), (q, s.cpu())):
         with pytest.raises(ValueError, match="one CUDA device or the CPU"):
             q4.Q4Weight(a, b, 32)
+
+
+def test_host_pack_keeps_the_current_device(cuda):
+    import torch
+    from aethermoe_b200 import q4
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two devices")
+    q, s = weights(cuda, 1, 64, 32, 32, torch.float32)
+    w = q4.Q4Weight(q[0].cpu(), s[0].cpu(), 32, device=1)
+    assert torch.cuda.current_device() == 0 and w.device == 1
+    x = torch.randn(2, 64, device="cuda:1")
+    assert torch.equal(q4.q4_matmul(x, w).cpu(), q4.q4_matmul(x.to(cuda), q4.Q4Weight(q[0], s[0], 32)).cpu())
+    assert torch.cuda.current_device() == 0
