@@ -1056,6 +1056,10 @@ aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, const XT* x
     a.NP = static_cast<int>(w->NP);
     a.x = x;
     a.err = device_error_word(w->device);
+    if (!a.err) {
+        set_error("%s: no device error word", what);
+        return AEM_ENOMEM;
+    }
     a.vec = reinterpret_cast<uintptr_t>(x) % (4 * sizeof(XT)) == 0 && a.ldx % 4 == 0 && a.K % 4 == 0;
     a.ovec = reinterpret_cast<uintptr_t>(a.out) % (a.out_bf16 ? 8 : 16) == 0 && a.ldo % 4 == 0;
     AEM_REQUIRE(a.M * kTerms<XT> < (1ll << 31), "%s: M=%lld out of range", what, (long long)a.M);
