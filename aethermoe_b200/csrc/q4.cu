@@ -11,22 +11,23 @@
 // packed weights become two operand registers by one mask, one rotation and
 // another mask.  The activations take part as e5m2 terms: with rho = the
 // power of two that brings the row's largest finite magnitude into
-// [2^14, 2^15), x * rho = t_0 + t_1 + ... where t_j is what is left after
+// [2^15, 2^16), x * rho = t_0 + t_1 + ... where t_j is what is left after
 // t_0 .. t_{j-1}, truncated to e5m2's three significant bits (down to 2^-16).
-// Three terms hold a bf16 value and eight a float32 value exactly unless its
-// last bits lie below rho * |x| = 2^-16; what is cut off there is under 2^-30
-// of the row's largest magnitude, below the rounding of a float32 sum that
-// holds it.  A row's terms sit side by side in MMA columns whose sums are
-// added (few rows: a tile is 16 columns at least), or follow one another into
-// the same column.  Every product is exact, sums are float32 (tcgen05,
-// accumulators in TMEM), and the scales multiply them in float32: no rounded
-// weight ever exists.
+// Three terms hold a bf16 value unless its last bits lie below that.  A float32
+// value takes three such windows, each 2^9 larger than the one before, with sums
+// of their own.  Elements that are 2^24 (float32: 2^26, 2^23 in few rows) below
+// their row's largest may end below the last window: what is left of them is
+// multiplied in float32 and added at the end, so every bit of x takes part.  A
+// row's terms sit side by side in MMA columns whose sums are added (few rows: a
+// tile is 16 columns at least), or follow one another into the window's column.
+// Every product is exact, sums are float32 (tcgen05, accumulators in TMEM), and
+// the scales multiply them in float32: no rounded weight ever exists.
 //
 // What has to be moved is the weight stream, K*N/2 bytes plus the scales.
 // 4096 x 14336, groups of 128, one bf16 row: 10.9 us, 2.8 TB/s of that stream
 // (about 2 us to the first product, 4 of products at the memory's rate, 1.5 of
 // sums between CTAs, the rest the launch).  64 rows of 14336 x 4096, groups of
-// 64: 22.2 us (18.8 for 4096 x 14336, groups of 128), where unpacking, taking
+// 64: 21.8 us (18.1 for 4096 x 14336, groups of 128), where unpacking, taking
 // the sums back from tensor memory and the latency from one unit to the next
 // bound it.  Forms that could not keep up (4096 x
 // 14336, one row): warp MMAs (mma.sync m16n8k16 occupies its sub-core's tensor
@@ -249,7 +250,8 @@ using namespace aem::dev;
 struct Q4Args {
     const uint8_t* w;
     const void* x;              // the caller's rows (ldx elements apart), for kernels that make the terms
-    const float* unscale;       // [M]: 2^9 / rho of a row, from the terms kernel
+    const uint32_t* tops;       // [M], from the terms kernel
+    const uint8_t* cuts;        // [M][NP], from the terms kernel, for rows with bit 31 of tops
     void* out;
     const int32_t* group_rows;  // nullptr: one group of M rows, weight group `group`
     int64_t ldx, ldo, M, N, K;
@@ -259,13 +261,31 @@ struct Q4Args {
     bool scale_bf16, out_bf16, relu, vec, ovec;  // vec, ovec: x, out can be moved in vectors of 4
 };
 
+// A row's activations as e5m2 terms, three to a window.  Window w holds
+// x * rho * 2^(9 w) from 2^16 down to 2^-16, so a float32 row's three reach
+// 2^-49 of its largest magnitude.
 template <typename XT>
-constexpr int kTerms = sizeof(XT) == 4 ? 8 : 3;
+constexpr int kWin = sizeof(XT) == 4 ? 3 : 1;
+template <typename XT>
+constexpr int kTerms = 3 * kWin<XT>;
+// Side by side a float32 row has eight, two in the last window: 16 columns hold
+// two rows, and blocks of one row stay 1 KB apart.
+template <typename XT>
+constexpr int kSide = sizeof(XT) == 4 ? 8 : 3;
+// An element whose exponent is further below the largest's may have bits that no
+// term holds; they are added apart (cut_sum).
+constexpr uint32_t span_of(int terms) { return terms == 9 ? 26 : terms == 8 ? 23 : 24; }
 
 // Four elements of a row from k on, zero past K, as they lie in memory.
 template <typename XT>
 struct Four {
     uint32_t w[sizeof(XT)];
+    // Running minimum of the magnitudes, zeros last, in the form that
+    // may_be_cut() reads.
+    __device__ __forceinline__ void any_low(uint32_t& m) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = min(m, 2 * __float_as_uint(get(i)) - 1);
+    }
     // VEC: rows of 4-element vectors, K a multiple of 4
     template <bool VEC>
     __device__ __forceinline__ void load(const XT* row, int64_t k, int64_t K) {
@@ -319,24 +339,30 @@ struct Four {
     }
 };
 // rho = 2^up for a row whose top magnitude has these bits; 2^9 / rho.
-__device__ __forceinline__ int rho_exponent(uint32_t top) { return 141 - static_cast<int>(top >> 23); }
+__device__ __forceinline__ int rho_exponent(uint32_t top) { return 142 - static_cast<int>(top >> 23); }
+// Whether the exponent of the smallest magnitude `low` is more than `span` below
+// the largest's.
+__device__ __forceinline__ bool may_be_cut(uint32_t low, uint32_t top, uint32_t span) {
+    return low < (top >> 23 > span ? ((top >> 23) - span << 24) - 1 : 0);
+}
 __device__ __forceinline__ float unscale_of(uint32_t top) {
-    const int e = 9 - rho_exponent(top);  // -132 .. 122
+    const int e = 9 - rho_exponent(top);  // -133 .. 121
     return __uint_as_float(e >= -126 ? static_cast<uint32_t>(127 + e) << 23 : 1u << (149 + e));
 }
 
-// The terms of four elements, one byte each.  e5m2 is the upper byte of an
-// fp16, so truncating an fp16 by a mask truncates the term; a scaled bf16 is
-// an fp16 (down to 2^-24, where the terms end at 2^-16), and a scaled float32
-// is taken apart nine bits, three terms, at a time.  An infinity or NaN is
-// all in the first term.
-template <typename XT>
-__device__ __forceinline__ void terms4(const Four<XT>& x, int up, uint32_t (&t)[kTerms<XT>]) {
-    constexpr int TERMS = kTerms<XT>, STEPS = (TERMS + 2) / 3;
+// The terms of four elements, one byte each; t[3 w + j] is term j of window w.
+// e5m2 is the upper byte of an fp16, so truncating an fp16 by a mask truncates
+// the term.  What a window's terms leave of a value goes to the next, 2^9
+// larger: three terms take nine significant bits of it or all down to 2^-16, so
+// less than 2^7 is left, and all 24 bits are taken unless they end below the
+// last window.  Every difference is exact.  An infinity or NaN is all in the
+// first term.  REST: also what all terms leave of x * rho * 2^(9 (kWin - 1)).
+template <bool REST, typename XT, int TERMS>
+__device__ __forceinline__ void terms4(const Four<XT>& x, int up, uint32_t (&t)[TERMS], float (&r)[4]) {
+    constexpr int WIN = kWin<XT>;
     // two factors: rho itself may be beyond float32
     const float f1 = __uint_as_float(static_cast<uint32_t>(127 + up / 2) << 23);
     const float f2 = __uint_as_float(static_cast<uint32_t>(127 + up - up / 2) << 23);
-    float r[4];
     uint32_t special = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -348,13 +374,13 @@ __device__ __forceinline__ void terms4(const Four<XT>& x, int up, uint32_t (&t)[
         }
     }
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
+    for (int s = 0; s < WIN; ++s) {
+        const bool on = REST || s + 1 < WIN;
         uint32_t h[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(h[i]) : "f"(r[2 * i + 1]), "f"(r[2 * i]));
-            if (STEPS > 1) {
-                h[i] &= 0xfffcfffcu;
+            if (on) {
                 const __half2 hh = *reinterpret_cast<const __half2*>(&h[i]);
                 r[2 * i] -= __low2float(hh);
                 r[2 * i + 1] -= __high2float(hh);
@@ -371,31 +397,61 @@ __device__ __forceinline__ void terms4(const Four<XT>& x, int up, uint32_t (&t)[
                 h[i] = *reinterpret_cast<const uint32_t*>(&left);
             }
         }
+        if (on)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const __half2 left = *reinterpret_cast<const __half2*>(&h[i]);
+                r[2 * i] = (r[2 * i] + __low2float(left)) * (s + 1 < WIN ? 512.0f : 1.0f);
+                r[2 * i + 1] = (r[2 * i + 1] + __high2float(left)) * (s + 1 < WIN ? 512.0f : 1.0f);
+            }
     }
     t[0] |= special;
 }
 
-// Activations as the products read them: bytes [terms / tn][M][tn][KP] (KP = K
-// rounded up to 128, zero padded), unscale [M].  gridDim.y blocks share a row:
+// What TERMS terms leave of four elements of a row whose largest magnitude has
+// the bits `top`.
+template <int TERMS, typename XT>
+__device__ __forceinline__ void cut4(const Four<XT>& x, uint32_t top, float (&r)[4]) {
+    const int up = rho_exponent(top);
+    uint32_t t[TERMS];
+    terms4<true>(x, up, t, r);
+    // (what is left has bits of x, and the first product fewer places: exact)
+    const float f1 = __uint_as_float(static_cast<uint32_t>(127 - up / 2) << 23);
+    const float f2 = __uint_as_float(static_cast<uint32_t>(127 - up + up / 2) << 23);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t u = __float_as_uint(x.get(i)) & 0x7fffffffu;
+        // far below the last window, where x * rho may not be a float32 any more
+        const bool all = (u >> 23) + 60 < top >> 23;
+        r[i] = all ? x.get(i) : r[i] * (kWin<XT> == 3 ? 0x1p-18f : 1.0f) * f1 * f2;
+    }
+}
+
+// Activations as the products read them: bytes [3][M][kWin][KP] (KP = K rounded
+// up to 128, zero padded), tops [M], the bits of a row's largest finite magnitude,
+// bit 31 where elements of the row may be cut, and cuts [M][KP / 128] for such a
+// row: not zero where those of a block may be.  gridDim.y blocks share a row:
 // each reads all of it for the largest magnitude and turns its slots (4 k a
 // thread) into terms.  32 rows of 14336: done 2.4 us after the first block's
 // start; one block of 1024 threads a row took 4.3 and kept whole SMs from the
 // product's CTAs.
 template <typename XT, bool VEC>
 __global__ void __launch_bounds__(512)
-    q4_terms_kernel(const XT* __restrict__ x, int64_t ldx, int64_t K, int64_t KP, int tn,
-                    uint8_t* __restrict__ out, float* __restrict__ unscale) {
-    constexpr int TERMS = kTerms<XT>, HELD = 8;  // slots that stay in registers
+    q4_terms_kernel(const XT* __restrict__ x, int64_t ldx, int64_t K, int64_t KP,
+                    uint8_t* __restrict__ out, uint32_t* __restrict__ row_tops, uint8_t* __restrict__ cuts) {
+    constexpr int TERMS = kTerms<XT>, WIN = kWin<XT>, HELD = 8;  // slots that stay in registers
     const int nt = blockDim.x, P = gridDim.y, y = blockIdx.y;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    __shared__ uint32_t tops[16];
+    __shared__ uint32_t tops[16], lows[16];
     const XT* row = x + blockIdx.x * ldx;
     Four<XT> v[HELD];
 #pragma unroll
     for (int i = 0; i < HELD; ++i) v[i].template load<VEC>(row, (i * nt + threadIdx.x) * 4ll, K);
-    uint32_t top = 0;
+    uint32_t top = 0, low = ~0u;
 #pragma unroll
     for (int i = 0; i < HELD; ++i) v[i].any_top(top);
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) v[i].any_low(low);
     if (Four<XT>::special(top)) {
         top = 0;
 #pragma unroll
@@ -407,20 +463,30 @@ __global__ void __launch_bounds__(512)
         Four<XT> u;
         u.template load<VEC>(row, k, K);
         top = max(top, u.top());
+        u.any_low(low);
     }
+    low = __reduce_min_sync(~0u, low);
     top = __reduce_max_sync(~0u, top);
-    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top, lows[threadIdx.x >> 5] = low;
     __syncthreads();
     top = __reduce_max_sync(~0u, tops[threadIdx.x & (nt / 32 - 1)]);
     const int up = rho_exponent(top);
-    if (threadIdx.x == 0 && y == 0) unscale[blockIdx.x] = unscale_of(top);
+    const bool cut = may_be_cut(__reduce_min_sync(~0u, lows[threadIdx.x & (nt / 32 - 1)]), top, span_of(TERMS));
+    if (threadIdx.x == 0 && y == 0) row_tops[blockIdx.x] = top | (cut ? 1u << 31 : 0u);
     auto put = [&](int64_t k, const Four<XT>& u) {
         uint32_t t[TERMS];
-        terms4(u, up, t);
+        float rest[4];
+        terms4<false>(u, up, t, rest);
+        if (cut) {  // a warp has a block
+            uint32_t m = ~0u;
+            u.any_low(m);
+            const bool any = __any_sync(~0u, may_be_cut(m, top, span_of(TERMS)));
+            if ((threadIdx.x & 31) == 0) cuts[blockIdx.x * (KP >> 7) + (k >> 7)] = any;
+        }
 #pragma unroll
         for (int j = 0; j < TERMS; ++j)
             *reinterpret_cast<uint32_t*>(
-                out + ((j / tn * static_cast<int64_t>(gridDim.x) + blockIdx.x) * tn + j % tn) * KP + k) = t[j];
+                out + ((j % 3 * static_cast<int64_t>(gridDim.x) + blockIdx.x) * WIN + j / 3) * KP + k) = t[j];
     };
     int next = y;  // this block's next slot
 #pragma unroll
@@ -524,8 +590,143 @@ __device__ __forceinline__ void fma2(float& a0, float& a1, float s, uint32_t v0,
         : "f"(s), "r"(v0), "r"(v1));
 }
 
+// What TERMS terms leave of a row, times the weights: the sums of four channels a
+// lane over blocks p, p + step, ... of the CTA's np (at w; x their elements, k of
+// them at most), in float32.  cuts, if given, says which blocks may have anything.
+template <int TERMS, typename XT>
+__device__ __forceinline__ float4 cut_sum(const XT* x, int64_t k, const uint8_t* cuts, const uint8_t* w, int p, int step,
+                                          int np, int block, bool scale_bf16, uint32_t top) {
+    const int lane = threadIdx.x & 31, gs = 128 * 128 * (scale_bf16 ? 2 : 4) / (block - 8192);
+    float sum[4] = {};
+    for (; p < np; p += 32 * step) {
+        unsigned on = 0;  // bit i: block p + i * step may have something
+        if (cuts) {
+            on = __ballot_sync(~0u, p + lane * step < np && cuts[p + lane * step]);
+        } else {
+#pragma unroll 4
+            for (int i = 0; i < 32 && p + i * step < np; ++i) {
+                Four<XT> v;
+                uint32_t low = ~0u;
+                v.template load<false>(x, (p + i * step) * 128 + lane * 4, k);
+                v.any_low(low);
+                on |= __any_sync(~0u, may_be_cut(low, top, span_of(TERMS))) ? 1u << i : 0u;
+            }
+        }
+        for (; on; on &= on - 1) {
+            const int at = p + (__ffs(on) - 1) * step;
+            const uint8_t* blk = w + static_cast<int64_t>(at) * block;
+            Four<XT> v;
+            float r[4];
+            v.template load<false>(x, at * 128 + lane * 4, k);
+            cut4<TERMS>(v, top, r);
+            const unsigned any = __ballot_sync(~0u, r[0] != 0.0f || r[1] != 0.0f || r[2] != 0.0f || r[3] != 0.0f);
+            for (int i = 0; i < 4; ++i) {  // 32 k, eight lanes
+                if (!(any >> 8 * i & 0xff)) continue;
+                uint4 q[4];
+                float s[4], part[4] = {};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int ch = lane * 4 + j, sc = i * 32 / gs * 128 + ch;
+                    q[j] = *reinterpret_cast<const uint4*>(blk + i * 2048 + ch * 16);
+                    s[j] = scale_bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(blk + 8192)[sc])
+                                      : reinterpret_cast<const float*>(blk + 8192)[sc];
+                }
+                for (int b = 0; b < 32; b += 4) {
+                    if (!(any >> (8 * i + b / 4) & 1)) continue;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float re = __shfl_sync(~0u, r[e], i * 8 + b / 4);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t lo = b & 8 ? q[j].y : q[j].x, hi = b & 8 ? q[j].w : q[j].z;
+                            const uint32_t word = b & 16 ? hi : lo, mag = word >> (8 * e + (b & 4)) & 7;
+                            const uint32_t neg = word >> (8 * e + (b & 4 ? 11 : 7) & 31) & 1;
+                            part[j] = fmaf(s[j] * (neg ? -static_cast<float>(mag) : static_cast<float>(mag)), re, part[j]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[j] += part[j];
+            }
+        }
+    }
+    return make_float4(sum[0], sum[1], sum[2], sum[3]);
+}
+
+// The end of a CTA, once the warpgroups' sums `fin` [2][ROWS][128] are in shared
+// memory: rank ks sends its rows' sums to the ranks that write them, which add
+// them in rank order in `recv` [S][share].  CUT: `cut` [ways of a row][128] holds
+// what to add to a row, in `ways` parts.
+struct Q4Sums {
+    const float* fin;
+    float *recv, *cut;
+    const uint32_t* row_top;
+    const uint8_t *cuts, *src;
+    int64_t m0;
+    int stride, rows, tile, ks, p0, np;
+};
+constexpr int kQ4Warps = 12, kQ4Threads = 32 * kQ4Warps;
+template <int ROWS, bool CUT>
+__device__ __forceinline__ void send_sums(const Q4Args& a, const Q4Sums& z, int ways) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int share = (z.rows + a.S - 1) / a.S;  // rows that a rank writes
+    const int64_t n = z.tile * 128ll + lane * 4;  // a warp has a row, a lane four channels of it
+    const float4* fin4 = reinterpret_cast<const float4*>(z.fin) + lane;
+    float4* recv4 = reinterpret_cast<float4*>(z.recv) + lane;
+    for (int c = w, to = 0, r = c; c < z.rows; c += kQ4Warps, r += kQ4Warps) {
+        while (r >= share) r -= share, ++to;  // row c is row r of rank `to`
+        const float4 u = fin4[c * 32], v = fin4[(ROWS + c) * 32];
+        const float f = unscale_of(z.row_top[c] & 0x7fffffffu);
+        float4 o = make_float4((u.x + v.x) * f, (u.y + v.y) * f, (u.z + v.z) * f, (u.w + v.w) * f);
+        if constexpr (CUT)
+            for (int i = 0; i < ways; ++i) {
+                const float4 t = reinterpret_cast<const float4*>(z.cut)[(c * ways + i) * 32 + lane];
+                o.x += t.x, o.y += t.y, o.z += t.z, o.w += t.w;
+            }
+        float4* p = recv4 + (z.ks * share + r) * 32;
+        if (a.S > 1 && to != z.ks)
+            st_cluster(p, to, o);
+        else if (a.S > 1)
+            *p = o;
+        else
+            store_out(a, z.m0 + c, n, o);
+    }
+    if (a.S == 1) return;
+    cluster_sync();
+    for (int r = w; r < share && z.ks * share + r < z.rows; r += kQ4Warps) {
+        float4 v = recv4[r * 32];
+        for (int s = 1; s < a.S; ++s) {
+            const float4 u = recv4[(s * share + r) * 32];
+            v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+        }
+        store_out(a, z.m0 + z.ks * share + r, n, v);
+    }
+}
+// The same where the terms may not hold all of a row, first the sums of what they
+// leave: a warp has a row, or few rows' blocks go to several.  This is rare (8
+// rows or more of 4096 x 14336 with one such element: 3 us more; a whole row of
+// them, 50).  A call that nothing outlives leaves the kernel's registers alone:
+// as part of the loop above it cost every CTA 1 us.
+template <typename XT, int ROWS, int TERMS>
+__device__ __noinline__ void send_sums_and_cuts(const Q4Args& a, Q4Sums z) {
+    const int lane = threadIdx.x & 31, ways = z.rows < kQ4Warps ? kQ4Warps / z.rows : 1;
+    for (int i = threadIdx.x >> 5; i < z.rows * ways; i += kQ4Warps) {
+        const int c = i / ways;
+        const uint32_t top = z.row_top[c] & 0x7fffffffu;
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (!z.cuts || z.row_top[c] != top)
+            sum = cut_sum<TERMS>(static_cast<const XT*>(a.x) + (z.m0 + c) * a.ldx + z.p0 * 128ll, a.K - z.p0 * 128ll,
+                                 z.cuts ? z.cuts + c * static_cast<int64_t>(z.stride) : nullptr, z.src, i - c * ways,
+                                 ways, z.np, a.block, a.scale_bf16, top);
+        reinterpret_cast<float4*>(z.cut)[i * 32 + lane] = sum;
+    }
+    __syncthreads();
+    send_sums<ROWS, true>(a, z, ways);
+}
+
 // Shape of the product kernel: COLS MMA columns, scale groups of GS k, a row's
-// TN * TK terms in TN columns, TK after one another.  A block of the packed
+// TN * TK terms in TN columns, TK after one another (TK == 1: all side by side,
+// window after window; else a column a window).  A block of the packed
 // weight is 128 channels x 128 k; a unit is what a warpgroup hands to the
 // tensor core at once: a block, with one accumulator per scale group side by
 // side, or a half or quarter where a block's accumulators would not fit.  Two
@@ -563,7 +764,13 @@ struct Q4Cfg {
     static constexpr int XRES = XIN ? MAXP * XSTEP : 0;
     static constexpr int WB = 8192 + (FULL * 512 + 1023) / 1024 * 1024;  // a block of weights and scales
     // the cluster's sums: S shares of ceil(rows / S) rows, for any S up to 8
-    static constexpr int RECV = (ROWS < 8 ? 8 : ROWS < 16 ? 14 : ROWS < 32 ? 21 : ROWS < 64 ? 36 : 70) * 128 * 4;
+    static constexpr int shares() {
+        int most = 0;
+        for (int rows = 1; rows <= ROWS; ++rows)
+            for (int s = 1; s <= 8; ++s) most = s * ((rows + s - 1) / s) > most ? s * ((rows + s - 1) / s) : most;
+        return most;
+    }
+    static constexpr int RECV = shares() * 128 * 4;
     // Even rings: a stage always comes back to the warpgroup that saw its
     // previous phase, so no parity wait can mistake a phase for the one two
     // back.  Activations stay in theirs until the MMAs are done, weights only
@@ -572,15 +779,16 @@ struct Q4Cfg {
     static constexpr int MOST = CTAS == 2 ? 113 * 1024 : 226 * 1024;
     static constexpr int FIT = (MOST - 2048 - XRES - RECV - NX * XB) / WB / 2 * 2;
     static constexpr int NW = FIT > 8 ? 8 : FIT;
-    static constexpr int USED = 1024 + NW * WB + NX * XB + XRES + RECV + (2 * (NW + NX) + 9) * 8 + 16 + ROWS * 4;
+    static constexpr int USED = 1024 + NW * WB + NX * XB + XRES + RECV + (2 * (NW + NX) + 9) * 8 + 12 + ROWS * 4;
     // so many CTAs on an SM and no more: no CTA ever waits for tensor memory
     static constexpr int LEAST = CTAS == 2 ? 78 * 1024 : 116 * 1024;
     static constexpr int SMEM = USED > LEAST ? USED : LEAST;
     static_assert(NA * UA + ND * SUB * COLS <= TW && NW >= 4 && SMEM <= MOST, "budgets");
     static_assert(ROWS * TN <= COLS && SUB >= 1, "a scale group inside a unit");
     static_assert(NW * WB >= ROWS * 1024, "the warpgroups' sums fit the ring");
+    static_assert(XRES + NX * XB >= (ROWS < 12 ? 12 : ROWS) * 512, "what is added to them fits the activations'");
 };
-constexpr int kQ4Threads = 12 * 32, kSMs = 148;
+constexpr int kSMs = 148;
 
 // A CTA computes 128 channels of one row tile over its part of K:
 //   warps 0-7   two warpgroups, thread = channel = TMEM lane, that take the
@@ -605,7 +813,7 @@ constexpr int kQ4Threads = 12 * 32, kSMs = 148;
 // Every wait is bounded; a timeout sets the error word and ends all roles.
 template <typename XT, int COLS, int GS, int ROWS, int TN, int TK, bool ALONE>
 __global__ void __launch_bounds__(kQ4Threads, ALONE ? 1 : 2)
-    q4_kernel(const __grid_constant__ CUtensorMap xmap, const Q4Args a) {
+    q4_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ Q4Args a) {
     using C = Q4Cfg<COLS, GS, ROWS, TN, TK, ALONE>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* xres = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -622,7 +830,8 @@ __global__ void __launch_bounds__(kQ4Threads, ALONE ? 1 : 2)
     uint64_t* x_made = done + 4;          // XIN: the terms are in shared memory
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(x_made + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    uint32_t* row_top = tmem_slot + 2;    // [ROWS]: XIN, top magnitudes; else the rows' unscale
+    volatile int* any_cut = abort_flag + 1;  // the terms may not hold all of a row
+    uint32_t* row_top = tmem_slot + 3;    // [ROWS]: the rows' tops
 
     constexpr int NX = C::XIN ? 1 : C::NX;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -680,7 +889,7 @@ __global__ void __launch_bounds__(kQ4Threads, ALONE ? 1 : 2)
             mbar_init(&done[j], 1);
         }
         mbar_init(x_made, 8);
-        *abort_flag = 0;
+        *abort_flag = *any_cut = 0;
         fence_barrier_init();
         for (int p = 0; p < min(np, C::NW); ++p) copy_weights(p);
     } else if (w == 11) {
@@ -719,13 +928,19 @@ __global__ void __launch_bounds__(kQ4Threads, ALONE ? 1 : 2)
                 if (lane == 0) atomicMax(&row_top[r], top);
             }
             asm volatile("bar.sync 1, 256;" ::: "memory");
+            bool cut = false;
             r = 0, p = w;
 #pragma unroll
             for (int h = 0; h < HELD; ++h, p += 8) {
                 while (p >= np) p -= np, ++r;
                 if (r >= rows) break;
                 uint32_t t[TN];
-                terms4(xv[h], rho_exponent(row_top[r]), t);
+                const uint32_t top = row_top[r];
+                uint32_t low = ~0u;
+                xv[h].any_low(low);
+                cut |= may_be_cut(low, top, span_of(TN));
+                float rest[4];
+                terms4<false>(xv[h], rho_exponent(top), t, rest);
 #pragma unroll
                 for (int j = 0; j < TN; ++j) {
                     const int col = r * TN + j;  // a 128-byte row of the swizzled tile
@@ -734,33 +949,47 @@ __global__ void __launch_bounds__(kQ4Threads, ALONE ? 1 : 2)
                 }
             }
             fence_proxy_async_smem();
+            if (cut) *any_cut = 1;
             __syncwarp();
             if (lane == 0) mbar_arrive(x_made);
         }
         const uint32_t quarter = static_cast<uint32_t>(32 * (w & 3)) << 16;
-        // columns taken back at once
-        constexpr int TC = C::SUB * COLS, CH = TC == 16 ? 16 : 32;
+        // columns taken back at once, PER of an accumulator
+        constexpr int TC = C::SUB * COLS, CH = COLS % 48 == 0 ? 48 : TC == 16 ? 16 : 32, PER = COLS < CH ? COLS : CH;
+        constexpr int WIN = kWin<XT>, SIDE = C::XIN ? 3 : 1;  // terms of a window side by side
         auto take = [&](int u, const float (&s)[C::SUB]) {  // unit u's sums, scaled
 #pragma unroll
             for (int c0 = 0; c0 < TC; c0 += CH) {
                 uint32_t r[CH];
                 const uint32_t at = td + quarter + u % C::ND * TC + c0;
-                if constexpr (CH == 16)
+                if constexpr (CH == 16) {
                     tc_ld_32x32b_x16(at, r);
-                else
+                } else if constexpr (CH == 32 && PER == 32 && ROWS * TN <= 24) {
+                    tc_ld_32x32b_x16(at, *reinterpret_cast<uint32_t(*)[16]>(r));
+                    tc_ld_32x32b_x8(at + 16, *reinterpret_cast<uint32_t(*)[8]>(r + 16));
+                } else if constexpr (CH == 32) {
                     tc_ld_32x32b_x32(at, r);
+                } else {
+                    tc_ld_32x32b_x32(at, *reinterpret_cast<uint32_t(*)[32]>(r));
+                    tc_ld_32x32b_x16(at + 32, *reinterpret_cast<uint32_t(*)[16]>(r + 32));
+                }
                 tc_wait_ld();
 #pragma unroll
-                for (int i = 0; i < CH / 16 * (16 / TN); ++i) {  // 16 columns hold 16 / TN whole rows
-                    const int c = i / (16 / TN) * 16 + i % (16 / TN) * TN, row = (c0 + c) % COLS / TN;
+                for (int i = 0; i < CH / PER * (PER / TN); ++i) {  // PER columns hold PER / TN whole rows
+                    const int c = i / (PER / TN) * PER + i % (PER / TN) * TN, row = (c0 + c) % COLS / TN;
                     if (row >= ROWS) continue;
                     if constexpr (TN == 1) {  // two rows an instruction
                         if (i % 2 == 0) fma2(acc[row], acc[row + 1], s[(c0 + c) / COLS], r[c], r[c + 1]);
                         continue;
                     }
-                    float v = __uint_as_float(r[c]);
+                    float v = 0.0f;
 #pragma unroll
-                    for (int t = 1; t < TN; ++t) v += __uint_as_float(r[c + t]);
+                    for (int win = WIN - 1; win >= 0; --win) {
+                        float a = __uint_as_float(r[c + win * SIDE]);
+#pragma unroll
+                        for (int t = 1; t < SIDE && win * SIDE + t < TN; ++t) a += __uint_as_float(r[c + win * SIDE + t]);
+                        v = win == WIN - 1 ? a : fmaf(v, 0x1p-9f, a);
+                    }
                     acc[row] = fmaf(s[(c0 + c) / COLS], v, acc[row]);
                 }
             }
@@ -866,9 +1095,12 @@ __global__ void __launch_bounds__(kQ4Threads, ALONE ? 1 : 2)
         }
     } else if (w == 10 || !C::XIN) {
         const bool weights = w == 10;
-        if (!weights) {  // x and its unscale are the terms kernel's
+        if (!weights) {  // the terms and the tops are the terms kernel's
             asm volatile("griddepcontrol.wait;" ::: "memory");
-            for (int r = lane; r < rows; r += 32) row_top[r] = __float_as_uint(a.unscale[m0 + r]);
+            for (int r = lane; r < rows; r += 32) {
+                row_top[r] = a.tops[m0 + r];
+                if (row_top[r] >> 31) *any_cut = 1;
+            }
         }
         const int ns = weights ? C::NW : C::NX;
         uint64_t *full = weights ? w_full : x_full, *empty = weights ? w_empty : x_empty;
@@ -903,33 +1135,12 @@ __global__ void __launch_bounds__(kQ4Threads, ALONE ? 1 : 2)
         for (int c = 0; c < ROWS; ++c) fin[(wg * ROWS + c) * 128 + ch] = acc[c];
     __syncthreads();
     if (a.S > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-    const int share = (rows + a.S - 1) / a.S;  // rows that a rank writes
-    const int64_t n = tile * 128ll + lane * 4;  // a warp has a row, a lane four channels of it
-    const float4* fin4 = reinterpret_cast<const float4*>(fin) + lane;
-    float4* recv4 = reinterpret_cast<float4*>(recv) + lane;
-    for (int c = w, to = 0, r = c; c < rows; c += kQ4Threads / 32, r += kQ4Threads / 32) {
-        while (r >= share) r -= share, ++to;  // row c is row r of rank `to`
-        const float4 u = fin4[c * 32], v = fin4[(ROWS + c) * 32];
-        const float f = C::XIN ? unscale_of(row_top[c]) : __uint_as_float(row_top[c]);
-        const float4 o = make_float4((u.x + v.x) * f, (u.y + v.y) * f, (u.z + v.z) * f, (u.w + v.w) * f);
-        float4* p = recv4 + (ks * share + r) * 32;
-        if (a.S > 1 && to != ks)
-            st_cluster(p, to, o);
-        else if (a.S > 1)
-            *p = o;
-        else
-            store_out(a, m0 + c, n, o);
-    }
-    if (a.S == 1) return;
-    cluster_sync();
-    for (int r = w; r < share && ks * share + r < rows; r += kQ4Threads / 32) {
-        float4 v = recv4[r * 32];
-        for (int s = 1; s < a.S; ++s) {
-            const float4 u = recv4[(s * share + r) * 32];
-            v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
-        }
-        store_out(a, m0 + ks * share + r, n, v);
-    }
+    const Q4Sums z{fin, recv, reinterpret_cast<float*>(xres), row_top, C::XIN ? nullptr : a.cuts + m0 * a.NP + p0, src, m0, a.NP,
+                   rows, tile, ks, p0, np};
+    if (*any_cut)
+        send_sums_and_cuts<XT, ROWS, TN * TK>(a, z);
+    else
+        send_sums<ROWS, false>(a, z, 0);
 }
 
 template <typename XT, int COLS, int GS, int ROWS, int TN, int TK, bool ALONE>
@@ -1005,9 +1216,7 @@ aem_status launch_tile(const uint8_t* terms, Q4Args a, int gs, int64_t slots, cu
     const dim3 grid(static_cast<unsigned>(a.NC * a.S), static_cast<unsigned>(slots));
     if (gs == 128) return launch_q4<XT, COLS, 128, ROWS, TN, TK, ALONE>(xmap, a, grid, s);
     if (gs == 64) return launch_q4<XT, COLS, 64, ROWS, TN, TK, ALONE>(xmap, a, grid, s);
-    if constexpr (ALONE || TK < 8) return launch_q4<XT, COLS, 32, ROWS, TN, TK, ALONE>(xmap, a, grid, s);
-    set_error("q4 product: no such row tile");  // eight terms and 32-k scales do not fit a ring of four
-    return AEM_EINVAL;
+    return launch_q4<XT, COLS, 32, ROWS, TN, TK, ALONE>(xmap, a, grid, s);
 }
 
 // Rows of a tile: as many as the call (grouped: an average group) has; few
@@ -1018,7 +1227,12 @@ aem_status launch_tile(const uint8_t* terms, Q4Args a, int gs, int64_t slots, cu
 // 8.2 (9.2), five 10.1 (9.5).  A tile of 32 rows where 16 would do: 17.9 us
 // instead of 15.0 (6 rows).  One of 64 takes 18.8 us where two of 32 take 25
 // (4096 x 14336), but 9.7 where those take 8.5 with K split three ways or more
-// inside one wave (2048 x 1408).
+// inside one wave (2048 x 1408).  A float32 row has three columns: 5 rows fill 16,
+// 10 fill 32, 16 fill 48 and 32 fill 96.  Eight in a tile of eight, of which
+// three quarters are read back: 16.7 us, in one of ten 17.3 (groups of 32), but
+// groups of 6 rows on average have 9 or 10 often enough: 43.7 and 41.0 (64 of 2048
+// x 1408).  Groups of 32 take three windows' sums back four times a block: 32
+// float32 rows 29.6 us, of 128 19.1.
 struct Q4Plan {
     bool few;
     int rows;
@@ -1030,14 +1244,15 @@ Q4Plan q4_plan(const Q4Weight* w, bool f32, int64_t M, bool grouped) {
     Q4Plan p;
     p.few = want <= (f32 ? 2 : 4) && w->NP <= 8 * 24;
     if (f32)
-        p.rows = p.few ? (want <= 1 ? 1 : 2) : want <= 4 ? 4 : want <= 8 ? 8 : want <= 16 && w->gs > 32 ? 16 : 32;
+        p.rows = p.few ? (want <= 1 ? 1 : 2)
+                 : want <= 5 ? 5 : want <= 8 && !grouped ? 8 : want <= 10 ? 10 : want <= 16 ? 16 : 32;
     else
         p.rows = p.few ? (want <= 2 ? 2 : 4) : want <= 16 ? 16 : want <= 32 || small ? 32 : 64;
     return p;
 }
 size_t q4_workspace(const Q4Weight* w, bool f32, int64_t M, bool grouped) {
     if (q4_plan(w, f32, M, grouped).few) return 0;
-    return static_cast<size_t>(M) * ((f32 ? kTerms<float> : kTerms<__nv_bfloat16>) * w->NP * 128 + 4);
+    return static_cast<size_t>(M) * ((f32 ? kTerms<float> : kTerms<__nv_bfloat16>) * w->NP * 128 + sizeof(uint32_t) + w->NP);
 }
 
 // x: the caller's rows.
@@ -1073,24 +1288,25 @@ aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, const XT* x
     const int64_t slots = a.group_rows ? n + (a.M - n) / a.rows : (a.M + a.rows - 1) / a.rows;
     AEM_REQUIRE(slots <= 65535, "%s: M=%lld rows are too many for one call", what, (long long)a.M);
     if (plan.few)
-        return a.rows == (F32 ? 1 : 2) ? launch_tile<XT, 16, F32 ? 1 : 2, F32 ? 8 : 3, 1>(nullptr, a, w->gs, slots, s)
-                                       : launch_tile<XT, 16, F32 ? 2 : 4, F32 ? 8 : 3, 1>(nullptr, a, w->gs, slots, s);
+        return a.rows == (F32 ? 1 : 2) ? launch_tile<XT, 16, F32 ? 1 : 2, kSide<XT>, 1>(nullptr, a, w->gs, slots, s)
+                                       : launch_tile<XT, 16, F32 ? 2 : 4, kSide<XT>, 1>(nullptr, a, w->gs, slots, s);
     void* own = nullptr;
     if (!workspace) {
         AEM_TRY_CUDA(cudaMallocAsync(&own, need, s));
         workspace = own;
     }
     auto* terms = static_cast<uint8_t*>(workspace);
-    auto* unscale = reinterpret_cast<float*>(terms + static_cast<size_t>(a.M) * kTerms<XT> * w->NP * 128);
-    a.unscale = unscale;
-    const int tn = F32 && a.rows < 16 ? 16 / a.rows : 1;
+    auto* tops = reinterpret_cast<uint32_t*>(terms + static_cast<size_t>(a.M) * kTerms<XT> * w->NP * 128);
+    auto* cuts = reinterpret_cast<uint8_t*>(tops + a.M);
+    a.tops = tops;
+    a.cuts = cuts;
     // at most 8 slots in registers up to K = 16384, and about two blocks an SM
     const int threads = w->K <= 4096 ? 128 : w->K <= 8192 ? 256 : 512;
     const int64_t slots_x = (w->NP * 32 + threads - 1) / threads;
     const dim3 blocks(static_cast<unsigned>(a.M),
                       static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(slots_x, 296 / a.M))));
     auto make_terms = a.vec ? q4_terms_kernel<XT, true> : q4_terms_kernel<XT, false>;
-    make_terms<<<blocks, threads, 0, s>>>(x, a.ldx, w->K, w->NP * 128, tn, terms, unscale);
+    make_terms<<<blocks, threads, 0, s>>>(x, a.ldx, w->K, w->NP * 128, terms, tops, cuts);
     count_launches(1);
     const cudaError_t e = cudaGetLastError();
     aem_status st;
@@ -1098,10 +1314,11 @@ aem_status q4_product(const Q4Weight* w, const char* what, Q4Args a, const XT* x
         set_error("%s: launch failed: %s", what, cudaGetErrorString(e));
         st = AEM_ECUDA;
     } else if constexpr (F32) {
-        st = a.rows == 4    ? launch_tile<XT, 16, 4, 4, 2>(terms, a, w->gs, slots, s)
-             : a.rows == 8  ? launch_tile<XT, 16, 8, 2, 4>(terms, a, w->gs, slots, s)
-             : a.rows == 16 ? launch_tile<XT, 16, 16, 1, 8>(terms, a, w->gs, slots, s)
-                            : launch_tile<XT, 32, 32, 1, 8, true>(terms, a, w->gs, slots, s);
+        st = a.rows == 5    ? launch_tile<XT, 16, 5, 3, 3>(terms, a, w->gs, slots, s)
+             : a.rows == 8  ? launch_tile<XT, 32, 8, 3, 3>(terms, a, w->gs, slots, s)
+             : a.rows == 10 ? launch_tile<XT, 32, 10, 3, 3>(terms, a, w->gs, slots, s)
+             : a.rows == 16 ? launch_tile<XT, 48, 16, 3, 3, true>(terms, a, w->gs, slots, s)
+                            : launch_tile<XT, 96, 32, 3, 3, true>(terms, a, w->gs, slots, s);
     } else {
         // 16 rows: an SM for each CTA while there are SMs (8 rows, 14336 x 4096:
         // 14.5 us, sharing 16.7), but not for many groups' tiles (64 tokens, 64

@@ -377,10 +377,11 @@ aem_status aem_q4weight_shape(aem_q4weight_t w, int64_t* G, int64_t* K, int64_t*
  * decoding step: one pass over the weights for up to 64 bf16 or 32 float32
  * rows, one more for every further such tile.
  * The integers are exact in the MMAs' operands, each scale multiplies a
- * float32 sum, and x takes part in full: what is cut from an element is
- * under 2^-30 of its row's largest finite magnitude (nothing for bf16
- * elements down to 2^-23 of it), so nothing is rounded before out but the
- * float32 sums.  Infinities and NaN act as in x @ w.  Rows of x are ldx
+ * float32 sum, and every bit of every element of x takes part, whatever else its
+ * row holds, so nothing is rounded before out but the float32 sums.  (Elements
+ * more than 2^24, float32 2^23, below their row's largest magnitude are added
+ * apart: a few cost 3 to 5 us, rows of them 40 us each.)  Infinities and NaN act as in
+ * x @ w, so an infinity times a weight of zero is NaN.  Rows of x are ldx
  * elements apart, rows of out ldo; any alignment works.  The workspace holds
  * x in the products' form: device scratch of aem_q4gemm_workspace(w,
  * x_dtype, M, 0) bytes (0 for the fewest rows), 16-byte aligned, or NULL to
