@@ -320,7 +320,7 @@ aem_status aem_dispatch_backward(const void* grad_rows, aem_dtype rows_dtype, in
                                  aem_dtype x_dtype, int64_t ldx, void* stream);
 /* out[t] = sum_j weights[t*ldw + j] * rows[row_of[t*k + j]]; weights NULL
  * means 1.  A token without any expert gets zero.  The weight of a unit
- * without an expert is not read. */
+ * without an expert has no effect, whatever it is. */
 aem_status aem_combine(const void* rows, aem_dtype rows_dtype, int64_t ldr, const float* weights,
                        int64_t ldw, const int32_t* row_of, int64_t T, int k, int64_t d, void* out,
                        aem_dtype out_dtype, int64_t ldo, void* stream);

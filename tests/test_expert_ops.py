@@ -243,3 +243,12 @@ def test_packing_refuses_tensors_of_two_devices():
     for a, b in ((q, s.to("meta")), (q.to("meta"), s), (q.to("meta"), s.to("meta"))):
         with pytest.raises(ValueError, match="one CUDA device or the CPU"):
             q4.Q4Weight(a, b, 32)
+
+
+def test_dispatch_backward_refusals():
+    def call(g=P, rd=_lib.F32, ldr=8, row_of=P, T=4, k=2, d=8, out=P, xd=_lib.BF16, ldx=8):
+        return L().aem_dispatch_backward(g, rd, ldr, row_of, T, k, d, out, xd, ldx, None)
+    for bad in (dict(g=None), dict(row_of=None), dict(out=None), dict(T=-1), dict(T=1 << 30), dict(k=0), dict(k=65),
+                dict(rd=3), dict(xd=3), dict(d=0), dict(ldx=7), dict(ldr=-1)):
+        assert call(**bad) == EINVAL, bad
+    assert call(T=0) == _lib.AEM_OK
