@@ -280,11 +280,18 @@ constexpr uint32_t span_of(int terms) { return terms == 9 ? 26 : terms == 8 ? 23
 template <typename XT>
 struct Four {
     uint32_t w[sizeof(XT)];
-    // Running minimum of the magnitudes, zeros last, in the form that
-    // may_be_cut() reads.
+    // Running minimum of the magnitudes, zeros last; low_of() gives the form that
+    // may_be_cut() reads.  bf16 in pairs: a magnitude less one, its sign set, orders
+    // as a signed number, and zero becomes the largest.
+    static constexpr uint32_t kNoLow = sizeof(XT) == 4 ? ~0u : 0x7fff7fffu;
     __device__ __forceinline__ void any_low(uint32_t& m) const {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) m = min(m, 2 * __float_as_uint(get(i)) - 1);
+        for (int i = 0; i < static_cast<int>(sizeof(XT)); ++i)
+            m = sizeof(XT) == 4 ? min(m, 2 * w[i] - 1) : __vmins2(m, (w[i] | 0x80008000u) - 0x00010001u);
+    }
+    __device__ static __forceinline__ uint32_t low_of(uint32_t m) {
+        m ^= sizeof(XT) == 4 ? 0u : 0x80008000u;
+        return sizeof(XT) == 4 ? m : min(m << 16, m & 0xffff0000u) << 1 | 0x1ffffu;
     }
     // VEC: rows of 4-element vectors, K a multiple of 4
     template <bool VEC>
@@ -447,7 +454,7 @@ __global__ void __launch_bounds__(512)
     Four<XT> v[HELD];
 #pragma unroll
     for (int i = 0; i < HELD; ++i) v[i].template load<VEC>(row, (i * nt + threadIdx.x) * 4ll, K);
-    uint32_t top = 0, low = ~0u;
+    uint32_t top = 0, low = Four<XT>::kNoLow;
 #pragma unroll
     for (int i = 0; i < HELD; ++i) v[i].any_top(top);
 #pragma unroll
@@ -465,7 +472,7 @@ __global__ void __launch_bounds__(512)
         top = max(top, u.top());
         u.any_low(low);
     }
-    low = __reduce_min_sync(~0u, low);
+    low = __reduce_min_sync(~0u, Four<XT>::low_of(low));
     top = __reduce_max_sync(~0u, top);
     if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top, lows[threadIdx.x >> 5] = low;
     __syncthreads();
@@ -478,9 +485,9 @@ __global__ void __launch_bounds__(512)
         float rest[4];
         terms4<false>(u, up, t, rest);
         if (cut) {  // a warp has a block
-            uint32_t m = ~0u;
+            uint32_t m = Four<XT>::kNoLow;
             u.any_low(m);
-            const bool any = __any_sync(~0u, may_be_cut(m, top, span_of(TERMS)));
+            const bool any = __any_sync(~0u, may_be_cut(Four<XT>::low_of(m), top, span_of(TERMS)));
             if ((threadIdx.x & 31) == 0) cuts[blockIdx.x * (KP >> 7) + (k >> 7)] = any;
         }
 #pragma unroll
@@ -606,10 +613,10 @@ __device__ __forceinline__ float4 cut_sum(const XT* x, int64_t k, const uint8_t*
 #pragma unroll 4
             for (int i = 0; i < 32 && p + i * step < np; ++i) {
                 Four<XT> v;
-                uint32_t low = ~0u;
+                uint32_t low = Four<XT>::kNoLow;
                 v.template load<false>(x, (p + i * step) * 128 + lane * 4, k);
                 v.any_low(low);
-                on |= __any_sync(~0u, may_be_cut(low, top, span_of(TERMS))) ? 1u << i : 0u;
+                on |= __any_sync(~0u, may_be_cut(Four<XT>::low_of(low), top, span_of(TERMS))) ? 1u << i : 0u;
             }
         }
         for (; on; on &= on - 1) {
@@ -936,9 +943,9 @@ __global__ void __launch_bounds__(kQ4Threads, ALONE ? 1 : 2)
                 if (r >= rows) break;
                 uint32_t t[TN];
                 const uint32_t top = row_top[r];
-                uint32_t low = ~0u;
+                uint32_t low = Four<XT>::kNoLow;
                 xv[h].any_low(low);
-                cut |= may_be_cut(low, top, span_of(TN));
+                cut |= may_be_cut(Four<XT>::low_of(low), top, span_of(TN));
                 float rest[4];
                 terms4<false>(xv[h], rho_exponent(top), t, rest);
 #pragma unroll
