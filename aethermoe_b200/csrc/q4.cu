@@ -24,16 +24,15 @@
 // the scales multiply them in float32: no rounded weight ever exists.
 //
 // What has to be moved is the weight stream, K*N/2 bytes plus the scales.
-// 4096 x 14336, groups of 128, one bf16 row: 10.9 us, 2.8 TB/s of that stream
-// (about 2 us to the first product, 4 of products at the memory's rate, 1.5 of
-// sums between CTAs, the rest the launch).  64 rows of 14336 x 4096, groups of
-// 64: 21.8 us (18.1 for 4096 x 14336, groups of 128), where unpacking, taking
-// the sums back from tensor memory and the latency from one unit to the next
-// bound it.  Forms that could not keep up (4096 x
-// 14336, one row): warp MMAs (mma.sync m16n8k16 occupies its sub-core's tensor
-// pipe for 32 cycles: 16.6 us, 47.6 for 64 rows), and bf16 operands for tcgen05
-// (7 logic operations and 4 subtractions per 8 weights, the logic pipe the
-// bound: 17.3 us).
+// 4096 x 14336, groups of 128, one bf16 row: 10.9 us, 2.8 TB/s of that stream,
+// from a cold L2 as from a warm one (about 2 us to the first product, 4 of
+// products, 1.5 of sums between CTAs, the rest the launch).  64 rows of 14336 x
+// 4096, groups of 64: 22.5 us (18.1 for 4096 x 14336, groups of 128), where
+// unpacking, taking the sums back from tensor memory and the latency from one
+// unit to the next bound it.  Forms that could not keep up (4096 x 14336, one
+// row): warp MMAs (mma.sync m16n8k16 occupies its sub-core's tensor pipe for 32
+// cycles: 16.6 us, 47.6 for 64 rows), and bf16 operands for tcgen05 (7 logic
+// operations and 4 subtractions per 8 weights, the logic pipe the bound: 17.3 us).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -78,8 +77,8 @@ constexpr int kThreads = 256;  // pack
 // of it, so the division itself is only made where the product lies that near a
 // half.  Adding 1.5 * 2^23 rounds to a whole number, ties to even, and leaves it
 // in the low byte (the conversion instructions run at a quarter of the rate).
-// 14336 x 4096, groups of 128: float32 53.4 us = 5.5 TB/s, memory bound (with a
-// division per element 103); bf16 47.7, the wait for the maxima between loads
+// 14336 x 4096, groups of 128: float32 51.4 us = 5.7 TB/s, memory bound (with a
+// division per element 103); bf16 46.5, the wait for the maxima between loads
 // and stores the bound.
 constexpr float kRint = 12582912.0f;
 // Maximum that keeps a NaN: its group's scale has to be one.
@@ -711,8 +710,8 @@ __device__ __forceinline__ void send_sums(const Q4Args& a, const Q4Sums& z, int 
 }
 // The same where the terms may not hold all of a row, first the sums of what they
 // leave: a warp has a row, or few rows' blocks go to several.  This is rare (8
-// rows or more of 4096 x 14336 with one such element: 3 us more; a whole row of
-// them, 50).  A call that nothing outlives leaves the kernel's registers alone:
+// rows or more of 4096 x 14336 with one such element: 3 us more; rows of them, 40
+// each).  A call that nothing outlives leaves the kernel's registers alone:
 // as part of the loop above it cost every CTA 1 us.
 template <typename XT, int ROWS, int TERMS>
 __device__ __noinline__ void send_sums_and_cuts(const Q4Args& a, Q4Sums z) {
@@ -740,12 +739,11 @@ __device__ __noinline__ void send_sums_and_cuts(const Q4Args& a, Q4Sums z) {
 // CTAs share an SM, so that one's set-up and end lie under the other's products,
 // or a CTA has one to itself (ALONE) with room for two units in tensor memory
 // and twice the registers: 32 rows, 4096 x 14336: 17.6 us shared, 15.7 alone; 64
-// rows 25.0 as two shared tiles, 18.8 as one alone; few rows 11.0 shared, 11.5
-// alone (one row), where the stream is the bound and more CTAs ask for it.
-// With TK ==
-// 1 (few rows) the CTA makes the terms of its part of K itself and keeps them
-// in shared memory; otherwise a terms kernel has made them and they come in a
-// ring of their own.
+// rows 25.0 as two shared tiles, 18.1 as one alone.  Few rows share: alone, one
+// row takes 0.4 us more and four 5 more, where the stream is the bound and more
+// CTAs ask for it.  With TK == 1 (few rows) the CTA makes the terms of its part
+// of K itself and keeps them in shared memory; otherwise a terms kernel has made
+// them and they come in a ring of their own.
 template <int COLS, int GS, int ROWS, int TN, int TK, bool ALONE>
 struct Q4Cfg {
     static constexpr bool XIN = TK == 1;
@@ -1229,11 +1227,11 @@ aem_status launch_tile(const uint8_t* terms, Q4Args a, int gs, int64_t slots, cu
 // Rows of a tile: as many as the call (grouped: an average group) has; few
 // rows put their terms side by side in the 16 columns of the narrowest MMA.
 // A CTA that makes its own terms spares the terms kernel and its wait, but
-// every CTA of a row then does that work.  4096 x 14336, bf16: one row 11.2 us
-// (with the kernel 14.5), three 13.9 (14.8), five 16.7 (14.9); 4096 x 4096: one
-// 8.2 (9.2), five 10.1 (9.5).  A tile of 32 rows where 16 would do: 17.9 us
-// instead of 15.0 (6 rows).  One of 64 takes 18.8 us where two of 32 take 25
-// (4096 x 14336), but 9.7 where those take 8.5 with K split three ways or more
+// every CTA of a row then does that work.  With the kernel, bf16 rows of 4096 x
+// 14336 take 2.3 us more (one), the same (three) or 1.5 less (four), of 4096 x
+// 4096 1.8 more (one) or 1.0 more (four).  A tile of 32 rows where 16 would do:
+// 17.9 us instead of 15.0 (6 rows).  One of 64 takes 18.1 us where two of 32 take
+// 25 (4096 x 14336), but 9.7 where those take 8.5 with K split three ways or more
 // inside one wave (2048 x 1408).  A float32 row has three columns: 5 rows fill 16,
 // 10 fill 32, 16 fill 48 and 32 fill 96.  Eight in a tile of eight, of which
 // three quarters are read back: 16.7 us, in one of ten 17.3 (groups of 32), but
