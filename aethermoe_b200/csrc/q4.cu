@@ -710,7 +710,7 @@ __device__ __forceinline__ void send_sums(const Q4Args& a, const Q4Sums& z, int 
 }
 // The same where the terms may not hold all of a row, first the sums of what they
 // leave: a warp has a row, or few rows' blocks go to several.  This is rare (8
-// rows or more of 4096 x 14336 with one such element: 3 us more; rows of them, 40
+// rows or more of 4096 x 14336 with one such element: 3 us more; rows of them, 30
 // each).  A call that nothing outlives leaves the kernel's registers alone:
 // as part of the loop above it cost every CTA 1 us.
 template <typename XT, int ROWS, int TERMS>

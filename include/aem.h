@@ -380,7 +380,7 @@ aem_status aem_q4weight_shape(aem_q4weight_t w, int64_t* G, int64_t* K, int64_t*
  * float32 sum, and every bit of every element of x takes part, whatever else its
  * row holds, so nothing is rounded before out but the float32 sums.  (Elements
  * more than 2^24, float32 2^23, below their row's largest magnitude are added
- * apart: a few cost 3 to 5 us, rows of them 40 us each.)  Infinities and NaN act as in
+ * apart: a few cost 3 to 5 us, rows of them 30 us each.)  Infinities and NaN act as in
  * x @ w, so an infinity times a weight of zero is NaN.  Rows of x are ldx
  * elements apart, rows of out ldo; any alignment works.  The workspace holds
  * x in the products' form: device scratch of aem_q4gemm_workspace(w,
