@@ -15,7 +15,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libaethermoe.so")
 
 AEM_OK, AEM_EINVAL, AEM_ECUDA, AEM_ENCCL, AEM_ETIMEOUT, AEM_ENOMEM, AEM_EUNSUPPORTED, AEM_EDEVICE = range(8)
-F32, BF16 = 0, 1
+F32, BF16, E4M3 = 0, 1, 2
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 GATING_EXACT, GATING_FAST, GATING_CERTIFIED = 0, 1, 2
 CAPACITY_UNLIMITED = (1 << 64) - 1
 MAX_EXPERTS = 256
@@ -42,6 +43,12 @@ class AemTimeout(AemError):
 class MoeConfig(ctypes.Structure):
     _fields_ = [("d_model", _i64), ("d_ffn", _i64), ("num_experts", _int), ("top_k", _int),
                 ("capacity", _u64), ("gating_mode", _int)]
+
+
+class RouteConfig(ctypes.Structure):
+    """``aem_route_config``: scores, groups and weights of a routing from logits."""
+    _fields_ = [("score", ctypes.c_int), ("k", ctypes.c_int), ("groups", ctypes.c_int), ("top_groups", ctypes.c_int),
+                ("group_top", ctypes.c_int), ("renormalize", ctypes.c_int), ("scale", ctypes.c_float)]
 
 
 class SeqSlice(ctypes.Structure):
@@ -133,6 +140,20 @@ _SIGS = {
     "aem_q4gemm": (_int, [_vp, _i64, _vp, _int, _i64, _i64, _vp, _int, _i64, _vp, ctypes.c_size_t, _vp]),
     "aem_grouped_q4gemm": (_int, [_vp, _vp, _vp, _int, _i64, _i64, _vp, _int, _i64, _int, _vp,
                                   ctypes.c_size_t, _vp]),
+    "aem_route_tokens": (_int, [ctypes.POINTER(RouteConfig), _vp, _int, _i64, _i64, _int, _vp, _vp, _vp, _vp]),
+    "aem_route_tokens_backward": (_int, [ctypes.POINTER(RouteConfig), _vp, _i64, _vp, _int, _i64, _i64, _int, _vp,
+                                         _i64, _vp, _i64, _vp]),
+    "aem_quantize_fp8": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp]),
+    "aem_quantize_fp8_weight": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "aem_fp8weight_pack": (_int, [_vp, _vp, _i64, _i64, _i64, _int, ctypes.POINTER(_vp)]),
+    "aem_fp8weight_pack_device": (_int, [_vp, _vp, _i64, _i64, _i64, _vp, ctypes.POINTER(_vp)]),
+    "aem_fp8weight_free": (_int, [_vp]),
+    "aem_fp8weight_shape": (_int, [_vp, ctypes.POINTER(_i64), ctypes.POINTER(_i64), ctypes.POINTER(_i64)]),
+    "aem_fp8gemm_workspace": (ctypes.c_size_t, [_vp, _int, _i64, _int]),
+    "aem_fp8gemm": (_int, [_vp, _i64, _int, _vp, _int, _i64, _vp, _i64, _i64, _vp, _int, _i64, _vp, ctypes.c_size_t,
+                           _vp]),
+    "aem_grouped_fp8gemm": (_int, [_vp, _vp, _int, _vp, _int, _i64, _vp, _i64, _i64, _vp, _int, _i64, _int, _int, _vp,
+                                   ctypes.c_size_t, _vp]),
     "aem_moe_create": (_int, [ctypes.POINTER(MoeConfig), _vp, _vp, _vp, ctypes.POINTER(_vp)]),
     "aem_moe_free": (_int, [_vp]),
     "aem_moe_forward": (_int, [_vp, _vp, _int, _i64, _vp, _int, _vp]),

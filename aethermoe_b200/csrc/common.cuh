@@ -83,6 +83,11 @@ aem_status make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType 
 aem_status make_tmap_3d_u8(CUtensorMap* map, const void* base, uint64_t dim0, uint64_t dim1, uint64_t dim2,
                            uint64_t row_bytes, uint64_t plane_bytes, uint32_t box1, uint32_t box2);
 
+// 2-D byte map: cols bytes innermost, rows row_bytes (a multiple of 16) apart; boxes
+// of 128 bytes x box_rows.
+aem_status make_tmap_2d_u8(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t row_bytes,
+                           uint32_t box_rows, CUtensorMapSwizzle swizzle);
+
 }  // namespace aem
 
 // ================================================================ device side
@@ -472,6 +477,29 @@ __host__ __device__ constexpr uint32_t idesc_e4m3_e5m2_f32(uint32_t m, uint32_t 
            | (1u << 10)           // B format e5m2
            | ((n >> 3) << 17)     // N >> 3
            | ((m >> 4) << 24);    // M >> 4
+}
+
+// D[tmem] (+)= A[smem desc] * B[smem desc]^T in the 8-bit form, issued as above, on
+// one SM and on a pair.
+__device__ __forceinline__ void tc_mma_f8_elect(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                                uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Instruction descriptor of kind::f8f6f4: e4m3 A and B, f32 D.  An operand is
+// K-major, or MN-major where its transpose bit is set.
+__host__ __device__ constexpr uint32_t idesc_e4m3_f32(uint32_t m, uint32_t n, bool a_mn, bool b_mn) {
+    return (1u << 4)                    // D format f32
+           | ((a_mn ? 1u : 0u) << 15)   // A is MN-major
+           | ((b_mn ? 1u : 0u) << 16)   // B is MN-major
+           | ((n >> 3) << 17)           // N >> 3
+           | ((m >> 4) << 24);          // M >> 4
 }
 
 }  // namespace dev

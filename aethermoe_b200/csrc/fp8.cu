@@ -1,0 +1,583 @@
+// Products of rows with 8-bit floating point weights, scales per block of 128:
+//
+//   out[m, n] = sum_b xs[m, b] ws[b, n / 128] sum_{k in block b} xq[m, k] wq[k, n]
+//
+// dense and grouped by expert, and with the transposed weight (the gradient of the
+// rows: the sum runs over the channels).  A block's sum is four tcgen05 MMAs of
+// K = 32 on e4m3 operands with float32 accumulators in TMEM; the block's scales
+// differ from row to row, so its sum is taken back and added to float32 registers
+// as one multiply-add per element.
+//
+// fp8_few_kernel: weights are the MMA's 128 rows (the channels), tokens its
+// columns; the weight stream is what bounds few rows.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "common.cuh"
+#include "fp8.h"
+#include "runtime.h"
+
+namespace aem {
+namespace {
+
+using namespace aem::dev;
+
+struct Fp8Args {
+    const uint8_t* w;           // packed tiles
+    const float* ws;            // their scales
+    const float* xs;            // [M][lds]
+    void* out;
+    const int32_t* group_rows;  // nullptr: one group of M rows, weight group `group`
+    int64_t lds, ldo, M, N;     // N: columns of out
+    int64_t group, group_tiles; // tiles of a weight group
+    int64_t out_step, sum_step; // tiles from one 128 of out's columns (of the sum) to the next
+    int nb, kb, G, S, rows;     // 128-blocks of out's columns and of the sum; S: CTAs (one cluster) that split
+                                // the sum; rows: rows of a row tile
+    int out_bf16, relu, ovec;   // ovec: out can be stored in vectors of 4
+    int* err;
+};
+
+// Row tile `slot` of the groups' row tiles: its group, first row and rows.
+// Every warp searches alike.  Offsets are clamped to [0, M].
+__device__ __forceinline__ bool find_rows(const Fp8Args& a, int slot, int64_t* g, int64_t* m0, int* rows) {
+    if (!a.group_rows) {
+        *g = a.group;
+        *m0 = static_cast<int64_t>(slot) * a.rows;
+        *rows = static_cast<int>(min(static_cast<int64_t>(a.rows), a.M - *m0));
+        return *rows > 0;
+    }
+    const int lane = threadIdx.x & 31, M = static_cast<int>(a.M);
+    int lo[8], hi[8];  // all offsets on their way at once
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        lo[i] = hi[i] = 0;
+        if (i * 32 + lane < a.G) {
+            lo[i] = a.group_rows[i * 32 + lane];
+            hi[i] = a.group_rows[i * 32 + lane + 1];
+        }
+    }
+    int before = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (i * 32 >= a.G) break;
+        lo[i] = min(max(lo[i], 0), M);
+        hi[i] = min(max(hi[i], 0), M);
+        const int n = hi[i] > lo[i] ? (hi[i] - lo[i] + a.rows - 1) / a.rows : 0;
+        int s = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(~0u, s, o);
+            if (lane >= o) s += v;
+        }
+        const int first = before + s - n;
+        const unsigned hit = __ballot_sync(~0u, slot >= first && slot < first + n);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            const int m = lo[i] + (slot - first) * a.rows;
+            *g = i * 32 + l;
+            *m0 = __shfl_sync(~0u, m, l);
+            *rows = __shfl_sync(~0u, min(a.rows, hi[i] - m), l);
+            return true;
+        }
+        before += __shfl_sync(~0u, s, 31);
+    }
+    return false;
+}
+
+// a0 += s0 * v0, a1 += s1 * v1 with s = f * (c0, c1)
+__device__ __forceinline__ void fma2(float& a0, float& a1, float f, float c0, float c1, uint32_t v0, uint32_t v1) {
+    asm("{\n.reg .b64 a, f, s, v;\nmov.b64 a, {%0, %1};\nmov.b64 f, {%2, %2};\nmov.b64 s, {%3, %4};\n"
+        "mov.b64 v, {%5, %6};\nmul.rn.f32x2 s, s, f;\nfma.rn.f32x2 a, s, v, a;\nmov.b64 {%0, %1}, a;\n}"
+        : "+f"(a0), "+f"(a1)
+        : "f"(f), "f"(c0), "f"(c1), "r"(v0), "r"(v1));
+}
+
+__device__ __forceinline__ void st_cluster(const float4* p, uint32_t rank, float4 v) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(mapa_u32(p, rank)), "f"(v.x),
+                 "f"(v.y), "f"(v.z), "f"(v.w)
+                 : "memory");
+}
+
+__device__ __forceinline__ float relu_of(float v) { return v < 0.0f ? 0.0f : v; }  // keeps a NaN
+
+// Four columns of a row of out.
+__device__ __forceinline__ void store_out(const Fp8Args& a, int64_t m, int64_t n, float4 v) {
+    if (a.relu) v = make_float4(relu_of(v.x), relu_of(v.y), relu_of(v.z), relu_of(v.w));
+    const int64_t at = m * a.ldo + n;
+    if (a.ovec && n + 3 < a.N) {
+        if (a.out_bf16) {
+            __nv_bfloat162 h[2] = {__floats2bfloat162_rn(v.x, v.y), __floats2bfloat162_rn(v.z, v.w)};
+            *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + at) = *reinterpret_cast<uint2*>(h);
+        } else {
+            *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = v;
+        }
+        return;
+    }
+    const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (n + j >= a.N) return;
+        if (a.out_bf16)
+            static_cast<__nv_bfloat16*>(a.out)[at + j] = __float2bfloat16_rn(e[j]);
+        else
+            static_cast<float*>(a.out)[at + j] = e[j];
+    }
+}
+
+// Operand descriptor of a packed tile and its step along K for 32 more: K-major
+// rows (32 bytes further), or MN-major (32 rows of 128 bytes further; the tile's 128
+// elements of M or N are one atom wide, 8 rows of K follow 1024 bytes apart).
+// Both have the same fields.
+template <bool MN>
+constexpr uint32_t kStep32 = MN ? 32 * 128 / 16 : 32 / 16;
+
+// 4 bytes global -> shared without waiting; lands before the barrier's phase ends.
+__device__ __forceinline__ void copy4_async(void* dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void arrive_after_copies(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// Few rows: a CTA computes 128 columns of out for a tile of TN rows over its part
+// of the sum.
+//   warps 0-7   thread = column of out = TMEM lane; warps 0-3 have the first half
+//               of the rows, 4-7 the second.  Per block of 128: its accumulator
+//               comes back and scale * sum is added to the row's register.
+//   warp 8      issues the MMAs (M = 128, N = rows, K = 32), four per block
+//   warp 9      copies the weights, one bulk copy of a 16 KB tile per block
+//   warp 10     copies the rows, one TMA box per block, and their scales
+// The S CTAs of a cluster take parts of the sum: each sends its sums to the rank
+// that writes those rows, which adds them in rank order.
+// Every wait is bounded; a timeout sets the error word and ends all roles.
+constexpr int kFewThreads = 11 * 32;
+template <int TN, bool ALONE>
+struct FewCfg {
+    static constexpr int CTAS = ALONE ? 1 : 2;  // on an SM
+    static constexpr int ND = 4;                // accumulators in TMEM
+    static constexpr int XB = TN * 128;
+    static constexpr int STAGE = kFp8Tile + XB + TN * 4;
+    static constexpr int MOST = ALONE ? 226 * 1024 : 113 * 1024;
+    static constexpr int FIXED = 1024 + 512;  // alignment; barriers
+    static constexpr int FIT = (MOST - FIXED) / STAGE;
+    static constexpr int NS = FIT > 12 ? 12 : FIT;
+    static constexpr int USED = FIXED + NS * STAGE;
+    // so many CTAs on an SM and no more: no CTA ever waits for tensor memory
+    static constexpr int LEAST = ALONE ? 116 * 1024 : 78 * 1024;
+    static constexpr int SMEM = USED > LEAST ? USED : LEAST;
+    static constexpr int COLS = ND * TN < 32 ? 32 : ND * TN;
+    static_assert(COLS * CTAS <= 512 && NS >= 3, "budgets");
+    // the CTA's sums [TN][128] and the cluster's [S][ceil(TN / S)][128], in the ring
+    static_assert((TN + TN + 7) * 512 <= NS * (kFp8Tile + XB), "sums fit the ring");
+};
+
+template <int TN, bool ALONE, bool TRANS>
+__global__ void __launch_bounds__(kFewThreads, ALONE ? 1 : 2)
+    fp8_few_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ Fp8Args a) {
+    using C = FewCfg<TN, ALONE>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                               ~static_cast<uintptr_t>(1023));
+    uint8_t* xring = ring + C::NS * kFp8Tile;
+    float* sring = reinterpret_cast<float*>(xring + C::NS * C::XB);
+    uint64_t* full = reinterpret_cast<uint64_t*>(sring + C::NS * TN);
+    uint64_t* empty = full + C::NS;
+    uint64_t* dfull = empty + C::NS;
+    uint64_t* dempty = dfull + C::ND;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dempty + C::ND);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int tile = static_cast<int>(blockIdx.x) / a.S, ks = static_cast<int>(blockIdx.x) % a.S;
+    int64_t g, m0;
+    int rows;
+    if (!find_rows(a, blockIdx.y, &g, &m0, &rows)) {  // the whole cluster alike
+        asm volatile("griddepcontrol.wait;" ::: "memory");  // this grid ends after the one that makes the rows
+        return;
+    }
+    const int p0 = static_cast<int>(static_cast<int64_t>(a.kb) * ks / a.S);
+    const int np = static_cast<int>(static_cast<int64_t>(a.kb) * (ks + 1) / a.S) - p0;
+    const int64_t t0 = g * a.group_tiles + tile * a.out_step + p0 * a.sum_step;  // the CTA's first tile
+    if (w == 8) {
+        tmem_alloc(tmem_slot, C::COLS);
+        tmem_relinquish();
+    } else if (w == 9 && lane == 0) {
+        for (int i = 0; i < C::NS; ++i) {
+            mbar_init(&full[i], 2 + 32);  // both copies' bytes and the scales of every lane
+            mbar_init(&empty[i], 1 + 8);  // the MMAs and the warps that read the scales
+        }
+        for (int i = 0; i < C::ND; ++i) {
+            mbar_init(&dfull[i], 1);
+            mbar_init(&dempty[i], 8);
+        }
+        *abort_flag = 0;
+        fence_barrier_init();
+    } else if (w == 10 && lane == 0) {
+        tma_prefetch_desc(&xmap);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    auto wait = [&](uint64_t* bar, int phase) {  // whole warps
+        if (__all_sync(~0u, mbar_try_wait(bar, phase & 1))) return true;
+        return __all_sync(~0u, mbar_wait_bounded(bar, phase & 1, abort_flag, a.err, ERR_GEMM_TIMEOUT)) != 0;
+    };
+
+    constexpr int CPT = TN / 2;  // rows of a thread
+    float acc[CPT] = {};
+    if (w < 8) {
+        const int h = w >> 2;
+        const uint32_t at = tmem + (static_cast<uint32_t>(32 * (w & 3)) << 16) + h * CPT;
+        float held = 0.0f;  // the weight scales of 32 blocks, one a lane
+        for (int u = 0; u < np; ++u) {
+            const int st = u % C::NS, b = u % C::ND;
+            if ((u & 31) == 0) held = u + lane < np ? a.ws[t0 + (u + lane) * a.sum_step] : 0.0f;
+            const float f = __shfl_sync(~0u, held, u & 31);
+            if (!wait(&full[st], u / C::NS) || !wait(&dfull[b], u / C::ND)) break;
+            tc_fence_after();
+            uint32_t d[CPT];
+            if constexpr (CPT == 8)
+                tc_ld_32x32b_x8(at + b * TN, d);
+            else if constexpr (CPT == 16)
+                tc_ld_32x32b_x16(at + b * TN, d);
+            else
+#pragma unroll
+                for (int c = 0; c < CPT; c += 32)
+                    tc_ld_32x32b_x32(at + b * TN + c, *reinterpret_cast<uint32_t(*)[32]>(d + c));
+            tc_wait_ld();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&dempty[b]);
+            const float4* sc = reinterpret_cast<const float4*>(sring + st * TN + h * CPT);
+#pragma unroll
+            for (int c = 0; c < CPT; c += 4) {
+                const float4 s = sc[c / 4];
+                fma2(acc[c], acc[c + 1], f, s.x, s.y, d[c], d[c + 1]);
+                fma2(acc[c + 2], acc[c + 3], f, s.z, s.w, d[c + 2], d[c + 3]);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[st]);
+        }
+    } else if (w == 8) {
+        const uint32_t idesc = idesc_e4m3_f32(128, static_cast<uint32_t>((rows + 15) & ~15), TRANS, false);
+        for (int u = 0; u < np; ++u) {
+            const int st = u % C::NS, b = u % C::ND;
+            if (!wait(&full[st], u / C::NS) || !wait(&dempty[b], u / C::ND + 1)) break;
+            tc_fence_after();
+            const uint64_t ad = smem_desc_sw128(smem_u32(ring + st * kFp8Tile));
+            const uint64_t bd = smem_desc_sw128(smem_u32(xring + st * C::XB));
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                tc_mma_f8_elect(tmem + b * TN, ad + i * kStep32<TRANS>, bd + i * kStep32<false>, idesc, i ? 1u : 0u);
+            tc_commit_elect(&empty[st]);
+            tc_commit_elect(&dfull[b]);
+        }
+    } else if (w == 9) {
+        if (lane == 0) {
+            int u = 0;
+            for (; u < np; ++u) {
+                const int st = u % C::NS;
+                if (!mbar_wait_bounded(&empty[st], (u / C::NS + 1) & 1, abort_flag, a.err, ERR_GEMM_TIMEOUT)) break;
+                mbar_arrive_expect_tx(&full[st], kFp8Tile);
+                bulk_load(ring + st * kFp8Tile, a.w + (t0 + u * a.sum_step) * kFp8Tile, kFp8Tile, &full[st]);
+            }
+            if (*abort_flag)  // a failed call leaves no copy in flight behind (bounded as well)
+                for (int i = max(0, u - C::NS); i < u; ++i)
+                    for (int t = 0; t < 1 << 14 && !mbar_try_wait(&full[i % C::NS], i / C::NS & 1); ++t) {
+                    }
+        }
+    } else {
+        asm volatile("griddepcontrol.wait;" ::: "memory");  // the rows may be another kernel's
+        const float* xs = a.xs + m0 * a.lds + p0;
+        int u = 0;
+        for (; u < np; ++u) {
+            const int st = u % C::NS;
+            if (!wait(&empty[st], u / C::NS + 1)) break;
+            if (lane == 0) {
+                mbar_arrive_expect_tx(&full[st], C::XB);
+                tma_load_2d(xring + st * C::XB, &xmap, &full[st], (p0 + u) * 128, static_cast<int>(m0));
+            }
+            for (int r = lane; r < rows; r += 32) copy4_async(sring + st * TN + r, xs + r * a.lds + u);
+            arrive_after_copies(&full[st]);
+        }
+        if (lane == 0 && *abort_flag)
+            for (int i = max(0, u - C::NS); i < u; ++i)
+                for (int t = 0; t < 1 << 14 && !mbar_try_wait(&full[i % C::NS], i / C::NS & 1); ++t) {
+                }
+    }
+
+    // every MMA has been waited for by the warps that read its sums (or the call
+    // failed): give the tensor memory back before any wait on another CTA
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (w == 8) tmem_dealloc(tmem, C::COLS);
+    float* fin = reinterpret_cast<float*>(ring);  // [TN][128]
+    float* recv = fin + TN * 128;                 // [S][share][128]
+    if (w < 8)
+#pragma unroll
+        for (int c = 0; c < CPT; ++c) fin[((w >> 2) * CPT + c) * 128 + (w & 3) * 32 + lane] = acc[c];
+    __syncthreads();
+    const int share = (rows + a.S - 1) / a.S;    // rows that a rank writes
+    const int64_t n = tile * 128ll + lane * 4;  // a warp has a row, a lane four columns of it
+    const float4* fin4 = reinterpret_cast<const float4*>(fin) + lane;
+    float4* recv4 = reinterpret_cast<float4*>(recv) + lane;
+    constexpr int WARPS = kFewThreads / 32;
+    if (a.S == 1) {
+        for (int r = w; r < rows; r += WARPS) store_out(a, m0 + r, n, fin4[r * 32]);
+        return;
+    }
+    cluster_sync();  // the ranks' rings are free
+    for (int r = w; r < rows; r += WARPS) {
+        const int to = r / share;
+        st_cluster(recv4 + (ks * share + r - to * share) * 32, to, fin4[r * 32]);
+    }
+    cluster_sync();
+    for (int r = w; r < share && ks * share + r < rows; r += WARPS) {
+        float4 v = recv4[r * 32];
+        for (int s = 1; s < a.S; ++s) {
+            const float4 u = recv4[(s * share + r) * 32];
+            v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+        }
+        store_out(a, m0 + ks * share + r, n, v);
+    }
+}
+
+// Rows of out outside every group.
+__global__ void __launch_bounds__(256)
+    zero_rest_kernel(const int32_t* __restrict__ group_rows, int G, int64_t M, int64_t N, int64_t ldo, int bf16, void* out) {
+    const int64_t first = min(max(static_cast<int64_t>(group_rows[0]), int64_t{0}), M);
+    const int64_t last = min(max(static_cast<int64_t>(group_rows[G]), int64_t{0}), M);
+    for (int64_t r = blockIdx.x; r < first + M - last; r += gridDim.x) {
+        const int64_t m = r < first ? r : last + r - first;
+        for (int64_t n = threadIdx.x; n < N; n += blockDim.x) {
+            if (bf16)
+                static_cast<__nv_bfloat16*>(out)[m * ldo + n] = __float2bfloat16_rn(0.0f);
+            else
+                static_cast<float*>(out)[m * ldo + n] = 0.0f;
+        }
+    }
+}
+
+constexpr int kSMs = 148;
+
+// CTAs (at most 8, one cluster) that split the sum, in blocks of a CTA: its set-up
+// and end take about 14, a hand-over between CTAs 6 more.
+int split_sum(int64_t ctas, int64_t blocks, int slots) {
+    int best = 1;
+    int64_t least = INT64_MAX;
+    for (int S = 1; S <= 8 && (S == 1 || blocks >= 2 * S); ++S) {
+        const int64_t each = (blocks + S - 1) / S, n = ctas * S;
+        const int64_t cost = (n + slots - 1) / slots * (14 + (S > 1 ? 6 : 0) + each);
+        if (cost < least) {
+            least = cost;
+            best = S;
+        }
+    }
+    return best;
+}
+
+template <int TN, bool ALONE>
+aem_status launch_few(Fp8Args a, const void* q, int64_t ldq, int64_t cols, bool transposed, bool dependent,
+                      int64_t slots, cudaStream_t s) {
+    using C = FewCfg<TN, ALONE>;
+    CUtensorMap xmap{};
+    AEM_TRY(make_tmap_2d_u8(&xmap, q, cols, a.M, ldq, TN, CU_TENSOR_MAP_SWIZZLE_128B));
+    auto kern = transposed ? fp8_few_kernel<TN, ALONE, true> : fp8_few_kernel<TN, ALONE, false>;
+    static std::atomic<uint64_t> ready[2];  // bit per device: the shared memory opt-in is done
+    const uint64_t bit = 1ull << (current_device() & 63);
+    if (!(ready[transposed].load(std::memory_order_relaxed) & bit)) {
+        AEM_TRY_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        ready[transposed].fetch_or(bit, std::memory_order_relaxed);
+    }
+    a.S = split_sum(a.nb * slots, a.kb, kSMs * C::CTAS);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(a.nb * a.S), static_cast<unsigned>(slots));
+    cfg.blockDim = dim3(kFewThreads);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2] = {};
+    int n = 0;
+    if (dependent) {  // starts under the kernel that quantises the rows
+        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (a.S > 1) {
+        at[n].id = cudaLaunchAttributeClusterDimension;
+        at[n].val.clusterDim.x = a.S;
+        at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    cfg.attrs = at;
+    cfg.numAttrs = n;
+    AEM_TRY_CUDA(cudaLaunchKernelEx(&cfg, kern, xmap, a));
+    count_launches(1);
+    return AEM_OK;
+}
+
+// Quantised rows in a workspace: bytes, then scales.
+struct Scratch {
+    int64_t ldq, lds;
+    size_t scale_at, bytes;
+};
+Scratch scratch_of(int64_t M, int64_t cols) {
+    Scratch z;
+    z.ldq = (cols + 15) / 16 * 16;
+    z.lds = ((cols + 127) / 128 + 3) / 4 * 4;
+    z.scale_at = align_up(static_cast<size_t>(M) * z.ldq, 16);
+    z.bytes = z.scale_at + static_cast<size_t>(M) * z.lds * sizeof(float);
+    return z;
+}
+
+struct Rows {  // the caller's x
+    const void* x;
+    aem_dtype dtype;
+    int64_t ldx;
+    const float* scale;
+    int64_t lds;
+};
+
+aem_status fp8_product(const Fp8Weight* w, const char* what, Fp8Args a, Rows x, bool transposed, int zero_rest,
+                       void* workspace, size_t workspace_bytes, cudaStream_t s) {
+    AEM_REQUIRE(current_device() == w->device, "%s: the weights are on device %d, the current one is %d", what,
+                w->device, current_device());
+    const int64_t cols = transposed ? w->N : w->K;
+    a.N = transposed ? w->K : w->N;
+    AEM_REQUIRE(a.ldo >= a.N, "%s: bad row stride of out", what);
+    a.w = w->data;
+    a.ws = w->scale;
+    a.group_tiles = w->NC * w->KC;
+    a.out_step = transposed ? 1 : w->KC;
+    a.sum_step = transposed ? w->KC : 1;
+    a.nb = static_cast<int>(transposed ? w->KC : w->NC);
+    a.kb = static_cast<int>(transposed ? w->NC : w->KC);
+    a.ovec = reinterpret_cast<uintptr_t>(a.out) % (a.out_bf16 ? 8 : 16) == 0 && a.ldo % 4 == 0;
+    a.err = device_error_word(w->device);
+    if (!a.err) {
+        set_error("%s: no device error word", what);
+        return AEM_ENOMEM;
+    }
+    // row tiles at most: n groups with rows have up to n + (M - n) / rows
+    const int64_t n = std::min<int64_t>(a.G, a.M);
+    const int64_t want = (a.M + n - 1) / n;
+    a.rows = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : 128;
+    const int64_t slots = a.group_rows ? n + (a.M - n) / a.rows : (a.M + a.rows - 1) / a.rows;
+    AEM_REQUIRE(slots <= 65535 && a.M < (1ll << 31), "%s: M=%lld rows are too many for one call", what, (long long)a.M);
+    void* own = nullptr;
+    const bool make = x.dtype != AEM_E4M3;
+    if (make) {
+        const Scratch z = scratch_of(a.M, cols);
+        AEM_REQUIRE(!workspace || (workspace_bytes >= z.bytes && reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
+                    "%s: workspace of %zu bytes (%zu needed, 16-byte aligned)", what, workspace_bytes, z.bytes);
+        if (!workspace) {
+            AEM_TRY_CUDA(cudaMallocAsync(&own, z.bytes, s));
+            workspace = own;
+        }
+        auto* q = static_cast<uint8_t*>(workspace);
+        auto* sc = reinterpret_cast<float*>(q + z.scale_at);
+        const aem_status st = launch_quantize_fp8(what, x.x, x.dtype, x.ldx, a.M, cols, q, z.ldq, sc, z.lds, s);
+        if (st != AEM_OK) {
+            if (own) cudaFreeAsync(own, s);
+            return st;
+        }
+        x = {q, AEM_E4M3, z.ldq, sc, z.lds};
+    }
+    a.xs = x.scale;
+    a.lds = x.lds;
+    aem_status st = a.rows == 16   ? launch_few<16, false>(a, x.x, x.ldx, cols, transposed, make, slots, s)
+                    : a.rows == 32 ? launch_few<32, false>(a, x.x, x.ldx, cols, transposed, make, slots, s)
+                    : a.rows == 64 ? launch_few<64, false>(a, x.x, x.ldx, cols, transposed, make, slots, s)
+                                   : launch_few<128, true>(a, x.x, x.ldx, cols, transposed, make, slots, s);
+    if (own) cudaFreeAsync(own, s);
+    AEM_TRY(st);
+    if (zero_rest) {
+        const auto grid = static_cast<unsigned>(std::min<int64_t>(a.M, kSMs * 8));
+        zero_rest_kernel<<<grid, 256, 0, s>>>(a.group_rows, a.G, a.M, a.N, a.ldo, a.out_bf16, a.out);
+        AEM_CHECK_LAUNCH();
+        count_launches(1);
+    }
+    return AEM_OK;
+}
+
+aem_status check_rows(const char* what, const Rows& x, int64_t cols, int64_t M) {
+    AEM_REQUIRE(x.dtype == AEM_F32 || x.dtype == AEM_BF16 || x.dtype == AEM_E4M3, "%s: bad dtype", what);
+    AEM_REQUIRE(x.ldx >= 0 && x.lds >= 0, "%s: bad row stride", what);
+    if (x.dtype == AEM_E4M3) {
+        AEM_REQUIRE(x.ldx >= cols && x.ldx % 16 == 0 && x.lds >= (cols + 127) / 128 && x.lds % 4 == 0,
+                    "%s: bad row stride of e4m3 rows or their scales", what);
+        AEM_REQUIRE(M == 0 || x.scale, "%s: e4m3 rows without scales", what);
+        AEM_REQUIRE(reinterpret_cast<uintptr_t>(x.x) % 16 == 0 && reinterpret_cast<uintptr_t>(x.scale) % 16 == 0,
+                    "%s: e4m3 rows and their scales must be 16-byte aligned", what);
+    } else {
+        AEM_REQUIRE(!x.scale, "%s: scales are for e4m3 rows", what);
+    }
+    return AEM_OK;
+}
+
+}  // namespace
+}  // namespace aem
+
+using aem::set_error;
+
+extern "C" {
+
+size_t aem_fp8gemm_workspace(aem_fp8weight_t wh, aem_dtype x_dtype, int64_t M, int transposed) {
+    if (!wh || M < 1 || (x_dtype != AEM_F32 && x_dtype != AEM_BF16)) return 0;
+    auto* w = reinterpret_cast<aem::Fp8Weight*>(wh);
+    return aem::scratch_of(M, transposed ? w->N : w->K).bytes;
+}
+
+aem_status aem_fp8gemm(aem_fp8weight_t wh, int64_t group, int transposed, const void* x, aem_dtype x_dtype,
+                       int64_t ldx, const float* x_scale, int64_t lds, int64_t M, void* out, aem_dtype out_dtype,
+                       int64_t ldo, void* workspace, size_t workspace_bytes, void* stream) {
+    AEM_REQUIRE(wh != nullptr, "aem_fp8gemm: weight handle is NULL");
+    auto* w = reinterpret_cast<aem::Fp8Weight*>(wh);
+    AEM_REQUIRE(group >= 0 && group < w->G, "aem_fp8gemm: group %lld out of range [0, %lld)", (long long)group,
+                (long long)w->G);
+    AEM_REQUIRE(M >= 0, "aem_fp8gemm: M must be >= 0");
+    AEM_REQUIRE(out_dtype == AEM_F32 || out_dtype == AEM_BF16, "aem_fp8gemm: bad dtype");
+    const aem::Rows rows{x, x_dtype, ldx, x_scale, lds};
+    AEM_TRY(aem::check_rows("aem_fp8gemm", rows, transposed ? w->N : w->K, M));
+    if (M == 0) return AEM_OK;
+    AEM_REQUIRE(x && out, "aem_fp8gemm: NULL buffer");
+    aem::Fp8Args a{};
+    a.out = out;
+    a.ldo = ldo;
+    a.M = M;
+    a.group = group;
+    a.G = 1;
+    a.out_bf16 = out_dtype == AEM_BF16;
+    return aem::fp8_product(w, "aem_fp8gemm", a, rows, transposed != 0, 0, workspace, workspace_bytes,
+                            static_cast<cudaStream_t>(stream));
+}
+
+aem_status aem_grouped_fp8gemm(aem_fp8weight_t wh, const int32_t* group_rows, int transposed, const void* x,
+                               aem_dtype x_dtype, int64_t ldx, const float* x_scale, int64_t lds, int64_t M, void* out,
+                               aem_dtype out_dtype, int64_t ldo, int relu, int zero_rest, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+    AEM_REQUIRE(wh != nullptr, "aem_grouped_fp8gemm: weight handle is NULL");
+    auto* w = reinterpret_cast<aem::Fp8Weight*>(wh);
+    AEM_REQUIRE(w->G <= AEM_MAX_EXPERTS, "aem_grouped_fp8gemm: %lld weight groups, at most %d", (long long)w->G,
+                AEM_MAX_EXPERTS);
+    AEM_REQUIRE(M >= 0, "aem_grouped_fp8gemm: M must be >= 0");
+    AEM_REQUIRE(out_dtype == AEM_F32 || out_dtype == AEM_BF16, "aem_grouped_fp8gemm: bad dtype");
+    const aem::Rows rows{x, x_dtype, ldx, x_scale, lds};
+    AEM_TRY(aem::check_rows("aem_grouped_fp8gemm", rows, transposed ? w->N : w->K, M));
+    if (M == 0) return AEM_OK;
+    AEM_REQUIRE(group_rows && x && out, "aem_grouped_fp8gemm: NULL buffer");
+    aem::Fp8Args a{};
+    a.out = out;
+    a.ldo = ldo;
+    a.M = M;
+    a.group_rows = group_rows;
+    a.G = static_cast<int>(w->G);
+    a.out_bf16 = out_dtype == AEM_BF16;
+    a.relu = relu != 0;
+    return aem::fp8_product(w, "aem_grouped_fp8gemm", a, rows, transposed != 0, zero_rest, workspace, workspace_bytes,
+                            static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -192,6 +192,26 @@ aem_status make_tmap_3d_u8(CUtensorMap* map, const void* base, uint64_t dim0, ui
     return AEM_OK;
 }
 
+aem_status make_tmap_2d_u8(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t row_bytes,
+                           uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+    AEM_TRY(tmap_encoder());
+    AEM_REQUIRE((reinterpret_cast<uintptr_t>(base) & 15) == 0 && row_bytes % 16 == 0,
+                "TMA base address and row stride must be multiples of 16 bytes");
+    cuuint64_t dims[2] = {cols, rows};
+    cuuint64_t strides[1] = {row_bytes};
+    cuuint32_t box[2] = {128, box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("cuTensorMapEncodeTiled failed (%d): %llu x %llu bytes", (int)r, (unsigned long long)cols,
+                  (unsigned long long)rows);
+        return AEM_ECUDA;
+    }
+    return AEM_OK;
+}
+
 // ------------------------------------------------------------------ launch counter
 namespace {
 std::atomic<uint64_t> g_launches{0};

@@ -182,9 +182,9 @@ def _ids(ids, num_experts):
         raise ValueError(f"k={ids.shape[1]} outside [1, {_lib.MAX_TOPK}]")
 
 
-def _weights(weights, shape):
+def _weights(weights, shape, name="weights"):
     if weights.dtype != torch.float32 or tuple(weights.shape) != tuple(shape):
-        raise ValueError(f"weights must be {tuple(shape)} float32, got {tuple(weights.shape)} {weights.dtype}")
+        raise ValueError(f"{name} must be {tuple(shape)} float32, got {tuple(weights.shape)} {weights.dtype}")
     if shape[1] > 1 and weights.stride(1) != 1:
         weights = weights.contiguous()
     return weights, weights.stride(0) if shape[0] > 1 else shape[1]

@@ -39,7 +39,11 @@ typedef enum {
     AEM_EDEVICE = 7       /* a kernel reported a failed in-kernel check (e.g. bad batch_position) */
 } aem_status;
 
-typedef enum { AEM_F32 = 0, AEM_BF16 = 1 } aem_dtype;
+typedef enum {
+    AEM_F32 = 0,
+    AEM_BF16 = 1,
+    AEM_E4M3 = 2 /* rows quantised by aem_quantize_fp8; only the fp8 products take them */
+} aem_dtype;
 
 /* Gating logit arithmetic.
  * EXACT: each product is a float32 product and products are summed in
@@ -403,6 +407,111 @@ aem_status aem_grouped_q4gemm(aem_q4weight_t w, const int32_t* group_rows, const
                               aem_dtype x_dtype, int64_t ldx, int64_t M, void* out,
                               aem_dtype out_dtype, int64_t ldo, int relu, void* workspace,
                               size_t workspace_bytes, void* stream);
+
+/* ---- routing of tokens to experts from logits, with its gradient ---------------------- */
+
+/* For callers with their own router projection (training, other scores than
+ * aem_gating's).  Row x of the logits and bias b (NULL: none), s = the scores:
+ *   key_e  = s_e + b_e; without a bias the logit (the scores' order)
+ *   value of a group of E/groups neighbouring experts = its largest key, or
+ *            (group_top = 2) the sum of its two largest, scores where there is
+ *            no bias; the top_groups largest groups stay
+ *   ids    = the k largest keys of the experts in them, in falling order
+ *   weight = scale * s, or with renormalize scale * s / (sum of the k s + 1e-20);
+ *            softmax scores are renormalised as the softmax of the k logits
+ * Ties go to the lower index.  The order is that of keys in 64-bit arithmetic,
+ * whatever a float32 exponential rounds to.  An expert whose logit or bias is
+ * -inf is never chosen; where fewer than k are left the id is -1 and the weight
+ * zero, which the dispatch and the combine take as a unit without an expert.  A
+ * NaN key ranks above every number, and its weights are NaN.  k <= AEM_MAX_TOPK
+ * and <= E / groups * top_groups, E <= AEM_MAX_EXPERTS.  The bias takes part in
+ * the choice alone, so it has no gradient.  The reference's gating
+ * (src/kernels/fused_gating_metal.py:236-307) has softmax weights without bias or
+ * groups, and no gradient. */
+typedef enum { AEM_SCORE_SOFTMAX = 0, AEM_SCORE_SIGMOID = 1 } aem_score;
+typedef struct {
+    aem_score score;
+    int k;
+    int groups;     /* 1: no groups */
+    int top_groups;
+    int group_top;  /* 1 or 2 */
+    int renormalize;
+    float scale;
+} aem_route_config;
+
+/* logits [T, E] (rows ld elements apart) -> ids int32 [T, k], weights float32 [T, k]. */
+aem_status aem_route_tokens(const aem_route_config* config, const void* logits, aem_dtype dtype,
+                            int64_t ld, int64_t T, int E, const float* bias, int32_t* ids,
+                            float* weights, void* stream);
+/* Gradient of the weights: grad_weights [T, k] (rows ldg apart) -> grad_logits
+ * [T, E] (rows ldo apart, the logits' dtype), for the ids [T, k] (rows ldi apart)
+ * of the forward call.  The choice itself has no gradient.  A negative id is a
+ * slot without an expert; so is one of E or more, which aem_device_status reports.
+ * An id that stands twice in a row counts twice. */
+aem_status aem_route_tokens_backward(const aem_route_config* config, const float* grad_weights,
+                                     int64_t ldg, const void* logits, aem_dtype dtype, int64_t ld,
+                                     int64_t T, int E, const int32_t* ids, int64_t ldi,
+                                     void* grad_logits, int64_t ldo, void* stream);
+
+/* ---- 8-bit floating point in blocks of 128 -------------------------------------------- */
+
+/* Rows in blocks of 128 elements: x [M, K] (float32 or bf16, rows ldx apart) ->
+ *   scale[m][b] = max(max |x| / 448, 2^-126) over block b, IEEE float32 division
+ *   q[m][k]     = x / scale (IEEE float32 division) rounded to e4m3, ties to even
+ * q: rows ldq bytes apart, ldq a multiple of 16, q 16-byte aligned; the bytes from
+ * K to the next multiple of 16 are zeroed.  scale: float32, rows lds apart, lds a
+ * multiple of 4, scale 16-byte aligned, ceil(K/128) to a row.  A NaN or infinity
+ * makes its block's scale one, and products with the row show it. */
+aem_status aem_quantize_fp8(const void* x, aem_dtype dtype, int64_t ldx, int64_t M, int64_t K,
+                            uint8_t* q, int64_t ldq, float* scale, int64_t lds, void* stream);
+/* Weights in blocks of 128 x 128: w [G][K][N] -> q [G][K][N] e4m3 and
+ * scale [G][ceil(K/128)][ceil(N/128)] by the same rule. */
+aem_status aem_quantize_fp8_weight(const void* w, aem_dtype dtype, int64_t G, int64_t K, int64_t N,
+                                   uint8_t* q, float* scale, void* stream);
+
+typedef struct aem_fp8weight_s* aem_fp8weight_t;
+
+/* Packs G groups (experts) of e4m3 weights q [G][K][N] with scales
+ * [G][ceil(K/128)][ceil(N/128)] into a device-resident copy laid out in tiles of
+ * 128 x 128 (16 KB each, K and N rounded up to 128).  From HOST memory onto
+ * `device`, which need not be the current one and does not become it, or from
+ * DEVICE memory in stream order. */
+aem_status aem_fp8weight_pack(const uint8_t* q, const float* scale, int64_t G, int64_t K, int64_t N,
+                              int device, aem_fp8weight_t* out);
+aem_status aem_fp8weight_pack_device(const uint8_t* q, const float* scale, int64_t G, int64_t K,
+                                     int64_t N, void* stream, aem_fp8weight_t* out);
+aem_status aem_fp8weight_free(aem_fp8weight_t w);
+/* Dimensions of a packed weight (any pointer may be NULL). */
+aem_status aem_fp8weight_shape(aem_fp8weight_t w, int64_t* G, int64_t* K, int64_t* N);
+
+/* out[m, n] = sum_b xs[m, b] ws[b, n/128] sum_{k in block b} xq[m, k] wq[k, n]:
+ * a block's sum on the tensor cores (e4m3 operands, float32 accumulators), the
+ * scales and the sum over the blocks in float32.  x is either float32 or bf16,
+ * rows ldx apart, and quantised as aem_quantize_fp8 does (x_scale NULL, lds 0),
+ * or AEM_E4M3 rows that it wrote, with their scales (ldx bytes and lds as there).
+ * transposed != 0 multiplies by the transposed weight instead, x [M, N] -> out
+ * [M, K]: the gradient of the rows from the same packed weight, x the gradient of
+ * the product.  The workspace holds float32 or bf16 rows in their quantised form:
+ * device scratch of aem_fp8gemm_workspace bytes (0 for AEM_E4M3), 16-byte aligned,
+ * or NULL to have the call allocate and free it in stream order.  Rows of out are
+ * ldo elements apart, any alignment works.  out must not overlap x or the
+ * workspace; the weights' device must be the current one; make the first call on a
+ * device before a stream capture.  Results repeat bit for bit. */
+size_t aem_fp8gemm_workspace(aem_fp8weight_t w, aem_dtype x_dtype, int64_t M, int transposed);
+aem_status aem_fp8gemm(aem_fp8weight_t w, int64_t group, int transposed, const void* x,
+                       aem_dtype x_dtype, int64_t ldx, const float* x_scale, int64_t lds, int64_t M,
+                       void* out, aem_dtype out_dtype, int64_t ldo, void* workspace,
+                       size_t workspace_bytes, void* stream);
+/* Grouped form (expert products of dispatched rows): rows [group_rows[g],
+ * group_rows[g+1]) of x (device int32 array of G+1 increasing offsets:
+ * aem_dispatch's starts) times weight group g, for all G <= AEM_MAX_EXPERTS groups
+ * of w, with out = relu(...) when relu != 0.  Offsets are clamped to [0, M].  Rows
+ * of out outside every group are zeroed when zero_rest != 0, else not written. */
+aem_status aem_grouped_fp8gemm(aem_fp8weight_t w, const int32_t* group_rows, int transposed,
+                               const void* x, aem_dtype x_dtype, int64_t ldx, const float* x_scale,
+                               int64_t lds, int64_t M, void* out, aem_dtype out_dtype, int64_t ldo,
+                               int relu, int zero_rest, void* workspace, size_t workspace_bytes,
+                               void* stream);
 
 /* ---- MoE layer (gating -> routing -> grouped INT8 expert FFN -> combine) --------- */
 
