@@ -492,6 +492,17 @@ __device__ __forceinline__ void tc_mma_f8_elect(uint32_t d_tmem, uint64_t a_desc
         : "memory");
 }
 
+__device__ __forceinline__ void tc_mma_f8_pair_elect(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                                     uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
 // Instruction descriptor of kind::f8f6f4: e4m3 A and B, f32 D.  An operand is
 // K-major, or MN-major where its transpose bit is set.
 __host__ __device__ constexpr uint32_t idesc_e4m3_f32(uint32_t m, uint32_t n, bool a_mn, bool b_mn) {

@@ -35,7 +35,7 @@ struct Fp8Args {
     int64_t out_step, sum_step; // tiles from one 128 of out's columns (of the sum) to the next
     int nb, kb, G, S, rows;     // 128-blocks of out's columns and of the sum; S: CTAs (one cluster) that split
                                 // the sum; rows: rows of a row tile
-    int out_bf16, relu, ovec;   // ovec: out can be stored in vectors of 4
+    int out_bf16, relu, ovec, ovec16;  // ovec: out can be stored in vectors of 4; ovec16: of 16 bytes
     int* err;
 };
 
@@ -346,6 +346,317 @@ __global__ void __launch_bounds__(kFewThreads, ALONE ? 1 : 2)
     }
 }
 
+// Many rows: a pair of SMs computes 256 rows x 256 columns of out, one CTA 128
+// rows of it.  Rows are the MMA's M (a thread has a row, so a block's two scales are
+// one factor for all of its columns), weights its N, half of them in each CTA's
+// shared memory, which halves what has to be read for them.  The pair is persistent
+// over tiles.
+//   warp 0      copies a block's rows and weights, 16 KB each, into the ring
+//   warp 1      issues the pair's MMAs (M = 256, N = 256, K = 32) in CTA 0, four a
+//               block, into one of two accumulators that fill tensor memory
+//   warps 4-11  thread = row = TMEM lane; warps 4-7 have the first 128 columns, 8-11
+//               the rest.  A block's accumulator comes back 32 columns at a time and
+//               factor * sum is added to 128 registers; at the tile's end these go
+//               through shared memory into whole pieces of rows.
+// Every wait is bounded; a timeout sets the error word and ends all roles of both CTAs.
+constexpr int kManyThreads = 12 * 32, kManyStages = 5, kManyTile = 256;
+constexpr int kManyStage = 2 * kFp8Tile;                      // of one CTA
+constexpr int kManyOut = 8 * 4096;                            // 32 rows x 128 bytes for each warp
+constexpr int kManyBars = (2 * kManyStages + 4) * 8 + 16;
+constexpr int kManySmem = 1024 + kManyStages * kManyStage + kManyOut + kManyBars + (2 * AEM_MAX_EXPERTS + 2) * 4;
+// Registers of a thread of warps 0-3 and of warps 4-11: together what the block is launched with.
+constexpr int kManyFewRegs = 40, kManyManyRegs = 232;
+static_assert(kManyFewRegs * 128 + kManyManyRegs * 256 <= 168 * kManyThreads, "register shares");
+constexpr int kBand = 16;  // row tiles that share the columns' weights before the next ones come
+
+// Bounded wait of a whole warp that, on giving up, raises the abort flag of both CTAs.
+__device__ __forceinline__ bool pair_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t peer,
+                                          int* err) {
+    if (__all_sync(~0u, mbar_try_wait(bar, parity & 1))) return true;
+    const uint64_t t0 = globaltimer_ns();
+    while (true) {
+        if (__all_sync(~0u, mbar_try_wait(bar, parity & 1))) return true;
+        if (__any_sync(~0u, *abort_flag != 0)) return false;
+        if (__any_sync(~0u, globaltimer_ns() - t0 > 2000000000ull)) {
+            *abort_flag = 1;
+            st_remote_u32(const_cast<int*>(abort_flag), peer, 1u);
+            atomicOr(err, ERR_GEMM_TIMEOUT);
+            return false;
+        }
+    }
+}
+
+// a0 += f * v0, a1 += f * v1
+__device__ __forceinline__ void fma2(float& a0, float& a1, float f, uint32_t v0, uint32_t v1) {
+    asm("{\n.reg .b64 a, f, v;\nmov.b64 a, {%0, %1};\nmov.b64 f, {%2, %2};\nmov.b64 v, {%3, %4};\n"
+        "fma.rn.f32x2 a, f, v, a;\nmov.b64 {%0, %1}, a;\n}"
+        : "+f"(a0), "+f"(a1)
+        : "f"(f), "r"(v0), "r"(v1));
+}
+
+__device__ __forceinline__ uint32_t bf16x2_of(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+struct ManyTile {
+    int64_t t0;    // first weight tile of the pair's columns
+    int m0, rows;  // first row and number of rows
+    int col;       // first 128-block of columns
+};
+__device__ __forceinline__ ManyTile many_tile(const Fp8Args& a, int t, const int* s_rows, const int* s_tiles) {
+    int lo = 0, hi = a.G;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s_tiles[mid] <= t) lo = mid; else hi = mid;
+    }
+    const int nc = (a.nb + 1) / 2, r = t - s_tiles[lo], n = (s_tiles[lo + 1] - s_tiles[lo]) / nc;
+    const int band = r / (kBand * nc), in = r - band * kBand * nc, high = min(kBand, n - band * kBand);
+    ManyTile o;
+    const int first = (band * kBand + in % high) * kManyTile;
+    o.col = in / high * 2;
+    o.m0 = s_rows[lo] + first;
+    o.rows = min(kManyTile, s_rows[lo + 1] - o.m0);
+    o.t0 = (a.group_rows ? lo : a.group) * a.group_tiles;
+    return o;
+}
+
+template <bool TRANS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads, 1)
+    fp8_many_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
+                    const __grid_constant__ Fp8Args a) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                               ~static_cast<uintptr_t>(1023));
+    uint8_t* outs = ring + kManyStages * kManyStage;
+    uint64_t* full = reinterpret_cast<uint64_t*>(outs + kManyOut);  // used in CTA 0
+    uint64_t* empty = full + kManyStages;
+    uint64_t* dfull = empty + kManyStages;
+    uint64_t* dempty = dfull + 2;  // used in CTA 0
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dempty + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* s_rows = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(full) + kManyBars);
+    int* s_tiles = s_rows + AEM_MAX_EXPERTS + 1;
+
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const uint32_t cta = cluster_rank(), peer = cta ^ 1u;
+    const int pair = static_cast<int>(blockIdx.x >> 1), pairs = static_cast<int>(gridDim.x >> 1);
+    if (w == 0 && lane == 0) {
+        for (int i = 0; i < kManyStages; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&dfull[i], 1);
+            mbar_init(&dempty[i], 16);  // the warps of both CTAs that read it
+        }
+        *abort_flag = 0;
+        fence_barrier_init();
+        tma_prefetch_desc(&xmap);
+        tma_prefetch_desc(&wmap);
+    } else if (w == 1) {
+        tmem_alloc_pair(tmem_slot, 512);  // the same warp of both CTAs
+        tmem_relinquish_pair();
+    } else if (w == 2) {
+        // first rows and first tiles of the groups, 32 groups at a time
+        const int nc = (a.nb + 1) / 2, M = static_cast<int>(a.M);
+        int before = 0;
+        for (int i = 0; i < a.G; i += 32) {
+            int lo = 0, hi = 0;
+            if (i + lane < a.G) {
+                lo = a.group_rows ? min(max(a.group_rows[i + lane], 0), M) : 0;
+                hi = a.group_rows ? min(max(a.group_rows[i + lane + 1], 0), M) : M;
+            }
+            const int n = hi > lo ? (hi - lo + kManyTile - 1) / kManyTile * nc : 0;
+            int s = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(~0u, s, o);
+                if (lane >= o) s += v;
+            }
+            if (i + lane < a.G) {
+                s_rows[i + lane] = lo;
+                s_tiles[i + lane] = before + s - n;
+                if (i + lane == a.G - 1) s_rows[a.G] = hi, s_tiles[a.G] = before + s;
+            }
+            before += __shfl_sync(~0u, s, 31);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // both CTAs' barriers are there before any remote arrival
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int total = s_tiles[a.G];
+
+    if (w < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kManyFewRegs));
+        if (w == 0) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");  // the rows may be another kernel's
+            int st = 0;
+            uint32_t phase = 0;
+            int issued = 0;
+            bool ok = true;
+            for (int t = pair; ok && t < total; t += pairs) {
+                const ManyTile z = many_tile(a, t, s_rows, s_tiles);
+                // an odd number of blocks: the last pair's second half takes the last block
+                // again, its results are not stored
+                const int64_t tile = z.t0 + min(z.col + static_cast<int>(cta), a.nb - 1) * a.out_step;
+                const int row = z.m0 + static_cast<int>(cta) * 128;
+                for (int u = 0; u < a.kb; ++u) {
+                    if (!(ok = pair_wait(&empty[st], phase ^ 1, abort_flag, peer, a.err))) break;
+                    if (lane == 0) {
+                        uint8_t* to = ring + st * kManyStage;
+                        // both CTAs' bytes complete on CTA 0's barrier
+                        if (cta == 0) mbar_arrive_expect_tx(&full[st], 2 * kManyStage);
+                        tma_load_2d_pair(to, &xmap, &full[st], 0, u * 128, row);
+                        tma_load_2d_pair(to + kFp8Tile, &wmap, &full[st], 0, 0,
+                                         static_cast<int>((tile + u * a.sum_step) * 128));
+                    }
+                    ++issued;
+                    if (++st == kManyStages) st = 0, phase ^= 1;
+                }
+            }
+            if (!ok && cta == 0 && lane == 0)  // a failed call leaves no copy in flight behind (bounded as well)
+                for (int i = max(0, issued - kManyStages); i < issued; ++i)
+                    for (int n = 0; n < 1 << 14 && !mbar_try_wait(&full[i % kManyStages], i / kManyStages & 1); ++n) {
+                    }
+        } else if (w == 1 && cta == 0) {
+            constexpr uint32_t idesc = idesc_e4m3_f32(256, 256, false, TRANS);
+            int st = 0;
+            uint32_t phase = 0, it = 0;
+            bool ok = true;
+            for (int t = pair; ok && t < total; t += pairs)
+                for (int u = 0; u < a.kb; ++u, ++it) {
+                    const uint32_t b = it & 1;
+                    if (!(ok = pair_wait(&full[st], phase, abort_flag, peer, a.err) &&
+                               pair_wait(&dempty[b], (it >> 1) + 1, abort_flag, peer, a.err)))
+                        break;
+                    tc_fence_after();
+                    const uint64_t ad = smem_desc_sw128(smem_u32(ring + st * kManyStage));
+                    const uint64_t bd = smem_desc_sw128(smem_u32(ring + st * kManyStage + kFp8Tile));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        tc_mma_f8_pair_elect(tmem + b * 256, ad + i * kStep32<false>, bd + i * kStep32<TRANS>, idesc,
+                                             i ? 1u : 0u);
+                    tc_commit_pair_elect(&empty[st], 0x3);
+                    tc_commit_pair_elect(&dfull[b], 0x3);
+                    if (++st == kManyStages) st = 0, phase ^= 1;
+                }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyManyRegs));
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        const int h = (w - 4) >> 2, q = w & 3;
+        const uint32_t at = tmem + (static_cast<uint32_t>(32 * q) << 16) + h * 128;
+        uint8_t* stage = outs + (w - 4) * 4096;
+        uint32_t it = 0;
+        bool ok = true;
+        for (int t = pair; ok && t < total; t += pairs) {
+            const ManyTile z = many_tile(a, t, s_rows, s_tiles);
+            const int r0 = static_cast<int>(cta) * 128 + q * 32;  // the warp's first row in the tile
+            const int64_t row = min(static_cast<int64_t>(z.m0) + r0 + lane, a.M - 1);
+            const float* xs = a.xs + row * a.lds;
+            const float* ws = a.ws + z.t0 + min(z.col + h, a.nb - 1) * a.out_step;
+            float acc[128];
+#pragma unroll
+            for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
+            float held = 0.0f;  // the weight scales of 32 blocks, one a lane
+            float4 sx = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int u = 0; u < a.kb; ++u, ++it) {
+                if ((u & 31) == 0) held = u + lane < a.kb ? ws[(u + lane) * a.sum_step] : 0.0f;
+                if ((u & 3) == 0) {
+                    if (u + 4 <= a.kb) {
+                        sx = *reinterpret_cast<const float4*>(xs + u);
+                    } else {
+                        sx.x = xs[u];
+                        sx.y = u + 1 < a.kb ? xs[u + 1] : 0.0f;
+                        sx.z = u + 2 < a.kb ? xs[u + 2] : 0.0f;
+                    }
+                }
+                const float f = sx.x * __shfl_sync(~0u, held, u & 31);
+                sx = make_float4(sx.y, sx.z, sx.w, 0.0f);
+                const uint32_t b = it & 1;
+                if (!(ok = pair_wait(&dfull[b], it >> 1, abort_flag, peer, a.err))) break;
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < 128; c += 32) {
+                    uint32_t d[32];
+                    tc_ld_32x32b_x32(at + b * 256 + c, d);
+                    tc_wait_ld();
+                    if (c == 96) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (cta == 0)
+                                mbar_arrive(&dempty[b]);
+                            else
+                                mbar_arrive_remote(&dempty[b], 0);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) fma2(acc[c + i], acc[c + i + 1], f, d[i], d[i + 1]);
+                }
+            }
+            if (!ok || r0 >= z.rows) continue;
+            if (a.relu)
+#pragma unroll
+                for (int i = 0; i < 128; ++i) acc[i] = relu_of(acc[i]);
+            // 128 bytes of each of the warp's rows at a time, 16-byte chunks swizzled
+            const int64_t n0 = (z.col + h) * 128ll;
+            const int per = a.out_bf16 ? 64 : 32;  // columns
+#pragma unroll
+            for (int c = 0; c < 128; c += 32) {
+                if (a.out_bf16 && (c & 32)) continue;
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    uint4 v;
+                    if (a.out_bf16) {
+                        if (c & 32) continue;
+                        const int i = c + 8 * j < 128 ? c + 8 * j : 0;
+                        v = make_uint4(bf16x2_of(acc[i], acc[i + 1]), bf16x2_of(acc[i + 2], acc[i + 3]),
+                                       bf16x2_of(acc[i + 4], acc[i + 5]), bf16x2_of(acc[i + 6], acc[i + 7]));
+                    } else {
+                        const int i = c + 4 * j;
+                        v = make_uint4(__float_as_uint(acc[i]), __float_as_uint(acc[i + 1]),
+                                       __float_as_uint(acc[i + 2]), __float_as_uint(acc[i + 3]));
+                    }
+                    *reinterpret_cast<uint4*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = v;
+                }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int r = i * 4 + (lane >> 3), j = lane & 7;
+                    const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((j ^ (r & 7)) << 4));
+                    if (r0 + r >= z.rows) continue;
+                    const int64_t n = n0 + c + j * (per / 8), o = (z.m0 + r0 + r) * a.ldo + n;
+                    if (a.ovec16 && n + per / 8 <= a.N) {
+                        *reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.out) + o * (a.out_bf16 ? 2 : 4)) = v;
+                        continue;
+                    }
+                    const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        if (k >= per / 8 || n + k >= a.N) break;
+                        if (a.out_bf16)
+                            static_cast<uint16_t*>(a.out)[o + k] = static_cast<uint16_t>(e[k / 2] >> (16 * (k & 1)));
+                        else
+                            static_cast<uint32_t*>(a.out)[o + k] = e[k & 3];
+                    }
+                }
+            }
+        }
+    }
+
+    // the pair's MMAs, commits and remote arrivals are done
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    if (w == 1) tmem_dealloc_pair(tmem, 512);
+}
+
 // Rows of out outside every group.
 __global__ void __launch_bounds__(256)
     zero_rest_kernel(const int32_t* __restrict__ group_rows, int G, int64_t M, int64_t N, int64_t ldo, int bf16, void* out) {
@@ -418,6 +729,58 @@ aem_status launch_few(Fp8Args a, const void* q, int64_t ldq, int64_t cols, bool 
     return AEM_OK;
 }
 
+// Pairs of SMs that can run the kernel at once.
+int max_pairs(int device) {
+    static std::atomic<int> cache[64];
+    int n = cache[device & 63].load(std::memory_order_relaxed);
+    if (n > 0) return n;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(2 * 512);
+    cfg.blockDim = dim3(kManyThreads);
+    cfg.dynamicSmemBytes = kManySmem;
+    if (cudaOccupancyMaxActiveClusters(&n, fp8_many_kernel<false>, &cfg) != cudaSuccess || n < 1) {
+        cudaGetLastError();
+        n = kSMs / 2;
+    }
+    cache[device & 63].store(n, std::memory_order_relaxed);
+    return n;
+}
+
+aem_status launch_many(const Fp8Args& a, const Fp8Weight* w, const void* q, int64_t ldq, int64_t cols, bool transposed,
+                       bool dependent, int64_t row_tiles, cudaStream_t s) {
+    CUtensorMap xmap{}, wmap{};
+    AEM_TRY(make_tmap_2d_u8(&xmap, q, cols, a.M, ldq, 128, CU_TENSOR_MAP_SWIZZLE_128B));
+    AEM_TRY(make_tmap_2d_u8(&wmap, w->data, 128, w->G * w->NC * w->KC * 128, 128, 128, CU_TENSOR_MAP_SWIZZLE_NONE));
+    static std::atomic<uint64_t> ready{0};  // bit per device: the shared memory opt-in is done
+    const int device = current_device();
+    const uint64_t bit = 1ull << (device & 63);
+    if (!(ready.load(std::memory_order_relaxed) & bit)) {
+        for (auto kern : {fp8_many_kernel<false>, fp8_many_kernel<true>}) {
+            AEM_TRY_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kManySmem));
+            cudaFuncAttributes f;
+            AEM_TRY_CUDA(cudaFuncGetAttributes(&f, kern));
+            if (f.numRegs * kManyThreads < kManyFewRegs * 128 + kManyManyRegs * 256) {
+                set_error("fp8_many_kernel: %d registers a thread cannot be shared out", f.numRegs);
+                return AEM_EUNSUPPORTED;
+            }
+        }
+        ready.fetch_or(bit, std::memory_order_relaxed);
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(2 * std::min<int64_t>(max_pairs(device), row_tiles * ((a.nb + 1) / 2))));
+    cfg.blockDim = dim3(kManyThreads);
+    cfg.dynamicSmemBytes = kManySmem;
+    cfg.stream = s;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // starts under the kernel that quantises the rows
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = dependent ? 1 : 0;
+    AEM_TRY_CUDA(cudaLaunchKernelEx(&cfg, transposed ? fp8_many_kernel<true> : fp8_many_kernel<false>, xmap, wmap, a));
+    count_launches(1);
+    return AEM_OK;
+}
+
 // Quantised rows in a workspace: bytes, then scales.
 struct Scratch {
     int64_t ldq, lds;
@@ -455,6 +818,7 @@ aem_status fp8_product(const Fp8Weight* w, const char* what, Fp8Args a, Rows x, 
     a.nb = static_cast<int>(transposed ? w->KC : w->NC);
     a.kb = static_cast<int>(transposed ? w->NC : w->KC);
     a.ovec = reinterpret_cast<uintptr_t>(a.out) % (a.out_bf16 ? 8 : 16) == 0 && a.ldo % 4 == 0;
+    a.ovec16 = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.ldo % (a.out_bf16 ? 8 : 4) == 0;
     a.err = device_error_word(w->device);
     if (!a.err) {
         set_error("%s: no device error word", what);
@@ -463,9 +827,10 @@ aem_status fp8_product(const Fp8Weight* w, const char* what, Fp8Args a, Rows x, 
     // row tiles at most: n groups with rows have up to n + (M - n) / rows
     const int64_t n = std::min<int64_t>(a.G, a.M);
     const int64_t want = (a.M + n - 1) / n;
-    a.rows = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : 128;
+    const bool many = want >= 192;
+    a.rows = many ? kManyTile : want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : 128;
     const int64_t slots = a.group_rows ? n + (a.M - n) / a.rows : (a.M + a.rows - 1) / a.rows;
-    AEM_REQUIRE(slots <= 65535 && a.M < (1ll << 31), "%s: M=%lld rows are too many for one call", what, (long long)a.M);
+    AEM_REQUIRE((many || slots <= 65535) && slots * ((a.nb + 1) / 2) < (1ll << 31) && a.M < (1ll << 31), "%s: M=%lld rows are too many for one call", what, (long long)a.M);
     void* own = nullptr;
     const bool make = x.dtype != AEM_E4M3;
     if (make) {
@@ -487,7 +852,8 @@ aem_status fp8_product(const Fp8Weight* w, const char* what, Fp8Args a, Rows x, 
     }
     a.xs = x.scale;
     a.lds = x.lds;
-    aem_status st = a.rows == 16   ? launch_few<16, false>(a, x.x, x.ldx, cols, transposed, make, slots, s)
+    aem_status st = many           ? launch_many(a, w, x.x, x.ldx, cols, transposed, make, slots, s)
+                    : a.rows == 16   ? launch_few<16, false>(a, x.x, x.ldx, cols, transposed, make, slots, s)
                     : a.rows == 32 ? launch_few<32, false>(a, x.x, x.ldx, cols, transposed, make, slots, s)
                     : a.rows == 64 ? launch_few<64, false>(a, x.x, x.ldx, cols, transposed, make, slots, s)
                                    : launch_few<128, true>(a, x.x, x.ldx, cols, transposed, make, slots, s);
