@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(kFewThreads, ALONE ? 1 : 2)
 
 // Many rows: a pair of SMs computes 256 rows x 256 columns of out, one CTA 128
 // rows of it.  Rows are the MMA's M (a thread has a row, so a block's two scales are
-// one factor for all of its columns), weights its N, half of them in each CTA's
+// one factor for all of its columns), the weights are its N, half of them in each CTA's
 // shared memory, which halves what has to be read for them.  The pair is persistent
 // over tiles.
 //   warp 0      copies a block's rows and weights, 16 KB each, into the ring
@@ -356,12 +356,13 @@ __global__ void __launch_bounds__(kFewThreads, ALONE ? 1 : 2)
 //               block, into one of two accumulators that fill tensor memory
 //   warps 4-11  thread = row = TMEM lane; warps 4-7 have the first 128 columns, 8-11
 //               the rest.  A block's accumulator comes back 32 columns at a time and
-//               factor * sum is added to 128 registers; at the tile's end these go
-//               through shared memory into whole pieces of rows.
+//               factor * sum is added to 128 registers; at the tile's end these leave
+//               through shared memory in bulk copies of whole pieces of rows.
 // Every wait is bounded; a timeout sets the error word and ends all roles of both CTAs.
-constexpr int kManyThreads = 12 * 32, kManyStages = 5, kManyTile = 256;
+constexpr int kManyThreads = 12 * 32, kManyStages = 4, kManyTile = 256;
 constexpr int kManyStage = 2 * kFp8Tile;                      // of one CTA
-constexpr int kManyOut = 8 * 4096;                            // 32 rows x 128 bytes for each warp
+constexpr int kManyPitch = 256 + 16;                          // a row's 256 bytes of out, in other banks than the next's
+constexpr int kManyOut = 8 * 32 * kManyPitch;
 constexpr int kManyBars = (2 * kManyStages + 4) * 8 + 16;
 constexpr int kManySmem = 1024 + kManyStages * kManyStage + kManyOut + kManyBars + (2 * AEM_MAX_EXPERTS + 2) * 4;
 // Registers of a thread of warps 0-3 and of warps 4-11: together what the block is launched with.
@@ -388,7 +389,7 @@ __device__ __forceinline__ bool pair_wait(uint64_t* bar, uint32_t parity, volati
 
 // a0 += f * v0, a1 += f * v1
 __device__ __forceinline__ void fma2(float& a0, float& a1, float f, uint32_t v0, uint32_t v1) {
-    asm("{\n.reg .b64 a, f, v;\nmov.b64 a, {%0, %1};\nmov.b64 f, {%2, %2};\nmov.b64 v, {%3, %4};\n"
+    asm volatile("{\n.reg .b64 a, f, v;\nmov.b64 a, {%0, %1};\nmov.b64 f, {%2, %2};\nmov.b64 v, {%3, %4};\n"
         "fma.rn.f32x2 a, f, v, a;\nmov.b64 {%0, %1}, a;\n}"
         : "+f"(a0), "+f"(a1)
         : "f"(f), "r"(v0), "r"(v1));
@@ -397,6 +398,19 @@ __device__ __forceinline__ void fma2(float& a0, float& a1, float f, uint32_t v0,
 __device__ __forceinline__ uint32_t bf16x2_of(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Waits for the loads from tensor memory; what they bring is used behind it.
+__device__ __forceinline__ void wait_ld(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                   "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                   "+r"(r[30])
+                 :
+                 : "memory");
+    asm volatile("" : "+r"(r[31])::"memory");
 }
 
 struct ManyTile {
@@ -549,7 +563,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads, 1)
         asm volatile("griddepcontrol.wait;" ::: "memory");
         const int h = (w - 4) >> 2, q = w & 3;
         const uint32_t at = tmem + (static_cast<uint32_t>(32 * q) << 16) + h * 128;
-        uint8_t* stage = outs + (w - 4) * 4096;
+        uint8_t* stage = outs + (w - 4) * 32 * kManyPitch;
         uint32_t it = 0;
         bool ok = true;
         for (int t = pair; ok && t < total; t += pairs) {
@@ -562,29 +576,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads, 1)
 #pragma unroll
             for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
             float held = 0.0f;  // the weight scales of 32 blocks, one a lane
-            float4 sx = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            // the row's scales, four blocks at a time, the next four on their way
+            auto scales = [&](int u) {
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (u + 4 <= a.kb) return *reinterpret_cast<const float4*>(xs + u);
+                if (u < a.kb) v.x = xs[u];
+                if (u + 1 < a.kb) v.y = xs[u + 1];
+                if (u + 2 < a.kb) v.z = xs[u + 2];
+                return v;
+            };
+            float4 sx, next = scales(0);
             for (int u = 0; u < a.kb; ++u, ++it) {
                 if ((u & 31) == 0) held = u + lane < a.kb ? ws[(u + lane) * a.sum_step] : 0.0f;
                 if ((u & 3) == 0) {
-                    if (u + 4 <= a.kb) {
-                        sx = *reinterpret_cast<const float4*>(xs + u);
-                    } else {
-                        sx.x = xs[u];
-                        sx.y = u + 1 < a.kb ? xs[u + 1] : 0.0f;
-                        sx.z = u + 2 < a.kb ? xs[u + 2] : 0.0f;
-                    }
+                    sx = next;
+                    next = scales(u + 4);
                 }
                 const float f = sx.x * __shfl_sync(~0u, held, u & 31);
                 sx = make_float4(sx.y, sx.z, sx.w, 0.0f);
                 const uint32_t b = it & 1;
                 if (!(ok = pair_wait(&dfull[b], it >> 1, abort_flag, peer, a.err))) break;
                 tc_fence_after();
+                uint32_t d[2][32];  // one on its way while the other is added
+                tc_ld_32x32b_x32(at + b * 256, d[0]);
 #pragma unroll
-                for (int c = 0; c < 128; c += 32) {
-                    uint32_t d[32];
-                    tc_ld_32x32b_x32(at + b * 256 + c, d);
-                    tc_wait_ld();
-                    if (c == 96) {
+                for (int c = 0; c < 4; ++c) {
+                    wait_ld(d[c & 1]);
+                    if (c < 3) {
+                        tc_ld_32x32b_x32(at + b * 256 + (c + 1) * 32, d[(c + 1) & 1]);
+                    } else {
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) {
@@ -595,58 +615,63 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads, 1)
                         }
                     }
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) fma2(acc[c + i], acc[c + i + 1], f, d[i], d[i + 1]);
+                    for (int i = 0; i < 32; i += 2)
+                        fma2(acc[c * 32 + i], acc[c * 32 + i + 1], f, d[c & 1][i], d[c & 1][i + 1]);
                 }
             }
             if (!ok || r0 >= z.rows) continue;
             if (a.relu)
 #pragma unroll
                 for (int i = 0; i < 128; ++i) acc[i] = relu_of(acc[i]);
-            // 128 bytes of each of the warp's rows at a time, 16-byte chunks swizzled
+            // 256 bytes of a row at a time: a lane leaves its row's in shared memory and
+            // one bulk copy takes them from there, while the next tile begins
             const int64_t n0 = (z.col + h) * 128ll;
-            const int per = a.out_bf16 ? 64 : 32;  // columns
+            const int es = a.out_bf16 ? 2 : 4, per = 256 / es;  // columns
 #pragma unroll
-            for (int c = 0; c < 128; c += 32) {
-                if (a.out_bf16 && (c & 32)) continue;
+            for (int c = 0; c < 128; c += 64) {
+                if (a.out_bf16 && c) break;
+                asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                 __syncwarp();
+                uint8_t* mine = stage + lane * kManyPitch;
+                if (a.out_bf16) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    uint4 v;
-                    if (a.out_bf16) {
-                        if (c & 32) continue;
-                        const int i = c + 8 * j < 128 ? c + 8 * j : 0;
-                        v = make_uint4(bf16x2_of(acc[i], acc[i + 1]), bf16x2_of(acc[i + 2], acc[i + 3]),
+                    for (int i = 0; i < 128; i += 8)
+                        *reinterpret_cast<uint4*>(mine + i * 2) =
+                            make_uint4(bf16x2_of(acc[i], acc[i + 1]), bf16x2_of(acc[i + 2], acc[i + 3]),
                                        bf16x2_of(acc[i + 4], acc[i + 5]), bf16x2_of(acc[i + 6], acc[i + 7]));
-                    } else {
-                        const int i = c + 4 * j;
-                        v = make_uint4(__float_as_uint(acc[i]), __float_as_uint(acc[i + 1]),
-                                       __float_as_uint(acc[i + 2]), __float_as_uint(acc[i + 3]));
-                    }
-                    *reinterpret_cast<uint4*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = v;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 64; i += 4)
+                        *reinterpret_cast<float4*>(mine + i * 4) =
+                            make_float4(acc[c + i], acc[c + i + 1], acc[c + i + 2], acc[c + i + 3]);
+                }
+                const int64_t n = n0 + c, left = min(static_cast<int64_t>(per), a.N - n);
+                if (left <= 0) break;
+                uint8_t* to = static_cast<uint8_t*>(a.out) + (static_cast<int64_t>(z.m0 + r0) * a.ldo + n) * es;
+                if (a.ovec16 && left * es % 16 == 0) {
+                    fence_proxy_async_smem();
+                    if (r0 + lane < z.rows)
+                        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(
+                                         to + lane * a.ldo * es),
+                                     "r"(smem_u32(mine)), "r"(static_cast<uint32_t>(left * es))
+                                     : "memory");
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    continue;
                 }
                 __syncwarp();
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int r = i * 4 + (lane >> 3), j = lane & 7;
-                    const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((j ^ (r & 7)) << 4));
-                    if (r0 + r >= z.rows) continue;
-                    const int64_t n = n0 + c + j * (per / 8), o = (z.m0 + r0 + r) * a.ldo + n;
-                    if (a.ovec16 && n + per / 8 <= a.N) {
-                        *reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.out) + o * (a.out_bf16 ? 2 : 4)) = v;
-                        continue;
-                    }
-                    const uint32_t e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        if (k >= per / 8 || n + k >= a.N) break;
+                const int rows = min(32, z.rows - r0);
+                for (int r = 0; r < rows; ++r)
+                    for (int k = lane; k < left; k += 32) {
                         if (a.out_bf16)
-                            static_cast<uint16_t*>(a.out)[o + k] = static_cast<uint16_t>(e[k / 2] >> (16 * (k & 1)));
+                            reinterpret_cast<uint16_t*>(to)[r * a.ldo + k] =
+                                reinterpret_cast<const uint16_t*>(stage + r * kManyPitch)[k];
                         else
-                            static_cast<uint32_t*>(a.out)[o + k] = e[k & 3];
+                            reinterpret_cast<uint32_t*>(to)[r * a.ldo + k] =
+                                reinterpret_cast<const uint32_t*>(stage + r * kManyPitch)[k];
                     }
-                }
             }
         }
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
 
     // the pair's MMAs, commits and remote arrivals are done
