@@ -348,9 +348,9 @@ __global__ void __launch_bounds__(kFewThreads, ALONE ? 1 : 2)
 
 // Many rows: a pair of SMs computes 256 rows x 256 columns of out, one CTA 128
 // rows of it.  Rows are the MMA's M (a thread has a row, so a block's two scales are
-// one factor for all of its columns), the weights are its N, half of them in each CTA's
-// shared memory, which halves what has to be read for them.  The pair is persistent
-// over tiles.
+// one factor for all of its columns), the weights are its N, half of them in each
+// CTA's shared memory, which halves what has to be read for them.  The pair is
+// persistent over tiles.
 //   warp 0      copies a block's rows and weights, 16 KB each, into the ring
 //   warp 1      issues the pair's MMAs (M = 256, N = 256, K = 32) in CTA 0, four a
 //               block, into one of two accumulators that fill tensor memory
@@ -358,41 +358,107 @@ __global__ void __launch_bounds__(kFewThreads, ALONE ? 1 : 2)
 //               the rest.  A block's accumulator comes back 32 columns at a time and
 //               factor * sum is added to 128 registers; at the tile's end these leave
 //               through shared memory in bulk copies of whole pieces of rows.
+// 4096 x 4096 x 14336, rows quantised before: 225 us, 2.1 PFLOP/s.  The MMAs alone take
+// 155; what bounds it is the warps that take the sums back, 830 cycles a block where
+// the MMAs take 512 (264 of them multiply-adds).  Accumulators of half the width, four
+// of them, wait twice as often: 258 us.
 // Every wait is bounded; a timeout sets the error word and ends all roles of both CTAs.
 constexpr int kManyThreads = 12 * 32, kManyStages = 4, kManyTile = 256;
 constexpr int kManyStage = 2 * kFp8Tile;                      // of one CTA
 constexpr int kManyPitch = 256 + 16;                          // a row's 256 bytes of out, in other banks than the next's
 constexpr int kManyOut = 8 * 32 * kManyPitch;
-constexpr int kManyBars = (2 * kManyStages + 4) * 8 + 16;
-constexpr int kManySmem = 1024 + kManyStages * kManyStage + kManyOut + kManyBars + (2 * AEM_MAX_EXPERTS + 2) * 4;
+constexpr int kManyScales = 2 * 256 * 16;                     // four blocks' scales of a thread's row, twice
 // Registers of a thread of warps 0-3 and of warps 4-11: together what the block is launched with.
 constexpr int kManyFewRegs = 40, kManyManyRegs = 232;
 static_assert(kManyFewRegs * 128 + kManyManyRegs * 256 <= 168 * kManyThreads, "register shares");
 constexpr int kBand = 16;  // row tiles that share the columns' weights before the next ones come
 
+// Shared memory of a CTA, in bytes from a 1024-byte boundary on.  Addresses are this
+// boundary's 32 bits and a constant: the sums leave few registers for anything else.
+constexpr int kManyOutAt = kManyStages * kManyStage, kManyScalesAt = kManyOutAt + kManyOut;
+constexpr int kManyFullAt = kManyScalesAt + kManyScales;             // [stages], used in CTA 0
+constexpr int kManyEmptyAt = kManyFullAt + 8 * kManyStages;          // [stages]
+constexpr int kManyDoneAt = kManyEmptyAt + 8 * kManyStages;          // [2]: an accumulator's sums are there
+constexpr int kManyFreeAt = kManyDoneAt + 16;                        // [2]: they have been read; used in CTA 0
+constexpr int kManySlotAt = kManyFreeAt + 16, kManyAbortAt = kManySlotAt + 4;
+constexpr int kManyRowsAt = kManySlotAt + 16, kManyTilesAt = kManyRowsAt + (AEM_MAX_EXPERTS + 1) * 4;
+constexpr int kManySmem = 1024 + kManyTilesAt + (AEM_MAX_EXPERTS + 1) * 4;
+
+__device__ __forceinline__ int lds_int(uint32_t at) {
+    int v;
+    asm volatile("ld.volatile.shared.s32 %0, [%1];" : "=r"(v) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ void sts_int(uint32_t at, int v) {
+    asm volatile("st.volatile.shared.s32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
+// Whether the phase with `parity` is complete: at once, or after a while.
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ uint32_t cluster_address(uint32_t at, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
+    return r;
+}
+// An arrival of the warp's first lane at a barrier of the cluster, without a branch.
+__device__ __forceinline__ void arrive_first_lane(uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .u32 l;\n\t"
+        "mov.u32 l, %%laneid;\n\t"
+        "setp.eq.u32 p, l, 0;\n\t"
+        "@p mbarrier.arrive.shared::cluster.b64 _, [%0];\n\t}" ::"r"(bar)
+        : "memory");
+}
 // Bounded wait of a whole warp that, on giving up, raises the abort flag of both CTAs.
-__device__ __forceinline__ bool pair_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t peer,
-                                          int* err) {
-    if (__all_sync(~0u, mbar_try_wait(bar, parity & 1))) return true;
-    const uint64_t t0 = globaltimer_ns();
-    while (true) {
-        if (__all_sync(~0u, mbar_try_wait(bar, parity & 1))) return true;
-        if (__any_sync(~0u, *abort_flag != 0)) return false;
-        if (__any_sync(~0u, globaltimer_ns() - t0 > 2000000000ull)) {
-            *abort_flag = 1;
-            st_remote_u32(const_cast<int*>(abort_flag), peer, 1u);
+// `done`: what a look at the barrier ahead of time saw (a look takes some 60 cycles).
+__device__ __forceinline__ bool pair_wait(uint32_t bar, uint32_t parity, bool done, uint32_t sb, int* err) {
+    if (__all_sync(~0u, done)) return true;
+    uint64_t t0 = 0;
+    for (int i = 0;; ++i) {  // the clock is read now and then: it is slow
+        if (__all_sync(~0u, bar_try(bar, parity))) return true;
+        if (i & 31) continue;
+        if (__any_sync(~0u, lds_int(sb + kManyAbortAt) != 0)) return false;
+        if (i == 0) continue;
+        const uint64_t t = globaltimer_ns();
+        if (t0 == 0) t0 = t;
+        if (__any_sync(~0u, t - t0 > 2000000000ull)) {
+            for (uint32_t r = 0; r < 2; ++r)
+                asm volatile("st.shared::cluster.u32 [%0], 1;" ::"r"(cluster_address(sb + kManyAbortAt, r)) : "memory");
             atomicOr(err, ERR_GEMM_TIMEOUT);
             return false;
         }
     }
 }
 
-// a0 += f * v0, a1 += f * v1
-__device__ __forceinline__ void fma2(float& a0, float& a1, float f, uint32_t v0, uint32_t v1) {
-    asm volatile("{\n.reg .b64 a, f, v;\nmov.b64 a, {%0, %1};\nmov.b64 f, {%2, %2};\nmov.b64 v, {%3, %4};\n"
-        "fma.rn.f32x2 a, f, v, a;\nmov.b64 {%0, %1}, a;\n}"
-        : "+f"(a0), "+f"(a1)
-        : "f"(f), "r"(v0), "r"(v1));
+// 32 columns: acc += f * d.  (Two columns an instruction: beside 128 single ones a
+// block, the MMAs take half as long again.)
+__device__ __forceinline__ void add_columns(float* acc, float f, const uint32_t (&d)[32]) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 2)
+        asm volatile("{\n.reg .b64 a, f, v;\nmov.b64 a, {%0, %1};\nmov.b64 f, {%2, %2};\nmov.b64 v, {%3, %4};\n"
+                     "fma.rn.f32x2 a, f, v, a;\nmov.b64 {%0, %1}, a;\n}"
+                     : "+f"(acc[i]), "+f"(acc[i + 1])
+                     : "f"(f), "r"(d[i]), "r"(d[i + 1]));
 }
 
 __device__ __forceinline__ uint32_t bf16x2_of(float lo, float hi) {
@@ -400,76 +466,57 @@ __device__ __forceinline__ uint32_t bf16x2_of(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Waits for the loads from tensor memory; what they bring is used behind it.
-__device__ __forceinline__ void wait_ld(uint32_t (&r)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
-                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
-                   "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
-                   "+r"(r[30])
-                 :
-                 : "memory");
-    asm volatile("" : "+r"(r[31])::"memory");
-}
-
 struct ManyTile {
     int64_t t0;    // first weight tile of the pair's columns
     int m0, rows;  // first row and number of rows
     int col;       // first 128-block of columns
 };
-__device__ __forceinline__ ManyTile many_tile(const Fp8Args& a, int t, const int* s_rows, const int* s_tiles) {
+__device__ __forceinline__ ManyTile many_tile(const Fp8Args& a, int t, uint32_t sb) {
     int lo = 0, hi = a.G;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (s_tiles[mid] <= t) lo = mid; else hi = mid;
+        if (lds_int(sb + kManyTilesAt + mid * 4) <= t) lo = mid; else hi = mid;
     }
-    const int nc = (a.nb + 1) / 2, r = t - s_tiles[lo], n = (s_tiles[lo + 1] - s_tiles[lo]) / nc;
+    const int first = lds_int(sb + kManyTilesAt + lo * 4), nc = (a.nb + 1) / 2;
+    const int r = t - first, n = (lds_int(sb + kManyTilesAt + lo * 4 + 4) - first) / nc;
     const int band = r / (kBand * nc), in = r - band * kBand * nc, high = min(kBand, n - band * kBand);
+    const int row = lds_int(sb + kManyRowsAt + lo * 4), end = lds_int(sb + kManyRowsAt + lo * 4 + 4);
     ManyTile o;
-    const int first = (band * kBand + in % high) * kManyTile;
     o.col = in / high * 2;
-    o.m0 = s_rows[lo] + first;
-    o.rows = min(kManyTile, s_rows[lo + 1] - o.m0);
+    o.m0 = row + (band * kBand + in % high) * kManyTile;
+    o.rows = min(kManyTile, end - o.m0);
     o.t0 = (a.group_rows ? lo : a.group) * a.group_tiles;
     return o;
 }
 
-template <bool TRANS>
+template <bool TRANS, bool BF16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads, 1)
     fp8_many_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
                     const __grid_constant__ Fp8Args a) {
     extern __shared__ uint8_t smem_raw[];
-    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                               ~static_cast<uintptr_t>(1023));
-    uint8_t* outs = ring + kManyStages * kManyStage;
-    uint64_t* full = reinterpret_cast<uint64_t*>(outs + kManyOut);  // used in CTA 0
-    uint64_t* empty = full + kManyStages;
-    uint64_t* dfull = empty + kManyStages;
-    uint64_t* dempty = dfull + 2;  // used in CTA 0
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dempty + 2);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    int* s_rows = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(full) + kManyBars);
-    int* s_tiles = s_rows + AEM_MAX_EXPERTS + 1;
-
+    const uint32_t sb = (smem_u32(smem_raw) + 1023) & ~1023u;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const uint32_t cta = cluster_rank(), peer = cta ^ 1u;
+    const uint32_t cta = cluster_rank();
     const int pair = static_cast<int>(blockIdx.x >> 1), pairs = static_cast<int>(gridDim.x >> 1);
     if (w == 0 && lane == 0) {
+        auto init = [&](uint32_t at, uint32_t count) {
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(sb + at), "r"(count) : "memory");
+        };
         for (int i = 0; i < kManyStages; ++i) {
-            mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 1);
+            init(kManyFullAt + 8 * i, 1);
+            init(kManyEmptyAt + 8 * i, 1);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&dfull[i], 1);
-            mbar_init(&dempty[i], 16);  // the warps of both CTAs that read it
+            init(kManyDoneAt + 8 * i, 1);
+            init(kManyFreeAt + 8 * i, 16);  // the warps of both CTAs that read it
         }
-        *abort_flag = 0;
+        sts_int(sb + kManyAbortAt, 0);
         fence_barrier_init();
         tma_prefetch_desc(&xmap);
         tma_prefetch_desc(&wmap);
-    } else if (w == 1) {
-        tmem_alloc_pair(tmem_slot, 512);  // the same warp of both CTAs
+    } else if (w == 1) {  // the same warp of both CTAs
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(sb + kManySlotAt)
+                     : "memory");
         tmem_relinquish_pair();
     } else if (w == 2) {
         // first rows and first tiles of the groups, 32 groups at a time
@@ -489,9 +536,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads, 1)
                 if (lane >= o) s += v;
             }
             if (i + lane < a.G) {
-                s_rows[i + lane] = lo;
-                s_tiles[i + lane] = before + s - n;
-                if (i + lane == a.G - 1) s_rows[a.G] = hi, s_tiles[a.G] = before + s;
+                sts_int(sb + kManyRowsAt + (i + lane) * 4, lo);
+                sts_int(sb + kManyTilesAt + (i + lane) * 4, before + s - n);
+                if (i + lane == a.G - 1) {
+                    sts_int(sb + kManyRowsAt + a.G * 4, hi);
+                    sts_int(sb + kManyTilesAt + a.G * 4, before + s);
+                }
             }
             before += __shfl_sync(~0u, s, 31);
         }
@@ -500,32 +550,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads, 1)
     __syncthreads();
     cluster_sync();  // both CTAs' barriers are there before any remote arrival
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
-    const int total = s_tiles[a.G];
+    const uint32_t tmem = static_cast<uint32_t>(lds_int(sb + kManySlotAt));
+    const int total = lds_int(sb + kManyTilesAt + a.G * 4);
 
     if (w < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kManyFewRegs));
         if (w == 0) {
             asm volatile("griddepcontrol.wait;" ::: "memory");  // the rows may be another kernel's
+            // both CTAs' bytes complete on CTA 0's barrier
+            const uint32_t full = cluster_address(sb + kManyFullAt, 0);
+            auto load = [&](uint32_t to, const CUtensorMap* map, uint32_t bar, int x, int y) {
+                asm volatile(
+                    "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+                    " [%0], [%1, {%3, %4}], [%2];" ::"r"(to),
+                    "l"(map), "r"(bar), "r"(x), "r"(y)
+                    : "memory");
+            };
             int st = 0;
             uint32_t phase = 0;
             int issued = 0;
             bool ok = true;
             for (int t = pair; ok && t < total; t += pairs) {
-                const ManyTile z = many_tile(a, t, s_rows, s_tiles);
+                const ManyTile z = many_tile(a, t, sb);
                 // an odd number of blocks: the last pair's second half takes the last block
                 // again, its results are not stored
-                const int64_t tile = z.t0 + min(z.col + static_cast<int>(cta), a.nb - 1) * a.out_step;
-                const int row = z.m0 + static_cast<int>(cta) * 128;
-                for (int u = 0; u < a.kb; ++u) {
-                    if (!(ok = pair_wait(&empty[st], phase ^ 1, abort_flag, peer, a.err))) break;
+                int tile = static_cast<int>((z.t0 + min(z.col + static_cast<int>(cta), a.nb - 1) * a.out_step) * 128);
+                const int row = z.m0 + static_cast<int>(cta) * 128, step = static_cast<int>(a.sum_step * 128);
+                for (int u = 0; u < a.kb; ++u, tile += step) {
+                    if (!(ok = pair_wait(sb + kManyEmptyAt + 8 * st, phase ^ 1, false, sb, a.err))) break;
                     if (lane == 0) {
-                        uint8_t* to = ring + st * kManyStage;
-                        // both CTAs' bytes complete on CTA 0's barrier
-                        if (cta == 0) mbar_arrive_expect_tx(&full[st], 2 * kManyStage);
-                        tma_load_2d_pair(to, &xmap, &full[st], 0, u * 128, row);
-                        tma_load_2d_pair(to + kFp8Tile, &wmap, &full[st], 0, 0,
-                                         static_cast<int>((tile + u * a.sum_step) * 128));
+                        const uint32_t to = sb + st * kManyStage;
+                        if (cta == 0)
+                            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(
+                                             sb + kManyFullAt + 8 * st),
+                                         "r"(2 * kManyStage)
+                                         : "memory");
+                        load(to, &xmap, full + 8 * st, u * 128, row);
+                        load(to + kFp8Tile, &wmap, full + 8 * st, 0, tile);
                     }
                     ++issued;
                     if (++st == kManyStages) st = 0, phase ^= 1;
@@ -533,142 +594,164 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads, 1)
             }
             if (!ok && cta == 0 && lane == 0)  // a failed call leaves no copy in flight behind (bounded as well)
                 for (int i = max(0, issued - kManyStages); i < issued; ++i)
-                    for (int n = 0; n < 1 << 14 && !mbar_try_wait(&full[i % kManyStages], i / kManyStages & 1); ++n) {
+                    for (int n = 0; n < 1 << 14 && !bar_try(sb + kManyFullAt + 8 * (i % kManyStages),
+                                                            i / kManyStages & 1); ++n) {
                     }
         } else if (w == 1 && cta == 0) {
             constexpr uint32_t idesc = idesc_e4m3_f32(256, 256, false, TRANS);
+            auto commit = [&](uint32_t bar) {  // to the barrier's place in both CTAs
+                asm volatile(
+                    "{\n\t.reg .pred e;\n\t"
+                    "elect.sync _|e, 0xffffffff;\n\t"
+                    "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+                    " [%0], %1;\n\t}" ::"r"(bar),
+                    "h"(static_cast<uint16_t>(3))
+                    : "memory");
+            };
             int st = 0;
-            uint32_t phase = 0, it = 0;
-            bool ok = true;
+            uint32_t phase = 0, used = 0;  // used: bit b: parity of the uses of accumulator b
+            bool ok = true, seen = false;  // seen: the next block's operands
             for (int t = pair; ok && t < total; t += pairs)
-                for (int u = 0; u < a.kb; ++u, ++it) {
-                    const uint32_t b = it & 1;
-                    if (!(ok = pair_wait(&full[st], phase, abort_flag, peer, a.err) &&
-                               pair_wait(&dempty[b], (it >> 1) + 1, abort_flag, peer, a.err)))
+                for (int u = 0; u < a.kb; ++u) {
+                    const uint32_t b = u & 1, parity = (used >> b & 1) ^ 1;
+                    const bool free = bar_test(sb + kManyFreeAt + 8 * b, parity);
+                    if (!(ok = pair_wait(sb + kManyFullAt + 8 * st, phase, seen, sb, a.err) &&
+                               pair_wait(sb + kManyFreeAt + 8 * b, parity, free, sb, a.err)))
                         break;
+                    used ^= 1u << b;
                     tc_fence_after();
-                    const uint64_t ad = smem_desc_sw128(smem_u32(ring + st * kManyStage));
-                    const uint64_t bd = smem_desc_sw128(smem_u32(ring + st * kManyStage + kFp8Tile));
+                    const uint64_t ad = smem_desc_sw128(sb + st * kManyStage);
+                    const uint64_t bd = smem_desc_sw128(sb + st * kManyStage + kFp8Tile);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         tc_mma_f8_pair_elect(tmem + b * 256, ad + i * kStep32<false>, bd + i * kStep32<TRANS>, idesc,
                                              i ? 1u : 0u);
-                    tc_commit_pair_elect(&empty[st], 0x3);
-                    tc_commit_pair_elect(&dfull[b], 0x3);
+                    commit(sb + kManyDoneAt + 8 * b);
+                    commit(sb + kManyEmptyAt + 8 * st);
                     if (++st == kManyStages) st = 0, phase ^= 1;
+                    seen = bar_test(sb + kManyFullAt + 8 * st, phase);
                 }
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyManyRegs));
         asm volatile("griddepcontrol.wait;" ::: "memory");
-        const int h = (w - 4) >> 2, q = w & 3;
-        const uint32_t at = tmem + (static_cast<uint32_t>(32 * q) << 16) + h * 128;
-        uint8_t* stage = outs + (w - 4) * 32 * kManyPitch;
-        uint32_t it = 0;
-        bool ok = true;
+        const uint32_t mine = sb + kManyScalesAt + (threadIdx.x - 128) * 16;
+        const uint32_t at = tmem + (static_cast<uint32_t>(32 * (w & 3)) << 16) + ((w - 4) >> 2) * 128;
+        const uint32_t free_at = cluster_address(sb + kManyFreeAt, 0);
+        uint32_t used = 0;
+        bool ok = true, seen = false;  // seen: the next block's sums are there
+#pragma unroll 1
         for (int t = pair; ok && t < total; t += pairs) {
-            const ManyTile z = many_tile(a, t, s_rows, s_tiles);
-            const int r0 = static_cast<int>(cta) * 128 + q * 32;  // the warp's first row in the tile
-            const int64_t row = min(static_cast<int64_t>(z.m0) + r0 + lane, a.M - 1);
-            const float* xs = a.xs + row * a.lds;
-            const float* ws = a.ws + z.t0 + min(z.col + h, a.nb - 1) * a.out_step;
             float acc[128];
 #pragma unroll
             for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
-            float held = 0.0f;  // the weight scales of 32 blocks, one a lane
-            // the row's scales, four blocks at a time, the next four on their way
-            auto scales = [&](int u) {
-                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (u + 4 <= a.kb) return *reinterpret_cast<const float4*>(xs + u);
-                if (u < a.kb) v.x = xs[u];
-                if (u + 1 < a.kb) v.y = xs[u + 1];
-                if (u + 2 < a.kb) v.z = xs[u + 2];
-                return v;
-            };
-            float4 sx, next = scales(0);
-            for (int u = 0; u < a.kb; ++u, ++it) {
-                if ((u & 31) == 0) held = u + lane < a.kb ? ws[(u + lane) * a.sum_step] : 0.0f;
-                if ((u & 3) == 0) {
-                    sx = next;
-                    next = scales(u + 4);
-                }
-                const float f = sx.x * __shfl_sync(~0u, held, u & 31);
-                sx = make_float4(sx.y, sx.z, sx.w, 0.0f);
-                const uint32_t b = it & 1;
-                if (!(ok = pair_wait(&dfull[b], it >> 1, abort_flag, peer, a.err))) break;
-                tc_fence_after();
-                uint32_t d[2][32];  // one on its way while the other is added
-                tc_ld_32x32b_x32(at + b * 256, d[0]);
+            {
+                const ManyTile z = many_tile(a, t, sb);
+                // the thread's row; rows behind the tile's compute something that nobody stores
+                const int64_t row = min(static_cast<int64_t>(z.m0) + static_cast<int>(cta) * 128 + (w & 3) * 32 + lane, a.M - 1);
+                const float* xs = a.xs + row * a.lds;
+                const float* ws = a.ws + z.t0 + min(z.col + ((w - 4) >> 2), a.nb - 1) * a.out_step;
+                // the row's scales, four blocks at a time, the next four on their way
+                auto fetch = [&](int u) {
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 16;\ncp.async.commit_group;" ::"r"(
+                                     mine + (u & 4) * 1024),
+                                 "l"(xs + u)
+                                 : "memory");
+                };
+                fetch(0);
+                float held = 0.0f;  // the weight scales of 32 blocks, one a lane
+                // block u in accumulator b
+                auto block = [&](int u, uint32_t b) {
+                    ok &= pair_wait(sb + kManyDoneAt + 8 * b, used >> b & 1, seen, sb, a.err);
+                    used ^= 1u << b;
+                    tc_fence_after();
+                    float f;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    wait_ld(d[c & 1]);
-                    if (c < 3) {
-                        tc_ld_32x32b_x32(at + b * 256 + (c + 1) * 32, d[(c + 1) & 1]);
-                    } else {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) {
-                            if (cta == 0)
-                                mbar_arrive(&dempty[b]);
-                            else
-                                mbar_arrive_remote(&dempty[b], 0);
+                    for (int c = 0; c < 128; c += 32) {
+                        uint32_t d[32];
+                        tc_ld_32x32b_x32(at + b * 256 + c, d);
+                        if (c == 0) {
+                            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(mine + (u & 4) * 1024 + (u & 3) * 4) : "memory");
+                            f *= __shfl_sync(~0u, held, u & 31);
                         }
+                        tc_wait_ld();
+                        if (c == 96) {
+                            tc_fence_before();
+                            __syncwarp();
+                            arrive_first_lane(free_at + b * 8);
+                            seen = bar_test(sb + kManyDoneAt + 8 * (b ^ 1), used >> (b ^ 1) & 1);
+                        }
+                        add_columns(acc + c, f, d);
                     }
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2)
-                        fma2(acc[c * 32 + i], acc[c * 32 + i + 1], f, d[c & 1][i], d[c & 1][i + 1]);
+                };
+                int u = 0;
+                auto next_four = [&]() {
+                    if ((u & 31) == 0) held = ws[min(u + lane, a.kb - 1) * a.sum_step];
+                    asm volatile("cp.async.wait_group 0;" ::: "memory");
+                    if (u + 4 < a.kb) fetch(u + 4);
+                };
+                // four blocks a round, so that few branches are left between their sums
+#pragma unroll 1
+                for (; u + 4 <= a.kb; u += 4) {
+                    next_four();
+                    block(u, 0);
+                    block(u + 1, 1);
+                    block(u + 2, 0);
+                    block(u + 3, 1);
                 }
+                if (u < a.kb) {
+                    next_four();
+#pragma unroll 1
+                    for (; u < a.kb; ++u) block(u, u & 1);
+                }
+                if (a.kb & 1) seen = false;  // the next tile begins with accumulator 0 again
             }
-            if (!ok || r0 >= z.rows) continue;
-            if (a.relu)
+            const ManyTile z = many_tile(a, t, sb);  // (kept from before, it would cost the sums registers)
+            const int r = static_cast<int>(cta) * 128 + (w & 3) * 32 + lane;
+            const int64_t n = (z.col + ((w - 4) >> 2)) * 128ll, left = min(static_cast<int64_t>(128), a.N - n);
+            if (!ok || left <= 0) continue;
+            constexpr int ES = BF16 ? 2 : 4, PER = 256 / ES;  // columns of a piece
+            uint8_t* to = static_cast<uint8_t*>(a.out) + ((z.m0 + r) * a.ldo + n) * ES;
+            auto column = [&](int i) { return a.relu ? relu_of(acc[i]) : acc[i]; };
+            if (!(a.ovec16 && left * ES % 16 == 0)) {
+                if (r < z.rows)
 #pragma unroll
-                for (int i = 0; i < 128; ++i) acc[i] = relu_of(acc[i]);
+                    for (int i = 0; i < 128; ++i)
+                        if (i < left) {
+                            if constexpr (BF16)
+                                reinterpret_cast<__nv_bfloat16*>(to)[i] = __float2bfloat16_rn(column(i));
+                            else
+                                reinterpret_cast<float*>(to)[i] = column(i);
+                        }
+                continue;
+            }
             // 256 bytes of a row at a time: a lane leaves its row's in shared memory and
             // one bulk copy takes them from there, while the next tile begins
-            const int64_t n0 = (z.col + h) * 128ll;
-            const int es = a.out_bf16 ? 2 : 4, per = 256 / es;  // columns
+            const uint32_t piece = sb + kManyOutAt + ((w - 4) * 32 + lane) * kManyPitch;
 #pragma unroll
-            for (int c = 0; c < 128; c += 64) {
-                if (a.out_bf16 && c) break;
+            for (int c = 0; c < 128; c += PER) {
                 asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                __syncwarp();
-                uint8_t* mine = stage + lane * kManyPitch;
-                if (a.out_bf16) {
 #pragma unroll
-                    for (int i = 0; i < 128; i += 8)
-                        *reinterpret_cast<uint4*>(mine + i * 2) =
-                            make_uint4(bf16x2_of(acc[i], acc[i + 1]), bf16x2_of(acc[i + 2], acc[i + 3]),
-                                       bf16x2_of(acc[i + 4], acc[i + 5]), bf16x2_of(acc[i + 6], acc[i + 7]));
-                } else {
+                for (int i = 0; i < 16; ++i) {
+                    uint32_t v[4];
 #pragma unroll
-                    for (int i = 0; i < 64; i += 4)
-                        *reinterpret_cast<float4*>(mine + i * 4) =
-                            make_float4(acc[c + i], acc[c + i + 1], acc[c + i + 2], acc[c + i + 3]);
-                }
-                const int64_t n = n0 + c, left = min(static_cast<int64_t>(per), a.N - n);
-                if (left <= 0) break;
-                uint8_t* to = static_cast<uint8_t*>(a.out) + (static_cast<int64_t>(z.m0 + r0) * a.ldo + n) * es;
-                if (a.ovec16 && left * es % 16 == 0) {
-                    fence_proxy_async_smem();
-                    if (r0 + lane < z.rows)
-                        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(
-                                         to + lane * a.ldo * es),
-                                     "r"(smem_u32(mine)), "r"(static_cast<uint32_t>(left * es))
-                                     : "memory");
-                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-                    continue;
-                }
-                __syncwarp();
-                const int rows = min(32, z.rows - r0);
-                for (int r = 0; r < rows; ++r)
-                    for (int k = lane; k < left; k += 32) {
-                        if (a.out_bf16)
-                            reinterpret_cast<uint16_t*>(to)[r * a.ldo + k] =
-                                reinterpret_cast<const uint16_t*>(stage + r * kManyPitch)[k];
+                    for (int k = 0; k < 4; ++k) {
+                        if constexpr (BF16)
+                            v[k] = bf16x2_of(column(8 * i + 2 * k), column(8 * i + 2 * k + 1));
                         else
-                            reinterpret_cast<uint32_t*>(to)[r * a.ldo + k] =
-                                reinterpret_cast<const uint32_t*>(stage + r * kManyPitch)[k];
+                            v[k] = __float_as_uint(column(c + 4 * i + k));
                     }
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(piece + 16 * i), "r"(v[0]), "r"(v[1]),
+                                 "r"(v[2]), "r"(v[3])
+                                 : "memory");
+                }
+                fence_proxy_async_smem();
+                const int64_t bytes = min(static_cast<int64_t>(256), (left - c) * ES);
+                if (r < z.rows && bytes > 0)
+                    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to + c * ES),
+                                 "r"(piece), "r"(static_cast<uint32_t>(bytes))
+                                 : "memory");
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
         }
         asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -763,7 +846,7 @@ int max_pairs(int device) {
     cfg.gridDim = dim3(2 * 512);
     cfg.blockDim = dim3(kManyThreads);
     cfg.dynamicSmemBytes = kManySmem;
-    if (cudaOccupancyMaxActiveClusters(&n, fp8_many_kernel<false>, &cfg) != cudaSuccess || n < 1) {
+    if (cudaOccupancyMaxActiveClusters(&n, fp8_many_kernel<false, true>, &cfg) != cudaSuccess || n < 1) {
         cudaGetLastError();
         n = kSMs / 2;
     }
@@ -780,7 +863,8 @@ aem_status launch_many(const Fp8Args& a, const Fp8Weight* w, const void* q, int6
     const int device = current_device();
     const uint64_t bit = 1ull << (device & 63);
     if (!(ready.load(std::memory_order_relaxed) & bit)) {
-        for (auto kern : {fp8_many_kernel<false>, fp8_many_kernel<true>}) {
+        for (auto kern : {fp8_many_kernel<false, false>, fp8_many_kernel<false, true>, fp8_many_kernel<true, false>,
+                          fp8_many_kernel<true, true>}) {
             AEM_TRY_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kManySmem));
             cudaFuncAttributes f;
             AEM_TRY_CUDA(cudaFuncGetAttributes(&f, kern));
@@ -801,7 +885,9 @@ aem_status launch_many(const Fp8Args& a, const Fp8Weight* w, const void* q, int6
     at.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &at;
     cfg.numAttrs = dependent ? 1 : 0;
-    AEM_TRY_CUDA(cudaLaunchKernelEx(&cfg, transposed ? fp8_many_kernel<true> : fp8_many_kernel<false>, xmap, wmap, a));
+    auto kern = transposed ? (a.out_bf16 ? fp8_many_kernel<true, true> : fp8_many_kernel<true, false>)
+                           : (a.out_bf16 ? fp8_many_kernel<false, true> : fp8_many_kernel<false, false>);
+    AEM_TRY_CUDA(cudaLaunchKernelEx(&cfg, kern, xmap, wmap, a));
     count_launches(1);
     return AEM_OK;
 }
