@@ -36,8 +36,14 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(v) : "f"(hi), "f"(lo));
     return v;
 }
+// The same for one, divided by 448: exact where nothing is subnormal.
 __device__ __forceinline__ float block_scale(uint32_t amax_bits) {
     const float a = __uint_as_float(amax_bits);  // a NaN's bits are above infinity's
+    if (a >= 0x1p-90f && a <= 0x1.fffffep+127f) {
+        constexpr float r = 1.0f / 448.0f;  // rounded
+        const float q = a * r;
+        return fmaf(fmaf(-448.0f, q, a), r, q);
+    }
     const float s = __fdiv_rn(a, 448.0f);
     return s < 0x1p-126f ? 0x1p-126f : s;
 }
@@ -96,41 +102,51 @@ struct Eight {
     }
 };
 
-// 16 lanes share a block, 8 elements each; a half warp takes kHeld blocks that
-// follow one another, all of their loads in flight at once.
-constexpr int kHeld = 4;
+// 8 lanes share a block, twice 8 elements each, 64 apart, so that a load's lanes lie
+// side by side; they take kHeld blocks that follow one another, all of their loads
+// in flight at once.  The divisions of a block's scale are shared by 16 elements (16
+// lanes of 8 each: 98304 x 2048 bf16 in 147 us).
+template <typename XT>
+constexpr int kHeld = sizeof(XT) == 2 ? 2 : 1;
 template <typename XT, bool VEC>
 __global__ void __launch_bounds__(kThreads)
     quantize_fp8_kernel(const XT* __restrict__ x, int64_t ldx, int64_t blocks, int64_t K, int64_t KB,
                         uint8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale, int64_t lds) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int sub = threadIdx.x & 15;
-    const int64_t first = (blockIdx.x * static_cast<int64_t>(kThreads / 16) + (threadIdx.x >> 4)) * kHeld;
-    int64_t m = first / KB;
+    constexpr int HELD = kHeld<XT>;
+    const int sub = threadIdx.x & 7;
+    const int64_t first = (blockIdx.x * static_cast<int64_t>(kThreads / 8) + (threadIdx.x >> 3)) * HELD;
+    // (a 32-bit division where it will do)
+    int64_t m = first < (1ll << 31) && KB < (1ll << 31) ? static_cast<uint32_t>(first) / static_cast<uint32_t>(KB) : first / KB;
     int64_t b = first - m * KB;
-    int64_t row[kHeld], kb[kHeld];
-    Eight<XT> v[kHeld];
+    int64_t row[HELD], kb[HELD];
+    Eight<XT> v[HELD][2];
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
+    for (int i = 0; i < HELD; ++i) {
         row[i] = m;
         kb[i] = b;
-        v[i].template load<VEC>(x + m * ldx, b * 128 + sub * 8, first + i < blocks ? K : 0);
+        const int64_t end = first + i < blocks ? K : 0;
+        v[i][0].template load<VEC>(x + m * ldx, b * 128 + sub * 8, end);
+        v[i][1].template load<VEC>(x + m * ldx, b * 128 + 64 + sub * 8, end);
         if (++b == KB) b = 0, ++m;
     }
+    const int64_t end = (K + 15) / 16 * 16;
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-        uint32_t top = v[i].top();
+    for (int i = 0; i < HELD; ++i) {
+        uint32_t top = max(v[i][0].top(), v[i][1].top());
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
+        for (int o = 4; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
         if (first + i >= blocks) continue;
         const float s = block_scale(top);
-        float f[8];
-        uint32_t o[2];
+        float f[16];
+        uint32_t o[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = v[i].get(j);
+        for (int j = 0; j < 16; ++j) f[j] = v[i][j / 8].get(j % 8);
         to_e4m3(f, s, o);
         const int64_t k = kb[i] * 128 + sub * 8;
-        if (k < (K + 15) / 16 * 16) *reinterpret_cast<uint2*>(q + row[i] * ldq + k) = make_uint2(o[0], o[1]);
+        uint8_t* to = q + row[i] * ldq + k;
+        if (k < end) *reinterpret_cast<uint2*>(to) = make_uint2(o[0], o[1]);
+        if (k + 64 < end) *reinterpret_cast<uint2*>(to + 64) = make_uint2(o[2], o[3]);
         if (sub == 0) scale[row[i] * lds + kb[i]] = s;
     }
 }
@@ -138,7 +154,7 @@ __global__ void __launch_bounds__(kThreads)
 // A block of 128 x 128 weights per thread block, in registers between its maximum
 // and its quotients: a lane has 16 bytes of a row at a time.
 template <typename WT, bool VEC>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, sizeof(WT) == 4 ? 3 : 4)
     quantize_fp8_weight_kernel(const WT* __restrict__ w, int64_t K, int64_t N, int64_t KB, int64_t NB,
                                uint8_t* __restrict__ q, float* __restrict__ scale) {
     constexpr int CL = 16 / sizeof(WT), LANES = 128 / CL, STEP = kThreads / LANES, R = 128 / STEP;
@@ -281,7 +297,7 @@ aem_status pack_fp8(const uint8_t* q, const float* scale, int64_t G, int64_t K, 
 
 aem_status launch_quantize_fp8(const char* what, const void* x, aem_dtype dtype, int64_t ldx, int64_t M, int64_t K,
                                uint8_t* q, int64_t ldq, float* scale, int64_t lds, cudaStream_t s) {
-    const int64_t KB = (K + 127) / 128, blocks = M * KB, per = kThreads / 16 * kHeld;
+    const int64_t KB = (K + 127) / 128, blocks = M * KB, per = kThreads / 8 * (dtype == AEM_F32 ? kHeld<float> : kHeld<__nv_bfloat16>);
     AEM_REQUIRE((blocks + per - 1) / per < (1ll << 31), "%s: M=%lld out of range", what, (long long)M);
     const auto grid = static_cast<unsigned>((blocks + per - 1) / per);
     const int es = dtype == AEM_F32 ? 4 : 2;

@@ -14,14 +14,20 @@
 // on their error; wherever two keys that decide the order (neighbours among the
 // k + 1 largest, the last group kept and the first dropped) are nearer than their
 // bounds, the warp chooses again with keys in 64 bits.  With normally distributed
-// logits that is a row in some hundred.  Logits themselves need no bound.
+// logits that is a row in some hundred, and costs 16384 rows of 256 about 5 us.
+// Logits themselves need no bound.
 //
 // A row lies across LANES lanes, 8 neighbouring experts a lane, so a lane's order
-// is the experts' and up to 32 rows share a warp.  What has to be moved is T*E
-// logits and 8 T*k bytes.
+// is the experts' and up to 32 rows share a warp.  A lane sorts its experts once
+// and leaves them in shared memory; a choice is then the maximum of the lanes'
+// first ones, and the lane that had it moves on to its next (looking through all 8
+// again for every choice took 29 us where this takes 24: 16384 rows of 256, top-8).
+// Groups of whole lanes take their two largest from the sorted lists; others are
+// read through shared memory.  What has to be moved is T*E logits and 8 T*k bytes.
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -44,7 +50,8 @@ struct RouteArgs {
     float* weights;
     int64_t ld, T, ldi, ldg, ldo;
     float scale;
-    int E, k, groups, top_groups, group_top, size, size_inv;  // size: experts of a group
+    int E, k, groups, top_groups, group_top, size;  // size: experts of a group
+    int size_inv, k_inv;                            // n * inv >> 16 == n / (size, k) for n < 256
     int sigmoid, renorm, vec, ovec;
     int* err;
 };
@@ -151,121 +158,160 @@ __device__ __forceinline__ void scores(const float (&x)[kV], bool sigmoid, F (&s
     for (int i = 0; i < kV; ++i) s[i] *= r;
 }
 
+// A warp's rows.
 struct RouteShared {
-    double by[kRouteWarps][256];     // a warp's rows: values of the experts (or float)
-    double value[kRouteWarps][256];  // of the groups
-    int32_t ids[kRouteWarps][256];   // [row][k]: LANES * 8 >= k
-    float v[kRouteWarps][256];
+    unsigned long long list[kRouteWarps][kV][32];  // the lanes' experts, sorted: ranks and indices
+    float take[kRouteWarps][256];                  // what becomes of a chosen expert
+    int32_t ids[kRouteWarps][256];                 // [row][k]: LANES * 8 >= k
+    double value[kRouteWarps][32];                 // of groups of whole lanes, chosen exactly
+};
+// Groups that are not whole lanes (or not a power of two of them): values of the
+// experts and of the groups.
+struct GroupShared {
+    double by[kRouteWarps][256], value[kRouteWarps][256];
 };
 
-// Chooses from keys (and, for groups, from `by`) and leaves ids and `take`n
-// values in shared memory.  CERT: returns whether a decision was nearer than the
-// keys' slack.
-template <int LANES, typename F, bool CERT>
-__device__ __forceinline__ bool choose(const RouteArgs& a, const F (&key)[kV], const F (&by)[kV], const F (&s)[kV],
-                                       const float (&take)[kV], RouteShared& sh) {
+// A rank and its expert's place in the lane; larger ones come first.
+__device__ __forceinline__ unsigned long long entry_of(uint32_t rank, int i) {
+    return static_cast<unsigned long long>(rank) << 32 | static_cast<uint32_t>(7 - i);
+}
+template <typename T>
+__device__ __forceinline__ void order2(T& a, T& b) {
+    const T hi = max(a, b), lo = min(a, b);
+    a = hi, b = lo;
+}
+// 8 values in falling order: 19 exchanges.
+template <typename T>
+__device__ __forceinline__ void sort8(T (&v)[8]) {
+    order2(v[0], v[1]), order2(v[2], v[3]), order2(v[4], v[5]), order2(v[6], v[7]);
+    order2(v[0], v[2]), order2(v[1], v[3]), order2(v[4], v[6]), order2(v[5], v[7]);
+    order2(v[1], v[2]), order2(v[5], v[6]), order2(v[0], v[4]), order2(v[3], v[7]);
+    order2(v[1], v[5]), order2(v[2], v[6]);
+    order2(v[1], v[4]), order2(v[3], v[6]);
+    order2(v[2], v[4]), order2(v[3], v[5]);
+    order2(v[3], v[4]);
+}
+
+// Which of the row's groups stay, for any size: keys of the others become -inf.
+// Returns whether the last that stayed and the first that did not are nearer than
+// `e`, the slack of the values.
+template <int LANES, typename F>
+__device__ __forceinline__ bool keep_groups(const RouteArgs& a, F (&key)[kV], const F (&by)[kV], float e, void* vals,
+                                            void* values) {
     using U = typename Rank<F>::type;
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, sub = lane % LANES, row = lane / LANES;
-    bool near = false;
-    U u[kV];
+    const int lane = threadIdx.x & 31, sub = lane % LANES, row = lane / LANES;
+    F* val = static_cast<F*>(vals) + row * LANES * kV;
+    F* gv = static_cast<F*>(values) + row * a.groups;
+    __syncwarp();
 #pragma unroll
-    for (int i = 0; i < kV; ++i) u[i] = rank_of(key[i]);
-    if (a.groups > 1) {
-        F* val = reinterpret_cast<F*>(sh.by[w]) + row * LANES * kV;
-        F* gv = reinterpret_cast<F*>(sh.value[w]) + row * LANES * kV;
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < kV; ++i) val[sub * kV + i] = by[i];
-        __syncwarp();
-        for (int g = sub; g < a.groups; g += LANES) {
-            U first = 0, second = 0;
-            for (int i = 0, at = g % a.size; i < a.size; ++i) {  // lanes start apart: other banks
-                const U r = rank_of(val[g * a.size + at]);
-                second = max(second, min(first, r));
-                first = max(first, r);
-                if (++at == a.size) at = 0;
-            }
-            F t = value_of(first);
-            if (a.group_top == 2 && second) t += value_of(second);
-            gv[g] = t;
+    for (int i = 0; i < kV; ++i) val[sub * kV + i] = by[i];
+    __syncwarp();
+    for (int g = sub; g < a.groups; g += LANES) {
+        U first = 0, second = 0;
+        for (int i = 0, at = g % a.size; i < a.size; ++i) {  // lanes start apart: other banks
+            const U r = rank_of(val[g * a.size + at]);
+            second = max(second, min(first, r));
+            first = max(first, r);
+            if (++at == a.size) at = 0;
         }
-        __syncwarp();
-        uint32_t kept[8] = {};  // a bit per group
-        F least = INFINITY, most = -INFINITY;
-        for (int g = sub; g < a.groups; g += LANES) {
-            const U mine = rank_of(gv[g]);
-            int before = 0;
-            for (int h = 0; h < a.groups; ++h) {
-                const U other = rank_of(gv[h]);
-                before += other > mine || (other == mine && h < g);
-            }
-            if (before < a.top_groups) {
-                least = gv[g] < least ? gv[g] : least;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) kept[i] |= g >> 5 == i ? 1u << (g & 31) : 0u;
-            } else {
-                most = gv[g] > most ? gv[g] : most;
-            }
+        F t = value_of(first);
+        if (a.group_top == 2 && second) t += value_of(second);
+        gv[g] = t;
+    }
+    __syncwarp();
+    uint32_t kept[8] = {};  // a bit per group
+    F least = INFINITY, most = -INFINITY;
+    for (int g = sub; g < a.groups; g += LANES) {
+        const U mine = rank_of(gv[g]);
+        int before = 0;
+        for (int h = 0; h < a.groups; ++h) {
+            const U other = rank_of(gv[h]);
+            before += other > mine || (other == mine && h < g);
         }
-        if constexpr (CERT) {
-            least = -seg_max<LANES>(-least);
-            most = seg_max<LANES>(most);
-            // a value is the sum of one or two keys of at most these sizes
-            float top = 0.0f, largest = 0.0f;
+        if (before < a.top_groups) {
+            least = gv[g] < least ? gv[g] : least;
 #pragma unroll
-            for (int i = 0; i < kV; ++i) {
-                top = fmaxf(top, s[i]);
-                if (by[i] != -INFINITY) largest = fmaxf(largest, fabsf(by[i]));
-            }
-            top = seg_max<LANES>(top);
-            largest = seg_max<LANES>(largest);
-            const float e = 4.0f * slack(top, largest) + 0x1p-22f * largest;
-            near |= most > -INFINITY && !(least - most > e);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i * 32 < a.groups) kept[i] = seg_reduce<LANES>(kept[i], [](uint32_t p, uint32_t q) { return p | q; });
-#pragma unroll
-        for (int i = 0; i < kV; ++i) {
-            const int g = (sub * kV + i) * a.size_inv >> 16;
-            uint32_t bits = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) bits = g >> 5 == j ? kept[j] : bits;
-            if (!(bits >> (g & 31) & 1)) u[i] = 0;
+            for (int i = 0; i < 8; ++i) kept[i] |= g >> 5 == i ? 1u << (g & 31) : 0u;
+        } else {
+            most = gv[g] > most ? gv[g] : most;
         }
     }
-    U best = 0;
+    bool near = false;
+    if constexpr (sizeof(F) == 4) {
+        least = -seg_max<LANES>(-least);
+        most = seg_max<LANES>(most);
+        near = e > 0.0f && most > -INFINITY && !(least - most > e);
+    }
 #pragma unroll
-    for (int i = 0; i < kV; ++i) best = max(best, u[i]);
+    for (int i = 0; i < 8; ++i)
+        if (i * 32 < a.groups) kept[i] = seg_reduce<LANES>(kept[i], [](uint32_t p, uint32_t q) { return p | q; });
+#pragma unroll
+    for (int i = 0; i < kV; ++i) {
+        const int g = (sub * kV + i) * a.size_inv >> 16;
+        uint32_t bits = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) bits = g >> 5 == j ? kept[j] : bits;
+        if (!(bits >> (g & 31) & 1)) key[i] = -INFINITY;
+    }
+    return near;
+}
+
+// The same for groups of whole lanes, `span` (a power of two) of them, from the
+// lane's two largest values: returns whether the lane's group stays.
+template <int LANES, typename F>
+__device__ __forceinline__ bool keep_lanes(const RouteArgs& a, int span, F first, F second, float e, bool& near) {
+    using U = typename Rank<F>::type;
+    const int lane = threadIdx.x & 31, base = lane & ~(LANES - 1), mine = lane & ~(span - 1);
+    U p = rank_of(first), q = a.group_top == 2 ? rank_of(second) : 0;
+    for (int o = 1; o < span; o <<= 1) {
+        const U r = __shfl_xor_sync(~0u, p, o), t = __shfl_xor_sync(~0u, q, o);
+        q = max(max(q, t), min(p, r));
+        p = max(p, r);
+    }
+    F v = value_of(p);
+    if (a.group_top == 2 && q) v += value_of(q);
+    const U rank = rank_of(v);
+    int before = 0;
+    for (int g = 0; g < a.groups; ++g) {
+        const int at = base + g * span;
+        const U other = __shfl_sync(~0u, rank, at);
+        before += other > rank || (other == rank && at < mine);
+    }
+    const bool stays = before < a.top_groups && lane - base < a.groups * span;
+    if constexpr (sizeof(F) == 4) {
+        const bool real = lane - base < a.groups * span;
+        const float least = -seg_max<LANES>(stays && v == v ? -v : -INFINITY);
+        const float most = seg_max<LANES>(real && !stays ? v : -INFINITY);
+        near |= e > 0.0f && most > -INFINITY && !(least - most > e);
+    }
+    return stays;
+}
+
+// The k largest of the lanes' sorted lists in shared memory, head of its list `best`
+// and `on` whether the lane takes part; their ids and, with a bound on the keys'
+// errors (CERT), whether a decision was nearer than that.
+template <int LANES, bool CERT>
+__device__ __forceinline__ bool extract(const RouteArgs& a, bool on, RouteShared& sh) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, sub = lane % LANES, row = lane / LANES;
     const unsigned segment = (LANES == 32 ? ~0u : (1u << LANES) - 1) << (row * LANES);
+    unsigned long long head = on ? sh.list[w][0][lane] : 0;
+    int next = 1;  // of the lane's list
+    bool near = false;
     float last_key = INFINITY, last_score = 0.0f;
     for (int j = 0; j < a.k + (CERT ? 1 : 0); ++j) {
-        const U m = seg_max<LANES>(best);
-        const int owner = __ffs(__ballot_sync(~0u, best == m) & segment) - 1;
-        int at = kV;
-        float score = 0.0f;
-#pragma unroll
-        for (int i = kV - 1; i >= 0; --i)
-            if (u[i] == m) at = i;
-        float t = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kV; ++i)
-            if (i == at) {
-                t = take[i];
-                if (CERT) score = s[i];
-                if (lane == owner) u[i] = 0;
-            }
-        if (j < a.k && lane == owner) {
-            sh.ids[w][row * a.k + j] = m ? sub * kV + at : -1;
-            sh.v[w][row * a.k + j] = t;
+        const uint32_t rank = static_cast<uint32_t>(head >> 32);
+        const uint32_t m = seg_max<LANES>(rank);
+        const int owner = __ffs(__ballot_sync(~0u, rank == m) & segment) - 1;
+        const int id = sub * kV + 7 - static_cast<int>(head & 7);
+        if (lane == owner) {
+            if (j < a.k) sh.ids[w][row * a.k + j] = m ? id : -1;
+            head = next < kV ? sh.list[w][next][lane] : 0;
+            ++next;
         }
-        best = 0;
-#pragma unroll
-        for (int i = 0; i < kV; ++i) best = max(best, u[i]);
         if constexpr (CERT) {
-            score = __shfl_sync(~0u, score, owner);
-            const float k = value_of(m);
-            if (a.bias && j > 0 && m) near |= !(last_key - k > slack(score, k) + slack(last_score, last_key));
+            const int at = __shfl_sync(~0u, id, owner);
+            const float score = sh.take[w][row * LANES * kV + at], k = value_of(m);
+            if (j > 0 && m) near |= !(last_key - k > slack(score, k) + slack(last_score, last_key));
             last_key = k;
             last_score = score;
         }
@@ -301,12 +347,12 @@ __device__ __forceinline__ void load_row(const RouteArgs& a, int64_t t, int e0, 
         if (e0 + i < a.E) x[i] = static_cast<float>(p[i]);
 }
 
-// The choice again with keys in 64 bits (rare: kept apart from the registers of
+// The choice again with keys in 64 bits (rare, and kept apart from the registers of
 // the ordinary path).
 template <int LANES>
-__device__ __noinline__ void choose_exactly(const RouteArgs& a, const float (&x)[kV], const float (&take)[kV],
-                                            RouteShared& sh) {
-    const int e0 = (threadIdx.x & 31) % LANES * kV;
+__device__ __noinline__ void choose_exactly(const RouteArgs& a, const float (&x)[kV], RouteShared& sh, double* values) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, sub = lane % LANES, row = lane / LANES, e0 = sub * kV;
+    const unsigned segment = (LANES == 32 ? ~0u : (1u << LANES) - 1) << (row * LANES);
     double s[kV], key[kV], by[kV];
     scores<LANES>(x, a.sigmoid, s);
 #pragma unroll
@@ -314,55 +360,138 @@ __device__ __noinline__ void choose_exactly(const RouteArgs& a, const float (&x)
         const float b = a.bias && e0 + i < a.E ? a.bias[e0 + i] : 0.0f;
         const bool none = x[i] == -INFINITY || b == -INFINITY;
         key[i] = none ? -INFINITY : a.bias ? s[i] + static_cast<double>(b) : static_cast<double>(x[i]);
-        by[i] = none ? -INFINITY : a.bias ? key[i] : s[i];
+        by[i] = none ? -INFINITY : a.bias ? key[i] : a.group_top == 2 ? s[i] : key[i];
     }
-    choose<LANES, double, false>(a, key, by, s, take, sh);
+    // the lists are no longer needed
+    if (a.groups > 1) keep_groups<LANES, double>(a, key, by, 0.0f, &sh.list[w][0][0], values);
+    unsigned long long u[kV];
+#pragma unroll
+    for (int i = 0; i < kV; ++i) u[i] = rank_of(key[i]);
+    for (int j = 0; j < a.k; ++j) {
+        unsigned long long best = 0;
+#pragma unroll
+        for (int i = 0; i < kV; ++i) best = max(best, u[i]);
+        const unsigned long long m = seg_max<LANES>(best);
+        const int owner = __ffs(__ballot_sync(~0u, best == m) & segment) - 1;
+        if (lane == owner) {
+            int at = kV;
+#pragma unroll
+            for (int i = kV - 1; i >= 0; --i) at = u[i] == m ? i : at;
+#pragma unroll
+            for (int i = 0; i < kV; ++i) u[i] = i == at ? 0 : u[i];
+            sh.ids[w][row * a.k + j] = m ? e0 + at : -1;
+        }
+        __syncwarp();
+    }
 }
 
-template <int LANES, typename LT>
-__global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteArgs a) {
+// Any groups that are not whole lanes go through shared memory (ANY).
+template <int LANES, typename LT, bool ANY>
+__global__ void __launch_bounds__(kRouteThreads, 4) route_kernel(const RouteArgs a) {
+    extern __shared__ uint8_t dynamic[];
     __shared__ RouteShared sh;
+    auto& gsh = *reinterpret_cast<GroupShared*>(dynamic);  // ANY
     constexpr int ROWS = 32 / LANES;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, sub = lane % LANES, row = lane / LANES, e0 = sub * kV;
     const int64_t t0 = (static_cast<int64_t>(blockIdx.x) * kRouteWarps + w) * ROWS;
     if (t0 >= a.T) return;
-    float x[kV], s[kV], key[kV], by[kV], take[kV];
+    float x[kV], s[kV], key[kV];
     load_row<LT>(a, t0 + row, e0, x);
     // renormalised softmax weights are the softmax of the chosen logits
     const bool of_logits = a.renorm && !a.sigmoid, two = a.groups > 1 && a.group_top == 2;
     const bool scored = !of_logits || a.bias || two;
     if (scored) scores<LANES>(x, a.sigmoid, s);
+    bool nan = false;  // a NaN among the scores is one in all of them
 #pragma unroll
     for (int i = 0; i < kV; ++i) {
         if (!scored) s[i] = 0.0f;
         const float b = a.bias && e0 + i < a.E ? a.bias[e0 + i] : 0.0f;
         const bool none = x[i] == -INFINITY || b == -INFINITY;
         key[i] = none ? -INFINITY : a.bias ? s[i] + b : x[i];
-        by[i] = none ? -INFINITY : a.bias ? key[i] : two ? s[i] : x[i];
-        take[i] = of_logits ? (s[i] == s[i] ? x[i] : s[i]) : s[i];
+        nan |= s[i] != s[i];
     }
-    if (a.bias || two) {
-        if (__any_sync(~0u, choose<LANES, float, true>(a, key, by, s, take, sh))) choose_exactly<LANES>(a, x, take, sh);
-    } else {
-        choose<LANES, float, false>(a, key, by, s, take, sh);
+    const bool sure = !a.bias && !two;  // keys are the logits themselves
+    float e = 0.0f;                     // slack of a group's value
+    if (!sure && a.groups > 1) {
+        float top = 0.0f, largest = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kV; ++i) {
+            top = fmaxf(top, s[i]);
+            if (key[i] != -INFINITY) largest = fmaxf(largest, fabsf(a.bias ? key[i] : s[i]));
+        }
+        top = seg_max<LANES>(top);
+        largest = seg_max<LANES>(largest);
+        e = 4.0f * slack(top, largest) + 0x1p-22f * largest;
+    }
+    bool near = false, on = true;
+    if constexpr (ANY) {
+        float by[kV];
+#pragma unroll
+        for (int i = 0; i < kV; ++i) by[i] = key[i] == -INFINITY ? -INFINITY : a.bias ? key[i] : two ? s[i] : key[i];
+        near = keep_groups<LANES, float>(a, key, by, e, gsh.by[w], gsh.value[w]);
+    }
+    unsigned long long v[kV];
+#pragma unroll
+    for (int i = 0; i < kV; ++i) v[i] = entry_of(rank_of(key[i]), i);
+    // what becomes of an expert: its score, for the bound and for the weights (a
+    // logit where they are the softmax of the chosen logits)
+#pragma unroll
+    for (int i = 0; i < kV; i += 4)
+        *reinterpret_cast<float4*>(&sh.take[w][lane * kV + i]) =
+            of_logits && !a.bias && !nan ? make_float4(x[i], x[i + 1], x[i + 2], x[i + 3])
+                                         : make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
+    sort8(v);
+#pragma unroll
+    for (int i = 0; i < kV; ++i) sh.list[w][i][lane] = v[i];
+    __syncwarp();
+    if (!ANY && a.groups > 1) {
+        float first = value_of(static_cast<uint32_t>(v[0] >> 32)), second = value_of(static_cast<uint32_t>(v[1] >> 32));
+        if (!a.bias && two) {  // values are scores, in the same order
+            const float* mine = &sh.take[w][lane * kV];
+            if (of_logits && !nan) {
+                // (their logits lie there; the scores are in registers)
+                float p = -INFINITY, q = -INFINITY;
+                const int i0 = 7 - static_cast<int>(v[0] & 7), i1 = 7 - static_cast<int>(v[1] & 7);
+#pragma unroll
+                for (int i = 0; i < kV; ++i) p = i == i0 ? s[i] : p, q = i == i1 ? s[i] : q;
+                first = first == -INFINITY ? first : p;
+                second = second == -INFINITY ? second : q;
+            } else {
+                first = first == -INFINITY ? first : mine[7 - static_cast<int>(v[0] & 7)];
+                second = second == -INFINITY ? second : mine[7 - static_cast<int>(v[1] & 7)];
+            }
+        }
+        on = keep_lanes<LANES, float>(a, a.size / kV, first, second, e, near);
+    }
+    if (a.bias)
+        near |= extract<LANES, true>(a, on, sh);
+    else
+        extract<LANES, false>(a, on, sh);
+    if (!sure && __any_sync(~0u, near)) choose_exactly<LANES>(a, x, sh, ANY ? gsh.value[w] : sh.value[w]);
+    if (of_logits && a.bias) {  // the scores have been compared
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kV; ++i) sh.take[w][lane * kV + i] = nan ? s[i] : x[i];
+        __syncwarp();
     }
     // weights: the sums over a row's k in the order of the slots
     const int n = static_cast<int>(min(static_cast<int64_t>(ROWS), a.T - t0)) * a.k;
     for (int i = lane; i < n; i += 32) {
-        const int r0 = i / a.k * a.k;
+        const int r = i * a.k_inv >> 16, r0 = r * a.k;
+        const float* take = &sh.take[w][r * LANES * kV];
         const int id = sh.ids[w][i];
-        float v = sh.v[w][i];
+        float v = id >= 0 ? take[id] : 0.0f;
         if (of_logits) {
             float m = -INFINITY, z = 0.0f;
             for (int j = r0; j < r0 + a.k; ++j)
-                if (sh.ids[w][j] >= 0) m = fmaxf(m, sh.v[w][j]);
+                if (sh.ids[w][j] >= 0) m = fmaxf(m, take[sh.ids[w][j]]);
             for (int j = r0; j < r0 + a.k; ++j)
-                if (sh.ids[w][j] >= 0) z += expf(sh.v[w][j] - m);
+                if (sh.ids[w][j] >= 0) z += expf(take[sh.ids[w][j]] - m);
             v = expf(v - m) / z;
         } else if (a.renorm) {
             float z = 0.0f;
             for (int j = r0; j < r0 + a.k; ++j)
-                if (sh.ids[w][j] >= 0) z += sh.v[w][j];
+                if (sh.ids[w][j] >= 0) z += take[sh.ids[w][j]];
             v /= z + 1e-20f;
         }
         a.ids[t0 * a.k + i] = id;
@@ -375,113 +504,119 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteArgs a)
 //   softmax, renormalised     dx_j = c q_j (g_j - sum_i g_i q_i), q = softmax of the chosen
 //   sigmoid                   dx_j = c g_j s_j (1 - s_j)
 //   sigmoid, renormalised     dx_j = c (g_j - sum_i g_i v_i / D) / D s_j (1 - s_j), D = sum v + 1e-20
-// and zero for the experts that were not chosen, in the last three.  A slot's
-// term is computed by a lane and left in shared memory; every lane adds the terms
-// of its own experts in the order of the slots.
+// and zero for the experts that were not chosen, in the last three.  A lane has a
+// slot: it leaves what the row's sums need in shared memory, takes the sums from
+// there in the slots' order, and leaves its term at its expert; of slots with the
+// same expert the first one adds the others' terms.  Then every lane writes its own 8
+// experts.
 template <int LANES, typename LT>
 __global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const RouteArgs a) {
     __shared__ int32_t s_ids[kRouteWarps][256];
-    __shared__ float s_x[kRouteWarps][256], s_g[kRouteWarps][256];
+    __shared__ float s_p[kRouteWarps][256], s_g[kRouteWarps][256], s_term[kRouteWarps][256];
+    __shared__ __align__(16) float s_row[kRouteWarps][256];
     constexpr int ROWS = 32 / LANES;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, sub = lane % LANES, row = lane / LANES, e0 = sub * kV;
     const int64_t t0 = (static_cast<int64_t>(blockIdx.x) * kRouteWarps + w) * ROWS;
     if (t0 >= a.T) return;
     const int64_t t = t0 + row;
     const bool all = !a.sigmoid && !a.renorm;
-    float x[kV], s[kV];
-    if (all) load_row<LT>(a, t, e0, x);
     const int n = static_cast<int>(min(static_cast<int64_t>(ROWS), a.T - t0)) * a.k;
-    for (int i = lane; i < n; i += 32) {
-        const int64_t r = t0 + i / a.k;
-        const int j = i % a.k;
-        const int id = a.ids_in[r * a.ldi + j];
-        const bool on = id >= 0 && id < a.E;
-        if (id >= a.E) atomicOr(a.err, ERR_ROUTE_EXPERT);
-        s_ids[w][i] = on ? id : -1;
-        s_x[w][i] = on ? static_cast<float>(static_cast<const LT*>(a.logits)[r * a.ld + id]) : 0.0f;
-        s_g[w][i] = on ? a.grad[r * a.ldg + j] * a.scale : 0.0f;
-    }
-    __syncwarp();
-    float dot = 0.0f;
+    float s[kV], m = 0.0f, r = 0.0f;
     if (all) {
-        float m = -INFINITY;
+        float x[kV], z = 0.0f;
+        load_row<LT>(a, t, e0, x);
+        m = -INFINITY;
 #pragma unroll
         for (int i = 0; i < kV; ++i) m = fmaxf(m, x[i]);
         m = seg_max<LANES>(m);
         if (m == -INFINITY) m = 0.0f;
-        float z = 0.0f;
 #pragma unroll
         for (int i = 0; i < kV; ++i) {
             s[i] = expf(x[i] - m);
             z += s[i];
         }
         z = seg_sum<LANES>(z);
-        const float r = z == 0.0f ? 0.0f : 1.0f / z;
+        r = z == 0.0f ? 0.0f : 1.0f / z;
 #pragma unroll
         for (int i = 0; i < kV; ++i) s[i] *= r;
-        if (t < a.T)
-            for (int j = sub; j < a.k; j += LANES)
-                if (s_ids[w][row * a.k + j] >= 0) dot += s_g[w][row * a.k + j] * (expf(s_x[w][row * a.k + j] - m) * r);
-        dot = seg_sum<LANES>(dot);
-    } else {
-        float d[8];  // a lane's slots: n <= 256
-        int at = 0;
-        for (int i = lane; i < n; i += 32, ++at) {
-            const int r0 = i / a.k * a.k;
-            float v = 0.0f;
-            if (s_ids[w][i] >= 0) {
-                const float g = s_g[w][i];
-                if (a.sigmoid) {
-                    const float e = expf(-fabsf(s_x[w][i])), q = 1.0f / (1.0f + e);
-                    const float up = s_x[w][i] < 0.0f ? e * q : q, down = s_x[w][i] < 0.0f ? q : e * q;
-                    v = g;
-                    if (a.renorm) {
-                        float z = 0.0f, p = 0.0f;
-                        for (int j = r0; j < r0 + a.k; ++j)
-                            if (s_ids[w][j] >= 0) {
-                                const float f = expf(-fabsf(s_x[w][j]));
-                                z += (s_x[w][j] < 0.0f ? f : 1.0f) / (1.0f + f);
-                            }
-                        z += 1e-20f;
-                        for (int j = r0; j < r0 + a.k; ++j)
-                            if (s_ids[w][j] >= 0) {
-                                const float f = expf(-fabsf(s_x[w][j]));
-                                p = fmaf(s_g[w][j], (s_x[w][j] < 0.0f ? f : 1.0f) / (1.0f + f) / z, p);
-                            }
-                        v = (g - p) / z;
-                    }
-                    v *= up * down;
-                } else {
-                    float m = -INFINITY, z = 0.0f, p = 0.0f;
-                    for (int j = r0; j < r0 + a.k; ++j)
-                        if (s_ids[w][j] >= 0) m = fmaxf(m, s_x[w][j]);
-                    for (int j = r0; j < r0 + a.k; ++j)
-                        if (s_ids[w][j] >= 0) z += expf(s_x[w][j] - m);
-                    for (int j = r0; j < r0 + a.k; ++j)
-                        if (s_ids[w][j] >= 0) p = fmaf(s_g[w][j], expf(s_x[w][j] - m) / z, p);
-                    v = expf(s_x[w][i] - m) / z * (g - p);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (j == at) d[j] = v;
-        }
-        __syncwarp();
-        at = 0;
-        for (int i = lane; i < n; i += 32, ++at)
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (j == at) s_g[w][i] = d[j];
-        __syncwarp();
     }
-    if (t >= a.T || e0 >= a.E) return;
-    float sum[kV] = {};
-    for (int j = 0; j < a.k; ++j) {
-        const int id = s_ids[w][row * a.k + j];
-        if (id < e0 || id >= e0 + kV) continue;
-        const float g = s_g[w][row * a.k + j];
 #pragma unroll
-        for (int i = 0; i < kV; ++i) sum[i] += id == e0 + i ? g : 0.0f;
+    for (int i = 0; i < kV; i += 4) *reinterpret_cast<float4*>(&s_row[w][lane * kV + i]) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    // a slot's id, gradient and score (softmax, renormalised: its logit)
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        const int i = i0 + lane, q = min(i, n - 1) * a.k_inv >> 16;
+        // the row's largest logit and its sum, from its lanes
+        const float mq = __shfl_sync(~0u, m, q * LANES), rq = __shfl_sync(~0u, r, q * LANES);
+        if (i >= n) continue;
+        const int id = a.ids_in[(t0 + q) * a.ldi + i - q * a.k];
+        const float g = a.grad[(t0 + q) * a.ldg + i - q * a.k] * a.scale;
+        const bool on = id >= 0 && id < a.E;
+        if (id >= a.E) atomicOr(a.err, ERR_ROUTE_EXPERT);
+        const float x = on ? static_cast<float>(static_cast<const LT*>(a.logits)[(t0 + q) * a.ld + id]) : 0.0f;
+        s_ids[w][i] = on ? id : -1;
+        s_g[w][i] = on ? g : 0.0f;
+        if (a.sigmoid) {
+            const float e = expf(-fabsf(x)), f = 1.0f / (1.0f + e);
+            s_p[w][i] = on ? (x < 0.0f ? e * f : f) : 0.0f;
+            s_term[w][i] = x < 0.0f ? f : e * f;  // 1 - s
+        } else {
+            s_p[w][i] = !on ? (all ? 0.0f : -INFINITY) : all ? expf(x - mq) * rq : x;
+        }
+    }
+    __syncwarp();
+    for (int i = lane; i < n; i += 32) {
+        const int j0 = (i * a.k_inv >> 16) * a.k, j1 = j0 + a.k;
+        const float g = s_g[w][i], p = s_p[w][i];
+        if (a.sigmoid) {
+            float v = g;
+            if (a.renorm) {
+                float z = 0.0f, sum = 0.0f;
+                for (int j = j0; j < j1; ++j) z += s_p[w][j];
+                z += 1e-20f;
+                const float f = 1.0f / z;
+                for (int j = j0; j < j1; ++j) sum = fmaf(s_g[w][j], s_p[w][j] * f, sum);
+                v = (g - sum) * f;
+            }
+            s_term[w][i] *= v * p;
+        } else if (a.renorm) {
+            float top = -INFINITY, z = 0.0f, sum = 0.0f;
+            for (int j = j0; j < j1; ++j) top = fmaxf(top, s_p[w][j]);
+            if (top == -INFINITY) top = 0.0f;
+            for (int j = j0; j < j1; ++j) {
+                const float q = expf(s_p[w][j] - top);
+                z += q;
+                sum = fmaf(s_g[w][j], q, sum);
+            }
+            s_term[w][i] = expf(p - top) / z * (g - sum / z);
+        } else {
+            s_term[w][i] = g;
+        }
+    }
+    float dot = 0.0f;
+    if (all) {
+        if (t < a.T)
+            for (int j = sub; j < a.k; j += LANES) dot = fmaf(s_g[w][row * a.k + j], s_p[w][row * a.k + j], dot);
+        dot = seg_sum<LANES>(dot);
+    }
+    __syncwarp();
+    for (int i = lane; i < n; i += 32) {
+        const int q = i * a.k_inv >> 16, id = s_ids[w][i], j0 = q * a.k;
+        bool first = id >= 0;
+        float v = 0.0f;
+        for (int j = j0; j < j0 + a.k; ++j) {
+            const bool same = s_ids[w][j] == id;
+            first &= !(same && j < i);
+            v += same ? s_term[w][j] : 0.0f;
+        }
+        if (first) s_row[w][q * LANES * kV + id] = v;
+    }
+    __syncwarp();
+    if (t >= a.T || e0 >= a.E) return;
+    float sum[kV];
+#pragma unroll
+    for (int i = 0; i < kV; i += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(&s_row[w][lane * kV + i]);
+        sum[i] = v.x, sum[i + 1] = v.y, sum[i + 2] = v.z, sum[i + 3] = v.w;
     }
     if (all)
 #pragma unroll
@@ -549,7 +684,8 @@ RouteArgs route_args(const aem_route_config* c, const void* logits, aem_dtype dt
     a.top_groups = c->top_groups;
     a.group_top = c->group_top;
     a.size = E / c->groups;
-    a.size_inv = (65536 + a.size - 1) / a.size;  // e * size_inv >> 16 == e / size for e < 256
+    a.size_inv = (65536 + a.size - 1) / a.size;
+    a.k_inv = (65536 + a.k - 1) / a.k;
     a.scale = c->scale;
     a.sigmoid = c->score == AEM_SCORE_SIGMOID;
     a.renorm = c->renormalize != 0;
@@ -588,10 +724,28 @@ aem_status aem_route_tokens(const aem_route_config* config, const void* logits, 
         st = aem::route_grid("aem_route_tokens", T, 32 / L, &blocks);
         if (st != AEM_OK) return;
         auto s = static_cast<cudaStream_t>(stream);
+        const int span = a.size / aem::kV;
+        const bool any = a.groups > 1 && (a.size % aem::kV != 0 || (span & (span - 1)) != 0);
+        auto go = [&](auto kern, auto any_groups) {
+            constexpr bool ANY = decltype(any_groups)::value;
+            if constexpr (ANY) {
+                static std::atomic<uint64_t> kernels[2];  // per dtype (the kernels have one type), a bit per
+                auto& ready = kernels[dtype];             // device: the shared memory opt-in is done
+                const uint64_t bit = 1ull << (aem::current_device() & 63);
+                if (!(ready.load(std::memory_order_relaxed) & bit)) {
+                    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                               static_cast<int>(sizeof(aem::GroupShared)));
+                    if (e == cudaSuccess) ready.fetch_or(bit, std::memory_order_relaxed);
+                }
+            }
+            kern<<<blocks, aem::kRouteThreads, ANY ? sizeof(aem::GroupShared) : 0, s>>>(a);
+        };
+        const std::true_type yes;
+        const std::false_type no;
         if (dtype == AEM_F32)
-            aem::route_kernel<L, float><<<blocks, aem::kRouteThreads, 0, s>>>(a);
+            any ? go(aem::route_kernel<L, float, true>, yes) : go(aem::route_kernel<L, float, false>, no);
         else
-            aem::route_kernel<L, __nv_bfloat16><<<blocks, aem::kRouteThreads, 0, s>>>(a);
+            any ? go(aem::route_kernel<L, __nv_bfloat16, true>, yes) : go(aem::route_kernel<L, __nv_bfloat16, false>, no);
     });
     AEM_TRY(st);
     AEM_CHECK_LAUNCH();
