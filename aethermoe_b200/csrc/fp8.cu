@@ -86,12 +86,12 @@ __device__ __forceinline__ bool find_rows(const Fp8Args& a, int slot, int64_t* g
     return false;
 }
 
-// a0 += s0 * v0, a1 += s1 * v1 with s = f * (c0, c1)
-__device__ __forceinline__ void fma2(float& a0, float& a1, float f, float c0, float c1, uint32_t v0, uint32_t v1) {
-    asm("{\n.reg .b64 a, f, s, v;\nmov.b64 a, {%0, %1};\nmov.b64 f, {%2, %2};\nmov.b64 s, {%3, %4};\n"
-        "mov.b64 v, {%5, %6};\nmul.rn.f32x2 s, s, f;\nfma.rn.f32x2 a, s, v, a;\nmov.b64 {%0, %1}, a;\n}"
-        : "+f"(a0), "+f"(a1)
-        : "f"(f), "f"(c0), "f"(c1), "r"(v0), "r"(v1));
+// a0 += s0 * v0, a1 += s1 * v1
+__device__ __forceinline__ void fma2(float& a0, float& a1, float s0, float s1, uint32_t v0, uint32_t v1) {
+    asm volatile("{\n.reg .b64 a, s, v;\nmov.b64 a, {%0, %1};\nmov.b64 s, {%2, %3};\nmov.b64 v, {%4, %5};\n"
+                 "fma.rn.f32x2 a, s, v, a;\nmov.b64 {%0, %1}, a;\n}"
+                 : "+f"(a0), "+f"(a1)
+                 : "f"(s0), "f"(s1), "r"(v0), "r"(v1));
 }
 
 __device__ __forceinline__ void st_cluster(const float4* p, uint32_t rank, float4 v) {
@@ -133,14 +133,6 @@ __device__ __forceinline__ void store_out(const Fp8Args& a, int64_t m, int64_t n
 template <bool MN>
 constexpr uint32_t kStep32 = MN ? 32 * 128 / 16 : 32 / 16;
 
-// 4 bytes global -> shared without waiting; lands before the barrier's phase ends.
-__device__ __forceinline__ void copy4_async(void* dst, const void* src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void arrive_after_copies(uint64_t* bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
 // Few rows: a CTA computes 128 columns of out for a tile of TN rows over its part
 // of the sum.
 //   warps 0-7   thread = column of out = TMEM lane; warps 0-3 have the first half
@@ -148,7 +140,8 @@ __device__ __forceinline__ void arrive_after_copies(uint64_t* bar) {
 //               comes back and scale * sum is added to the row's register.
 //   warp 8      issues the MMAs (M = 128, N = rows, K = 32), four per block
 //   warp 9      copies the weights, one bulk copy of a 16 KB tile per block
-//   warp 10     copies the rows, one TMA box per block, and their scales
+//   warp 10     copies the rows, one TMA box per block, and leaves the products of
+//               their scales with the block's beside them
 // The S CTAs of a cluster take parts of the sum: each sends its sums to the rank
 // that writes those rows, which adds them in rank order.
 // Every wait is bounded; a timeout sets the error word and ends all roles.
@@ -200,12 +193,16 @@ __global__ void __launch_bounds__(kFewThreads, ALONE ? 1 : 2)
     const int p0 = static_cast<int>(static_cast<int64_t>(a.kb) * ks / a.S);
     const int np = static_cast<int>(static_cast<int64_t>(a.kb) * (ks + 1) / a.S) - p0;
     const int64_t t0 = g * a.group_tiles + tile * a.out_step + p0 * a.sum_step;  // the CTA's first tile
+    auto copy_weights = [&](int u) {
+        mbar_arrive_expect_tx(&full[u % C::NS], kFp8Tile);
+        bulk_load(ring + u % C::NS * kFp8Tile, a.w + (t0 + u * a.sum_step) * kFp8Tile, kFp8Tile, &full[u % C::NS]);
+    };
     if (w == 8) {
         tmem_alloc(tmem_slot, C::COLS);
         tmem_relinquish();
     } else if (w == 9 && lane == 0) {
         for (int i = 0; i < C::NS; ++i) {
-            mbar_init(&full[i], 2 + 32);  // both copies' bytes and the scales of every lane
+            mbar_init(&full[i], 3);  // both copies' bytes and the scales
             mbar_init(&empty[i], 1 + 8);  // the MMAs and the warps that read the scales
         }
         for (int i = 0; i < C::ND; ++i) {
@@ -214,6 +211,8 @@ __global__ void __launch_bounds__(kFewThreads, ALONE ? 1 : 2)
         }
         *abort_flag = 0;
         fence_barrier_init();
+        // the first weights are on their way before the rest of the set-up
+        for (int u = 0; u < min(np, C::NS); ++u) copy_weights(u);
     } else if (w == 10 && lane == 0) {
         tma_prefetch_desc(&xmap);
     }
@@ -231,11 +230,8 @@ __global__ void __launch_bounds__(kFewThreads, ALONE ? 1 : 2)
     if (w < 8) {
         const int h = w >> 2;
         const uint32_t at = tmem + (static_cast<uint32_t>(32 * (w & 3)) << 16) + h * CPT;
-        float held = 0.0f;  // the weight scales of 32 blocks, one a lane
         for (int u = 0; u < np; ++u) {
             const int st = u % C::NS, b = u % C::ND;
-            if ((u & 31) == 0) held = u + lane < np ? a.ws[t0 + (u + lane) * a.sum_step] : 0.0f;
-            const float f = __shfl_sync(~0u, held, u & 31);
             if (!wait(&full[st], u / C::NS) || !wait(&dfull[b], u / C::ND)) break;
             tc_fence_after();
             uint32_t d[CPT];
@@ -255,8 +251,8 @@ __global__ void __launch_bounds__(kFewThreads, ALONE ? 1 : 2)
 #pragma unroll
             for (int c = 0; c < CPT; c += 4) {
                 const float4 s = sc[c / 4];
-                fma2(acc[c], acc[c + 1], f, s.x, s.y, d[c], d[c + 1]);
-                fma2(acc[c + 2], acc[c + 3], f, s.z, s.w, d[c + 2], d[c + 3]);
+                fma2(acc[c], acc[c + 1], s.x, s.y, d[c], d[c + 1]);
+                fma2(acc[c + 2], acc[c + 3], s.z, s.w, d[c + 2], d[c + 3]);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[st]);
@@ -277,12 +273,10 @@ __global__ void __launch_bounds__(kFewThreads, ALONE ? 1 : 2)
         }
     } else if (w == 9) {
         if (lane == 0) {
-            int u = 0;
+            int u = min(np, C::NS);
             for (; u < np; ++u) {
-                const int st = u % C::NS;
-                if (!mbar_wait_bounded(&empty[st], (u / C::NS + 1) & 1, abort_flag, a.err, ERR_GEMM_TIMEOUT)) break;
-                mbar_arrive_expect_tx(&full[st], kFp8Tile);
-                bulk_load(ring + st * kFp8Tile, a.w + (t0 + u * a.sum_step) * kFp8Tile, kFp8Tile, &full[st]);
+                if (!mbar_wait_bounded(&empty[u % C::NS], (u / C::NS + 1) & 1, abort_flag, a.err, ERR_GEMM_TIMEOUT)) break;
+                copy_weights(u);
             }
             if (*abort_flag)  // a failed call leaves no copy in flight behind (bounded as well)
                 for (int i = max(0, u - C::NS); i < u; ++i)
@@ -290,18 +284,44 @@ __global__ void __launch_bounds__(kFewThreads, ALONE ? 1 : 2)
                     }
         }
     } else {
+        // scales: the weights' of 32 blocks, one a lane, and the rows' of a lane's rows,
+        // four blocks at a time and four ahead
+        constexpr int R = (TN + 31) / 32;
+        float held = a.ws[t0 + min(lane, np - 1) * a.sum_step], now[R][4], next[R][4];
         asm volatile("griddepcontrol.wait;" ::: "memory");  // the rows may be another kernel's
         const float* xs = a.xs + m0 * a.lds + p0;
+        auto fetch = [&](int u) {
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) next[r][k] = xs[min(r * 32 + lane, rows - 1) * a.lds + min(u + k, np - 1)];
+        };
+        fetch(0);
         int u = 0;
-        for (; u < np; ++u) {
-            const int st = u % C::NS;
-            if (!wait(&empty[st], u / C::NS + 1)) break;
-            if (lane == 0) {
-                mbar_arrive_expect_tx(&full[st], C::XB);
-                tma_load_2d(xring + st * C::XB, &xmap, &full[st], (p0 + u) * 128, static_cast<int>(m0));
+        for (bool ok = true; ok && u < np;) {
+            if (u && (u & 31) == 0) held = a.ws[t0 + min(u + lane, np - 1) * a.sum_step];
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) now[r][k] = next[r][k];
+            fetch(u + 4);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (u >= np) break;
+                const int st = u % C::NS;
+                const float sw = __shfl_sync(~0u, held, u & 31);
+                if (!(ok = wait(&empty[st], u / C::NS + 1))) break;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&full[st], C::XB);
+                    tma_load_2d(xring + st * C::XB, &xmap, &full[st], (p0 + u) * 128, static_cast<int>(m0));
+                }
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+                    if (r * 32 + lane < TN) sring[st * TN + r * 32 + lane] = now[r][k] * sw;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full[st]);
+                ++u;
             }
-            for (int r = lane; r < rows; r += 32) copy4_async(sring + st * TN + r, xs + r * a.lds + u);
-            arrive_after_copies(&full[st]);
         }
         if (lane == 0 && *abort_flag)
             for (int i = max(0, u - C::NS); i < u; ++i)
@@ -783,21 +803,34 @@ __global__ void __launch_bounds__(256)
 
 constexpr int kSMs = 148;
 
-// CTAs (at most 8, one cluster) that split the sum, in blocks of a CTA: its set-up
-// and end take about 14, a hand-over between CTAs 6 more.
-int split_sum(int64_t ctas, int64_t blocks, int slots) {
-    int best = 1;
+// What a product takes, in units of 10 ns, from its CTAs (pairs), the blocks of the
+// sum and the rows of a tile.
+//
+// Few rows: CTAs (at most 8, one cluster) split the sum.  Row tiles of 16 and 32
+// share an SM by twos while there are more CTAs than SMs, the wider ones have one to
+// themselves.  One row, 4096 x 4096 (32 tiles): 1, 2, 4, 8 CTAs a tile 12.8, 9.4, 7.3,
+// 8.1 us; 14336 x 4096: 38.8, 22.1, 14.8, 13.9; 4096 x 14336 (112 tiles): 14.3, 13.9,
+// 17.5, 24.2.  128 rows, 4096 x 4096: 21.1, 16.7, 13.8, 32.1.
+int64_t few_cost(int64_t ctas, int64_t blocks, int rows, int* split) {
     int64_t least = INT64_MAX;
     for (int S = 1; S <= 8 && (S == 1 || blocks >= 2 * S); ++S) {
         const int64_t each = (blocks + S - 1) / S, n = ctas * S;
-        const int64_t cost = (n + slots - 1) / slots * (14 + (S > 1 ? 6 : 0) + each);
+        int64_t cost;
+        if (rows <= 32)
+            cost = n <= kSMs ? 530 + 30 * each : (n + 2 * kSMs - 1) / (2 * kSMs) * (720 + 45 * each);
+        else
+            cost = (n + kSMs - 1) / kSMs * (700 + (S > 1 ? 200 : 0) + (rows <= 64 ? 34 : 55) * each);
         if (cost < least) {
             least = cost;
-            best = S;
+            *split = S;
         }
     }
-    return best;
+    return least;
 }
+// Many rows: persistent pairs.  256 rows, 4096 x 14336 (56 tiles): 21.4 us where the
+// kernel for few rows takes 43.7; 14336 x 4096 (16 tiles): 53.9 and 34.6.  64 experts of
+// 2048 x 1408 with 128, 192, 256 rows each: 81, 87, 92 us and 85, 141, 155.
+int64_t many_cost(int64_t tiles, int64_t blocks, int pairs) { return (tiles + pairs - 1) / pairs * (570 + 47 * blocks); }
 
 template <int TN, bool ALONE>
 aem_status launch_few(Fp8Args a, const void* q, int64_t ldq, int64_t cols, bool transposed, bool dependent,
@@ -812,7 +845,6 @@ aem_status launch_few(Fp8Args a, const void* q, int64_t ldq, int64_t cols, bool 
         AEM_TRY_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
         ready[transposed].fetch_or(bit, std::memory_order_relaxed);
     }
-    a.S = split_sum(a.nb * slots, a.kb, kSMs * C::CTAS);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(a.nb * a.S), static_cast<unsigned>(slots));
     cfg.blockDim = dim3(kFewThreads);
@@ -837,20 +869,30 @@ aem_status launch_few(Fp8Args a, const void* q, int64_t ldq, int64_t cols, bool 
     return AEM_OK;
 }
 
-// Pairs of SMs that can run the kernel at once.
+// Pairs of SMs that can run the kernel at once (0: it cannot).
 int max_pairs(int device) {
     static std::atomic<int> cache[64];
-    int n = cache[device & 63].load(std::memory_order_relaxed);
-    if (n > 0) return n;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(2 * 512);
-    cfg.blockDim = dim3(kManyThreads);
-    cfg.dynamicSmemBytes = kManySmem;
-    if (cudaOccupancyMaxActiveClusters(&n, fp8_many_kernel<false, true>, &cfg) != cudaSuccess || n < 1) {
-        cudaGetLastError();
-        n = kSMs / 2;
+    const int known = cache[device & 63].load(std::memory_order_relaxed);
+    if (known) return known - 1;
+    int n = 0;
+    for (auto kern : {fp8_many_kernel<false, false>, fp8_many_kernel<false, true>, fp8_many_kernel<true, false>,
+                      fp8_many_kernel<true, true>}) {
+        cudaFuncAttributes f;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(2 * 512);
+        cfg.blockDim = dim3(kManyThreads);
+        cfg.dynamicSmemBytes = kManySmem;
+        // a launch with fewer registers could not share them out as the kernel does
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kManySmem) != cudaSuccess ||
+            cudaFuncGetAttributes(&f, kern) != cudaSuccess ||
+            f.numRegs * kManyThreads < kManyFewRegs * 128 + kManyManyRegs * 256 ||
+            cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+            cudaGetLastError();
+            n = 0;
+            break;
+        }
     }
-    cache[device & 63].store(n, std::memory_order_relaxed);
+    cache[device & 63].store(n + 1, std::memory_order_relaxed);
     return n;
 }
 
@@ -859,24 +901,8 @@ aem_status launch_many(const Fp8Args& a, const Fp8Weight* w, const void* q, int6
     CUtensorMap xmap{}, wmap{};
     AEM_TRY(make_tmap_2d_u8(&xmap, q, cols, a.M, ldq, 128, CU_TENSOR_MAP_SWIZZLE_128B));
     AEM_TRY(make_tmap_2d_u8(&wmap, w->data, 128, w->G * w->NC * w->KC * 128, 128, 128, CU_TENSOR_MAP_SWIZZLE_NONE));
-    static std::atomic<uint64_t> ready{0};  // bit per device: the shared memory opt-in is done
-    const int device = current_device();
-    const uint64_t bit = 1ull << (device & 63);
-    if (!(ready.load(std::memory_order_relaxed) & bit)) {
-        for (auto kern : {fp8_many_kernel<false, false>, fp8_many_kernel<false, true>, fp8_many_kernel<true, false>,
-                          fp8_many_kernel<true, true>}) {
-            AEM_TRY_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kManySmem));
-            cudaFuncAttributes f;
-            AEM_TRY_CUDA(cudaFuncGetAttributes(&f, kern));
-            if (f.numRegs * kManyThreads < kManyFewRegs * 128 + kManyManyRegs * 256) {
-                set_error("fp8_many_kernel: %d registers a thread cannot be shared out", f.numRegs);
-                return AEM_EUNSUPPORTED;
-            }
-        }
-        ready.fetch_or(bit, std::memory_order_relaxed);
-    }
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(2 * std::min<int64_t>(max_pairs(device), row_tiles * ((a.nb + 1) / 2))));
+    cfg.gridDim = dim3(static_cast<unsigned>(2 * std::min<int64_t>(max_pairs(w->device), row_tiles * ((a.nb + 1) / 2))));
     cfg.blockDim = dim3(kManyThreads);
     cfg.dynamicSmemBytes = kManySmem;
     cfg.stream = s;
@@ -935,11 +961,14 @@ aem_status fp8_product(const Fp8Weight* w, const char* what, Fp8Args a, Rows x, 
         set_error("%s: no device error word", what);
         return AEM_ENOMEM;
     }
+    const int64_t n = std::min<int64_t>(a.G, a.M), want = (a.M + n - 1) / n;
+    a.rows = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : 128;
+    // (the groups' sizes are not known here: all as large as the average)
+    const int64_t cost = few_cost(n * ((want + a.rows - 1) / a.rows) * a.nb, a.kb, a.rows, &a.S);
+    const int pairs = want > 64 ? max_pairs(w->device) : 0;
+    const bool many = pairs > 0 && many_cost(n * ((want + kManyTile - 1) / kManyTile) * ((a.nb + 1) / 2), a.kb, pairs) < cost;
+    if (many) a.rows = kManyTile;
     // row tiles at most: n groups with rows have up to n + (M - n) / rows
-    const int64_t n = std::min<int64_t>(a.G, a.M);
-    const int64_t want = (a.M + n - 1) / n;
-    const bool many = want >= 192;
-    a.rows = many ? kManyTile : want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : 128;
     const int64_t slots = a.group_rows ? n + (a.M - n) / a.rows : (a.M + a.rows - 1) / a.rows;
     AEM_REQUIRE((many || slots <= 65535) && slots * ((a.nb + 1) / 2) < (1ll << 31) && a.M < (1ll << 31), "%s: M=%lld rows are too many for one call", what, (long long)a.M);
     void* own = nullptr;
@@ -966,7 +995,7 @@ aem_status fp8_product(const Fp8Weight* w, const char* what, Fp8Args a, Rows x, 
     aem_status st = many           ? launch_many(a, w, x.x, x.ldx, cols, transposed, make, slots, s)
                     : a.rows == 16   ? launch_few<16, false>(a, x.x, x.ldx, cols, transposed, make, slots, s)
                     : a.rows == 32 ? launch_few<32, false>(a, x.x, x.ldx, cols, transposed, make, slots, s)
-                    : a.rows == 64 ? launch_few<64, false>(a, x.x, x.ldx, cols, transposed, make, slots, s)
+                    : a.rows == 64 ? launch_few<64, true>(a, x.x, x.ldx, cols, transposed, make, slots, s)
                                    : launch_few<128, true>(a, x.x, x.ldx, cols, transposed, make, slots, s);
     if (own) cudaFreeAsync(own, s);
     AEM_TRY(st);
