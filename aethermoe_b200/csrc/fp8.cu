@@ -966,7 +966,8 @@ aem_status fp8_product(const Fp8Weight* w, const char* what, Fp8Args a, Rows x, 
     // (the groups' sizes are not known here: all as large as the average)
     const int64_t cost = few_cost(n * ((want + a.rows - 1) / a.rows) * a.nb, a.kb, a.rows, &a.S);
     const int pairs = want > 64 ? max_pairs(w->device) : 0;
-    const bool many = pairs > 0 && many_cost(n * ((want + kManyTile - 1) / kManyTile) * ((a.nb + 1) / 2), a.kb, pairs) < cost;
+    const bool many = pairs > 0 && (a.M > 65535ll * 64 ||  // (more row tiles than a grid of the other kernel has)
+                                    many_cost(n * ((want + kManyTile - 1) / kManyTile) * ((a.nb + 1) / 2), a.kb, pairs) < cost);
     if (many) a.rows = kManyTile;
     // row tiles at most: n groups with rows have up to n + (M - n) / rows
     const int64_t slots = a.group_rows ? n + (a.M - n) / a.rows : (a.M + a.rows - 1) / a.rows;

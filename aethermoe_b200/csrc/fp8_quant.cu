@@ -219,29 +219,44 @@ __global__ void __launch_bounds__(kThreads, sizeof(WT) == 4 ? 3 : 4)
     }
 }
 
-// Once per weight: a tile of 128 k x 128 channels turned round in shared memory.
+// Once per weight: a tile of 128 k x 128 channels turned round, 4 x 4 bytes at a time
+// in registers and the rest in shared memory, where a row of 4-byte pieces of k
+// belongs to a channel.
+template <bool VEC>
 __global__ void __launch_bounds__(kThreads)
     pack_fp8_kernel(const uint8_t* __restrict__ q, const float* __restrict__ scale, int64_t K, int64_t N, int64_t NC,
                     int64_t KC, uint8_t* __restrict__ out, float* __restrict__ out_scale) {
-    __shared__ uint8_t tile[128][132];
+    __shared__ uint32_t tile[128][33];  // [channel][piece of 4 k]
     const int64_t g = blockIdx.x / (NC * KC), t = blockIdx.x % (NC * KC), nc = t / KC, kc = t % KC;
-    for (int i = threadIdx.x; i < 128 * 128; i += kThreads) {
-        const int r = i >> 7, c = i & 127;
-        const int64_t k = kc * 128 + r, n = nc * 128 + c;
-        tile[r][c] = k < K && n < N ? q[(g * K + k) * N + n] : 0;
+    const int n0 = threadIdx.x % 32 * 4;
+    for (int p = threadIdx.x / 32; p < 32; p += kThreads / 32) {
+        uint32_t v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t k = kc * 128 + p * 4 + i, n = nc * 128 + n0;
+            const uint8_t* from = q + (g * K + k) * N + n;
+            v[i] = 0;
+            if (k >= K) continue;
+            if (VEC && n < N) {
+                v[i] = *reinterpret_cast<const uint32_t*>(from);
+            } else if (!VEC) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (n + j < N) v[i] |= static_cast<uint32_t>(from[j]) << (8 * j);
+            }
+        }
+        const uint32_t a = __byte_perm(v[0], v[1], 0x5140), b = __byte_perm(v[2], v[3], 0x5140);
+        const uint32_t c = __byte_perm(v[0], v[1], 0x7362), d = __byte_perm(v[2], v[3], 0x7362);
+        tile[n0][p] = __byte_perm(a, b, 0x5410);
+        tile[n0 + 1][p] = __byte_perm(a, b, 0x7632);
+        tile[n0 + 2][p] = __byte_perm(c, d, 0x5410);
+        tile[n0 + 3][p] = __byte_perm(c, d, 0x7632);
     }
     __syncthreads();
     for (int i = threadIdx.x; i < 128 * 8; i += kThreads) {
-        const int n = i & 127, c = i >> 7;
-        uint32_t v[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            v[j] = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[j] |= static_cast<uint32_t>(tile[c * 16 + j * 4 + e][n]) << (8 * e);
-        }
+        const int n = i >> 3, c = i & 7;
         *reinterpret_cast<uint4*>(out + blockIdx.x * static_cast<int64_t>(kFp8Tile) + n * 128 + ((c ^ (n & 7)) << 4)) =
-            make_uint4(v[0], v[1], v[2], v[3]);
+            make_uint4(tile[n][4 * c], tile[n][4 * c + 1], tile[n][4 * c + 2], tile[n][4 * c + 3]);
     }
     if (threadIdx.x == 0) out_scale[blockIdx.x] = scale[(g * KC + kc) * NC + nc];
 }
@@ -281,7 +296,8 @@ aem_status pack_fp8(const uint8_t* q, const float* scale, int64_t G, int64_t K, 
         return AEM_ENOMEM;
     }
     w->scale = reinterpret_cast<float*>(w->data + tiles * kFp8Tile);
-    pack_fp8_kernel<<<static_cast<unsigned>(tiles), kThreads, 0, s>>>(q, scale, K, N, w->NC, w->KC, w->data, w->scale);
+    auto kern = N % 4 == 0 && reinterpret_cast<uintptr_t>(q) % 4 == 0 ? pack_fp8_kernel<true> : pack_fp8_kernel<false>;
+    kern<<<static_cast<unsigned>(tiles), kThreads, 0, s>>>(q, scale, K, N, w->NC, w->KC, w->data, w->scale);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) {
         free_fp8(w);

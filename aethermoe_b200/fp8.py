@@ -35,6 +35,12 @@ def _blocks(n):
     return -(-n // BLOCK)
 
 
+def _no_gradient(what, x, name):
+    _no_tangent(what, x)
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{what} has no gradient: detach {name} or call it under torch.no_grad()")
+
+
 class Fp8Rows:
     """Rows in blocks of 128: ``q [M, K]`` float8_e4m3fn and ``scale [M,
     ceil(K/128)]`` float32, CUDA tensors; row m, block b stands for
@@ -52,6 +58,7 @@ class Fp8Rows:
             raise ValueError(f"scale must be {want} float32, got {tuple(scale.shape)} {scale.dtype}")
         if scale.device != q.device:
             raise ValueError(f"q and scale are on {q.device} and {scale.device}")
+        _no_gradient("Fp8Rows", scale, "scale")
         self.q, self.scale, self.shape, self.device = q, scale, q.shape, q.device
 
     def record_stream(self, stream):
@@ -90,12 +97,6 @@ def _quantize(x, s):
     return Fp8Rows(q, scale)
 
 
-def _no_gradient(what, x, name):
-    _no_tangent(what, x)
-    if x.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError(f"{what} has no gradient: detach {name} or call it under torch.no_grad()")
-
-
 def quantize_fp8(x, stream=None):
     """``Fp8Rows`` of ``x [M, K]`` (float32 or bfloat16): blocks of 128 along a row share
     ``scale = max(amax / 448, 2^-126)``, ``q = e4m3(x / scale)``.  No gradient: the
@@ -129,7 +130,7 @@ def quantize_fp8_weight(w, stream=None):
 class Fp8Weight:
     """Packed e4m3 weight groups: ``q [K, N]`` or ``[G, K, N]`` float8_e4m3fn and
     ``scale [(G,) ceil(K/128), ceil(N/128)]`` float32.  CUDA tensors are packed on the
-    device, in stream order, CPU tensors through ``aem_fp8weight_pack`` onto
+    device (the call waits for it), CPU tensors through ``aem_fp8weight_pack`` onto
     ``device``."""
 
     def __init__(self, q, scale, device=0, stream=None):
@@ -143,14 +144,15 @@ class Fp8Weight:
             raise ValueError(f"scale must be {want} float32, got {tuple(scale.shape)} {scale.dtype}")
         if q.device.type not in ("cpu", "cuda") or scale.device != q.device:
             raise ValueError(f"q and scale must be on one CUDA device or the CPU, got {q.device} and {scale.device}")
-        if scale.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("Fp8Weight has no gradient: detach scale")
+        _no_gradient("Fp8Weight", scale, "scale")
         h = ctypes.c_void_p()
         if q.is_cuda:
             def pack(q, scale, s):
                 q, scale = q.contiguous(), scale.contiguous()  # on the call's stream
                 _lib.check(_lib.lib().aem_fp8weight_pack_device(q.data_ptr(), scale.data_ptr(), g, k, n, s,
                                                                 ctypes.byref(h)), "aem_fp8weight_pack_device")
+                # any stream may use the weight from here on
+                torch.cuda.current_stream(q.device).synchronize()
             _on(stream, pack, (q, scale), (q, scale))
             device = q.device.index
         else:

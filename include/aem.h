@@ -488,7 +488,9 @@ aem_status aem_fp8weight_shape(aem_fp8weight_t w, int64_t* G, int64_t* K, int64_
  * a block's sum on the tensor cores (e4m3 operands, float32 accumulators), the
  * scales and the sum over the blocks in float32.  x is either float32 or bf16,
  * rows ldx apart, and quantised as aem_quantize_fp8 does (x_scale NULL, lds 0),
- * or AEM_E4M3 rows that it wrote, with their scales (ldx bytes and lds as there).
+ * or AEM_E4M3 rows that it wrote, with their scales (ldx bytes and lds as there; all
+ * lds floats of a row may be read).  The product of two scales should be a normal
+ * number: one that overflows makes an infinity or a NaN of its block.
  * transposed != 0 multiplies by the transposed weight instead, x [M, N] -> out
  * [M, K]: the gradient of the rows from the same packed weight, x the gradient of
  * the product.  The workspace holds float32 or bf16 rows in their quantised form:
