@@ -70,8 +70,10 @@ def plain_route(x, k, score="softmax", bias=None, groups=1, top_groups=1, group_
 
 
 def span(x):
-    x = np.where(np.isfinite(x), x, np.nan)
-    return np.nan_to_num(np.nanmax(x, 1, keepdims=True) - np.nanmin(x, 1, keepdims=True))
+    """Range of a row's finite logits."""
+    on = np.isfinite(x)
+    top, low = np.where(on, x, -np.inf).max(1, keepdims=True), np.where(on, x, np.inf).min(1, keepdims=True)
+    return np.where(on.any(1, keepdims=True), top - low, 0.0)
 
 
 def check_route(logits, ids, weights, how):
