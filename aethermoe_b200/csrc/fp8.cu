@@ -375,13 +375,17 @@ __global__ void __launch_bounds__(kFewThreads, ALONE ? 1 : 2)
 //   warp 1      issues the pair's MMAs (M = 256, N = 256, K = 32) in CTA 0, four a
 //               block, into one of two accumulators that fill tensor memory
 //   warps 4-11  thread = row = TMEM lane; warps 4-7 have the first 128 columns, 8-11
-//               the rest.  A block's accumulator comes back 32 columns at a time and
+//               the rest.  A block's accumulator comes back 16 columns at a time and
 //               factor * sum is added to 128 registers; at the tile's end these leave
 //               through shared memory in bulk copies of whole pieces of rows.
-// 4096 x 4096 x 14336, rows quantised before: 225 us, 2.1 PFLOP/s.  The MMAs alone take
-// 155; what bounds it is the warps that take the sums back, 830 cycles a block where
-// the MMAs take 512 (264 of them multiply-adds).  Accumulators of half the width, four
-// of them, wait twice as often: 258 us.
+// 4096 x 4096 x 14336, rows quantised before: 218 to 224 us, 2.2 PFLOP/s.  The MMAs with
+// their barriers alone take 155; what bounds it is the warps that take the sums back,
+// about 800 cycles a block where the MMAs take 512 (264 are multiply-adds of the two
+// warps that share a sub-core), and what writes 117 MB of out takes from the loads (16
+// us).  Accumulators of half the width, four of them, wait twice as often: 261 us.
+// The registers decide: 128 sums, 32 columns under way, and every variable more that
+// was kept through the loop was moved about in it (two accumulators' worth of columns
+// under way 238 us, pointers kept 245, one float4 of scales 225 instead of 218).
 // Every wait is bounded; a timeout sets the error word and ends all roles of both CTAs.
 constexpr int kManyThreads = 12 * 32, kManyStages = 4, kManyTile = 256;
 constexpr int kManyStage = 2 * kFp8Tile;                      // of one CTA
@@ -470,11 +474,11 @@ __device__ __forceinline__ bool pair_wait(uint32_t bar, uint32_t parity, bool do
     }
 }
 
-// 32 columns: acc += f * d.  (Two columns an instruction: beside 128 single ones a
+// 16 columns: acc += f * d.  (Two columns an instruction: beside 128 single ones a
 // block, the MMAs take half as long again.)
-__device__ __forceinline__ void add_columns(float* acc, float f, const uint32_t (&d)[32]) {
+__device__ __forceinline__ void add_columns(float* acc, float f, const uint32_t (&d)[16]) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 2)
+    for (int i = 0; i < 16; i += 2)
         asm volatile("{\n.reg .b64 a, f, v;\nmov.b64 a, {%0, %1};\nmov.b64 f, {%2, %2};\nmov.b64 v, {%3, %4};\n"
                      "fma.rn.f32x2 a, f, v, a;\nmov.b64 {%0, %1}, a;\n}"
                      : "+f"(acc[i]), "+f"(acc[i + 1])
@@ -685,23 +689,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads, 1)
                     ok &= pair_wait(sb + kManyDoneAt + 8 * b, used >> b & 1, seen, sb, a.err);
                     used ^= 1u << b;
                     tc_fence_after();
+                    uint32_t d[2][16];  // 16 columns on their way while the last 16 are added
+                    tc_ld_32x32b_x16(at + b * 256, d[0]);
                     float f;
+                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(mine + (u & 4) * 1024 + (u & 3) * 4) : "memory");
+                    f *= __shfl_sync(~0u, held, u & 31);
 #pragma unroll
-                    for (int c = 0; c < 128; c += 32) {
-                        uint32_t d[32];
-                        tc_ld_32x32b_x32(at + b * 256 + c, d);
-                        if (c == 0) {
-                            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(mine + (u & 4) * 1024 + (u & 3) * 4) : "memory");
-                            f *= __shfl_sync(~0u, held, u & 31);
-                        }
+                    for (int c = 0; c < 8; ++c) {
                         tc_wait_ld();
-                        if (c == 96) {
+                        if (c < 7) {
+                            tc_ld_32x32b_x16(at + b * 256 + (c + 1) * 16, d[(c + 1) & 1]);
+                        } else {
                             tc_fence_before();
                             __syncwarp();
                             arrive_first_lane(free_at + b * 8);
                             seen = bar_test(sb + kManyDoneAt + 8 * (b ^ 1), used >> (b ^ 1) & 1);
                         }
-                        add_columns(acc + c, f, d);
+                        add_columns(acc + c * 16, f, d[c & 1]);
                     }
                 };
                 int u = 0;

@@ -119,12 +119,14 @@ struct Rank<double> {
     using type = unsigned long long;
 };
 
-// A float32 key's distance from the real one: the score's relative error is
-// under 2^-19 (exp: 2 ulp, its argument: |x - m| 2^-24 for |x - m| <= 32, further
-// down the score is under 2^-46 and the last term holds it; the sum of 256: 11
-// halves of an ulp; the quotient 2), and the sum with the bias is rounded once.
-__device__ __forceinline__ float slack(float score, float key) {
-    return fmaf(0x1p-19f, score, fmaf(0x1p-23f, fabsf(key), 0x1p-64f));
+// A float32 key's distance from the real one.  A sigmoid's relative error is under
+// 2^-22 (exp: 1 ulp, the sum and the quotient half an ulp each).  A softmax's score
+// has that of its exponential, whose argument rounds by |x - m| 2^-24, of the sum of
+// 256 (13 additions) and of two products: (|x - m| + 19) 2^-24, so under 2^-18 for
+// |x - m| <= 45, and further down it is under 2^-64 altogether.  The sum with the bias
+// is rounded once.
+__device__ __forceinline__ float slack(bool sigmoid, float score, float key) {
+    return fmaf(sigmoid ? 0x1p-21f : 0x1p-18f, score, fmaf(0x1p-23f, fabsf(key), 0x1p-64f));
 }
 
 __device__ __forceinline__ float exp_of(float v) { return expf(v); }
@@ -311,7 +313,7 @@ __device__ __forceinline__ bool extract(const RouteArgs& a, bool on, RouteShared
         if constexpr (CERT) {
             const int at = __shfl_sync(~0u, id, owner);
             const float score = sh.take[w][row * LANES * kV + at], k = value_of(m);
-            if (j > 0 && m) near |= !(last_key - k > slack(score, k) + slack(last_score, last_key));
+            if (j > 0 && m) near |= !(last_key - k > slack(a.sigmoid, score, k) + slack(a.sigmoid, last_score, last_key));
             last_key = k;
             last_score = score;
         }
@@ -421,7 +423,7 @@ __global__ void __launch_bounds__(kRouteThreads, 4) route_kernel(const RouteArgs
         }
         top = seg_max<LANES>(top);
         largest = seg_max<LANES>(largest);
-        e = 4.0f * slack(top, largest) + 0x1p-22f * largest;
+        e = 4.0f * slack(a.sigmoid, top, largest) + 0x1p-22f * largest;
     }
     bool near = false, on = true;
     if constexpr (ANY) {

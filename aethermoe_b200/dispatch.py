@@ -93,7 +93,10 @@ class TokenOrder:
 
 try:  # the handle alone, without a Stream object (3 us of a call's 15 on the host)
     _stream_handle = torch._C._cuda_getCurrentRawStream
+    _current_device = torch._C._cuda_getDevice  # (there is a CUDA tensor: nothing to initialise)
 except AttributeError:
+    _current_device = torch.cuda.current_device
+
     def _stream_handle(device):
         return torch.cuda.current_stream(device).cuda_stream
 
@@ -108,7 +111,7 @@ def _on(stream, fn, tensors, args):
     for t in tensors:
         if t is not None and t.device != dev:
             raise ValueError(f"tensors are on {dev} and {t.device}")
-    if stream is None and torch.cuda.current_device() == dev.index:
+    if stream is None and _current_device() == dev.index:
         return fn(*args, _stream_handle(dev.index))
     if stream is None:
         stream = torch.cuda.current_stream(dev)
