@@ -9,7 +9,9 @@
 // as one multiply-add per element.
 //
 // fp8_few_kernel: weights are the MMA's 128 rows (the channels), tokens its
-// columns; the weight stream is what bounds few rows.
+// columns; the weight stream is what bounds few rows.  One bf16 row, 4096 x 14336:
+// 15.4 us with its quantisation, 13.9 without, 4.2 TB/s of weights; 64 rows 17.8 us;
+// 384 rows of 64 experts of 2048 x 1408 36 us, 5.1 TB/s.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -378,14 +380,14 @@ __global__ void __launch_bounds__(kFewThreads, ALONE ? 1 : 2)
 //               the rest.  A block's accumulator comes back 16 columns at a time and
 //               factor * sum is added to 128 registers; at the tile's end these leave
 //               through shared memory in bulk copies of whole pieces of rows.
-// 4096 x 4096 x 14336, rows quantised before: 218 to 224 us, 2.2 PFLOP/s.  The MMAs with
+// 4096 x 4096 x 14336, rows quantised before: 220 us, 2.2 PFLOP/s.  The MMAs with
 // their barriers alone take 155; what bounds it is the warps that take the sums back,
 // about 800 cycles a block where the MMAs take 512 (264 are multiply-adds of the two
 // warps that share a sub-core), and what writes 117 MB of out takes from the loads (16
 // us).  Accumulators of half the width, four of them, wait twice as often: 261 us.
 // The registers decide: 128 sums, 32 columns under way, and every variable more that
 // was kept through the loop was moved about in it (two accumulators' worth of columns
-// under way 238 us, pointers kept 245, one float4 of scales 225 instead of 218).
+// under way 238 us, pointers kept 245, one float4 of scales 225 instead of 220).
 // Every wait is bounded; a timeout sets the error word and ends all roles of both CTAs.
 constexpr int kManyThreads = 12 * 32, kManyStages = 4, kManyTile = 256;
 constexpr int kManyStage = 2 * kFp8Tile;                      // of one CTA

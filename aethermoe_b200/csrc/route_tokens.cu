@@ -14,8 +14,8 @@
 // on their error; wherever two keys that decide the order (neighbours among the
 // k + 1 largest, the last group kept and the first dropped) are nearer than their
 // bounds, the warp chooses again with keys in 64 bits.  With normally distributed
-// logits that is a row in some hundred, and costs 16384 rows of 256 about 5 us.
-// Logits themselves need no bound.
+// logits and 256 experts, top-8, that is a row in 2400 (sigmoid with a bias), and a
+// call with such a row takes 5 us longer.  Logits themselves need no bound.
 //
 // A row lies across LANES lanes, 8 neighbouring experts a lane, so a lane's order
 // is the experts' and up to 32 rows share a warp.  A lane sorts its experts once
@@ -23,7 +23,10 @@
 // first ones, and the lane that had it moves on to its next (looking through all 8
 // again for every choice took 29 us where this takes 24: 16384 rows of 256, top-8).
 // Groups of whole lanes take their two largest from the sorted lists; others are
-// read through shared memory.  What has to be moved is T*E logits and 8 T*k bytes.
+// read through shared memory.  What has to be moved is T*E logits and 8 T*k bytes,
+// but a choice of k costs k warp-wide maxima, and those bound it.  256 float32 logits,
+// top-8: 1 row 3.8 us softmax and 5.5 sigmoid with bias and 8 groups, 16383 rows 24
+// and 44 us, 262144 rows 310 and 498 us (0.9 and 0.6 TB/s of logits).
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -52,7 +55,7 @@ struct RouteArgs {
     float scale;
     int E, k, groups, top_groups, group_top, size;  // size: experts of a group
     int size_inv, k_inv;                            // n * inv >> 16 == n / (size, k) for n < 256
-    int sigmoid, renorm, vec, ovec;
+    int sigmoid, renorm, vec, bvec, ovec;  // rows, the bias, gradients can be moved in 16 bytes
     int* err;
 };
 
@@ -119,18 +122,26 @@ struct Rank<double> {
     using type = unsigned long long;
 };
 
-// A float32 key's distance from the real one.  A sigmoid's relative error is under
-// 2^-22 (exp: 1 ulp, the sum and the quotient half an ulp each).  A softmax's score
-// has that of its exponential, whose argument rounds by |x - m| 2^-24, of the sum of
-// 256 (13 additions) and of two products: (|x - m| + 19) 2^-24, so under 2^-18 for
-// |x - m| <= 45, and further down it is under 2^-64 altogether.  The sum with the bias
-// is rounded once.
+// A float32 key's distance from the real one.  A sigmoid's relative error, from
+// exp's 2 ulp (at most 2^-22, which reach the quotient by the factor 1 - s), the sum's
+// 2^-24 and the quotient's, is under 2^-24 (2 + 4 (1 - s)).  A softmax's score has that
+// of its exponential, whose argument rounds by |x - m| 2^-24, of the sum of 256 (13
+// additions) and of two products: (|x - m| + 19) 2^-24, so under 2^-18 for |x - m| <=
+// 45, and further down it is under 2^-64 altogether.  The sum with the bias is rounded
+// once.  One or two hundredths more cover the bound's own roundings.
 __device__ __forceinline__ float slack(bool sigmoid, float score, float key) {
-    return fmaf(sigmoid ? 0x1p-21f : 0x1p-18f, score, fmaf(0x1p-23f, fabsf(key), 0x1p-64f));
+    const float by = sigmoid ? fmaf(score, -0x1p-22f, 6.02f * 0x1p-24f) : 0x1p-18f;
+    return fmaf(by, score, fmaf(1.01f * 0x1p-24f, fabsf(key), 0x1p-64f));
 }
 
 __device__ __forceinline__ float exp_of(float v) { return expf(v); }
 __device__ __forceinline__ double exp_of(double v) { return exp(v); }
+// (1 <= b <= 2; a reciprocal of 2 ulp, and a step that takes the quotient's rest)
+__device__ __forceinline__ float quotient(float a, float b) {
+    const float r = __fdividef(1.0f, b), q = a * r;
+    return fmaf(fmaf(-q, b, a), r, q);
+}
+__device__ __forceinline__ double quotient(double a, double b) { return a / b; }
 
 // Scores of a lane's experts; a row without any finite logit has zeros.
 template <int LANES, typename F>
@@ -139,7 +150,7 @@ __device__ __forceinline__ void scores(const float (&x)[kV], bool sigmoid, F (&s
 #pragma unroll
         for (int i = 0; i < kV; ++i) {
             const F t = exp_of(-fabs(static_cast<F>(x[i])));
-            s[i] = (x[i] < 0.0f ? t : F(1)) / (F(1) + t);
+            s[i] = quotient(x[i] < 0.0f ? t : F(1), F(1) + t);
         }
         return;
     }
@@ -349,12 +360,15 @@ __device__ __forceinline__ void load_row(const RouteArgs& a, int64_t t, int e0, 
         if (e0 + i < a.E) x[i] = static_cast<float>(p[i]);
 }
 
-// The choice again with keys in 64 bits (rare, and kept apart from the registers of
-// the ordinary path).
-template <int LANES>
-__device__ __noinline__ void choose_exactly(const RouteArgs& a, const float (&x)[kV], RouteShared& sh, double* values) {
+// The choice again with keys in 64 bits.  It is rare and apart from the registers of
+// the ordinary path, so it fetches the logits again: handed over they would lie in
+// memory for every warp (262144 x 256 sigmoid with a bias: 407 us, so 397).
+template <int LANES, typename LT>
+__device__ __noinline__ void choose_exactly(const RouteArgs& a, int64_t t0, RouteShared& sh, double* values) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, sub = lane % LANES, row = lane / LANES, e0 = sub * kV;
     const unsigned segment = (LANES == 32 ? ~0u : (1u << LANES) - 1) << (row * LANES);
+    float x[kV];
+    load_row<LT>(a, t0 + row, e0, x);
     double s[kV], key[kV], by[kV];
     scores<LANES>(x, a.sigmoid, s);
 #pragma unroll
@@ -404,12 +418,19 @@ __global__ void __launch_bounds__(kRouteThreads, 4) route_kernel(const RouteArgs
     const bool scored = !of_logits || a.bias || two;
     if (scored) scores<LANES>(x, a.sigmoid, s);
     bool nan = false;  // a NaN among the scores is one in all of them
+    float b[kV] = {};
+    if (a.bvec && e0 < a.E) {
+        const float4 u = *reinterpret_cast<const float4*>(a.bias + e0), v = *reinterpret_cast<const float4*>(a.bias + e0 + 4);
+        b[0] = u.x, b[1] = u.y, b[2] = u.z, b[3] = u.w, b[4] = v.x, b[5] = v.y, b[6] = v.z, b[7] = v.w;
+    } else if (a.bias) {
+#pragma unroll
+        for (int i = 0; i < kV; ++i) b[i] = e0 + i < a.E ? a.bias[e0 + i] : 0.0f;
+    }
 #pragma unroll
     for (int i = 0; i < kV; ++i) {
         if (!scored) s[i] = 0.0f;
-        const float b = a.bias && e0 + i < a.E ? a.bias[e0 + i] : 0.0f;
-        const bool none = x[i] == -INFINITY || b == -INFINITY;
-        key[i] = none ? -INFINITY : a.bias ? s[i] + b : x[i];
+        const bool none = x[i] == -INFINITY || b[i] == -INFINITY;
+        key[i] = none ? -INFINITY : a.bias ? s[i] + b[i] : x[i];
         nan |= s[i] != s[i];
     }
     const bool sure = !a.bias && !two;  // keys are the logits themselves
@@ -469,7 +490,7 @@ __global__ void __launch_bounds__(kRouteThreads, 4) route_kernel(const RouteArgs
         near |= extract<LANES, true>(a, on, sh);
     else
         extract<LANES, false>(a, on, sh);
-    if (!sure && __any_sync(~0u, near)) choose_exactly<LANES>(a, x, sh, ANY ? gsh.value[w] : sh.value[w]);
+    if (!sure && __any_sync(~0u, near)) choose_exactly<LANES, LT>(a, t0, sh, ANY ? gsh.value[w] : sh.value[w]);
     if (of_logits && a.bias) {  // the scores have been compared
         __syncwarp();
 #pragma unroll
@@ -510,7 +531,8 @@ __global__ void __launch_bounds__(kRouteThreads, 4) route_kernel(const RouteArgs
 // slot: it leaves what the row's sums need in shared memory, takes the sums from
 // there in the slots' order, and leaves its term at its expert; of slots with the
 // same expert the first one adds the others' terms.  Then every lane writes its own 8
-// experts.
+// experts.  Memory bound: 262144 rows of 256 float32, top-8, with the sums over all
+// experts 173 us (3.1 TB/s), over the chosen ones alone 146 us.
 template <int LANES, typename LT>
 __global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const RouteArgs a) {
     __shared__ int32_t s_ids[kRouteWarps][256];
@@ -717,6 +739,7 @@ aem_status aem_route_tokens(const aem_route_config* config, const void* logits, 
     AEM_REQUIRE(logits && ids && weights, "aem_route_tokens: NULL buffer");
     aem::RouteArgs a = aem::route_args(config, logits, dtype, ld, T, E);
     a.bias = bias;
+    a.bvec = bias && E % aem::kV == 0 && reinterpret_cast<uintptr_t>(bias) % 16 == 0;
     a.ids = ids;
     a.weights = weights;
     aem_status st = AEM_OK;

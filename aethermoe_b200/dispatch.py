@@ -85,6 +85,9 @@ class TokenOrder:
             self._starts = self._buf.as_strided((self.num_experts + 1,), (1,), 2 * self.shape[0] * self.shape[1])
         return self._starts
 
+    def get_device(self):
+        return self.device.index if self.device.type == "cuda" else -1
+
     def record_stream(self, stream):
         for t in (self._buf, self._starts, self._row_of, self._unit_of):
             if t is not None:
@@ -105,14 +108,15 @@ def _on(stream, fn, tensors, args):
     """``fn(*args, stream handle)`` with the tensors' device current and ``stream``
     (default: that device's current stream) as its current stream, so that
     outputs and scratch belong to the stream that uses them."""
-    dev = tensors[0].device
-    if dev.type != "cuda":
-        raise ValueError(f"tensors must be on a CUDA device, got {dev}")
+    at = tensors[0].get_device()  # the index alone, without a device object
+    if at < 0:
+        raise ValueError(f"tensors must be on a CUDA device, got {tensors[0].device}")
     for t in tensors:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors are on {dev} and {t.device}")
-    if stream is None and _current_device() == dev.index:
-        return fn(*args, _stream_handle(dev.index))
+        if t is not None and t.get_device() != at:
+            raise ValueError(f"tensors are on {tensors[0].device} and {t.device}")
+    if stream is None and _current_device() == at:
+        return fn(*args, _stream_handle(at))
+    dev = tensors[0].device
     if stream is None:
         stream = torch.cuda.current_stream(dev)
     elif stream.device != dev:

@@ -59,7 +59,14 @@ class Fp8Rows:
         if scale.device != q.device:
             raise ValueError(f"q and scale are on {q.device} and {scale.device}")
         _no_gradient("Fp8Rows", scale, "scale")
+        self._set(q, scale)
+
+    def _set(self, q, scale):
         self.q, self.scale, self.shape, self.device = q, scale, q.shape, q.device
+        return self
+
+    def get_device(self):
+        return self.q.get_device()
 
     def record_stream(self, stream):
         self.q.record_stream(stream)
@@ -94,7 +101,7 @@ def _quantize(x, s):
     q, scale, ldq, lds = _new_rows(m, k, x)
     _lib.check(_lib.lib().aem_quantize_fp8(x.data_ptr(), _DT[x.dtype], ldx, m, k, q.data_ptr(), ldq,
                                            scale.data_ptr(), lds, s), "aem_quantize_fp8")
-    return Fp8Rows(q, scale)
+    return Fp8Rows.__new__(Fp8Rows)._set(q, scale)
 
 
 def quantize_fp8(x, stream=None):
@@ -194,7 +201,7 @@ def _product(x, w, starts, group, transposed, relu, zero_rest, out_dtype, out, s
         default = x.dtype
     if not w.handle:
         raise ValueError("the weight is closed")
-    if like.device.index != w.device:
+    if like.get_device() != w.device:
         raise ValueError(f"x is on {like.device}, the weight on cuda:{w.device}")
     given = out
     out, ldo = _output(out, (m, n), out_dtype or (default if out is None else out.dtype), like)
