@@ -378,16 +378,19 @@ __global__ void __launch_bounds__(kFewThreads, ALONE ? 1 : 2)
 //               block, into one of two accumulators that fill tensor memory
 //   warps 4-11  thread = row = TMEM lane; warps 4-7 have the first 128 columns, 8-11
 //               the rest.  A block's accumulator comes back 16 columns at a time and
-//               factor * sum is added to 128 registers; at the tile's end these leave
-//               through shared memory in bulk copies of whole pieces of rows.
+//               factor * sum is added to 128 registers; at the tile's end these are
+//               left in shared memory
+//   warps 2, 3  write them from there, whole rows of 128 columns, under the next tile
+//               (a bulk copy of each row by the summing warps held those up for 3200
+//               cycles a tile, 90 a copy: 98304 x 2048 x 1408 by 64 experts 342 us, so 309)
 // 4096 x 4096 x 14336, rows quantised before: 220 us, 2.2 PFLOP/s.  The MMAs with
 // their barriers alone take 155; what bounds it is the warps that take the sums back,
-// about 800 cycles a block where the MMAs take 512 (264 are multiply-adds of the two
-// warps that share a sub-core), and what writes 117 MB of out takes from the loads (16
-// us).  Accumulators of half the width, four of them, wait twice as often: 261 us.
+// about 700 cycles a block where the MMAs take 512 (264 are multiply-adds of the two
+// warps that share a sub-core), and a tile's first and last block, which overlap with
+// no other's MMAs.  Accumulators of half the width, four of them, wait twice as often: 261 us.
 // The registers decide: 128 sums, 32 columns under way, and every variable more that
 // was kept through the loop was moved about in it (two accumulators' worth of columns
-// under way 238 us, pointers kept 245, one float4 of scales 225 instead of 220).
+// under way 238 us, the next block's first columns 231, pointers kept 245, one float4 of scales 225 instead of 220).
 // Every wait is bounded; a timeout sets the error word and ends all roles of both CTAs.
 constexpr int kManyThreads = 12 * 32, kManyStages = 4, kManyTile = 256;
 constexpr int kManyStage = 2 * kFp8Tile;                      // of one CTA
@@ -406,9 +409,15 @@ constexpr int kManyFullAt = kManyScalesAt + kManyScales;             // [stages]
 constexpr int kManyEmptyAt = kManyFullAt + 8 * kManyStages;          // [stages]
 constexpr int kManyDoneAt = kManyEmptyAt + 8 * kManyStages;          // [2]: an accumulator's sums are there
 constexpr int kManyFreeAt = kManyDoneAt + 16;                        // [2]: they have been read; used in CTA 0
-constexpr int kManySlotAt = kManyFreeAt + 16, kManyAbortAt = kManySlotAt + 4;
+constexpr int kManyStagedAt = kManyFreeAt + 16;                      // [2]: results of 128 columns lie in shared memory
+constexpr int kManyCopiedAt = kManyStagedAt + 16;                    // [2]: they have been read from there
+constexpr int kManySlotAt = kManyCopiedAt + 16, kManyAbortAt = kManySlotAt + 4;
 constexpr int kManyRowsAt = kManySlotAt + 16, kManyTilesAt = kManyRowsAt + (AEM_MAX_EXPERTS + 1) * 4;
-constexpr int kManySmem = 1024 + kManyTilesAt + (AEM_MAX_EXPERTS + 1) * 4;
+// A pair's first tiles, looked up side by side at the start: three roles ask for each
+// one, and of 64 groups a search takes some 500 cycles.
+constexpr int kManyKept = 256, kManyKeptAt = (kManyTilesAt + (AEM_MAX_EXPERTS + 1) * 4 + 15) / 16 * 16;
+constexpr int kManySmem = 1024 + kManyKeptAt + kManyKept * 16;
+static_assert(kManyKept <= kManyThreads && kManySmem <= 227 * 1024, "a thread looks a tile up; shared memory");
 
 __device__ __forceinline__ int lds_int(uint32_t at) {
     int v;
@@ -497,7 +506,10 @@ struct ManyTile {
     int m0, rows;  // first row and number of rows
     int col;       // first 128-block of columns
 };
-__device__ __forceinline__ ManyTile many_tile(const Fp8Args& a, int t, uint32_t sb) {
+struct ManyKept {
+    int m0, rows, col, g;  // the same with the group
+};
+__device__ __forceinline__ ManyKept find_tile(const Fp8Args& a, int t, uint32_t sb) {
     int lo = 0, hi = a.G;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -507,12 +519,23 @@ __device__ __forceinline__ ManyTile many_tile(const Fp8Args& a, int t, uint32_t 
     const int r = t - first, n = (lds_int(sb + kManyTilesAt + lo * 4 + 4) - first) / nc;
     const int band = r / (kBand * nc), in = r - band * kBand * nc, high = min(kBand, n - band * kBand);
     const int row = lds_int(sb + kManyRowsAt + lo * 4), end = lds_int(sb + kManyRowsAt + lo * 4 + 4);
-    ManyTile o;
+    ManyKept o;
     o.col = in / high * 2;
     o.m0 = row + (band * kBand + in % high) * kManyTile;
     o.rows = min(kManyTile, end - o.m0);
-    o.t0 = (a.group_rows ? lo : a.group) * a.group_tiles;
+    o.g = lo;
     return o;
+}
+// Tile t, the pair's turn-th.
+__device__ __forceinline__ ManyTile many_tile(const Fp8Args& a, int t, int turn, uint32_t sb) {
+    ManyKept k;
+    if (turn < kManyKept)
+        asm volatile("ld.volatile.shared.v4.s32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(k.m0), "=r"(k.rows), "=r"(k.col), "=r"(k.g)
+                     : "r"(sb + kManyKeptAt + turn * 16));
+    else
+        k = find_tile(a, t, sb);
+    return {(a.group_rows ? k.g : a.group) * a.group_tiles, k.m0, k.rows, k.col};
 }
 
 template <bool TRANS, bool BF16>
@@ -535,6 +558,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads, 1)
         for (int i = 0; i < 2; ++i) {
             init(kManyDoneAt + 8 * i, 1);
             init(kManyFreeAt + 8 * i, 16);  // the warps of both CTAs that read it
+            init(kManyStagedAt + 8 * i, 4);
+            init(kManyCopiedAt + 8 * i, 32);
         }
         sts_int(sb + kManyAbortAt, 0);
         fence_barrier_init();
@@ -574,10 +599,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads, 1)
     }
     tc_fence_before();
     __syncthreads();
+    const int total = lds_int(sb + kManyTilesAt + a.G * 4);
+    if (const int i = threadIdx.x; i < kManyKept && pair + i * pairs < total) {
+        const ManyKept k = find_tile(a, pair + i * pairs, sb);
+        asm volatile("st.volatile.shared.v4.s32 [%0], {%1, %2, %3, %4};" ::"r"(sb + kManyKeptAt + i * 16), "r"(k.m0),
+                     "r"(k.rows), "r"(k.col), "r"(k.g)
+                     : "memory");
+    }
+    __syncthreads();
     cluster_sync();  // both CTAs' barriers are there before any remote arrival
     tc_fence_after();
     const uint32_t tmem = static_cast<uint32_t>(lds_int(sb + kManySlotAt));
-    const int total = lds_int(sb + kManyTilesAt + a.G * 4);
 
     if (w < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kManyFewRegs));
@@ -596,8 +628,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads, 1)
             uint32_t phase = 0;
             int issued = 0;
             bool ok = true;
-            for (int t = pair; ok && t < total; t += pairs) {
-                const ManyTile z = many_tile(a, t, sb);
+            for (int t = pair, turn = 0; ok && t < total; t += pairs, ++turn) {
+                const ManyTile z = many_tile(a, t, turn, sb);
                 // an odd number of blocks: the last pair's second half takes the last block
                 // again, its results are not stored
                 int tile = static_cast<int>((z.t0 + min(z.col + static_cast<int>(cta), a.nb - 1) * a.out_step) * 128);
@@ -623,6 +655,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads, 1)
                     for (int n = 0; n < 1 << 14 && !bar_try(sb + kManyFullAt + 8 * (i % kManyStages),
                                                             i / kManyStages & 1); ++n) {
                     }
+        } else if (w >= 2) {
+            // results of a tile's first or last 128 columns, from shared memory to out
+            const int half = w - 2;
+            constexpr int ES = BF16 ? 2 : 4, PER = 256 / ES;  // columns of a piece
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int t = pair, turn = 0; ok && t < total; t += pairs, ++turn) {
+                const ManyTile z = many_tile(a, t, turn, sb);
+                const int64_t n = (z.col + half) * 128ll;
+                const int left = static_cast<int>(min(static_cast<int64_t>(128), a.N - n));
+                if (left <= 0 || !(a.ovec16 && left * ES % 16 == 0)) continue;
+                const int first = static_cast<int>(cta) * 128 + (lane >> 4);
+                const int rows = min(128, z.rows - static_cast<int>(cta) * 128);
+                uint8_t* to = static_cast<uint8_t*>(a.out) + ((z.m0 + first) * a.ldo + n) * ES + (lane & 15) * 16;
+                const uint32_t piece = sb + kManyOutAt + (half * 128 + (lane >> 4)) * kManyPitch + (lane & 15) * 16;
+                const int64_t step = 2 * a.ldo * ES;
+                for (int c = 0; c < left; c += PER) {
+                    if (!(ok = pair_wait(sb + kManyStagedAt + 8 * half, phase, false, sb, a.err))) break;
+                    phase ^= 1;
+                    const bool inside = c + (lane & 15) * (16 / ES) < left;
+                    uint8_t* dst = to + c * ES;
+                    // two whole rows at a time, the next two on their way
+#pragma unroll 1
+                    for (int r = 0; r < rows; r += 4) {
+                        uint32_t v[2][4];
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+                            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                         : "=r"(v[k][0]), "=r"(v[k][1]), "=r"(v[k][2]), "=r"(v[k][3])
+                                         : "r"(piece + (r + 2 * k) * kManyPitch)
+                                         : "memory");
+#pragma unroll
+                        for (int k = 0; k < 2; ++k, dst += step)
+                            if (inside && r + 2 * k + (lane >> 4) < rows)
+                                *reinterpret_cast<uint4*>(dst) = make_uint4(v[k][0], v[k][1], v[k][2], v[k][3]);
+                    }
+                    __syncwarp();
+                    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(sb + kManyCopiedAt + 8 * half)
+                                 : "memory");
+                }
+            }
         } else if (w == 1 && cta == 0) {
             constexpr uint32_t idesc = idesc_e4m3_f32(256, 256, false, TRANS);
             auto commit = [&](uint32_t bar) {  // to the barrier's place in both CTAs
@@ -666,26 +739,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads, 1)
         const uint32_t free_at = cluster_address(sb + kManyFreeAt, 0);
         uint32_t used = 0;
         bool ok = true, seen = false;  // seen: the next block's sums are there
+        // where the scales of the thread's row (rows behind the tile's compute something
+        // that nobody stores) and of the warp's columns begin
+        auto scales_of = [&](int t, int turn, const float*& xs, const float*& ws) {
+            const ManyTile z = many_tile(a, t, turn, sb);
+            xs = a.xs + min(static_cast<int64_t>(z.m0) + static_cast<int>(cta) * 128 + (w & 3) * 32 + lane, a.M - 1) * a.lds;
+            ws = a.ws + z.t0 + min(z.col + ((w - 4) >> 2), a.nb - 1) * a.out_step;
+        };
+        // the row's scales of blocks u to u + 3 on their way to shared memory
+        auto fetch = [&](const float* xs, int u) {
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 16;\ncp.async.commit_group;" ::"r"(mine + (u & 4) * 1024),
+                         "l"(xs + u)
+                         : "memory");
+        };
+        float held = 0.0f;  // the weight scales of 32 blocks, one a lane
+        // a tile's first scales, asked for before the last tile's results are written
+        auto fetch_first = [&](int t, int turn) {
+            if (t >= total) return;
+            const float *xs, *ws;
+            scales_of(t, turn, xs, ws);
+            fetch(xs, 0);
+            held = ws[min(lane, a.kb - 1) * a.sum_step];
+        };
+        fetch_first(pair, 0);
 #pragma unroll 1
-        for (int t = pair; ok && t < total; t += pairs) {
+        for (int t = pair, turn = 0; ok && t < total; t += pairs, ++turn) {
             float acc[128];
 #pragma unroll
             for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
             {
-                const ManyTile z = many_tile(a, t, sb);
-                // the thread's row; rows behind the tile's compute something that nobody stores
-                const int64_t row = min(static_cast<int64_t>(z.m0) + static_cast<int>(cta) * 128 + (w & 3) * 32 + lane, a.M - 1);
-                const float* xs = a.xs + row * a.lds;
-                const float* ws = a.ws + z.t0 + min(z.col + ((w - 4) >> 2), a.nb - 1) * a.out_step;
-                // the row's scales, four blocks at a time, the next four on their way
-                auto fetch = [&](int u) {
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 16;\ncp.async.commit_group;" ::"r"(
-                                     mine + (u & 4) * 1024),
-                                 "l"(xs + u)
-                                 : "memory");
-                };
-                fetch(0);
-                float held = 0.0f;  // the weight scales of 32 blocks, one a lane
+                const float *xs, *ws;
+                scales_of(t, turn, xs, ws);
                 // block u in accumulator b
                 auto block = [&](int u, uint32_t b) {
                     ok &= pair_wait(sb + kManyDoneAt + 8 * b, used >> b & 1, seen, sb, a.err);
@@ -712,9 +796,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads, 1)
                 };
                 int u = 0;
                 auto next_four = [&]() {
-                    if ((u & 31) == 0) held = ws[min(u + lane, a.kb - 1) * a.sum_step];
+                    if (u && (u & 31) == 0) held = ws[min(u + lane, a.kb - 1) * a.sum_step];
                     asm volatile("cp.async.wait_group 0;" ::: "memory");
-                    if (u + 4 < a.kb) fetch(u + 4);
+                    if (u + 4 < a.kb) fetch(xs, u + 4);
                 };
                 // four blocks a round, so that few branches are left between their sums
 #pragma unroll 1
@@ -732,7 +816,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads, 1)
                 }
                 if (a.kb & 1) seen = false;  // the next tile begins with accumulator 0 again
             }
-            const ManyTile z = many_tile(a, t, sb);  // (kept from before, it would cost the sums registers)
+            fetch_first(t + pairs, turn + 1);
+            const ManyTile z = many_tile(a, t, turn, sb);  // (kept from before, it would cost the sums registers)
             const int r = static_cast<int>(cta) * 128 + (w & 3) * 32 + lane;
             const int64_t n = (z.col + ((w - 4) >> 2)) * 128ll, left = min(static_cast<int64_t>(128), a.N - n);
             if (!ok || left <= 0) continue;
@@ -751,12 +836,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads, 1)
                         }
                 continue;
             }
-            // 256 bytes of a row at a time: a lane leaves its row's in shared memory and
-            // one bulk copy takes them from there, while the next tile begins
+            // 256 bytes of a row at a time, left in shared memory for the warp that copies
             const uint32_t piece = sb + kManyOutAt + ((w - 4) * 32 + lane) * kManyPitch;
 #pragma unroll
             for (int c = 0; c < 128; c += PER) {
-                asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                ok &= pair_wait(sb + kManyCopiedAt + 8 * ((w - 4) >> 2), (used >> 2 & 1) ^ 1, false, sb, a.err);
+                used ^= 4;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     uint32_t v[4];
@@ -771,16 +856,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads, 1)
                                  "r"(v[2]), "r"(v[3])
                                  : "memory");
                 }
-                fence_proxy_async_smem();
-                const int64_t bytes = min(static_cast<int64_t>(256), (left - c) * ES);
-                if (r < z.rows && bytes > 0)
-                    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to + c * ES),
-                                 "r"(piece), "r"(static_cast<uint32_t>(bytes))
-                                 : "memory");
-                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                __syncwarp();
+                arrive_first_lane(cluster_address(sb + kManyStagedAt + 8 * ((w - 4) >> 2), cta));
+                if (c + PER >= left) break;
             }
         }
-        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
 
     // the pair's MMAs, commits and remote arrivals are done

@@ -157,6 +157,27 @@ def test_weights_packed_on_one_stream_are_used_on_another(cuda):
         assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("odt,N", [("bfloat16", 8192), ("float32", 8136)])
+def test_more_tiles_than_are_looked_up_at_once(cuda, odt, N):
+    """Some 260 tiles for a pair of SMs.  A row's results depend on no other row, so rows
+    that repeat give the same bits wherever they lie."""
+    import torch
+    from aethermoe_b200 import _lib, fp8
+    K, times = 64, 310
+    q, s = weights(cuda, 2, K, N, seed=5)
+    w = fp8.Fp8Weight(q, s)
+    x = torch.randn(512, K, device=cuda)
+    starts = torch.tensor([0, 512 * 7, 512 * times], dtype=torch.int32, device=cuda)
+    y = fp8.grouped_fp8_matmul(x.repeat(times, 1), w, starts, out_dtype=getattr(torch, odt))
+    xv = value(*plain_rows(x))
+    for first, e in ((0, 0), (7, 1)):
+        check(y[512 * first:512 * (first + 1)], xv, weight_value(q[e], s[e]), blocks(K))
+    y = y.view(times, 512, N)
+    for i in range(times):
+        assert torch.equal(y[i], y[0 if i < 7 else 7]), i
+    _lib.check(_lib.lib().aem_device_status(None))
+
+
 @pytest.mark.parametrize("E,k,groups,top", [(256, 8, 8, 4), (64, 6, 4, 2), (60, 6, 4, 2), (16, 4, 2, 1)])
 def test_route_with_many_near_ties(cuda, E, k, groups, top):
     """Every row needs the 64-bit choice: biases that undo the scores of one row's
