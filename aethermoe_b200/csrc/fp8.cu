@@ -914,10 +914,14 @@ int64_t few_cost(int64_t ctas, int64_t blocks, int rows, int* split) {
     }
     return least;
 }
-// Many rows: persistent pairs.  256 rows, 4096 x 14336 (56 tiles): 21.4 us where the
-// kernel for few rows takes 43.7; 14336 x 4096 (16 tiles): 53.9 and 34.6.  64 experts of
-// 2048 x 1408 with 128, 192, 256 rows each: 81, 87, 92 us and 85, 141, 155.
-int64_t many_cost(int64_t tiles, int64_t blocks, int pairs) { return (tiles + pairs - 1) / pairs * (570 + 47 * blocks); }
+// Many rows: persistent pairs.  4096 x 14336 (56 tiles), 64, 128, 256 and 384 rows:
+// 23.4, 23.4, 23.4 and 41.1 us, the kernel for few rows 20.6, 24.1, 45.8 and 65.7; 14336
+// x 4096 (16 tiles) 55 to 56 us, the other 19.4, 25.4, 35.6 and 76.7.  64 experts of 2048
+// x 1408 with 32, 64, 96, 128 and 256 rows each: 60, 62, 63, 64 and 67 us, the other 44,
+// 67, 74, 79 and 141.
+int64_t many_cost(int64_t tiles, int64_t blocks, int pairs) {
+    return 600 + (tiles + pairs - 1) / pairs * (320 + 41 * blocks);
+}
 
 template <int TN, bool ALONE>
 aem_status launch_few(Fp8Args a, const void* q, int64_t ldq, int64_t cols, bool transposed, bool dependent,
@@ -1052,13 +1056,14 @@ aem_status fp8_product(const Fp8Weight* w, const char* what, Fp8Args a, Rows x, 
     a.rows = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : 128;
     // (the groups' sizes are not known here: all as large as the average)
     const int64_t cost = few_cost(n * ((want + a.rows - 1) / a.rows) * a.nb, a.kb, a.rows, &a.S);
-    const int pairs = want > 64 ? max_pairs(w->device) : 0;
+    const int pairs = want > 32 ? max_pairs(w->device) : 0;
     const bool many = pairs > 0 && (a.M > 65535ll * 64 ||  // (more row tiles than a grid of the other kernel has)
                                     many_cost(n * ((want + kManyTile - 1) / kManyTile) * ((a.nb + 1) / 2), a.kb, pairs) < cost);
     if (many) a.rows = kManyTile;
     // row tiles at most: n groups with rows have up to n + (M - n) / rows
     const int64_t slots = a.group_rows ? n + (a.M - n) / a.rows : (a.M + a.rows - 1) / a.rows;
-    AEM_REQUIRE((many || slots <= 65535) && slots * ((a.nb + 1) / 2) < (1ll << 31) && a.M < (1ll << 31), "%s: M=%lld rows are too many for one call", what, (long long)a.M);
+    AEM_REQUIRE((many || slots <= 65535) && slots * ((a.nb + 1) / 2) < (1ll << 31) && a.M < (1ll << 31),
+                "%s: M=%lld rows are too many for one call", what, (long long)a.M);
     void* own = nullptr;
     const bool make = x.dtype != AEM_E4M3;
     if (make) {
@@ -1080,11 +1085,11 @@ aem_status fp8_product(const Fp8Weight* w, const char* what, Fp8Args a, Rows x, 
     }
     a.xs = x.scale;
     a.lds = x.lds;
-    aem_status st = many           ? launch_many(a, w, x.x, x.ldx, cols, transposed, make, slots, s)
+    aem_status st = many             ? launch_many(a, w, x.x, x.ldx, cols, transposed, make, slots, s)
                     : a.rows == 16   ? launch_few<16, false>(a, x.x, x.ldx, cols, transposed, make, slots, s)
-                    : a.rows == 32 ? launch_few<32, false>(a, x.x, x.ldx, cols, transposed, make, slots, s)
-                    : a.rows == 64 ? launch_few<64, true>(a, x.x, x.ldx, cols, transposed, make, slots, s)
-                                   : launch_few<128, true>(a, x.x, x.ldx, cols, transposed, make, slots, s);
+                    : a.rows == 32   ? launch_few<32, false>(a, x.x, x.ldx, cols, transposed, make, slots, s)
+                    : a.rows == 64   ? launch_few<64, true>(a, x.x, x.ldx, cols, transposed, make, slots, s)
+                                     : launch_few<128, true>(a, x.x, x.ldx, cols, transposed, make, slots, s);
     if (own) cudaFreeAsync(own, s);
     AEM_TRY(st);
     if (zero_rest) {
