@@ -12,8 +12,10 @@ Python kernel API:
 plus the composed layer (``aethermoe_b200.moe``): a single-GPU MoE layer and
 the expert-parallel layer over NCCL; and the pieces for callers that run their
 own experts: token dispatch and combine with their gradients
-(``aethermoe_b200.dispatch``) and 4-bit weights with group scales
-(``aethermoe_b200.q4``).
+(``aethermoe_b200.dispatch``), routing from a router's logits
+(``aethermoe_b200.routing``), 4-bit weights with group scales
+(``aethermoe_b200.q4``) and 8-bit floating point products
+(``aethermoe_b200.fp8``).
 """
 from ._lib import (AemError, AemTimeout, CAPACITY_UNLIMITED, GATING_EXACT, GATING_FAST, Gate,
                    MoeConfig, QWeight, check, context, device_count, lib)
