@@ -387,7 +387,8 @@ __global__ void __launch_bounds__(kFewThreads, ALONE ? 1 : 2)
 // their barriers alone take 155; what bounds it is the warps that take the sums back,
 // about 700 cycles a block where the MMAs take 512 (264 are multiply-adds of the two
 // warps that share a sub-core), and a tile's first and last block, which overlap with
-// no other's MMAs.  Accumulators of half the width, four of them, wait twice as often: 261 us.
+// no other's MMAs.  For seconds on end it takes 249 us: the power limit (990 W) leaves
+// 1.5 GHz.  Accumulators of half the width, four of them, wait twice as often: 261 us.
 // The registers decide: 128 sums, 32 columns under way, and every variable more that
 // was kept through the loop was moved about in it (two accumulators' worth of columns
 // under way 238 us, the next block's first columns 231, pointers kept 245, one float4 of scales 225 instead of 220).
