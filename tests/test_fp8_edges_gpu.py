@@ -157,6 +157,33 @@ def test_weights_packed_on_one_stream_are_used_on_another(cuda):
         assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("odt", ["bfloat16", "float32"])
+@pytest.mark.parametrize("N", [520, 130, 47, 256])
+def test_many_rows_into_rows_of_any_stride(cuda, N, odt):
+    """20000 rows: the kernel for many rows, whose results leave by whole rows of 16-byte
+    pieces where they can.  The same bits wherever they go, and nothing beside them."""
+    import torch
+    from aethermoe_b200 import _lib, fp8
+    K, M, odt = 96, 20000, getattr(torch, odt)
+    q, s = weights(cuda, 2, K, N, seed=N)
+    w = fp8.Fp8Weight(q, s)
+    x = torch.randn(M, K, device=cuda).bfloat16()
+    starts = torch.tensor([0, 9001, M - 300], dtype=torch.int32, device=cuda)
+    want, grouped = fp8.fp8_matmul(x, w, 1, out_dtype=odt), torch.full((M, N), 7.0, device=cuda, dtype=odt)
+    check(want, value(*plain_rows(x)), weight_value(q[1], s[1]), blocks(K))
+    fp8.grouped_fp8_matmul(x, w, starts, out=grouped)
+    assert torch.equal(grouped[9001:M - 300], want[9001:M - 300]) and (grouped[M - 300:] == 7).all()
+    for before, after in ((0, 8), (8, 0), (4, 4), (2, 2), (1, 0), (0, 3)):
+        out = torch.full((M + 2, before + N + after), 7.0, device=cuda, dtype=odt)
+        inner = out[1:M + 1, before:before + N]
+        assert torch.equal(fp8.fp8_matmul(x, w, 1, out=inner), want), (before, after)
+        fp8.grouped_fp8_matmul(x, w, starts, out=inner.fill_(7.0))
+        assert torch.equal(inner, grouped), (before, after)
+        inner.fill_(7.0)
+        assert (out == 7).all(), (before, after)
+    _lib.check(_lib.lib().aem_device_status(None))
+
+
 @pytest.mark.parametrize("odt,N", [("bfloat16", 8192), ("float32", 8136)])
 def test_more_tiles_than_are_looked_up_at_once(cuda, odt, N):
     """Some 260 tiles for a pair of SMs.  A row's results depend on no other row, so rows

@@ -115,6 +115,22 @@ def test_route(cuda, T, E, k, groups, top, dt, score):
                 check_route(x, ids, w, dict(how, bias=None if b is None else b.cpu().numpy()))
 
 
+@pytest.mark.parametrize("E,k,groups,top", [(64, 6, 1, 1), (256, 8, 8, 4), (60, 4, 4, 2)])
+def test_bias_and_logits_at_any_address(cuda, E, k, groups, top):
+    """Vectors are loaded where addresses and strides allow it: the same results."""
+    import torch
+    from aethermoe_b200 import routing
+    x, bias = make(cuda, 70, E, torch.float32, seed=E), 0.1 * torch.randn(E, device=cuda)
+    how = dict(score="sigmoid", groups=groups, top_groups=top, group_top=2, renormalize=True)
+    ids, w = routing.route_tokens(x, k, bias=bias, **how)
+    for off in (1, 2, 4):
+        b = torch.zeros(E + off, device=cuda)[off:].copy_(bias)
+        y = torch.zeros(70, E + off, device=cuda)[:, off:].copy_(x)
+        for xx, bb in ((x, b), (y, bias), (y, b)):
+            got = routing.route_tokens(xx, k, bias=bb, **how)
+            assert torch.equal(got[0], ids) and torch.equal(got[1], w), off
+
+
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_near_and_equal_keys(cuda, score):
     """Keys that float32 cannot tell apart are ordered as 64 bits order them, and
