@@ -177,6 +177,8 @@ struct RouteShared {
     float take[kRouteWarps][256];                  // what becomes of a chosen expert
     int32_t ids[kRouteWarps][256];                 // [row][k]: LANES * 8 >= k
     double value[kRouteWarps][32];                 // of groups of whole lanes, chosen exactly
+    uint32_t rank[kRouteWarps][256 + 32];          // [row][k + 1]: of the chosen and of the next one
+    int32_t next[kRouteWarps][32];                 // [row]: the next one
 };
 // Groups that are not whole lanes (or not a power of two of them): values of the
 // experts and of the groups.
@@ -309,27 +311,33 @@ __device__ __forceinline__ bool extract(const RouteArgs& a, bool on, RouteShared
     const unsigned segment = (LANES == 32 ? ~0u : (1u << LANES) - 1) << (row * LANES);
     unsigned long long head = on ? sh.list[w][0][lane] : 0;
     int next = 1;  // of the lane's list
-    bool near = false;
-    float last_key = INFINITY, last_score = 0.0f;
+    uint32_t* ranks = &sh.rank[w][row * (a.k + 1)];
+    int32_t* ids = &sh.ids[w][row * a.k];
     for (int j = 0; j < a.k + (CERT ? 1 : 0); ++j) {
         const uint32_t rank = static_cast<uint32_t>(head >> 32);
         const uint32_t m = seg_max<LANES>(rank);
-        const int owner = __ffs(__ballot_sync(~0u, rank == m) & segment) - 1;
-        const int id = sub * kV + 7 - static_cast<int>(head & 7);
-        if (lane == owner) {
-            if (j < a.k) sh.ids[w][row * a.k + j] = m ? id : -1;
+        if (lane == __ffs(__ballot_sync(~0u, rank == m) & segment) - 1) {
+            const int id = m ? sub * kV + 7 - static_cast<int>(head & 7) : -1;
+            if (j < a.k) ids[j] = id;
+            if constexpr (CERT) {
+                ranks[j] = m;
+                if (j == a.k) sh.next[w][row] = id;
+            }
             head = next < kV ? sh.list[w][next][lane] : 0;
             ++next;
         }
-        if constexpr (CERT) {
-            const int at = __shfl_sync(~0u, id, owner);
-            const float score = sh.take[w][row * LANES * kV + at], k = value_of(m);
-            if (j > 0 && m) near |= !(last_key - k > slack(a.sigmoid, score, k) + slack(a.sigmoid, last_score, last_key));
-            last_key = k;
-            last_score = score;
-        }
     }
     __syncwarp();
+    bool near = false;
+    if constexpr (CERT) {
+        const float* take = &sh.take[w][row * LANES * kV];
+        for (int j = sub; j < a.k; j += LANES) {
+            if (ranks[j + 1] == 0) break;
+            const float key = value_of(ranks[j]), then = value_of(ranks[j + 1]);
+            const int id = j + 1 < a.k ? ids[j + 1] : sh.next[w][row];
+            near |= !(key - then > slack(a.sigmoid, take[ids[j]], key) + slack(a.sigmoid, take[id], then));
+        }
+    }
     return near;
 }
 
