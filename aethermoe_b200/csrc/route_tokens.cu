@@ -25,8 +25,8 @@
 // Groups of whole lanes take their two largest from the sorted lists; others are
 // read through shared memory.  What has to be moved is T*E logits and 8 T*k bytes,
 // but a choice of k costs k warp-wide maxima, and those bound it.  256 float32 logits,
-// top-8: 1 row 3.8 us softmax and 5.5 sigmoid with bias and 8 groups, 16383 rows 24
-// and 44 us, 262144 rows 310 and 498 us (0.9 and 0.6 TB/s of logits).
+// top-8: 1 row 3.6 us softmax and 4.9 sigmoid with bias and 8 groups, 16383 rows 23
+// and 38 us, 262144 rows 303 and 443 us (0.9 and 0.6 TB/s of logits).
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -75,10 +75,6 @@ __device__ __forceinline__ double seg_sum(double v) {
     return seg_reduce<LANES>(v, [](double a, double b) { return a + b; });
 }
 template <int LANES>
-__device__ __forceinline__ float seg_max(float v) {
-    return seg_reduce<LANES>(v, [](float a, float b) { return fmaxf(a, b); });
-}
-template <int LANES>
 __device__ __forceinline__ uint32_t seg_max(uint32_t v) {
     if constexpr (LANES == 32) return __reduce_max_sync(~0u, v);
     return seg_reduce<LANES>(v, [](uint32_t a, uint32_t b) { return max(a, b); });
@@ -104,6 +100,13 @@ __device__ __forceinline__ unsigned long long rank_of(double v) {
 }
 __device__ __forceinline__ float value_of(uint32_t r) {
     return r == ~0u ? NAN : r == 0 ? -INFINITY : __uint_as_float(r ^ (r >> 31 ? 0x80000000u : ~0u));
+}
+// (a NaN wins where a warp is one row; every caller's results are NaN then anyway, or
+// none comes here)
+template <int LANES>
+__device__ __forceinline__ float seg_max(float v) {
+    if constexpr (LANES == 32) return value_of(__reduce_max_sync(~0u, rank_of(v)));
+    return seg_reduce<LANES>(v, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ __forceinline__ double value_of(unsigned long long r) {
     return r == ~0ull ? NAN
@@ -450,8 +453,9 @@ __global__ void __launch_bounds__(kRouteThreads, 4) route_kernel(const RouteArgs
             top = fmaxf(top, s[i]);
             if (key[i] != -INFINITY) largest = fmaxf(largest, fabsf(a.bias ? key[i] : s[i]));
         }
-        top = seg_max<LANES>(top);
-        largest = seg_max<LANES>(largest);
+        // (neither is negative: their bits have the same order)
+        top = __uint_as_float(seg_max<LANES>(__float_as_uint(top)));
+        largest = __uint_as_float(seg_max<LANES>(__float_as_uint(largest)));
         e = 4.0f * slack(a.sigmoid, top, largest) + 0x1p-22f * largest;
     }
     bool near = false, on = true;
