@@ -13,9 +13,11 @@
 // rounding of a float32 exp or sum.  Keys are computed in float32 beside a bound
 // on their error; wherever two keys that decide the order (neighbours among the
 // k + 1 largest, the last group kept and the first dropped) are nearer than their
-// bounds, the warp chooses again with keys in 64 bits.  With normally distributed
-// logits and 256 experts, top-8, that is a row in 2400 (sigmoid with a bias), and a
-// call with such a row takes 5 us longer.  Logits themselves need no bound.
+// bounds, the warp decides with keys in 64 bits: those of the chosen experts where only
+// their order is open (with normally distributed logits and 256 experts, top-8,
+// sigmoid with a bias, a row in 2400), else of all of them (an eighth of those rows; a
+// call with such a row takes 5 us longer, and when all took that way 16383 rows took
+// 38 us instead of 32).  Logits themselves need no bound.
 //
 // A row lies across LANES lanes, 8 neighbouring experts a lane, so a lane's order
 // is the experts' and up to 32 rows share a warp.  A lane sorts its experts once
@@ -26,7 +28,7 @@
 // read through shared memory.  What has to be moved is T*E logits and 8 T*k bytes,
 // but a choice of k costs k warp-wide maxima, and those bound it.  256 float32 logits,
 // top-8: 1 row 3.6 us softmax and 4.9 sigmoid with bias and 8 groups, 16383 rows 23
-// and 38 us, 262144 rows 303 and 443 us (0.9 and 0.6 TB/s of logits).
+// and 32 us, 262144 rows 307 and 447 us (0.9 and 0.6 TB/s of logits).
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -181,7 +183,6 @@ struct RouteShared {
     int32_t ids[kRouteWarps][256];                 // [row][k]: LANES * 8 >= k
     double value[kRouteWarps][32];                 // of groups of whole lanes, chosen exactly
     uint32_t rank[kRouteWarps][256 + 32];          // [row][k + 1]: of the chosen and of the next one
-    int32_t next[kRouteWarps][32];                 // [row]: the next one
 };
 // Groups that are not whole lanes (or not a power of two of them): values of the
 // experts and of the groups.
@@ -307,9 +308,12 @@ __device__ __forceinline__ bool keep_lanes(const RouteArgs& a, int span, F first
 
 // The k largest of the lanes' sorted lists in shared memory, head of its list `best`
 // and `on` whether the lane takes part; their ids and, with a bound on the keys'
-// errors (CERT), whether a decision was nearer than that.
+// errors (CERT), what was nearer than that: 1: the order of two of them, 2: the last of
+// them and the next.  The neighbours' bounds prove the order of all the chosen ones;
+// an expert behind the next one may have a larger error than it, `limit` at most
+// apart from the rounding of its key.
 template <int LANES, bool CERT>
-__device__ __forceinline__ bool extract(const RouteArgs& a, bool on, RouteShared& sh) {
+__device__ __forceinline__ int extract(const RouteArgs& a, bool on, float limit, RouteShared& sh) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, sub = lane % LANES, row = lane / LANES;
     const unsigned segment = (LANES == 32 ? ~0u : (1u << LANES) - 1) << (row * LANES);
     unsigned long long head = on ? sh.list[w][0][lane] : 0;
@@ -324,24 +328,48 @@ __device__ __forceinline__ bool extract(const RouteArgs& a, bool on, RouteShared
             if (j < a.k) ids[j] = id;
             if constexpr (CERT) {
                 ranks[j] = m;
-                if (j == a.k) sh.next[w][row] = id;
             }
             head = next < kV ? sh.list[w][next][lane] : 0;
             ++next;
         }
     }
     __syncwarp();
-    bool near = false;
+    int near = 0;
     if constexpr (CERT) {
         const float* take = &sh.take[w][row * LANES * kV];
         for (int j = sub; j < a.k; j += LANES) {
             if (ranks[j + 1] == 0) break;
             const float key = value_of(ranks[j]), then = value_of(ranks[j + 1]);
-            const int id = j + 1 < a.k ? ids[j + 1] : sh.next[w][row];
-            near |= !(key - then > slack(a.sigmoid, take[ids[j]], key) + slack(a.sigmoid, take[id], then));
+            const float other = j + 1 < a.k ? slack(a.sigmoid, take[ids[j + 1]], then)
+                                            : fmaf(1.01f * 0x1p-24f, fabsf(then), limit);
+            if (!(key - then > slack(a.sigmoid, take[ids[j]], key) + other)) near |= j + 1 < a.k ? 1 : 2;
         }
     }
     return near;
+}
+
+// The chosen experts in the order of their keys in 64 bits, where it is known that
+// they are the ones: a slot a lane (k <= LANES, sigmoid scores with a bias).
+template <int LANES, typename LT>
+__device__ __noinline__ void order_exactly(const RouteArgs& a, int64_t t0, int32_t* ids) {
+    const int lane = threadIdx.x & 31, sub = lane % LANES, row = lane / LANES;
+    const bool slot = sub < a.k && t0 + row < a.T;
+    ids += row * a.k;
+    const int id = slot ? ids[sub] : -1;
+    unsigned long long rank = 0;
+    if (id >= 0) {
+        const double v = static_cast<float>(static_cast<const LT*>(a.logits)[(t0 + row) * a.ld + id]), t = exp(-fabs(v));
+        rank = rank_of((v < 0.0 ? t : 1.0) / (1.0 + t) + static_cast<double>(a.bias[id]));
+    }
+    int at = 0;
+    for (int i = 0; i < a.k; ++i) {
+        const unsigned long long other = __shfl_sync(~0u, rank, row * LANES + i);
+        const int that = __shfl_sync(~0u, id, row * LANES + i);
+        at += other > rank || (other == rank && (that < id || (that == id && i < sub)));
+    }
+    __syncwarp();
+    if (slot) ids[at] = id;
+    __syncwarp();
 }
 
 template <typename LT>
@@ -498,11 +526,25 @@ __global__ void __launch_bounds__(kRouteThreads, 4) route_kernel(const RouteArgs
         }
         on = keep_lanes<LANES, float>(a, a.size / kV, first, second, e, near);
     }
-    if (a.bias)
-        near |= extract<LANES, true>(a, on, sh);
-    else
-        extract<LANES, false>(a, on, sh);
-    if (!sure && __any_sync(~0u, near)) choose_exactly<LANES, LT>(a, t0, sh, ANY ? gsh.value[w] : sh.value[w]);
+    int close = near ? 2 : 0;
+    if (a.bias) {
+        // s (6.02 - 4 s) is at most 2.27; a softmax's largest score bounds the others
+        float limit = 2.27f * 0x1p-24f + 0x1p-64f;
+        if (!a.sigmoid) {
+            float top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kV; ++i) top = fmaxf(top, s[i]);
+            limit = fmaf(0x1p-18f, __uint_as_float(seg_max<LANES>(__float_as_uint(top))), 0x1p-64f);
+        }
+        close |= extract<LANES, true>(a, on, limit, sh);
+    } else {
+        extract<LANES, false>(a, on, 0.0f, sh);
+    }
+    if (!sure) close = __reduce_or_sync(~0u, close);
+    if (!sure && close == 1 && a.sigmoid && a.k <= LANES)
+        order_exactly<LANES, LT>(a, t0, sh.ids[w]);
+    else if (!sure && close)
+        choose_exactly<LANES, LT>(a, t0, sh, ANY ? gsh.value[w] : sh.value[w]);
     if (of_logits && a.bias) {  // the scores have been compared
         __syncwarp();
 #pragma unroll
