@@ -585,19 +585,21 @@ __global__ void __launch_bounds__(kRouteThreads, 4) route_kernel(const RouteArgs
 // slot: it leaves what the row's sums need in shared memory, takes the sums from
 // there in the slots' order, and leaves its term at its expert; of slots with the
 // same expert the first one adds the others' terms.  Then every lane writes its own 8
-// experts.  Memory bound: 262144 rows of 256 float32, top-8, with the sums over all
-// experts 173 us (3.1 TB/s), over the chosen ones alone 146 us.
-template <int LANES, typename LT>
-__global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const RouteArgs a) {
-    __shared__ int32_t s_ids[kRouteWarps][256];
-    __shared__ float s_p[kRouteWarps][256], s_g[kRouteWarps][256], s_term[kRouteWarps][256];
-    __shared__ __align__(16) float s_row[kRouteWarps][256];
-    constexpr int ROWS = 32 / LANES;
+// experts, or, where the chosen ones alone have a gradient, pieces of whole lines.  There
+// a warp has four rows, so that its lanes have slots: 16383 rows of 256 float32, top-8,
+// in 6.3 us, one row a warp 9.8.  Memory bound: 262144 such rows in 90 us (2.9 TB/s
+// written, 0.8 read), with the sums over all experts 173 us (3.1 TB/s).
+template <int LANES, typename LT, int RB>
+__global__ void __launch_bounds__(kRouteThreads / (RB > 1 ? 2 : 1)) route_backward_kernel(const RouteArgs a) {
+    constexpr int WARPS = kRouteWarps / (RB > 1 ? 2 : 1), ROWS = 32 / LANES * RB;  // RB rows of a lane
+    __shared__ int32_t s_ids[WARPS][256];
+    __shared__ float s_p[WARPS][256], s_g[WARPS][256], s_term[WARPS][256];
+    __shared__ __align__(16) float s_row[WARPS][256 * RB];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, sub = lane % LANES, row = lane / LANES, e0 = sub * kV;
-    const int64_t t0 = (static_cast<int64_t>(blockIdx.x) * kRouteWarps + w) * ROWS;
+    const int64_t t0 = (static_cast<int64_t>(blockIdx.x) * WARPS + w) * ROWS;
     if (t0 >= a.T) return;
     const int64_t t = t0 + row;
-    const bool all = !a.sigmoid && !a.renorm;
+    const bool all = RB == 1 && !a.sigmoid && !a.renorm;
     const int n = static_cast<int>(min(static_cast<int64_t>(ROWS), a.T - t0)) * a.k;
     float s[kV], m = 0.0f, r = 0.0f;
     if (all) {
@@ -619,7 +621,8 @@ __global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const Rou
         for (int i = 0; i < kV; ++i) s[i] *= r;
     }
 #pragma unroll
-    for (int i = 0; i < kV; i += 4) *reinterpret_cast<float4*>(&s_row[w][lane * kV + i]) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i = 0; i < kV * RB; i += 4)
+        *reinterpret_cast<float4*>(&s_row[w][lane * 4 + i * 32]) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     // a slot's id, gradient and score (softmax, renormalised: its logit)
     for (int i0 = 0; i0 < n; i0 += 32) {
         const int i = i0 + lane, q = min(i, n - 1) * a.k_inv >> 16;
@@ -689,32 +692,50 @@ __global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const Rou
         if (first) s_row[w][q * LANES * kV + id] = v;
     }
     __syncwarp();
-    if (t >= a.T || e0 >= a.E) return;
-    float sum[kV];
+    if (!all && sizeof(LT) == 4 && a.ovec) {  // nothing is in registers: whole lines at once
 #pragma unroll
-    for (int i = 0; i < kV; i += 4) {
-        const float4 v = *reinterpret_cast<const float4*>(&s_row[w][lane * kV + i]);
-        sum[i] = v.x, sum[i + 1] = v.y, sum[i + 2] = v.z, sum[i + 3] = v.w;
-    }
-    if (all)
+        for (int q = 0; q < RB; ++q) {
+            const int64_t t = t0 + q * (32 / LANES) + row;
+            if (t >= a.T) return;
 #pragma unroll
-        for (int i = 0; i < kV; ++i) sum[i] = s[i] * (sum[i] - dot);
-    LT* p = static_cast<LT*>(a.grad_logits) + t * a.ldo + e0;
-    if (a.ovec) {
-        if constexpr (sizeof(LT) == 4) {
-            *reinterpret_cast<float4*>(p) = make_float4(sum[0], sum[1], sum[2], sum[3]);
-            *reinterpret_cast<float4*>(p + 4) = make_float4(sum[4], sum[5], sum[6], sum[7]);
-        } else {
-            __nv_bfloat162 h[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(sum[2 * i], sum[2 * i + 1]);
-            *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(h);
+            for (int e = sub * 4; e < LANES * kV; e += LANES * 4)
+                if (e < a.E)
+                    *reinterpret_cast<float4*>(static_cast<float*>(a.grad_logits) + t * a.ldo + e) =
+                        *reinterpret_cast<const float4*>(&s_row[w][q * 256 + row * LANES * kV + e]);
         }
         return;
     }
+    if (e0 >= a.E) return;
 #pragma unroll
-    for (int i = 0; i < kV; ++i)
-        if (e0 + i < a.E) p[i] = static_cast<LT>(sum[i]);
+    for (int q = 0; q < RB; ++q) {
+        const int64_t t = t0 + q * (32 / LANES) + row;
+        if (t >= a.T) return;
+        float sum[kV];
+#pragma unroll
+        for (int i = 0; i < kV; i += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(&s_row[w][q * 256 + lane * kV + i]);
+            sum[i] = v.x, sum[i + 1] = v.y, sum[i + 2] = v.z, sum[i + 3] = v.w;
+        }
+        if (all)
+#pragma unroll
+            for (int i = 0; i < kV; ++i) sum[i] = s[i] * (sum[i] - dot);
+        LT* p = static_cast<LT*>(a.grad_logits) + t * a.ldo + e0;
+        if (a.ovec) {
+            if constexpr (sizeof(LT) == 4) {
+                *reinterpret_cast<float4*>(p) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+                *reinterpret_cast<float4*>(p + 4) = make_float4(sum[4], sum[5], sum[6], sum[7]);
+            } else {
+                __nv_bfloat162 h[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(sum[2 * i], sum[2 * i + 1]);
+                *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(h);
+            }
+            continue;
+        }
+#pragma unroll
+        for (int i = 0; i < kV; ++i)
+            if (e0 + i < a.E) p[i] = static_cast<LT>(sum[i]);
+    }
 }
 
 // Lanes of a row: 8 experts each.
@@ -772,8 +793,8 @@ RouteArgs route_args(const aem_route_config* c, const void* logits, aem_dtype dt
     return a;
 }
 
-aem_status route_grid(const char* what, int64_t T, int rows, unsigned* blocks) {
-    const int64_t n = (T + rows * kRouteWarps - 1) / (rows * kRouteWarps);
+aem_status route_grid(const char* what, int64_t T, int rows, int warps, unsigned* blocks) {
+    const int64_t n = (T + rows * warps - 1) / (rows * warps);
     AEM_REQUIRE(n < (1ll << 31), "%s: T=%lld out of range", what, (long long)T);
     *blocks = static_cast<unsigned>(n);
     return AEM_OK;
@@ -800,7 +821,7 @@ aem_status aem_route_tokens(const aem_route_config* config, const void* logits, 
     aem::with_lanes(E, [&](auto lanes) {
         constexpr int L = decltype(lanes)::value;
         unsigned blocks;
-        st = aem::route_grid("aem_route_tokens", T, 32 / L, &blocks);
+        st = aem::route_grid("aem_route_tokens", T, 32 / L, aem::kRouteWarps, &blocks);
         if (st != AEM_OK) return;
         auto s = static_cast<cudaStream_t>(stream);
         const int span = a.size / aem::kV;
@@ -857,13 +878,23 @@ aem_status aem_route_tokens_backward(const aem_route_config* config, const float
     aem::with_lanes(E, [&](auto lanes) {
         constexpr int L = decltype(lanes)::value;
         unsigned blocks;
-        st = aem::route_grid("aem_route_tokens_backward", T, 32 / L, &blocks);
-        if (st != AEM_OK) return;
         auto s = static_cast<cudaStream_t>(stream);
-        if (dtype == AEM_F32)
-            aem::route_backward_kernel<L, float><<<blocks, aem::kRouteThreads, 0, s>>>(a);
+        auto go = [&](auto rows) {
+            constexpr int RB = decltype(rows)::value;
+            st = aem::route_grid("aem_route_tokens_backward", T, 32 / L * RB, aem::kRouteWarps / (RB > 1 ? 2 : 1), &blocks);
+            if (st != AEM_OK) return;
+            const int threads = aem::kRouteThreads / (RB > 1 ? 2 : 1);
+            if (dtype == AEM_F32)
+                aem::route_backward_kernel<L, float, RB><<<blocks, threads, 0, s>>>(a);
+            else
+                aem::route_backward_kernel<L, __nv_bfloat16, RB><<<blocks, threads, 0, s>>>(a);
+        };
+        // four rows a warp; with softmax scores of all experts a row's are in registers
+        constexpr int RB = L == 32 ? 4 : L == 16 ? 2 : 1;
+        if (a.sigmoid || a.renorm)
+            go(std::integral_constant<int, RB>{});
         else
-            aem::route_backward_kernel<L, __nv_bfloat16><<<blocks, aem::kRouteThreads, 0, s>>>(a);
+            go(std::integral_constant<int, 1>{});
     });
     AEM_TRY(st);
     AEM_CHECK_LAUNCH();
