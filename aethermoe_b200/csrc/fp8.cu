@@ -390,8 +390,9 @@ __global__ void __launch_bounds__(kFewThreads, ALONE ? 1 : 2)
 // no other's MMAs.  For seconds on end it takes 249 us: the power limit (990 W) leaves
 // 1.5 GHz.  Accumulators of half the width, four of them, wait twice as often: 261 us.
 // The registers decide: 128 sums, 32 columns under way, and every variable more that
-// was kept through the loop was moved about in it (two accumulators' worth of columns
-// under way 238 us, the next block's first columns 231, pointers kept 245, one float4 of scales 225 instead of 220).
+// was kept through the loop was moved about in it (32 columns a load 238 us, the next
+// block's first columns ahead 231, pointers kept 245, one float4 of scales 225 instead of
+// 220).
 // Every wait is bounded; a timeout sets the error word and ends all roles of both CTAs.
 constexpr int kManyThreads = 12 * 32, kManyStages = 4, kManyTile = 256;
 constexpr int kManyStage = 2 * kFp8Tile;                      // of one CTA
