@@ -317,7 +317,9 @@ __device__ __forceinline__ int extract(const RouteArgs& a, bool on, float limit,
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, sub = lane % LANES, row = lane / LANES;
     const unsigned segment = (LANES == 32 ? ~0u : (1u << LANES) - 1) << (row * LANES);
     unsigned long long head = on ? sh.list[w][0][lane] : 0;
-    int next = 1;  // of the lane's list
+    // of the lane's list; past its end for a lane of a dropped group, which has the
+    // row's maximum too once nothing is left (rank 0) and must not move on
+    int next = on ? 1 : kV;
     uint32_t* ranks = &sh.rank[w][row * (a.k + 1)];
     int32_t* ids = &sh.ids[w][row * a.k];
     for (int j = 0; j < a.k + (CERT ? 1 : 0); ++j) {
