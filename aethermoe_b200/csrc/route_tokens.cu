@@ -36,6 +36,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "route_bounds.h"
 #include "runtime.h"
 
 namespace aem {
@@ -126,18 +127,6 @@ template <>
 struct Rank<double> {
     using type = unsigned long long;
 };
-
-// A float32 key's distance from the real one.  A sigmoid's relative error, from
-// exp's 2 ulp (at most 2^-22, which reach the quotient by the factor 1 - s), the sum's
-// 2^-24 and the quotient's, is under 2^-24 (2 + 4 (1 - s)).  A softmax's score has that
-// of its exponential, whose argument rounds by |x - m| 2^-24, of the sum of 256 (13
-// additions) and of two products: (|x - m| + 19) 2^-24, so under 2^-18 for |x - m| <=
-// 45, and further down it is under 2^-64 altogether.  The sum with the bias is rounded
-// once.  One or two hundredths more cover the bound's own roundings.
-__device__ __forceinline__ float slack(bool sigmoid, float score, float key) {
-    const float by = sigmoid ? fmaf(score, -0x1p-22f, 6.02f * 0x1p-24f) : 0x1p-18f;
-    return fmaf(by, score, fmaf(1.01f * 0x1p-24f, fabsf(key), 0x1p-64f));
-}
 
 __device__ __forceinline__ float exp_of(float v) { return expf(v); }
 __device__ __forceinline__ double exp_of(double v) { return exp(v); }
@@ -342,9 +331,9 @@ __device__ __forceinline__ int extract(const RouteArgs& a, bool on, float limit,
         for (int j = sub; j < a.k; j += LANES) {
             if (ranks[j + 1] == 0) break;
             const float key = value_of(ranks[j]), then = value_of(ranks[j + 1]);
-            const float other = j + 1 < a.k ? slack(a.sigmoid, take[ids[j + 1]], then)
+            const float other = j + 1 < a.k ? key_slack(a.sigmoid, take[ids[j + 1]], then)
                                             : fmaf(1.01f * 0x1p-24f, fabsf(then), limit);
-            if (!(key - then > slack(a.sigmoid, take[ids[j]], key) + other)) near |= j + 1 < a.k ? 1 : 2;
+            if (!(key - then > key_slack(a.sigmoid, take[ids[j]], key) + other)) near |= j + 1 < a.k ? 1 : 2;
         }
     }
     return near;
@@ -476,17 +465,23 @@ __global__ void __launch_bounds__(kRouteThreads, 4) route_kernel(const RouteArgs
     }
     const bool sure = !a.bias && !two;  // keys are the logits themselves
     float e = 0.0f;                     // slack of a group's value
-    if (!sure && a.groups > 1) {
-        float top = 0.0f, largest = 0.0f;
+    // the bound of any score's error in the row
+    auto any_score = [&]() {
+        float top = 0.0f;
+        if (!a.sigmoid) {
 #pragma unroll
-        for (int i = 0; i < kV; ++i) {
-            top = fmaxf(top, s[i]);
-            if (key[i] != -INFINITY) largest = fmaxf(largest, fabsf(a.bias ? key[i] : s[i]));
+            for (int i = 0; i < kV; ++i) top = fmaxf(top, s[i]);
+            // (none is negative: their bits have the same order)
+            top = __uint_as_float(seg_max<LANES>(__float_as_uint(top)));
         }
-        // (neither is negative: their bits have the same order)
-        top = __uint_as_float(seg_max<LANES>(__float_as_uint(top)));
-        largest = __uint_as_float(seg_max<LANES>(__float_as_uint(largest)));
-        e = 4.0f * slack(a.sigmoid, top, largest) + 0x1p-22f * largest;
+        return score_slack(a.sigmoid, top);
+    };
+    if (!sure && a.groups > 1) {
+        float largest = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kV; ++i)
+            if (key[i] != -INFINITY) largest = fmaxf(largest, fabsf(a.bias ? key[i] : s[i]));
+        e = group_slack(any_score(), __uint_as_float(seg_max<LANES>(__float_as_uint(largest))));
     }
     bool near = false, on = true;
     if constexpr (ANY) {
@@ -530,15 +525,7 @@ __global__ void __launch_bounds__(kRouteThreads, 4) route_kernel(const RouteArgs
     }
     int close = near ? 2 : 0;
     if (a.bias) {
-        // s (6.02 - 4 s) is at most 2.27; a softmax's largest score bounds the others
-        float limit = 2.27f * 0x1p-24f + 0x1p-64f;
-        if (!a.sigmoid) {
-            float top = 0.0f;
-#pragma unroll
-            for (int i = 0; i < kV; ++i) top = fmaxf(top, s[i]);
-            limit = fmaf(0x1p-18f, __uint_as_float(seg_max<LANES>(__float_as_uint(top))), 0x1p-64f);
-        }
-        close |= extract<LANES, true>(a, on, limit, sh);
+        close |= extract<LANES, true>(a, on, any_score(), sh);
     } else {
         extract<LANES, false>(a, on, 0.0f, sh);
     }
