@@ -37,4 +37,28 @@ AEM_BOUND float group_slack(float score, float largest) {
     return 4.0f * fmaf(1.01f * 0x1p-24f, largest, score) + 0x1p-22f * largest;
 }
 
+// What the keys leave open, as bits that the rows of a warp put together.
+enum : int {
+    OPEN_ORDER = 1,   // of two chosen ones that follow one another
+    OPEN_SET = 2,     // the last chosen one or the next
+    OPEN_BEHIND = 4,  // the next one or another chosen one, should that be open with the last
+};
+
+// The last chosen key (with its slack) and the next one.  An expert behind the next one
+// may have a larger error than it, and an earlier chosen one than the last: `score` at
+// most, apart from the rounding of its key.  Keys in falling order whose neighbours'
+// bounds are apart prove that all earlier ones lie above the last; where that is not so
+// (OPEN_ORDER), only OPEN_BEHIND shows whether they lie above the next.
+AEM_BOUND int open_at_end(float key, float slack, float then, float score) {
+    const float behind = fmaf(1.01f * 0x1p-24f, fabsf(then), score);
+    const float ahead = fmaf(1.01f * 0x1p-24f, fabsf(key), score);
+    return (key - then > slack + behind ? 0 : OPEN_SET) | (key - then > ahead + behind ? 0 : OPEN_BEHIND);
+}
+
+// 0: nothing has to be decided in 64 bits; 1: the order of the chosen ones; 2: who they are.
+AEM_BOUND int to_decide(int open) {
+    if (!(open & (OPEN_ORDER | OPEN_SET))) return 0;
+    return open == OPEN_ORDER ? 1 : 2;
+}
+
 }  // namespace aem

@@ -295,14 +295,12 @@ __device__ __forceinline__ bool keep_lanes(const RouteArgs& a, int span, F first
     return stays;
 }
 
-// The k largest of the lanes' sorted lists in shared memory, head of its list `best`
-// and `on` whether the lane takes part; their ids and, with a bound on the keys'
-// errors (CERT), what was nearer than that: 1: the order of two of them, 2: the last of
-// them and the next.  The neighbours' bounds prove the order of all the chosen ones;
-// an expert behind the next one may have a larger error than it, `limit` at most
-// apart from the rounding of its key.
+// The k largest of the lanes' sorted lists in shared memory, `on` whether the lane
+// takes part; their ids and, with a bound on the keys' errors (CERT), what is nearer
+// than that and so open.  `score` bounds the errors of
+// all the row's scores.
 template <int LANES, bool CERT>
-__device__ __forceinline__ int extract(const RouteArgs& a, bool on, float limit, RouteShared& sh) {
+__device__ __forceinline__ int extract(const RouteArgs& a, bool on, float score, RouteShared& sh) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, sub = lane % LANES, row = lane / LANES;
     const unsigned segment = (LANES == 32 ? ~0u : (1u << LANES) - 1) << (row * LANES);
     unsigned long long head = on ? sh.list[w][0][lane] : 0;
@@ -325,18 +323,20 @@ __device__ __forceinline__ int extract(const RouteArgs& a, bool on, float limit,
         }
     }
     __syncwarp();
-    int near = 0;
+    int open = 0;
     if constexpr (CERT) {
         const float* take = &sh.take[w][row * LANES * kV];
         for (int j = sub; j < a.k; j += LANES) {
             if (ranks[j + 1] == 0) break;
             const float key = value_of(ranks[j]), then = value_of(ranks[j + 1]);
-            const float other = j + 1 < a.k ? key_slack(a.sigmoid, take[ids[j + 1]], then)
-                                            : fmaf(1.01f * 0x1p-24f, fabsf(then), limit);
-            if (!(key - then > key_slack(a.sigmoid, take[ids[j]], key) + other)) near |= j + 1 < a.k ? 1 : 2;
+            const float slack = key_slack(a.sigmoid, take[ids[j]], key);
+            if (j + 1 == a.k)
+                open |= open_at_end(key, slack, then, score);
+            else if (!(key - then > slack + key_slack(a.sigmoid, take[ids[j + 1]], then)))
+                open |= OPEN_ORDER;
         }
     }
-    return near;
+    return open;
 }
 
 // The chosen experts in the order of their keys in 64 bits, where it is known that
@@ -523,16 +523,16 @@ __global__ void __launch_bounds__(kRouteThreads, 4) route_kernel(const RouteArgs
         }
         on = keep_lanes<LANES, float>(a, a.size / kV, first, second, e, near);
     }
-    int close = near ? 2 : 0;
+    int open = near ? OPEN_SET : 0;
     if (a.bias) {
-        close |= extract<LANES, true>(a, on, any_score(), sh);
+        open |= extract<LANES, true>(a, on, any_score(), sh);
     } else {
         extract<LANES, false>(a, on, 0.0f, sh);
     }
-    if (!sure) close = __reduce_or_sync(~0u, close);
-    if (!sure && close == 1 && a.sigmoid && a.k <= LANES)
+    const int decide = sure ? 0 : to_decide(__reduce_or_sync(~0u, open));
+    if (decide == 1 && a.sigmoid && a.k <= LANES)
         order_exactly<LANES, LT>(a, t0, sh.ids[w]);
-    else if (!sure && close)
+    else if (decide)
         choose_exactly<LANES, LT>(a, t0, sh, ANY ? gsh.value[w] : sh.value[w]);
     if (of_logits && a.bias) {  // the scores have been compared
         __syncwarp();
