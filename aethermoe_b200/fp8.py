@@ -58,6 +58,7 @@ class Fp8Rows:
             raise ValueError(f"scale must be {want} float32, got {tuple(scale.shape)} {scale.dtype}")
         if scale.device != q.device:
             raise ValueError(f"q and scale are on {q.device} and {scale.device}")
+        _no_gradient("Fp8Rows", q, "q")
         _no_gradient("Fp8Rows", scale, "scale")
         self._set(q, scale)
 
@@ -151,6 +152,7 @@ class Fp8Weight:
             raise ValueError(f"scale must be {want} float32, got {tuple(scale.shape)} {scale.dtype}")
         if q.device.type not in ("cpu", "cuda") or scale.device != q.device:
             raise ValueError(f"q and scale must be on one CUDA device or the CPU, got {q.device} and {scale.device}")
+        _no_gradient("Fp8Weight", q, "q")
         _no_gradient("Fp8Weight", scale, "scale")
         h = ctypes.c_void_p()
         if q.is_cuda:
