@@ -145,9 +145,9 @@ def _matrix(t, name, d=None, rows=None):
 
 
 def _output(out, shape, dtype, like, name="out"):
+    if dtype not in _DT:
+        raise ValueError(f"{name}: unsupported dtype {dtype} (float32 or bfloat16)")
     if out is None:
-        if dtype not in _DT:
-            raise ValueError(f"{name}: unsupported dtype {dtype} (float32 or bfloat16)")
         return like.new_empty(shape, dtype=dtype), shape[1]
     if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
         raise ValueError(f"{name} must be {tuple(shape)} {dtype}, got {tuple(out.shape)} {out.dtype}")
