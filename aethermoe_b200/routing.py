@@ -31,7 +31,10 @@ _SCORES = {"softmax": _lib.SCORE_SOFTMAX, "sigmoid": _lib.SCORE_SIGMOID}
 def _config(k, score, groups, top_groups, group_top, renormalize, scale):
     if score not in _SCORES:
         raise ValueError(f"score={score!r} is not 'softmax' or 'sigmoid'")
-    return _lib.RouteConfig(_SCORES[score], k, groups, top_groups, group_top, 1 if renormalize else 0, scale)
+    c = _lib.RouteConfig(_SCORES[score], k, groups, top_groups, group_top, 1 if renormalize else 0, scale)
+    if c.k != k or c.groups != groups or c.top_groups != top_groups or c.group_top != group_top:
+        raise ValueError(f"k={k}, groups={groups}, top_groups={top_groups} or group_top={group_top} is out of range")
+    return c
 
 
 def _check_bias(bias, logits):
