@@ -1064,7 +1064,7 @@ aem_status fp8_product(const Fp8Weight* w, const char* what, Fp8Args a, Rows x, 
     if (many) a.rows = kManyTile;
     // row tiles at most: n groups with rows have up to n + (M - n) / rows
     const int64_t slots = a.group_rows ? n + (a.M - n) / a.rows : (a.M + a.rows - 1) / a.rows;
-    AEM_REQUIRE((many || slots <= 65535) && slots * ((a.nb + 1) / 2) < (1ll << 31) && a.M < (1ll << 31),
+    AEM_REQUIRE((many || slots <= 65535) && slots * ((a.nb + 1) / 2) < (1ll << 31),
                 "%s: M=%lld rows are too many for one call", what, (long long)a.M);
     void* own = nullptr;
     const bool make = x.dtype != AEM_E4M3;
@@ -1103,6 +1103,13 @@ aem_status fp8_product(const Fp8Weight* w, const char* what, Fp8Args a, Rows x, 
     return AEM_OK;
 }
 
+// Rows are indexed in 32 bits, a tile past the last one included.
+aem_status check_most_rows(const char* what, int64_t M) {
+    AEM_REQUIRE(M >= 0, "%s: M must be >= 0", what);
+    AEM_REQUIRE(M < (1ll << 31) - kManyTile, "%s: M=%lld rows are too many for one call", what, (long long)M);
+    return AEM_OK;
+}
+
 aem_status check_rows(const char* what, const Rows& x, int64_t cols, int64_t M) {
     AEM_REQUIRE(x.dtype == AEM_F32 || x.dtype == AEM_BF16 || x.dtype == AEM_E4M3, "%s: bad dtype", what);
     AEM_REQUIRE(x.ldx >= 0 && x.lds >= 0, "%s: bad row stride", what);
@@ -1135,10 +1142,10 @@ aem_status aem_fp8gemm(aem_fp8weight_t wh, int64_t group, int transposed, const 
                        int64_t ldx, const float* x_scale, int64_t lds, int64_t M, void* out, aem_dtype out_dtype,
                        int64_t ldo, void* workspace, size_t workspace_bytes, void* stream) {
     AEM_REQUIRE(wh != nullptr, "aem_fp8gemm: weight handle is NULL");
+    AEM_TRY(aem::check_most_rows("aem_fp8gemm", M));
     auto* w = reinterpret_cast<aem::Fp8Weight*>(wh);
     AEM_REQUIRE(group >= 0 && group < w->G, "aem_fp8gemm: group %lld out of range [0, %lld)", (long long)group,
                 (long long)w->G);
-    AEM_REQUIRE(M >= 0, "aem_fp8gemm: M must be >= 0");
     AEM_REQUIRE(out_dtype == AEM_F32 || out_dtype == AEM_BF16, "aem_fp8gemm: bad dtype");
     const aem::Rows rows{x, x_dtype, ldx, x_scale, lds};
     AEM_TRY(aem::check_rows("aem_fp8gemm", rows, transposed ? w->N : w->K, M));
@@ -1160,10 +1167,10 @@ aem_status aem_grouped_fp8gemm(aem_fp8weight_t wh, const int32_t* group_rows, in
                                aem_dtype out_dtype, int64_t ldo, int relu, int zero_rest, void* workspace,
                                size_t workspace_bytes, void* stream) {
     AEM_REQUIRE(wh != nullptr, "aem_grouped_fp8gemm: weight handle is NULL");
+    AEM_TRY(aem::check_most_rows("aem_grouped_fp8gemm", M));
     auto* w = reinterpret_cast<aem::Fp8Weight*>(wh);
     AEM_REQUIRE(w->G <= AEM_MAX_EXPERTS, "aem_grouped_fp8gemm: %lld weight groups, at most %d", (long long)w->G,
                 AEM_MAX_EXPERTS);
-    AEM_REQUIRE(M >= 0, "aem_grouped_fp8gemm: M must be >= 0");
     AEM_REQUIRE(out_dtype == AEM_F32 || out_dtype == AEM_BF16, "aem_grouped_fp8gemm: bad dtype");
     const aem::Rows rows{x, x_dtype, ldx, x_scale, lds};
     AEM_TRY(aem::check_rows("aem_grouped_fp8gemm", rows, transposed ? w->N : w->K, M));

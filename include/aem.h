@@ -498,7 +498,7 @@ aem_status aem_fp8weight_shape(aem_fp8weight_t w, int64_t* G, int64_t* K, int64_
  * or NULL to have the call allocate and free it in stream order.  Rows of out are
  * ldo elements apart, any alignment works.  out must not overlap x or the
  * workspace; the weights' device must be the current one; make the first call on a
- * device before a stream capture.  Results repeat bit for bit. */
+ * device before a stream capture.  M < 2^31 - 256.  Results repeat bit for bit. */
 size_t aem_fp8gemm_workspace(aem_fp8weight_t w, aem_dtype x_dtype, int64_t M, int transposed);
 aem_status aem_fp8gemm(aem_fp8weight_t w, int64_t group, int transposed, const void* x,
                        aem_dtype x_dtype, int64_t ldx, const float* x_scale, int64_t lds, int64_t M,
