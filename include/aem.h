@@ -423,8 +423,10 @@ aem_status aem_grouped_q4gemm(aem_q4weight_t w, const int32_t* group_rows, const
  * whatever a float32 exponential rounds to.  An expert whose logit or bias is
  * -inf is never chosen; where fewer than k are left the id is -1 and the weight
  * zero, which the dispatch and the combine take as a unit without an expert.  A
- * NaN key ranks above every number, and its weights are NaN.  k <= AEM_MAX_TOPK
- * and <= E / groups * top_groups, E <= AEM_MAX_EXPERTS.  The bias takes part in
+ * NaN key ranks above every number.  A NaN logit makes its expert's weight NaN, and
+ * with softmax or renormalised scores all of the row's; a NaN bias only ranks its
+ * expert first, the weight is that of its score.  k <= AEM_MAX_TOPK and <= E / groups
+ * * top_groups, E <= AEM_MAX_EXPERTS.  The bias takes part in
  * the choice alone, so it has no gradient.  The reference's gating
  * (src/kernels/fused_gating_metal.py:236-307) has softmax weights without bias or
  * groups, and no gradient. */

@@ -1,6 +1,6 @@
-"""Routing from logits where masks leave fewer experts than slots, on the GPU,
-against the plain implementation in 64 bits of test_routing_gpu.py (ids equal,
-weights within its bound)."""
+"""Routing from logits where masks leave fewer experts than slots, and NaN among
+the biases, on the GPU, against the plain implementation in 64 bits of
+test_routing_gpu.py (ids equal, weights within its bound)."""
 import numpy as np
 import pytest
 
@@ -64,3 +64,19 @@ def test_biases_that_leave_fewer_experts_than_slots(cuda, E, groups, top):
                 how = dict(k=min(4, size * top), score=score, groups=groups, top_groups=top, group_top=group_top)
                 ids, w = routing.route_tokens(x, bias=bias, **how)
                 check_route(x, ids, w, dict(how, bias=bias.cpu().numpy()))
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renorm", [False, True])
+def test_nan_bias(cuda, score, renorm):
+    """A NaN among the biases ranks its expert first; the weight is that of its score."""
+    import torch
+    from aethermoe_b200 import routing
+    for E in (8, 24, 64, 256):
+        x = make(cuda, 20, E, torch.float32, seed=E)
+        bias = 0.1 * torch.randn(E, device=cuda)
+        bias[5] = np.nan
+        for groups, top, gt in ((1, 1, 1), (4, 2, 2), (4, 2, 1)):
+            how = dict(k=3, score=score, groups=groups, top_groups=top, group_top=gt, renormalize=renorm)
+            ids, w = routing.route_tokens(x, bias=bias, **how)
+            assert (ids[:, 0] == 5).all() and torch.isfinite(w).all()
+            check_route(x, ids, w, dict(how, bias=bias.cpu().numpy()))
