@@ -8,7 +8,6 @@
 
 namespace aem {
 
-constexpr int kFp8Block = 128;        // elements that share a scale
 constexpr int kFp8Tile = 128 * 128;   // bytes of a packed tile
 
 // Packed e4m3 weight (device): [G][NC][KC] tiles of 128 channels x 128 k, NC =
