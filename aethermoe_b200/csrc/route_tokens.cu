@@ -529,7 +529,16 @@ __global__ void __launch_bounds__(kRouteThreads, 4) route_kernel(const RouteArgs
     } else {
         extract<LANES, false>(a, on, 0.0f, sh);
     }
-    const int decide = sure ? 0 : to_decide(__reduce_or_sync(~0u, open));
+    int decide = 0;
+    if (!sure) {
+        // (Lanes leave the comparisons one after the other.  A reduction of the bits, put
+        // right behind them by the compiler, did not see all lanes in rows of 8 experts.)
+        __syncwarp();
+        int bits = 0;
+#pragma unroll
+        for (int bit : {OPEN_ORDER, OPEN_SET, OPEN_BEHIND}) bits |= __any_sync(~0u, open & bit) ? bit : 0;
+        decide = to_decide(bits);
+    }
     if (decide == 1 && a.sigmoid && a.k <= LANES)
         order_exactly<LANES, LT>(a, t0, sh.ids[w]);
     else if (decide)
