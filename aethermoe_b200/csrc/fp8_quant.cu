@@ -20,18 +20,17 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Two quotients -x / s, rounded as IEEE division does: with n = -1/s rounded and
-// q = x n, the residual x + s q is exact in a fused multiply-add, and q + n (x + s q)
+// Two quotients x / s, rounded as IEEE division does: with r = 1/s rounded and
+// q = x r, the residual x - s q is exact in a fused multiply-add, and q + r (x - s q)
 // is the rounded quotient (P. Markstein, IBM J. Res. Dev. 34, 1990).  The residual
 // has to stay normal, which holds for s in [2^-90, 2^126): a quotient that e4m3
-// does not round to zero is 2^-11 at least, so x is 2^-101.  The quotient is taken
-// with the other sign because a zero's survives so: the residual of either zero is +0,
-// and n times it is the -0 that leaves a zero alone.
-__device__ __forceinline__ void quotient2(float x0, float x1, float s, float n, float& q0, float& q1) {
-    asm("{\n.reg .b64 x, s, n, q, e;\nmov.b64 x, {%2, %3};\nmov.b64 s, {%5, %5};\nmov.b64 n, {%4, %4};\n"
-        "mul.rn.f32x2 q, x, n;\nfma.rn.f32x2 e, s, q, x;\nfma.rn.f32x2 q, e, n, q;\nmov.b64 {%0, %1}, q;\n}"
+// does not round to zero is 2^-11 at least, so x is 2^-101.  It is rounded downward, so
+// that one of zero is -0 and a quotient of either zero keeps its sign.
+__device__ __forceinline__ void quotient2(float x0, float x1, float s, float r, float& q0, float& q1) {
+    asm("{\n.reg .b64 x, s, n, r, q, e;\nmov.b64 x, {%2, %3};\nmov.b64 n, {%5, %5};\nmov.b64 r, {%4, %4};\n"
+        "mul.rn.f32x2 q, x, r;\nfma.rm.f32x2 e, n, q, x;\nfma.rn.f32x2 q, e, r, q;\nmov.b64 {%0, %1}, q;\n}"
         : "=f"(q0), "=f"(q1)
-        : "f"(x0), "f"(x1), "f"(n), "f"(s));
+        : "f"(x0), "f"(x1), "f"(r), "f"(-s));
 }
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     uint16_t v;
@@ -53,18 +52,16 @@ __device__ __forceinline__ float block_scale(uint32_t amax_bits) {
 template <int N>
 __device__ __forceinline__ void to_e4m3(const float (&v)[N], float s, uint32_t (&o)[N / 4]) {
     float q[N];
-    const bool steps = s >= 0x1p-90f && s < 0x1p126f;
-    if (steps) {
-        const float n = -__frcp_rn(s);
+    if (s >= 0x1p-90f && s < 0x1p126f) {
+        const float r = __frcp_rn(s);
 #pragma unroll
-        for (int i = 0; i < N; i += 2) quotient2(v[i], v[i + 1], s, n, q[i], q[i + 1]);
+        for (int i = 0; i < N; i += 2) quotient2(v[i], v[i + 1], s, r, q[i], q[i + 1]);
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) q[i] = __fdiv_rn(v[i], s);
     }
-    const uint32_t sign = steps ? 0x80808080u : 0;
 #pragma unroll
-    for (int i = 0; i < N; i += 4) o[i / 4] = (e4m3x2(q[i], q[i + 1]) | e4m3x2(q[i + 2], q[i + 3]) << 16) ^ sign;
+    for (int i = 0; i < N; i += 4) o[i / 4] = e4m3x2(q[i], q[i + 1]) | e4m3x2(q[i + 2], q[i + 3]) << 16;
 }
 
 // 8 elements of a row from k on as they lie in memory, zero past K.
