@@ -534,10 +534,9 @@ __global__ void __launch_bounds__(kRouteThreads, 4) route_kernel(const RouteArgs
         // (Lanes leave the comparisons one after the other.  A reduction of the bits, put
         // right behind them by the compiler, did not see all lanes in rows of 8 experts.)
         __syncwarp();
-        int bits = 0;
-#pragma unroll
-        for (int bit : {OPEN_ORDER, OPEN_SET, OPEN_BEHIND}) bits |= __any_sync(~0u, open & bit) ? bit : 0;
-        decide = to_decide(bits);
+        if (__any_sync(~0u, open & (OPEN_ORDER | OPEN_SET)))
+            decide = to_decide(OPEN_ORDER | (__any_sync(~0u, open & OPEN_SET) ? OPEN_SET : 0) |
+                               (__any_sync(~0u, open & OPEN_BEHIND) ? OPEN_BEHIND : 0));
     }
     if (decide == 1 && a.sigmoid && a.k <= LANES)
         order_exactly<LANES, LT>(a, t0, sh.ids[w]);
