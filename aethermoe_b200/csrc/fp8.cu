@@ -387,8 +387,9 @@ __global__ void __launch_bounds__(kFewThreads, ALONE ? 1 : 2)
 // their barriers alone take 155; what bounds it is the warps that take the sums back,
 // about 700 cycles a block where the MMAs take 512 (264 are multiply-adds of the two
 // warps that share a sub-core), and a tile's first and last block, which overlap with
-// no other's MMAs.  For seconds on end it takes 249 us: the power limit (990 W) leaves
-// 1.5 GHz.  Accumulators of half the width, four of them, wait twice as often: 261 us.
+// no other's MMAs.  For seconds on end it takes 249 us (258 a call with the rows'
+// quantisation): the power limit (990 W) leaves 1.5 GHz.  Accumulators of half the width,
+// four of them, wait twice as often: 261 us.
 // The registers decide: 128 sums, 32 columns under way, and every variable more that
 // was kept through the loop was moved about in it (32 columns a load 238 us, the next
 // block's first columns ahead 231, pointers kept 245, one float4 of scales 225 instead of
@@ -893,7 +894,9 @@ __global__ void __launch_bounds__(256)
 constexpr int kSMs = 148;
 
 // What a product takes, in units of 10 ns, from its CTAs (pairs), the blocks of the
-// sum and the rows of a tile.
+// sum and the rows of a tile.  Neither counts the bytes of out: they were measured with
+// sums of 16 blocks and more or few rows; with a sum of one or two blocks and many
+// columns the stores decide, and which kernel is the faster one there was not measured.
 //
 // Few rows: CTAs (at most 8, one cluster) split the sum.  Row tiles of 16 and 32
 // share an SM by twos while there are more CTAs than SMs, the wider ones have one to
@@ -1056,7 +1059,8 @@ aem_status fp8_product(const Fp8Weight* w, const char* what, Fp8Args a, Rows x, 
     }
     const int64_t n = std::min<int64_t>(a.G, a.M), want = (a.M + n - 1) / n;
     a.rows = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : 128;
-    // (the groups' sizes are not known here: all as large as the average)
+    // (the groups' sizes are not known here: all as large as the average.  Where a few
+    // groups have most rows their weights pass once for each tile of the average's size)
     const int64_t cost = few_cost(n * ((want + a.rows - 1) / a.rows) * a.nb, a.kb, a.rows, &a.S);
     const int pairs = want > 32 ? max_pairs(w->device) : 0;
     const bool many = pairs > 0 && (a.M > 65535ll * 64 ||  // (more row tiles than a grid of the other kernel has)

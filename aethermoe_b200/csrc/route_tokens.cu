@@ -11,10 +11,10 @@
 //
 // The order has to be the one of 64-bit arithmetic, so that it depends on no
 // rounding of a float32 exp or sum.  Keys are computed in float32 beside a bound
-// on their error; wherever two keys that decide the order (neighbours among the
-// k + 1 largest, the last group kept and the first dropped) are nearer than their
-// bounds, the warp decides with keys in 64 bits: those of the chosen experts where only
-// their order is open (with normally distributed logits and 256 experts, top-8,
+// on their error (route_bounds.h); wherever two keys that decide the order (neighbours
+// among the k + 1 largest, the last group kept and the first dropped) are nearer than
+// their bounds, the warp decides with keys in 64 bits: those of the chosen experts where
+// only their order is open (with normally distributed logits and 256 experts, top-8,
 // sigmoid with a bias, a row in 2400), else of all of them (an eighth of those rows; a
 // call with such a row takes 5 us longer, and when all took that way 16383 rows took
 // 38 us instead of 32).  Logits themselves need no bound.
@@ -584,8 +584,10 @@ __global__ void __launch_bounds__(kRouteThreads, 4) route_kernel(const RouteArgs
 // same expert the first one adds the others' terms.  Then every lane writes its own 8
 // experts, or, where the chosen ones alone have a gradient, pieces of whole lines.  There
 // a warp has four rows, so that its lanes have slots: 16383 rows of 256 float32, top-8,
-// in 6.3 us, one row a warp 9.8.  Memory bound: 262144 such rows in 90 us (2.9 TB/s
-// written, 0.8 read), with the sums over all experts 173 us (3.1 TB/s).
+// in 6.3 us, one row a warp 9.8.  262144 such rows take 90 us (2.9 TB/s written, 0.8
+// read), with the sums over all experts 173 us (3.1 TB/s), 55 to 60% of what a copy
+// reaches: a warp's ids, the logits that they name, the sums and the stores follow one
+// another, and it does this once.
 template <int LANES, typename LT, int RB>
 __global__ void __launch_bounds__(kRouteThreads / (RB > 1 ? 2 : 1)) route_backward_kernel(const RouteArgs a) {
     constexpr int WARPS = kRouteWarps / (RB > 1 ? 2 : 1), ROWS = 32 / LANES * RB;  // RB rows of a lane

@@ -420,14 +420,16 @@ aem_status aem_grouped_q4gemm(aem_q4weight_t w, const int32_t* group_rows, const
  *   weight = scale * s, or with renormalize scale * s / (sum of the k s + 1e-20);
  *            softmax scores are renormalised as the softmax of the k logits
  * Ties go to the lower index.  The order is that of keys in 64-bit arithmetic,
- * whatever a float32 exponential rounds to.  An expert whose logit or bias is
+ * whatever a float32 exponential rounds to (keys that differ in their last bits alone
+ * as CUDA's double exponential rounds them); weights are computed in float32, scores
+ * below 2^-126 with fewer digits.  An expert whose logit or bias is
  * -inf is never chosen; where fewer than k are left the id is -1 and the weight
  * zero, which the dispatch and the combine take as a unit without an expert.  A
  * NaN key ranks above every number.  A NaN logit makes its expert's weight NaN, and
  * with softmax or renormalised scores all of the row's; a NaN bias only ranks its
- * expert first, the weight is that of its score.  k <= AEM_MAX_TOPK and <= E / groups
- * * top_groups, E <= AEM_MAX_EXPERTS.  The bias takes part in
- * the choice alone, so it has no gradient.  The reference's gating
+ * expert first, the weight is that of its score.  k <= AEM_MAX_TOPK and no more than
+ * E / groups * top_groups, E <= AEM_MAX_EXPERTS.  The bias takes part in the choice
+ * alone, so it has no gradient.  The reference's gating
  * (src/kernels/fused_gating_metal.py:236-307) has softmax weights without bias or
  * groups, and no gradient. */
 typedef enum { AEM_SCORE_SOFTMAX = 0, AEM_SCORE_SIGMOID = 1 } aem_score;
